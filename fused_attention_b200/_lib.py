@@ -29,6 +29,10 @@ EXPORTED_SYMBOLS = (
     "fa_b200_describe_schedule",
     "fa_b200_selftest_bounded_wait",
     "fa_b200_selftest_debug_checks",
+    "fa_b200_cache_append",
+    "fa_b200_cache_select",
+    "fa_b200_cache_attention",
+    "fa_b200_cache_attention_scratch",
 )
 
 # Status codes and flags, mirrored from include/fa_b200.h.
@@ -43,6 +47,8 @@ ERR_DRIVER = -7
 ERR_FLAGS = -8
 ERR_DEVICE_TIMEOUT = -9
 ERR_TOO_LARGE = -10
+ERR_PAGE = -11
+ERR_DTYPE = -12
 
 FLAG_DEFAULT = 0
 FLAG_FORCE_SIMPLE = 1
@@ -52,6 +58,24 @@ FLAG_NO_OVERLAP = 8
 FLAG_NO_SPLIT = 16
 FLAG_FORCE_PAIR = 32
 FLAG_NO_PAIR = 64
+
+FP16 = 0
+BF16 = 1
+CACHE_NEIGHBOURS = 1
+CACHE_ALL_KEYS = 2
+
+
+class Cache(ctypes.Structure):
+    """``fa_b200_cache`` of include/fa_b200.h."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "bounds", "status")] + [
+        (n, ctypes.c_int64) for n in ("k_page_stride", "k_head_stride", "k_token_stride", "v_page_stride", "v_head_stride", "v_token_stride")] + [
+        (n, ctypes.c_uint32) for n in ("n_pages", "kv_heads", "page_size", "head_dim")]
+
+
+class Sequences(ctypes.Structure):
+    """``fa_b200_sequences`` of include/fa_b200.h."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("table", "lengths", "counts")] + [("table_stride", ctypes.c_int64)] + [
+        (n, ctypes.c_uint32) for n in ("table_width", "B", "T")]
 
 _lock = threading.Lock()
 _lib = None
@@ -105,6 +129,16 @@ def load() -> ctypes.CDLL:
         lib.fa_b200_select_kernel.argtypes = [u32, u32, u32, u32, i32, u32]
         lib.fa_b200_describe_schedule.restype = i32
         lib.fa_b200_describe_schedule.argtypes = [u32, u32, u32, u32, u32, u32, ctypes.POINTER(ctypes.c_uint32)]
+        i64, u64 = ctypes.c_int64, ctypes.c_uint64
+        cache, seqs, rows = ctypes.POINTER(Cache), ctypes.POINTER(Sequences), [vp, i64, i64]
+        lib.fa_b200_cache_append.restype = i32
+        lib.fa_b200_cache_append.argtypes = [cache, seqs] + 3 * rows + [u32, vp, vp, vp, u32, u32, u32, i32, vp]
+        lib.fa_b200_cache_select.restype = i32
+        lib.fa_b200_cache_select.argtypes = [cache, seqs] + rows + [u32, u32, u32, u32, u32, vp, vp, u64, i32, vp]
+        lib.fa_b200_cache_attention.restype = i32
+        lib.fa_b200_cache_attention.argtypes = [cache, seqs] + rows + [u32, u32, vp, u32, u32, vp, vp, u64, i32, vp]
+        lib.fa_b200_cache_attention_scratch.restype = i32
+        lib.fa_b200_cache_attention_scratch.argtypes = 8 * [u32] + [i32, ctypes.POINTER(u64)]
         _lib = lib
         return lib
 

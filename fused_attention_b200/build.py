@@ -53,6 +53,22 @@ def lib_sources() -> list[str]:
         os.path.join(ROOT, "include", "fa_b200.h")]
 
 
+def cache_sources() -> list[str]:
+    return [os.path.join(CSRC, f) for f in ("fa_cache.cu", "fa_cache.cuh", "fa_cache_append.cuh", "fa_cache_rows.cuh", "fa_cache_select.cuh",
+                                            "fa_ptx.cuh")] + [os.path.join(ROOT, "include", "fa_b200.h")]
+
+
+def build_cache_object(force: bool = False, verbose: bool = False) -> str:
+    """Compile csrc/fa_cache.cu, the key/value cache's part, once for all variants of the library."""
+    out = os.path.join(LIBDIR, "fa_cache.o")
+    if force or _stale(out, cache_sources()):
+        os.makedirs(LIBDIR, exist_ok=True)
+        flags = [f for f in NVCC_FLAGS if f != "-shared"]
+        subprocess.run([_nvcc(), *flags, "-I", os.path.join(ROOT, "include"), "-I", CSRC, *(["-Xptxas", "-v"] if verbose else []),
+                        "-c", "-o", out, os.path.join(CSRC, "fa_cache.cu")], check=True)
+    return out
+
+
 def build_lib(force: bool = False, verbose: bool = False, debug: bool = False, cycles: bool = False,
               timeline: bool = False) -> str:
     """Compile csrc/fa_b200.cu into lib/libfa_b200.so (cross-compiles without a GPU).
@@ -65,7 +81,8 @@ def build_lib(force: bool = False, verbose: bool = False, debug: bool = False, c
     the kernel on pairs of CTAs also stamps the events of every key step (cycles.py --timeline)."""
     os.makedirs(LIBDIR, exist_ok=True)
     out = DEBUG_LIB if debug else (TIMELINE_LIB if timeline else (CYCLES_LIB if cycles else LIB))
-    if not force and not _stale(out, lib_sources()):
+    cache = build_cache_object(force=force and out == LIB, verbose=verbose)
+    if not force and not _stale(out, lib_sources() + [cache]):
         return out
     cmd = [_nvcc(), *NVCC_FLAGS, "-I", os.path.join(ROOT, "include"), "-I", CSRC]
     if debug:
@@ -76,7 +93,7 @@ def build_lib(force: bool = False, verbose: bool = False, debug: bool = False, c
         cmd += ["-DFA_CYCLES"]
     if verbose:
         cmd += ["-Xptxas", "-v"]
-    cmd += ["-o", out, os.path.join(CSRC, "fa_b200.cu")]
+    cmd += ["-o", out, os.path.join(CSRC, "fa_b200.cu"), cache]
     subprocess.run(cmd, check=True)
     return out
 

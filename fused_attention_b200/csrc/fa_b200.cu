@@ -1133,6 +1133,8 @@ const char* fa_b200_strerror(int code) {
         case FA_B200_ERR_FLAGS: return "unknown or contradictory flags";
         case FA_B200_ERR_DEVICE_TIMEOUT: return "a bounded wait inside the kernel expired; see fa_b200_read_status";
         case FA_B200_ERR_TOO_LARGE: return "the problem exceeds the fixed capacity of this entry point";
+        case FA_B200_ERR_PAGE: return "page_size must be 16, 32, 64 or 128";
+        case FA_B200_ERR_DTYPE: return "16-bit tensors must be fp16 or bf16";
         default: break;
     }
     if (code > 0) return cudaGetErrorString(static_cast<cudaError_t>(code));

@@ -1,0 +1,327 @@
+// C entry points of the paged 8-bit key/value cache (include/fa_b200.h): checks, the choice of a kernel, launches.
+#include <atomic>
+#include <cstdint>
+
+#include "fa_b200.h"
+#include "fa_cache.cuh"
+#include "fa_cache_append.cuh"
+#include "fa_cache_rows.cuh"
+#include "fa_cache_select.cuh"
+
+namespace {
+
+constexpr int kMaxDevices = 64;
+
+// What is asked of a device once.
+struct Device {
+    std::atomic<int> sms{0};   // 0: not asked yet
+    std::atomic<uint32_t> attr_done{0};   // bit per kernel instance whose shared-memory attribute is set
+};
+Device g_device[kMaxDevices];
+
+int device_of(int device, Device** out) {
+    if (device < 0 || device >= kMaxDevices) return static_cast<int>(cudaErrorInvalidDevice);
+    Device& d = g_device[device];
+    if (d.sms.load(std::memory_order_acquire) == 0) {
+        int major = 0, sms = 0;
+        cudaError_t e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device);
+        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+        if (e != cudaSuccess) return static_cast<int>(e);
+        if (major != 10) return FA_B200_ERR_ARCH;
+        d.sms.store(sms, std::memory_order_release);
+    }
+    *out = &d;
+    return FA_B200_OK;
+}
+
+// Makes `device` current for a call and puts the old one back.
+struct OnDevice {
+    int before = -1, rc = 0;
+    bool changed = false;
+    explicit OnDevice(int device) {
+        cudaError_t e = cudaGetDevice(&before);
+        if (e == cudaSuccess && before != device) {
+            e = cudaSetDevice(device);
+            changed = e == cudaSuccess;
+        }
+        rc = static_cast<int>(e);
+    }
+    ~OnDevice() {
+        if (changed) (void)cudaSetDevice(before);
+    }
+};
+
+// (the kernels wait for the one before them on the stream before they touch memory)
+template <typename... KArgs, typename... Args>
+int launch(void (*kernel)(KArgs...), uint32_t grid, uint32_t block, size_t smem, cudaStream_t stream, const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid, 1, 1);
+    cfg.blockDim = dim3(block, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
+}
+
+template <typename Kernel>
+int allow_smem(Device& d, uint32_t bit, Kernel* kernel, int bytes) {
+    if (d.attr_done.load(std::memory_order_acquire) & (1u << bit)) return FA_B200_OK;   // (setting it twice is harmless)
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    d.attr_done.fetch_or(1u << bit, std::memory_order_release);
+    return FA_B200_OK;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool multiple16(int64_t x) { return (x & 15) == 0; }
+bool head_dim_ok(uint32_t H) { return H == 16 || H == 32 || H == 64 || H == 128; }
+bool page_ok(uint32_t p) { return p == 16 || p == 32 || p == 64 || p == 128; }
+uint32_t log2_of(uint32_t p) { return p == 16 ? 4 : p == 32 ? 5 : p == 64 ? 6 : 7; }
+
+int view_of(const fa_b200_cache* c, fa::CacheView* v) {
+    if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale || !c->bounds || !c->status) return FA_B200_ERR_NULL_POINTER;
+    if (!head_dim_ok(c->head_dim)) return FA_B200_ERR_HEAD_DIM;
+    if (!page_ok(c->page_size)) return FA_B200_ERR_PAGE;
+    if (c->n_pages == 0 || c->n_pages > 0x7FFFFFFFu || c->kv_heads == 0) return FA_B200_ERR_SHAPE;
+    if (!aligned16(c->k) || !aligned16(c->v) || !aligned16(c->bounds) || !multiple16(c->k_page_stride) || !multiple16(c->k_head_stride) ||
+        !multiple16(c->k_token_stride) || !multiple16(c->v_page_stride) || !multiple16(c->v_head_stride) || !multiple16(c->v_token_stride) ||
+        (reinterpret_cast<uintptr_t>(c->k_scale) & 3u) || (reinterpret_cast<uintptr_t>(c->v_scale) & 3u) || (reinterpret_cast<uintptr_t>(c->status) & 3u))
+        return FA_B200_ERR_ALIGNMENT;
+    v->k = static_cast<uint8_t*>(c->k);
+    v->v = static_cast<uint8_t*>(c->v);
+    v->k_scale = c->k_scale;
+    v->v_scale = c->v_scale;
+    v->bounds = static_cast<uint8_t*>(c->bounds);
+    v->status = c->status;
+    v->k_page = c->k_page_stride, v->k_head = c->k_head_stride, v->k_token = c->k_token_stride;
+    v->v_page = c->v_page_stride, v->v_head = c->v_head_stride, v->v_token = c->v_token_stride;
+    v->n_pages = c->n_pages, v->heads = c->kv_heads, v->page = c->page_size, v->page_shift = log2_of(c->page_size);
+    return FA_B200_OK;
+}
+
+int seqs_of(const fa_b200_sequences* s, const fa::CacheView& c, fa::CacheSeqs* out) {
+    if (!s || !s->table || !s->lengths) return FA_B200_ERR_NULL_POINTER;
+    if (s->B == 0 || s->T == 0 || s->table_width == 0 || s->B > (1u << 24) || s->T > (1u << 24) ||
+        s->table_width > (0x7FFFFFFFu >> c.page_shift))   // positions are 31-bit numbers
+        return FA_B200_ERR_SHAPE;
+    if ((reinterpret_cast<uintptr_t>(s->table) | reinterpret_cast<uintptr_t>(s->lengths) | reinterpret_cast<uintptr_t>(s->counts)) & 3u)
+        return FA_B200_ERR_ALIGNMENT;
+    out->table = s->table, out->lengths = s->lengths, out->counts = s->counts, out->table_stride = s->table_stride;
+    out->width = s->table_width, out->B = s->B, out->T = s->T;
+    return FA_B200_OK;
+}
+
+// Rows of 16-bit values: base and strides in elements, all rows on 16-byte boundaries.
+int rows_ok(const void* base, int64_t batch_stride, int64_t token_stride) {
+    if (!base) return FA_B200_ERR_NULL_POINTER;
+    return aligned16(base) && multiple16(2 * batch_stride) && multiple16(2 * token_stride) ? FA_B200_OK : FA_B200_ERR_ALIGNMENT;
+}
+
+constexpr uint64_t kMostCtas = 0x7FFFFFFFull;
+
+// ----------------------------------------------------------------------------- attention for few rows
+struct RowsPlan {
+    uint32_t mt, rows, row_tiles, grid;
+    uint64_t problems, units;   // units: of one problem, at most
+    uint64_t o_bytes, ml_bytes, share_bytes;
+    uint64_t scratch() const { return o_bytes + ml_bytes + share_bytes; }
+};
+
+RowsPlan plan_rows(uint32_t H, uint32_t heads, uint32_t group, uint32_t page, uint32_t B, uint32_t T, uint32_t width, uint32_t keep, uint32_t sms) {
+    RowsPlan r = {};
+    if (keep != 0) {   // a problem has rows of one token
+        r.rows = group;
+        if (group > 32)
+            for (r.rows = 32; group % r.rows != 0;) --r.rows;
+        r.mt = r.rows > 16 ? 2 : 1;
+        r.row_tiles = T * (group / r.rows);
+    } else {
+        const uint64_t all = static_cast<uint64_t>(T) * group;
+        r.mt = all > 16 ? 2 : 1;
+        r.rows = static_cast<uint32_t>(all < 16u * r.mt ? all : 16u * r.mt);
+        r.row_tiles = static_cast<uint32_t>((all + r.rows - 1) / r.rows);
+    }
+    const uint64_t tokens = static_cast<uint64_t>(keep != 0 ? keep : width) * page;
+    r.units = (tokens + fa::kRowsUnit - 1) / fa::kRowsUnit;
+    r.problems = static_cast<uint64_t>(B) * heads * r.row_tiles;
+    const uint64_t ctas = static_cast<uint64_t>(sms) * (r.mt == 1 ? 3 : 2), all_units = r.problems * r.units;
+    r.grid = static_cast<uint32_t>(ctas < all_units ? ctas : all_units);
+    const uint64_t slots = 2ull * r.grid * 16 * r.mt;
+    r.o_bytes = slots * H * 4;
+    r.ml_bytes = slots * 8;
+    r.share_bytes = r.problems * 8;
+    return r;
+}
+
+template <int H, int MT>
+int launch_rows(Device& d, uint32_t bit, const fa::RowsArgs& a, const RowsPlan& plan, cudaStream_t stream) {
+    using Cfg = fa::RowsCfg<H, MT>;
+    int rc = allow_smem(d, bit, &fa::fa_cache_rows<H, MT>, Cfg::kSmem);
+    if (rc == FA_B200_OK) rc = launch(&fa::fa_cache_rows<H, MT>, plan.grid, fa::kRowsWarps * 32, Cfg::kSmem, stream, a);
+    if (rc == FA_B200_OK && plan.units > 1) rc = launch(&fa::fa_cache_join<H, MT>, static_cast<uint32_t>(plan.problems * plan.rows), 128, 0, stream, a);
+    return rc;
+}
+template <int H>
+int launch_rows(Device& d, uint32_t bit, const fa::RowsArgs& a, const RowsPlan& plan, cudaStream_t stream) {
+    return plan.mt == 1 ? launch_rows<H, 1>(d, bit, a, plan, stream) : launch_rows<H, 2>(d, bit + 1, a, plan, stream);
+}
+
+// ----------------------------------------------------------------------------- appending
+template <int H>
+int launch_append(const fa::AppendArgs& a, bool warp_tasks, uint32_t task_ctas, cudaStream_t stream) {
+    return warp_tasks ? launch(&fa::fa_cache_append<H, 32>, task_ctas + a.query_ctas, fa::kAppendThreads, 0, stream, a)
+                      : launch(&fa::fa_cache_append<H, 128>, task_ctas + a.query_ctas, fa::kAppendThreads, 0, stream, a);
+}
+
+}  // namespace
+
+extern "C" {
+
+int fa_b200_cache_append(const fa_b200_cache* cache, const fa_b200_sequences* sequences, const void* keys, int64_t keys_batch_stride,
+                         int64_t keys_token_stride, const void* values, int64_t values_batch_stride, int64_t values_token_stride,
+                         const void* queries_or_null, int64_t queries_batch_stride, int64_t queries_token_stride, uint32_t q_heads, void* rotated,
+                         const float* cos_or_null, const float* sin_or_null, uint32_t positions, uint32_t dtype, uint32_t flags, int device,
+                         void* cuda_stream) {
+    fa::AppendArgs a = {};
+    int rc = view_of(cache, &a.c);
+    if (rc == FA_B200_OK) rc = seqs_of(sequences, a.c, &a.s);
+    if (rc == FA_B200_OK) rc = rows_ok(keys, keys_batch_stride, keys_token_stride);
+    if (rc == FA_B200_OK) rc = rows_ok(values, values_batch_stride, values_token_stride);
+    if (rc == FA_B200_OK && queries_or_null) rc = rows_ok(queries_or_null, queries_batch_stride, queries_token_stride);
+    if (rc == FA_B200_OK && queries_or_null) rc = rows_ok(rotated, 0, 0);
+    if (rc != FA_B200_OK) return rc;
+    if (dtype > FA_B200_BF16) return FA_B200_ERR_DTYPE;
+    if (flags & ~FA_B200_CACHE_NEIGHBOURS) return FA_B200_ERR_FLAGS;
+    if (queries_or_null && q_heads == 0) return FA_B200_ERR_SHAPE;
+    if ((cos_or_null == nullptr) != (sin_or_null == nullptr)) return FA_B200_ERR_NULL_POINTER;
+    if (cos_or_null && (!aligned16(cos_or_null) || !aligned16(sin_or_null))) return FA_B200_ERR_ALIGNMENT;
+    const uint32_t H = cache->head_dim;
+    a.keys = static_cast<const uint8_t*>(keys), a.keys_b = 2 * keys_batch_stride, a.keys_t = 2 * keys_token_stride;
+    a.values = static_cast<const uint8_t*>(values), a.values_b = 2 * values_batch_stride, a.values_t = 2 * values_token_stride;
+    a.queries = static_cast<const uint8_t*>(queries_or_null), a.queries_b = 2 * queries_batch_stride, a.queries_t = 2 * queries_token_stride;
+    a.rotated = static_cast<uint8_t*>(rotated);
+    a.cos = cos_or_null, a.sin = sin_or_null, a.positions = positions;
+    a.q_heads = q_heads, a.bf16 = dtype == FA_B200_BF16, a.interleaved = flags & FA_B200_CACHE_NEIGHBOURS;
+    a.blocks = (a.s.T + a.c.page - 2) / a.c.page + 1;   // that T tokens touch at most
+    const uint64_t tasks = 2ull * a.s.B * a.blocks * a.c.heads;
+    const uint64_t q_threads = queries_or_null ? static_cast<uint64_t>(a.s.B) * a.s.T * q_heads * (H / 16) : 0;
+    uint64_t q_ctas = (q_threads + fa::kAppendThreads - 1) / fa::kAppendThreads;
+    if (q_ctas > 16384) q_ctas = 16384;
+    if (tasks + q_ctas > kMostCtas) return FA_B200_ERR_SHAPE;
+    a.tasks = static_cast<uint32_t>(tasks), a.query_ctas = static_cast<uint32_t>(q_ctas);
+    const bool warp_tasks = a.s.T <= 4;
+    const uint32_t task_ctas = static_cast<uint32_t>(warp_tasks ? (tasks + 3) / 4 : tasks);
+    Device* d = nullptr;
+    if ((rc = device_of(device, &d)) != FA_B200_OK) return rc;
+    OnDevice on(device);
+    if (on.rc != 0) return on.rc;
+    const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+    switch (H) {
+        case 16: return launch_append<16>(a, warp_tasks, task_ctas, stream);
+        case 32: return launch_append<32>(a, warp_tasks, task_ctas, stream);
+        case 64: return launch_append<64>(a, warp_tasks, task_ctas, stream);
+        default: return launch_append<128>(a, warp_tasks, task_ctas, stream);
+    }
+}
+
+int fa_b200_cache_select(const fa_b200_cache* cache, const fa_b200_sequences* sequences, const void* queries, int64_t queries_batch_stride,
+                         int64_t queries_token_stride, uint32_t q_heads, uint32_t dtype, uint32_t keep, uint32_t first, uint32_t last,
+                         int32_t* pages, void* scratch, uint64_t scratch_bytes, int device, void* cuda_stream) {
+    fa::SelectArgs a = {};
+    int rc = view_of(cache, &a.c);
+    if (rc == FA_B200_OK) rc = seqs_of(sequences, a.c, &a.s);
+    if (rc == FA_B200_OK) rc = rows_ok(queries, queries_batch_stride, queries_token_stride);
+    if (rc != FA_B200_OK) return rc;
+    if (!pages || !scratch) return FA_B200_ERR_NULL_POINTER;
+    if (dtype > FA_B200_BF16) return FA_B200_ERR_DTYPE;
+    if (q_heads == 0 || q_heads % a.c.heads != 0 || keep == 0 || keep > 0x7FFFFFFFu || last == 0) return FA_B200_ERR_SHAPE;
+    if ((reinterpret_cast<uintptr_t>(pages) | reinterpret_cast<uintptr_t>(scratch)) & 3u) return FA_B200_ERR_ALIGNMENT;
+    const uint64_t rows = static_cast<uint64_t>(a.s.B) * a.s.T * a.c.heads;
+    if (rows > kMostCtas) return FA_B200_ERR_SHAPE;
+    if (scratch_bytes < 4 * rows * a.s.width) return FA_B200_ERR_TOO_LARGE;
+    a.q = static_cast<const uint8_t*>(queries), a.q_b = 2 * queries_batch_stride, a.q_t = 2 * queries_token_stride;
+    a.keys = static_cast<uint32_t*>(scratch), a.pages = pages;
+    a.group = q_heads / a.c.heads, a.keep = keep, a.first = first, a.last = last, a.bf16 = dtype == FA_B200_BF16;
+    a.chunks = (a.s.width + fa::kScorePages - 1) / fa::kScorePages;
+    if (static_cast<uint64_t>(a.s.B) * a.c.heads * a.chunks > kMostCtas) return FA_B200_ERR_SHAPE;
+    Device* d = nullptr;
+    if ((rc = device_of(device, &d)) != FA_B200_OK) return rc;
+    OnDevice on(device);
+    if (on.rc != 0) return on.rc;
+    const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+    const uint32_t grid = a.s.B * a.c.heads * a.chunks;
+    constexpr uint32_t kBlock = fa::kScoreWarps * 32;
+    switch (cache->head_dim) {
+        case 16: rc = launch(&fa::fa_cache_scores<16>, grid, kBlock, 0, stream, a); break;
+        case 32: rc = launch(&fa::fa_cache_scores<32>, grid, kBlock, 0, stream, a); break;
+        case 64: rc = launch(&fa::fa_cache_scores<64>, grid, kBlock, 0, stream, a); break;
+        default: rc = launch(&fa::fa_cache_scores<128>, grid, kBlock, 0, stream, a); break;
+    }
+    if (rc != FA_B200_OK) return rc;
+    const uint32_t per = (a.s.width + fa::kTakeThreads - 1) / fa::kTakeThreads;
+    if (per <= 2) return launch(&fa::fa_cache_take<2>, static_cast<uint32_t>(rows), fa::kTakeThreads, 0, stream, a);
+    if (per <= 8) return launch(&fa::fa_cache_take<8>, static_cast<uint32_t>(rows), fa::kTakeThreads, 0, stream, a);
+    if (per <= 32) return launch(&fa::fa_cache_take<32>, static_cast<uint32_t>(rows), fa::kTakeThreads, 0, stream, a);
+    return launch(&fa::fa_cache_take<0>, static_cast<uint32_t>(rows), fa::kTakeThreads, 0, stream, a);
+}
+
+int fa_b200_cache_attention_scratch(uint32_t head_dim, uint32_t kv_heads, uint32_t q_heads, uint32_t page_size, uint32_t B, uint32_t T,
+                                    uint32_t table_width, uint32_t keep, int device, uint64_t out[1]) {
+    if (!out) return FA_B200_ERR_NULL_POINTER;
+    if (!head_dim_ok(head_dim)) return FA_B200_ERR_HEAD_DIM;
+    if (!page_ok(page_size)) return FA_B200_ERR_PAGE;
+    if (kv_heads == 0 || q_heads == 0 || q_heads % kv_heads != 0 || B == 0 || T == 0 || table_width == 0) return FA_B200_ERR_SHAPE;
+    Device* d = nullptr;
+    const int rc = device_of(device, &d);
+    if (rc != FA_B200_OK) return rc;
+    out[0] = plan_rows(head_dim, kv_heads, q_heads / kv_heads, page_size, B, T, table_width, keep, static_cast<uint32_t>(d->sms.load())).scratch();
+    return FA_B200_OK;
+}
+
+int fa_b200_cache_attention(const fa_b200_cache* cache, const fa_b200_sequences* sequences, const void* queries, int64_t queries_batch_stride,
+                            int64_t queries_token_stride, uint32_t q_heads, uint32_t dtype, const int32_t* pages_or_null, uint32_t keep,
+                            uint32_t flags, void* y, void* scratch, uint64_t scratch_bytes, int device, void* cuda_stream) {
+    fa::RowsArgs a = {};
+    int rc = view_of(cache, &a.c);
+    if (rc == FA_B200_OK) rc = seqs_of(sequences, a.c, &a.s);
+    if (rc == FA_B200_OK) rc = rows_ok(queries, queries_batch_stride, queries_token_stride);
+    if (rc == FA_B200_OK) rc = rows_ok(y, 0, 0);
+    if (rc != FA_B200_OK) return rc;
+    if (!scratch) return FA_B200_ERR_NULL_POINTER;
+    if (dtype > FA_B200_BF16) return FA_B200_ERR_DTYPE;
+    if (flags & ~FA_B200_CACHE_ALL_KEYS) return FA_B200_ERR_FLAGS;
+    if (q_heads == 0 || q_heads % a.c.heads != 0 || (pages_or_null != nullptr) != (keep != 0)) return FA_B200_ERR_SHAPE;
+    if (static_cast<uint64_t>(keep) * a.c.page > 0x7FFFFFFFull || static_cast<uint64_t>(a.s.T) * q_heads > 0x7FFFFFFFull) return FA_B200_ERR_SHAPE;
+    if (!aligned16(scratch) || (reinterpret_cast<uintptr_t>(pages_or_null) & 3u)) return FA_B200_ERR_ALIGNMENT;
+    Device* d = nullptr;
+    if ((rc = device_of(device, &d)) != FA_B200_OK) return rc;
+    const uint32_t H = cache->head_dim;
+    const RowsPlan plan = plan_rows(H, a.c.heads, q_heads / a.c.heads, a.c.page, a.s.B, a.s.T, a.s.width, keep, static_cast<uint32_t>(d->sms.load()));
+    if (plan.problems * plan.rows > kMostCtas) return FA_B200_ERR_SHAPE;
+    if (scratch_bytes < plan.scratch()) return FA_B200_ERR_TOO_LARGE;
+    a.q = static_cast<const uint8_t*>(queries), a.q_b = 2 * queries_batch_stride, a.q_t = 2 * queries_token_stride;
+    a.y = static_cast<uint8_t*>(y), a.pages = pages_or_null, a.keep = keep;
+    a.group = q_heads / a.c.heads, a.causal = (flags & FA_B200_CACHE_ALL_KEYS) ? 0u : 1u, a.bf16 = dtype == FA_B200_BF16;
+    a.rows = plan.rows, a.row_tiles = plan.row_tiles, a.min_units = 2;
+    a.scale_log2 = static_cast<float>(1.4426950408889634 / (H == 16 ? 4.0 : H == 32 ? 5.656854249492381 : H == 64 ? 8.0 : 11.313708498984761));
+    uint8_t* const at = static_cast<uint8_t*>(scratch);
+    a.part_o = reinterpret_cast<float*>(at);
+    a.part_ml = reinterpret_cast<float2*>(at + plan.o_bytes);
+    a.shares = reinterpret_cast<int2*>(at + plan.o_bytes + plan.ml_bytes);
+    OnDevice on(device);
+    if (on.rc != 0) return on.rc;
+    const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+    switch (H) {
+        case 16: return launch_rows<16>(*d, 0, a, plan, stream);
+        case 32: return launch_rows<32>(*d, 2, a, plan, stream);
+        case 64: return launch_rows<64>(*d, 4, a, plan, stream);
+        default: return launch_rows<128>(*d, 6, a, plan, stream);
+    }
+}
+
+}  // extern "C"

@@ -1,0 +1,312 @@
+// Appending keys and values to the cache, with the position rotation of keys and queries on the way.
+//
+// A task is one page and head of the keys or of the values that a sequence's new tokens touch.  Its new tokens are read and
+// (keys) rotated in fp32, x1 c - x2 s and x2 c + x1 s with every product and sum rounded by itself.  The largest magnitude `a`
+// gives the scale, the smallest power of two with a / scale <= 448, 2^-100 at least.  A page that held tokens keeps its scale
+// unless the new tokens need a larger one; its old codes are then moved to it, which loses nothing but bits of the smallest
+// (subnormal) codes, since both scales are powers of two: a page that is filled token by token ends as close to its values as
+// one that is filled at once.  A value that is not finite makes the page's scale NaN and its codes zero.
+//
+// Bound by memory for prompts (2 bytes read and 1 written a value) and by the chain length -> table entry -> old scale ->
+// codes for single tokens, which is why a task is a warp there: B=256 sequences of 8 heads are 4096 tasks.
+#pragma once
+
+#include "fa_cache.cuh"
+
+namespace fa {
+
+struct AppendArgs {
+    CacheView c;
+    CacheSeqs s;
+    const uint8_t* keys;      // 16-bit rows of heads * H values
+    const uint8_t* values;
+    const uint8_t* queries;   // null: none
+    uint8_t* rotated;         // [B, T, q_heads * H] contiguous
+    const float* cos;         // [positions, H / 2]; null: no rotation
+    const float* sin;
+    int64_t keys_b, keys_t, values_b, values_t, queries_b, queries_t;   // strides in bytes
+    uint32_t positions, q_heads, blocks, bf16, interleaved;
+    uint32_t tasks, query_ctas;
+};
+
+// The 16 values of a head that one thread works on: dimensions [8 j, 8 j + 8) and [H/2 + 8 j, H/2 + 8 j + 8).
+struct Sixteen {
+    float a[8], b[8];
+};
+template <int H>
+__device__ __forceinline__ Sixteen load_sixteen(const uint8_t* row, uint32_t j, bool bf16) {
+    const uint4 x = *reinterpret_cast<const uint4*>(row + 16 * j), y = *reinterpret_cast<const uint4*>(row + H + 16 * j);
+    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+    Sixteen r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 p = unpack_16(xs[i], bf16), q = unpack_16(ys[i], bf16);
+        r.a[2 * i] = p.x, r.a[2 * i + 1] = p.y, r.b[2 * i] = q.x, r.b[2 * i + 1] = q.y;
+    }
+    return r;
+}
+__device__ __forceinline__ void turn(float& x, float& y, float c, float s) {
+    const float u = __fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s));
+    y = __fadd_rn(__fmul_rn(y, c), __fmul_rn(x, s));
+    x = u;
+}
+// cos and sin of the pairs that the sixteen values form: (i, i + H/2), or neighbours (2i, 2i + 1).
+template <int H>
+__device__ __forceinline__ void rotate(Sixteen& r, const AppendArgs& p, uint32_t position, uint32_t j) {
+    const float* c = p.cos + static_cast<size_t>(position) * (H / 2);
+    const float* s = p.sin + static_cast<size_t>(position) * (H / 2);
+    if (p.interleaved) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const float4 cc = *reinterpret_cast<const float4*>(c + half * (H / 4) + 4 * j);
+            const float4 ss = *reinterpret_cast<const float4*>(s + half * (H / 4) + 4 * j);
+            float* x = half ? r.b : r.a;
+            turn(x[0], x[1], cc.x, ss.x);
+            turn(x[2], x[3], cc.y, ss.y);
+            turn(x[4], x[5], cc.z, ss.z);
+            turn(x[6], x[7], cc.w, ss.w);
+        }
+    } else {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const float4 cc = *reinterpret_cast<const float4*>(c + 8 * j + 4 * q);
+            const float4 ss = *reinterpret_cast<const float4*>(s + 8 * j + 4 * q);
+            turn(r.a[4 * q], r.b[4 * q], cc.x, ss.x);
+            turn(r.a[4 * q + 1], r.b[4 * q + 1], cc.y, ss.y);
+            turn(r.a[4 * q + 2], r.b[4 * q + 2], cc.z, ss.z);
+            turn(r.a[4 * q + 3], r.b[4 * q + 3], cc.w, ss.w);
+        }
+    }
+}
+
+// The smallest power of two, 2^-100 at least, that brings `most` to 448 or below; NaN if `most` is not finite.
+__device__ __forceinline__ float append_scale(float most) {
+    if (!(most < __int_as_float(0x7F800000))) return __int_as_float(0x7FC00000);
+    const uint32_t bits = __float_as_uint(most);
+    const int32_t k = static_cast<int32_t>(bits >> 23) - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);   // 448 = 1.75 * 2^8
+    return __uint_as_float(static_cast<uint32_t>(max(k, 27)) << 23);
+}
+// (the larger of the two, NaN if one is)
+__device__ __forceinline__ float larger_scale(float x, float y) { return x > y || x != x ? x : y; }
+
+__device__ __forceinline__ uint32_t half2_min(uint32_t x, uint32_t y) {
+    const __half2 r = __hmin2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t half2_max(uint32_t x, uint32_t y) {
+    const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+// Four codes, their values multiplied by a power of two <= 1.
+__device__ __forceinline__ uint32_t moved_codes(uint32_t four, float shrink) {
+    uint32_t lo, hi;
+    e4m3x4_to_half2(four, lo, hi);
+    const float2 x = unpack_half2(lo), y = unpack_half2(hi);
+    return floats_to_e4m3x2(x.x * shrink, x.y * shrink) | (floats_to_e4m3x2(y.x * shrink, y.y * shrink) << 16);
+}
+
+constexpr int kAppendThreads = 128;
+
+// kTask threads a task (32: a warp, 128: the CTA).
+template <int H, int kTask>
+__global__ void __launch_bounds__(kAppendThreads) fa_cache_append(const AppendArgs p) {
+    constexpr int kPerToken = H / 16;                    // threads that share a token
+    constexpr int kTokens = kTask / kPerToken;           // tokens at a time
+    __shared__ float s_most[kAppendThreads / 32];
+    __shared__ uint32_t s_low[kAppendThreads / 32][H / 2], s_high[kAppendThreads / 32][H / 2];
+    grid_dep_wait();
+    grid_dep_launch();
+    const bool bf16 = p.bf16 != 0;
+
+    const uint32_t task_ctas = gridDim.x - p.query_ctas;
+    if (blockIdx.x >= task_ctas) {   // ---- queries: 16 values a thread
+        const uint64_t n = static_cast<uint64_t>(p.s.B) * p.s.T * p.q_heads * kPerToken;
+        for (uint64_t i = static_cast<uint64_t>(blockIdx.x - task_ctas) * kAppendThreads + threadIdx.x; i < n;
+             i += static_cast<uint64_t>(p.query_ctas) * kAppendThreads) {
+            const uint32_t j = static_cast<uint32_t>(i % kPerToken);
+            const uint64_t head_row = i / kPerToken;
+            const uint32_t head = static_cast<uint32_t>(head_row % p.q_heads);
+            const uint64_t row = head_row / p.q_heads;
+            const uint32_t t = static_cast<uint32_t>(row % p.s.T), b = static_cast<uint32_t>(row / p.s.T);
+            uint8_t* out = p.rotated + head_row * (2 * H) + 16 * j;
+            uint4 x = make_uint4(0, 0, 0, 0), y = x;
+            const uint64_t at = static_cast<uint64_t>(max(p.s.lengths[b], 0)) + t;
+            if (t < cache_count(p.s, b) && (p.cos == nullptr || at < p.positions)) {
+                Sixteen r = load_sixteen<H>(p.queries + b * p.queries_b + t * p.queries_t + static_cast<int64_t>(head) * (2 * H), j, bf16);
+                if (p.cos != nullptr) rotate<H>(r, p, static_cast<uint32_t>(at), j);
+                x = make_uint4(pack_16(r.a[0], r.a[1], bf16), pack_16(r.a[2], r.a[3], bf16), pack_16(r.a[4], r.a[5], bf16), pack_16(r.a[6], r.a[7], bf16));
+                y = make_uint4(pack_16(r.b[0], r.b[1], bf16), pack_16(r.b[2], r.b[3], bf16), pack_16(r.b[4], r.b[5], bf16), pack_16(r.b[6], r.b[7], bf16));
+            }
+            *reinterpret_cast<uint4*>(out) = x;
+            *reinterpret_cast<uint4*>(out + H) = y;
+        }
+        return;
+    }
+
+    // ---- one page and head of the keys or the values
+    const uint32_t tid = threadIdx.x % kTask, lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const uint32_t task = blockIdx.x * (kAppendThreads / kTask) + threadIdx.x / kTask;
+    if (task >= p.tasks) return;   // (whole warps; whole CTAs where a task is one)
+    const bool is_v = task & 1u;
+    uint32_t rest = task >> 1;
+    const uint32_t head = rest % p.c.heads;
+    rest /= p.c.heads;
+    const uint32_t b = rest / p.blocks, nth = rest % p.blocks;
+    const int32_t held_signed = p.s.lengths[b];
+    const uint32_t n = cache_count(p.s, b);
+    if (n == 0) return;
+    const uint32_t held = held_signed < 0 ? 0u : static_cast<uint32_t>(held_signed);
+    const uint64_t block = (held >> p.c.page_shift) + static_cast<uint64_t>(nth);
+    const uint64_t first = block << p.c.page_shift;               // position of the block's first token
+    if (first >= static_cast<uint64_t>(held) + n) return;
+    const uint32_t begin = nth == 0 ? held & (p.c.page - 1) : 0u;   // slots [begin, end) are new
+    const uint32_t end = static_cast<uint32_t>(min(static_cast<uint64_t>(p.c.page), static_cast<uint64_t>(held) + n - first));
+    int32_t page = -1;
+    if (held_signed >= 0 && block < p.s.width) page = p.s.table[b * p.s.table_stride + block];
+    const bool fits = held_signed >= 0 && block < p.s.width && (p.cos == nullptr || first + end <= p.positions);
+    if (!fits || static_cast<uint32_t>(page) >= p.c.n_pages) {
+        if (tid == 0) cache_report(p.c.status, fits ? kCacheBadPage : kCacheBadPosition);
+        return;
+    }
+    const uint32_t j = tid % kPerToken, sub = tid / kPerToken;
+    const uint8_t* rows = is_v ? p.values + b * p.values_b : p.keys + b * p.keys_b;
+    const int64_t row_pitch = is_v ? p.values_t : p.keys_t;
+    rows += static_cast<int64_t>(head) * (2 * H);
+    auto load = [&](uint32_t slot) {
+        const uint32_t t = static_cast<uint32_t>(first + slot - held);
+        Sixteen r = load_sixteen<H>(rows + t * row_pitch, j, bf16);
+        if (!is_v && p.cos != nullptr) rotate<H>(r, p, static_cast<uint32_t>(first) + slot, j);
+        return r;
+    };
+    float* const scale_at = (is_v ? p.c.v_scale : p.c.k_scale) + static_cast<size_t>(page) * p.c.heads + head;
+    const float before = begin != 0 ? *scale_at : 0.0f;
+
+    float most = 0.0f;
+    bool finite = true;
+    for (uint32_t slot = begin + sub; slot < end; slot += kTokens) {
+        const Sixteen r = load(slot);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            most = fmaxf(most, fmaxf(fabsf(r.a[i]), fabsf(r.b[i])));
+            finite = finite && r.a[i] - r.a[i] == 0.0f && r.b[i] - r.b[i] == 0.0f;
+        }
+    }
+    if (!finite) most = __int_as_float(0x7F800000);
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
+    if (kTask > 32) {
+        if (lane == 0) s_most[warp] = most;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kAppendThreads / 32; ++w) most = fmaxf(most, s_most[w]);
+    }
+    float scale = append_scale(most);
+    if (begin != 0) scale = larger_scale(before, scale);
+    const bool good = scale == scale;
+    // (a power of two: the product is the quotient)
+    const float inverse = good ? 1.0f / scale : 0.0f;
+
+    uint8_t* const base = (is_v ? p.c.v + static_cast<int64_t>(page) * p.c.v_page + static_cast<int64_t>(head) * p.c.v_head
+                                : p.c.k + static_cast<int64_t>(page) * p.c.k_page + static_cast<int64_t>(head) * p.c.k_head);
+    const int64_t pitch = is_v ? p.c.v_token : p.c.k_token;
+    const bool grown = begin != 0 && !(before == scale);
+    const float shrink = good ? before * inverse : 0.0f;
+    if (grown) {   // the tokens that the page held move to the larger scale
+        for (uint32_t slot = sub; slot < begin; slot += kTokens) {
+            uint4* const at = reinterpret_cast<uint4*>(base + slot * pitch + 16 * j);
+            uint4 w = *at;
+            w.x = good ? moved_codes(w.x, shrink) : 0u;
+            w.y = good ? moved_codes(w.y, shrink) : 0u;
+            w.z = good ? moved_codes(w.z, shrink) : 0u;
+            w.w = good ? moved_codes(w.w, shrink) : 0u;
+            *at = w;
+        }
+    }
+    uint32_t low[8], high[8];   // fp16 pairs: the bounds of the thread's dimensions
+#pragma unroll
+    for (int i = 0; i < 8; ++i) low[i] = 0x7C007C00u, high[i] = 0xFC00FC00u;
+    for (uint32_t slot = begin + sub; slot < end; slot += kTokens) {
+        const Sixteen r = load(slot);
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = good ? floats_to_e4m3x2(r.a[2 * i] * inverse, r.a[2 * i + 1] * inverse) : 0u;
+            w[4 + i] = good ? floats_to_e4m3x2(r.b[2 * i] * inverse, r.b[2 * i + 1] * inverse) : 0u;
+        }
+        uint8_t* const at = base + slot * pitch + 8 * j;
+        *reinterpret_cast<uint2*>(at) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+        *reinterpret_cast<uint2*>(at + H / 2) = make_uint2(w[4] | (w[5] << 16), w[6] | (w[7] << 16));
+        if (!is_v) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t x = e4m3x2_to_half2(w[i]);
+                low[i] = half2_min(low[i], x);
+                high[i] = half2_max(high[i], x);
+            }
+        }
+    }
+    if (!is_v) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+            for (int d = 16; d >= kPerToken; d >>= 1) {
+                low[i] = half2_min(low[i], __shfl_xor_sync(0xFFFFFFFFu, low[i], d));
+                high[i] = half2_max(high[i], __shfl_xor_sync(0xFFFFFFFFu, high[i], d));
+            }
+        }
+        if (kTask > 32) {
+            if (lane < kPerToken)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t d2 = (i < 4 ? 0 : H / 4) + 4 * lane + (i & 3);   // pair of dimensions
+                    s_low[warp][d2] = low[i];
+                    s_high[warp][d2] = high[i];
+                }
+            __syncthreads();
+        }
+        if (tid < kPerToken) {
+            uint8_t* const bounds = p.c.bounds + (static_cast<size_t>(page) * p.c.heads + head) * (2 * H);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t lo[4], hi[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    lo[i] = low[4 * half + i], hi[i] = high[4 * half + i];
+                    if (kTask > 32) {
+                        const uint32_t d2 = half * (H / 4) + 4 * j + i;
+#pragma unroll
+                        for (int w = 0; w < kAppendThreads / 32; ++w) lo[i] = half2_min(lo[i], s_low[w][d2]), hi[i] = half2_max(hi[i], s_high[w][d2]);
+                    }
+                }
+                uint2* const lo_at = reinterpret_cast<uint2*>(bounds + half * (H / 2) + 8 * j);
+                uint2* const hi_at = reinterpret_cast<uint2*>(bounds + H + half * (H / 2) + 8 * j);
+                if (begin != 0) {
+                    const uint2 ol = *lo_at, oh = *hi_at;
+                    uint32_t was[4], x[4];
+                    was[0] = ol.x, was[1] = ol.y, was[2] = oh.x, was[3] = oh.y;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (grown) was[i] = good ? moved_codes(was[i], shrink) : 0u;
+                    }
+                    e4m3x4_to_half2(was[0], x[0], x[1]);
+                    e4m3x4_to_half2(was[1], x[2], x[3]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) lo[i] = half2_min(lo[i], x[i]);
+                    e4m3x4_to_half2(was[2], x[0], x[1]);
+                    e4m3x4_to_half2(was[3], x[2], x[3]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) hi[i] = half2_max(hi[i], x[i]);
+                }
+                auto codes = [](uint32_t x, uint32_t y) {
+                    const float2 u = unpack_half2(x), v = unpack_half2(y);
+                    return floats_to_e4m3x2(u.x, u.y) | (floats_to_e4m3x2(v.x, v.y) << 16);
+                };
+                *lo_at = make_uint2(codes(lo[0], lo[1]), codes(lo[2], lo[3]));
+                *hi_at = make_uint2(codes(hi[0], hi[1]), codes(hi[2], hi[3]));
+            }
+        }
+    }
+    if (tid == 0) *scale_at = scale;   // (every thread of the task has read the old one: the reductions lie in between)
+}
+
+}  // namespace fa

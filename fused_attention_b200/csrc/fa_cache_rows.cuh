@@ -1,0 +1,600 @@
+// Attention over the cache for few query rows a key/value head: single tokens, drafted tokens, tokens with a list of pages.
+//
+// The query heads that share a key/value head, and the sequence's T tokens, are rows of one problem: row t * group + i.  A
+// problem is 16 * MT of these rows of one sequence and key/value head (with a list of pages: the rows of one token).  What
+// bounds it is memory, 2 H bytes a token and head, so the work is cut by keys: all problems' units of 128 tokens stand in one
+// row, CTA c of G takes units [c W / G, (c + 1) W / G) of the W there are, whatever problems they belong to, and a problem that
+// several CTAs share is put together by fa_cache_join.  Lengths are only known on the device, so every CTA adds them up itself.
+//
+// Inside a CTA each warp takes 32 tokens of a unit, through a ring of its own in shared memory that cp.async fills: nobody
+// waits for another warp before the end of the problem.  Both products are mma.sync m16n8k16 in fp16 (tcgen05 would need 128
+// rows to be worth its tile): a thread reads the codes of its own fragment straight from the ring, the order of the dimensions
+// in Q K^T and of the tokens in P V being chosen so that they are 16 contiguous bytes, and turns them into fp16, which is exact.
+//
+// Scales: the key scale is multiplied into the fp32 scores.  The value scale goes into the exponent: w = 2^(s + log2 scale - M)
+// with M the running maximum of just that exponent, so that P needs no second rounding and cannot leave fp16, whatever the
+// scales; the row sum takes it out again, l = sum over pages of (sum of w) / scale, in fp32.  M moves only when an exponent passes
+// it by more than 8 (w <= 2^8), so the sums are seldom rescaled.
+#pragma once
+
+#include "fa_cache.cuh"
+
+namespace fa {
+
+constexpr int kRowsWarps = 4;
+constexpr int kRowsStage = 32;                       // tokens of a warp's stage
+constexpr int kRowsUnit = kRowsWarps * kRowsStage;   // tokens of a unit
+constexpr float kRowsSlack = 8.0f;                   // how far an exponent may pass M before M moves
+constexpr uint32_t kNoToken = 0x7FFFFFFFu;           // position of tokens that are not there
+
+struct RowsArgs {
+    CacheView c;
+    CacheSeqs s;
+    const uint8_t* q;
+    uint8_t* y;              // [B, T, heads * H] contiguous
+    const int32_t* pages;    // [B, T, kv heads, keep] or null
+    int64_t q_b, q_t;        // strides in bytes
+    uint32_t group, keep, causal, bf16;
+    uint32_t row_tiles;      // problems of a sequence and key/value head
+    uint32_t rows;           // rows of a problem (at most 16 MT; the last may have fewer)
+    uint32_t min_units;      // units that a CTA takes at least
+    float scale_log2;        // log2(e) / sqrt(H)
+    float* part_o;           // [2 G slots, 16 MT rows, H]
+    float2* part_ml;         // [2 G slots, 16 MT rows]
+    int2* shares;            // [problems]: first and last CTA
+};
+
+template <int H, int MT>
+struct RowsCfg {
+    static constexpr int kRows = 16 * MT;
+    static constexpr int kCodes = kRowsStage * H;                  // bytes of a stage's keys (or values)
+    static constexpr int kMeta = 32;                               // a stage's scales and positions
+    static constexpr int kStageBytes = 2 * kCodes + kMeta;
+    static constexpr int kStages = 2;
+    static constexpr int kRing = kRowsWarps * kStages * kStageBytes;
+    static constexpr int kMerge = kRowsWarps * kRows * H * 4;
+    static constexpr int kTiles = kRing > kMerge ? kRing : kMerge;
+    static constexpr int kQ = kRows * H * 2;
+    static constexpr int kSmem = kTiles + kQ + kRows * 8 + kRowsWarps * kRows * 8 + 64;
+    static constexpr int kCtas = MT == 1 ? 3 : 2;                  // per SM
+};
+
+// Where a CTA's units lie: problems in front of it and inside its sequence.
+struct RowsWork {
+    uint64_t total;   // units of all problems
+    uint32_t ctas;    // that take part
+};
+
+__device__ __forceinline__ uint32_t rows_units(const RowsArgs& p, uint32_t b) {
+    const uint32_t tokens = p.pages != nullptr ? p.keep << p.c.page_shift : cache_length(p.c, p.s, b);
+    return max(1u, (tokens + kRowsUnit - 1) / kRowsUnit);
+}
+// CTA that takes unit u: the last one whose first unit is not behind it.
+__device__ __forceinline__ uint32_t rows_owner(uint64_t u, const RowsWork& w) {
+    return static_cast<uint32_t>(((u + 1) * w.ctas - 1) / w.total);
+}
+
+// 16 bytes of the ring: chunk `c` of row `r`, rows of H bytes, chunks moved about so that the reads below meet few conflicts.
+template <int H>
+__device__ __forceinline__ uint32_t key_chunk(uint32_t r, uint32_t c) {
+    return r * H + ((H == 128 ? c ^ ((r & 1u) << 2) : c) << 4);
+}
+template <int H>
+__device__ __forceinline__ uint32_t value_chunk(uint32_t r, uint32_t c) {
+    return r * H + ((H == 128 ? c ^ (r & 6u) : H == 64 ? c ^ ((r >> 1) & 3u) : c) << 4);
+}
+template <int kBytes>
+__device__ __forceinline__ void ld_codes(uint32_t addr, uint32_t (&w)[kBytes / 4 > 0 ? kBytes / 4 : 1]) {
+    if constexpr (kBytes == 16) {
+        ld_shared_v4(addr, w);
+    } else if constexpr (kBytes == 8) {
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+    } else if constexpr (kBytes == 4) {
+        w[0] = ld_shared_u32(addr);
+    } else {
+        uint16_t h;
+        asm volatile("ld.shared.b16 %0, [%1];" : "=h"(h) : "r"(addr));
+        w[0] = h;
+    }
+}
+
+template <int H, int MT>
+__global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cache_rows(const RowsArgs p) {
+    using Cfg = RowsCfg<H, MT>;
+    constexpr int kThreads = kRowsWarps * 32;
+    constexpr int kHalves = H == 128 ? 2 : 1;            // 64-byte halves of a key row
+    constexpr int kKeyBytes = H >= 64 ? 16 : H / 4;      // that a thread reads of a half
+    constexpr int kValueBytes = H / 8;                   // that a thread reads of a value row
+    constexpr int kTilesN = H / 8;                       // n-tiles of P V
+    extern __shared__ __align__(128) uint8_t smem[];
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, t4 = lane & 3u;
+    const uint32_t ring = smem_u32(smem) + warp * (Cfg::kStages * Cfg::kStageBytes);
+    uint8_t* const q_frag = smem + Cfg::kTiles;
+    float* const s_coef = reinterpret_cast<float*>(q_frag + Cfg::kQ);
+    uint32_t* const s_limit = reinterpret_cast<uint32_t*>(s_coef + Cfg::kRows);
+    float2* const s_ml = reinterpret_cast<float2*>(s_limit + Cfg::kRows);
+    unsigned long long* const s_sum = reinterpret_cast<unsigned long long*>(s_ml + kRowsWarps * Cfg::kRows);
+    grid_dep_wait();
+    grid_dep_launch();
+    const bool bf16 = p.bf16 != 0;
+    const uint32_t per_seq = p.c.heads * p.row_tiles;   // problems of a sequence
+
+    // ---- this CTA's units
+    RowsWork work;
+    {
+        unsigned long long mine = 0;
+        if (p.pages != nullptr) {
+            mine = tid == 0 ? static_cast<unsigned long long>(rows_units(p, 0)) * p.s.B : 0ull;
+        } else {
+            for (uint32_t b = tid; b < p.s.B; b += kThreads) mine += rows_units(p, b);
+        }
+#pragma unroll
+        for (int d = 16; d >= 1; d >>= 1) mine += __shfl_xor_sync(0xFFFFFFFFu, mine, d);
+        if (lane == 0) s_sum[warp] = mine;
+        __syncthreads();
+        work.total = 0;
+#pragma unroll
+        for (int w = 0; w < kRowsWarps; ++w) work.total += s_sum[w];
+        work.total *= per_seq;
+        work.ctas = static_cast<uint32_t>(min(static_cast<uint64_t>(gridDim.x), (work.total + p.min_units - 1) / p.min_units));
+    }
+    if (blockIdx.x >= work.ctas) return;
+    uint64_t unit = blockIdx.x * work.total / work.ctas;
+    const uint64_t unit_end = (blockIdx.x + 1) * work.total / work.ctas;
+    // the sequence of the first unit: warp 0 adds up 32 sequences at a time
+    uint32_t b = 0;
+    uint64_t before = 0;   // units of the sequences in front of b
+    if (p.pages != nullptr) {
+        const uint64_t one = static_cast<uint64_t>(rows_units(p, 0)) * per_seq;
+        b = static_cast<uint32_t>(unit / one);
+        before = b * one;
+    } else {
+        for (uint32_t b0 = 0; b0 < p.s.B; b0 += 32) {   // (every warp for itself)
+            const uint64_t mine = b0 + lane < p.s.B ? static_cast<uint64_t>(rows_units(p, b0 + lane)) * per_seq : 0;
+            uint64_t upto = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint64_t x = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+                if (lane >= d) upto += x;
+            }
+            const uint32_t behind = __ballot_sync(0xFFFFFFFFu, before + upto > unit);
+            if (behind != 0) {
+                const uint32_t at = __ffs(behind) - 1;
+                b = b0 + at;
+                before += __shfl_sync(0xFFFFFFFFu, upto - mine, at);
+                break;
+            }
+            before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+        }
+    }
+
+    uint32_t slot = 2 * blockIdx.x;
+    for (bool first_segment = true; unit < unit_end; first_segment = false) {
+        const uint32_t n_units = rows_units(p, b);
+        const uint32_t within = static_cast<uint32_t>(unit - before);
+        const uint32_t problem = within / n_units, u0 = within % n_units;
+        const uint32_t u1 = static_cast<uint32_t>(min(static_cast<uint64_t>(n_units), u0 + (unit_end - unit)));
+        const uint32_t head = problem / p.row_tiles, tile = problem % p.row_tiles;
+        const uint32_t row0 = tile * p.rows;   // rows of the sequence and head: T * group
+        const uint32_t n_rows = min(p.rows, p.s.T * p.group - row0);
+        const uint32_t held = cache_length(p.c, p.s, b), count = cache_count(p.s, b);
+        if (tid == 0 && u0 == 0 && !cache_length_ok(p.c, p.s, b)) cache_report(p.c.status, kCacheBadPosition);
+
+        // ---- queries into fragments: rows whose fp16 form could overflow (bf16) are scaled by a power of two
+        for (uint32_t r = warp; r < Cfg::kRows; r += kRowsWarps) {
+            const uint32_t t = (row0 + r) / p.group, i = (row0 + r) % p.group;
+            float coef = p.scale_log2;
+            uint32_t limit = r < n_rows ? 0u : kNoToken;   // rows that are not there hold nobody up
+            if (r < n_rows && t < count) {
+                limit = p.causal ? (held + t >= count ? held + t - count + 1 : 0u) : held;
+                limit = min(limit, held);
+                if (bf16) {
+                    const uint16_t* row = reinterpret_cast<const uint16_t*>(p.q + b * p.q_b + t * p.q_t + static_cast<int64_t>(head * p.group + i) * (2 * H));
+                    float most = 0.0f;
+                    for (int d = lane; d < H; d += 32) most = fmaxf(most, fabsf(__uint_as_float(static_cast<uint32_t>(row[d]) << 16)));
+#pragma unroll
+                    for (int d = 16; d >= 1; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
+                    const uint32_t e = max(__float_as_uint(most) >> 23, 40u);   // biased: 2^(e - 127) <= most, unless that is tiny
+                    // to [2^7, 2^8): what does not lie in fp16's range then is 2^-22 of the row's largest or less
+                    if (e < 255) coef *= __uint_as_float((e - 7) << 23);
+                }
+            }
+            if (lane == 0) s_coef[r] = coef, s_limit[r] = limit;
+        }
+        __syncthreads();
+        constexpr int kPart = H >= 32 ? 16 : 8;                          // bytes of a fragment's part: 8 (4) dimensions
+        constexpr int kParts = H >= 64 ? 2 : 1;
+        for (uint32_t item = warp; item < MT * kHalves * 2 * kParts; item += kRowsWarps) {
+            const uint32_t part = item % kParts, upper = item / kParts % 2, half = item / (2 * kParts) % kHalves, mt = item / (2 * kParts * kHalves);
+            const uint32_t r = mt * 16 + upper * 8 + g;
+            const uint32_t t = (row0 + r) / p.group, i = (row0 + r) % p.group;
+            uint32_t w[4] = {0, 0, 0, 0};
+            if (r < n_rows && t < count) {
+                const uint8_t* at = p.q + b * p.q_b + t * p.q_t + static_cast<int64_t>(head * p.group + i) * (2 * H) +
+                                    2 * (half * 64 + t4 * kKeyBytes + part * 8);
+                if constexpr (kPart == 16) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(at);
+                    w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+                } else {
+                    const uint2 x = *reinterpret_cast<const uint2*>(at);
+                    w[0] = x.x, w[1] = x.y;
+                }
+                if (bf16) {
+                    const float f = p.scale_log2 / s_coef[r];   // a power of two
+#pragma unroll
+                    for (int e = 0; e < kPart / 4; ++e) {
+                        const float2 x = unpack_16(w[e], true);
+                        w[e] = pack_half2(x.x * f, x.y * f);
+                    }
+                }
+            }
+            uint8_t* const to = q_frag + (item * 32 + lane) * kPart;
+            if constexpr (kPart == 16) *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+            else *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+        }
+        __syncthreads();
+
+        float coef[MT][2], m[MT][2], l[MT][2], o[MT][kTilesN][4];
+        uint32_t limit[MT][2], nearest = kNoToken, farthest = 0;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                coef[mt][u] = s_coef[mt * 16 + u * 8 + g];
+                limit[mt][u] = s_limit[mt * 16 + u * 8 + g];
+                m[mt][u] = -INFINITY, l[mt][u] = 0.0f;
+            }
+        for (uint32_t r = 0; r < n_rows; ++r) nearest = min(nearest, s_limit[r]), farthest = max(farthest, s_limit[r]);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int j = 0; j < kTilesN; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[mt][j][e] = 0.0f;
+
+        // ---- the ring.  Lane l knows the pages of group l (16 tokens) of the warp's next 16 stages.
+        const uint32_t n_stages = u1 - u0;
+        const uint32_t token_row = (row0 / p.group);   // with a list of pages: the token of the problem
+        const int32_t* const list =
+            p.pages != nullptr ? p.pages + ((static_cast<uint64_t>(b) * p.s.T + token_row) * p.c.heads + head) * p.keep : nullptr;
+        const int32_t* const table = p.s.table + b * p.s.table_stride;
+        int32_t my_page = -1;
+        uint32_t my_at = kNoToken;   // position of the group's first token
+        auto look_up = [&](uint32_t stage) {
+            const uint32_t token = (u0 + stage + (lane >> 1)) * kRowsUnit + warp * kRowsStage + (lane & 1u) * 16;
+            my_page = -1, my_at = kNoToken;
+            if (stage + (lane >> 1) >= n_stages) return;
+            uint32_t block = token >> p.c.page_shift;
+            bool bad = false;
+            if (list != nullptr) {
+                const int32_t chosen = block < p.keep ? list[block] : -1;
+                if (chosen < 0) return;   // (not filled)
+                block = static_cast<uint32_t>(chosen);
+                bad = block >= p.s.width;
+            }
+            const uint64_t at = (static_cast<uint64_t>(block) << p.c.page_shift) + (token & (p.c.page - 1));
+            if (!bad && at < farthest) {
+                my_page = table[block];
+                bad = static_cast<uint32_t>(my_page) >= p.c.n_pages;
+                my_at = static_cast<uint32_t>(at);
+            }
+            if (bad) {
+                my_page = -1, my_at = kNoToken;
+                cache_report(p.c.status, kCacheBadPage);
+            }
+        };
+        auto issue = [&](uint32_t stage) {
+            if (stage < n_stages) {
+                if ((stage & 15u) == 0) look_up(stage);
+                const uint32_t to = ring + (stage % Cfg::kStages) * Cfg::kStageBytes, from_lane = 2 * (stage & 15u);
+                const int32_t page[2] = {__shfl_sync(0xFFFFFFFFu, my_page, from_lane), __shfl_sync(0xFFFFFFFFu, my_page, from_lane + 1)};
+                const uint32_t at[2] = {__shfl_sync(0xFFFFFFFFu, my_at, from_lane), __shfl_sync(0xFFFFFFFFu, my_at, from_lane + 1)};
+                // the first stage of a list may start in the middle of a page, but a group of 16 tokens never spans two
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const bool there = page[half] >= 0;
+                    const int64_t ph = there ? page[half] : 0;
+                    const uint32_t in_page = there ? at[half] & (p.c.page - 1) : 0u;
+                    const uint8_t* const k0 = p.c.k + ph * p.c.k_page + static_cast<int64_t>(head) * p.c.k_head + static_cast<int64_t>(in_page) * p.c.k_token;
+                    const uint8_t* const v0 = p.c.v + ph * p.c.v_page + static_cast<int64_t>(head) * p.c.v_head + static_cast<int64_t>(in_page) * p.c.v_token;
+                    constexpr uint32_t kChunks = H / 16;                 // of a row
+                    const uint32_t c = lane % kChunks;
+#pragma unroll
+                    for (uint32_t r = lane / kChunks; r < 16; r += 32 / kChunks) {
+                        const bool in = there && at[half] + r < farthest;   // (what no row may see is not read: its codes may be anything)
+                        cp_async_16_zero(to + key_chunk<H>(half * 16 + r, c), k0 + (in ? r * p.c.k_token + c * 16 : 0), in);
+                        cp_async_16_zero(to + Cfg::kCodes + value_chunk<H>(half * 16 + r, c), v0 + (in ? r * p.c.v_token + c * 16 : 0), in);
+                    }
+                    if (lane == half) {
+                        const uint32_t meta = to + 2 * Cfg::kCodes + 4 * half;
+                        st_shared_u32(meta + 16, at[half]);
+                        const uint64_t s_at = static_cast<uint64_t>(ph) * p.c.heads + head;
+                        if (there) {
+                            cp_async_4(meta, reinterpret_cast<uint64_t>(p.c.k_scale + s_at));
+                            cp_async_4(meta + 8, reinterpret_cast<uint64_t>(p.c.v_scale + s_at));
+                        } else {
+                            st_shared_u32(meta, 0x3F800000u);
+                            st_shared_u32(meta + 8, 0x3F800000u);
+                        }
+                    }
+                }
+            }
+            cp_async_commit();
+        };
+        issue(0);
+        for (uint32_t stage = 0; stage < n_stages; ++stage) {
+            issue(stage + 1);
+            cp_async_wait_group<1>();
+            __syncwarp();
+            const uint32_t tile_at = ring + (stage % Cfg::kStages) * Cfg::kStageBytes;
+            const uint32_t meta = tile_at + 2 * Cfg::kCodes;
+            const uint32_t at[2] = {ld_shared_u32(meta + 16), ld_shared_u32(meta + 20)};
+            if (min(at[0], at[1]) < farthest) {   // (else no row sees any of it)
+                // ---- S = Q K^T: four n-tiles of 8 tokens
+                float s[MT][4][4];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int n = 0; n < 4; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[mt][n][e] = 0.0f;
+#pragma unroll
+                for (int half = 0; half < kHalves; ++half) {
+                    uint32_t kw[4][kKeyBytes / 4];
+#pragma unroll
+                    for (int n = 0; n < 4; ++n)
+                        if constexpr (H >= 64) ld_codes<16>(tile_at + key_chunk<H>(n * 8 + g, half * 4 + t4), kw[n]);
+                        else ld_codes<kKeyBytes>(tile_at + (n * 8 + g) * H + t4 * kKeyBytes, kw[n]);
+                    uint32_t kf[4][kKeyBytes / 4][2];
+#pragma unroll
+                    for (int n = 0; n < 4; ++n)
+#pragma unroll
+                        for (int j = 0; j < kKeyBytes / 4; ++j) e4m3x4_to_half2(kw[n][j], kf[n][j][0], kf[n][j][1]);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        constexpr int kRegs = kKeyBytes / 2;   // fp16 pairs of a row's half
+                        uint32_t qa[2][kRegs];
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int part = 0; part < kParts; ++part) {
+                                const uint32_t item = ((mt * kHalves + half) * 2 + u) * kParts + part;
+                                const uint32_t from = smem_u32(q_frag) + (item * 32 + lane) * kPart;
+                                uint32_t w[kPart / 4];
+                                ld_codes<kPart>(from, w);
+#pragma unroll
+                                for (int e = 0; e < kPart / 4; ++e) qa[u][part * 4 + e] = w[e];
+                            }
+#pragma unroll
+                        for (int j = 0; j < kKeyBytes / 4; ++j) {
+                            const uint32_t a[4] = {qa[0][2 * j], qa[1][2 * j], qa[0][2 * j + 1], qa[1][2 * j + 1]};
+#pragma unroll
+                            for (int n = 0; n < 4; ++n) mma_m16n8k16(s[mt][n], a, kf[n][j][0], kf[n][j][1]);
+                        }
+                    }
+                }
+                // ---- exponents, weights, row sums
+                float ks[2], vlog[2], vinv[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    ks[u] = __uint_as_float(ld_shared_u32(meta + 4 * u));
+                    const float vs = __uint_as_float(ld_shared_u32(meta + 8 + 4 * u));
+                    const float held_up = vs < 0x1p-100f ? 0x1p-100f : vs;   // (a scale of zero has no logarithm)
+                    vlog[u] = __log2f(held_up);
+                    vinv[u] = exp2f(-vlog[u]);   // of the rounded logarithm, so that the two cancel
+                    if (held_up != held_up) vinv[u] = held_up;
+                }
+                const bool whole = max(at[0], at[1]) < kNoToken && max(at[0], at[1]) + 16 <= nearest;
+                uint32_t pf[MT][4][2];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                    for (int n = 0; n < 4; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int u = e >> 1;
+                            float x = fmaf(s[mt][n][e], coef[mt][u] * ks[n >> 1], vlog[n >> 1]);
+                            if (!whole) {
+                                const uint32_t pos = at[n >> 1] + (n & 1) * 8 + 2 * t4 + (e & 1);
+                                x = at[n >> 1] != kNoToken && pos < limit[mt][u] ? x : -INFINITY;
+                            }
+                            s[mt][n][e] = x;
+                            top[u] = fmaxf(top[u], x);
+                        }
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        top[u] = fmaxf(top[u], __shfl_xor_sync(0xFFFFFFFFu, top[u], 1));
+                        top[u] = fmaxf(top[u], __shfl_xor_sync(0xFFFFFFFFu, top[u], 2));
+                    }
+                    const bool moves = top[0] > m[mt][0] + kRowsSlack || top[1] > m[mt][1] + kRowsSlack;
+                    if (__any_sync(0xFFFFFFFFu, moves)) {
+                        float f[2];
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const float was = m[mt][u];
+                            if (top[u] > was + kRowsSlack) m[mt][u] = top[u];
+                            f[u] = was == m[mt][u] ? 1.0f : ex2_approx(was - m[mt][u]);   // (-inf: 0)
+                            l[mt][u] *= f[u];
+                        }
+#pragma unroll
+                        for (int j = 0; j < kTilesN; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[mt][j][e] *= f[e >> 1];
+                    }
+                    float sum[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+                    const float ref[2] = {m[mt][0] == -INFINITY ? 0.0f : m[mt][0], m[mt][1] == -INFINITY ? 0.0f : m[mt][1]};
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            s[mt][n][e] = ex2_approx(s[mt][n][e] - ref[e >> 1]);
+                            sum[n >> 1][e >> 1] += s[mt][n][e];
+                        }
+                        pf[mt][n][0] = pack_half2(s[mt][n][0], s[mt][n][1]);
+                        pf[mt][n][1] = pack_half2(s[mt][n][2], s[mt][n][3]);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int h2 = 0; h2 < 2; ++h2)   // (a page none of whose tokens the row sees adds nothing, whatever its scale)
+                            l[mt][u] += sum[h2][u] == 0.0f ? 0.0f : sum[h2][u] * vinv[h2];
+                }
+                // ---- O += P V: 16 tokens at a time
+#pragma unroll
+                for (int k16 = 0; k16 < 2; ++k16) {
+                    uint32_t vw[4][kValueBytes / 4 > 0 ? kValueBytes / 4 : 1];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t r = k16 * 16 + (i >> 1) * 8 + 2 * t4 + (i & 1);
+                        uint32_t from = tile_at + Cfg::kCodes;
+                        if constexpr (H == 128) from += value_chunk<H>(r, g);
+                        else if constexpr (H == 64) from += value_chunk<H>(r, g >> 1) + (g & 1u) * 8;
+                        else from += r * H + g * kValueBytes;
+                        ld_codes<kValueBytes>(from, vw[i]);
+                    }
+#pragma unroll
+                    for (int w = 0; w < (kValueBytes + 3) / 4; ++w) {
+                        // byte j of the words of two tokens side by side -> one register of fp16 pairs a dimension
+                        uint32_t b0[4], b1[4];
+                        e4m3x4_to_half2(__byte_perm(vw[0][w], vw[1][w], 0x5140), b0[0], b0[1]);
+                        e4m3x4_to_half2(__byte_perm(vw[2][w], vw[3][w], 0x5140), b1[0], b1[1]);
+                        if constexpr (kValueBytes >= 4) {
+                            e4m3x4_to_half2(__byte_perm(vw[0][w], vw[1][w], 0x7362), b0[2], b0[3]);
+                            e4m3x4_to_half2(__byte_perm(vw[2][w], vw[3][w], 0x7362), b1[2], b1[3]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < (kValueBytes < 4 ? kValueBytes : 4); ++j)
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) {
+                                const uint32_t a[4] = {pf[mt][2 * k16][0], pf[mt][2 * k16][1], pf[mt][2 * k16 + 1][0], pf[mt][2 * k16 + 1][1]};
+                                mma_m16n8k16(o[mt][4 * w + j], a, b0[j], b1[j]);
+                            }
+                    }
+                }
+            }
+            __syncwarp();   // the stage may be filled again
+        }
+        cp_async_wait_all();
+
+        // ---- the four warps' sums together, through the ring's memory
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                l[mt][u] += __shfl_xor_sync(0xFFFFFFFFu, l[mt][u], 1);
+                l[mt][u] += __shfl_xor_sync(0xFFFFFFFFu, l[mt][u], 2);
+                if (t4 == 0) s_ml[warp * Cfg::kRows + mt * 16 + u * 8 + g] = make_float2(m[mt][u], l[mt][u]);
+            }
+        __syncthreads();   // every warp has read its last stage
+        float* const area = reinterpret_cast<float*>(smem) + warp * (Cfg::kRows * H);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t r = mt * 16 + u * 8 + g;
+                float top = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kRowsWarps; ++w) top = fmaxf(top, s_ml[w * Cfg::kRows + r].x);
+                const float f = m[mt][u] == -INFINITY ? 0.0f : ex2_approx(m[mt][u] - top);
+                // n-tile j, column 2 t4 + e: dimension (2 t4 + e) * kTilesN + j
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int j = 0; j < kTilesN; j += 2) {
+                        const uint32_t d = (2 * t4 + e) * kTilesN + j;
+                        float2* const to = reinterpret_cast<float2*>(area + r * H + (d ^ (H >= 64 ? (g & 3u) * 2 : 0u)));
+                        *to = make_float2(o[mt][j][2 * u + e] * f, o[mt][j + 1][2 * u + e] * f);
+                    }
+            }
+        __syncthreads();
+        const bool alone = u0 == 0 && u1 == n_units;
+        for (uint32_t i = tid; i < n_rows * (H / 2); i += kThreads) {
+            const uint32_t r = i / (H / 2), d = 2 * (i % (H / 2));
+            float top = -INFINITY, sum = 0.0f;
+            float2 x = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kRowsWarps; ++w) top = fmaxf(top, s_ml[w * Cfg::kRows + r].x);
+#pragma unroll
+            for (int w = 0; w < kRowsWarps; ++w) {
+                const float2 ml = s_ml[w * Cfg::kRows + r];
+                sum += ml.y * (ml.x == -INFINITY ? 0.0f : ex2_approx(ml.x - top));
+                const float2 y = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(smem) + (w * Cfg::kRows + r) * H +
+                                                                  (d ^ (H >= 64 ? (r & 3u) * 2 : 0u)));
+                x.x += y.x, x.y += y.y;
+            }
+            if (alone) {
+                const uint32_t t = (row0 + r) / p.group, h = head * p.group + (row0 + r) % p.group;
+                const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+                uint8_t* const to = p.y + ((static_cast<uint64_t>(b) * p.s.T + t) * (p.c.heads * p.group) + h) * (2 * H) + 2 * d;
+                *reinterpret_cast<uint32_t*>(to) = pack_16(x.x * f, x.y * f, bf16);
+            } else {
+                const uint32_t s_at = slot + (first_segment ? 0u : 1u);
+                *reinterpret_cast<float2*>(p.part_o + (static_cast<uint64_t>(s_at) * Cfg::kRows + r) * H + d) = x;
+                if (d == 0) p.part_ml[static_cast<uint64_t>(s_at) * Cfg::kRows + r] = make_float2(top, sum);
+            }
+        }
+        if (tid == 0 && u0 == 0) {   // who has a share of the problem, for fa_cache_join
+            const uint64_t begins = before + static_cast<uint64_t>(problem) * n_units;
+            p.shares[static_cast<uint64_t>(b) * per_seq + problem] =
+                make_int2(alone ? -1 : static_cast<int>(2 * blockIdx.x + (first_segment ? 0 : 1)), static_cast<int>(rows_owner(begins + n_units - 1, work)));
+        }
+        unit += u1 - u0;
+        if (unit == before + static_cast<uint64_t>(n_units) * per_seq) before = unit, ++b;
+        __syncthreads();   // the sums have been read: the ring, the rows' data and the fragments may be written again
+    }
+}
+
+// Puts the parts of divided problems together: a CTA per problem and row, a warp per part in turn.
+template <int H, int MT>
+__global__ void __launch_bounds__(128) fa_cache_join(const RowsArgs p) {
+    constexpr int kRows = 16 * MT;
+    __shared__ float s_o[4][H];
+    __shared__ float2 s_ml[4];
+    grid_dep_wait();
+    grid_dep_launch();
+    const bool bf16 = p.bf16 != 0;
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const uint64_t index = blockIdx.x / p.rows;
+    const uint32_t r = blockIdx.x % p.rows;
+    const int2 share = p.shares[index];
+    if (share.x < 0) return;
+    const uint32_t per_seq = p.c.heads * p.row_tiles;
+    const uint32_t b = static_cast<uint32_t>(index / per_seq), problem = static_cast<uint32_t>(index % per_seq);
+    const uint32_t head = problem / p.row_tiles, row = problem % p.row_tiles * p.rows + r;
+    if (row >= p.s.T * p.group) return;
+    const uint32_t first = static_cast<uint32_t>(share.x), last = 2 * static_cast<uint32_t>(share.y);   // slots: first, then the even ones behind it
+    const uint32_t n = (last - (first & ~1u)) / 2 + 1;
+    auto slot = [&](uint32_t i) { return static_cast<uint64_t>(i == 0 ? first : (first & ~1u) + 2 * i) * kRows + r; };
+    float top = -INFINITY;
+    for (uint32_t i = lane; i < n; i += 32) top = fmaxf(top, p.part_ml[slot(i)].x);
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    float sum = 0.0f, x[(H + 31) / 32];
+#pragma unroll
+    for (int d = 0; d < (H + 31) / 32; ++d) x[d] = 0.0f;
+    for (uint32_t i = warp; i < n; i += 4) {
+        const float2 ml = p.part_ml[slot(i)];
+        const float f = ml.x == -INFINITY ? 0.0f : ex2_approx(ml.x - top);
+        sum += ml.y * f;
+#pragma unroll
+        for (int d = 0; d < (H + 31) / 32; ++d)
+            if (H >= 32 || lane < H) x[d] += p.part_o[slot(i) * H + d * 32 + lane] * f;
+    }
+#pragma unroll
+    for (int d = 0; d < (H + 31) / 32; ++d)
+        if (H >= 32 || lane < H) s_o[warp][d * 32 + lane] = x[d];
+    if (lane == 0) s_ml[warp].y = sum;
+    __syncthreads();
+    if (threadIdx.x < H / 2) {
+        const uint32_t d = 2 * threadIdx.x;
+        const float total = (s_ml[0].y + s_ml[1].y) + (s_ml[2].y + s_ml[3].y);
+        const float f = total == 0.0f ? 0.0f : 1.0f / total;
+        const float lo = (s_o[0][d] + s_o[1][d]) + (s_o[2][d] + s_o[3][d]), hi = (s_o[0][d + 1] + s_o[1][d + 1]) + (s_o[2][d + 1] + s_o[3][d + 1]);
+        const uint32_t t = row / p.group, h = head * p.group + row % p.group;
+        uint8_t* const to = p.y + ((static_cast<uint64_t>(b) * p.s.T + t) * (p.c.heads * p.group) + h) * (2 * H) + 2 * d;
+        *reinterpret_cast<uint32_t*>(to) = pack_16(lo * f, hi * f, bf16);
+    }
+}
+
+}  // namespace fa

@@ -1,0 +1,271 @@
+// Selecting the pages of a sequence that a query attends to.
+//
+// Score of a page for a query head: sum over the dimensions of max(q8 lo8, q8 hi8), the largest product that any key within the
+// page's bounds can have, where q8 = rint(q * (1 / max |q| * 127)) and lo8, hi8 = rint(code / 4) are whole numbers of 8 bits.  All
+// sums are whole numbers below 2^24 and exact in fp32 in any order, so that which pages are taken does not depend on how the
+// work is cut, and ties are ties.  The score is multiplied by max |q| * (1 / 127), the maximum over the query heads that share the
+// key/value head is taken and multiplied by the page's key scale.  A product with hi8 is the larger one where q8 >= 0, with lo8
+// where q8 <= 0, so the sum is two matrix products, of the positive part of q8 with hi8 and of the negative part with lo8:
+// mma.sync m16n8k16 on fp16, which holds these numbers exactly.
+//
+// fa_cache_scores reads 2 H + 4 bytes a page and head and is bound by that; a warp takes eight pages, and for several tokens a
+// sequence keeps their bounds in registers for all of them.  fa_cache_take then finds the `keep` highest of a query's scores: the
+// threshold by a search over the bits of the sortable form of the scores, held in registers, then the pages in order.
+#pragma once
+
+#include "fa_cache.cuh"
+
+namespace fa {
+
+struct SelectArgs {
+    CacheView c;
+    CacheSeqs s;
+    const uint8_t* q;
+    int64_t q_b, q_t;        // strides in bytes
+    uint32_t* keys;          // [B, T, kv heads, width]: sortable scores
+    int32_t* pages;          // [B, T, kv heads, keep]
+    uint32_t group, keep, first, last, bf16;
+    uint32_t chunks;         // CTAs that share the pages of a sequence and head
+};
+
+constexpr int kScoreWarps = 4;
+constexpr int kScorePages = 8 * kScoreWarps;   // pages of a CTA at a time
+constexpr int kTakeThreads = 256;
+
+// Whole numbers of the same order as the floats (a NaN above all).
+__device__ __forceinline__ uint32_t sortable(float x) {
+    const uint32_t u = __float_as_uint(x + 0.0f);   // (-0 is 0)
+    return u ^ (u & 0x80000000u ? 0xFFFFFFFFu : 0x80000000u);
+}
+
+// What the queries see: token t of `count` stands at position held - count + t; -1 where there is none.
+__device__ __forceinline__ int64_t query_position(const CacheView& c, const CacheSeqs& s, uint32_t b, uint32_t t) {
+    const int64_t held = cache_length(c, s, b), count = cache_count(s, b);
+    const int64_t at = held - count + t;
+    return t < count && at >= 0 ? at : -1;
+}
+
+template <int H>
+__global__ void __launch_bounds__(kScoreWarps * 32) fa_cache_scores(const SelectArgs p) {
+    constexpr int kHalves = H == 128 ? 2 : 1, kBytes = H >= 64 ? 16 : H / 4, kWords = kBytes / 4;
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3u;
+    grid_dep_wait();
+    grid_dep_launch();
+    const bool bf16 = p.bf16 != 0;
+    uint32_t rest = blockIdx.x;
+    const uint32_t chunk = rest % p.chunks;
+    rest /= p.chunks;
+    const uint32_t head = rest % p.c.heads, b = rest / p.c.heads;
+    const uint32_t held = cache_length(p.c, p.s, b), count = cache_count(p.s, b);
+    if (threadIdx.x == 0 && chunk == 0 && head == 0 && !cache_length_ok(p.c, p.s, b)) cache_report(p.c.status, kCacheBadPosition);
+    if (held == 0 || count == 0) return;
+    const uint32_t n_pages = (held + p.c.page - 1) >> p.c.page_shift;
+
+    for (uint32_t p0 = chunk * kScorePages + warp * 8; p0 < n_pages; p0 += p.chunks * kScorePages) {
+        // ---- bounds of page p0 + g: whole numbers in fp16
+        uint32_t hi[kHalves][kWords][2], lo[kHalves][kWords][2];
+        float scale = 0.0f;
+        const uint32_t mine = p0 + g;
+        int32_t page = -1;
+        if (mine < n_pages) {
+            page = p.s.table[b * p.s.table_stride + mine];
+            if (static_cast<uint32_t>(page) >= p.c.n_pages) {
+                if (t4 == 0) cache_report(p.c.status, kCacheBadPage);
+                page = -1;
+            }
+        }
+        if (page >= 0) scale = p.c.k_scale[static_cast<uint64_t>(page) * p.c.heads + head];
+        const uint8_t* const at = p.c.bounds + (static_cast<uint64_t>(page < 0 ? 0 : page) * p.c.heads + head) * (2 * H) + t4 * kBytes;
+#pragma unroll
+        for (int half = 0; half < kHalves; ++half)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                uint32_t w[4] = {0, 0, 0, 0};
+                if (page >= 0) {
+                    const uint8_t* from = at + e * H + half * 64;
+                    if constexpr (kBytes == 16) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(from);
+                        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+                    } else if constexpr (kBytes == 8) {
+                        const uint2 x = *reinterpret_cast<const uint2*>(from);
+                        w[0] = x.x, w[1] = x.y;
+                    } else {
+                        w[0] = *reinterpret_cast<const uint32_t*>(from);
+                    }
+                }
+                const __half2 quarter = __float2half2_rn(0.25f), round = __float2half2_rn(1536.0f);   // (the unit of fp16 there is 1)
+#pragma unroll
+                for (int j = 0; j < kWords; ++j) {
+                    uint32_t x[2];
+                    e4m3x4_to_half2(w[j], x[0], x[1]);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const __half2 y = __hsub2(__hfma2(*reinterpret_cast<const __half2*>(&x[i]), quarter, round), round);
+                        (e ? hi : lo)[half][j][i] = *reinterpret_cast<const uint32_t*>(&y);
+                    }
+                }
+            }
+        for (uint32_t t = 0; t < count; ++t) {
+            float best[2] = {-INFINITY, -INFINITY};   // of pages p0 + 2 t4, + 1
+            for (uint32_t r0 = 0; r0 < p.group; r0 += 16) {
+                // ---- q8 of heads r0 + g and r0 + g + 8
+                float most[2], raw[2][kHalves][kBytes];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t r = r0 + u * 8 + g;
+                    most[u] = 0.0f;
+                    const uint8_t* const row = p.q + b * p.q_b + t * p.q_t + static_cast<int64_t>(head * p.group + (r < p.group ? r : 0)) * (2 * H) + 2 * t4 * kBytes;
+#pragma unroll
+                    for (int half = 0; half < kHalves; ++half)
+#pragma unroll
+                        for (int j = 0; j < kBytes / 4; ++j) {
+                            uint2 w = make_uint2(0, 0);
+                            if (r < p.group) w = *reinterpret_cast<const uint2*>(row + half * 128 + 8 * j);
+                            const float2 x = unpack_16(w.x, bf16), y = unpack_16(w.y, bf16);
+                            raw[u][half][4 * j] = x.x, raw[u][half][4 * j + 1] = x.y, raw[u][half][4 * j + 2] = y.x, raw[u][half][4 * j + 3] = y.y;
+                            most[u] = fmaxf(most[u], fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y))));
+                        }
+                    most[u] = fmaxf(most[u], __shfl_xor_sync(0xFFFFFFFFu, most[u], 1));
+                    most[u] = fmaxf(most[u], __shfl_xor_sync(0xFFFFFFFFu, most[u], 2));
+                }
+                const float up[2] = {most[0] > 0.0f ? __fmul_rn(__frcp_rn(most[0]), 127.0f) : 0.0f, most[1] > 0.0f ? __fmul_rn(__frcp_rn(most[1]), 127.0f) : 0.0f};
+                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int half = 0; half < kHalves; ++half)
+#pragma unroll
+                    for (int j = 0; j < kWords; ++j) {
+                        uint32_t plus[4], minus[4];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) {
+                                const float x = rintf(__fmul_rn(raw[u][half][4 * j + 2 * i], up[u])), y = rintf(__fmul_rn(raw[u][half][4 * j + 2 * i + 1], up[u]));
+                                plus[2 * i + u] = pack_half2(fmaxf(x, 0.0f), fmaxf(y, 0.0f));
+                                minus[2 * i + u] = pack_half2(fminf(x, 0.0f), fminf(y, 0.0f));
+                            }
+                        mma_m16n8k16(d, plus, hi[half][j][0], hi[half][j][1]);
+                        mma_m16n8k16(d, minus, lo[half][j][0], lo[half][j][1]);
+                    }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int u = e >> 1;
+                    const float x = r0 + u * 8 + g < p.group ? __fmul_rn(d[e], __fmul_rn(most[u], 1.0f / 127.0f)) : -INFINITY;
+                    best[e & 1] = fmaxf(best[e & 1], x);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int dlt = 4; dlt <= 16; dlt <<= 1) best[e] = fmaxf(best[e], __shfl_xor_sync(0xFFFFFFFFu, best[e], dlt));
+            // lane (g, t4) has pages 2 t4 and 2 t4 + 1, the scale of page g: lanes with g = 2 t4 + e write page g
+            const float other = __shfl_sync(0xFFFFFFFFu, best[1], lane >> 3), mine_best = __shfl_sync(0xFFFFFFFFu, best[0], lane >> 3);
+            if (t4 == 0 && mine < n_pages) {
+                const int64_t position = query_position(p.c, p.s, b, t);
+                const int64_t own = position >> p.c.page_shift;
+                float score = __fmul_rn(g & 1u ? other : mine_best, scale);
+                if (page < 0) score = -INFINITY;   // (not to be taken unless it has to be)
+                if (mine < p.first || static_cast<int64_t>(mine) > own - static_cast<int64_t>(p.last)) score = INFINITY;
+                uint32_t key = sortable(score);
+                if (position < 0 || static_cast<int64_t>(mine) > own) key = 0;   // behind the query
+                p.keys[((static_cast<uint64_t>(b) * p.s.T + t) * p.c.heads + head) * p.s.width + mine] = key;
+            }
+        }
+    }
+}
+
+// The CTA's sum of three counts, to all threads.
+__device__ __forceinline__ void count_three(uint32_t (&n)[3], uint32_t (*s)[3], uint32_t& turn) {
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) n[i] = __reduce_add_sync(0xFFFFFFFFu, n[i]);
+    uint32_t (*const at)[3] = s + (turn & 1u) * (kTakeThreads / 32);   // (two buffers: one barrier a sum)
+    ++turn;
+    if (lane == 0)
+#pragma unroll
+        for (int i = 0; i < 3; ++i) at[warp][i] = n[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        n[i] = 0;
+#pragma unroll
+        for (int w = 0; w < kTakeThreads / 32; ++w) n[i] += at[w][i];
+    }
+}
+
+// kHeld: keys of a thread in registers (0: any number, from memory each time).
+template <int kHeld>
+__global__ void __launch_bounds__(kTakeThreads) fa_cache_take(const SelectArgs p) {
+    __shared__ uint32_t s_count[2 * (kTakeThreads / 32)][3];
+    __shared__ uint32_t s_scan[kTakeThreads / 32][2];
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    grid_dep_wait();
+    grid_dep_launch();
+    const uint64_t index = blockIdx.x;   // (b, t, head)
+    const uint64_t bt = index / p.c.heads;
+    const uint32_t t = static_cast<uint32_t>(bt % p.s.T), b = static_cast<uint32_t>(bt / p.s.T);
+    const int64_t position = query_position(p.c, p.s, b, t);
+    const uint32_t n = position < 0 ? 0u : static_cast<uint32_t>((position >> p.c.page_shift) + 1);   // pages that the query sees
+    const uint32_t* const keys = p.keys + index * p.s.width;
+    int32_t* const out = p.pages + index * p.keep;
+    if (n <= p.keep) {
+        for (uint32_t i = tid; i < p.keep; i += kTakeThreads) out[i] = i < n ? static_cast<int32_t>(i) : -1;
+        return;
+    }
+    const uint32_t per = (n + kTakeThreads - 1) / kTakeThreads;   // keys of a thread, one behind the other
+    const uint32_t begin = min(n, tid * per), end = min(n, begin + per);
+    uint32_t mine[kHeld > 0 ? kHeld : 1];
+    if (kHeld > 0) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) mine[i] = begin + i < end ? keys[begin + i] : 0u;   // 0: below every key of a page that is seen
+    }
+    auto each = [&](auto&& f) {
+        if (kHeld > 0) {
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) f(begin + i, mine[i]);
+        } else {
+            for (uint32_t i = begin; i < end; ++i) f(i, keys[i]);
+        }
+    };
+    // the largest value that at least `keep` keys reach, two bits at a time
+    uint32_t least = 0, turn_no = 0;
+    for (int shift = 30; shift >= 0; shift -= 2) {
+        uint32_t reach[3] = {0, 0, 0};
+        each([&](uint32_t, uint32_t key) {
+#pragma unroll
+            for (uint32_t d = 0; d < 3; ++d) reach[d] += key >= (least | ((d + 1) << shift)) ? 1u : 0u;
+        });
+        count_three(reach, s_count, turn_no);
+        least |= (reach[2] >= p.keep ? 3u : reach[1] >= p.keep ? 2u : reach[0] >= p.keep ? 1u : 0u) << shift;
+    }
+    uint32_t above[3] = {0, 0, 0};   // keys above it, of the CTA; and of the thread, above and equal
+    uint32_t mine_above = 0, mine_equal = 0;
+    each([&](uint32_t i, uint32_t key) {
+        if (i < end) mine_above += key > least ? 1u : 0u, mine_equal += key == least ? 1u : 0u;
+    });
+    above[0] = mine_above;
+    count_three(above, s_count, turn_no);
+    const uint32_t ties = p.keep - above[0];   // of the equal ones, the first so many
+    // how many of either the threads in front have
+    uint32_t upto_above = mine_above, upto_equal = mine_equal;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, upto_above, d), y = __shfl_up_sync(0xFFFFFFFFu, upto_equal, d);
+        if (lane >= d) upto_above += x, upto_equal += y;
+    }
+    if (lane == 31) s_scan[warp][0] = upto_above, s_scan[warp][1] = upto_equal;
+    __syncthreads();
+    uint32_t front_above = upto_above - mine_above, front_equal = upto_equal - mine_equal;
+    for (uint32_t w = 0; w < warp; ++w) front_above += s_scan[w][0], front_equal += s_scan[w][1];
+    each([&](uint32_t i, uint32_t key) {
+        if (i >= end) return;
+        if (key > least) {
+            out[front_above + min(front_equal, ties)] = static_cast<int32_t>(i);
+            ++front_above;
+        } else if (key == least) {
+            if (front_equal < ties) out[front_above + front_equal] = static_cast<int32_t>(i);
+            ++front_equal;
+        }
+    });
+}
+
+}  // namespace fa

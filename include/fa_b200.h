@@ -37,7 +37,10 @@ enum {
     FA_B200_ERR_DRIVER = -7,         /* cuTensorMapEncodeTiled unavailable or failed           */
     FA_B200_ERR_FLAGS = -8,          /* contradictory or unknown flag bits                     */
     FA_B200_ERR_DEVICE_TIMEOUT = -9, /* a bounded device-side wait expired (see read_status)   */
-    FA_B200_ERR_TOO_LARGE = -10      /* a fixed-capacity entry point was given too much work   */
+    FA_B200_ERR_TOO_LARGE = -10,     /* a fixed-capacity entry point was given too much work, or
+                                        a call less scratch than it needs                      */
+    FA_B200_ERR_PAGE = -11,          /* page_size not in {16, 32, 64, 128}                     */
+    FA_B200_ERR_DTYPE = -12          /* dtype is neither FA_B200_FP16 nor FA_B200_BF16         */
 };
 
 /* flags for fa_b200_attention_forward */
@@ -290,6 +293,97 @@ int fa_b200_select_kernel(uint32_t B, uint32_t L, uint32_t F, uint32_t head_dim,
  */
 int fa_b200_describe_schedule(uint32_t B, uint32_t L, uint32_t F, uint32_t head_dim,
                               uint32_t flags, uint32_t sm_count, uint32_t out[7]);
+
+/*
+ * ---- The paged 8-bit key/value cache: fa_b200_cache_append, fa_b200_cache_select, fa_b200_cache_attention.
+ *
+ * The keys and values of sequences, in pages of page_size tokens.  A page has for each of kv_heads heads e4m3 codes and one
+ * fp32 scale for its keys and one for its values (a value is code * scale), and the bounds of its keys, the lowest and the
+ * highest code by dimension.  The i-th block of page_size tokens of sequence b lies in page table[b][i].  The scales that
+ * fa_b200_cache_append writes are powers of two; attention and selection take any that are positive.
+ *
+ * What these functions are given is checked before anything is launched, as far as the host can see it.  What lies in device
+ * memory (table, lengths, counts, selected pages) the kernels look at before they use it: tokens whose page is outside the
+ * cache are left out, tokens behind the table or the rotation's last position are not appended, a length that the table has no
+ * room for is cut, and the cache's status block receives the first such code and the number of reports: 1 a page outside the
+ * cache or the table, 2 a position or length outside, 0x100 and above a bounded wait that expired.
+ *
+ * All three are asynchronous on `cuda_stream`, and repeat bit for bit.  None allocates: scratch comes from the caller, need not
+ * be initialised, and may be used again by the next work on the same stream.
+ */
+enum { FA_B200_FP16 = 0u, FA_B200_BF16 = 1u };   /* dtype of 16-bit tensors */
+enum {
+    FA_B200_CACHE_NEIGHBOURS = 1u,   /* fa_b200_cache_append: the rotation's pairs are dimensions (2i, 2i + 1), not (i, i + H/2)   */
+    FA_B200_CACHE_ALL_KEYS = 2u      /* fa_b200_cache_attention: every query sees every key of its sequence                       */
+};
+
+typedef struct fa_b200_cache {
+    void* k;             /* e4m3 codes: page p, head h, token t at p * k_page_stride + h * k_head_stride + t * k_token_stride,   */
+    void* v;             /* head_dim of them in a row.  Strides in bytes, multiples of 16; k, v and bounds on 16-byte boundaries */
+    float* k_scale;      /* [n_pages, kv_heads] */
+    float* v_scale;
+    void* bounds;        /* [n_pages, kv_heads, 2, head_dim]: lowest and highest key code */
+    uint32_t* status;    /* two words, zero until something is wrong */
+    int64_t k_page_stride, k_head_stride, k_token_stride;
+    int64_t v_page_stride, v_head_stride, v_token_stride;
+    uint32_t n_pages, kv_heads, page_size, head_dim;
+} fa_b200_cache;
+
+typedef struct fa_b200_sequences {
+    const int32_t* table;     /* [B, table_width], rows table_stride elements apart; entries that no token reaches may be anything */
+    const int32_t* lengths;   /* [B]: tokens that the cache holds when the call begins */
+    const int32_t* counts;    /* [B]: how many of the call's T tokens a sequence has, or NULL: all of them */
+    int64_t table_stride;
+    uint32_t table_width, B, T;
+} fa_b200_sequences;
+
+/*
+ * Append T tokens to each sequence, at positions lengths[b], lengths[b] + 1, ...: keys and values [B, T, kv_heads * head_dim]
+ * of 16-bit values with the last axis contiguous (strides in elements; rows on 16-byte boundaries).  With cos and sin (fp32
+ * [positions, head_dim / 2]) keys are rotated by their position, x1 c - x2 s and x2 c + x1 s, and so are the queries, which are
+ * written to `rotated` ([B, T, q_heads * head_dim] contiguous, rounded once; zeros where a sequence has no token; without cos
+ * and sin they are copied).  Lengths are not changed.
+ *
+ * A page's scale is the smallest power of two, 2^-100 at least, with which the largest magnitude of its tokens is 448 or less;
+ * a page that held tokens keeps a larger one, and where its scale grows its old codes are moved to the new one (exact but for
+ * subnormal codes).  Codes are rounded to nearest even.  A value that is not finite makes the scale of its page and head NaN and
+ * the codes zero.  Sequences of one call must not append to the same page.
+ */
+int fa_b200_cache_append(const fa_b200_cache* cache, const fa_b200_sequences* sequences, const void* keys, int64_t keys_batch_stride,
+                         int64_t keys_token_stride, const void* values, int64_t values_batch_stride, int64_t values_token_stride,
+                         const void* queries_or_null, int64_t queries_batch_stride, int64_t queries_token_stride, uint32_t q_heads,
+                         void* rotated, const float* cos_or_null, const float* sin_or_null, uint32_t positions, uint32_t dtype,
+                         uint32_t flags, int device, void* cuda_stream);
+
+/*
+ * For each query and key/value head the `keep` pages with the highest scores among those up to the query's own, ascending, into
+ * pages [B, T, kv_heads, keep] (block indices of the sequence, not page numbers; -1 behind the last).  Query t of a sequence
+ * stands at position lengths[b] - counts[b] + t.  Score of a page: with q8 = rint(q * (1 / max |q| * 127)) of a query head and
+ * lo8, hi8 = rint(bound / 4), sum over the dimensions of max(q8 lo8, q8 hi8), a whole number; times max |q| * (1 / 127); the largest
+ * of the query heads of the key/value head; times the page's key scale (each product and quotient rounded to fp32).  Ties go to the lower page.  The first `first` blocks
+ * and the last `last` up to the query's own (at least one) are taken before all others.  Scratch: 4 * B * T * kv_heads *
+ * table_width bytes.
+ */
+int fa_b200_cache_select(const fa_b200_cache* cache, const fa_b200_sequences* sequences, const void* queries, int64_t queries_batch_stride,
+                         int64_t queries_token_stride, uint32_t q_heads, uint32_t dtype, uint32_t keep, uint32_t first, uint32_t last,
+                         int32_t* pages, void* scratch, uint64_t scratch_bytes, int device, void* cuda_stream);
+
+/*
+ * y = softmax(q K^T / sqrt(head_dim)) V over the cache: queries [B, T, q_heads * head_dim] (q_heads a multiple of kv_heads:
+ * query head h has key/value head h / (q_heads / kv_heads)), the last ones of their sequences: query t stands at position
+ * lengths[b] - counts[b] + t and sees the keys up to its own, or all with FA_B200_CACHE_ALL_KEYS.  With `pages`
+ * ([B, T, kv_heads, keep], as fa_b200_cache_select writes them, -1 for nothing) only those blocks.  y is contiguous, of the
+ * queries' type; a query that sees no key, or that its sequence does not have, gets zeros.  Scores, weights and sums are held in
+ * fp32; the weights are rounded to fp16 for the product with V.  Scratch: as fa_b200_cache_attention_scratch says, on a 16-byte
+ * boundary.
+ */
+int fa_b200_cache_attention(const fa_b200_cache* cache, const fa_b200_sequences* sequences, const void* queries, int64_t queries_batch_stride,
+                            int64_t queries_token_stride, uint32_t q_heads, uint32_t dtype, const int32_t* pages_or_null, uint32_t keep,
+                            uint32_t flags, void* y, void* scratch, uint64_t scratch_bytes, int device, void* cuda_stream);
+
+/* out[0] = bytes of scratch that such a call needs (keep = 0 without a list of pages).  Pure arithmetic on the device's facts. */
+int fa_b200_cache_attention_scratch(uint32_t head_dim, uint32_t kv_heads, uint32_t q_heads, uint32_t page_size, uint32_t B, uint32_t T,
+                                    uint32_t table_width, uint32_t keep, int device, uint64_t out[1]);
 
 #ifdef __cplusplus
 }
