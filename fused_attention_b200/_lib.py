@@ -139,6 +139,9 @@ def load() -> ctypes.CDLL:
         lib.fa_b200_cache_attention.argtypes = [cache, seqs] + rows + [u32, u32, vp, u32, u32, vp, vp, u64, i32, vp]
         lib.fa_b200_cache_attention_scratch.restype = i32
         lib.fa_b200_cache_attention_scratch.argtypes = 8 * [u32] + [i32, ctypes.POINTER(u64)]
+        # for the extension module's calls
+        lib.cache_entries = tuple(ctypes.cast(f, vp).value for f in (lib.fa_b200_cache_append, lib.fa_b200_cache_select, lib.fa_b200_cache_attention,
+                                                                     lib.fa_b200_cache_attention_scratch))
         _lib = lib
         return lib
 

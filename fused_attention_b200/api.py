@@ -81,8 +81,8 @@ def _is_fp16_cuda(t, device: int) -> bool:
     return isinstance(t, torch.Tensor) and t.dtype is torch.float16 and t.is_cuda and t.get_device() == device and t.is_contiguous()
 
 
-def _load_native():
-    """The call in native code, from the extension module where it has been built: checks, allocation and launch without
+def _load_native(name: str = "_forward_through"):
+    """A call (``attention_forward``'s, by default) in native code, from the extension module where it has been built: checks, allocation and launch without
     ctypes (B=1 R=4 L=256 H=64: 5.7 us a call, 8.4 through ctypes).  A function that always answers None where there is none,
     or, with a warning, one that cannot be loaded (built for another torch, or from older sources)."""
     from .build import ext_path
@@ -93,7 +93,7 @@ def _load_native():
         spec = importlib.util.spec_from_file_location("fused_attn", path)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
-        return module._forward_through
+        return getattr(module, name)
     except (ImportError, AttributeError, OSError) as e:
         warnings.warn(f"{path} cannot be used, so calls go through ctypes, which takes some 3 us more each: {e}; rebuild it with "
                       "python -m fused_attention_b200.build --ext", RuntimeWarning, stacklevel=3)

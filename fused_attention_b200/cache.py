@@ -22,7 +22,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .api import _raw_stream
+from .api import _load_native, _raw_stream
 
 _DTYPES = {torch.float16: _lib.FP16, torch.bfloat16: _lib.BF16}
 _CODES = torch.float8_e4m3fn
@@ -32,9 +32,23 @@ PAGE_SIZES = (16, 32, 64, 128)
 STATUS = {0: "nothing", 1: "a page outside the cache or the table", 2: "a position or length outside the table or the rotation"}
 
 
+_native = None   # the extension module's calls, and the library's entries that they go to
+
+
 def _require(cond: bool, what: str) -> None:
     if not cond:
         raise RuntimeError(f"cache: {what}")
+
+
+def _calls():
+    """(append, select, attention, entries).  A native call answers None for what is not a plain call with every precondition met,
+    which then goes through the checks and ctypes below; an int is the status of a launch that failed.  (One token of a short
+    sequence: attention 5.6 us a call, 18.8 through ctypes.)"""
+    global _native
+    if _native is None:
+        lib = _lib.load()   # raises when the CUDA library is missing: no fallback
+        _native = tuple(_load_native(f"_cache_{name}_through") for name in ("append", "select", "attention")) + (lib.cache_entries,)
+    return _native
 
 
 class KVCache:
@@ -73,6 +87,7 @@ class KVCache:
         self._status = torch.zeros(2, dtype=torch.int32, device=k.device)
         self._handle = _lib.Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), bounds.data_ptr(), self._status.data_ptr(),
                                   *k.stride()[:3], *v.stride()[:3], n, heads, page, H)
+        self._address = ctypes.addressof(self._handle)
         # (pages on top of one another can be read, as those of a stand-in for a cache, but not written)
         self._writable = all(t.stride(i) > 0 or t.shape[i] == 1 for t in (k, v) for i in range(3))
 
@@ -136,6 +151,13 @@ def cache_append(cache: KVCache, keys: torch.Tensor, values: torch.Tensor, table
     Two sequences must not append to the same page in one call (they may share full pages).
     """
     _require(isinstance(cache, KVCache), "the first argument must be a KVCache")
+    append, _, _, entries = _calls()
+    if cache._writable:
+        done = append(entries[0], cache._address, cache._index, keys, values, table, lengths, counts, queries, rotation, interleaved)
+        if done is not None:
+            if done.__class__ is int:
+                _lib.check(done)
+            return None if done is True else done
     _check_rows(keys, "keys", cache, None, None, cache.head_dim, None)
     B, T, F = keys.shape
     _require(F == cache.kv_heads * cache.head_dim, "keys must have kv_heads * head_dim features")
@@ -180,6 +202,12 @@ def cache_select(cache: KVCache, queries: torch.Tensor, table: torch.Tensor, len
     for ``cache_attention``.  The bounds are rounded to 8 bits for this, and so are the queries.
     """
     _require(isinstance(cache, KVCache), "the first argument must be a KVCache")
+    _, select, _, entries = _calls()
+    pages = select(entries[1], cache._address, cache._index, queries, table, lengths, counts, keep, first, last)
+    if pages is not None:
+        if pages.__class__ is int:
+            _lib.check(pages)
+        return pages
     _check_rows(queries, "queries", cache, None, None, cache.kv_heads * cache.head_dim, None)
     B, T, F = queries.shape
     sequences = _sequences(cache, table, lengths, counts, B, T)
@@ -213,6 +241,12 @@ def cache_attention(cache: KVCache, queries: torch.Tensor, table: torch.Tensor, 
     sequence, each at most once, -1 for nothing.  A query that sees no key, or that its sequence does not have, gets zeros.
     """
     _require(isinstance(cache, KVCache), "the first argument must be a KVCache")
+    _, _, attention, entries = _calls()
+    y = attention(entries[2], entries[3], cache._address, cache._index, queries, table, lengths, counts, pages, causal, out)
+    if y is not None:
+        if y.__class__ is int:
+            _lib.check(y)
+        return y
     _check_rows(queries, "queries", cache, None, None, cache.kv_heads * cache.head_dim, None)
     B, T, F = queries.shape
     sequences = _sequences(cache, table, lengths, counts, B, T)

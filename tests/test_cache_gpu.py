@@ -485,3 +485,42 @@ def test_refusals():
         refuses(what, fa.KVCache, *parts[:i], bad, *parts[i + 1:])
     stacked = fa.KVCache(cache.k[:1].expand(8, G, page, H), cache.v, *parts[2:])
     refuses("on top of one another", fa.cache_append, stacked, kv, kv, table, lengths)
+
+
+def test_native_calls_take_plain_calls_and_agree_with_ctypes(monkeypatch):
+    """The extension module answers every plain call itself, with the bits of the call through ctypes; a slice, a graph or a
+    keyword more do not change that."""
+    import os
+
+    from fused_attention_b200 import build, cache as module
+    assert os.path.exists(build.ext_path()), "the extension module has not been built"
+    H, G, page = 64, 2, 32
+    a, b = random_cache(H, G, 20, page, 1), random_cache(H, G, 20, page, 1)
+    table, lengths = table_of([70, 5], page, 20, 2, width=4)
+    table[table < 0] = 19
+    keys, q, counts = queries_of(2, 3, G * H, torch.bfloat16, 1), queries_of(2, 3, 6 * H, torch.bfloat16, 2), torch.tensor([3, 2], dtype=torch.int32, device="cuda")
+
+    def everything(cache):
+        out = [fa.cache_append(cache, keys, keys, table, lengths, counts=counts, queries=q, rotation=angles(80, H), interleaved=True), cache.k.view(torch.uint8).clone()]
+        assert fa.cache_append(cache, keys, keys, table, lengths) is None
+        pages = fa.cache_select(cache, q, table, lengths, 2, counts=counts, first=0, last=2)
+        given = torch.empty_like(q)
+        y = fa.cache_attention(cache, q, table, lengths, counts=counts, pages=pages, out=given)
+        assert y.data_ptr() == given.data_ptr()
+        return out + [pages, y, fa.cache_attention(cache, q[:, 1:], table, lengths, causal=False)]
+
+    calls = module._calls()
+    answers = []
+
+    def noting(f):
+        def call(*args):
+            answers.append(f(*args))
+            return answers[-1]
+        return call
+
+    monkeypatch.setattr(module, "_native", tuple(noting(f) for f in calls[:3]) + (calls[3],))
+    got = everything(a)
+    assert len(answers) == 5 and not [x for x in answers if x is None or x.__class__ is int]
+    monkeypatch.setattr(module, "_native", (lambda *args: None,) * 3 + (calls[3],))
+    for x, y in zip(got, everything(b)):
+        assert torch.equal(x, y)
