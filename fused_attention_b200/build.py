@@ -54,7 +54,7 @@ def lib_sources() -> list[str]:
 
 
 def cache_sources() -> list[str]:
-    return [os.path.join(CSRC, f) for f in ("fa_cache.cu", "fa_cache.cuh", "fa_cache_append.cuh", "fa_cache_rows.cuh", "fa_cache_select.cuh",
+    return [os.path.join(CSRC, f) for f in ("fa_cache.cu", "fa_cache.cuh", "fa_cache_append.cuh", "fa_cache_prompt.cuh", "fa_cache_rows.cuh", "fa_cache_select.cuh",
                                             "fa_ptx.cuh")] + [os.path.join(ROOT, "include", "fa_b200.h")]
 
 

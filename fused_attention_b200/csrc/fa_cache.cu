@@ -5,6 +5,7 @@
 #include "fa_b200.h"
 #include "fa_cache.cuh"
 #include "fa_cache_append.cuh"
+#include "fa_cache_prompt.cuh"
 #include "fa_cache_rows.cuh"
 #include "fa_cache_select.cuh"
 
@@ -81,6 +82,10 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 bool multiple16(int64_t x) { return (x & 15) == 0; }
 bool head_dim_ok(uint32_t H) { return H == 16 || H == 32 || H == 64 || H == 128; }
 bool page_ok(uint32_t p) { return p == 16 || p == 32 || p == 64 || p == 128; }
+// log2(e) / sqrt(H)
+float scale_log2(uint32_t H) {
+    return static_cast<float>(1.4426950408889634 / (H == 16 ? 4.0 : H == 32 ? 5.656854249492381 : H == 64 ? 8.0 : 11.313708498984761));
+}
 uint32_t log2_of(uint32_t p) { return p == 16 ? 4 : p == 32 ? 5 : p == 64 ? 6 : 7; }
 
 int view_of(const fa_b200_cache* c, fa::CacheView* v) {
@@ -169,6 +174,46 @@ int launch_rows(Device& d, uint32_t bit, const fa::RowsArgs& a, const RowsPlan& 
 template <int H>
 int launch_rows(Device& d, uint32_t bit, const fa::RowsArgs& a, const RowsPlan& plan, cudaStream_t stream) {
     return plan.mt == 1 ? launch_rows<H, 1>(d, bit, a, plan, stream) : launch_rows<H, 2>(d, bit + 1, a, plan, stream);
+}
+
+// ----------------------------------------------------------------------------- attention for many rows
+struct PromptPlan {
+    uint32_t pairs, parts, grid;
+    uint64_t items;             // with their parts
+    uint64_t o_bytes, ml_bytes;
+    uint64_t scratch() const { return 16 + o_bytes + ml_bytes; }   // (never none: there is an address then)
+};
+
+bool use_prompt(uint32_t group, uint32_t T, uint32_t keep) { return keep == 0 && static_cast<uint64_t>(T) * group >= 128; }
+
+// Items of fewer than a round are cut into parts of their keys.  In key steps, a round costs the steps of an item and about two
+// for its beginning and end, with parts three more (their sums go through memory, and a kernel that joins them follows).
+PromptPlan plan_prompt(uint32_t H, uint32_t heads, uint32_t group, uint32_t page, uint32_t B, uint32_t T, uint32_t width, uint32_t sms) {
+    PromptPlan r = {};
+    const uint64_t rows = static_cast<uint64_t>(T) * group;
+    r.pairs = static_cast<uint32_t>((rows + 2 * fa::kPromptTile - 1) / (2 * fa::kPromptTile));
+    const uint64_t whole = static_cast<uint64_t>(B) * heads * r.pairs;
+    const uint64_t steps = (static_cast<uint64_t>(width) * page + fa::kPromptTile - 1) / fa::kPromptTile;
+    uint64_t best = ~0ull;
+    for (uint64_t parts = 1; parts <= 32 && parts <= steps; ++parts) {
+        const uint64_t items = whole * parts;
+        if (parts > 1 && items > 2ull * sms) break;
+        const uint64_t rounds = (items + sms - 1) / sms, cost = rounds * ((steps + parts - 1) / parts + 2) + (parts > 1 ? 3 : 0);
+        if (cost < best) best = cost, r.parts = static_cast<uint32_t>(parts), r.items = items;
+    }
+    r.grid = static_cast<uint32_t>(r.items < sms ? r.items : sms);
+    r.o_bytes = r.parts > 1 ? r.items * 2 * fa::kPromptTile * H * 4 : 0;
+    r.ml_bytes = r.parts > 1 ? r.items * 2 * fa::kPromptTile * 8 : 0;
+    return r;
+}
+
+template <int H>
+int launch_prompt(Device& d, uint32_t bit, const fa::PromptArgs& a, const PromptPlan& plan, cudaStream_t stream) {
+    int rc = allow_smem(d, bit, &fa::fa_cache_prompt<H>, fa::PromptCfg<H>::kSmemBytes);
+    if (rc == FA_B200_OK) rc = launch(&fa::fa_cache_prompt<H>, plan.grid, fa::kPromptThreads, fa::PromptCfg<H>::kSmemBytes, stream, a);
+    if (rc == FA_B200_OK && plan.parts > 1)
+        rc = launch(&fa::fa_cache_prompt_join<H>, static_cast<uint32_t>(plan.items / plan.parts * 2 * fa::kPromptTile / 4), 128, 0, stream, a);
+    return rc;
 }
 
 // ----------------------------------------------------------------------------- appending
@@ -279,7 +324,9 @@ int fa_b200_cache_attention_scratch(uint32_t head_dim, uint32_t kv_heads, uint32
     Device* d = nullptr;
     const int rc = device_of(device, &d);
     if (rc != FA_B200_OK) return rc;
-    out[0] = plan_rows(head_dim, kv_heads, q_heads / kv_heads, page_size, B, T, table_width, keep, static_cast<uint32_t>(d->sms.load())).scratch();
+    const uint32_t sms = static_cast<uint32_t>(d->sms.load()), group = q_heads / kv_heads;
+    out[0] = use_prompt(group, T, keep) ? plan_prompt(head_dim, kv_heads, group, page_size, B, T, table_width, sms).scratch()
+                                        : plan_rows(head_dim, kv_heads, group, page_size, B, T, table_width, keep, sms).scratch();
     return FA_B200_OK;
 }
 
@@ -301,6 +348,28 @@ int fa_b200_cache_attention(const fa_b200_cache* cache, const fa_b200_sequences*
     Device* d = nullptr;
     if ((rc = device_of(device, &d)) != FA_B200_OK) return rc;
     const uint32_t H = cache->head_dim;
+    if (use_prompt(q_heads / a.c.heads, a.s.T, keep)) {
+        const PromptPlan plan = plan_prompt(H, a.c.heads, q_heads / a.c.heads, a.c.page, a.s.B, a.s.T, a.s.width, static_cast<uint32_t>(d->sms.load()));
+        if (plan.items * (2 * fa::kPromptTile) > kMostCtas) return FA_B200_ERR_SHAPE;
+        if (scratch_bytes < plan.scratch()) return FA_B200_ERR_TOO_LARGE;
+        fa::PromptArgs b = {};
+        b.c = a.c, b.s = a.s;
+        b.q = static_cast<const uint8_t*>(queries), b.q_b = 2 * queries_batch_stride, b.q_t = 2 * queries_token_stride;
+        b.y = static_cast<uint8_t*>(y), b.group = q_heads / a.c.heads;
+        b.causal = (flags & FA_B200_CACHE_ALL_KEYS) ? 0u : 1u, b.bf16 = dtype == FA_B200_BF16;
+        b.pairs = plan.pairs, b.parts = plan.parts, b.items = static_cast<uint32_t>(plan.items), b.scale_log2 = scale_log2(H);
+        b.part_o = static_cast<float*>(scratch);
+        b.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(scratch) + plan.o_bytes);
+        OnDevice on(device);
+        if (on.rc != 0) return on.rc;
+        const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+        switch (H) {
+            case 16: return launch_prompt<16>(*d, 8, b, plan, stream);
+            case 32: return launch_prompt<32>(*d, 9, b, plan, stream);
+            case 64: return launch_prompt<64>(*d, 10, b, plan, stream);
+            default: return launch_prompt<128>(*d, 11, b, plan, stream);
+        }
+    }
     const RowsPlan plan = plan_rows(H, a.c.heads, q_heads / a.c.heads, a.c.page, a.s.B, a.s.T, a.s.width, keep, static_cast<uint32_t>(d->sms.load()));
     if (plan.problems * plan.rows > kMostCtas) return FA_B200_ERR_SHAPE;
     if (scratch_bytes < plan.scratch()) return FA_B200_ERR_TOO_LARGE;
@@ -308,7 +377,7 @@ int fa_b200_cache_attention(const fa_b200_cache* cache, const fa_b200_sequences*
     a.y = static_cast<uint8_t*>(y), a.pages = pages_or_null, a.keep = keep;
     a.group = q_heads / a.c.heads, a.causal = (flags & FA_B200_CACHE_ALL_KEYS) ? 0u : 1u, a.bf16 = dtype == FA_B200_BF16;
     a.rows = plan.rows, a.row_tiles = plan.row_tiles, a.min_units = 2;
-    a.scale_log2 = static_cast<float>(1.4426950408889634 / (H == 16 ? 4.0 : H == 32 ? 5.656854249492381 : H == 64 ? 8.0 : 11.313708498984761));
+    a.scale_log2 = scale_log2(H);
     uint8_t* const at = static_cast<uint8_t*>(scratch);
     a.part_o = reinterpret_cast<float*>(at);
     a.part_ml = reinterpret_cast<float2*>(at + plan.o_bytes);

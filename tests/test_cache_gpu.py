@@ -305,8 +305,8 @@ def check_append(cache, before, keys, values, table, held, counts, rotation, int
         start = int(held[b])
         at = start + torch.arange(n, device="cuda")
         if queries is not None:
-            want, size = oracle.rotate(queries[b, :n].double().view(n, -1, H), at, rotation, interleaved)
-            got = rotated[b, :n].double().view(n, -1, H)
+            want, size = oracle.rotate(queries[b, :n].double().view(n, queries.shape[2] // H, H), at, rotation, interleaved)
+            got = rotated[b, :n].double().view(n, queries.shape[2] // H, H)
             unit = UNIT[queries.dtype]
             assert ((got - want).abs() <= unit * want.abs() + 2.0 ** -22 * size + 2.0 ** -25).all() and not rotated[b, n:].any()
         new_k, size = oracle.rotate(keys[b, :n].double().view(n, G, H), at, rotation, interleaved)
@@ -339,7 +339,11 @@ def check_append(cache, before, keys, values, table, held, counts, rotation, int
                     assert ((got[kept:end] - x).abs() <= grain / 2 + 2.0 ** -22 * slack[rows, g] / got_scale).all()
                     if name == "k":
                         bounds = cache.bounds.view(torch.uint8)[p, g].view(torch.float8_e4m3fn).double()
-                        assert torch.equal(bounds, torch.stack((got[:end].amin(0), got[:end].amax(0))))
+                        low, high = got[kept:end].amin(0), got[kept:end].amax(0)
+                        if kept:   # (tokens that the page held and that were taken back since may still be in them)
+                            old = oracle.codes_of(before[2][p, g].view(torch.float8_e4m3fn).double() * (old_scale / got_scale))
+                            low, high = torch.minimum(low, old[0]), torch.maximum(high, old[1])
+                        assert torch.equal(bounds, torch.stack((low, high)))
     for name, now, was in (("k", cache.k.view(torch.uint8), before[0][0]), ("v", cache.v.view(torch.uint8), before[1][0])):
         assert torch.equal(now[untouched[name]], was[untouched[name]])
     for name, now, was in (("ks", cache.k_scale, before[0][1]), ("vs", cache.v_scale, before[1][1])):
