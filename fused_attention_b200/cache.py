@@ -79,6 +79,7 @@ class KVCache:
         for t, name in ((k, "k"), (v, "v")):
             _require(t.stride(3) == 1, f"the last axis of {name} must be contiguous")
             _require(not any(s % 16 for s in t.stride()[:3]), f"the strides of {name} must be multiples of 16")
+            _require(max(t.stride()) < 1 << 31 and t.stride(2) <= 1 << 24, f"the strides of {name} must be below 2^31, its tokens' at most 2^24")
         _require(not any(t.data_ptr() % 16 for t in (k, v, bounds)), "k, v and bounds must start on 16-byte boundaries")
         self.k, self.v, self.k_scale, self.v_scale, self.bounds = k, v, k_scale, v_scale, bounds
         self.n_pages, self.kv_heads, self.page_size, self.head_dim = n, heads, page, H

@@ -97,6 +97,10 @@ int view_of(const fa_b200_cache* c, fa::CacheView* v) {
         !multiple16(c->k_token_stride) || !multiple16(c->v_page_stride) || !multiple16(c->v_head_stride) || !multiple16(c->v_token_stride) ||
         (reinterpret_cast<uintptr_t>(c->k_scale) & 3u) || (reinterpret_cast<uintptr_t>(c->v_scale) & 3u) || (reinterpret_cast<uintptr_t>(c->status) & 3u))
         return FA_B200_ERR_ALIGNMENT;
+    // strides that 32 bits hold (offsets are 64-bit numbers): what a page or a token is apart, in bytes
+    for (int64_t stride : {c->k_page_stride, c->k_head_stride, c->k_token_stride, c->v_page_stride, c->v_head_stride, c->v_token_stride})
+        if (stride < 0 || stride > 0x7FFFFFFFll) return FA_B200_ERR_SHAPE;
+    if (c->k_token_stride > (1 << 24) || c->v_token_stride > (1 << 24)) return FA_B200_ERR_SHAPE;
     v->k = static_cast<uint8_t*>(c->k);
     v->v = static_cast<uint8_t*>(c->v);
     v->k_scale = c->k_scale;
@@ -179,31 +183,38 @@ int launch_rows(Device& d, uint32_t bit, const fa::RowsArgs& a, const RowsPlan& 
 // ----------------------------------------------------------------------------- attention for many rows
 struct PromptPlan {
     uint32_t pairs, parts, grid;
-    uint64_t items;             // with their parts
+    uint64_t whole, items;      // that are not cut; all, with their parts
     uint64_t o_bytes, ml_bytes;
     uint64_t scratch() const { return 16 + o_bytes + ml_bytes; }   // (never none: there is an address then)
 };
 
 bool use_prompt(uint32_t group, uint32_t T, uint32_t keep) { return keep == 0 && static_cast<uint64_t>(T) * group >= 128; }
+// The kernel for many rows knows a page's place as a 32-bit number of 16 bytes.
+bool prompt_reaches(const fa::CacheView& c) {
+    const auto end = [&](int64_t page, int64_t token) { return static_cast<uint64_t>(c.n_pages) * page + static_cast<uint64_t>(c.page) * token; };
+    return end(c.k_page, c.k_token) < (1ull << 36) && end(c.v_page, c.v_token) < (1ull << 36);
+}
 
-// Items of fewer than a round are cut into parts of their keys.  In key steps, a round costs the steps of an item and about two
-// for its beginning and end, with parts three more (their sums go through memory, and a kernel that joins them follows).
+// The items of the last, partial round (all, where there are fewer than SMs) are cut into parts of their keys.  In key steps, a
+// round costs the steps of an item and about two for its beginning and end, with parts three more (their sums go through memory,
+// and a kernel that joins them follows).
 PromptPlan plan_prompt(uint32_t H, uint32_t heads, uint32_t group, uint32_t page, uint32_t B, uint32_t T, uint32_t width, uint32_t sms) {
     PromptPlan r = {};
     const uint64_t rows = static_cast<uint64_t>(T) * group;
     r.pairs = static_cast<uint32_t>((rows + 2 * fa::kPromptTile - 1) / (2 * fa::kPromptTile));
-    const uint64_t whole = static_cast<uint64_t>(B) * heads * r.pairs;
+    const uint64_t all = static_cast<uint64_t>(B) * heads * r.pairs, tail = all % sms;
     const uint64_t steps = (static_cast<uint64_t>(width) * page + fa::kPromptTile - 1) / fa::kPromptTile;
-    uint64_t best = ~0ull;
-    for (uint64_t parts = 1; parts <= 32 && parts <= steps; ++parts) {
-        const uint64_t items = whole * parts;
-        if (parts > 1 && items > 2ull * sms) break;
-        const uint64_t rounds = (items + sms - 1) / sms, cost = rounds * ((steps + parts - 1) / parts + 2) + (parts > 1 ? 3 : 0);
-        if (cost < best) best = cost, r.parts = static_cast<uint32_t>(parts), r.items = items;
+    r.whole = all, r.parts = 1, r.items = all;
+    if (tail != 0) {
+        uint64_t best = steps + 2;
+        for (uint64_t parts = 2; parts <= 32 && parts <= steps && tail * parts <= 2ull * sms; ++parts) {
+            const uint64_t cost = (tail * parts + sms - 1) / sms * ((steps + parts - 1) / parts + 2) + 3;
+            if (cost < best) best = cost, r.parts = static_cast<uint32_t>(parts), r.whole = all - tail, r.items = all - tail + tail * parts;
+        }
     }
     r.grid = static_cast<uint32_t>(r.items < sms ? r.items : sms);
-    r.o_bytes = r.parts > 1 ? r.items * 2 * fa::kPromptTile * H * 4 : 0;
-    r.ml_bytes = r.parts > 1 ? r.items * 2 * fa::kPromptTile * 8 : 0;
+    r.o_bytes = (r.items - r.whole) * 2 * fa::kPromptTile * H * 4;
+    r.ml_bytes = (r.items - r.whole) * 2 * fa::kPromptTile * 8;
     return r;
 }
 
@@ -212,7 +223,7 @@ int launch_prompt(Device& d, uint32_t bit, const fa::PromptArgs& a, const Prompt
     int rc = allow_smem(d, bit, &fa::fa_cache_prompt<H>, fa::PromptCfg<H>::kSmemBytes);
     if (rc == FA_B200_OK) rc = launch(&fa::fa_cache_prompt<H>, plan.grid, fa::kPromptThreads, fa::PromptCfg<H>::kSmemBytes, stream, a);
     if (rc == FA_B200_OK && plan.parts > 1)
-        rc = launch(&fa::fa_cache_prompt_join<H>, static_cast<uint32_t>(plan.items / plan.parts * 2 * fa::kPromptTile / 4), 128, 0, stream, a);
+        rc = launch(&fa::fa_cache_prompt_join<H>, static_cast<uint32_t>((plan.items - plan.whole) / plan.parts * 2 * fa::kPromptTile / 4), 128, 0, stream, a);
     return rc;
 }
 
@@ -325,8 +336,12 @@ int fa_b200_cache_attention_scratch(uint32_t head_dim, uint32_t kv_heads, uint32
     const int rc = device_of(device, &d);
     if (rc != FA_B200_OK) return rc;
     const uint32_t sms = static_cast<uint32_t>(d->sms.load()), group = q_heads / kv_heads;
-    out[0] = use_prompt(group, T, keep) ? plan_prompt(head_dim, kv_heads, group, page_size, B, T, table_width, sms).scratch()
-                                        : plan_rows(head_dim, kv_heads, group, page_size, B, T, table_width, keep, sms).scratch();
+    // (which kernel has a call for many rows depends on the cache too: room for either)
+    out[0] = plan_rows(head_dim, kv_heads, group, page_size, B, T, table_width, keep, sms).scratch();
+    if (use_prompt(group, T, keep)) {
+        const uint64_t prompt = plan_prompt(head_dim, kv_heads, group, page_size, B, T, table_width, sms).scratch();
+        if (prompt > out[0]) out[0] = prompt;
+    }
     return FA_B200_OK;
 }
 
@@ -348,16 +363,16 @@ int fa_b200_cache_attention(const fa_b200_cache* cache, const fa_b200_sequences*
     Device* d = nullptr;
     if ((rc = device_of(device, &d)) != FA_B200_OK) return rc;
     const uint32_t H = cache->head_dim;
-    if (use_prompt(q_heads / a.c.heads, a.s.T, keep)) {
+    if (use_prompt(q_heads / a.c.heads, a.s.T, keep) && prompt_reaches(a.c) && q_heads / a.c.heads < 65536) {
         const PromptPlan plan = plan_prompt(H, a.c.heads, q_heads / a.c.heads, a.c.page, a.s.B, a.s.T, a.s.width, static_cast<uint32_t>(d->sms.load()));
         if (plan.items * (2 * fa::kPromptTile) > kMostCtas) return FA_B200_ERR_SHAPE;
         if (scratch_bytes < plan.scratch()) return FA_B200_ERR_TOO_LARGE;
         fa::PromptArgs b = {};
         b.c = a.c, b.s = a.s;
         b.q = static_cast<const uint8_t*>(queries), b.q_b = 2 * queries_batch_stride, b.q_t = 2 * queries_token_stride;
-        b.y = static_cast<uint8_t*>(y), b.group = q_heads / a.c.heads;
+        b.y = static_cast<uint8_t*>(y), b.group = q_heads / a.c.heads, b.by_group = static_cast<uint32_t>((1ull << 32) / b.group + 1);
         b.causal = (flags & FA_B200_CACHE_ALL_KEYS) ? 0u : 1u, b.bf16 = dtype == FA_B200_BF16;
-        b.pairs = plan.pairs, b.parts = plan.parts, b.items = static_cast<uint32_t>(plan.items), b.scale_log2 = scale_log2(H);
+        b.pairs = plan.pairs, b.parts = plan.parts, b.whole = static_cast<uint32_t>(plan.whole), b.items = static_cast<uint32_t>(plan.items), b.scale_log2 = scale_log2(H);
         b.part_o = static_cast<float*>(scratch);
         b.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(scratch) + plan.o_bytes);
         OnDevice on(device);

@@ -10,6 +10,7 @@
 //   warps 8-11       loading: codes of 128 keys and values a step into registers, a step ahead, from there as fp16 into the ring of
 //                    operand tiles in shared memory (the conversion is exact: no scale is applied to it); queries; scales
 //   warp 12, 14      issue Q K^T, P V (tcgen05.mma, fp32 sums in tensor memory)
+//   warp 13          works out the items
 //
 // Scales.  A step's keys have eight groups of 16 with a scale each for K and V (pages are 16 tokens or more).  As in
 // fa_cache_rows.cuh the exponent of a weight is score * (row's factor * key scale) + log2(value scale) - M, one multiply-add
@@ -36,12 +37,12 @@ struct PromptArgs {
     const uint8_t* q;
     uint8_t* y;              // [B, T, heads * H] contiguous
     int64_t q_b, q_t;        // strides in bytes
-    uint32_t group, causal, bf16;
+    uint32_t group, by_group, causal, bf16;
     uint32_t pairs;          // items of a sequence and key/value head, without their parts
-    uint32_t parts, items;   // items: with their parts
+    uint32_t whole, parts, items;   // the first `whole` items are worked on whole, the others cut into `parts`; items: with their parts
     float scale_log2;        // log2(e) / sqrt(H)
-    float* part_o;           // [items, 256, H]
-    float2* part_ml;         // [items, 256]
+    float* part_o;           // [items - whole, 256, H]
+    float2* part_ml;         // [items - whole, 256]
 };
 
 template <int H>
@@ -57,58 +58,102 @@ struct PromptCfg {
     static constexpr uint32_t kColP0 = kSharedS ? 128 : 320, kColP1 = kSharedS ? 192 : 448;
     static constexpr uint32_t kColO0 = 256, kColO1 = 384;
     static constexpr int kSmemBytes = (2 * kQBuffers + kSlots) * kTileBytes + 1024;
+    // Registers of a thread by role: 128 a thread at launch, so twice the softmax warps' and the others' are 512 at most.  A row of
+    // scores is 128 of them; loading holds 32 of codes at H = 128, 16 or fewer below.
+    static constexpr int kSoftmaxRegs = H == 128 ? 192 : 200, kLoadRegs = H == 128 ? 80 : 64, kIssueRegs = 48;
+    static_assert(2 * kSoftmaxRegs + kLoadRegs + kIssueRegs <= 512, "registers of the four warpgroups");
     // barriers
     static constexpr int QFULL = 0, QEMPTY = QFULL + kQBuffers, FULL = QEMPTY + kQBuffers, EMPTY = FULL + kSlots, S0 = EMPTY + kSlots, SFREE0 = S0 + 2,
-                         P0 = SFREE0 + 2, PV0 = P0 + 2, FINAL = PV0 + 2, FINAL2 = FINAL + 1, COEF = FINAL2 + 1, SCALE = COEF + 4, kBarriers = SCALE + kSlots;
+                         P0 = SFREE0 + 2, PV0 = P0 + 2, FINAL = PV0 + 2, FINAL2 = FINAL + 1, COEF = FINAL2 + 1, SCALE = COEF + 8, ITEM = SCALE + kSlots, IFREE = ITEM + 4,
+                         kBarriers = IFREE + 4;
 };
 
 // Scales of a step's groups as the softmax takes them.
 struct __align__(16) PromptScales {
     float ks[kPromptGroups], vlog[kPromptGroups], vinv[kPromptGroups];
 };
+// Two groups' values.  Volatile: they are loaded where they are used, and not held in registers, of which a row's scores take most.
+__device__ __forceinline__ float2 two_groups(uint32_t addr) {
+    float2 x;
+    asm volatile("ld.volatile.shared.v2.f32 {%0, %1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(addr));
+    return x;
+}
 
 __device__ __forceinline__ uint32_t prompt_swizzled(uint32_t row, uint32_t piece, uint32_t span) {
     return row * span + ((piece ^ ((row * span >> 7) & (span / 16u - 1u))) << 4);
 }
 
-// What an item is, the same for every role.
+// 16 bytes of global memory (zeros where `in` is false: nothing is read then), or 8 and the 8 at `from` + 64.  Volatile: these stand
+// where their registers have just been let go of, long before their use.
+__device__ __forceinline__ void ld_zero_16(const uint8_t* from, bool in, uint4& w) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+                 "@p ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+                 : "=&r"(w.x), "=&r"(w.y), "=&r"(w.z), "=&r"(w.w) : "l"(from), "r"(static_cast<uint32_t>(in)));
+}
+__device__ __forceinline__ void ld_16(const uint8_t* from, uint4& w) {
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "l"(from));
+}
+__device__ __forceinline__ void ld_8_8(const uint8_t* from, uint4& w) {
+    asm volatile("ld.global.v2.u32 {%0, %1}, [%4];\n\tld.global.v2.u32 {%2, %3}, [%4 + 64];" : "=&r"(w.x), "=&r"(w.y), "=&r"(w.z), "=&r"(w.w) : "l"(from));
+}
+
+// What an item is: one warp works it out ahead of the others (lengths come from memory, rows and heads from divisions) and passes it
+// on in shared memory.
 struct PromptItem {
-    uint32_t b, head, row0, part;   // row0: first row, of T * group
-    uint32_t held, count, n_rows;
+    uint32_t b, head;
+    uint32_t t0, first;             // the first row is row `first` of `group` of token t0
+    uint32_t n_rows, held, count;
     uint32_t farthest;              // keys [0, farthest) are seen by some row
     uint32_t step0, steps;          // this part's
+    uint32_t tile_steps[2];         // ... that query tile 0, 1 takes part in: the first of them
+    uint32_t slot;                  // of the part's sums; kNoToken: not a part
+    uint32_t there;                 // 0 behind the last item
 };
-template <int H>
-__device__ __forceinline__ uint32_t prompt_index(const PromptArgs& p, uint32_t round) {
-    const uint32_t c = (round & 1u) ? gridDim.x - 1u - blockIdx.x : blockIdx.x;   // there and back: whoever had the longest of a round has the shortest of the next
-    return round * gridDim.x + c;
+constexpr uint32_t kPromptItems = 4;   // that are known ahead
+
+// Keys [0, ...) that some of the rows [row0, row0 + rows) sees.
+__device__ __forceinline__ uint32_t prompt_farthest(const PromptArgs& p, const PromptItem& it, uint32_t row0, uint32_t rows) {
+    const uint32_t t_first = row0 / p.group, t_end = rows == 0 ? 0u : min(it.count, (row0 + rows - 1u) / p.group + 1u);   // tokens [t_first, t_end)
+    if (t_first >= t_end) return 0;
+    return p.causal ? (it.held + t_end > it.count ? min(it.held, it.held + t_end - it.count) : 0u) : it.held;
 }
 __device__ __forceinline__ PromptItem prompt_item(const PromptArgs& p, uint32_t index) {
     PromptItem it;
     const uint32_t heads = p.s.B * p.c.heads;
-    it.part = index % p.parts;
-    index /= p.parts;
-    const uint32_t bh = index % heads, pair = p.pairs - 1u - index / heads;
+    uint32_t part = 0, parts = 1;
+    it.slot = kNoToken;
+    if (index >= p.whole) {
+        it.slot = index - p.whole;
+        parts = p.parts, part = it.slot % parts, index = p.whole + it.slot / parts;
+    }
+    const uint32_t bh = index % heads, pair = p.pairs - 1u - index / heads, row0 = pair * (2 * kPromptTile);
     it.b = bh / p.c.heads;
     it.head = bh % p.c.heads;
-    it.row0 = pair * (2 * kPromptTile);
-    it.n_rows = min(2u * kPromptTile, p.s.T * p.group - it.row0);
+    it.t0 = row0 / p.group;
+    it.first = row0 % p.group;
+    it.n_rows = min(2u * kPromptTile, p.s.T * p.group - row0);
     it.held = cache_length(p.c, p.s, it.b);
     it.count = cache_count(p.s, it.b);
-    const uint32_t t_first = it.row0 / p.group, t_end = min(it.count, (it.row0 + it.n_rows - 1u) / p.group + 1u);   // tokens [t_first, t_end)
-    it.farthest = 0;
-    if (t_first < t_end) it.farthest = p.causal ? (it.held + t_end > it.count ? min(it.held, it.held + t_end - it.count) : 0u) : it.held;
+    const uint32_t half = min(it.n_rows, static_cast<uint32_t>(kPromptTile));
+    const uint32_t far[2] = {prompt_farthest(p, it, row0, half), prompt_farthest(p, it, row0 + half, it.n_rows - half)};
+    it.farthest = max(far[0], far[1]);
     const uint32_t all = (it.farthest + kPromptTile - 1u) / kPromptTile;
-    it.step0 = all * it.part / p.parts;
-    it.steps = all * (it.part + 1u) / p.parts - it.step0;
+    it.step0 = all * part / parts;
+    it.steps = all * (part + 1u) / parts - it.step0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t mine = (far[i] + kPromptTile - 1u) / kPromptTile;
+        it.tile_steps[i] = mine <= it.step0 ? 0u : min(it.steps, mine - it.step0);
+    }
+    it.there = 1;
     return it;
 }
-// Keys that row r of the item sees.
-__device__ __forceinline__ uint32_t prompt_limit(const PromptArgs& p, const PromptItem& it, uint32_t r) {
-    const uint32_t t = (it.row0 + r) / p.group;
-    if (r >= it.n_rows || t >= it.count) return 0;
-    if (!p.causal) return it.held;
-    return it.held + t >= it.count ? min(it.held, it.held + t - it.count + 1u) : 0u;
+// Token and query head (of the key/value head's) of row r of an item.  `by_group`: 2^32 / group rounded up, with which the product's
+// upper half is the quotient (group < 2^16, and what is divided is less than group + 256).
+__device__ __forceinline__ void prompt_row(const PromptArgs& p, uint32_t t0, uint32_t first, uint32_t r, uint32_t& t, uint32_t& i) {
+    const uint32_t n = first + r, q = p.group == 1 ? n : __umulhi(n, p.by_group);
+    t = t0 + q;
+    i = n - q * p.group;
 }
 
 template <int H>
@@ -131,51 +176,66 @@ __device__ __forceinline__ void prompt_issue_pv(uint32_t tO, uint32_t tP, uint32
     for (int ks = 0; ks < kPromptTile / 16; ++ks) mma_ts(tO, tP + ks * 8, dv + ((ks * 16 * C::kSwz) >> 4), idesc, (accumulate | ks) ? 1u : 0u);
 }
 
-// Weights of the groups [kG0, kG1) of a row, packed as fp16 pairs (8 words a group); adds the groups' sums to `raw`, and to `l`
-// with the value scale divided out.  The exponent is one multiply-add, score * cu + (vlog - ref): `ref` is a whole number, so that
-// with scales that are powers of two the bracket is exact.  kAnySize: of a reference that is too large for that (2^22 and more,
-// where a score's product is no longer known to a fraction) it is taken off the rounded exponent.
-constexpr float kPromptLargeRef = 4194304.0f;
-template <int kG0, int kG1, bool kAnySize = false>
-__device__ __forceinline__ void prompt_weights(const float (&s)[kPromptTile], const PromptScales& sc, float coef, float ref, uint32_t* pk, float& raw, float& l) {
+// Weights of the groups kG0 and kG0 + 1 of a row, packed as fp16 pairs (8 words a group); adds the groups' sums to `l`, with the value
+// scale divided out.  The exponent is one multiply-add, score * cu + (vlog - ref): `ref` is a whole number, so that with scales
+// that are powers of two the bracket is exact.  `shrink`: see prompt_reference.
+template <int kG0>
+__device__ __forceinline__ void prompt_weights(const float (&s)[kPromptTile], uint32_t sc, float coef, float shrink, float ref, uint32_t (&pk)[16], float& l) {
+    const float2 ks = two_groups(sc + 4 * kG0), vlog = two_groups(sc + 4 * (kPromptGroups + kG0)), vinv = two_groups(sc + 4 * (2 * kPromptGroups + kG0));
 #pragma unroll
-    for (int u = kG0; u < kG1; ++u) {
+    for (int half = 0; half < 2; ++half) {
+        const int u = kG0 + half;
         // (at least 1e-37: a masked score, -inf, must stay that)
-        const bool large = kAnySize && fabsf(ref) > kPromptLargeRef;
-        const float cu = fmaxf(coef * sc.ks[u], 1e-37f), add = large ? sc.vlog[u] : sc.vlog[u] - ref, behind = large ? -ref : 0.0f;
+        const float cu = fmaxf(coef * (half ? ks.y : ks.x), 1e-37f), add = fmaf(half ? vlog.y : vlog.x, shrink, -ref);
         const uint64_t c2 = pack_f32x2(cu, cu), a2 = pack_f32x2(add, add);
         uint64_t sum_a = 0, sum_b = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             float x0, x1;
             unpack_f32x2(fma_f32x2(pack_f32x2(s[u * 16 + 2 * e], s[u * 16 + 2 * e + 1]), c2, a2), x0, x1);
-            if (kAnySize) x0 += behind, x1 += behind;
             const float w0 = ex2_approx(x0), w1 = ex2_approx(x1);
             if (e & 1) sum_b = add_f32x2(sum_b, pack_f32x2(w0, w1));
             else sum_a = add_f32x2(sum_a, pack_f32x2(w0, w1));
-            pk[(u - kG0) * 8 + e] = pack_half2(w0, w1);
+            pk[half * 8 + e] = pack_half2(w0, w1);
         }
         float lo, hi;
         unpack_f32x2(add_f32x2(sum_a, sum_b), lo, hi);
-        raw += lo + hi;
-        l = fmaf(lo + hi, sc.vinv[u], l);
+        l = fmaf(lo + hi, half ? vinv.y : vinv.x, l);
     }
 }
-// Largest exponent of a row, rounded up to a whole number.
-__device__ __forceinline__ float prompt_top(const float (&s)[kPromptTile], const PromptScales& sc, float coef) {
+// Largest exponent of a row.
+__device__ __forceinline__ float prompt_top(const float (&s)[kPromptTile], uint32_t sc, float coef, float shrink) {
     float top = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < kPromptGroups; ++u) {
-        float a = max3(s[u * 16], s[u * 16 + 1], s[u * 16 + 2]), b = max3(s[u * 16 + 3], s[u * 16 + 4], s[u * 16 + 5]);
+    for (int u = 0; u < kPromptGroups; u += 2) {
+        const float2 ks = two_groups(sc + 4 * u), vlog = two_groups(sc + 4 * (kPromptGroups + u));
 #pragma unroll
-        for (int e = 6; e < 14; e += 4) {
-            a = max3(a, s[u * 16 + e], s[u * 16 + e + 1]);
-            b = max3(b, s[u * 16 + e + 2], s[u * 16 + e + 3]);
+        for (int half = 0; half < 2; ++half) {
+            const float* x = s + (u + half) * 16;
+            float a = max3(x[0], x[1], x[2]), b = max3(x[3], x[4], x[5]);
+#pragma unroll
+            for (int e = 6; e < 14; e += 4) {
+                a = max3(a, x[e], x[e + 1]);
+                b = max3(b, x[e + 2], x[e + 3]);
+            }
+            top = fmaxf(top, fmaf(max3(a, b, fmaxf(x[14], x[15])), fmaxf(coef * (half ? ks.y : ks.x), 1e-37f), (half ? vlog.y : vlog.x) * shrink));
         }
-        a = max3(a, s[u * 16 + 14], s[u * 16 + 15]);
-        top = fmaxf(top, fmaf(fmaxf(a, b), fmaxf(coef * sc.ks[u], 1e-37f), sc.vlog[u]));
     }
-    return ceilf(top);
+    return top;
+}
+// A new reference for a row whose largest exponent is `top`, and the factor for the sums so far.  Beside one of 2^22 and more an
+// exponent would not be known to a fraction, and a weight could exceed fp16: all the row's exponents are then shrunk by a power of
+// two that brings it below.  The largest stays the largest, and exponents of that size differ by whole numbers or not at all, so
+// that hardly anything but the largest counts before and after.
+__device__ __forceinline__ float prompt_reference(float top, float& m, float& coef, float& shrink) {
+    const float grown = 1.0f / shrink, whole = top * grown;
+    const uint32_t size = (__float_as_uint(whole) >> 23) & 0xFFu;   // biased exponent
+    const float now = size > 127u + 22u ? __uint_as_float((127u + 127u + 22u - size) << 23) : 1.0f;
+    const float m_new = ceilf(whole * now), alpha = ex2_approx(m * grown - m_new * (1.0f / now));
+    m = m_new;
+    coef *= grown * now;
+    shrink = now;
+    return alpha;
 }
 
 template <int H>
@@ -185,9 +245,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[C::kBarriers];
     __shared__ PromptScales scales[NS];           // of step g in entry g % NS (free when the V tile of that step is)
-    // Rows' factors, by item.  Four: item k + 4's are written once the last Q K^T of item k + 2 (or a later one) has retired, which
-    // needs the scores of item k + 1 read; whoever read those has long taken its factor of item k.
-    __shared__ float s_coef[4][2 * kPromptTile];
+    // Rows' factors, by item.  Eight, because loading may be ahead of a softmax by no more than the ring has steps (four at most):
+    // a step's V tile is let go of when both tiles that take part in the step have given their P.
+    __shared__ float s_coef[8][2 * kPromptTile];
+    __shared__ PromptItem items[kPromptItems];
     __shared__ uint32_t tmem_slot, abort_flag;
 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
@@ -203,7 +264,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
         for (int i = 0; i < C::kBarriers; ++i) {
             const bool by_loaders = (i >= C::QFULL && i < C::QEMPTY) || (i >= C::FULL && i < C::EMPTY) || (i >= C::COEF && i < C::SCALE);
             const bool by_softmax = i >= C::SFREE0 && i < C::PV0;
-            mbar_init(bar(i), by_loaders || by_softmax ? 4u : 1u);
+            // (an item is let go of by 8 softmax warps, 4 loading and 2 issuing)
+            mbar_init(bar(i), i >= C::IFREE ? 14u : by_loaders || by_softmax ? 4u : 1u);
         }
         abort_flag = 0;
         fence_mbar_init();
@@ -218,29 +280,40 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
     grid_dep_wait();
     grid_dep_launch();
     const uint32_t tmem = tmem_slot;
+    auto item_wait = [&](uint32_t n) { return mbar_wait(bar(C::ITEM + n % kPromptItems), (n / kPromptItems) & 1u, ctl, kCacheTimeout | C::ITEM); };
+    auto item_done = [&](uint32_t n) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::IFREE + n % kPromptItems));
+    };
 
     if (warp < 8) {
         // ---------------------------------------------------------------- softmax of tile i
-        setmaxnreg_inc<184>();
+        setmaxnreg_inc<C::kSoftmaxRegs>();
         const uint32_t i = warp >> 2, r = tid & 127u, lane_off = ((warp & 3u) * 32u) << 16;
         const uint32_t tS = tmem + lane_off + (i ? C::kColS1 : C::kColS0), tP = tmem + lane_off + (i ? C::kColP1 : C::kColP0),
                        tO = tmem + lane_off + (i ? C::kColO1 : C::kColO0);
-        uint32_t g = 0, k = 0;
-        for (uint32_t round = 0;; ++round) {
-            const uint32_t index = prompt_index<H>(p, round);
-            if (round * gridDim.x >= p.items) break;
-            if (index >= p.items) continue;
-            const PromptItem it = prompt_item(p, index);
-            const uint32_t row = i * kPromptTile + r, limit = prompt_limit(p, it, row);
-            // rows that see nothing count as seeing everything: nobody waits for them, and they are written as zeros
+        uint32_t g = 0, k = 0, before = 0;   // this tile's steps, items with steps, steps of the items in front of this one
+        for (uint32_t nth = 0;; ++nth) {
+            if (!item_wait(nth)) break;
+            const volatile PromptItem& it = items[nth % kPromptItems];   // (read where it is needed, not held in registers)
+            if (it.there == 0) break;
+            const uint32_t row = i * kPromptTile + r, steps = it.tile_steps[i];
+            uint32_t key0 = it.step0 * kPromptTile, step = before, limit, t, h;
+            prompt_row(p, it.t0, it.first, row, t, h);
+            {   // keys that the row sees
+                const uint32_t held = it.held, count = it.count;
+                limit = !p.causal ? held : held + t >= count ? min(held, held + t - count + 1u) : 0u;
+                if (row >= it.n_rows || t >= count) limit = 0;
+            }
+            // a row that sees nothing counts as seeing everything, so that nobody waits for it, and is written as zeros
             const uint32_t masked_from = limit == 0 ? kNoToken : limit;
-            float m = -INFINITY, l = 0.0f, coef = 0.0f;
-            if (it.steps > 0) {
-                mbar_wait(bar(C::COEF + (k & 3u)), (k >> 2) & 1u, ctl, kCacheTimeout | C::COEF);
-                coef = s_coef[k & 3u][row];
+            float m = -INFINITY, l = 0.0f, coef = 0.0f, shrink = 1.0f;
+            if (steps > 0) {
+                mbar_wait(bar(C::COEF + (k & 7u)), (k >> 3) & 1u, ctl, kCacheTimeout | C::COEF);
+                coef = s_coef[k & 7u][row];
             }
 #pragma unroll 1
-            for (uint32_t j = 0; j < it.steps; ++j, ++g) {
+            for (uint32_t j = 0; j < steps; ++j, ++g, ++step, key0 += kPromptTile) {
                 mbar_wait(bar(C::S0 + i), g & 1u, ctl, kCacheTimeout | (C::S0 + i));
                 tc_fence_after();
                 __syncwarp();
@@ -251,80 +324,56 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(C::SFREE0 + (C::kSharedS ? 0 : i)));
-                const PromptScales& sc = scales[g % NS];
-                mbar_wait(bar(C::SCALE + g % NS), (g / NS) & 1u, ctl, kCacheTimeout | C::SCALE);
-                const uint32_t key0 = (it.step0 + j) * kPromptTile;
+                const uint32_t sc = smem_u32(scales) + (step % NS) * static_cast<uint32_t>(sizeof(PromptScales));
+                mbar_wait(bar(C::SCALE + step % NS), (step / NS) & 1u, ctl, kCacheTimeout | C::SCALE);
                 if (__any_sync(0xFFFFFFFFu, key0 + kPromptTile > masked_from)) {
                     const int valid = static_cast<int>(masked_from) - static_cast<int>(key0);
 #pragma unroll
-                    for (int e = 0; e < kPromptTile; ++e)
-                        if (e >= valid) s[e] = -INFINITY;
+                    for (int w = 0; w < 4; ++w) {   // (a bit a score: fewer instructions than a comparison each, 180 us against 184 with 16 prompts of 777)
+                        const int left = valid - w * 32;
+                        const uint32_t seen = left >= 32 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << left) - 1u;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!(seen >> e & 1u)) s[w * 32 + e] = -INFINITY;
+                    }
                 }
-                if (j == 0) m = prompt_top(s, sc, coef);
-                // the first quarter's weights are kept in registers: the last step's P V may still be reading P
-                uint32_t held[16];
-                float raw = 0.0f, sum = 0.0f;
+                // The reference moves when an exponent exceeds it by more than 8 (weights stay below 2^9); a row that has seen nothing
+                // yet takes the first that it sees.
+                const float top = prompt_top(s, sc, coef, shrink);
+                float alpha = 1.0f;
+                if (__any_sync(0xFFFFFFFFu, top > m + kRowsSlack)) {
+                    if (top > m + kRowsSlack) alpha = prompt_reference(top, m, coef, shrink);
+                    l *= alpha;
+                }
                 const float ref = m == -INFINITY ? 0.0f : m;
-                prompt_weights<0, 2>(s, sc, coef, ref, held, raw, sum);
+                // the first quarter's weights are kept in registers: the last step's P V may still be reading P
+                uint32_t pk[16];
+                prompt_weights<0>(s, sc, coef, shrink, ref, pk, l);
                 if (g > 0) {
                     mbar_wait(bar(C::PV0 + i), (g - 1u) & 1u, ctl, kCacheTimeout | (C::PV0 + i));
                     tc_fence_after();
                 }
                 __syncwarp();
-                tmem_st16(tP, held);
+                tmem_st16(tP, pk);
+                prompt_weights<2>(s, sc, coef, shrink, ref, pk, l);
+                tmem_st16(tP + 16, pk);
+                prompt_weights<4>(s, sc, coef, shrink, ref, pk, l);
+                tmem_st16(tP + 32, pk);
+                prompt_weights<6>(s, sc, coef, shrink, ref, pk, l);
+                tmem_st16(tP + 48, pk);
+                if (j > 0 && __any_sync(0xFFFFFFFFu, alpha != 1.0f)) {   // (an item's first P V overwrites O)
+                    // here, where the scores' registers are free; the last step's P V has retired, and the next waits for P
+                    constexpr int kCols = 16;
+#pragma unroll 1
+                    for (int c = 0; c < H; c += kCols) {
+                        float o[kCols];
+                        uint32_t w[kCols];
+                        tmem_ld16(tO + c, o);
+                        tmem_wait_ld();
 #pragma unroll
-                for (int c = 1; c < 4; ++c) {
-                    uint32_t pk[16];
-                    if (c == 1) prompt_weights<2, 4>(s, sc, coef, ref, pk, raw, sum);
-                    if (c == 2) prompt_weights<4, 6>(s, sc, coef, ref, pk, raw, sum);
-                    if (c == 3) prompt_weights<6, 8>(s, sc, coef, ref, pk, raw, sum);
-                    tmem_st16(tP + c * 16, pk);
-                }
-                // M has to move when a weight exceeds 2^8, which none does while the row's sum stays below; a row that has seen
-                // nothing so far takes the maximum of what it sees first
-                bool moved = false;
-                float top = m;
-                const bool large = fabsf(m) > kPromptLargeRef && m != -INFINITY;
-                if (__any_sync(0xFFFFFFFFu, !(raw <= 255.0f) || (m == -INFINITY && j > 0) || large)) {
-                    top = prompt_top(s, sc, coef);
-                    moved = top > m + kRowsSlack;
-                }
-                if (__any_sync(0xFFFFFFFFu, moved || large)) {
-                    const float m_new = moved ? top : m, alpha = moved ? ex2_approx(m - m_new) : 1.0f;
-                    m = m_new;
-                    const float ref2 = m == -INFINITY ? 0.0f : m;
-                    raw = sum = 0.0f;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t pk[16];
-                        if (c == 0) prompt_weights<0, 2, true>(s, sc, coef, ref2, pk, raw, sum);
-                        if (c == 1) prompt_weights<2, 4, true>(s, sc, coef, ref2, pk, raw, sum);
-                        if (c == 2) prompt_weights<4, 6, true>(s, sc, coef, ref2, pk, raw, sum);
-                        if (c == 3) prompt_weights<6, 8, true>(s, sc, coef, ref2, pk, raw, sum);
-                        tmem_st16(tP + c * 16, pk);
+                        for (int e = 0; e < kCols; ++e) w[e] = __float_as_uint(o[e] * alpha);
+                        tmem_st16(tO + c, w);
                     }
-                    l = l * alpha + sum;
-                    if (j > 0) {   // (an item's first P V overwrites O)
-                        constexpr int kCols = H < 32 ? 16 : 32;
-#pragma unroll
-                        for (int c = 0; c < H; c += kCols) {
-                            float o[kCols];
-                            tmem_ld<kCols>(tO + c, o);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int e = 0; e < kCols; ++e) o[e] *= alpha;
-                            if constexpr (kCols == 32) {
-                                tmem_st32(tO + c, o);
-                            } else {
-                                uint32_t w[16];
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(o[e]);
-                                tmem_st16(tO + c, w);
-                            }
-                        }
-                    }
-                } else {
-                    l += sum;
                 }
                 tmem_wait_st();
                 tc_fence_before();
@@ -332,22 +381,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
                 if (lane == 0) mbar_arrive(bar(C::P0 + i));
             }
             // ---- the item's end: this row of O.  (The next item's first P V waits for P from these warps.)
-            if (it.steps > 0) {
-                ++k;
+            const bool any = steps > 0, there = row < it.n_rows;
+            if (it.steps > 0) ++k, before += it.steps;
+            if (any) {
                 mbar_wait(bar(C::PV0 + i), (g - 1u) & 1u, ctl, kCacheTimeout | (C::PV0 + i));
                 tc_fence_after();
                 __syncwarp();
             }
-            const bool there = row < it.n_rows;
-            if (p.parts == 1) {
-                const float f = limit == 0 || l == 0.0f ? 0.0f : 1.0f / l;
-                const uint32_t t = (it.row0 + row) / p.group, h = it.head * p.group + (it.row0 + row) % p.group;
-                uint8_t* const to = p.y + ((static_cast<uint64_t>(it.b) * p.s.T + t) * (p.c.heads * p.group) + h) * (2 * H);
+            const uint32_t slot = it.slot;
+            if (slot == kNoToken) {
+                const float f = masked_from == kNoToken || l == 0.0f ? 0.0f : 1.0f / l;
+                prompt_row(p, it.t0, it.first, row, t, h);
+                uint8_t* const to = p.y + ((static_cast<uint64_t>(it.b) * p.s.T + t) * (p.c.heads * p.group) + it.head * p.group + h) * (2 * H);
                 constexpr int kCols = H < 32 ? 16 : 32;
 #pragma unroll 1
                 for (int c = 0; c < H; c += kCols) {
                     float o[kCols];
-                    if (it.steps > 0) {
+                    if (any) {
                         tmem_ld<kCols>(tO + c, o);
                         tmem_wait_ld();
                     }
@@ -355,7 +405,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
 #pragma unroll
                         for (int e = 0; e < kCols; e += 8) {
                             uint4 w = make_uint4(0, 0, 0, 0);
-                            if (limit != 0)
+                            if (masked_from != kNoToken)
                                 w = make_uint4(pack_16(o[e] * f, o[e + 1] * f, p.bf16), pack_16(o[e + 2] * f, o[e + 3] * f, p.bf16),
                                                pack_16(o[e + 4] * f, o[e + 5] * f, p.bf16), pack_16(o[e + 6] * f, o[e + 7] * f, p.bf16));
                             *reinterpret_cast<uint4*>(to + 2 * (c + e)) = w;
@@ -363,10 +413,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
                     }
                 }
             } else {
-                const uint64_t at = static_cast<uint64_t>(index) * (2 * kPromptTile) + row;
+                const uint64_t at = static_cast<uint64_t>(slot) * (2 * kPromptTile) + row;
                 constexpr int kCols = H < 32 ? 16 : 32;
-                if (there) p.part_ml[at] = make_float2(limit == 0 || it.steps == 0 ? -INFINITY : m, limit == 0 || it.steps == 0 ? 0.0f : l);
-                if (it.steps > 0)
+                if (there) p.part_ml[at] = make_float2(masked_from == kNoToken || !any ? -INFINITY : m / shrink, masked_from == kNoToken || !any ? 0.0f : l);
+                if (any)
 #pragma unroll 1
                     for (int c = 0; c < H; c += kCols) {
                         float o[kCols];
@@ -379,113 +429,129 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
                     }
             }
             tc_fence_before();
+            item_done(nth);
         }
     } else if (warp < 12) {
         // ---------------------------------------------------------------- loading
-        setmaxnreg_dec<80>();
+        setmaxnreg_dec<C::kLoadRegs>();
         constexpr uint32_t kLanes = H / 16;                // that share a row of codes, 16 each
         constexpr uint32_t kRowsPass = 128 / kLanes;
         constexpr uint32_t kPasses = kPromptTile / kRowsPass;
+        constexpr uint32_t kFirst = H == 128 ? 8 : 16;     // distance of the lanes' first codes
         const uint32_t lt = tid - 256u, j16 = lt % kLanes, r_in = lt / kLanes;
         uint32_t n = 0, k = 0, g = 0;   // ring items, items, steps so far
-        for (uint32_t round = 0;; ++round) {
-            const uint32_t index = prompt_index<H>(p, round);
-            if (round * gridDim.x >= p.items) break;
-            if (index >= p.items) continue;
-            const PromptItem it = prompt_item(p, index);
+        for (uint32_t nth = 0;; ++nth) {
+            if (!item_wait(nth)) break;
+            const PromptItem& it = items[nth % kPromptItems];
+            if (it.there == 0) break;
             if (it.steps == 0) {
-                if (lt == 0 && !cache_length_ok(p.c, p.s, it.b)) cache_report(p.c.status, kCacheBadPosition);
+                item_done(nth);
                 continue;
             }
-            if (lt == 0 && it.part == 0 && !cache_length_ok(p.c, p.s, it.b)) cache_report(p.c.status, kCacheBadPosition);
             const int32_t* const table = p.s.table + it.b * p.s.table_stride;
             // ---- a step's pages: lane l (of every warp) has group l's.  The table entry is asked for a step ahead, the scales half
             // a step: nothing may depend at once on what has just been asked for.
-            int32_t page = -1, entry = -1;
-            bool wanted = false;
+            // A group's place is a multiple of 16 bytes from its head's first page; what is not there is read from that page and thrown
+            // away (`spoilt`), so that loads depend on nothing but their address.
+            int32_t entry = -1;
+            bool wanted = false, none = false;
             float ks = 1.0f, vs = 1.0f;
+            uint32_t k_at = 0, v_at = 0;
             auto ask = [&](uint32_t step) {
                 const uint32_t at = (it.step0 + step) * kPromptTile + (lane & 7u) * 16u;
                 wanted = step < it.steps && at < it.farthest;
                 entry = wanted ? table[at >> p.c.page_shift] : -1;
             };
             auto look_up = [&] {
-                page = entry, ks = 1.0f, vs = 1.0f;
-                if (static_cast<uint32_t>(page) >= p.c.n_pages) {
+                ks = 1.0f, vs = 1.0f;
+                none = static_cast<uint32_t>(entry) >= p.c.n_pages;
+                k_at = v_at = 0;
+                if (none) {
                     if (wanted && lane < 8 && warp == 8) cache_report(p.c.status, kCacheBadPage);
-                    page = -1;
                 } else {
-                    const uint64_t s_at = static_cast<uint64_t>(page) * p.c.heads + it.head;
+                    const uint64_t s_at = static_cast<uint64_t>(entry) * p.c.heads + it.head;
                     ks = p.c.k_scale[s_at], vs = p.c.v_scale[s_at];
+                    const uint32_t in_page = ((lane & 7u) * 16u) & (p.c.page - 1);
+                    k_at = static_cast<uint32_t>((static_cast<uint64_t>(entry) * p.c.k_page + in_page * p.c.k_token) >> 4);
+                    v_at = static_cast<uint32_t>((static_cast<uint64_t>(entry) * p.c.v_page + in_page * p.c.v_token) >> 4);
                 }
             };
             uint4 codes[kPasses];
-            // pass c of a step's keys (values): this thread's 16 codes; zeros where no row sees the token
-            auto load = [&](uint32_t c, uint32_t step, bool is_v) {
-                const uint32_t r = c * kRowsPass + r_in, at = (it.step0 + step) * kPromptTile + r;
-                const int32_t pg = __shfl_sync(0xFFFFFFFFu, page, r >> 4);
-                uint4 w = make_uint4(0, 0, 0, 0);
-                if (pg >= 0 && at < it.farthest) {
-                    const int64_t in_page = at & (p.c.page - 1);
-                    w = *reinterpret_cast<const uint4*>(is_v ? p.c.v + pg * p.c.v_page + it.head * p.c.v_head + in_page * p.c.v_token + 16 * j16
-                                                             : p.c.k + pg * p.c.k_page + it.head * p.c.k_head + in_page * p.c.k_token + 16 * j16);
-                }
-                codes[c] = w;
+            const uint8_t* const k_base = p.c.k + it.head * p.c.k_head + (r_in & 15u) * p.c.k_token + kFirst * j16;
+            const uint8_t* const v_base = p.c.v + it.head * p.c.v_head + (r_in & 15u) * p.c.v_token + kFirst * j16;
+            // pass c of a step's keys (values): this thread's 16 codes
+            auto load = [&](uint32_t c, bool is_v) {
+                const uint32_t group_at = __shfl_sync(0xFFFFFFFFu, is_v ? v_at : k_at, (c * kRowsPass + r_in) >> 4);
+                const uint8_t* const from = (is_v ? v_base : k_base) + static_cast<uint64_t>(group_at) * 16u;
+                if constexpr (H == 128) ld_8_8(from, codes[c]);   // eight codes of either operand box
+                else ld_16(from, codes[c]);
             };
             ask(0);
+            // ---- queries, several rows of a thread in flight
+            if (k >= C::kQBuffers) mbar_wait(bar(C::QEMPTY + k % C::kQBuffers), (k / C::kQBuffers - 1u) & 1u, ctl, kCacheTimeout | C::QEMPTY);
+            constexpr uint32_t kQLanes = H / 8, kQRows = 128 / kQLanes, kQPasses = 2 * kPromptTile / kQRows, kFlight = kQPasses < 8 ? kQPasses : 8;
+            const uint32_t piece = lt % kQLanes;
+#pragma unroll 1
+            for (uint32_t pass = 0; pass < kQPasses; pass += kFlight) {
+                uint4 in_flight[kFlight];
+#pragma unroll
+                for (uint32_t f = 0; f < kFlight; ++f) {
+                    const uint32_t r = (pass + f) * kQRows + lt / kQLanes;
+                    uint32_t t, h;
+                    prompt_row(p, it.t0, it.first, r, t, h);
+                    const bool in = r < it.n_rows && t < it.count;
+                    ld_zero_16(p.q + (in ? it.b * p.q_b + t * p.q_t + static_cast<int64_t>(it.head * p.group + h) * (2 * H) + 16 * piece : 0), in, in_flight[f]);
+                }
+#pragma unroll
+                for (uint32_t f = 0; f < kFlight; ++f) {
+                    const uint32_t r = (pass + f) * kQRows + lt / kQLanes;
+                    uint4 w = in_flight[f];
+                    float coef = p.scale_log2;
+                    if (p.bf16) {   // to the range of fp16, by a power of two a row
+                        uint32_t x[4] = {w.x, w.y, w.z, w.w};
+                        float most = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 y = unpack_16(x[e], true);
+                            most = fmaxf(most, fmaxf(fabsf(y.x), fabsf(y.y)));
+                        }
+#pragma unroll
+                        for (uint32_t d = kQLanes / 2; d >= 1; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
+                        const uint32_t e8 = max(__float_as_uint(most) >> 23, 40u);   // biased: 2^(e8 - 127) <= most, unless that is tiny
+                        float up = 1.0f;
+                        if (e8 < 255) coef *= __uint_as_float((e8 - 7) << 23), up = __uint_as_float((261 - e8) << 23);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 y = unpack_16(x[e], true);
+                            x[e] = pack_half2(y.x * up, y.y * up);
+                        }
+                        w = make_uint4(x[0], x[1], x[2], x[3]);
+                    }
+                    constexpr uint32_t kPieces = C::kSwz / 16;   // of a box's row
+                    st_shared_v4(q_addr(k, r >> 7) + (piece / kPieces) * C::kBoxBytes + prompt_swizzled(r & 127u, piece % kPieces, C::kSwz), w.x, w.y, w.z, w.w);
+                    if (piece == 0) s_coef[k & 7u][r] = coef;
+                }
+            }
             look_up();
 #pragma unroll
-            for (uint32_t c = 0; c < kPasses; ++c) load(c, 0, false);
-
-            // ---- queries
-            if (k >= C::kQBuffers) mbar_wait(bar(C::QEMPTY + k % C::kQBuffers), (k / C::kQBuffers - 1u) & 1u, ctl, kCacheTimeout | C::QEMPTY);
-            constexpr uint32_t kQLanes = H / 8, kQRows = 128 / kQLanes;
-            const uint32_t piece = lt % kQLanes;
-#pragma unroll 4
-            for (uint32_t r = lt / kQLanes; r < 2 * kPromptTile; r += kQRows) {
-                const uint32_t t = (it.row0 + r) / p.group, h = it.head * p.group + (it.row0 + r) % p.group;
-                uint4 w = make_uint4(0, 0, 0, 0);
-                if (r < it.n_rows && t < it.count) w = *reinterpret_cast<const uint4*>(p.q + it.b * p.q_b + t * p.q_t + static_cast<int64_t>(h) * (2 * H) + 16 * piece);
-                float coef = p.scale_log2;
-                if (p.bf16) {   // to the range of fp16, by a power of two a row
-                    uint32_t x[4] = {w.x, w.y, w.z, w.w};
-                    float most = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 f = unpack_16(x[e], true);
-                        most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
-                    }
-#pragma unroll
-                    for (uint32_t d = kQLanes / 2; d >= 1; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
-                    const uint32_t e8 = max(__float_as_uint(most) >> 23, 40u);   // biased: 2^(e8 - 127) <= most, unless that is tiny
-                    float f = 1.0f;
-                    if (e8 < 255) coef *= __uint_as_float((e8 - 7) << 23), f = __uint_as_float((261 - e8) << 23);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 y = unpack_16(x[e], true);
-                        x[e] = pack_half2(y.x * f, y.y * f);
-                    }
-                    w = make_uint4(x[0], x[1], x[2], x[3]);
-                }
-                constexpr uint32_t kPieces = C::kSwz / 16;   // of a box's row
-                st_shared_v4(q_addr(k, r >> 7) + (piece / kPieces) * C::kBoxBytes + prompt_swizzled(r & 127u, piece % kPieces, C::kSwz), w.x, w.y, w.z, w.w);
-                if (piece == 0) s_coef[k & 3u][r] = coef;
-            }
+            for (uint32_t c = 0; c < kPasses; ++c) load(c, false);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(bar(C::QFULL + k % C::kQBuffers));
-                mbar_arrive(bar(C::COEF + (k & 3u)));
+                mbar_arrive(bar(C::COEF + (k & 7u)));
             }
             ++k;
 
             // ---- keys and values, K and V of a step in turn
 #pragma unroll 1
             for (uint32_t step = 0; step < it.steps; ++step, ++g) {
-                const uint32_t poisoned = __ballot_sync(0xFFFFFFFFu, ks != ks || vs != vs) & 0xFFu;   // groups
-                const bool none = page < 0;
+                // groups without a page (lower byte), and with a scale that is NaN; whether the keys end within the step
+                const uint32_t gone = __ballot_sync(0xFFFFFFFFu, none) & 0xFFu, poisoned = __ballot_sync(0xFFFFFFFFu, ks != ks || vs != vs) & 0xFFu;
+                const uint32_t left = it.farthest - (it.step0 + step) * kPromptTile;
+                const bool spoilt = (gone | poisoned) != 0 || left < kPromptTile;
                 ask(step + 1);
-#pragma unroll 1
+#pragma unroll
                 for (uint32_t is_v = 0; is_v < 2; ++is_v, ++n) {
                     if (n >= NS) mbar_wait(bar(C::EMPTY + n % NS), (n / NS - 1u) & 1u, ctl, kCacheTimeout | (C::EMPTY + n % NS));
                     if (is_v == 0 && lane < kGroups && warp == 8) {   // (the V tile of the step that had this entry has been let go of)
@@ -506,25 +572,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
                         e4m3x4_to_half2(codes[c].y, x[2], x[3]);
                         e4m3x4_to_half2(codes[c].z, x[4], x[5]);
                         e4m3x4_to_half2(codes[c].w, x[6], x[7]);
-                        if (poisoned >> (r >> 4) & 1u) {
+                        if (spoilt) {
+                            const bool out = r >= left || (gone >> (r >> 4) & 1u), bad = poisoned >> (r >> 4) & 1u;
+                            const uint32_t instead = !out && bad && !is_v ? 0x7E007E00u : 0u;
+                            if (out || bad)
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) x[e] = is_v ? 0u : 0x7E007E00u;
+                                for (int e = 0; e < 8; ++e) x[e] = instead;
                         }
-                        // two pieces of 8 values; the lanes of the second box write theirs in the other order (their banks are those of the first)
+                        // two pieces of 8 values: eight lanes, one row (two at H = 64), all banks
                         constexpr uint32_t kPieces = C::kSwz / 16;
-                        const uint32_t first = 2 * j16, swap = H == 128 ? j16 >> 2 : 0u;
-                        const uint32_t box = to + (first / kPieces) * C::kBoxBytes;
-                        const uint32_t a0 = box + prompt_swizzled(r, (first + swap) % kPieces, C::kSwz), a1 = box + prompt_swizzled(r, (first + 1 - swap) % kPieces, C::kSwz);
-                        if (swap) {
-                            st_shared_v4(a0, x[4], x[5], x[6], x[7]);
-                            st_shared_v4(a1, x[0], x[1], x[2], x[3]);
+                        if constexpr (H == 128) {
+                            const uint32_t at = to + prompt_swizzled(r, j16, C::kSwz);
+                            st_shared_v4(at, x[0], x[1], x[2], x[3]);
+                            st_shared_v4(at + C::kBoxBytes, x[4], x[5], x[6], x[7]);
                         } else {
-                            st_shared_v4(a0, x[0], x[1], x[2], x[3]);
-                            st_shared_v4(a1, x[4], x[5], x[6], x[7]);
+                            static_assert(H == 128 || H == C::kBoxCols, "one box");
+                            st_shared_v4(to + prompt_swizzled(r, (2 * j16) % kPieces, C::kSwz), x[0], x[1], x[2], x[3]);
+                            st_shared_v4(to + prompt_swizzled(r, (2 * j16 + 1) % kPieces, C::kSwz), x[4], x[5], x[6], x[7]);
                         }
                         // what comes next takes the registers' place
-                        if (is_v == 0) load(c, step, true);
-                        else if (step + 1 < it.steps) load(c, step + 1, false);
+                        load(c, is_v == 0);   // (behind the last step: the first page's, not used)
                     }
                     fence_proxy_async_smem();
                     __syncwarp();
@@ -534,20 +601,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
                     }
                 }
             }
+            item_done(nth);
         }
     } else {
         // ---------------------------------------------------------------- issue: warp 12 Q K^T, warp 14 P V
-        setmaxnreg_dec<64>();
+        setmaxnreg_dec<C::kIssueRegs>();
         if (warp == 12 || warp == 14) {
             const bool leader = elect_one();
             bool ok = true;   // once a wait has given up nothing more is issued
             auto wait = [&](int b, uint32_t parity) { ok &= mbar_wait(bar(b), parity, ctl, kCacheTimeout | static_cast<uint32_t>(b)); };
-            uint32_t g = 0, k = 0;
-            for (uint32_t round = 0;; ++round) {
-                const uint32_t index = prompt_index<H>(p, round);
-                if (round * gridDim.x >= p.items) break;
-                if (index >= p.items) continue;
-                const uint32_t steps = prompt_item(p, index).steps;
+            uint32_t g = 0, k = 0, done[2] = {0, 0};   // steps, items, steps of either tile
+            for (uint32_t nth = 0;; ++nth) {
+                if (!item_wait(nth)) break;
+                const PromptItem& it = items[nth % kPromptItems];
+                if (it.there == 0) break;
+                const uint32_t steps = it.steps, tile_steps[2] = {it.tile_steps[0], it.tile_steps[1]};
+                item_done(nth);   // (everything about it is in registers)
                 if (steps == 0) continue;
 #pragma unroll 1
                 for (uint32_t j = 0; j < steps; ++j, ++g) {
@@ -556,8 +625,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
                         wait(C::FULL + (2 * g) % NS, (2 * g / NS) & 1u);
 #pragma unroll
                         for (uint32_t i = 0; i < 2; ++i) {
-                            // one score tile: its use 2 g + i needs the reading of the one before; two: the reading of step g - 1's
-                            if (C::kSharedS ? g + i > 0 : g > 0) wait(C::SFREE0 + (C::kSharedS ? 0 : i), C::kSharedS ? 1u - i : (g - 1u) & 1u);
+                            if (j >= tile_steps[i]) continue;
+                            // a score tile's next use needs the reading of the one before (with one tile for both: whosever that was)
+                            const uint32_t uses = C::kSharedS ? done[0] + done[1] : done[i];
+                            if (uses > 0) wait(C::SFREE0 + (C::kSharedS ? 0 : i), (uses - 1u) & 1u);
+                            ++done[i];
                             tc_fence_after();
                             if (leader && ok) {
                                 prompt_issue_qk<H>(tmem + (i ? C::kColS1 : C::kColS0), q_addr(k, i), slot_addr(2 * g));
@@ -572,7 +644,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
                         wait(C::FULL + (2 * g + 1) % NS, ((2 * g + 1) / NS) & 1u);
 #pragma unroll
                         for (uint32_t i = 0; i < 2; ++i) {
-                            wait(C::P0 + i, g & 1u);
+                            if (j >= tile_steps[i]) continue;
+                            wait(C::P0 + i, done[i] & 1u);
+                            ++done[i];
                             tc_fence_after();
                             if (leader && ok) {
                                 prompt_issue_pv<H>(tmem + (i ? C::kColO1 : C::kColO0), tmem + (i ? C::kColP1 : C::kColP0), slot_addr(2 * g + 1), j > 0 ? 1u : 0u);
@@ -590,6 +664,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
             if (leader) tc_commit(bar(last));
             __syncwarp();
             mbar_wait_certain(bar(last), 0, ctl, kCacheTimeout | static_cast<uint32_t>(last));
+        } else if (warp == 13 && lane == 0) {
+            // ------------------------------------------------------------ items, in rounds of a CTA each, there and back: whoever had the
+            // longest of a round has the shortest of the next
+            uint32_t nth = 0;
+            for (uint32_t round = 0;; ++round) {
+                const uint32_t index = round * gridDim.x + ((round & 1u) ? gridDim.x - 1u - blockIdx.x : blockIdx.x);
+                const bool end = round * gridDim.x >= p.items;
+                if (!end && index >= p.items) continue;
+                PromptItem it = {};
+                if (!end) it = prompt_item(p, index);
+                if (!end && it.step0 == 0 && !cache_length_ok(p.c, p.s, it.b)) cache_report(p.c.status, kCacheBadPosition);
+                if (nth >= kPromptItems && !mbar_wait(bar(C::IFREE + nth % kPromptItems), (nth / kPromptItems - 1u) & 1u, ctl, kCacheTimeout | C::IFREE)) break;
+                items[nth % kPromptItems] = it;
+                mbar_arrive(bar(C::ITEM + nth % kPromptItems));
+                ++nth;
+                if (end) break;
+            }
         }
     }
     tc_fence_before();
@@ -608,12 +699,12 @@ __global__ void __launch_bounds__(128) fa_cache_prompt_join(const PromptArgs p) 
     grid_dep_launch();
     const uint32_t lane = threadIdx.x & 31u;
     const uint64_t at = static_cast<uint64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    const uint32_t row = static_cast<uint32_t>(at % (2 * kPromptTile)), whole = static_cast<uint32_t>(at / (2 * kPromptTile));
-    const uint32_t heads = p.s.B * p.c.heads, bh = whole % heads, pair = p.pairs - 1u - whole / heads;
-    if (whole >= p.items / p.parts) return;
+    const uint32_t row = static_cast<uint32_t>(at % (2 * kPromptTile)), item = static_cast<uint32_t>(at / (2 * kPromptTile));   // of those that are cut
+    if (item >= (p.items - p.whole) / p.parts) return;
+    const uint32_t heads = p.s.B * p.c.heads, bh = (p.whole + item) % heads, pair = p.pairs - 1u - (p.whole + item) / heads;
     const uint32_t r = pair * (2 * kPromptTile) + row;
     if (r >= p.s.T * p.group) return;
-    auto slot = [&](uint32_t part) { return (static_cast<uint64_t>(whole) * p.parts + part) * (2 * kPromptTile) + row; };
+    auto slot = [&](uint32_t part) { return (static_cast<uint64_t>(item) * p.parts + part) * (2 * kPromptTile) + row; };
     float top = -INFINITY;
     for (uint32_t i = lane; i < p.parts; i += 32) top = fmaxf(top, p.part_ml[slot(i)].x);
 #pragma unroll
