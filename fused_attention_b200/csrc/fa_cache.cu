@@ -135,10 +135,10 @@ constexpr uint64_t kMostCtas = 0x7FFFFFFFull;
 
 // ----------------------------------------------------------------------------- attention for few rows
 struct RowsPlan {
-    uint32_t mt, rows, row_tiles, grid;
+    uint32_t mt, rows, row_tiles, grid, min_units;
     uint64_t problems, units;   // units: of one problem, at most
     uint64_t o_bytes, ml_bytes, share_bytes;
-    uint64_t scratch() const { return o_bytes + ml_bytes + share_bytes; }
+    uint64_t scratch() const { return 16 + o_bytes + ml_bytes + share_bytes; }
 };
 
 RowsPlan plan_rows(uint32_t H, uint32_t heads, uint32_t group, uint32_t page, uint32_t B, uint32_t T, uint32_t width, uint32_t keep, uint32_t sms) {
@@ -157,10 +157,12 @@ RowsPlan plan_rows(uint32_t H, uint32_t heads, uint32_t group, uint32_t page, ui
     }
     const uint64_t tokens = static_cast<uint64_t>(keep != 0 ? keep : width) * page;
     r.units = (tokens + fa::kRowsUnit - 1) / fa::kRowsUnit;
-    r.problems = static_cast<uint64_t>(B) * heads * r.row_tiles;
+    r.problems = static_cast<uint64_t>(B) * heads * r.row_tiles;   // (below 2^31 in every call that is taken)
     const uint64_t ctas = static_cast<uint64_t>(sms) * (r.mt == 1 ? 3 : 2), all_units = r.problems * r.units;
-    r.grid = static_cast<uint32_t>(ctas < all_units ? ctas : all_units);
-    const uint64_t slots = 2ull * r.grid * 16 * r.mt;
+    // Problems of up to 512 tokens are not divided: joining costs more than what is left of them takes.
+    r.min_units = r.units <= 4 ? 0 : 2;
+    r.grid = static_cast<uint32_t>(r.min_units == 0 ? r.problems : ctas < all_units ? ctas : all_units);
+    const uint64_t slots = r.min_units == 0 ? 0 : 2ull * r.grid * 16 * r.mt;
     r.o_bytes = slots * H * 4;
     r.ml_bytes = slots * 8;
     r.share_bytes = r.problems * 8;
@@ -172,7 +174,7 @@ int launch_rows(Device& d, uint32_t bit, const fa::RowsArgs& a, const RowsPlan& 
     using Cfg = fa::RowsCfg<H, MT>;
     int rc = allow_smem(d, bit, &fa::fa_cache_rows<H, MT>, Cfg::kSmem);
     if (rc == FA_B200_OK) rc = launch(&fa::fa_cache_rows<H, MT>, plan.grid, fa::kRowsWarps * 32, Cfg::kSmem, stream, a);
-    if (rc == FA_B200_OK && plan.units > 1) rc = launch(&fa::fa_cache_join<H, MT>, static_cast<uint32_t>(plan.problems * plan.rows), 128, 0, stream, a);
+    if (rc == FA_B200_OK && plan.min_units != 0) rc = launch(&fa::fa_cache_join<H, MT>, static_cast<uint32_t>(plan.problems * plan.rows), fa::kJoinWarps * 32, 0, stream, a);
     return rc;
 }
 template <int H>
@@ -391,7 +393,7 @@ int fa_b200_cache_attention(const fa_b200_cache* cache, const fa_b200_sequences*
     a.q = static_cast<const uint8_t*>(queries), a.q_b = 2 * queries_batch_stride, a.q_t = 2 * queries_token_stride;
     a.y = static_cast<uint8_t*>(y), a.pages = pages_or_null, a.keep = keep;
     a.group = q_heads / a.c.heads, a.causal = (flags & FA_B200_CACHE_ALL_KEYS) ? 0u : 1u, a.bf16 = dtype == FA_B200_BF16;
-    a.rows = plan.rows, a.row_tiles = plan.row_tiles, a.min_units = 2;
+    a.rows = plan.rows, a.row_tiles = plan.row_tiles, a.min_units = plan.min_units;
     a.scale_log2 = scale_log2(H);
     uint8_t* const at = static_cast<uint8_t*>(scratch);
     a.part_o = reinterpret_cast<float*>(at);

@@ -37,7 +37,7 @@ struct RowsArgs {
     uint32_t group, keep, causal, bf16;
     uint32_t row_tiles;      // problems of a sequence and key/value head
     uint32_t rows;           // rows of a problem (at most 16 MT; the last may have fewer)
-    uint32_t min_units;      // units that a CTA takes at least
+    uint32_t min_units;      // units that a CTA takes at least; 0: a CTA takes a problem
     float scale_log2;        // log2(e) / sqrt(H)
     float* part_o;           // [2 G slots, 16 MT rows, H]
     float2* part_ml;         // [2 G slots, 16 MT rows]
@@ -83,6 +83,9 @@ template <int H>
 __device__ __forceinline__ uint32_t value_chunk(uint32_t r, uint32_t c) {
     return r * H + ((H == 128 ? c ^ (r & 6u) : H == 64 ? c ^ ((r >> 1) & 3u) : c) << 4);
 }
+__device__ __forceinline__ void cp_async_16_all(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 template <int kBytes>
 __device__ __forceinline__ void ld_codes(uint32_t addr, uint32_t (&w)[kBytes / 4 > 0 ? kBytes / 4 : 1]) {
     if constexpr (kBytes == 16) {
@@ -121,12 +124,19 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
 
     // ---- this CTA's units
     RowsWork work;
-    {
+    uint64_t unit, unit_end, before = 0;   // `before`: units of the sequences in front of b
+    uint32_t b = 0;
+    if (p.min_units == 0) {
+        work.total = 0, work.ctas = gridDim.x;
+        b = blockIdx.x / per_seq;
+        unit = static_cast<uint64_t>(blockIdx.x % per_seq) * rows_units(p, b);
+        unit_end = unit + rows_units(p, b);
+    } else {
         unsigned long long mine = 0;
         if (p.pages != nullptr) {
             mine = tid == 0 ? static_cast<unsigned long long>(rows_units(p, 0)) * p.s.B : 0ull;
         } else {
-            for (uint32_t b = tid; b < p.s.B; b += kThreads) mine += rows_units(p, b);
+            for (uint32_t i = tid; i < p.s.B; i += kThreads) mine += rows_units(p, i);
         }
 #pragma unroll
         for (int d = 16; d >= 1; d >>= 1) mine += __shfl_xor_sync(0xFFFFFFFFu, mine, d);
@@ -137,34 +147,32 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
         for (int w = 0; w < kRowsWarps; ++w) work.total += s_sum[w];
         work.total *= per_seq;
         work.ctas = static_cast<uint32_t>(min(static_cast<uint64_t>(gridDim.x), (work.total + p.min_units - 1) / p.min_units));
-    }
-    if (blockIdx.x >= work.ctas) return;
-    uint64_t unit = blockIdx.x * work.total / work.ctas;
-    const uint64_t unit_end = (blockIdx.x + 1) * work.total / work.ctas;
-    // the sequence of the first unit: warp 0 adds up 32 sequences at a time
-    uint32_t b = 0;
-    uint64_t before = 0;   // units of the sequences in front of b
-    if (p.pages != nullptr) {
-        const uint64_t one = static_cast<uint64_t>(rows_units(p, 0)) * per_seq;
-        b = static_cast<uint32_t>(unit / one);
-        before = b * one;
-    } else {
-        for (uint32_t b0 = 0; b0 < p.s.B; b0 += 32) {   // (every warp for itself)
-            const uint64_t mine = b0 + lane < p.s.B ? static_cast<uint64_t>(rows_units(p, b0 + lane)) * per_seq : 0;
-            uint64_t upto = mine;
+        if (blockIdx.x >= work.ctas) return;
+        unit = blockIdx.x * work.total / work.ctas;
+        unit_end = (blockIdx.x + 1) * work.total / work.ctas;
+        // the sequence of the first unit: every warp adds up 32 sequences at a time
+        if (p.pages != nullptr) {
+            const uint64_t one = static_cast<uint64_t>(rows_units(p, 0)) * per_seq;
+            b = static_cast<uint32_t>(unit / one);
+            before = b * one;
+        } else {
+            for (uint32_t b0 = 0; b0 < p.s.B; b0 += 32) {
+                const uint64_t mine32 = b0 + lane < p.s.B ? static_cast<uint64_t>(rows_units(p, b0 + lane)) * per_seq : 0;
+                uint64_t upto = mine32;
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const uint64_t x = __shfl_up_sync(0xFFFFFFFFu, upto, d);
-                if (lane >= d) upto += x;
+                for (int d = 1; d < 32; d <<= 1) {
+                    const uint64_t x = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+                    if (lane >= d) upto += x;
+                }
+                const uint32_t behind = __ballot_sync(0xFFFFFFFFu, before + upto > unit);
+                if (behind != 0) {
+                    const uint32_t at = __ffs(behind) - 1;
+                    b = b0 + at;
+                    before += __shfl_sync(0xFFFFFFFFu, upto - mine32, at);
+                    break;
+                }
+                before += __shfl_sync(0xFFFFFFFFu, upto, 31);
             }
-            const uint32_t behind = __ballot_sync(0xFFFFFFFFu, before + upto > unit);
-            if (behind != 0) {
-                const uint32_t at = __ffs(behind) - 1;
-                b = b0 + at;
-                before += __shfl_sync(0xFFFFFFFFu, upto - mine, at);
-                break;
-            }
-            before += __shfl_sync(0xFFFFFFFFu, upto, 31);
         }
     }
 
@@ -179,85 +187,26 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
         const uint32_t n_rows = min(p.rows, p.s.T * p.group - row0);
         const uint32_t held = cache_length(p.c, p.s, b), count = cache_count(p.s, b);
         if (tid == 0 && u0 == 0 && !cache_length_ok(p.c, p.s, b)) cache_report(p.c.status, kCacheBadPosition);
-
-        // ---- queries into fragments: rows whose fp16 form could overflow (bf16) are scaled by a power of two
-        for (uint32_t r = warp; r < Cfg::kRows; r += kRowsWarps) {
-            const uint32_t t = (row0 + r) / p.group, i = (row0 + r) % p.group;
-            float coef = p.scale_log2;
-            uint32_t limit = r < n_rows ? 0u : kNoToken;   // rows that are not there hold nobody up
-            if (r < n_rows && t < count) {
-                limit = p.causal ? (held + t >= count ? held + t - count + 1 : 0u) : held;
-                limit = min(limit, held);
-                if (bf16) {
-                    const uint16_t* row = reinterpret_cast<const uint16_t*>(p.q + b * p.q_b + t * p.q_t + static_cast<int64_t>(head * p.group + i) * (2 * H));
-                    float most = 0.0f;
-                    for (int d = lane; d < H; d += 32) most = fmaxf(most, fabsf(__uint_as_float(static_cast<uint32_t>(row[d]) << 16)));
-#pragma unroll
-                    for (int d = 16; d >= 1; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
-                    const uint32_t e = max(__float_as_uint(most) >> 23, 40u);   // biased: 2^(e - 127) <= most, unless that is tiny
-                    // to [2^7, 2^8): what does not lie in fp16's range then is 2^-22 of the row's largest or less
-                    if (e < 255) coef *= __uint_as_float((e - 7) << 23);
-                }
-            }
-            if (lane == 0) s_coef[r] = coef, s_limit[r] = limit;
-        }
-        __syncthreads();
-        constexpr int kPart = H >= 32 ? 16 : 8;                          // bytes of a fragment's part: 8 (4) dimensions
-        constexpr int kParts = H >= 64 ? 2 : 1;
-        for (uint32_t item = warp; item < MT * kHalves * 2 * kParts; item += kRowsWarps) {
-            const uint32_t part = item % kParts, upper = item / kParts % 2, half = item / (2 * kParts) % kHalves, mt = item / (2 * kParts * kHalves);
-            const uint32_t r = mt * 16 + upper * 8 + g;
-            const uint32_t t = (row0 + r) / p.group, i = (row0 + r) % p.group;
-            uint32_t w[4] = {0, 0, 0, 0};
-            if (r < n_rows && t < count) {
-                const uint8_t* at = p.q + b * p.q_b + t * p.q_t + static_cast<int64_t>(head * p.group + i) * (2 * H) +
-                                    2 * (half * 64 + t4 * kKeyBytes + part * 8);
-                if constexpr (kPart == 16) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(at);
-                    w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
-                } else {
-                    const uint2 x = *reinterpret_cast<const uint2*>(at);
-                    w[0] = x.x, w[1] = x.y;
-                }
-                if (bf16) {
-                    const float f = p.scale_log2 / s_coef[r];   // a power of two
-#pragma unroll
-                    for (int e = 0; e < kPart / 4; ++e) {
-                        const float2 x = unpack_16(w[e], true);
-                        w[e] = pack_half2(x.x * f, x.y * f);
-                    }
-                }
-            }
-            uint8_t* const to = q_frag + (item * 32 + lane) * kPart;
-            if constexpr (kPart == 16) *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-            else *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
-        }
-        __syncthreads();
-
-        float coef[MT][2], m[MT][2], l[MT][2], o[MT][kTilesN][4];
-        uint32_t limit[MT][2], nearest = kNoToken, farthest = 0;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                coef[mt][u] = s_coef[mt * 16 + u * 8 + g];
-                limit[mt][u] = s_limit[mt * 16 + u * 8 + g];
-                m[mt][u] = -INFINITY, l[mt][u] = 0.0f;
-            }
-        for (uint32_t r = 0; r < n_rows; ++r) nearest = min(nearest, s_limit[r]), farthest = max(farthest, s_limit[r]);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int j = 0; j < kTilesN; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[mt][j][e] = 0.0f;
+        // keys that a row of token t sees; of all rows [nearest, farthest)
+        auto limit_of = [&](uint32_t t) {
+            if (t >= count) return 0u;
+            if (!p.causal) return held;
+            return held + t >= count ? min(held, held + t - count + 1u) : 0u;
+        };
+        const uint32_t t_first = row0 / p.group, t_last = (row0 + n_rows - 1) / p.group;
+        const uint32_t nearest = min(limit_of(t_first), limit_of(t_last));
+        const uint32_t farthest = t_first >= count ? 0u : limit_of(min(t_last, count - 1u));
 
         // ---- the ring.  Lane l knows the pages of group l (16 tokens) of the warp's next 16 stages.
         const uint32_t n_stages = u1 - u0;
-        const uint32_t token_row = (row0 / p.group);   // with a list of pages: the token of the problem
-        const int32_t* const list =
-            p.pages != nullptr ? p.pages + ((static_cast<uint64_t>(b) * p.s.T + token_row) * p.c.heads + head) * p.keep : nullptr;
+        const int32_t* const list = p.pages != nullptr ? p.pages + ((static_cast<uint64_t>(b) * p.s.T + t_first) * p.c.heads + head) * p.keep : nullptr;
         const int32_t* const table = p.s.table + b * p.s.table_stride;
+        constexpr uint32_t kChunks = H / 16;                 // of a row; 32 lanes copy 32 / kChunks rows at a time
+        constexpr uint32_t kRowsAtOnce = 32 / kChunks;
+        const uint32_t copy_row = lane / kChunks, copy_chunk = lane % kChunks;
+        const bool copies = copy_row < 16;                   // (H = 16: half the lanes)
+        const uint8_t* const k_base = p.c.k + static_cast<int64_t>(head) * p.c.k_head + static_cast<int64_t>(copy_row) * p.c.k_token + copy_chunk * 16;
+        const uint8_t* const v_base = p.c.v + static_cast<int64_t>(head) * p.c.v_head + static_cast<int64_t>(copy_row) * p.c.v_token + copy_chunk * 16;
         int32_t my_page = -1;
         uint32_t my_at = kNoToken;   // position of the group's first token
         auto look_up = [&](uint32_t stage) {
@@ -287,41 +236,117 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
             if (stage < n_stages) {
                 if ((stage & 15u) == 0) look_up(stage);
                 const uint32_t to = ring + (stage % Cfg::kStages) * Cfg::kStageBytes, from_lane = 2 * (stage & 15u);
-                const int32_t page[2] = {__shfl_sync(0xFFFFFFFFu, my_page, from_lane), __shfl_sync(0xFFFFFFFFu, my_page, from_lane + 1)};
-                const uint32_t at[2] = {__shfl_sync(0xFFFFFFFFu, my_at, from_lane), __shfl_sync(0xFFFFFFFFu, my_at, from_lane + 1)};
-                // the first stage of a list may start in the middle of a page, but a group of 16 tokens never spans two
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const bool there = page[half] >= 0;
-                    const int64_t ph = there ? page[half] : 0;
-                    const uint32_t in_page = there ? at[half] & (p.c.page - 1) : 0u;
-                    const uint8_t* const k0 = p.c.k + ph * p.c.k_page + static_cast<int64_t>(head) * p.c.k_head + static_cast<int64_t>(in_page) * p.c.k_token;
-                    const uint8_t* const v0 = p.c.v + ph * p.c.v_page + static_cast<int64_t>(head) * p.c.v_head + static_cast<int64_t>(in_page) * p.c.v_token;
-                    constexpr uint32_t kChunks = H / 16;                 // of a row
-                    const uint32_t c = lane % kChunks;
+                for (int half = 0; half < 2; ++half) {   // (a group of 16 tokens never spans two pages)
+                    const int32_t page = __shfl_sync(0xFFFFFFFFu, my_page, from_lane + half);
+                    const uint32_t at = __shfl_sync(0xFFFFFFFFu, my_at, from_lane + half), in_page = at & (p.c.page - 1);
+                    const uint32_t meta = to + 2 * Cfg::kCodes + 4 * half;
+                    if (lane == 0) st_shared_u32(meta + 16, at);
+                    const uint64_t ph = page < 0 ? 0u : static_cast<uint32_t>(page);
+                    const uint8_t* k0 = k_base + ph * static_cast<uint32_t>(p.c.k_page) + in_page * static_cast<uint32_t>(p.c.k_token);
+                    const uint8_t* v0 = v_base + ph * static_cast<uint32_t>(p.c.v_page) + in_page * static_cast<uint32_t>(p.c.v_token);
+                    if (!copies) {
+                    } else if (page >= 0 && at + 16 <= farthest) {
 #pragma unroll
-                    for (uint32_t r = lane / kChunks; r < 16; r += 32 / kChunks) {
-                        const bool in = there && at[half] + r < farthest;   // (what no row may see is not read: its codes may be anything)
-                        cp_async_16_zero(to + key_chunk<H>(half * 16 + r, c), k0 + (in ? r * p.c.k_token + c * 16 : 0), in);
-                        cp_async_16_zero(to + Cfg::kCodes + value_chunk<H>(half * 16 + r, c), v0 + (in ? r * p.c.v_token + c * 16 : 0), in);
-                    }
-                    if (lane == half) {
-                        const uint32_t meta = to + 2 * Cfg::kCodes + 4 * half;
-                        st_shared_u32(meta + 16, at[half]);
-                        const uint64_t s_at = static_cast<uint64_t>(ph) * p.c.heads + head;
-                        if (there) {
-                            cp_async_4(meta, reinterpret_cast<uint64_t>(p.c.k_scale + s_at));
-                            cp_async_4(meta + 8, reinterpret_cast<uint64_t>(p.c.v_scale + s_at));
-                        } else {
-                            st_shared_u32(meta, 0x3F800000u);
-                            st_shared_u32(meta + 8, 0x3F800000u);
+                        for (uint32_t r = 0; r < 16; r += kRowsAtOnce) {
+                            cp_async_16_all(to + key_chunk<H>(half * 16 + r + copy_row, copy_chunk), k0);
+                            cp_async_16_all(to + Cfg::kCodes + value_chunk<H>(half * 16 + r + copy_row, copy_chunk), v0);
+                            k0 += kRowsAtOnce * static_cast<uint32_t>(p.c.k_token), v0 += kRowsAtOnce * static_cast<uint32_t>(p.c.v_token);
                         }
+                    } else {   // what no row may see is not read (its codes may be anything), but filled with zeros
+#pragma unroll
+                        for (uint32_t r = 0; r < 16; r += kRowsAtOnce) {
+                            const bool in = page >= 0 && at + r + copy_row < farthest;
+                            cp_async_16_zero(to + key_chunk<H>(half * 16 + r + copy_row, copy_chunk), in ? k0 : p.c.k, in);
+                            cp_async_16_zero(to + Cfg::kCodes + value_chunk<H>(half * 16 + r + copy_row, copy_chunk), in ? v0 : p.c.v, in);
+                            k0 += kRowsAtOnce * static_cast<uint32_t>(p.c.k_token), v0 += kRowsAtOnce * static_cast<uint32_t>(p.c.v_token);
+                        }
+                    }
+                    if (lane < 2) {
+                        const float* const scale = (lane ? p.c.v_scale : p.c.k_scale) + ph * p.c.heads + head;
+                        if (page >= 0) cp_async_4(meta + 8 * lane, reinterpret_cast<uint64_t>(scale));
+                        else st_shared_u32(meta + 8 * lane, 0x3F800000u);
                     }
                 }
             }
             cp_async_commit();
         };
         issue(0);
+
+        // ---- queries into fragments, a warp 8 rows: those whose fp16 form could overflow (bf16) are scaled by a power of two
+        constexpr int kPart = H >= 32 ? 16 : 8;                          // bytes of a fragment's part: 8 (4) dimensions
+        constexpr int kParts = H >= 64 ? 2 : 1;
+        if (warp < 2 * MT) {
+            const uint32_t r = warp * 8 + g, t = (row0 + r) / p.group, i = (row0 + r) % p.group;
+            const bool in = r < n_rows && t < count;
+            uint32_t w[kHalves * kParts][kPart / 4];
+#pragma unroll
+            for (int x = 0; x < kHalves * kParts; ++x) {
+#pragma unroll
+                for (int e = 0; e < kPart / 4; ++e) w[x][e] = 0;
+                if (in) {
+                    const uint8_t* at = p.q + b * p.q_b + t * p.q_t + static_cast<int64_t>(head * p.group + i) * (2 * H) +
+                                        2 * ((x / kParts) * 64 + t4 * kKeyBytes + (x % kParts) * 8);
+                    if constexpr (kPart == 16) {
+                        const uint4 y = *reinterpret_cast<const uint4*>(at);
+                        w[x][0] = y.x, w[x][1] = y.y, w[x][2] = y.z, w[x][3] = y.w;
+                    } else {
+                        const uint2 y = *reinterpret_cast<const uint2*>(at);
+                        w[x][0] = y.x, w[x][1] = y.y;
+                    }
+                }
+            }
+            float coef = p.scale_log2;
+            if (bf16) {
+                float most = 0.0f;
+#pragma unroll
+                for (int x = 0; x < kHalves * kParts; ++x)
+#pragma unroll
+                    for (int e = 0; e < kPart / 4; ++e) {
+                        const float2 y = unpack_16(w[x][e], true);
+                        most = fmaxf(most, fmaxf(fabsf(y.x), fabsf(y.y)));
+                    }
+                most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
+                const uint32_t e8 = max(__float_as_uint(most) >> 23, 40u);   // biased: 2^(e8 - 127) <= most, unless that is tiny
+                // to [2^7, 2^8): what does not lie in fp16's range then is 2^-22 of the row's largest or less
+                float up = 1.0f;
+                if (e8 < 255) coef *= __uint_as_float((e8 - 7) << 23), up = __uint_as_float((261 - e8) << 23);
+#pragma unroll
+                for (int x = 0; x < kHalves * kParts; ++x)
+#pragma unroll
+                    for (int e = 0; e < kPart / 4; ++e) {
+                        const float2 y = unpack_16(w[x][e], true);
+                        w[x][e] = pack_half2(y.x * up, y.y * up);
+                    }
+            }
+#pragma unroll
+            for (int x = 0; x < kHalves * kParts; ++x) {   // (rows of a warp: m-tile warp / 2, its upper or lower eight)
+                const uint32_t item = (((warp >> 1) * kHalves + x / kParts) * 2 + (warp & 1u)) * kParts + x % kParts;
+                uint8_t* const to = q_frag + (item * 32 + lane) * kPart;
+                if constexpr (kPart == 16) *reinterpret_cast<uint4*>(to) = make_uint4(w[x][0], w[x][1], w[x][2], w[x][3]);
+                else *reinterpret_cast<uint2*>(to) = make_uint2(w[x][0], w[x][1]);
+            }
+            if (t4 == 0) s_coef[r] = coef, s_limit[r] = r < n_rows ? limit_of(t) : kNoToken;   // (rows that are not there hold nobody up)
+        }
+        __syncthreads();
+        float coef[MT][2], m[MT][2], l[MT][2], o[MT][kTilesN][4];
+        uint32_t limit[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                coef[mt][u] = s_coef[mt * 16 + u * 8 + g];
+                limit[mt][u] = s_limit[mt * 16 + u * 8 + g];
+                m[mt][u] = -INFINITY, l[mt][u] = 0.0f;
+            }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int j = 0; j < kTilesN; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[mt][j][e] = 0.0f;
+
         for (uint32_t stage = 0; stage < n_stages; ++stage) {
             issue(stage + 1);
             cp_async_wait_group<1>();
@@ -388,47 +413,60 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
                 uint32_t pf[MT][4][2];
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
-                    float top[2] = {-INFINITY, -INFINITY};
+                    // exponents against M, a whole number, so that with scales that are powers of two nothing is rounded but the result
+                    float top[2] = {-INFINITY, -INFINITY}, cu[2][2], add[2][2];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const float ref = m[mt][u] == -INFINITY ? 0.0f : m[mt][u];
+#pragma unroll
+                        for (int h2 = 0; h2 < 2; ++h2) cu[u][h2] = coef[mt][u] * ks[h2], add[u][h2] = vlog[h2] - ref;
+                    }
 #pragma unroll
                     for (int n = 0; n < 4; ++n)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int u = e >> 1;
-                            float x = fmaf(s[mt][n][e], coef[mt][u] * ks[n >> 1], vlog[n >> 1]);
-                            if (!whole) {
+                        for (int e = 0; e < 4; ++e) s[mt][n][e] = fmaf(s[mt][n][e], cu[e >> 1][n >> 1], add[e >> 1][n >> 1]);
+                    if (!whole) {
+#pragma unroll
+                        for (int n = 0; n < 4; ++n)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
                                 const uint32_t pos = at[n >> 1] + (n & 1) * 8 + 2 * t4 + (e & 1);
-                                x = at[n >> 1] != kNoToken && pos < limit[mt][u] ? x : -INFINITY;
+                                if (at[n >> 1] == kNoToken || pos >= limit[mt][e >> 1]) s[mt][n][e] = -INFINITY;
                             }
-                            s[mt][n][e] = x;
-                            top[u] = fmaxf(top[u], x);
-                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) top[0] = max3(top[0], s[mt][n][0], s[mt][n][1]), top[1] = max3(top[1], s[mt][n][2], s[mt][n][3]);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         top[u] = fmaxf(top[u], __shfl_xor_sync(0xFFFFFFFFu, top[u], 1));
                         top[u] = fmaxf(top[u], __shfl_xor_sync(0xFFFFFFFFu, top[u], 2));
                     }
-                    const bool moves = top[0] > m[mt][0] + kRowsSlack || top[1] > m[mt][1] + kRowsSlack;
-                    if (__any_sync(0xFFFFFFFFu, moves)) {
-                        float f[2];
+                    const bool moves[2] = {top[0] > kRowsSlack || (m[mt][0] == -INFINITY && top[0] > -INFINITY),
+                                           top[1] > kRowsSlack || (m[mt][1] == -INFINITY && top[1] > -INFINITY)};
+                    if (__any_sync(0xFFFFFFFFu, moves[0] || moves[1])) {
+                        float f[2], by[2];
 #pragma unroll
                         for (int u = 0; u < 2; ++u) {
-                            const float was = m[mt][u];
-                            if (top[u] > was + kRowsSlack) m[mt][u] = top[u];
-                            f[u] = was == m[mt][u] ? 1.0f : ex2_approx(was - m[mt][u]);   // (-inf: 0)
+                            by[u] = moves[u] ? ceilf(top[u]) : 0.0f;
+                            f[u] = !moves[u] ? 1.0f : m[mt][u] == -INFINITY ? 0.0f : ex2_approx(-by[u]);
+                            if (moves[u]) m[mt][u] = (m[mt][u] == -INFINITY ? 0.0f : m[mt][u]) + by[u];
                             l[mt][u] *= f[u];
                         }
+#pragma unroll
+                        for (int n = 0; n < 4; ++n)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s[mt][n][e] -= by[e >> 1];
 #pragma unroll
                         for (int j = 0; j < kTilesN; ++j)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) o[mt][j][e] *= f[e >> 1];
                     }
                     float sum[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
-                    const float ref[2] = {m[mt][0] == -INFINITY ? 0.0f : m[mt][0], m[mt][1] == -INFINITY ? 0.0f : m[mt][1]};
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            s[mt][n][e] = ex2_approx(s[mt][n][e] - ref[e >> 1]);
+                            s[mt][n][e] = ex2_approx(s[mt][n][e]);
                             sum[n >> 1][e >> 1] += s[mt][n][e];
                         }
                         pf[mt][n][0] = pack_half2(s[mt][n][0], s[mt][n][1]);
@@ -534,7 +572,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
                 if (d == 0) p.part_ml[static_cast<uint64_t>(s_at) * Cfg::kRows + r] = make_float2(top, sum);
             }
         }
-        if (tid == 0 && u0 == 0) {   // who has a share of the problem, for fa_cache_join
+        if (tid == 0 && u0 == 0 && p.min_units != 0) {   // who has a share of the problem, for fa_cache_join
             const uint64_t begins = before + static_cast<uint64_t>(problem) * n_units;
             p.shares[static_cast<uint64_t>(b) * per_seq + problem] =
                 make_int2(alone ? -1 : static_cast<int>(2 * blockIdx.x + (first_segment ? 0 : 1)), static_cast<int>(rows_owner(begins + n_units - 1, work)));
@@ -545,16 +583,17 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
     }
 }
 
-// Puts the parts of divided problems together: a CTA per problem and row, a warp per part in turn.
+// Puts the parts of divided problems together: a CTA per problem and row, a warp per part in turn, several parts in flight.
+constexpr int kJoinWarps = 8;
 template <int H, int MT>
-__global__ void __launch_bounds__(128) fa_cache_join(const RowsArgs p) {
-    constexpr int kRows = 16 * MT;
-    __shared__ float s_o[4][H];
-    __shared__ float2 s_ml[4];
+__global__ void __launch_bounds__(kJoinWarps * 32) fa_cache_join(const RowsArgs p) {
+    constexpr int kRows = 16 * MT, kThreads = kJoinWarps * 32;
+    constexpr int kWide = H >= 64 ? H / 32 : 2;   // dimensions of a lane
+    __shared__ __align__(16) float s_o[kJoinWarps][H];
+    __shared__ float s_top[kJoinWarps], s_sum[kJoinWarps], s_f[kThreads];
     grid_dep_wait();
     grid_dep_launch();
-    const bool bf16 = p.bf16 != 0;
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     const uint64_t index = blockIdx.x / p.rows;
     const uint32_t r = blockIdx.x % p.rows;
     const int2 share = p.shares[index];
@@ -566,34 +605,60 @@ __global__ void __launch_bounds__(128) fa_cache_join(const RowsArgs p) {
     const uint32_t first = static_cast<uint32_t>(share.x), last = 2 * static_cast<uint32_t>(share.y);   // slots: first, then the even ones behind it
     const uint32_t n = (last - (first & ~1u)) / 2 + 1;
     auto slot = [&](uint32_t i) { return static_cast<uint64_t>(i == 0 ? first : (first & ~1u) + 2 * i) * kRows + r; };
-    float top = -INFINITY;
-    for (uint32_t i = lane; i < n; i += 32) top = fmaxf(top, p.part_ml[slot(i)].x);
+    float top = -INFINITY, sum = 0.0f, x[kWide];
 #pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-    float sum = 0.0f, x[(H + 31) / 32];
+    for (int d = 0; d < kWide; ++d) x[d] = 0.0f;
+    for (uint32_t i0 = 0; i0 < n; i0 += kThreads) {   // (more than one turn only where a problem has more parts than threads)
+        const uint32_t i = i0 + tid;
+        const float2 ml = i < n ? p.part_ml[slot(i)] : make_float2(-INFINITY, 0.0f);
+        float mine = ml.x;
 #pragma unroll
-    for (int d = 0; d < (H + 31) / 32; ++d) x[d] = 0.0f;
-    for (uint32_t i = warp; i < n; i += 4) {
-        const float2 ml = p.part_ml[slot(i)];
-        const float f = ml.x == -INFINITY ? 0.0f : ex2_approx(ml.x - top);
-        sum += ml.y * f;
+        for (int d = 16; d >= 1; d >>= 1) mine = fmaxf(mine, __shfl_xor_sync(0xFFFFFFFFu, mine, d));
+        if (i0 > 0) __syncthreads();
+        if (lane == 0) s_top[warp] = mine;
+        __syncthreads();
+        float now = top;
 #pragma unroll
-        for (int d = 0; d < (H + 31) / 32; ++d)
-            if (H >= 32 || lane < H) x[d] += p.part_o[slot(i) * H + d * 32 + lane] * f;
+        for (int w = 0; w < kJoinWarps; ++w) now = fmaxf(now, s_top[w]);
+        const float f = ml.x == -INFINITY ? 0.0f : ex2_approx(ml.x - now);
+        const float again = top == now || top == -INFINITY ? 1.0f : ex2_approx(top - now);   // for what the turns before have added up
+        s_f[tid] = f;
+        sum = sum * again + ml.y * f;
+#pragma unroll
+        for (int d = 0; d < kWide; ++d) x[d] *= again;
+        top = now;
+        __syncthreads();
+        const uint32_t here = min(n - i0, static_cast<uint32_t>(kThreads));
+        if (lane * kWide < H)
+#pragma unroll 4
+            for (uint32_t k = warp; k < here; k += kJoinWarps) {
+                const float* const from = p.part_o + slot(i0 + k) * H + lane * kWide;
+                const float fk = s_f[k];
+                if constexpr (kWide == 4) {
+                    const float4 y = *reinterpret_cast<const float4*>(from);
+                    x[0] += y.x * fk, x[1] += y.y * fk, x[2] += y.z * fk, x[3] += y.w * fk;
+                } else {
+                    const float2 y = *reinterpret_cast<const float2*>(from);
+                    x[0] += y.x * fk, x[1] += y.y * fk;
+                }
+            }
     }
 #pragma unroll
-    for (int d = 0; d < (H + 31) / 32; ++d)
-        if (H >= 32 || lane < H) s_o[warp][d * 32 + lane] = x[d];
-    if (lane == 0) s_ml[warp].y = sum;
+    for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+    if (lane == 0) s_sum[warp] = sum;
+    if (lane * kWide < H)
+#pragma unroll
+        for (int d = 0; d < kWide; ++d) s_o[warp][lane * kWide + d] = x[d];
     __syncthreads();
-    if (threadIdx.x < H / 2) {
-        const uint32_t d = 2 * threadIdx.x;
-        const float total = (s_ml[0].y + s_ml[1].y) + (s_ml[2].y + s_ml[3].y);
+    if (tid < H / 2) {
+        const uint32_t d = 2 * tid;
+        float total = 0.0f, lo = 0.0f, hi = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) total += s_sum[w], lo += s_o[w][d], hi += s_o[w][d + 1];
         const float f = total == 0.0f ? 0.0f : 1.0f / total;
-        const float lo = (s_o[0][d] + s_o[1][d]) + (s_o[2][d] + s_o[3][d]), hi = (s_o[0][d + 1] + s_o[1][d + 1]) + (s_o[2][d + 1] + s_o[3][d + 1]);
         const uint32_t t = row / p.group, h = head * p.group + row % p.group;
         uint8_t* const to = p.y + ((static_cast<uint64_t>(b) * p.s.T + t) * (p.c.heads * p.group) + h) * (2 * H) + 2 * d;
-        *reinterpret_cast<uint32_t*>(to) = pack_16(lo * f, hi * f, bf16);
+        *reinterpret_cast<uint32_t*>(to) = pack_16(lo * f, hi * f, p.bf16 != 0);
     }
 }
 
