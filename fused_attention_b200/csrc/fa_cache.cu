@@ -388,7 +388,7 @@ int fa_b200_cache_attention(const fa_b200_cache* cache, const fa_b200_sequences*
         }
     }
     const RowsPlan plan = plan_rows(H, a.c.heads, q_heads / a.c.heads, a.c.page, a.s.B, a.s.T, a.s.width, keep, static_cast<uint32_t>(d->sms.load()));
-    if (plan.problems * plan.rows > kMostCtas) return FA_B200_ERR_SHAPE;
+    if (plan.problems * plan.rows > kMostCtas || plan.problems * plan.units > 0xFFFFFFFFull) return FA_B200_ERR_SHAPE;
     if (scratch_bytes < plan.scratch()) return FA_B200_ERR_TOO_LARGE;
     a.q = static_cast<const uint8_t*>(queries), a.q_b = 2 * queries_batch_stride, a.q_t = 2 * queries_token_stride;
     a.y = static_cast<uint8_t*>(y), a.pages = pages_or_null, a.keep = keep;

@@ -59,19 +59,19 @@ struct RowsCfg {
     static constexpr int kCtas = MT == 1 ? 3 : 2;                  // per SM
 };
 
-// Where a CTA's units lie: problems in front of it and inside its sequence.
+// How the units of all problems (below 2^32) are dealt out: CTA c takes `each` from c * each + min(c, more) on, the first `more` CTAs
+// one more.
 struct RowsWork {
-    uint64_t total;   // units of all problems
-    uint32_t ctas;    // that take part
+    uint32_t ctas, each, more;
 };
-
+__device__ __forceinline__ uint32_t rows_begin(const RowsWork& w, uint32_t c) { return c * w.each + min(c, w.more); }
+__device__ __forceinline__ uint32_t rows_owner(const RowsWork& w, uint32_t unit) {
+    const uint32_t longer = w.more * (w.each + 1);
+    return unit < longer ? unit / (w.each + 1) : w.more + (unit - longer) / w.each;
+}
 __device__ __forceinline__ uint32_t rows_units(const RowsArgs& p, uint32_t b) {
     const uint32_t tokens = p.pages != nullptr ? p.keep << p.c.page_shift : cache_length(p.c, p.s, b);
     return max(1u, (tokens + kRowsUnit - 1) / kRowsUnit);
-}
-// CTA that takes unit u: the last one whose first unit is not behind it.
-__device__ __forceinline__ uint32_t rows_owner(uint64_t u, const RowsWork& w) {
-    return static_cast<uint32_t>(((u + 1) * w.ctas - 1) / w.total);
 }
 
 // 16 bytes of the ring: chunk `c` of row `r`, rows of H bytes, chunks moved about so that the reads below meet few conflicts.
@@ -82,6 +82,17 @@ __device__ __forceinline__ uint32_t key_chunk(uint32_t r, uint32_t c) {
 template <int H>
 __device__ __forceinline__ uint32_t value_chunk(uint32_t r, uint32_t c) {
     return r * H + ((H == 128 ? c ^ (r & 6u) : H == 64 ? c ^ ((r >> 1) & 3u) : c) << 4);
+}
+// 16 (8) bytes of global memory, zeros where `in` is false.  Volatile: asked for where it stands.
+template <int kBytes>
+__device__ __forceinline__ void ld_or_zero(const uint8_t* from, bool in, uint32_t (&w)[kBytes / 4]) {
+    if constexpr (kBytes == 16)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+                     "@p ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+                     : "=&r"(w[0]), "=&r"(w[1]), "=&r"(w[2]), "=&r"(w[3]) : "l"(from), "r"(static_cast<uint32_t>(in)));
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\t@p ld.global.v2.u32 {%0, %1}, [%2];\n\t}"
+                     : "=&r"(w[0]), "=&r"(w[1]) : "l"(from), "r"(static_cast<uint32_t>(in)));
 }
 __device__ __forceinline__ void cp_async_16_all(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -116,62 +127,75 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
     float* const s_coef = reinterpret_cast<float*>(q_frag + Cfg::kQ);
     uint32_t* const s_limit = reinterpret_cast<uint32_t*>(s_coef + Cfg::kRows);
     float2* const s_ml = reinterpret_cast<float2*>(s_limit + Cfg::kRows);
-    unsigned long long* const s_sum = reinterpret_cast<unsigned long long*>(s_ml + kRowsWarps * Cfg::kRows);
+    uint32_t* const s_sum = reinterpret_cast<uint32_t*>(s_ml + kRowsWarps * Cfg::kRows);
+    uint32_t* const s_first = s_sum + kRowsWarps;   // {first sequence, units in front of it}, {CTAs, units each, CTAs with one more}
     grid_dep_wait();
     grid_dep_launch();
     const bool bf16 = p.bf16 != 0;
     const uint32_t per_seq = p.c.heads * p.row_tiles;   // problems of a sequence
 
     // ---- this CTA's units
-    RowsWork work;
-    uint64_t unit, unit_end, before = 0;   // `before`: units of the sequences in front of b
-    uint32_t b = 0;
+    RowsWork work = {gridDim.x, 1, 0};
+    uint32_t unit, unit_end, before = 0, b = 0;   // `before`: units of the sequences in front of b
     if (p.min_units == 0) {
-        work.total = 0, work.ctas = gridDim.x;
         b = blockIdx.x / per_seq;
-        unit = static_cast<uint64_t>(blockIdx.x % per_seq) * rows_units(p, b);
-        unit_end = unit + rows_units(p, b);
+        const uint32_t n = rows_units(p, b);
+        unit = (blockIdx.x - b * per_seq) * n;
+        unit_end = unit + n;
     } else {
-        unsigned long long mine = 0;
+        // the units of all sequences; with up to kThreads of them every thread keeps what lies in front of its own
+        uint32_t total = 0, mine = 0, upto = 0;
         if (p.pages != nullptr) {
-            mine = tid == 0 ? static_cast<unsigned long long>(rows_units(p, 0)) * p.s.B : 0ull;
+            mine = rows_units(p, 0) * per_seq;
+            total = mine * p.s.B;
         } else {
             for (uint32_t i = tid; i < p.s.B; i += kThreads) mine += rows_units(p, i);
+            mine *= per_seq;
+            upto = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+                if (lane >= d) upto += x;
+            }
+            if (lane == 31) s_sum[warp] = upto;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kRowsWarps; ++w) {
+                if (w < warp) upto += s_sum[w];
+                total += s_sum[w];
+            }
         }
-#pragma unroll
-        for (int d = 16; d >= 1; d >>= 1) mine += __shfl_xor_sync(0xFFFFFFFFu, mine, d);
-        if (lane == 0) s_sum[warp] = mine;
-        __syncthreads();
-        work.total = 0;
-#pragma unroll
-        for (int w = 0; w < kRowsWarps; ++w) work.total += s_sum[w];
-        work.total *= per_seq;
-        work.ctas = static_cast<uint32_t>(min(static_cast<uint64_t>(gridDim.x), (work.total + p.min_units - 1) / p.min_units));
+        work.ctas = min(gridDim.x, (total + p.min_units - 1) / p.min_units);
         if (blockIdx.x >= work.ctas) return;
-        unit = blockIdx.x * work.total / work.ctas;
-        unit_end = (blockIdx.x + 1) * work.total / work.ctas;
-        // the sequence of the first unit: every warp adds up 32 sequences at a time
+        work.each = total / work.ctas;
+        work.more = total - work.each * work.ctas;
+        if (tid == 0) s_first[2] = work.ctas, s_first[3] = work.each, s_first[4] = work.more;
+        unit = rows_begin(work, blockIdx.x);
+        unit_end = rows_begin(work, blockIdx.x + 1);
         if (p.pages != nullptr) {
-            const uint64_t one = static_cast<uint64_t>(rows_units(p, 0)) * per_seq;
-            b = static_cast<uint32_t>(unit / one);
-            before = b * one;
+            b = unit / mine;
+            before = b * mine;
+        } else if (p.s.B <= kThreads) {
+            if (tid < p.s.B && unit < upto && unit >= upto - mine) s_first[0] = tid, s_first[1] = upto - mine;
+            __syncthreads();
+            b = s_first[0], before = s_first[1];
         } else {
-            for (uint32_t b0 = 0; b0 < p.s.B; b0 += 32) {
-                const uint64_t mine32 = b0 + lane < p.s.B ? static_cast<uint64_t>(rows_units(p, b0 + lane)) * per_seq : 0;
-                uint64_t upto = mine32;
+            for (uint32_t b0 = 0; b0 < p.s.B; b0 += 32) {   // every warp adds up 32 sequences at a time
+                const uint32_t mine32 = b0 + lane < p.s.B ? rows_units(p, b0 + lane) * per_seq : 0u;
+                uint32_t upto32 = mine32;
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) {
-                    const uint64_t x = __shfl_up_sync(0xFFFFFFFFu, upto, d);
-                    if (lane >= d) upto += x;
+                    const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, upto32, d);
+                    if (lane >= d) upto32 += x;
                 }
-                const uint32_t behind = __ballot_sync(0xFFFFFFFFu, before + upto > unit);
+                const uint32_t behind = __ballot_sync(0xFFFFFFFFu, before + upto32 > unit);
                 if (behind != 0) {
                     const uint32_t at = __ffs(behind) - 1;
                     b = b0 + at;
-                    before += __shfl_sync(0xFFFFFFFFu, upto - mine32, at);
+                    before += __shfl_sync(0xFFFFFFFFu, upto32 - mine32, at);
                     break;
                 }
-                before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+                before += __shfl_sync(0xFFFFFFFFu, upto32, 31);
             }
         }
     }
@@ -179,9 +203,9 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
     uint32_t slot = 2 * blockIdx.x;
     for (bool first_segment = true; unit < unit_end; first_segment = false) {
         const uint32_t n_units = rows_units(p, b);
-        const uint32_t within = static_cast<uint32_t>(unit - before);
+        const uint32_t within = unit - before;
         const uint32_t problem = within / n_units, u0 = within % n_units;
-        const uint32_t u1 = static_cast<uint32_t>(min(static_cast<uint64_t>(n_units), u0 + (unit_end - unit)));
+        const uint32_t u1 = min(n_units, u0 + (unit_end - unit));
         const uint32_t head = problem / p.row_tiles, tile = problem % p.row_tiles;
         const uint32_t row0 = tile * p.rows;   // rows of the sequence and head: T * group
         const uint32_t n_rows = min(p.rows, p.s.T * p.group - row0);
@@ -214,18 +238,20 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
             my_page = -1, my_at = kNoToken;
             if (stage + (lane >> 1) >= n_stages) return;
             uint32_t block = token >> p.c.page_shift;
-            bool bad = false;
             if (list != nullptr) {
                 const int32_t chosen = block < p.keep ? list[block] : -1;
                 if (chosen < 0) return;   // (not filled)
                 block = static_cast<uint32_t>(chosen);
-                bad = block >= p.s.width;
             }
+            const bool inside = block < p.s.width;
             const uint64_t at = (static_cast<uint64_t>(block) << p.c.page_shift) + (token & (p.c.page - 1));
+            if (inside) my_page = table[block];   // (an entry that no token reaches may be anything)
+            bool bad = list != nullptr && !inside;
             if (!bad && at < farthest) {
-                my_page = table[block];
                 bad = static_cast<uint32_t>(my_page) >= p.c.n_pages;
                 my_at = static_cast<uint32_t>(at);
+            } else {
+                my_page = -1;
             }
             if (bad) {
                 my_page = -1, my_at = kNoToken;
@@ -271,31 +297,21 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
             }
             cp_async_commit();
         };
-        issue(0);
-
-        // ---- queries into fragments, a warp 8 rows: those whose fp16 form could overflow (bf16) are scaled by a power of two
+        // ---- queries, a warp 8 rows, asked for ahead of the first keys
         constexpr int kPart = H >= 32 ? 16 : 8;                          // bytes of a fragment's part: 8 (4) dimensions
         constexpr int kParts = H >= 64 ? 2 : 1;
+        const uint32_t q_row = warp * 8 + g, q_token = (row0 + q_row) / p.group;
+        uint32_t w[kHalves * kParts][kPart / 4];
         if (warp < 2 * MT) {
-            const uint32_t r = warp * 8 + g, t = (row0 + r) / p.group, i = (row0 + r) % p.group;
-            const bool in = r < n_rows && t < count;
-            uint32_t w[kHalves * kParts][kPart / 4];
+            const uint32_t i = (row0 + q_row) - q_token * p.group;
+            const bool in = q_row < n_rows && q_token < count;
+            const uint8_t* const q_at = p.q + (in ? b * p.q_b + q_token * p.q_t + static_cast<int64_t>(head * p.group + i) * (2 * H) + 2 * t4 * kKeyBytes : 0);
 #pragma unroll
-            for (int x = 0; x < kHalves * kParts; ++x) {
-#pragma unroll
-                for (int e = 0; e < kPart / 4; ++e) w[x][e] = 0;
-                if (in) {
-                    const uint8_t* at = p.q + b * p.q_b + t * p.q_t + static_cast<int64_t>(head * p.group + i) * (2 * H) +
-                                        2 * ((x / kParts) * 64 + t4 * kKeyBytes + (x % kParts) * 8);
-                    if constexpr (kPart == 16) {
-                        const uint4 y = *reinterpret_cast<const uint4*>(at);
-                        w[x][0] = y.x, w[x][1] = y.y, w[x][2] = y.z, w[x][3] = y.w;
-                    } else {
-                        const uint2 y = *reinterpret_cast<const uint2*>(at);
-                        w[x][0] = y.x, w[x][1] = y.y;
-                    }
-                }
-            }
+            for (int x = 0; x < kHalves * kParts; ++x) ld_or_zero<kPart>(q_at + 2 * ((x / kParts) * 64 + (x % kParts) * 8), in, w[x]);
+        }
+        issue(0);
+        // ---- into fragments: rows whose fp16 form could overflow (bf16) are scaled by a power of two
+        if (warp < 2 * MT) {
             float coef = p.scale_log2;
             if (bf16) {
                 float most = 0.0f;
@@ -327,7 +343,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
                 if constexpr (kPart == 16) *reinterpret_cast<uint4*>(to) = make_uint4(w[x][0], w[x][1], w[x][2], w[x][3]);
                 else *reinterpret_cast<uint2*>(to) = make_uint2(w[x][0], w[x][1]);
             }
-            if (t4 == 0) s_coef[r] = coef, s_limit[r] = r < n_rows ? limit_of(t) : kNoToken;   // (rows that are not there hold nobody up)
+            if (t4 == 0) s_coef[q_row] = coef, s_limit[q_row] = q_row < n_rows ? limit_of(q_token) : kNoToken;   // (rows that are not there hold nobody up)
         }
         __syncthreads();
         float coef[MT][2], m[MT][2], l[MT][2], o[MT][kTilesN][4];
@@ -573,12 +589,11 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
             }
         }
         if (tid == 0 && u0 == 0 && p.min_units != 0) {   // who has a share of the problem, for fa_cache_join
-            const uint64_t begins = before + static_cast<uint64_t>(problem) * n_units;
             p.shares[static_cast<uint64_t>(b) * per_seq + problem] =
-                make_int2(alone ? -1 : static_cast<int>(2 * blockIdx.x + (first_segment ? 0 : 1)), static_cast<int>(rows_owner(begins + n_units - 1, work)));
+                make_int2(alone ? -1 : static_cast<int>(2 * blockIdx.x + (first_segment ? 0 : 1)), static_cast<int>(rows_owner(RowsWork{s_first[2], s_first[3], s_first[4]}, before + problem * n_units + n_units - 1)));
         }
         unit += u1 - u0;
-        if (unit == before + static_cast<uint64_t>(n_units) * per_seq) before = unit, ++b;
+        if (unit == before + n_units * per_seq) before = unit, ++b;
         __syncthreads();   // the sums have been read: the ring, the rows' data and the fragments may be written again
     }
 }
