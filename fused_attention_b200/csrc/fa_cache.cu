@@ -267,10 +267,9 @@ int fa_b200_cache_append(const fa_b200_cache* cache, const fa_b200_sequences* se
     a.q_heads = q_heads, a.bf16 = dtype == FA_B200_BF16, a.interleaved = flags & FA_B200_CACHE_NEIGHBOURS;
     a.blocks = (a.s.T + a.c.page - 2) / a.c.page + 1;   // that T tokens touch at most
     const uint64_t tasks = 2ull * a.s.B * a.blocks * a.c.heads;
-    const uint64_t q_threads = queries_or_null ? static_cast<uint64_t>(a.s.B) * a.s.T * q_heads * (H / 16) : 0;
-    uint64_t q_ctas = (q_threads + fa::kAppendThreads - 1) / fa::kAppendThreads;
-    if (q_ctas > 16384) q_ctas = 16384;
-    if (tasks + q_ctas > kMostCtas) return FA_B200_ERR_SHAPE;
+    const uint64_t q_threads = queries_or_null ? static_cast<uint64_t>(a.s.B) * a.s.T * ((q_heads + fa::kAppendHeads - 1) / fa::kAppendHeads) * (H / 16) : 0;
+    const uint64_t q_ctas = (q_threads + fa::kAppendThreads - 1) / fa::kAppendThreads;
+    if (tasks + q_ctas > kMostCtas || q_threads > 0xFFFFFF00ull) return FA_B200_ERR_SHAPE;
     a.tasks = static_cast<uint32_t>(tasks), a.query_ctas = static_cast<uint32_t>(q_ctas);
     const bool warp_tasks = a.s.T <= 4;
     const uint32_t task_ctas = static_cast<uint32_t>(warp_tasks ? (tasks + 3) / 4 : tasks);
@@ -305,20 +304,30 @@ int fa_b200_cache_select(const fa_b200_cache* cache, const fa_b200_sequences* se
     a.q = static_cast<const uint8_t*>(queries), a.q_b = 2 * queries_batch_stride, a.q_t = 2 * queries_token_stride;
     a.keys = static_cast<uint32_t*>(scratch), a.pages = pages;
     a.group = q_heads / a.c.heads, a.keep = keep, a.first = first, a.last = last, a.bf16 = dtype == FA_B200_BF16;
-    a.chunks = (a.s.width + fa::kScorePages - 1) / fa::kScorePages;
-    if (static_cast<uint64_t>(a.s.B) * a.c.heads * a.chunks > kMostCtas) return FA_B200_ERR_SHAPE;
+    // Query rows in tiles of 16: the heads of several tokens, or a part of one token's.
+    a.per_tile = a.group > 16 ? 1 : 16 / a.group;
+    const uint32_t all_tiles = a.group > 16 ? (a.group + 15) / 16 : (a.s.T + a.per_tile - 1) / a.per_tile;
+    a.tiles = all_tiles < fa::kScoreTiles ? all_tiles : fa::kScoreTiles;
+    a.turns = a.group > 16 ? (all_tiles + a.tiles - 1) / a.tiles : 1;
+    a.token_chunks = a.group > 16 ? a.s.T : (all_tiles + a.tiles - 1) / a.tiles;
     Device* d = nullptr;
     if ((rc = device_of(device, &d)) != FA_B200_OK) return rc;
+    // about eight CTAs an SM, each with 64 pages at least
+    const uint64_t problems = static_cast<uint64_t>(a.s.B) * a.c.heads * a.token_chunks, sms = static_cast<uint64_t>(d->sms.load());
+    const uint64_t most = (a.s.width + fa::kScoreWarps * fa::kScorePages - 1) / (fa::kScoreWarps * fa::kScorePages), wanted = (8 * sms + problems - 1) / problems;
+    a.chunks = static_cast<uint32_t>(wanted < most ? wanted : most);
+    if (problems * a.chunks > kMostCtas) return FA_B200_ERR_SHAPE;
     OnDevice on(device);
     if (on.rc != 0) return on.rc;
     const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-    const uint32_t grid = a.s.B * a.c.heads * a.chunks;
+    const uint32_t grid = static_cast<uint32_t>(problems * a.chunks);
+    const size_t smem = static_cast<size_t>(a.tiles) * (cache->head_dim / 16) * 2 * 32 * sizeof(uint4);   // 32 KB at most
     constexpr uint32_t kBlock = fa::kScoreWarps * 32;
     switch (cache->head_dim) {
-        case 16: rc = launch(&fa::fa_cache_scores<16>, grid, kBlock, 0, stream, a); break;
-        case 32: rc = launch(&fa::fa_cache_scores<32>, grid, kBlock, 0, stream, a); break;
-        case 64: rc = launch(&fa::fa_cache_scores<64>, grid, kBlock, 0, stream, a); break;
-        default: rc = launch(&fa::fa_cache_scores<128>, grid, kBlock, 0, stream, a); break;
+        case 16: rc = launch(&fa::fa_cache_scores<16>, grid, kBlock, smem, stream, a); break;
+        case 32: rc = launch(&fa::fa_cache_scores<32>, grid, kBlock, smem, stream, a); break;
+        case 64: rc = launch(&fa::fa_cache_scores<64>, grid, kBlock, smem, stream, a); break;
+        default: rc = launch(&fa::fa_cache_scores<128>, grid, kBlock, smem, stream, a); break;
     }
     if (rc != FA_B200_OK) return rc;
     const uint32_t per = (a.s.width + fa::kTakeThreads - 1) / fa::kTakeThreads;

@@ -33,10 +33,15 @@ struct AppendArgs {
 struct Sixteen {
     float a[8], b[8];
 };
+struct RawSixteen {
+    uint4 x, y;
+};
 template <int H>
-__device__ __forceinline__ Sixteen load_sixteen(const uint8_t* row, uint32_t j, bool bf16) {
-    const uint4 x = *reinterpret_cast<const uint4*>(row + 16 * j), y = *reinterpret_cast<const uint4*>(row + H + 16 * j);
-    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+__device__ __forceinline__ RawSixteen load_sixteen(const uint8_t* row, uint32_t j) {
+    return RawSixteen{*reinterpret_cast<const uint4*>(row + 16 * j), *reinterpret_cast<const uint4*>(row + H + 16 * j)};
+}
+__device__ __forceinline__ Sixteen unpack_sixteen(const RawSixteen& w, bool bf16) {
+    const uint32_t xs[4] = {w.x.x, w.x.y, w.x.z, w.x.w}, ys[4] = {w.y.x, w.y.y, w.y.z, w.y.w};
     Sixteen r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -50,32 +55,33 @@ __device__ __forceinline__ void turn(float& x, float& y, float c, float s) {
     y = __fadd_rn(__fmul_rn(y, c), __fmul_rn(x, s));
     x = u;
 }
-// cos and sin of the pairs that the sixteen values form: (i, i + H/2), or neighbours (2i, 2i + 1).
+// cos and sin of the eight pairs that the sixteen values form: (i, i + H/2), or neighbours (2i, 2i + 1).
+struct Angles {
+    float c[8], s[8];
+};
 template <int H>
-__device__ __forceinline__ void rotate(Sixteen& r, const AppendArgs& p, uint32_t position, uint32_t j) {
-    const float* c = p.cos + static_cast<size_t>(position) * (H / 2);
-    const float* s = p.sin + static_cast<size_t>(position) * (H / 2);
-    if (p.interleaved) {
+__device__ __forceinline__ Angles load_angles(const AppendArgs& p, uint32_t position, uint32_t j) {
+    Angles a;
+    const size_t at = static_cast<size_t>(position) * (H / 2);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const float4 cc = *reinterpret_cast<const float4*>(c + half * (H / 4) + 4 * j);
-            const float4 ss = *reinterpret_cast<const float4*>(s + half * (H / 4) + 4 * j);
-            float* x = half ? r.b : r.a;
-            turn(x[0], x[1], cc.x, ss.x);
-            turn(x[2], x[3], cc.y, ss.y);
-            turn(x[4], x[5], cc.z, ss.z);
-            turn(x[6], x[7], cc.w, ss.w);
+    for (int q = 0; q < 2; ++q) {
+        const size_t from = at + (p.interleaved ? q * (H / 4) + 4 * j : 8 * j + 4 * q);
+        const float4 c = *reinterpret_cast<const float4*>(p.cos + from), s = *reinterpret_cast<const float4*>(p.sin + from);
+        a.c[4 * q] = c.x, a.c[4 * q + 1] = c.y, a.c[4 * q + 2] = c.z, a.c[4 * q + 3] = c.w;
+        a.s[4 * q] = s.x, a.s[4 * q + 1] = s.y, a.s[4 * q + 2] = s.z, a.s[4 * q + 3] = s.w;
+    }
+    return a;
+}
+__device__ __forceinline__ void rotate(Sixteen& r, const Angles& a, bool interleaved) {
+    if (interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            turn(r.a[2 * i], r.a[2 * i + 1], a.c[i], a.s[i]);
+            turn(r.b[2 * i], r.b[2 * i + 1], a.c[4 + i], a.s[4 + i]);
         }
     } else {
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const float4 cc = *reinterpret_cast<const float4*>(c + 8 * j + 4 * q);
-            const float4 ss = *reinterpret_cast<const float4*>(s + 8 * j + 4 * q);
-            turn(r.a[4 * q], r.b[4 * q], cc.x, ss.x);
-            turn(r.a[4 * q + 1], r.b[4 * q + 1], cc.y, ss.y);
-            turn(r.a[4 * q + 2], r.b[4 * q + 2], cc.z, ss.z);
-            turn(r.a[4 * q + 3], r.b[4 * q + 3], cc.w, ss.w);
-        }
+        for (int i = 0; i < 8; ++i) turn(r.a[i], r.b[i], a.c[i], a.s[i]);
     }
 }
 
@@ -106,6 +112,7 @@ __device__ __forceinline__ uint32_t moved_codes(uint32_t four, float shrink) {
 }
 
 constexpr int kAppendThreads = 128;
+constexpr uint32_t kAppendHeads = 4;   // query heads of a thread: they share the angles
 
 // kTask threads a task (32: a warp, 128: the CTA).
 template <int H, int kTask>
@@ -119,26 +126,33 @@ __global__ void __launch_bounds__(kAppendThreads) fa_cache_append(const AppendAr
     const bool bf16 = p.bf16 != 0;
 
     const uint32_t task_ctas = gridDim.x - p.query_ctas;
-    if (blockIdx.x >= task_ctas) {   // ---- queries: 16 values a thread
-        const uint64_t n = static_cast<uint64_t>(p.s.B) * p.s.T * p.q_heads * kPerToken;
-        for (uint64_t i = static_cast<uint64_t>(blockIdx.x - task_ctas) * kAppendThreads + threadIdx.x; i < n;
-             i += static_cast<uint64_t>(p.query_ctas) * kAppendThreads) {
-            const uint32_t j = static_cast<uint32_t>(i % kPerToken);
-            const uint64_t head_row = i / kPerToken;
-            const uint32_t head = static_cast<uint32_t>(head_row % p.q_heads);
-            const uint64_t row = head_row / p.q_heads;
-            const uint32_t t = static_cast<uint32_t>(row % p.s.T), b = static_cast<uint32_t>(row / p.s.T);
-            uint8_t* out = p.rotated + head_row * (2 * H) + 16 * j;
+    if (blockIdx.x >= task_ctas) {   // ---- queries: 16 values of up to four heads a thread
+        const uint32_t fours = (p.q_heads + kAppendHeads - 1) / kAppendHeads, i = (blockIdx.x - task_ctas) * kAppendThreads + threadIdx.x;
+        const uint32_t j = i % kPerToken, four = i / kPerToken % fours, row = i / kPerToken / fours, b = row / p.s.T, t = row - b * p.s.T;
+        if (b >= p.s.B) return;
+        const uint32_t head = four * kAppendHeads, n = min(kAppendHeads, p.q_heads - head);
+        const uint8_t* const from = p.queries + b * p.queries_b + t * p.queries_t + static_cast<int64_t>(head) * (2 * H);
+        uint8_t* const out = p.rotated + (static_cast<uint64_t>(row) * p.q_heads + head) * (2 * H) + 16 * j;
+        RawSixteen raw[kAppendHeads];
+#pragma unroll
+        for (uint32_t h = 0; h < kAppendHeads; ++h)
+            if (h < n) raw[h] = load_sixteen<H>(from + h * (2 * H), j);
+        const uint64_t at = static_cast<uint64_t>(max(p.s.lengths[b], 0)) + t;
+        const bool there = t < cache_count(p.s, b) && (p.cos == nullptr || at < p.positions);
+        Angles angles;
+        if (there && p.cos != nullptr) angles = load_angles<H>(p, static_cast<uint32_t>(at), j);
+#pragma unroll
+        for (uint32_t h = 0; h < kAppendHeads; ++h) {
+            if (h >= n) break;
             uint4 x = make_uint4(0, 0, 0, 0), y = x;
-            const uint64_t at = static_cast<uint64_t>(max(p.s.lengths[b], 0)) + t;
-            if (t < cache_count(p.s, b) && (p.cos == nullptr || at < p.positions)) {
-                Sixteen r = load_sixteen<H>(p.queries + b * p.queries_b + t * p.queries_t + static_cast<int64_t>(head) * (2 * H), j, bf16);
-                if (p.cos != nullptr) rotate<H>(r, p, static_cast<uint32_t>(at), j);
+            if (there) {
+                Sixteen r = unpack_sixteen(raw[h], bf16);
+                if (p.cos != nullptr) rotate(r, angles, p.interleaved != 0);
                 x = make_uint4(pack_16(r.a[0], r.a[1], bf16), pack_16(r.a[2], r.a[3], bf16), pack_16(r.a[4], r.a[5], bf16), pack_16(r.a[6], r.a[7], bf16));
                 y = make_uint4(pack_16(r.b[0], r.b[1], bf16), pack_16(r.b[2], r.b[3], bf16), pack_16(r.b[4], r.b[5], bf16), pack_16(r.b[6], r.b[7], bf16));
             }
-            *reinterpret_cast<uint4*>(out) = x;
-            *reinterpret_cast<uint4*>(out + H) = y;
+            *reinterpret_cast<uint4*>(out + h * (2 * H)) = x;
+            *reinterpret_cast<uint4*>(out + h * (2 * H) + H) = y;
         }
         return;
     }
@@ -172,25 +186,42 @@ __global__ void __launch_bounds__(kAppendThreads) fa_cache_append(const AppendAr
     const uint8_t* rows = is_v ? p.values + b * p.values_b : p.keys + b * p.keys_b;
     const int64_t row_pitch = is_v ? p.values_t : p.keys_t;
     rows += static_cast<int64_t>(head) * (2 * H);
-    auto load = [&](uint32_t slot) {
-        const uint32_t t = static_cast<uint32_t>(first + slot - held);
-        Sixteen r = load_sixteen<H>(rows + t * row_pitch, j, bf16);
-        if (!is_v && p.cos != nullptr) rotate<H>(r, p, static_cast<uint32_t>(first) + slot, j);
+    // A CTA's task is read once: a page's tokens fit its threads' registers (a warp's has a few tokens, or is read again).
+    constexpr int kHeld = kTask > 32 ? (128 + kTokens - 1) / kTokens : 1;
+    RawSixteen raw[kHeld];
+    auto from = [&](uint32_t slot) { return load_sixteen<H>(rows + static_cast<uint32_t>(first + slot - held) * row_pitch, j); };
+    if (kTask > 32) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i)
+            if (begin + sub + i * kTokens < end) raw[i] = from(begin + sub + i * kTokens);
+    }
+    const bool turned = !is_v && p.cos != nullptr;
+    auto values_of = [&](const RawSixteen& w, uint32_t slot) {
+        Sixteen r = unpack_sixteen(w, bf16);
+        if (turned) rotate(r, load_angles<H>(p, static_cast<uint32_t>(first) + slot, j), p.interleaved != 0);
         return r;
+    };
+    auto each = [&](auto&& f) {   // f(slot, values) for this thread's new tokens
+        if (kTask > 32) {
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i)
+                if (begin + sub + i * kTokens < end) f(begin + sub + i * kTokens, values_of(raw[i], begin + sub + i * kTokens));
+        } else {
+            for (uint32_t slot = begin + sub; slot < end; slot += kTokens) f(slot, values_of(from(slot), slot));
+        }
     };
     float* const scale_at = (is_v ? p.c.v_scale : p.c.k_scale) + static_cast<size_t>(page) * p.c.heads + head;
     const float before = begin != 0 ? *scale_at : 0.0f;
 
     float most = 0.0f;
     bool finite = true;
-    for (uint32_t slot = begin + sub; slot < end; slot += kTokens) {
-        const Sixteen r = load(slot);
+    each([&](uint32_t, const Sixteen& r) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             most = fmaxf(most, fmaxf(fabsf(r.a[i]), fabsf(r.b[i])));
             finite = finite && r.a[i] - r.a[i] == 0.0f && r.b[i] - r.b[i] == 0.0f;
         }
-    }
+    });
     if (!finite) most = __int_as_float(0x7F800000);
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
@@ -225,8 +256,7 @@ __global__ void __launch_bounds__(kAppendThreads) fa_cache_append(const AppendAr
     uint32_t low[8], high[8];   // fp16 pairs: the bounds of the thread's dimensions
 #pragma unroll
     for (int i = 0; i < 8; ++i) low[i] = 0x7C007C00u, high[i] = 0xFC00FC00u;
-    for (uint32_t slot = begin + sub; slot < end; slot += kTokens) {
-        const Sixteen r = load(slot);
+    each([&](uint32_t slot, const Sixteen& r) {
         uint32_t w[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -244,7 +274,7 @@ __global__ void __launch_bounds__(kAppendThreads) fa_cache_append(const AppendAr
                 high[i] = half2_max(high[i], x);
             }
         }
-    }
+    });
     if (!is_v) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {

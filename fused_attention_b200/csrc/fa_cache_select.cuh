@@ -25,11 +25,17 @@ struct SelectArgs {
     uint32_t* keys;          // [B, T, kv heads, width]: sortable scores
     int32_t* pages;          // [B, T, kv heads, keep]
     uint32_t group, keep, first, last, bf16;
+    uint32_t per_tile;       // tokens whose heads share a tile of 16 rows (1 where they are more than 16)
+    uint32_t tiles;          // tiles that a CTA holds
+    uint32_t turns;          // groups of 16 * tiles heads of a token (1 but for more than 64 of them)
+    uint32_t token_chunks;   // CTAs that share the tokens
     uint32_t chunks;         // CTAs that share the pages of a sequence and head
 };
 
 constexpr int kScoreWarps = 4;
-constexpr int kScorePages = 8 * kScoreWarps;   // pages of a CTA at a time
+constexpr int kScorePages = 16;    // of a warp at a time: two n-tiles
+constexpr int kScoreTiles = 4;     // of 16 query rows that a CTA holds at most
+
 constexpr int kTakeThreads = 256;
 
 // Whole numbers of the same order as the floats (a NaN above all).
@@ -47,7 +53,10 @@ __device__ __forceinline__ int64_t query_position(const CacheView& c, const Cach
 
 template <int H>
 __global__ void __launch_bounds__(kScoreWarps * 32) fa_cache_scores(const SelectArgs p) {
-    constexpr int kHalves = H == 128 ? 2 : 1, kBytes = H >= 64 ? 16 : H / 4, kWords = kBytes / 4;
+    constexpr int kHalves = H == 128 ? 2 : 1, kBytes = H >= 64 ? 16 : H / 4, kWords = kBytes / 4, kSteps = kHalves * kWords;
+    extern __shared__ __align__(16) uint4 s_frag[];   // [tiles][kSteps][positive, negative part][lane]
+    __shared__ float s_qs[kScoreTiles][16];
+    __shared__ float s_val[kScoreWarps][16][kScorePages + 1];
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3u;
     grid_dep_wait();
     grid_dep_launch();
@@ -55,119 +64,168 @@ __global__ void __launch_bounds__(kScoreWarps * 32) fa_cache_scores(const Select
     uint32_t rest = blockIdx.x;
     const uint32_t chunk = rest % p.chunks;
     rest /= p.chunks;
-    const uint32_t head = rest % p.c.heads, b = rest / p.c.heads;
+    const uint32_t head = rest % p.c.heads;
+    rest /= p.c.heads;
+    const uint32_t token_chunk = rest % p.token_chunks, b = rest / p.token_chunks;
     const uint32_t held = cache_length(p.c, p.s, b), count = cache_count(p.s, b);
-    if (threadIdx.x == 0 && chunk == 0 && head == 0 && !cache_length_ok(p.c, p.s, b)) cache_report(p.c.status, kCacheBadPosition);
-    if (held == 0 || count == 0) return;
+    if (threadIdx.x == 0 && chunk == 0 && head == 0 && token_chunk == 0 && !cache_length_ok(p.c, p.s, b)) cache_report(p.c.status, kCacheBadPosition);
+    const bool many = p.group > 16;   // heads of a token: a token a CTA
+    const uint32_t t0 = many ? token_chunk : token_chunk * p.tiles * p.per_tile;
+    if (held == 0 || t0 >= count) return;
     const uint32_t n_pages = (held + p.c.page - 1) >> p.c.page_shift;
+    // what the CTA's last query sees bounds its pages
+    const uint32_t t_end = min(count, t0 + (many ? 1u : p.tiles * p.per_tile));
 
-    for (uint32_t p0 = chunk * kScorePages + warp * 8; p0 < n_pages; p0 += p.chunks * kScorePages) {
-        // ---- bounds of page p0 + g: whole numbers in fp16
-        uint32_t hi[kHalves][kWords][2], lo[kHalves][kWords][2];
-        float scale = 0.0f;
-        const uint32_t mine = p0 + g;
-        int32_t page = -1;
-        if (mine < n_pages) {
-            page = p.s.table[b * p.s.table_stride + mine];
-            if (static_cast<uint32_t>(page) >= p.c.n_pages) {
-                if (t4 == 0) cache_report(p.c.status, kCacheBadPage);
-                page = -1;
-            }
-        }
-        if (page >= 0) scale = p.c.k_scale[static_cast<uint64_t>(page) * p.c.heads + head];
-        const uint8_t* const at = p.c.bounds + (static_cast<uint64_t>(page < 0 ? 0 : page) * p.c.heads + head) * (2 * H) + t4 * kBytes;
+    for (uint32_t turn = 0; turn < p.turns; ++turn) {
+        if (turn > 0) __syncthreads();
+        // ---- q8 into fragments, a warp a tile
+        for (uint32_t tile = warp; tile < p.tiles; tile += kScoreWarps) {
+            float most[2], raw[2][kHalves][kBytes];
 #pragma unroll
-        for (int half = 0; half < kHalves; ++half)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                uint32_t w[4] = {0, 0, 0, 0};
-                if (page >= 0) {
-                    const uint8_t* from = at + e * H + half * 64;
-                    if constexpr (kBytes == 16) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(from);
-                        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
-                    } else if constexpr (kBytes == 8) {
-                        const uint2 x = *reinterpret_cast<const uint2*>(from);
-                        w[0] = x.x, w[1] = x.y;
-                    } else {
-                        w[0] = *reinterpret_cast<const uint32_t*>(from);
-                    }
-                }
-                const __half2 quarter = __float2half2_rn(0.25f), round = __float2half2_rn(1536.0f);   // (the unit of fp16 there is 1)
-#pragma unroll
-                for (int j = 0; j < kWords; ++j) {
-                    uint32_t x[2];
-                    e4m3x4_to_half2(w[j], x[0], x[1]);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const __half2 y = __hsub2(__hfma2(*reinterpret_cast<const __half2*>(&x[i]), quarter, round), round);
-                        (e ? hi : lo)[half][j][i] = *reinterpret_cast<const uint32_t*>(&y);
-                    }
-                }
-            }
-        for (uint32_t t = 0; t < count; ++t) {
-            float best[2] = {-INFINITY, -INFINITY};   // of pages p0 + 2 t4, + 1
-            for (uint32_t r0 = 0; r0 < p.group; r0 += 16) {
-                // ---- q8 of heads r0 + g and r0 + g + 8
-                float most[2], raw[2][kHalves][kBytes];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const uint32_t r = r0 + u * 8 + g;
-                    most[u] = 0.0f;
-                    const uint8_t* const row = p.q + b * p.q_b + t * p.q_t + static_cast<int64_t>(head * p.group + (r < p.group ? r : 0)) * (2 * H) + 2 * t4 * kBytes;
-#pragma unroll
-                    for (int half = 0; half < kHalves; ++half)
-#pragma unroll
-                        for (int j = 0; j < kBytes / 4; ++j) {
-                            uint2 w = make_uint2(0, 0);
-                            if (r < p.group) w = *reinterpret_cast<const uint2*>(row + half * 128 + 8 * j);
-                            const float2 x = unpack_16(w.x, bf16), y = unpack_16(w.y, bf16);
-                            raw[u][half][4 * j] = x.x, raw[u][half][4 * j + 1] = x.y, raw[u][half][4 * j + 2] = y.x, raw[u][half][4 * j + 3] = y.y;
-                            most[u] = fmaxf(most[u], fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y))));
-                        }
-                    most[u] = fmaxf(most[u], __shfl_xor_sync(0xFFFFFFFFu, most[u], 1));
-                    most[u] = fmaxf(most[u], __shfl_xor_sync(0xFFFFFFFFu, most[u], 2));
-                }
-                const float up[2] = {most[0] > 0.0f ? __fmul_rn(__frcp_rn(most[0]), 127.0f) : 0.0f, most[1] > 0.0f ? __fmul_rn(__frcp_rn(most[1]), 127.0f) : 0.0f};
-                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t r = u * 8 + g;
+                const uint32_t t = many ? t0 : t0 + tile * p.per_tile + r / p.group, i = many ? (turn * p.tiles + tile) * 16 + r : r % p.group;
+                const bool in = t < t_end && (many ? i < p.group : r < p.per_tile * p.group);
+                const uint8_t* const row = p.q + (in ? b * p.q_b + t * p.q_t + static_cast<int64_t>(head * p.group + i) * (2 * H) + 2 * t4 * kBytes : 0);
+                most[u] = 0.0f;
 #pragma unroll
                 for (int half = 0; half < kHalves; ++half)
 #pragma unroll
                     for (int j = 0; j < kWords; ++j) {
-                        uint32_t plus[4], minus[4];
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-#pragma unroll
-                            for (int u = 0; u < 2; ++u) {
-                                const float x = rintf(__fmul_rn(raw[u][half][4 * j + 2 * i], up[u])), y = rintf(__fmul_rn(raw[u][half][4 * j + 2 * i + 1], up[u]));
-                                plus[2 * i + u] = pack_half2(fmaxf(x, 0.0f), fmaxf(y, 0.0f));
-                                minus[2 * i + u] = pack_half2(fminf(x, 0.0f), fminf(y, 0.0f));
-                            }
-                        mma_m16n8k16(d, plus, hi[half][j][0], hi[half][j][1]);
-                        mma_m16n8k16(d, minus, lo[half][j][0], lo[half][j][1]);
+                        uint2 w = make_uint2(0, 0);
+                        if (in) w = *reinterpret_cast<const uint2*>(row + half * 128 + 8 * j);
+                        const float2 x = unpack_16(w.x, bf16), y = unpack_16(w.y, bf16);
+                        raw[u][half][4 * j] = x.x, raw[u][half][4 * j + 1] = x.y, raw[u][half][4 * j + 2] = y.x, raw[u][half][4 * j + 3] = y.y;
+                        most[u] = fmaxf(most[u], fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y))));
                     }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int u = e >> 1;
-                    const float x = r0 + u * 8 + g < p.group ? __fmul_rn(d[e], __fmul_rn(most[u], 1.0f / 127.0f)) : -INFINITY;
-                    best[e & 1] = fmaxf(best[e & 1], x);
-                }
+                most[u] = fmaxf(most[u], __shfl_xor_sync(0xFFFFFFFFu, most[u], 1));
+                most[u] = fmaxf(most[u], __shfl_xor_sync(0xFFFFFFFFu, most[u], 2));
+                // (rows that are not there must not be the largest)
+                if (t4 == 0) s_qs[tile][r] = in ? __fmul_rn(most[u], 1.0f / 127.0f) : -1.0f;
             }
+            const float up[2] = {most[0] > 0.0f ? __fmul_rn(__frcp_rn(most[0]), 127.0f) : 0.0f, most[1] > 0.0f ? __fmul_rn(__frcp_rn(most[1]), 127.0f) : 0.0f};
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int half = 0; half < kHalves; ++half)
 #pragma unroll
-                for (int dlt = 4; dlt <= 16; dlt <<= 1) best[e] = fmaxf(best[e], __shfl_xor_sync(0xFFFFFFFFu, best[e], dlt));
-            // lane (g, t4) has pages 2 t4 and 2 t4 + 1, the scale of page g: lanes with g = 2 t4 + e write page g
-            const float other = __shfl_sync(0xFFFFFFFFu, best[1], lane >> 3), mine_best = __shfl_sync(0xFFFFFFFFu, best[0], lane >> 3);
-            if (t4 == 0 && mine < n_pages) {
-                const int64_t position = query_position(p.c, p.s, b, t);
-                const int64_t own = position >> p.c.page_shift;
-                float score = __fmul_rn(g & 1u ? other : mine_best, scale);
-                if (page < 0) score = -INFINITY;   // (not to be taken unless it has to be)
-                if (mine < p.first || static_cast<int64_t>(mine) > own - static_cast<int64_t>(p.last)) score = INFINITY;
-                uint32_t key = sortable(score);
-                if (position < 0 || static_cast<int64_t>(mine) > own) key = 0;   // behind the query
-                p.keys[((static_cast<uint64_t>(b) * p.s.T + t) * p.c.heads + head) * p.s.width + mine] = key;
+                for (int j = 0; j < kWords; ++j) {
+                    uint32_t plus[4], minus[4];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const float x = rintf(__fmul_rn(raw[u][half][4 * j + 2 * i], up[u])), y = rintf(__fmul_rn(raw[u][half][4 * j + 2 * i + 1], up[u]));
+                            plus[2 * i + u] = pack_half2(fmaxf(x, 0.0f), fmaxf(y, 0.0f));
+                            minus[2 * i + u] = pack_half2(fminf(x, 0.0f), fminf(y, 0.0f));
+                        }
+                    uint4* const to = s_frag + ((tile * kSteps + half * kWords + j) * 2) * 32 + lane;
+                    to[0] = make_uint4(plus[0], plus[1], plus[2], plus[3]);
+                    to[32] = make_uint4(minus[0], minus[1], minus[2], minus[3]);
+                }
+        }
+        __syncthreads();
+
+        const uint32_t stride = p.chunks * kScoreWarps * kScorePages;
+        for (uint32_t p0 = (chunk * kScoreWarps + warp) * kScorePages; p0 < n_pages; p0 += stride) {
+            // ---- bounds of pages p0 + g and p0 + 8 + g: whole numbers in fp16
+            uint32_t hi[2][kHalves][kWords][2], lo[2][kHalves][kWords][2];
+            uint4 raw[2][kHalves][2];
+            float scale[2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const uint32_t mine = p0 + 8 * n + g;
+                int32_t page = mine < n_pages ? p.s.table[b * p.s.table_stride + mine] : -1;
+                if (static_cast<uint32_t>(page) >= p.c.n_pages) {
+                    if (mine < n_pages && t4 == 0 && turn == 0) cache_report(p.c.status, kCacheBadPage);
+                    page = -1;
+                }
+                // (a page that is not there: read the first, and never take it for its score)
+                const uint64_t at = static_cast<uint64_t>(page < 0 ? 0 : page) * p.c.heads + head;
+                scale[n] = page < 0 ? -1.0f : p.c.k_scale[at];
+                const uint8_t* const from = p.c.bounds + at * (2 * H) + t4 * kBytes;
+#pragma unroll
+                for (int half = 0; half < kHalves; ++half)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        if constexpr (kBytes == 16) {
+                            raw[n][half][e] = *reinterpret_cast<const uint4*>(from + e * H + half * 64);
+                        } else if constexpr (kBytes == 8) {
+                            const uint2 x = *reinterpret_cast<const uint2*>(from + e * H);
+                            raw[n][half][e] = make_uint4(x.x, x.y, 0, 0);
+                        } else {
+                            raw[n][half][e] = make_uint4(*reinterpret_cast<const uint32_t*>(from + e * H), 0, 0, 0);
+                        }
+                    }
+            }
+            const __half2 quarter = __float2half2_rn(0.25f), round = __float2half2_rn(1536.0f);   // (the unit of fp16 there is 1)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int half = 0; half < kHalves; ++half)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t w[4] = {raw[n][half][e].x, raw[n][half][e].y, raw[n][half][e].z, raw[n][half][e].w};
+#pragma unroll
+                        for (int j = 0; j < kWords; ++j) {
+                            uint32_t x[2];
+                            e4m3x4_to_half2(w[j], x[0], x[1]);
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const __half2 y = __hsub2(__hfma2(*reinterpret_cast<const __half2*>(&x[i]), quarter, round), round);
+                                (e ? hi : lo)[n][half][j][i] = *reinterpret_cast<const uint32_t*>(&y);
+                            }
+                        }
+                    }
+            // scales of the pages that this lane writes: page p0 + lane % 16
+            const float scale_lo = __shfl_sync(0xFFFFFFFFu, scale[0], (lane & 7u) * 4), scale_hi = __shfl_sync(0xFFFFFFFFu, scale[1], (lane & 7u) * 4);
+            const float my_scale = lane & 8u ? scale_hi : scale_lo;
+            const uint32_t my_page = p0 + (lane & 15u);
+            float best = -INFINITY;   // (many)
+            for (uint32_t tile = 0; tile < p.tiles; ++tile) {
+                float d[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+                for (int half = 0; half < kHalves; ++half)
+#pragma unroll
+                    for (int j = 0; j < kWords; ++j) {
+                        const uint4* const from = s_frag + ((tile * kSteps + half * kWords + j) * 2) * 32 + lane;
+                        const uint4 x = from[0], y = from[32];
+                        const uint32_t plus[4] = {x.x, x.y, x.z, x.w}, minus[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) {
+                            mma_m16n8k16(d[n], plus, hi[n][half][j][0], hi[n][half][j][1]);
+                            mma_m16n8k16(d[n], minus, lo[n][half][j][0], lo[n][half][j][1]);
+                        }
+                    }
+                // ---- the largest of a token's heads, through the warp's own corner of shared memory
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const float qs = s_qs[tile][u * 8 + g];
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) s_val[warp][u * 8 + g][n * 8 + 2 * t4 + e] = qs < 0.0f ? -INFINITY : __fmul_rn(d[n][2 * u + e], qs);
+                }
+                __syncwarp();
+                for (uint32_t i = lane >> 4; i < (many ? 1u : p.per_tile); i += 2) {
+                    const uint32_t t = many ? t0 : t0 + tile * p.per_tile + i, rows = many ? 16u : p.group;
+                    if (t >= t_end) break;
+                    float x = best;
+                    for (uint32_t r = 0; r < rows; ++r) x = fmaxf(x, s_val[warp][(many ? 0u : i * p.group) + r][lane & 15u]);
+                    if (many) {
+                        best = x;
+                        if (tile + 1 < p.tiles) break;
+                    }
+                    if (my_page < n_pages) {
+                        const int64_t position = query_position(p.c, p.s, b, t);
+                        const int64_t own = position >> p.c.page_shift;
+                        float score = my_scale == -1.0f ? -INFINITY : __fmul_rn(x, my_scale);
+                        if (my_page < p.first || static_cast<int64_t>(my_page) > own - static_cast<int64_t>(p.last)) score = INFINITY;
+                        uint32_t key = sortable(score);
+                        if (position < 0 || static_cast<int64_t>(my_page) > own) key = 0;   // behind the query
+                        uint32_t* const at = p.keys + ((static_cast<uint64_t>(b) * p.s.T + t) * p.c.heads + head) * p.s.width + my_page;
+                        *at = turn > 0 ? max(key, *at) : key;
+                    }
+                }
+                __syncwarp();
             }
         }
     }
