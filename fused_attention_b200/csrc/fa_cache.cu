@@ -312,9 +312,9 @@ int fa_b200_cache_select(const fa_b200_cache* cache, const fa_b200_sequences* se
     a.token_chunks = a.group > 16 ? a.s.T : (all_tiles + a.tiles - 1) / a.tiles;
     Device* d = nullptr;
     if ((rc = device_of(device, &d)) != FA_B200_OK) return rc;
-    // about eight CTAs an SM, each with 64 pages at least
+    // as many CTAs as are resident at once, each with 64 pages at least: what a CTA does before its first page is much of its time
     const uint64_t problems = static_cast<uint64_t>(a.s.B) * a.c.heads * a.token_chunks, sms = static_cast<uint64_t>(d->sms.load());
-    const uint64_t most = (a.s.width + fa::kScoreWarps * fa::kScorePages - 1) / (fa::kScoreWarps * fa::kScorePages), wanted = (8 * sms + problems - 1) / problems;
+    const uint64_t most = (a.s.width + fa::kScoreWarps * fa::kScorePages - 1) / (fa::kScoreWarps * fa::kScorePages), wanted = problems < fa::kScoreCtas * sms ? fa::kScoreCtas * sms / problems : 1;
     a.chunks = static_cast<uint32_t>(wanted < most ? wanted : most);
     if (problems * a.chunks > kMostCtas) return FA_B200_ERR_SHAPE;
     OnDevice on(device);

@@ -95,6 +95,17 @@ __device__ __forceinline__ float append_scale(float most) {
 // (the larger of the two, NaN if one is)
 __device__ __forceinline__ float larger_scale(float x, float y) { return x > y || x != x ? x : y; }
 
+// NaN if one is.
+__device__ __forceinline__ float max_nan(float x, float y) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float min_nan(float x, float y) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+    return r;
+}
 __device__ __forceinline__ uint32_t half2_min(uint32_t x, uint32_t y) {
     const __half2 r = __hmin2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y));
     return *reinterpret_cast<const uint32_t*>(&r);
@@ -116,7 +127,7 @@ constexpr uint32_t kAppendHeads = 4;   // query heads of a thread: they share th
 
 // kTask threads a task (32: a warp, 128: the CTA).
 template <int H, int kTask>
-__global__ void __launch_bounds__(kAppendThreads) fa_cache_append(const AppendArgs p) {
+__global__ void __launch_bounds__(kAppendThreads, 5) fa_cache_append(const AppendArgs p) {
     constexpr int kPerToken = H / 16;                    // threads that share a token
     constexpr int kTokens = kTask / kPerToken;           // tokens at a time
     __shared__ float s_most[kAppendThreads / 32];
@@ -133,12 +144,12 @@ __global__ void __launch_bounds__(kAppendThreads) fa_cache_append(const AppendAr
         const uint32_t head = four * kAppendHeads, n = min(kAppendHeads, p.q_heads - head);
         const uint8_t* const from = p.queries + b * p.queries_b + t * p.queries_t + static_cast<int64_t>(head) * (2 * H);
         uint8_t* const out = p.rotated + (static_cast<uint64_t>(row) * p.q_heads + head) * (2 * H) + 16 * j;
+        const uint64_t at = static_cast<uint64_t>(max(p.s.lengths[b], 0)) + t;
+        const bool there = t < cache_count(p.s, b) && (p.cos == nullptr || at < p.positions);
         RawSixteen raw[kAppendHeads];
 #pragma unroll
         for (uint32_t h = 0; h < kAppendHeads; ++h)
-            if (h < n) raw[h] = load_sixteen<H>(from + h * (2 * H), j);
-        const uint64_t at = static_cast<uint64_t>(max(p.s.lengths[b], 0)) + t;
-        const bool there = t < cache_count(p.s, b) && (p.cos == nullptr || at < p.positions);
+            if (there && h < n) raw[h] = load_sixteen<H>(from + h * (2 * H), j);
         Angles angles;
         if (there && p.cos != nullptr) angles = load_angles<H>(p, static_cast<uint32_t>(at), j);
 #pragma unroll
@@ -176,24 +187,20 @@ __global__ void __launch_bounds__(kAppendThreads) fa_cache_append(const AppendAr
     const uint32_t begin = nth == 0 ? held & (p.c.page - 1) : 0u;   // slots [begin, end) are new
     const uint32_t end = static_cast<uint32_t>(min(static_cast<uint64_t>(p.c.page), static_cast<uint64_t>(held) + n - first));
     int32_t page = -1;
-    if (held_signed >= 0 && block < p.s.width) page = p.s.table[b * p.s.table_stride + block];
     const bool fits = held_signed >= 0 && block < p.s.width && (p.cos == nullptr || first + end <= p.positions);
-    if (!fits || static_cast<uint32_t>(page) >= p.c.n_pages) {
-        if (tid == 0) cache_report(p.c.status, fits ? kCacheBadPage : kCacheBadPosition);
-        return;
-    }
+    if (fits) page = p.s.table[b * p.s.table_stride + block];   // (asked for ahead of the tokens, used behind them)
     const uint32_t j = tid % kPerToken, sub = tid / kPerToken;
     const uint8_t* rows = is_v ? p.values + b * p.values_b : p.keys + b * p.keys_b;
     const int64_t row_pitch = is_v ? p.values_t : p.keys_t;
     rows += static_cast<int64_t>(head) * (2 * H);
-    // A CTA's task is read once: a page's tokens fit its threads' registers (a warp's has a few tokens, or is read again).
-    constexpr int kHeld = kTask > 32 ? (128 + kTokens - 1) / kTokens : 1;
-    RawSixteen raw[kHeld];
+    // Tokens are read for the scale and, from the caches, again for the codes: holding them takes registers that are worth more as
+    // CTAs (34 us against 39 with four prompts of up to 2048); the first of each thread is asked for ahead of all else.
+    RawSixteen raw;
     auto from = [&](uint32_t slot) { return load_sixteen<H>(rows + static_cast<uint32_t>(first + slot - held) * row_pitch, j); };
-    if (kTask > 32) {
-#pragma unroll
-        for (int i = 0; i < kHeld; ++i)
-            if (begin + sub + i * kTokens < end) raw[i] = from(begin + sub + i * kTokens);
+    if (begin + sub < end) raw = from(begin + sub);
+    if (!fits || static_cast<uint32_t>(page) >= p.c.n_pages) {
+        if (tid == 0) cache_report(p.c.status, fits ? kCacheBadPage : kCacheBadPosition);
+        return;
     }
     const bool turned = !is_v && p.cos != nullptr;
     auto values_of = [&](const RawSixteen& w, uint32_t slot) {
@@ -202,27 +209,35 @@ __global__ void __launch_bounds__(kAppendThreads) fa_cache_append(const AppendAr
         return r;
     };
     auto each = [&](auto&& f) {   // f(slot, values) for this thread's new tokens
-        if (kTask > 32) {
-#pragma unroll
-            for (int i = 0; i < kHeld; ++i)
-                if (begin + sub + i * kTokens < end) f(begin + sub + i * kTokens, values_of(raw[i], begin + sub + i * kTokens));
-        } else {
-            for (uint32_t slot = begin + sub; slot < end; slot += kTokens) f(slot, values_of(from(slot), slot));
-        }
+        for (uint32_t slot = begin + sub; slot < end; slot += kTokens) f(slot, values_of(slot == begin + sub ? raw : from(slot), slot));
     };
     float* const scale_at = (is_v ? p.c.v_scale : p.c.k_scale) + static_cast<size_t>(page) * p.c.heads + head;
     const float before = begin != 0 ? *scale_at : 0.0f;
 
+    // the largest magnitude, NaN if a value is; for keys from the lowest and highest value by dimension, whose codes are the bounds
+    // (rounding keeps their order)
     float most = 0.0f;
-    bool finite = true;
-    each([&](uint32_t, const Sixteen& r) {
+    float lowest[16], highest[16];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            most = fmaxf(most, fmaxf(fabsf(r.a[i]), fabsf(r.b[i])));
-            finite = finite && r.a[i] - r.a[i] == 0.0f && r.b[i] - r.b[i] == 0.0f;
-        }
-    });
-    if (!finite) most = __int_as_float(0x7F800000);
+    for (int i = 0; i < 16; ++i) lowest[i] = __int_as_float(0x7F800000), highest[i] = __int_as_float(0xFF800000);
+    if (is_v) {
+        each([&](uint32_t, const Sixteen& r) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) most = max_nan(max_nan(most, fabsf(r.a[i])), fabsf(r.b[i]));
+        });
+    } else {
+        each([&](uint32_t, const Sixteen& r) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                lowest[i] = min_nan(lowest[i], r.a[i]), highest[i] = max_nan(highest[i], r.a[i]);
+                lowest[8 + i] = min_nan(lowest[8 + i], r.b[i]), highest[8 + i] = max_nan(highest[8 + i], r.b[i]);
+            }
+        });
+        if (begin + sub < end)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) most = max_nan(max_nan(most, -lowest[i]), highest[i]);
+    }
+    if (!(most < __int_as_float(0x7F800000))) most = __int_as_float(0x7F800000);
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
     if (kTask > 32) {
@@ -253,9 +268,6 @@ __global__ void __launch_bounds__(kAppendThreads) fa_cache_append(const AppendAr
             *at = w;
         }
     }
-    uint32_t low[8], high[8];   // fp16 pairs: the bounds of the thread's dimensions
-#pragma unroll
-    for (int i = 0; i < 8; ++i) low[i] = 0x7C007C00u, high[i] = 0xFC00FC00u;
     each([&](uint32_t slot, const Sixteen& r) {
         uint32_t w[8];
 #pragma unroll
@@ -266,18 +278,14 @@ __global__ void __launch_bounds__(kAppendThreads) fa_cache_append(const AppendAr
         uint8_t* const at = base + slot * pitch + 8 * j;
         *reinterpret_cast<uint2*>(at) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
         *reinterpret_cast<uint2*>(at + H / 2) = make_uint2(w[4] | (w[5] << 16), w[6] | (w[7] << 16));
-        if (!is_v) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t x = e4m3x2_to_half2(w[i]);
-                low[i] = half2_min(low[i], x);
-                high[i] = half2_max(high[i], x);
-            }
-        }
     });
     if (!is_v) {
+        uint32_t low[8], high[8];   // fp16 pairs: the bounds of the thread's dimensions
+        const bool some = begin + sub < end;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
+            low[i] = some ? (good ? e4m3x2_to_half2(floats_to_e4m3x2(lowest[2 * i] * inverse, lowest[2 * i + 1] * inverse)) : 0u) : 0x7C007C00u;
+            high[i] = some ? (good ? e4m3x2_to_half2(floats_to_e4m3x2(highest[2 * i] * inverse, highest[2 * i + 1] * inverse)) : 0u) : 0xFC00FC00u;
 #pragma unroll
             for (int d = 16; d >= kPerToken; d >>= 1) {
                 low[i] = half2_min(low[i], __shfl_xor_sync(0xFFFFFFFFu, low[i], d));

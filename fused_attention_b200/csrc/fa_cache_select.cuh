@@ -34,6 +34,7 @@ struct SelectArgs {
 
 constexpr int kScoreWarps = 4;
 constexpr int kScorePages = 16;    // of a warp at a time: two n-tiles
+constexpr int kScoreCtas = 4;      // on an SM
 constexpr int kScoreTiles = 4;     // of 16 query rows that a CTA holds at most
 
 constexpr int kTakeThreads = 256;
@@ -51,8 +52,17 @@ __device__ __forceinline__ int64_t query_position(const CacheView& c, const Cach
     return t < count && at >= 0 ? at : -1;
 }
 
+// 16, 8 or 4 bytes of bounds.  Volatile: asked for where it stands, a turn ahead of its use.
+template <int kBytes>
+__device__ __forceinline__ void ld_bounds(const uint8_t* from, uint4& w) {
+    w = make_uint4(0, 0, 0, 0);
+    if constexpr (kBytes == 16) asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "l"(from));
+    else if constexpr (kBytes == 8) asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(w.x), "=r"(w.y) : "l"(from));
+    else asm volatile("ld.global.u32 %0, [%1];" : "=r"(w.x) : "l"(from));
+}
+
 template <int H>
-__global__ void __launch_bounds__(kScoreWarps * 32) fa_cache_scores(const SelectArgs p) {
+__global__ void __launch_bounds__(kScoreWarps * 32, kScoreCtas) fa_cache_scores(const SelectArgs p) {
     constexpr int kHalves = H == 128 ? 2 : 1, kBytes = H >= 64 ? 16 : H / 4, kWords = kBytes / 4, kSteps = kHalves * kWords;
     extern __shared__ __align__(16) uint4 s_frag[];   // [tiles][kSteps][positive, negative part][lane]
     __shared__ float s_qs[kScoreTiles][16];
@@ -124,38 +134,48 @@ __global__ void __launch_bounds__(kScoreWarps * 32) fa_cache_scores(const Select
         }
         __syncthreads();
 
+        // ---- 16 pages at a time: the table entries are asked for two turns ahead, the bounds one, when the registers of this turn's
+        // are free again
         const uint32_t stride = p.chunks * kScoreWarps * kScorePages;
-        for (uint32_t p0 = (chunk * kScoreWarps + warp) * kScorePages; p0 < n_pages; p0 += stride) {
-            // ---- bounds of pages p0 + g and p0 + 8 + g: whole numbers in fp16
-            uint32_t hi[2][kHalves][kWords][2], lo[2][kHalves][kWords][2];
-            uint4 raw[2][kHalves][2];
-            float scale[2];
+        int32_t entry[2];
+        float scale[2];
+        bool there[2];
+        uint4 raw[2][kHalves][2];
+        auto ask_pages = [&](uint32_t p0) {
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 const uint32_t mine = p0 + 8 * n + g;
-                int32_t page = mine < n_pages ? p.s.table[b * p.s.table_stride + mine] : -1;
+                entry[n] = mine < n_pages ? p.s.table[b * p.s.table_stride + mine] : -1;
+            }
+        };
+        auto ask_bounds = [&](uint32_t p0) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                int32_t page = entry[n];
                 if (static_cast<uint32_t>(page) >= p.c.n_pages) {
-                    if (mine < n_pages && t4 == 0 && turn == 0) cache_report(p.c.status, kCacheBadPage);
+                    if (p0 + 8 * n + g < n_pages && t4 == 0 && turn == 0) cache_report(p.c.status, kCacheBadPage);
                     page = -1;
                 }
                 // (a page that is not there: read the first, and never take it for its score)
                 const uint64_t at = static_cast<uint64_t>(page < 0 ? 0 : page) * p.c.heads + head;
-                scale[n] = page < 0 ? -1.0f : p.c.k_scale[at];
+                there[n] = page >= 0;
+                scale[n] = p.c.k_scale[at];   // (nothing may wait for it here)
                 const uint8_t* const from = p.c.bounds + at * (2 * H) + t4 * kBytes;
 #pragma unroll
                 for (int half = 0; half < kHalves; ++half)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        if constexpr (kBytes == 16) {
-                            raw[n][half][e] = *reinterpret_cast<const uint4*>(from + e * H + half * 64);
-                        } else if constexpr (kBytes == 8) {
-                            const uint2 x = *reinterpret_cast<const uint2*>(from + e * H);
-                            raw[n][half][e] = make_uint4(x.x, x.y, 0, 0);
-                        } else {
-                            raw[n][half][e] = make_uint4(*reinterpret_cast<const uint32_t*>(from + e * H), 0, 0, 0);
-                        }
-                    }
+                    for (int e = 0; e < 2; ++e) ld_bounds<kBytes>(from + e * H + half * 64, raw[n][half][e]);
             }
+        };
+        uint32_t p0 = (chunk * kScoreWarps + warp) * kScorePages;
+        if (p0 < n_pages) {
+            ask_pages(p0);
+            ask_bounds(p0);
+            ask_pages(p0 + stride);
+        }
+        for (; p0 < n_pages; p0 += stride) {
+            // ---- bounds of pages p0 + g and p0 + 8 + g: whole numbers in fp16
+            uint32_t hi[2][kHalves][kWords][2], lo[2][kHalves][kWords][2];
             const __half2 quarter = __float2half2_rn(0.25f), round = __float2half2_rn(1536.0f);   // (the unit of fp16 there is 1)
 #pragma unroll
             for (int n = 0; n < 2; ++n)
@@ -176,8 +196,13 @@ __global__ void __launch_bounds__(kScoreWarps * 32) fa_cache_scores(const Select
                         }
                     }
             // scales of the pages that this lane writes: page p0 + lane % 16
-            const float scale_lo = __shfl_sync(0xFFFFFFFFu, scale[0], (lane & 7u) * 4), scale_hi = __shfl_sync(0xFFFFFFFFu, scale[1], (lane & 7u) * 4);
+            const float scale_lo = __shfl_sync(0xFFFFFFFFu, there[0] ? scale[0] : -1.0f, (lane & 7u) * 4),
+                        scale_hi = __shfl_sync(0xFFFFFFFFu, there[1] ? scale[1] : -1.0f, (lane & 7u) * 4);
             const float my_scale = lane & 8u ? scale_hi : scale_lo;
+            if (p0 + stride < n_pages) {
+                ask_bounds(p0 + stride);
+                ask_pages(p0 + 2 * stride);
+            }
             const uint32_t my_page = p0 + (lane & 15u);
             float best = -INFINITY;   // (many)
             for (uint32_t tile = 0; tile < p.tiles; ++tile) {
@@ -293,7 +318,12 @@ __global__ void __launch_bounds__(kTakeThreads) fa_cache_take(const SelectArgs p
             for (uint32_t d = 0; d < 3; ++d) reach[d] += key >= (least | ((d + 1) << shift)) ? 1u : 0u;
         });
         count_three(reach, s_count, turn_no);
-        least |= (reach[2] >= p.keep ? 3u : reach[1] >= p.keep ? 2u : reach[0] >= p.keep ? 1u : 0u) << shift;
+        const uint32_t digit = reach[2] >= p.keep ? 3u : reach[1] >= p.keep ? 2u : reach[0] >= p.keep ? 1u : 0u;
+        least |= digit << shift;
+        if (digit != 0 && reach[digit - 1] == p.keep) {   // just as many as are wanted: all above the next lower value
+            --least;
+            break;
+        }
     }
     uint32_t above[3] = {0, 0, 0};   // keys above it, of the CTA; and of the thread, above and equal
     uint32_t mine_above = 0, mine_equal = 0;
