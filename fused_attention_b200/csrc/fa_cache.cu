@@ -312,15 +312,14 @@ int fa_b200_cache_select(const fa_b200_cache* cache, const fa_b200_sequences* se
     a.token_chunks = a.group > 16 ? a.s.T : (all_tiles + a.tiles - 1) / a.tiles;
     Device* d = nullptr;
     if ((rc = device_of(device, &d)) != FA_B200_OK) return rc;
-    // as many CTAs as are resident at once, each with 64 pages at least: what a CTA does before its first page is much of its time
-    const uint64_t problems = static_cast<uint64_t>(a.s.B) * a.c.heads * a.token_chunks, sms = static_cast<uint64_t>(d->sms.load());
-    const uint64_t most = (a.s.width + fa::kScoreWarps * fa::kScorePages - 1) / (fa::kScoreWarps * fa::kScorePages), wanted = problems < fa::kScoreCtas * sms ? fa::kScoreCtas * sms / problems : 1;
-    a.chunks = static_cast<uint32_t>(wanted < most ? wanted : most);
-    if (problems * a.chunks > kMostCtas) return FA_B200_ERR_SHAPE;
+    // as many CTAs as are resident at once, if there are as many units of 64 pages
+    const uint64_t problems = static_cast<uint64_t>(a.s.B) * a.c.heads * a.token_chunks, resident = static_cast<uint64_t>(fa::kScoreCtas) * d->sms.load();
+    const uint64_t units = problems * ((a.s.width + fa::kScoreWarps * fa::kScorePages - 1) / (fa::kScoreWarps * fa::kScorePages));
+    if (units > 0xFFFFFFFFull) return FA_B200_ERR_SHAPE;
     OnDevice on(device);
     if (on.rc != 0) return on.rc;
     const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-    const uint32_t grid = static_cast<uint32_t>(problems * a.chunks);
+    const uint32_t grid = static_cast<uint32_t>(units < resident ? units : resident);
     const size_t smem = static_cast<size_t>(a.tiles) * (cache->head_dim / 16) * 2 * 32 * sizeof(uint4);   // 32 KB at most
     constexpr uint32_t kBlock = fa::kScoreWarps * 32;
     switch (cache->head_dim) {

@@ -58,6 +58,79 @@ __device__ __forceinline__ uint32_t cache_count(const CacheSeqs& s, uint32_t b) 
     return n < 0 ? 0u : min(static_cast<uint32_t>(n), s.T);
 }
 
+// ----------------------------------------------------------------------------- work dealt out by the device
+// Sequences have units of work (below 2^32 in all), sequence b units(b) * per_seq; CTA c of C takes `each` from c * each +
+// min(c, more) on, the first `more` CTAs one more.  C is the grid, or fewer so that each has `least`.  Lengths are only known on the
+// device, so every CTA adds up the units itself.  s_share (8 + kWarps words): what share_owner needs to know.
+constexpr int kShareWords = 8;
+__device__ __forceinline__ uint32_t share_owner(const uint32_t* s_share, uint32_t unit) {
+    const uint32_t each = s_share[3], more = s_share[4], longer = more * (each + 1);
+    return unit < longer ? unit / (each + 1) : more + (unit - longer) / each;
+}
+// False: this CTA has none.  b: the sequence of its first unit; before: units in front of b.  `alike`: all sequences have as many.
+template <int kWarps, typename Units>
+__device__ __forceinline__ bool share_of(const Units& units, bool alike, uint32_t B, uint32_t per_seq, uint32_t least, uint32_t* s_share, uint32_t& unit,
+                                         uint32_t& unit_end, uint32_t& b, uint32_t& before) {
+    constexpr uint32_t kThreads = kWarps * 32;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    uint32_t* const s_sum = s_share + kShareWords;
+    // the units of all sequences; with up to kThreads of them every thread keeps what lies in front of its own
+    uint32_t total = 0, mine = 0, upto = 0;
+    if (alike) {
+        mine = units(0) * per_seq;
+        total = mine * B;
+    } else {
+        for (uint32_t i = tid; i < B; i += kThreads) mine += units(i);
+        mine *= per_seq;
+        upto = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+            if (lane >= d) upto += x;
+        }
+        if (lane == 31) s_sum[warp] = upto;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t w = 0; w < kWarps; ++w) {
+            if (w < warp) upto += s_sum[w];
+            total += s_sum[w];
+        }
+    }
+    const uint32_t ctas = min(gridDim.x, (total + least - 1) / least), each = total / ctas, more = total - each * ctas, c = blockIdx.x;
+    if (c >= ctas) return false;
+    if (tid == 0) s_share[3] = each, s_share[4] = more;
+    unit = c * each + min(c, more);
+    unit_end = (c + 1) * each + min(c + 1, more);
+    before = 0;
+    if (alike) {
+        b = unit / mine;
+        before = b * mine;
+    } else if (B <= kThreads) {
+        if (tid < B && unit < upto && unit >= upto - mine) s_share[0] = tid, s_share[1] = upto - mine;
+        __syncthreads();
+        b = s_share[0], before = s_share[1];
+    } else {
+        for (uint32_t b0 = 0; b0 < B; b0 += 32) {   // every warp adds up 32 sequences at a time
+            const uint32_t mine32 = b0 + lane < B ? units(b0 + lane) * per_seq : 0u;
+            uint32_t upto32 = mine32;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, upto32, d);
+                if (lane >= d) upto32 += x;
+            }
+            const uint32_t behind = __ballot_sync(0xFFFFFFFFu, before + upto32 > unit);
+            if (behind != 0) {
+                const uint32_t at = __ffs(behind) - 1;
+                b = b0 + at;
+                before += __shfl_sync(0xFFFFFFFFu, upto32 - mine32, at);
+                break;
+            }
+            before += __shfl_sync(0xFFFFFFFFu, upto32, 31);
+        }
+    }
+    return true;
+}
+
 // ----------------------------------------------------------------------------- e4m3 <-> fp16
 // Two codes (the lower 16 bits) -> two fp16 values; every e4m3 value is one of fp16.
 __device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t two) {

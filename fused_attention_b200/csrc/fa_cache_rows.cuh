@@ -59,16 +59,6 @@ struct RowsCfg {
     static constexpr int kCtas = MT == 1 ? 3 : 2;                  // per SM
 };
 
-// How the units of all problems (below 2^32) are dealt out: CTA c takes `each` from c * each + min(c, more) on, the first `more` CTAs
-// one more.
-struct RowsWork {
-    uint32_t ctas, each, more;
-};
-__device__ __forceinline__ uint32_t rows_begin(const RowsWork& w, uint32_t c) { return c * w.each + min(c, w.more); }
-__device__ __forceinline__ uint32_t rows_owner(const RowsWork& w, uint32_t unit) {
-    const uint32_t longer = w.more * (w.each + 1);
-    return unit < longer ? unit / (w.each + 1) : w.more + (unit - longer) / w.each;
-}
 __device__ __forceinline__ uint32_t rows_units(const RowsArgs& p, uint32_t b) {
     const uint32_t tokens = p.pages != nullptr ? p.keep << p.c.page_shift : cache_length(p.c, p.s, b);
     return max(1u, (tokens + kRowsUnit - 1) / kRowsUnit);
@@ -127,15 +117,14 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
     float* const s_coef = reinterpret_cast<float*>(q_frag + Cfg::kQ);
     uint32_t* const s_limit = reinterpret_cast<uint32_t*>(s_coef + Cfg::kRows);
     float2* const s_ml = reinterpret_cast<float2*>(s_limit + Cfg::kRows);
-    uint32_t* const s_sum = reinterpret_cast<uint32_t*>(s_ml + kRowsWarps * Cfg::kRows);
-    uint32_t* const s_first = s_sum + kRowsWarps;   // {first sequence, units in front of it}, {CTAs, units each, CTAs with one more}
+    uint32_t* const s_share = reinterpret_cast<uint32_t*>(s_ml + kRowsWarps * Cfg::kRows);
+    volatile uint32_t* const s_now = s_share + kShareWords + kRowsWarps;
     grid_dep_wait();
     grid_dep_launch();
     const bool bf16 = p.bf16 != 0;
     const uint32_t per_seq = p.c.heads * p.row_tiles;   // problems of a sequence
 
     // ---- this CTA's units
-    RowsWork work = {gridDim.x, 1, 0};
     uint32_t unit, unit_end, before = 0, b = 0;   // `before`: units of the sequences in front of b
     if (p.min_units == 0) {
         b = blockIdx.x / per_seq;
@@ -143,61 +132,8 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
         unit = (blockIdx.x - b * per_seq) * n;
         unit_end = unit + n;
     } else {
-        // the units of all sequences; with up to kThreads of them every thread keeps what lies in front of its own
-        uint32_t total = 0, mine = 0, upto = 0;
-        if (p.pages != nullptr) {
-            mine = rows_units(p, 0) * per_seq;
-            total = mine * p.s.B;
-        } else {
-            for (uint32_t i = tid; i < p.s.B; i += kThreads) mine += rows_units(p, i);
-            mine *= per_seq;
-            upto = mine;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, upto, d);
-                if (lane >= d) upto += x;
-            }
-            if (lane == 31) s_sum[warp] = upto;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < kRowsWarps; ++w) {
-                if (w < warp) upto += s_sum[w];
-                total += s_sum[w];
-            }
-        }
-        work.ctas = min(gridDim.x, (total + p.min_units - 1) / p.min_units);
-        if (blockIdx.x >= work.ctas) return;
-        work.each = total / work.ctas;
-        work.more = total - work.each * work.ctas;
-        if (tid == 0) s_first[2] = work.ctas, s_first[3] = work.each, s_first[4] = work.more;
-        unit = rows_begin(work, blockIdx.x);
-        unit_end = rows_begin(work, blockIdx.x + 1);
-        if (p.pages != nullptr) {
-            b = unit / mine;
-            before = b * mine;
-        } else if (p.s.B <= kThreads) {
-            if (tid < p.s.B && unit < upto && unit >= upto - mine) s_first[0] = tid, s_first[1] = upto - mine;
-            __syncthreads();
-            b = s_first[0], before = s_first[1];
-        } else {
-            for (uint32_t b0 = 0; b0 < p.s.B; b0 += 32) {   // every warp adds up 32 sequences at a time
-                const uint32_t mine32 = b0 + lane < p.s.B ? rows_units(p, b0 + lane) * per_seq : 0u;
-                uint32_t upto32 = mine32;
-#pragma unroll
-                for (int d = 1; d < 32; d <<= 1) {
-                    const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, upto32, d);
-                    if (lane >= d) upto32 += x;
-                }
-                const uint32_t behind = __ballot_sync(0xFFFFFFFFu, before + upto32 > unit);
-                if (behind != 0) {
-                    const uint32_t at = __ffs(behind) - 1;
-                    b = b0 + at;
-                    before += __shfl_sync(0xFFFFFFFFu, upto32 - mine32, at);
-                    break;
-                }
-                before += __shfl_sync(0xFFFFFFFFu, upto32, 31);
-            }
-        }
+        const bool alike = p.pages != nullptr;   // every sequence has as many
+        if (!share_of<kRowsWarps>([&](uint32_t i) { return rows_units(p, i); }, alike, p.s.B, per_seq, p.min_units, s_share, unit, unit_end, b, before)) return;
     }
 
     uint32_t slot = 2 * blockIdx.x;
@@ -223,8 +159,9 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
 
         // ---- the ring.  Lane l knows the pages of group l (16 tokens) of the warp's next 16 stages.
         const uint32_t n_stages = u1 - u0;
-        const int32_t* const list = p.pages != nullptr ? p.pages + ((static_cast<uint64_t>(b) * p.s.T + t_first) * p.c.heads + head) * p.keep : nullptr;
-        const int32_t* const table = p.s.table + b * p.s.table_stride;
+        // (what is needed once in 16 stages is kept in shared memory, not in registers)
+        if (tid == 0) s_now[0] = b, s_now[1] = (b * p.s.T + t_first) * p.c.heads + head, s_now[2] = u0;
+        __syncthreads();
         constexpr uint32_t kChunks = H / 16;                 // of a row; 32 lanes copy 32 / kChunks rows at a time
         constexpr uint32_t kRowsAtOnce = 32 / kChunks;
         const uint32_t copy_row = lane / kChunks, copy_chunk = lane % kChunks;
@@ -234,7 +171,9 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
         int32_t my_page = -1;
         uint32_t my_at = kNoToken;   // position of the group's first token
         auto look_up = [&](uint32_t stage) {
-            const uint32_t token = (u0 + stage + (lane >> 1)) * kRowsUnit + warp * kRowsStage + (lane & 1u) * 16;
+            const int32_t* const table = p.s.table + s_now[0] * p.s.table_stride;
+            const int32_t* const list = p.pages != nullptr ? p.pages + static_cast<uint64_t>(s_now[1]) * p.keep : nullptr;
+            const uint32_t token = (s_now[2] + stage + (lane >> 1)) * kRowsUnit + warp * kRowsStage + (lane & 1u) * 16;
             my_page = -1, my_at = kNoToken;
             if (stage + (lane >> 1) >= n_stages) return;
             uint32_t block = token >> p.c.page_shift;
@@ -590,7 +529,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
         }
         if (tid == 0 && u0 == 0 && p.min_units != 0) {   // who has a share of the problem, for fa_cache_join
             p.shares[static_cast<uint64_t>(b) * per_seq + problem] =
-                make_int2(alone ? -1 : static_cast<int>(2 * blockIdx.x + (first_segment ? 0 : 1)), static_cast<int>(rows_owner(RowsWork{s_first[2], s_first[3], s_first[4]}, before + problem * n_units + n_units - 1)));
+                make_int2(alone ? -1 : static_cast<int>(2 * blockIdx.x + (first_segment ? 0 : 1)), static_cast<int>(share_owner(s_share, before + problem * n_units + n_units - 1)));
         }
         unit += u1 - u0;
         if (unit == before + n_units * per_seq) before = unit, ++b;

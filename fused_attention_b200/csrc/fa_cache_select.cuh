@@ -28,13 +28,12 @@ struct SelectArgs {
     uint32_t per_tile;       // tokens whose heads share a tile of 16 rows (1 where they are more than 16)
     uint32_t tiles;          // tiles that a CTA holds
     uint32_t turns;          // groups of 16 * tiles heads of a token (1 but for more than 64 of them)
-    uint32_t token_chunks;   // CTAs that share the tokens
-    uint32_t chunks;         // CTAs that share the pages of a sequence and head
+    uint32_t token_chunks;   // of a CTA's tokens each
 };
 
 constexpr int kScoreWarps = 4;
 constexpr int kScorePages = 16;    // of a warp at a time: two n-tiles
-constexpr int kScoreCtas = 4;      // on an SM
+constexpr int kScoreCtas = 3;      // on an SM (four take registers that its pages are held in: 52 us against 45 with 32 long sequences)
 constexpr int kScoreTiles = 4;     // of 16 query rows that a CTA holds at most
 
 constexpr int kTakeThreads = 256;
@@ -61,33 +60,22 @@ __device__ __forceinline__ void ld_bounds(const uint8_t* from, uint4& w) {
     else asm volatile("ld.global.u32 %0, [%1];" : "=r"(w.x) : "l"(from));
 }
 
+// Scores of the pages [64 u0, 64 u1) of sequence b, for a head and the tokens of a chunk.  All threads of the CTA.
 template <int H>
-__global__ void __launch_bounds__(kScoreWarps * 32, kScoreCtas) fa_cache_scores(const SelectArgs p) {
+__device__ __forceinline__ void score_pages(const SelectArgs& p, uint32_t b, uint32_t head, uint32_t token_chunk, uint32_t u0, uint32_t u1, uint4* s_frag,
+                                            float (*s_qs)[16], float (*s_val)[16][kScorePages + 1]) {
     constexpr int kHalves = H == 128 ? 2 : 1, kBytes = H >= 64 ? 16 : H / 4, kWords = kBytes / 4, kSteps = kHalves * kWords;
-    extern __shared__ __align__(16) uint4 s_frag[];   // [tiles][kSteps][positive, negative part][lane]
-    __shared__ float s_qs[kScoreTiles][16];
-    __shared__ float s_val[kScoreWarps][16][kScorePages + 1];
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3u;
-    grid_dep_wait();
-    grid_dep_launch();
-    const bool bf16 = p.bf16 != 0;
-    uint32_t rest = blockIdx.x;
-    const uint32_t chunk = rest % p.chunks;
-    rest /= p.chunks;
-    const uint32_t head = rest % p.c.heads;
-    rest /= p.c.heads;
-    const uint32_t token_chunk = rest % p.token_chunks, b = rest / p.token_chunks;
+    const bool bf16 = p.bf16 != 0, many = p.group > 16;   // many: a token a CTA
     const uint32_t held = cache_length(p.c, p.s, b), count = cache_count(p.s, b);
-    if (threadIdx.x == 0 && chunk == 0 && head == 0 && token_chunk == 0 && !cache_length_ok(p.c, p.s, b)) cache_report(p.c.status, kCacheBadPosition);
-    const bool many = p.group > 16;   // heads of a token: a token a CTA
+    if (threadIdx.x == 0 && u0 == 0 && head == 0 && token_chunk == 0 && !cache_length_ok(p.c, p.s, b)) cache_report(p.c.status, kCacheBadPosition);
     const uint32_t t0 = many ? token_chunk : token_chunk * p.tiles * p.per_tile;
     if (held == 0 || t0 >= count) return;
-    const uint32_t n_pages = (held + p.c.page - 1) >> p.c.page_shift;
-    // what the CTA's last query sees bounds its pages
+    const uint32_t n_pages = min((held + p.c.page - 1) >> p.c.page_shift, u1 * (kScoreWarps * kScorePages));   // (pages in front of this are the call's)
     const uint32_t t_end = min(count, t0 + (many ? 1u : p.tiles * p.per_tile));
 
     for (uint32_t turn = 0; turn < p.turns; ++turn) {
-        if (turn > 0) __syncthreads();
+        __syncthreads();   // what was there has been read
         // ---- q8 into fragments, a warp a tile
         for (uint32_t tile = warp; tile < p.tiles; tile += kScoreWarps) {
             float most[2], raw[2][kHalves][kBytes];
@@ -136,7 +124,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32, kScoreCtas) fa_cache_scores(
 
         // ---- 16 pages at a time: the table entries are asked for two turns ahead, the bounds one, when the registers of this turn's
         // are free again
-        const uint32_t stride = p.chunks * kScoreWarps * kScorePages;
+        constexpr uint32_t stride = kScoreWarps * kScorePages;
         int32_t entry[2];
         float scale[2];
         bool there[2];
@@ -167,7 +155,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32, kScoreCtas) fa_cache_scores(
                     for (int e = 0; e < 2; ++e) ld_bounds<kBytes>(from + e * H + half * 64, raw[n][half][e]);
             }
         };
-        uint32_t p0 = (chunk * kScoreWarps + warp) * kScorePages;
+        uint32_t p0 = (u0 * kScoreWarps + warp) * kScorePages;
         if (p0 < n_pages) {
             ask_pages(p0);
             ask_bounds(p0);
@@ -253,6 +241,29 @@ __global__ void __launch_bounds__(kScoreWarps * 32, kScoreCtas) fa_cache_scores(
                 __syncwarp();
             }
         }
+    }
+}
+
+template <int H>
+__global__ void __launch_bounds__(kScoreWarps * 32, kScoreCtas) fa_cache_scores(const SelectArgs p) {
+    extern __shared__ __align__(16) uint4 s_frag[];   // [tiles][kSteps][positive, negative part][lane]
+    __shared__ float s_qs[kScoreTiles][16];
+    __shared__ float s_val[kScoreWarps][16][kScorePages + 1];
+    grid_dep_wait();
+    grid_dep_launch();
+    __shared__ uint32_t s_share[kShareWords + kScoreWarps];
+    const uint32_t per_seq = p.c.heads * p.token_chunks;
+    constexpr uint32_t kUnit = kScoreWarps * kScorePages;   // pages
+    auto units = [&](uint32_t i) { return max(1u, (cache_length(p.c, p.s, i) + kUnit * p.c.page - 1) / (kUnit * p.c.page)); };
+    uint32_t unit, unit_end, b, before;
+    if (!share_of<kScoreWarps>(units, false, p.s.B, per_seq, 1, s_share, unit, unit_end, b, before)) return;
+    while (unit < unit_end) {
+        const uint32_t n_units = units(b), problem = (unit - before) / n_units, u0 = unit - before - problem * n_units, u1 = min(n_units, u0 + (unit_end - unit));
+        unit += u1 - u0;
+        const uint32_t b_now = b, b_next = unit == before + n_units * per_seq ? b + 1 : b;
+        if (b_next != b) before = unit;
+        b = b_next;
+        score_pages<H>(p, b_now, problem % p.c.heads, problem / p.c.heads, u0, u1, s_frag, s_qs, s_val);
     }
 }
 
