@@ -174,7 +174,11 @@ int launch_rows(Device& d, uint32_t bit, const fa::RowsArgs& a, const RowsPlan& 
     using Cfg = fa::RowsCfg<H, MT>;
     int rc = allow_smem(d, bit, &fa::fa_cache_rows<H, MT>, Cfg::kSmem);
     if (rc == FA_B200_OK) rc = launch(&fa::fa_cache_rows<H, MT>, plan.grid, fa::kRowsWarps * 32, Cfg::kSmem, stream, a);
-    if (rc == FA_B200_OK && plan.min_units != 0) rc = launch(&fa::fa_cache_join<H, MT>, static_cast<uint32_t>(plan.problems * plan.rows), fa::kJoinWarps * 32, 0, stream, a);
+    if (rc != FA_B200_OK || plan.min_units == 0) return rc;
+    const uint64_t rows = plan.problems * plan.rows;
+    // a problem has about grid / problems parts, and one more
+    if (plan.grid < 8 * plan.problems) rc = launch(&fa::fa_cache_join_few<H, MT>, static_cast<uint32_t>((rows + fa::kJoinWarps - 1) / fa::kJoinWarps), fa::kJoinWarps * 32, 0, stream, a);
+    else rc = launch(&fa::fa_cache_join<H, MT>, static_cast<uint32_t>(rows), fa::kJoinWarps * 32, 0, stream, a);
     return rc;
 }
 template <int H>

@@ -616,4 +616,64 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fa_cache_join(const RowsArgs 
     }
 }
 
+// The same for problems of few parts: a warp per problem and row.
+template <int H, int MT>
+__global__ void __launch_bounds__(kJoinWarps * 32) fa_cache_join_few(const RowsArgs p) {
+    constexpr int kRows = 16 * MT;
+    constexpr int kWide = H >= 64 ? H / 32 : 2;   // dimensions of a lane
+    grid_dep_wait();
+    grid_dep_launch();
+    const uint32_t lane = threadIdx.x & 31u;
+    const uint64_t at = static_cast<uint64_t>(blockIdx.x) * kJoinWarps + (threadIdx.x >> 5);
+    const uint32_t per_seq = p.c.heads * p.row_tiles, r = static_cast<uint32_t>(at % p.rows);
+    const uint64_t index = at / p.rows;
+    if (index >= static_cast<uint64_t>(p.s.B) * per_seq) return;
+    const int2 share = p.shares[index];
+    if (share.x < 0) return;
+    const uint32_t b = static_cast<uint32_t>(index / per_seq), problem = static_cast<uint32_t>(index % per_seq);
+    const uint32_t head = problem / p.row_tiles, row = problem % p.row_tiles * p.rows + r;
+    if (row >= p.s.T * p.group) return;
+    const uint32_t first = static_cast<uint32_t>(share.x), last = 2 * static_cast<uint32_t>(share.y);
+    const uint32_t n = (last - (first & ~1u)) / 2 + 1;
+    auto slot = [&](uint32_t i) { return static_cast<uint64_t>(i == 0 ? first : (first & ~1u) + 2 * i) * kRows + r; };
+    float top = -INFINITY, sum = 0.0f, x[kWide];
+#pragma unroll
+    for (int d = 0; d < kWide; ++d) x[d] = 0.0f;
+    for (uint32_t i0 = 0; i0 < n; i0 += 32) {
+        const float2 ml = i0 + lane < n ? p.part_ml[slot(i0 + lane)] : make_float2(-INFINITY, 0.0f);
+        float now = fmaxf(top, ml.x);
+#pragma unroll
+        for (int d = 16; d >= 1; d >>= 1) now = fmaxf(now, __shfl_xor_sync(0xFFFFFFFFu, now, d));
+        const float f = ml.x == -INFINITY ? 0.0f : ex2_approx(ml.x - now);
+        const float again = top == now || top == -INFINITY ? 1.0f : ex2_approx(top - now);
+        sum = sum * again + ml.y * f;
+#pragma unroll
+        for (int d = 0; d < kWide; ++d) x[d] *= again;
+        top = now;
+        const uint32_t here = min(n - i0, 32u);
+#pragma unroll 4
+        for (uint32_t k = 0; k < here; ++k) {
+            const float fk = __shfl_sync(0xFFFFFFFFu, f, k);
+            if (lane * kWide < H) {
+                const float* const from = p.part_o + slot(i0 + k) * H + lane * kWide;
+                if constexpr (kWide == 4) {
+                    const float4 y = *reinterpret_cast<const float4*>(from);
+                    x[0] += y.x * fk, x[1] += y.y * fk, x[2] += y.z * fk, x[3] += y.w * fk;
+                } else {
+                    const float2 y = *reinterpret_cast<const float2*>(from);
+                    x[0] += y.x * fk, x[1] += y.y * fk;
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const uint32_t t = row / p.group, h = head * p.group + row % p.group;
+    uint8_t* const to = p.y + ((static_cast<uint64_t>(b) * p.s.T + t) * (p.c.heads * p.group) + h) * (2 * H);
+    if (lane * kWide < H)
+#pragma unroll
+        for (int d = 0; d < kWide; d += 2) *reinterpret_cast<uint32_t*>(to + 2 * (lane * kWide + d)) = pack_16(x[d] * f, x[d + 1] * f, p.bf16 != 0);
+}
+
 }  // namespace fa

@@ -105,3 +105,18 @@ def test_attention_rejections(lib):
     assert attention(lib, flags=1) == _lib.ERR_FLAGS
     for bad in (dict(heads=3), dict(heads=0), dict(pages=A), dict(keep=3), dict(pages=A, keep=1 << 28)):
         assert attention(lib, **bad) == _lib.ERR_SHAPE
+
+
+def test_python_refuses_what_is_not_on_a_gpu():
+    import torch
+
+    import fused_attention_b200 as fa
+    codes = torch.zeros(2, 1, 16, 64, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        fa.KVCache(codes, codes, torch.ones(2, 1), torch.ones(2, 1), torch.zeros(2, 1, 2, 64, dtype=torch.uint8).view(torch.float8_e4m3fn))
+    for bad in (dict(head_dim=48), dict(page_size=8), dict(n_pages=0), dict(kv_heads=0)):
+        with pytest.raises(RuntimeError, match="must be"):
+            fa.cache_create(**{**dict(head_dim=64, kv_heads=2, n_pages=8, page_size=16), **bad})
+    for f in (lambda: fa.cache_attention(None, None, None, None), lambda: fa.cache_select(None, None, None, None, 1), lambda: fa.cache_append(None, None, None, None, None)):
+        with pytest.raises(RuntimeError, match="KVCache"):
+            f()

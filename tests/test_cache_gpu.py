@@ -227,6 +227,43 @@ def test_strides_streams_and_graphs():
         assert torch.equal(out, fa.cache_attention(base, q.contiguous(), whole, lengths))
 
 
+def test_many_sequences_of_all_lengths():
+    """More sequences than a CTA has threads; empty ones, and some of a single token, among them."""
+    H, G, page, B = 32, 2, 32, 200
+    lens = torch.randint(0, 900, (B,), generator=gen_of(7), device="cuda").tolist()
+    lens[0], lens[1], lens[130], lens[199] = 0, 1, 0, 899
+    cache = random_cache(H, G, B * 29 + 3, page, 2)
+    table, lengths = table_of(lens, page, B * 29 + 3, 3)
+    q = queries_of(B, 1, G * 3 * H, torch.float16, 4)
+    y = check_attention(cache, q, table, lengths)
+    assert not y[0].any() and not y[130].any()
+    got = fa.cache_select(cache, q, table, lengths, 6)
+    assert torch.equal(got.cpu(), oracle.select(cache, q, table, lengths, 6))
+    check_attention(cache, q, table, lengths, pages=got)
+
+
+@pytest.mark.parametrize("H,dtype,causal", [(64, torch.float16, True), (128, torch.bfloat16, False), (32, torch.bfloat16, True)])
+def test_more_items_than_multiprocessors(H, dtype, causal):
+    """192 items of 256 query rows, the last 44 of them cut by keys; sequences without a token for the call between them."""
+    G, group, page, T = 8, 2, 64, 300
+    lens, counts = [300, 700, 512, 301, 900, 640, 300, 333], torch.tensor([300, 300, 0, 1, 129, 300, 257, 300], dtype=torch.int32, device="cuda")
+    cache = random_cache(H, G, 8 * 16, page, H)
+    table, lengths = table_of(lens, page, 8 * 16, 5)
+    q = queries_of(8, T, G * group * H, dtype, 6)
+    check_attention(cache, q, table, lengths, causal=causal)
+    y = check_attention(cache, q, table, lengths, counts=counts, causal=causal)
+    assert not y[2].any() and not y[3, 1:].any()
+
+
+def test_one_pair_of_query_tiles_and_a_row_more():
+    """Rows that end on a tile's edge, one in front of it and one behind it, and a tile that has hardly any."""
+    H, G, page = 64, 1, 16
+    cache = random_cache(H, G, 80, page, 9)
+    for T in (127, 128, 129, 255, 256, 257, 385):
+        table, lengths = table_of([T, 600], page, 80, T)
+        check_attention(cache, queries_of(2, T, H, torch.float16, T), table, lengths)
+
+
 def test_offsets_beyond_32_bits():
     """A page whose codes lie more than 2^32 bytes from the first, and one more than 2^31 tokens... of strides, not of memory read."""
     H, G, page = 128, 1, 128
@@ -257,7 +294,8 @@ def test_offsets_beyond_32_bits():
 @pytest.mark.parametrize("H,G,group,page,T,lengths,keep,first,last,dtype", [
     (128, 2, 4, 64, 1, [1, 64, 65, 5000], 4, 1, 1, torch.float16), (64, 3, 5, 16, 4, [4, 200, 1000], 9, 0, 2, torch.bfloat16),
     (32, 1, 17, 32, 2, [2, 900], 5, 2, 1, torch.float16), (16, 2, 1, 128, 3, [1500], 3, 1, 1, torch.bfloat16),
-    (128, 1, 40, 16, 1, [9000], 33, 1, 2, torch.bfloat16), (128, 1, 1, 16, 2, [40000], 64, 1, 3, torch.float16), (64, 1, 2, 16, 50, [50, 400], 7, 3, 9, torch.float16)])
+    (128, 1, 40, 16, 1, [9000], 33, 1, 2, torch.bfloat16), (128, 1, 1, 16, 2, [40000], 64, 1, 3, torch.float16), (64, 1, 2, 16, 50, [50, 400], 7, 3, 9, torch.float16),
+    (64, 1, 70, 16, 2, [900, 33], 5, 1, 1, torch.bfloat16), (128, 2, 3, 32, 40, [2000], 9, 1, 2, torch.bfloat16)])
 def test_select(H, G, group, page, T, lengths, keep, first, last, dtype):
     n = sum(-(-x // page) for x in lengths) + len(lengths) * (max(lengths) // page + 1)
     cache = random_cache(H, G, n, page, keep)
