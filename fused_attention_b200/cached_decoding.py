@@ -94,7 +94,7 @@ def main() -> int:
     counts = torch.randint(max(1, a.prompt // 2), a.prompt + 1, (a.batch,), generator=gen, device="cuda", dtype=torch.int32)
     prompts = torch.randint(0, len(model.embedding), (a.batch, a.prompt), generator=gen, device="cuda")
     begin, middle, end = (torch.cuda.Event(enable_timing=True) for _ in range(3))
-    model.forward(prompts[:, :1])   # (first calls)
+    model.forward(prompts, counts)   # (first calls)
     model.lengths.zero_()
     begin.record()
     logits = model.forward(prompts, counts)

@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
             ask(0);
             // ---- queries, several rows of a thread in flight
             if (k >= C::kQBuffers) mbar_wait(bar(C::QEMPTY + k % C::kQBuffers), (k / C::kQBuffers - 1u) & 1u, ctl, kCacheTimeout | C::QEMPTY);
-            constexpr uint32_t kQLanes = H / 8, kQRows = 128 / kQLanes, kQPasses = 2 * kPromptTile / kQRows, kFlight = kQPasses < 8 ? kQPasses : 8;
+            constexpr uint32_t kQLanes = H / 8, kQRows = 128 / kQLanes, kQPasses = 2 * kPromptTile / kQRows, kFlight = kQPasses < 4 ? kQPasses : 4;
             const uint32_t piece = lt % kQLanes;
 #pragma unroll 1
             for (uint32_t pass = 0; pass < kQPasses; pass += kFlight) {

@@ -24,6 +24,9 @@ namespace fa {
 constexpr int kRowsWarps = 4;
 constexpr int kRowsStage = 32;                       // tokens of a warp's stage
 constexpr int kRowsUnit = kRowsWarps * kRowsStage;   // tokens of a unit
+// What a problem costs a CTA beside its tokens (queries, the way to the first key, joining the warps), in units: counted when the
+// work is dealt out, so that a CTA with many short sequences gets fewer tokens.
+constexpr uint32_t kRowsSetup = 2;
 constexpr float kRowsSlack = 8.0f;                   // how far an exponent may pass M before M moves
 constexpr uint32_t kNoToken = 0x7FFFFFFFu;           // position of tokens that are not there
 
@@ -55,7 +58,7 @@ struct RowsCfg {
     static constexpr int kMerge = kRowsWarps * kRows * H * 4;
     static constexpr int kTiles = kRing > kMerge ? kRing : kMerge;
     static constexpr int kQ = kRows * H * 2;
-    static constexpr int kSmem = kTiles + kQ + kRows * 8 + kRowsWarps * kRows * 8 + 64;
+    static constexpr int kSmem = kTiles + kQ + kRows * 8 + kRowsWarps * kRows * 8 + 128;
     static constexpr int kCtas = MT == 1 ? 3 : 2;                  // per SM
 };
 
@@ -102,7 +105,9 @@ __device__ __forceinline__ void ld_codes(uint32_t addr, uint32_t (&w)[kBytes / 4
     }
 }
 
-template <int H, int MT>
+// kRest: what the weights lose when they are rounded to fp16 is multiplied too (for results in fp16, whose own rounding is no larger:
+// with it the error is that of the results' rounding alone, without it 1.4 times that).
+template <int H, int MT, bool kRest>
 __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cache_rows(const RowsArgs p) {
     using Cfg = RowsCfg<H, MT>;
     constexpr int kThreads = kRowsWarps * 32;
@@ -133,15 +138,17 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
         unit_end = unit + n;
     } else {
         const bool alike = p.pages != nullptr;   // every sequence has as many
-        if (!share_of<kRowsWarps>([&](uint32_t i) { return rows_units(p, i); }, alike, p.s.B, per_seq, p.min_units, s_share, unit, unit_end, b, before)) return;
+        if (!share_of<kRowsWarps>([&](uint32_t i) { return rows_units(p, i) + kRowsSetup; }, alike, p.s.B, per_seq, p.min_units, s_share, unit, unit_end, b, before)) return;
     }
 
-    uint32_t slot = 2 * blockIdx.x;
-    for (bool first_segment = true; unit < unit_end; first_segment = false) {
-        const uint32_t n_units = rows_units(p, b);
+    const uint32_t setup = p.min_units == 0 ? 0u : kRowsSetup;   // units in front of a problem's own
+    for (bool first_segment = true; unit < unit_end;) {
+        const uint32_t n_units = rows_units(p, b), all_units = n_units + setup;
         const uint32_t within = unit - before;
-        const uint32_t problem = within / n_units, u0 = within % n_units;
-        const uint32_t u1 = min(n_units, u0 + (unit_end - unit));
+        const uint32_t problem = within / all_units, w0 = within - problem * all_units, w1 = min(all_units, w0 + (unit_end - unit));
+        const uint32_t u0 = max(w0, setup) - setup, u1 = max(w1, setup) - setup;
+        unit += w1 - w0;
+        if (u1 == 0) continue;   // (the next CTA begins with the problem's first unit)
         const uint32_t head = problem / p.row_tiles, tile = problem % p.row_tiles;
         const uint32_t row0 = tile * p.rows;   // rows of the sequence and head: T * group
         const uint32_t n_rows = min(p.rows, p.s.T * p.group - row0);
@@ -160,7 +167,13 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
         // ---- the ring.  Lane l knows the pages of group l (16 tokens) of the warp's next 16 stages.
         const uint32_t n_stages = u1 - u0;
         // (what is needed once in 16 stages is kept in shared memory, not in registers)
-        if (tid == 0) s_now[0] = b, s_now[1] = (b * p.s.T + t_first) * p.c.heads + head, s_now[2] = u0;
+        if (tid == 0) {
+            s_now[0] = b, s_now[1] = (b * p.s.T + t_first) * p.c.heads + head, s_now[2] = u0;
+            // whether the problem is this CTA's alone, its last unit, the place of its sums; where the work goes on
+            const bool over = unit == before + all_units * per_seq;
+            s_now[3] = u0 == 0 && u1 == n_units, s_now[4] = before + (problem + 1) * all_units - 1, s_now[5] = 2 * blockIdx.x + (first_segment ? 0u : 1u);
+            s_now[6] = unit, s_now[7] = unit_end, s_now[8] = over ? unit : before, s_now[9] = over ? b + 1 : b, s_now[10] = problem;
+        }
         __syncthreads();
         constexpr uint32_t kChunks = H / 16;                 // of a row; 32 lanes copy 32 / kChunks rows at a time
         constexpr uint32_t kRowsAtOnce = 32 / kChunks;
@@ -365,7 +378,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
                     if (held_up != held_up) vinv[u] = held_up;
                 }
                 const bool whole = max(at[0], at[1]) < kNoToken && max(at[0], at[1]) + 16 <= nearest;
-                uint32_t pf[MT][4][2];
+                uint32_t pf[MT][4][2], rest[MT][4][2];
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     // exponents against M, a whole number, so that with scales that are powers of two nothing is rounded but the result
@@ -426,6 +439,11 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
                         }
                         pf[mt][n][0] = pack_half2(s[mt][n][0], s[mt][n][1]);
                         pf[mt][n][1] = pack_half2(s[mt][n][2], s[mt][n][3]);
+                        if (kRest) {
+                            const float2 x = unpack_half2(pf[mt][n][0]), y = unpack_half2(pf[mt][n][1]);
+                            rest[mt][n][0] = pack_half2(s[mt][n][0] - x.x, s[mt][n][1] - x.y);
+                            rest[mt][n][1] = pack_half2(s[mt][n][2] - y.x, s[mt][n][3] - y.y);
+                        }
                     }
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
@@ -462,6 +480,10 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
                             for (int mt = 0; mt < MT; ++mt) {
                                 const uint32_t a[4] = {pf[mt][2 * k16][0], pf[mt][2 * k16][1], pf[mt][2 * k16 + 1][0], pf[mt][2 * k16 + 1][1]};
                                 mma_m16n8k16(o[mt][4 * w + j], a, b0[j], b1[j]);
+                                if (kRest) {
+                                    const uint32_t r[4] = {rest[mt][2 * k16][0], rest[mt][2 * k16][1], rest[mt][2 * k16 + 1][0], rest[mt][2 * k16 + 1][1]};
+                                    mma_m16n8k16(o[mt][4 * w + j], r, b0[j], b1[j]);
+                                }
                             }
                     }
                 }
@@ -501,7 +523,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
                     }
             }
         __syncthreads();
-        const bool alone = u0 == 0 && u1 == n_units;
+        const bool alone = s_now[3] != 0;
         for (uint32_t i = tid; i < n_rows * (H / 2); i += kThreads) {
             const uint32_t r = i / (H / 2), d = 2 * (i % (H / 2));
             float top = -INFINITY, sum = 0.0f;
@@ -522,17 +544,16 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
                 uint8_t* const to = p.y + ((static_cast<uint64_t>(b) * p.s.T + t) * (p.c.heads * p.group) + h) * (2 * H) + 2 * d;
                 *reinterpret_cast<uint32_t*>(to) = pack_16(x.x * f, x.y * f, bf16);
             } else {
-                const uint32_t s_at = slot + (first_segment ? 0u : 1u);
+                const uint32_t s_at = s_now[5];
                 *reinterpret_cast<float2*>(p.part_o + (static_cast<uint64_t>(s_at) * Cfg::kRows + r) * H + d) = x;
                 if (d == 0) p.part_ml[static_cast<uint64_t>(s_at) * Cfg::kRows + r] = make_float2(top, sum);
             }
         }
-        if (tid == 0 && u0 == 0 && p.min_units != 0) {   // who has a share of the problem, for fa_cache_join
-            p.shares[static_cast<uint64_t>(b) * per_seq + problem] =
-                make_int2(alone ? -1 : static_cast<int>(2 * blockIdx.x + (first_segment ? 0 : 1)), static_cast<int>(share_owner(s_share, before + problem * n_units + n_units - 1)));
+        if (tid == 0 && s_now[2] == 0 && p.min_units != 0) {   // who has a share of the problem, for fa_cache_join
+            p.shares[static_cast<uint64_t>(b) * per_seq + s_now[10]] = make_int2(alone ? -1 : static_cast<int>(s_now[5]), static_cast<int>(share_owner(s_share, s_now[4])));
         }
-        unit += u1 - u0;
-        if (unit == before + n_units * per_seq) before = unit, ++b;
+        unit = s_now[6], unit_end = s_now[7], before = s_now[8], b = s_now[9];
+        first_segment = false;
         __syncthreads();   // the sums have been read: the ring, the rows' data and the fragments may be written again
     }
 }
