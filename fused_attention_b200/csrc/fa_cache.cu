@@ -16,7 +16,7 @@ constexpr int kMaxDevices = 64;
 // What is asked of a device once.
 struct Device {
     std::atomic<int> sms{0};   // 0: not asked yet
-    std::atomic<uint32_t> attr_done{0};   // bit per kernel instance whose shared-memory attribute is set
+    std::atomic<uint64_t> attr_done{0};   // bit per kernel instance whose shared-memory attribute is set
 };
 Device g_device[kMaxDevices];
 
@@ -71,10 +71,10 @@ int launch(void (*kernel)(KArgs...), uint32_t grid, uint32_t block, size_t smem,
 
 template <typename Kernel>
 int allow_smem(Device& d, uint32_t bit, Kernel* kernel, int bytes) {
-    if (d.attr_done.load(std::memory_order_acquire) & (1u << bit)) return FA_B200_OK;   // (setting it twice is harmless)
+    if (d.attr_done.load(std::memory_order_acquire) & (1ull << bit)) return FA_B200_OK;   // (setting it twice is harmless)
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return static_cast<int>(e);
-    d.attr_done.fetch_or(1u << bit, std::memory_order_release);
+    d.attr_done.fetch_or(1ull << bit, std::memory_order_release);
     return FA_B200_OK;
 }
 
@@ -231,8 +231,10 @@ PromptPlan plan_prompt(uint32_t H, uint32_t heads, uint32_t group, uint32_t page
 
 template <int H>
 int launch_prompt(Device& d, uint32_t bit, const fa::PromptArgs& a, const PromptPlan& plan, cudaStream_t stream) {
-    int rc = allow_smem(d, bit, &fa::fa_cache_prompt<H>, fa::PromptCfg<H>::kSmemBytes);
-    if (rc == FA_B200_OK) rc = launch(&fa::fa_cache_prompt<H>, plan.grid, fa::kPromptThreads, fa::PromptCfg<H>::kSmemBytes, stream, a);
+    const int same = a.c.page >= 64 ? 2 : a.c.page == 32 ? 1 : 0;
+    const auto kernel = same == 2 ? &fa::fa_cache_prompt<H, 4> : same == 1 ? &fa::fa_cache_prompt<H, 2> : &fa::fa_cache_prompt<H, 1>;
+    int rc = allow_smem(d, bit + same, kernel, fa::PromptCfg<H>::kSmemBytes);
+    if (rc == FA_B200_OK) rc = launch(kernel, plan.grid, fa::kPromptThreads, fa::PromptCfg<H>::kSmemBytes, stream, a);
     if (rc == FA_B200_OK && plan.parts > 1)
         rc = launch(&fa::fa_cache_prompt_join<H>, static_cast<uint32_t>((plan.items - plan.whole) / plan.parts * 2 * fa::kPromptTile / 4), 128, 0, stream, a);
     return rc;
@@ -398,10 +400,10 @@ int fa_b200_cache_attention(const fa_b200_cache* cache, const fa_b200_sequences*
         if (on.rc != 0) return on.rc;
         const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
         switch (H) {
-            case 16: return launch_prompt<16>(*d, 8, b, plan, stream);
-            case 32: return launch_prompt<32>(*d, 9, b, plan, stream);
-            case 64: return launch_prompt<64>(*d, 10, b, plan, stream);
-            default: return launch_prompt<128>(*d, 11, b, plan, stream);
+            case 16: return launch_prompt<16>(*d, 32, b, plan, stream);
+            case 32: return launch_prompt<32>(*d, 35, b, plan, stream);
+            case 64: return launch_prompt<64>(*d, 38, b, plan, stream);
+            default: return launch_prompt<128>(*d, 41, b, plan, stream);
         }
     }
     RowsPlan plan = plan_rows(H, a.c.heads, q_heads / a.c.heads, a.c.page, a.s.B, a.s.T, a.s.width, keep, static_cast<uint32_t>(d->sms.load()));

@@ -72,7 +72,12 @@ struct PromptCfg {
 struct __align__(16) PromptScales {
     float ks[kPromptGroups], vlog[kPromptGroups], vinv[kPromptGroups];
 };
-// Two groups' values.  Volatile: they are loaded where they are used, and not held in registers, of which a row's scores take most.
+// One, two groups' values.  Volatile: they are loaded where they are used, and not held in registers, of which a row's scores take most.
+__device__ __forceinline__ float one_group(uint32_t addr) {
+    float x;
+    asm volatile("ld.volatile.shared.f32 %0, [%1];" : "=f"(x) : "r"(addr));
+    return x;
+}
 __device__ __forceinline__ float2 two_groups(uint32_t addr) {
     float2 x;
     asm volatile("ld.volatile.shared.v2.f32 {%0, %1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(addr));
@@ -179,16 +184,24 @@ __device__ __forceinline__ void prompt_issue_pv(uint32_t tO, uint32_t tP, uint32
 // Weights of the groups kG0 and kG0 + 1 of a row, packed as fp16 pairs (8 words a group); adds the groups' sums to `l`, with the value
 // scale divided out.  The exponent is one multiply-add, score * cu + (vlog - ref): `ref` is a whole number, so that with scales
 // that are powers of two the bracket is exact.  `shrink`: see prompt_reference.
-template <int kG0>
+template <int kG0, int kSame>
 __device__ __forceinline__ void prompt_weights(const float (&s)[kPromptTile], uint32_t sc, float coef, float shrink, float ref, uint32_t (&pk)[16], float& l) {
-    const float2 ks = two_groups(sc + 4 * kG0), vlog = two_groups(sc + 4 * (kPromptGroups + kG0)), vinv = two_groups(sc + 4 * (2 * kPromptGroups + kG0));
+    constexpr int kAt = kSame == 4 ? kG0 & ~3 : kG0;
+    float2 ks, vlog, vinv;
+    if constexpr (kSame == 1) {
+        ks = two_groups(sc + 4 * kAt), vlog = two_groups(sc + 4 * (kPromptGroups + kAt)), vinv = two_groups(sc + 4 * (2 * kPromptGroups + kAt));
+    } else {
+        ks.x = one_group(sc + 4 * kAt), vlog.x = one_group(sc + 4 * (kPromptGroups + kAt)), vinv.x = one_group(sc + 4 * (2 * kPromptGroups + kAt));
+    }
+    uint64_t sum_a = 0, sum_b = 0, c2 = 0, a2 = 0;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
         const int u = kG0 + half;
-        // (at least 1e-37: a masked score, -inf, must stay that)
-        const float cu = fmaxf(coef * (half ? ks.y : ks.x), 1e-37f), add = fmaf(half ? vlog.y : vlog.x, shrink, -ref);
-        const uint64_t c2 = pack_f32x2(cu, cu), a2 = pack_f32x2(add, add);
-        uint64_t sum_a = 0, sum_b = 0;
+        if (half == 0 || kSame == 1) {
+            // (at least 1e-37: a masked score, -inf, must stay that)
+            const float cu = fmaxf(coef * (half ? ks.y : ks.x), 1e-37f), add = fmaf(half ? vlog.y : vlog.x, shrink, -ref);
+            c2 = pack_f32x2(cu, cu), a2 = pack_f32x2(add, add);
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             float x0, x1;
@@ -198,28 +211,34 @@ __device__ __forceinline__ void prompt_weights(const float (&s)[kPromptTile], ui
             else sum_a = add_f32x2(sum_a, pack_f32x2(w0, w1));
             pk[half * 8 + e] = pack_half2(w0, w1);
         }
-        float lo, hi;
-        unpack_f32x2(add_f32x2(sum_a, sum_b), lo, hi);
-        l = fmaf(lo + hi, half ? vinv.y : vinv.x, l);
+        if (half == 1 || kSame == 1) {
+            float lo, hi;
+            unpack_f32x2(add_f32x2(sum_a, sum_b), lo, hi);
+            l = fmaf(lo + hi, half && kSame == 1 ? vinv.y : vinv.x, l);
+            sum_a = sum_b = 0;
+        }
     }
 }
+// Largest of 16 scores.
+__device__ __forceinline__ float largest_of_16(const float* x) {
+    float a = max3(x[0], x[1], x[2]), b = max3(x[3], x[4], x[5]);
+#pragma unroll
+    for (int e = 6; e < 14; e += 4) {
+        a = max3(a, x[e], x[e + 1]);
+        b = max3(b, x[e + 2], x[e + 3]);
+    }
+    return max3(a, b, fmaxf(x[14], x[15]));
+}
 // Largest exponent of a row.
+template <int kSame>
 __device__ __forceinline__ float prompt_top(const float (&s)[kPromptTile], uint32_t sc, float coef, float shrink) {
     float top = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < kPromptGroups; u += 2) {
-        const float2 ks = two_groups(sc + 4 * u), vlog = two_groups(sc + 4 * (kPromptGroups + u));
+    for (int u = 0; u < kPromptGroups; u += kSame) {
+        float most = largest_of_16(s + u * 16);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const float* x = s + (u + half) * 16;
-            float a = max3(x[0], x[1], x[2]), b = max3(x[3], x[4], x[5]);
-#pragma unroll
-            for (int e = 6; e < 14; e += 4) {
-                a = max3(a, x[e], x[e + 1]);
-                b = max3(b, x[e + 2], x[e + 3]);
-            }
-            top = fmaxf(top, fmaf(max3(a, b, fmaxf(x[14], x[15])), fmaxf(coef * (half ? ks.y : ks.x), 1e-37f), (half ? vlog.y : vlog.x) * shrink));
-        }
+        for (int v = 1; v < kSame; ++v) most = fmaxf(most, largest_of_16(s + (u + v) * 16));
+        top = fmaxf(top, fmaf(most, fmaxf(coef * one_group(sc + 4 * u), 1e-37f), one_group(sc + 4 * (kPromptGroups + u)) * shrink));
     }
     return top;
 }
@@ -238,7 +257,10 @@ __device__ __forceinline__ float prompt_reference(float top, float& m, float& co
     return alpha;
 }
 
-template <int H>
+// kSame: how many groups in a row have one scale (a page's: 4 at 64 tokens and more, 2 at 32, 1 at 16).  The softmax reads and
+// combines the scales once for so many: with pages of 64 tokens 391 us against 408 (a prompt of 2048 tokens on 16384, 32 heads of
+// 128), 150 against 157 (16 prompts of 777, heads of 64).
+template <int H, int kSame>
 __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const PromptArgs p) {
     using C = PromptCfg<H>;
     constexpr uint32_t NS = C::kSlots, kGroups = kPromptGroups;
@@ -339,7 +361,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
                 }
                 // The reference moves when an exponent exceeds it by more than 8 (weights stay below 2^9); a row that has seen nothing
                 // yet takes the first that it sees.
-                const float top = prompt_top(s, sc, coef, shrink);
+                const float top = prompt_top<kSame>(s, sc, coef, shrink);
                 float alpha = 1.0f;
                 if (__any_sync(0xFFFFFFFFu, top > m + kRowsSlack)) {
                     if (top > m + kRowsSlack) alpha = prompt_reference(top, m, coef, shrink);
@@ -348,18 +370,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
                 const float ref = m == -INFINITY ? 0.0f : m;
                 // the first quarter's weights are kept in registers: the last step's P V may still be reading P
                 uint32_t pk[16];
-                prompt_weights<0>(s, sc, coef, shrink, ref, pk, l);
+                prompt_weights<0, kSame>(s, sc, coef, shrink, ref, pk, l);
                 if (g > 0) {
                     mbar_wait(bar(C::PV0 + i), (g - 1u) & 1u, ctl, kCacheTimeout | (C::PV0 + i));
                     tc_fence_after();
                 }
                 __syncwarp();
                 tmem_st16(tP, pk);
-                prompt_weights<2>(s, sc, coef, shrink, ref, pk, l);
+                prompt_weights<2, kSame>(s, sc, coef, shrink, ref, pk, l);
                 tmem_st16(tP + 16, pk);
-                prompt_weights<4>(s, sc, coef, shrink, ref, pk, l);
+                prompt_weights<4, kSame>(s, sc, coef, shrink, ref, pk, l);
                 tmem_st16(tP + 32, pk);
-                prompt_weights<6>(s, sc, coef, shrink, ref, pk, l);
+                prompt_weights<6, kSame>(s, sc, coef, shrink, ref, pk, l);
                 tmem_st16(tP + 48, pk);
                 if (j > 0 && __any_sync(0xFFFFFFFFu, alpha != 1.0f)) {   // (an item's first P V overwrites O)
                     // here, where the scores' registers are free; the last step's P V has retired, and the next waits for P
