@@ -144,6 +144,9 @@ struct RowsPlan {
 
 RowsPlan plan_rows(uint32_t H, uint32_t heads, uint32_t group, uint32_t page, uint32_t B, uint32_t T, uint32_t width, uint32_t keep, uint32_t sms) {
     RowsPlan r = {};
+    // One m-tile or two.  With more than 16 rows the second reads the keys once for 32 of them (32 rows on 16 sequences of 2000 tokens:
+    // 36 us, 39 with one, which takes the keys twice; 64 rows on 64 of 4000: 305 and 360); with 16 or fewer it is work for nothing
+    // (64 sequences of 4000 tokens: 96 us with one, 148 with two).
     if (keep != 0) {   // a problem has rows of one token
         r.rows = group;
         if (group > 32)
@@ -163,8 +166,10 @@ RowsPlan plan_rows(uint32_t H, uint32_t heads, uint32_t group, uint32_t page, ui
     // What the rounding of the weights takes away is multiplied too where results are fp16 and a CTA has few units (64 sequences of up
     // to 8192 tokens, 75 units a CTA: 97 us without, 111 with; one of 301 tokens: 9.6 and 9.8).
     r.rest = all_units <= 8 * ctas;
-    // Problems of up to 512 tokens are not divided: joining costs more than what is left of them takes.
-    r.min_units = r.units <= 4 ? 0 : 2;
+    // Problems of up to 512 tokens are not divided, those of up to 1024 where there is one for every CTA: joining costs more than what
+    // is left of them takes.  (Tables of 512 tokens: 1 sequence of 8 heads 9.7 us, divided 10.5, 16 sequences 10.3 and 14.3; of 1024:
+    // 1 sequence 14.7 and 10.4, 32 sequences of any lengths 21.5 and 19.1, 64 27.6 and 29.1, 256 74 and 84; of 2048: 64 41.5 and 41.1.)
+    r.min_units = r.units <= 4 || (r.units <= 8 && r.problems >= ctas) ? 0 : 2;
     r.grid = static_cast<uint32_t>(r.min_units == 0 ? r.problems : ctas < all_units ? ctas : all_units);
     const uint64_t slots = r.min_units == 0 ? 0 : 2ull * r.grid * 16 * r.mt;
     r.o_bytes = slots * H * 4;
@@ -181,7 +186,9 @@ int launch_rows(Device& d, uint32_t bit, const fa::RowsArgs& a, const RowsPlan& 
     if (rc == FA_B200_OK) rc = launch(kernel, plan.grid, fa::kRowsWarps * 32, Cfg::kSmem, stream, a);
     if (rc != FA_B200_OK || plan.min_units == 0) return rc;
     const uint64_t rows = plan.problems * plan.rows;
-    // a problem has about grid / problems parts, and one more
+    // a problem has about grid / problems parts, and one more.  A warp a row, or a CTA a row where there are eight or more: 55 parts 32.4
+    // us with a warp and 22.6 with a CTA (the whole call, 1 sequence of 32768 tokens), 14 parts 56.3 and 54.4, 7 parts 94.0 and 93.1, 3.5
+    // parts 33.6 and 34.8 (16 of 4096).
     if (plan.grid < 8 * plan.problems) rc = launch(&fa::fa_cache_join_few<H, MT>, static_cast<uint32_t>((rows + fa::kJoinWarps - 1) / fa::kJoinWarps), fa::kJoinWarps * 32, 0, stream, a);
     else rc = launch(&fa::fa_cache_join<H, MT>, static_cast<uint32_t>(rows), fa::kJoinWarps * 32, 0, stream, a);
     return rc;
@@ -199,7 +206,10 @@ struct PromptPlan {
     uint64_t scratch() const { return 16 + o_bytes + ml_bytes; }   // (never none: there is an address then)
 };
 
-bool use_prompt(uint32_t group, uint32_t T, uint32_t keep) { return keep == 0 && static_cast<uint64_t>(T) * group >= 128; }
+// Rows from which the tensor tiles of fa_cache_prompt.cuh pay, although they are 256 rows high: us by fa_cache_rows.cuh and by it with
+// 32, 64, 96, 128 rows: 1 sequence of 16384 tokens 25 and 34, 34 and 36, 43 and 38, 50 and 40; 64 of 3000 tokens 130 and 223, 243 and
+// 227, 357 and 233, 467 and 238; 16 of 1300 tokens with 16 heads of 64 30 and 49, 48 and 49, 67 and 51, 84 and 52.
+bool use_prompt(uint32_t group, uint32_t T, uint32_t keep) { return keep == 0 && static_cast<uint64_t>(T) * group >= 64; }
 // The kernel for many rows knows a page's place as a 32-bit number of 16 bytes.
 bool prompt_reaches(const fa::CacheView& c) {
     const auto end = [&](int64_t page, int64_t token) { return static_cast<uint64_t>(c.n_pages) * page + static_cast<uint64_t>(c.page) * token; };
@@ -282,7 +292,10 @@ int fa_b200_cache_append(const fa_b200_cache* cache, const fa_b200_sequences* se
     const uint64_t q_ctas = (q_threads + fa::kAppendThreads - 1) / fa::kAppendThreads;
     if (tasks + q_ctas > kMostCtas || q_threads > 0xFFFFFF00ull) return FA_B200_ERR_SHAPE;
     a.tasks = static_cast<uint32_t>(tasks), a.query_ctas = static_cast<uint32_t>(q_ctas);
-    const bool warp_tasks = a.s.T <= 4;
+    // A warp a task, not a CTA of four: where a task has few tokens, or the tasks fill the device many times over in either form.  (Pages
+    // of 64 tokens, 8 heads of 128, us as CTAs and as warps: 32 sequences of 4 tokens 5.3 and 4.5, of 16 6.2 and 8.0; 128 of 16 16.6 and
+    // 11.4; 64 of 32 13.4 and 15.7; 128 of 32 28 and 24; 32 of 512 82 and 85; 64 of 512 164 and 158; 4 of 4096 82 and 94.)
+    const bool warp_tasks = a.s.T <= 4 || tasks >= 128ull * (a.s.T < a.c.page ? a.s.T : a.c.page);
     const uint32_t task_ctas = static_cast<uint32_t>(warp_tasks ? (tasks + 3) / 4 : tasks);
     Device* d = nullptr;
     if ((rc = device_of(device, &d)) != FA_B200_OK) return rc;
@@ -341,6 +354,8 @@ int fa_b200_cache_select(const fa_b200_cache* cache, const fa_b200_sequences* se
     }
     if (rc != FA_B200_OK) return rc;
     const uint32_t per = (a.s.width + fa::kTakeThreads - 1) / fa::kTakeThreads;
+    // As many keys of a thread in registers as there are at most (1 query on 2048 pages: 12 us so, 15.4 out of memory, 15.7 with 32; on
+    // 469 pages 9.2, 11.0 out of memory, 10.7 with 8, 14.4 with 32).
     if (per <= 2) return launch(&fa::fa_cache_take<2>, static_cast<uint32_t>(rows), fa::kTakeThreads, 0, stream, a);
     if (per <= 8) return launch(&fa::fa_cache_take<8>, static_cast<uint32_t>(rows), fa::kTakeThreads, 0, stream, a);
     if (per <= 32) return launch(&fa::fa_cache_take<32>, static_cast<uint32_t>(rows), fa::kTakeThreads, 0, stream, a);
