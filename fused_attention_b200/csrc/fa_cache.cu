@@ -354,8 +354,8 @@ int fa_b200_cache_select(const fa_b200_cache* cache, const fa_b200_sequences* se
     }
     if (rc != FA_B200_OK) return rc;
     const uint32_t per = (a.s.width + fa::kTakeThreads - 1) / fa::kTakeThreads;
-    // As many keys of a thread in registers as there are at most (1 query on 2048 pages: 12 us so, 15.4 out of memory, 15.7 with 32; on
-    // 469 pages 9.2, 11.0 out of memory, 10.7 with 8, 14.4 with 32).
+    // As many keys of a thread in registers as there are at most (32 queries on 2048 pages: 47.8 us so, 52.9 out of memory, 49.2 with 32;
+    // on 313 17.3, 19.9 out of memory, 18.2 with 8, 20.5 with 32; on 8192 147, 244 out of memory).
     if (per <= 2) return launch(&fa::fa_cache_take<2>, static_cast<uint32_t>(rows), fa::kTakeThreads, 0, stream, a);
     if (per <= 8) return launch(&fa::fa_cache_take<8>, static_cast<uint32_t>(rows), fa::kTakeThreads, 0, stream, a);
     if (per <= 32) return launch(&fa::fa_cache_take<32>, static_cast<uint32_t>(rows), fa::kTakeThreads, 0, stream, a);

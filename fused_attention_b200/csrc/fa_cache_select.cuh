@@ -8,9 +8,12 @@
 // where q8 <= 0, so the sum is two matrix products, of the positive part of q8 with hi8 and of the negative part with lo8:
 // mma.sync m16n8k16 on fp16, which holds these numbers exactly.
 //
-// fa_cache_scores reads 2 H + 4 bytes a page and head and is bound by that; a warp takes eight pages, and for several tokens a
-// sequence keeps their bounds in registers for all of them.  fa_cache_take then finds the `keep` highest of a query's scores: the
-// threshold by a search over the bits of the sortable form of the scores, held in registers, then the pages in order.
+// fa_cache_scores reads 2 H + 4 bytes a page and head: 84 MB in 32 us with 32 sequences of 30000 to 131072 tokens, 2.6 TB/s.  Reading
+// alone is not what bounds it: each value of the bounds is unpacked, rounded to 8 bits and packed again (about two instructions a
+// value), with three CTAs an SM, as many as its registers allow, to hide the way to memory.  The pages of all sequences are dealt
+// out to the CTAs in equal shares; a warp takes 16 pages at a time, whose bounds it asks for a turn ahead, and multiplies them by
+// all of the sequence's queries, which are rounded once a CTA; queries of several tokens share tiles of 16 rows.
+// fa_cache_take then finds the `keep` highest of a query's scores.
 #pragma once
 
 #include "fa_cache.cuh"
@@ -37,6 +40,9 @@ constexpr int kScoreCtas = 3;      // on an SM (four take registers that its pag
 constexpr int kScoreTiles = 4;     // of 16 query rows that a CTA holds at most
 
 constexpr int kTakeThreads = 256;
+constexpr int kTakeBinBits = 9;      // (32 queries on 20001 tokens, the whole call: 8 bits 17.3 us, 9 17.4, 10 18.3, 11 22.2; on 60000 in pages of 16: 76.1, 74.9, 76.0, 77.3)
+constexpr uint32_t kTakeBins = 1u << kTakeBinBits;
+constexpr uint32_t kTakeAlways = 0xFF800000u;   // score of a page that is taken whatever its bounds: infinity (NaN is above it)
 
 // Whole numbers of the same order as the floats (a NaN above all).
 __device__ __forceinline__ uint32_t sortable(float x) {
@@ -267,31 +273,32 @@ __global__ void __launch_bounds__(kScoreWarps * 32, kScoreCtas) fa_cache_scores(
     }
 }
 
-// The CTA's sum of three counts, to all threads.
-__device__ __forceinline__ void count_three(uint32_t (&n)[3], uint32_t (*s)[3], uint32_t& turn) {
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+// Sum over the lanes of this one and those in front of it.
+__device__ __forceinline__ uint32_t sum_upto(uint32_t x, uint32_t lane) {
 #pragma unroll
-    for (int i = 0; i < 3; ++i) n[i] = __reduce_add_sync(0xFFFFFFFFu, n[i]);
-    uint32_t (*const at)[3] = s + (turn & 1u) * (kTakeThreads / 32);   // (two buffers: one barrier a sum)
-    ++turn;
-    if (lane == 0)
-#pragma unroll
-        for (int i = 0; i < 3; ++i) at[warp][i] = n[i];
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        n[i] = 0;
-#pragma unroll
-        for (int w = 0; w < kTakeThreads / 32; ++w) n[i] += at[w][i];
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, x, d);
+        if (lane >= static_cast<uint32_t>(d)) x += y;
     }
+    return x;
 }
 
+// The `keep` highest keys of a query, the lowest pages of equal ones, in the order of the pages.  Their threshold is found by counting:
+// the keys' range, lowest to highest, is cut into kTakeBins equal bins, the keys of each are counted, and the bin that the threshold
+// lies in is the next range, unless all of its keys are wanted or it has one value.  The range is 32 bits, so four counts are enough
+// for any keys; spread as scores are, one or two are needed.  Bound by the way through its barriers: 3 us of the 8.1 that one query on
+// 313 pages takes.  A search over the threshold's bits, up to 16 counts, took 4 (the whole call with 32 queries on 20001 tokens: 17.4
+// us and 21.8, on 131072: 47.7 and 51.8).
 // kHeld: keys of a thread in registers (0: any number, from memory each time).
 template <int kHeld>
 __global__ void __launch_bounds__(kTakeThreads) fa_cache_take(const SelectArgs p) {
-    __shared__ uint32_t s_count[2 * (kTakeThreads / 32)][3];
-    __shared__ uint32_t s_scan[kTakeThreads / 32][2];
+    constexpr uint32_t kWarps = kTakeThreads / 32, kBinsEach = kTakeBins / kTakeThreads;
+    __shared__ uint32_t s_bins[kTakeBins];
+    __shared__ uint32_t s_low[kWarps], s_high[kWarps], s_sum[kWarps];
+    __shared__ uint32_t s_scan[kWarps][2], s_found[3];
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+#pragma unroll
+    for (uint32_t i = 0; i < kBinsEach; ++i) s_bins[i * kTakeThreads + tid] = 0;
     grid_dep_wait();
     grid_dep_launch();
     const uint64_t index = blockIdx.x;   // (b, t, head)
@@ -310,53 +317,81 @@ __global__ void __launch_bounds__(kTakeThreads) fa_cache_take(const SelectArgs p
     uint32_t mine[kHeld > 0 ? kHeld : 1];
     if (kHeld > 0) {
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) mine[i] = begin + i < end ? keys[begin + i] : 0u;   // 0: below every key of a page that is seen
+        for (int i = 0; i < kHeld; ++i) mine[i] = begin + i < end ? keys[begin + i] : 0u;
     }
     auto each = [&](auto&& f) {
         if (kHeld > 0) {
 #pragma unroll
-            for (int i = 0; i < kHeld; ++i) f(begin + i, mine[i]);
+            for (int i = 0; i < kHeld; ++i)
+                if (begin + i < end) f(begin + i, mine[i]);
         } else {
             for (uint32_t i = begin; i < end; ++i) f(i, keys[i]);
         }
     };
-    // the largest value that at least `keep` keys reach, two bits at a time
-    uint32_t least = 0, turn_no = 0;
-    for (int shift = 30; shift >= 0; shift -= 2) {
-        uint32_t reach[3] = {0, 0, 0};
-        each([&](uint32_t, uint32_t key) {
+    // The range, without the pages that are always taken, or of those alone where there are more of them than are wanted.
+    uint32_t low = kTakeAlways, high = 0, always = 0;
+    each([&](uint32_t, uint32_t key) {
+        if (key >= kTakeAlways) ++always;
+        else low = min(low, key), high = max(high, key);
+    });
+    low = __reduce_min_sync(0xFFFFFFFFu, low), high = __reduce_max_sync(0xFFFFFFFFu, high), always = __reduce_add_sync(0xFFFFFFFFu, always);
+    if (lane == 0) s_low[warp] = low, s_high[warp] = high, s_sum[warp] = always;
+    __syncthreads();
+    always = 0;
 #pragma unroll
-            for (uint32_t d = 0; d < 3; ++d) reach[d] += key >= (least | ((d + 1) << shift)) ? 1u : 0u;
+    for (uint32_t w = 0; w < kWarps; ++w) low = min(low, s_low[w]), high = max(high, s_high[w]), always += s_sum[w];
+    uint32_t want = p.keep - always, range = high - low;   // of the keys in [low, low + range], which are more than that
+    if (always >= p.keep) want = p.keep, low = kTakeAlways, range = ~kTakeAlways;
+    uint32_t least, ties;   // taken: the keys above `least`, and the first `ties` that are equal to it
+    for (;;) {
+        const uint32_t shift = max(32 - __clz(range), kTakeBinBits) - kTakeBinBits;   // range >> shift < kTakeBins
+        each([&](uint32_t, uint32_t key) {
+            if (key >= low && key - low <= range) atomicAdd(&s_bins[(key - low) >> shift], 1u);
         });
-        count_three(reach, s_count, turn_no);
-        const uint32_t digit = reach[2] >= p.keep ? 3u : reach[1] >= p.keep ? 2u : reach[0] >= p.keep ? 1u : 0u;
-        least |= digit << shift;
-        if (digit != 0 && reach[digit - 1] == p.keep) {   // just as many as are wanted: all above the next lower value
-            --least;
+        __syncthreads();
+        // keys from the highest bin on: thread 0 has the highest bins
+        uint32_t count[kBinsEach], sum = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kBinsEach; ++i) {
+            uint32_t& bin = s_bins[kTakeBins - 1 - (tid * kBinsEach + i)];
+            sum += count[i] = bin;
+            bin = 0;
+        }
+        const uint32_t upto = sum_upto(sum, lane);
+        if (lane == 31) s_sum[warp] = upto;
+        __syncthreads();
+        uint32_t front = upto - sum;
+#pragma unroll
+        for (uint32_t w = 0; w < kWarps; ++w) front += w < warp ? s_sum[w] : 0u;
+        if (front < want && want <= front + sum) {   // one thread's
+#pragma unroll
+            for (uint32_t i = 0; i < kBinsEach; ++i) {
+                if (front < want && want <= front + count[i])
+                    s_found[0] = kTakeBins - 1 - (tid * kBinsEach + i), s_found[1] = want - front, s_found[2] = count[i];
+                front += count[i];
+            }
+        }
+        __syncthreads();
+        low += s_found[0] << shift, want = s_found[1];
+        if (want == s_found[2]) {   // the whole bin (it is not the one with the lowest key, n > keep, so that `low` is not 0)
+            least = low - 1, ties = 0;
             break;
         }
+        if (shift == 0) {
+            least = low, ties = want;
+            break;
+        }
+        range = (1u << shift) - 1u;
     }
-    uint32_t above[3] = {0, 0, 0};   // keys above it, of the CTA; and of the thread, above and equal
+    // how many that are above, equal the threads in front have
     uint32_t mine_above = 0, mine_equal = 0;
-    each([&](uint32_t i, uint32_t key) {
-        if (i < end) mine_above += key > least ? 1u : 0u, mine_equal += key == least ? 1u : 0u;
-    });
-    above[0] = mine_above;
-    count_three(above, s_count, turn_no);
-    const uint32_t ties = p.keep - above[0];   // of the equal ones, the first so many
-    // how many of either the threads in front have
-    uint32_t upto_above = mine_above, upto_equal = mine_equal;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, upto_above, d), y = __shfl_up_sync(0xFFFFFFFFu, upto_equal, d);
-        if (lane >= d) upto_above += x, upto_equal += y;
-    }
+    each([&](uint32_t, uint32_t key) { mine_above += key > least ? 1u : 0u, mine_equal += key == least ? 1u : 0u; });
+    const uint32_t upto_above = sum_upto(mine_above, lane), upto_equal = sum_upto(mine_equal, lane);
     if (lane == 31) s_scan[warp][0] = upto_above, s_scan[warp][1] = upto_equal;
     __syncthreads();
     uint32_t front_above = upto_above - mine_above, front_equal = upto_equal - mine_equal;
     for (uint32_t w = 0; w < warp; ++w) front_above += s_scan[w][0], front_equal += s_scan[w][1];
     each([&](uint32_t i, uint32_t key) {
-        if (i >= end) return;
         if (key > least) {
             out[front_above + min(front_equal, ties)] = static_cast<int32_t>(i);
             ++front_above;
