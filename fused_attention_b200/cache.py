@@ -43,7 +43,7 @@ def _require(cond: bool, what: str) -> None:
 def _calls():
     """(append, select, attention, entries).  A native call answers None for what is not a plain call with every precondition met,
     which then goes through the checks and ctypes below; an int is the status of a launch that failed.  (One token of a short
-    sequence: attention 5.6 us a call, 18.8 through ctypes.)"""
+    sequence: attention 14.6 us a call and 18.8 through ctypes, with the same kernel.)"""
     global _native
     if _native is None:
         lib = _lib.load()   # raises when the CUDA library is missing: no fallback

@@ -19,7 +19,9 @@
 //
 // Bound by the tensor pipe and the exponentials as fa_fwd_pipelined is (per step and tile 1024 tensor clocks of products at
 // H = 128 and 1024 clocks of exponentials); what is added here is shared-memory traffic, 64 KB a step written by the loading
-// warps beside the 192 KB that the products read.
+// warps beside the 192 KB that the products read.  Measured: a prompt of 4096 tokens on 8000 keys, 32 heads of 128, 391 to 425 us,
+// 57 to 63 % of the products' peak; 16 prompts of 777 tokens, 16 heads of 64, 146 to 150 us.  A step of both tiles takes 4800 clocks, in
+// which the issuing and loading warps wait for the softmax: registers are what it lacks, a row's 128 scores leave few.
 #pragma once
 
 #include "fa_cache.cuh"
@@ -258,7 +260,7 @@ __device__ __forceinline__ float prompt_reference(float top, float& m, float& co
 }
 
 // kSame: how many groups in a row have one scale (a page's: 4 at 64 tokens and more, 2 at 32, 1 at 16).  The softmax reads and
-// combines the scales once for so many: with pages of 64 tokens 391 us against 408 (a prompt of 2048 tokens on 16384, 32 heads of
+// combines the scales once for so many: with pages of 64 tokens 391 us against 408 (a prompt of 4096 tokens on 8000 keys, 32 heads of
 // 128), 150 against 157 (16 prompts of 777, heads of 64).
 template <int H, int kSame>
 __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const PromptArgs p) {
@@ -351,7 +353,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
                 if (__any_sync(0xFFFFFFFFu, key0 + kPromptTile > masked_from)) {
                     const int valid = static_cast<int>(masked_from) - static_cast<int>(key0);
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {   // (a bit a score: fewer instructions than a comparison each, 180 us against 184 with 16 prompts of 777)
+                    for (int w = 0; w < 4; ++w) {   // (a bit a score: fewer instructions than a comparison each, 168 us against 173 with 16 prompts of 777)
                         const int left = valid - w * 32;
                         const uint32_t seen = left >= 32 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << left) - 1u;
 #pragma unroll
