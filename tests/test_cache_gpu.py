@@ -566,3 +566,71 @@ def test_native_calls_take_plain_calls_and_agree_with_ctypes(monkeypatch):
     monkeypatch.setattr(module, "_native", (lambda *args: None,) * 3 + (calls[3],))
     for x, y in zip(got, everything(b)):
         assert torch.equal(x, y)
+
+
+# ----------------------------------------------------------------------------- where one kernel takes over from another
+
+@pytest.mark.parametrize("H,dtype", [(16, torch.bfloat16), (32, torch.float16), (64, torch.bfloat16), (128, torch.float16)])
+@pytest.mark.parametrize("page", [16, 32, 128])
+@pytest.mark.parametrize("group,T", [(3, 21), (4, 16), (5, 13), (1, 127), (16, 4), (64, 1)])
+def test_attention_with_about_64_rows(H, dtype, page, group, T):
+    G, lens = 2, [T, 300, 1111, T + 1]
+    n = sum(-(-x // page) for x in lens) + 4 * (1111 // page + 1)
+    cache = random_cache(H, G, n, page, T)
+    table, lengths = table_of(lens, page, n, T)
+    counts = torch.tensor([T, 0, T - T // 2, 1], dtype=torch.int32, device="cuda")
+    q = queries_of(4, T, G * group * H, dtype, T)
+    check_attention(cache, q, table, lengths)
+    check_attention(cache, q, table, lengths, counts=counts, causal=False)
+
+
+@pytest.mark.parametrize("longest", [512, 513, 1024, 1025])
+def test_attention_of_many_short_sequences(longest):
+    H, G, page, B = 32, 3, 32, 150
+    lens = torch.randint(0, longest, (B,), generator=gen_of(longest), device="cuda").tolist()
+    lens[3], lens[4], lens[149] = longest, 0, longest - 1
+    width = -(-longest // page)
+    cache = random_cache(H, G, B * width, page, 2)
+    table, lengths = table_of(lens, page, B * width, 3)
+    check_attention(cache, queries_of(B, 1, G * 2 * H, torch.float16, 4), table, lengths)
+
+
+@pytest.mark.parametrize("T,page,pairs", [(5, 64, False), (9, 16, True), (16, 128, False), (40, 32, True), (64, 16, False)])
+def test_appending_many_sequences_is_appending_a_few_at_a_time(T, page, pairs):
+    """Bit for bit, whichever form each call takes."""
+    H, G, B = 64, 4, 200
+    held = torch.randint(0, 3 * page, (B,), generator=gen_of(T), device="cuda", dtype=torch.int32)
+    counts = torch.randint(0, T + 1, (B,), generator=gen_of(T + 1), device="cuda", dtype=torch.int32)
+    width = -(-(3 * page + T) // page)
+    one = random_cache(H, G, B * width, page, T)
+    few = fa.cache_create(H, G, B * width, page)
+    for a, b in ((one.k, few.k), (one.v, few.v), (one.bounds, few.bounds)):
+        b.view(torch.uint8).copy_(a.view(torch.uint8))
+    few.k_scale.copy_(one.k_scale), few.v_scale.copy_(one.v_scale)
+    table = torch.randperm(B * width, generator=gen_of(1), device="cuda").to(torch.int32).view(B, width)
+    keys, values, q = (queries_of(B, T, h * H, torch.bfloat16, h) for h in (G, G, 2 * G))
+    values = values.flip(0).contiguous()
+    args = dict(rotation=angles(3 * page + T, H), interleaved=pairs)
+    rotated = fa.cache_append(one, keys, values, table, held, counts=counts, queries=q, **args)
+    for b in range(0, B, 4):
+        s = slice(b, b + 4)
+        part = fa.cache_append(few, keys[s], values[s], table[s], held[s], counts=counts[s], queries=q[s], **args)
+        assert torch.equal(part, rotated[s])
+    for a, b in ((one.k, few.k), (one.v, few.v), (one.bounds, few.bounds)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    assert torch.equal(one.k_scale, few.k_scale) and torch.equal(one.v_scale, few.v_scale) and one.read_status() == few.read_status() == (0, 0)
+
+
+@pytest.mark.parametrize("W", [70, 700, 2500, 8200])
+@pytest.mark.parametrize("keep,first,last", [(1, 0, 1), (40, 1, 2), (64, 40, 40), (69, 0, 1)])
+def test_select_of_scores_far_apart(W, keep, first, last):
+    """Scores from 2^-60 to 2^60 of either sign, most of them close together: the counting has to go on in a narrow range."""
+    H, G, page = 16, 2, 16
+    cache = random_cache(H, G, W, page, W + keep)
+    g = gen_of(W)
+    cache.k_scale.copy_(torch.where(torch.rand(W, G, generator=g, device="cuda") < 0.05, torch.exp2(torch.randint(-60, 61, (W, G), generator=g, device="cuda").float()), 0.25))
+    table = torch.randperm(W, generator=g, device="cuda").to(torch.int32)[None].contiguous()
+    lengths = torch.tensor([W * page], dtype=torch.int32, device="cuda")
+    q = queries_of(1, 2, 4 * H, torch.float16, 1)
+    got = fa.cache_select(cache, q, table, lengths, keep, first=first, last=last)
+    assert torch.equal(got.cpu(), oracle.select(cache, q, table, lengths, keep, first=first, last=last))
