@@ -169,6 +169,7 @@ RowsPlan plan_rows(uint32_t H, uint32_t heads, uint32_t group, uint32_t page, ui
     // Problems of up to 512 tokens are not divided, those of up to 1024 where there is one for every CTA: joining costs more than what
     // is left of them takes.  (Tables of 512 tokens: 1 sequence of 8 heads 9.7 us, divided 10.5, 16 sequences 10.3 and 14.3; of 1024:
     // 1 sequence 14.7 and 10.4, 32 sequences of any lengths 21.5 and 19.1, 64 27.6 and 29.1, 256 74 and 84; of 2048: 64 41.5 and 41.1.)
+    // Two units a CTA at least: with one the same times, with four 12.3 us for 10.2 (1 sequence of 1000).
     r.min_units = r.units <= 4 || (r.units <= 8 && r.problems >= ctas) ? 0 : 2;
     r.grid = static_cast<uint32_t>(r.min_units == 0 ? r.problems : ctas < all_units ? ctas : all_units);
     const uint64_t slots = r.min_units == 0 ? 0 : 2ull * r.grid * 16 * r.mt;

@@ -19,8 +19,8 @@
 //
 // Bound by the tensor pipe and the exponentials as fa_fwd_pipelined is (per step and tile 1024 tensor clocks of products at
 // H = 128 and 1024 clocks of exponentials); what is added here is shared-memory traffic, 64 KB a step written by the loading
-// warps beside the 192 KB that the products read.  Measured: a prompt of 4096 tokens on 8000 keys, 32 heads of 128, 391 to 425 us,
-// 57 to 63 % of the products' peak; 16 prompts of 777 tokens, 16 heads of 64, 146 to 150 us.  A step of both tiles takes 4800 clocks, in
+// warps beside the 192 KB that the products read.  Measured: a prompt of 4096 tokens on 8000 keys, 32 heads of 128, 390 to 425 us,
+// 57 to 63 % of the products' peak; 16 prompts of 777 tokens, 16 heads of 64, 144 to 149 us.  A step of both tiles takes 4800 clocks, in
 // which the issuing and loading warps wait for the softmax: registers are what it lacks, a row's 128 scores leave few.
 #pragma once
 
@@ -61,8 +61,10 @@ struct PromptCfg {
     static constexpr uint32_t kColO0 = 256, kColO1 = 384;
     static constexpr int kSmemBytes = (2 * kQBuffers + kSlots) * kTileBytes + 1024;
     // Registers of a thread by role: 128 a thread at launch, so twice the softmax warps' and the others' are 512 at most.  A row of
-    // scores is 128 of them; loading holds 32 of codes at H = 128, 16 or fewer below.
-    static constexpr int kSoftmaxRegs = H == 128 ? 192 : 200, kLoadRegs = H == 128 ? 80 : 64, kIssueRegs = 48;
+    // scores is 128 of them; loading holds 32 of codes at H = 128, 16 or fewer below.  Softmax, loading and issuing at H = 64 (16 prompts
+    // of 777 tokens): 200, 64, 48 150 us, 208, 64, 32 144, 208, 56, 40 153, 216, 48, 32 181; at H = 128 (4096 tokens on 8000 keys): 192, 80,
+    // 48 394, 192, 88, 40 390, 200, 72, 40 420, 184, 96, 48 462.
+    static constexpr int kSoftmaxRegs = H == 128 ? 192 : 208, kLoadRegs = H == 128 ? 88 : 64, kIssueRegs = H == 128 ? 40 : 32;
     static_assert(2 * kSoftmaxRegs + kLoadRegs + kIssueRegs <= 512, "registers of the four warpgroups");
     // barriers
     static constexpr int QFULL = 0, QEMPTY = QFULL + kQBuffers, FULL = QEMPTY + kQBuffers, EMPTY = FULL + kSlots, S0 = EMPTY + kSlots, SFREE0 = S0 + 2,

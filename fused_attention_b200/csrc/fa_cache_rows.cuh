@@ -28,8 +28,8 @@ constexpr int kRowsWarps = 4;
 constexpr int kRowsStage = 32;                       // tokens of a warp's stage
 constexpr int kRowsUnit = kRowsWarps * kRowsStage;   // tokens of a unit
 // What a problem costs a CTA beside its tokens (queries, the way to the first key, joining the warps), in units: counted when the
-// work is dealt out, so that a CTA with many short sequences gets fewer tokens.  (0, 1, 2, 3 units: 127, 117, 111, 113 us with 64
-// sequences of 100 to 8192 tokens and kRest.)
+// work is dealt out, so that a CTA with many short sequences gets fewer tokens.  (0, 1, 2, 3 units: 117, 106, 96, 99 us with 64
+// sequences of 100 to 8192 tokens; 36.0, 34.7, 33.8, 33.6 with 16 and lists of 64 pages.)
 constexpr uint32_t kRowsSetup = 2;
 constexpr float kRowsSlack = 8.0f;                   // how far an exponent may pass M before M moves
 constexpr uint32_t kNoToken = 0x7FFFFFFFu;           // position of tokens that are not there
