@@ -149,6 +149,20 @@ __device__ __forceinline__ uint32_t floats_to_e4m3x2(float lo, float hi) {
     return r;
 }
 
+// ----------------------------------------------------------------------------- sums of weights whose value scales lie far apart
+// The value scale is part of a weight's exponent, w = 2^(s + log2 scale - M), and the row's sum takes it out again, w / scale.  Where scales
+// lie further apart than this many bits (pages of zeros, 2^-100, beside values of 100 and more) a weight that counts in the sum can be
+// less than the smallest fp32 number: 2^(s - M) is then an exponential of its own.  (95: what is lost up to there is below 2^-29 of the
+// largest weight; where the weights are multiplied, in fp16, all below 2^-25 is.)
+constexpr int kSpanOfScales = 95;
+// s - M lies between -121 and 108 for scales of 2^-100 to 2^120: exponentials are taken of it and 12, near the middle.
+constexpr float kSumLift = 12.0f, kSumUnlift = 0x1p-12f;
+// x * 2^d for d <= 0, also where 2^d is less than the smallest fp32 number.  (A d that is not a number counts as a small one.)
+__device__ __forceinline__ float times_power(float x, float d) {
+    const float y = x * ex2_approx(fmaxf(d, -126.0f));
+    return d < -126.0f ? y * ex2_approx(d + 126.0f) : y;
+}
+
 __device__ __forceinline__ float2 unpack_half2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 __device__ __forceinline__ float2 unpack_16(uint32_t w, bool bf16) {
     if (bf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));

@@ -10,11 +10,12 @@
 //   warps 8-11       loading: codes of 128 keys and values a step into registers, a step ahead, from there as fp16 into the ring of
 //                    operand tiles in shared memory (the conversion is exact: no scale is applied to it); queries; scales
 //   warp 12, 14      issue Q K^T, P V (tcgen05.mma, fp32 sums in tensor memory)
-//   warp 13          works out the items
+//   warp 13          works out the items, and which of them have value scales far apart
 //
 // Scales.  A step's keys have eight groups of 16 with a scale each for K and V (pages are 16 tokens or more).  As in
 // fa_cache_rows.cuh the exponent of a weight is score * (row's factor * key scale) + log2(value scale) - M, one multiply-add
-// a pair of scores with factors that change from group to group, and the row sum divides the value scale out again.
+// a pair of scores with factors that change from group to group, and the row sum divides the value scale out again (items whose value
+// scales lie far apart, kSpanOfScales, go through a loop of their own that takes an exponential more a score).
 // A page whose scale is NaN becomes keys that are NaN and values that are zero, so that only rows that see it are NaN.
 //
 // Bound by the tensor pipe and the exponentials as fa_fwd_pipelined is (per step and tile 1024 tensor clocks of products at
@@ -23,6 +24,8 @@
 // 57 to 63 % of the products' peak; 16 prompts of 777 tokens, 16 heads of 64, 144 to 149 us.  A step of both tiles takes 4800 clocks, in
 // which the issuing and loading warps wait for the softmax: registers are what it lacks, a row's 128 scores leave few.
 #pragma once
+
+#include <type_traits>
 
 #include "fa_cache.cuh"
 #include "fa_cache_rows.cuh"
@@ -108,6 +111,8 @@ __device__ __forceinline__ void ld_8_8(const uint8_t* from, uint4& w) {
 
 // What an item is: one warp works it out ahead of the others (lengths come from memory, rows and heads from divisions) and passes it
 // on in shared memory.
+using PlainItem = std::integral_constant<bool, false>;
+using WideItem = std::integral_constant<bool, true>;   // value scales far apart
 struct PromptItem {
     uint32_t b, head;
     uint32_t t0, first;             // the first row is row `first` of `group` of token t0
@@ -157,6 +162,20 @@ __device__ __forceinline__ PromptItem prompt_item(const PromptArgs& p, uint32_t 
     it.there = 1;
     return it;
 }
+// Whether the value scales of a head's pages with the keys [key0, end) lie further apart than kSpanOfScales.  All lanes of a warp.
+__device__ __forceinline__ bool prompt_wide(const PromptArgs& p, uint32_t b, uint32_t head, uint32_t key0, uint32_t end, uint32_t lane) {
+    const int32_t* const table = p.s.table + b * p.s.table_stride;
+    const uint32_t blocks = ((end - 1u) >> p.c.page_shift) + 1u;
+    int least = 255, most = 0;   // biased exponents
+#pragma unroll 2
+    for (uint32_t block = (key0 >> p.c.page_shift) + lane; block < blocks; block += 32) {
+        const uint32_t page = static_cast<uint32_t>(table[block]);
+        if (page >= p.c.n_pages) continue;
+        const int size = max(__float_as_int(p.c.v_scale[static_cast<uint64_t>(page) * p.c.heads + head]) >> 23, 27);   // (2^-100 at least)
+        least = min(least, size), most = max(most, size);
+    }
+    return __reduce_max_sync(0xFFFFFFFFu, most) - __reduce_min_sync(0xFFFFFFFFu, least) > kSpanOfScales;
+}
 // Token and query head (of the key/value head's) of row r of an item.  `by_group`: 2^32 / group rounded up, with which the product's
 // upper half is the quotient (group < 2^16, and what is divided is less than group + 256).
 __device__ __forceinline__ void prompt_row(const PromptArgs& p, uint32_t t0, uint32_t first, uint32_t r, uint32_t& t, uint32_t& i) {
@@ -187,8 +206,8 @@ __device__ __forceinline__ void prompt_issue_pv(uint32_t tO, uint32_t tP, uint32
 
 // Weights of the groups kG0 and kG0 + 1 of a row, packed as fp16 pairs (8 words a group); adds the groups' sums to `l`, with the value
 // scale divided out.  The exponent is one multiply-add, score * cu + (vlog - ref): `ref` is a whole number, so that with scales
-// that are powers of two the bracket is exact.  `shrink`: see prompt_reference.
-template <int kG0, int kSame>
+// that are powers of two the bracket is exact.  `shrink`: see prompt_reference.  kWide: see kSpanOfScales.
+template <int kG0, int kSame, bool kWide>
 __device__ __forceinline__ void prompt_weights(const float (&s)[kPromptTile], uint32_t sc, float coef, float shrink, float ref, uint32_t (&pk)[16], float& l) {
     constexpr int kAt = kSame == 4 ? kG0 & ~3 : kG0;
     float2 ks, vlog, vinv;
@@ -197,7 +216,7 @@ __device__ __forceinline__ void prompt_weights(const float (&s)[kPromptTile], ui
     } else {
         ks.x = one_group(sc + 4 * kAt), vlog.x = one_group(sc + 4 * (kPromptGroups + kAt)), vinv.x = one_group(sc + 4 * (2 * kPromptGroups + kAt));
     }
-    uint64_t sum_a = 0, sum_b = 0, c2 = 0, a2 = 0;
+    uint64_t sum_a = 0, sum_b = 0, c2 = 0, a2 = 0, bare2 = 0;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
         const int u = kG0 + half;
@@ -205,20 +224,29 @@ __device__ __forceinline__ void prompt_weights(const float (&s)[kPromptTile], ui
             // (at least 1e-37: a masked score, -inf, must stay that)
             const float cu = fmaxf(coef * (half ? ks.y : ks.x), 1e-37f), add = fmaf(half ? vlog.y : vlog.x, shrink, -ref);
             c2 = pack_f32x2(cu, cu), a2 = pack_f32x2(add, add);
+            if (kWide) {   // (a page that is not there adds nothing)
+                const float bare = (half ? vinv.y : vinv.x) == 0.0f ? -INFINITY : kSumLift - ref;
+                bare2 = pack_f32x2(bare, bare);
+            }
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             float x0, x1;
             unpack_f32x2(fma_f32x2(pack_f32x2(s[u * 16 + 2 * e], s[u * 16 + 2 * e + 1]), c2, a2), x0, x1);
             const float w0 = ex2_approx(x0), w1 = ex2_approx(x1);
-            if (e & 1) sum_b = add_f32x2(sum_b, pack_f32x2(w0, w1));
-            else sum_a = add_f32x2(sum_a, pack_f32x2(w0, w1));
             pk[half * 8 + e] = pack_half2(w0, w1);
+            uint64_t both = pack_f32x2(w0, w1);
+            if (kWide) {
+                unpack_f32x2(fma_f32x2(pack_f32x2(s[u * 16 + 2 * e], s[u * 16 + 2 * e + 1]), c2, bare2), x0, x1);
+                both = pack_f32x2(ex2_approx(x0), ex2_approx(x1));
+            }
+            if (e & 1) sum_b = add_f32x2(sum_b, both);
+            else sum_a = add_f32x2(sum_a, both);
         }
         if (half == 1 || kSame == 1) {
             float lo, hi;
             unpack_f32x2(add_f32x2(sum_a, sum_b), lo, hi);
-            l = fmaf(lo + hi, half && kSame == 1 ? vinv.y : vinv.x, l);
+            l = fmaf(lo + hi, kWide ? kSumUnlift : half && kSame == 1 ? vinv.y : vinv.x, l);
             sum_a = sum_b = 0;
         }
     }
@@ -246,16 +274,18 @@ __device__ __forceinline__ float prompt_top(const float (&s)[kPromptTile], uint3
     }
     return top;
 }
-// A new reference for a row whose largest exponent is `top`, and the factor for the sums so far.  Beside one of 2^22 and more an
+// A new reference for a row whose largest exponent is `top`, and the factor for O so far; `l` is multiplied by it.  Beside one of 2^22 and more an
 // exponent would not be known to a fraction, and a weight could exceed fp16: all the row's exponents are then shrunk by a power of
 // two that brings it below.  The largest stays the largest, and exponents of that size differ by whole numbers or not at all, so
 // that hardly anything but the largest counts before and after.
-__device__ __forceinline__ float prompt_reference(float top, float& m, float& coef, float& shrink) {
+template <bool kWide>
+__device__ __forceinline__ float prompt_reference(float top, float& m, float& coef, float& shrink, float& l) {
     const float grown = 1.0f / shrink, whole = top * grown;
     const uint32_t size = (__float_as_uint(whole) >> 23) & 0xFFu;   // biased exponent
     const float now = size > 127u + 22u ? __uint_as_float((127u + 127u + 22u - size) << 23) : 1.0f;
-    const float m_new = ceilf(whole * now), alpha = ex2_approx(m * grown - m_new * (1.0f / now));
+    const float m_new = ceilf(whole * now), by = m * grown - m_new * (1.0f / now), alpha = ex2_approx(by);
     m = m_new;
+    l = kWide ? times_power(l, by) : l * alpha;
     coef *= grown * now;
     shrink = now;
     return alpha;
@@ -275,6 +305,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
     // a step's V tile is let go of when both tiles that take part in the step have given their P.
     __shared__ float s_coef[8][2 * kPromptTile];
     __shared__ PromptItem items[kPromptItems];
+    __shared__ uint32_t s_wide[8];                // whether an item's value scales lie far apart (kSpanOfScales); by item, as s_coef
     __shared__ uint32_t tmem_slot, abort_flag;
 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
@@ -288,10 +319,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
 
     if (tid == 0) {
         for (int i = 0; i < C::kBarriers; ++i) {
-            const bool by_loaders = (i >= C::QFULL && i < C::QEMPTY) || (i >= C::FULL && i < C::EMPTY) || (i >= C::COEF && i < C::SCALE);
+            const bool by_loaders = (i >= C::QFULL && i < C::QEMPTY) || (i >= C::FULL && i < C::EMPTY);
             const bool by_softmax = i >= C::SFREE0 && i < C::PV0;
-            // (an item is let go of by 8 softmax warps, 4 loading and 2 issuing)
-            mbar_init(bar(i), i >= C::IFREE ? 14u : by_loaders || by_softmax ? 4u : 1u);
+            // (an item is let go of by 8 softmax warps, 4 loading and 2 issuing; of its rows' factors warp 13 is one more, with s_wide)
+            mbar_init(bar(i), i >= C::IFREE ? 14u : i >= C::COEF && i < C::SCALE ? 5u : by_loaders || by_softmax ? 4u : 1u);
         }
         abort_flag = 0;
         fence_mbar_init();
@@ -338,73 +369,79 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
                 mbar_wait(bar(C::COEF + (k & 7u)), (k >> 3) & 1u, ctl, kCacheTimeout | C::COEF);
                 coef = s_coef[k & 7u][row];
             }
+            auto pass = [&](auto is_wide) {   // over the item's steps
+                constexpr bool kWide = decltype(is_wide)::value;
 #pragma unroll 1
-            for (uint32_t j = 0; j < steps; ++j, ++g, ++step, key0 += kPromptTile) {
-                mbar_wait(bar(C::S0 + i), g & 1u, ctl, kCacheTimeout | (C::S0 + i));
-                tc_fence_after();
-                __syncwarp();
-                float s[kPromptTile];
-#pragma unroll
-                for (int c = 0; c < kPromptTile; c += 32) tmem_ld32(tS + c, s + c);
-                tmem_wait_ld();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(C::SFREE0 + (C::kSharedS ? 0 : i)));
-                const uint32_t sc = smem_u32(scales) + (step % NS) * static_cast<uint32_t>(sizeof(PromptScales));
-                mbar_wait(bar(C::SCALE + step % NS), (step / NS) & 1u, ctl, kCacheTimeout | C::SCALE);
-                if (__any_sync(0xFFFFFFFFu, key0 + kPromptTile > masked_from)) {
-                    const int valid = static_cast<int>(masked_from) - static_cast<int>(key0);
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {   // (a bit a score: fewer instructions than a comparison each, 168 us against 173 with 16 prompts of 777)
-                        const int left = valid - w * 32;
-                        const uint32_t seen = left >= 32 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << left) - 1u;
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (!(seen >> e & 1u)) s[w * 32 + e] = -INFINITY;
-                    }
-                }
-                // The reference moves when an exponent exceeds it by more than 8 (weights stay below 2^9); a row that has seen nothing
-                // yet takes the first that it sees.
-                const float top = prompt_top<kSame>(s, sc, coef, shrink);
-                float alpha = 1.0f;
-                if (__any_sync(0xFFFFFFFFu, top > m + kRowsSlack)) {
-                    if (top > m + kRowsSlack) alpha = prompt_reference(top, m, coef, shrink);
-                    l *= alpha;
-                }
-                const float ref = m == -INFINITY ? 0.0f : m;
-                // the first quarter's weights are kept in registers: the last step's P V may still be reading P
-                uint32_t pk[16];
-                prompt_weights<0, kSame>(s, sc, coef, shrink, ref, pk, l);
-                if (g > 0) {
-                    mbar_wait(bar(C::PV0 + i), (g - 1u) & 1u, ctl, kCacheTimeout | (C::PV0 + i));
+                for (uint32_t j = 0; j < steps; ++j, ++g, ++step, key0 += kPromptTile) {
+                    mbar_wait(bar(C::S0 + i), g & 1u, ctl, kCacheTimeout | (C::S0 + i));
                     tc_fence_after();
-                }
-                __syncwarp();
-                tmem_st16(tP, pk);
-                prompt_weights<2, kSame>(s, sc, coef, shrink, ref, pk, l);
-                tmem_st16(tP + 16, pk);
-                prompt_weights<4, kSame>(s, sc, coef, shrink, ref, pk, l);
-                tmem_st16(tP + 32, pk);
-                prompt_weights<6, kSame>(s, sc, coef, shrink, ref, pk, l);
-                tmem_st16(tP + 48, pk);
-                if (j > 0 && __any_sync(0xFFFFFFFFu, alpha != 1.0f)) {   // (an item's first P V overwrites O)
-                    // here, where the scores' registers are free; the last step's P V has retired, and the next waits for P
-                    constexpr int kCols = 16;
-#pragma unroll 1
-                    for (int c = 0; c < H; c += kCols) {
-                        float o[kCols];
-                        uint32_t w[kCols];
-                        tmem_ld16(tO + c, o);
-                        tmem_wait_ld();
+                    __syncwarp();
+                    float s[kPromptTile];
 #pragma unroll
-                        for (int e = 0; e < kCols; ++e) w[e] = __float_as_uint(o[e] * alpha);
-                        tmem_st16(tO + c, w);
+                    for (int c = 0; c < kPromptTile; c += 32) tmem_ld32(tS + c, s + c);
+                    tmem_wait_ld();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(C::SFREE0 + (C::kSharedS ? 0 : i)));
+                    const uint32_t sc = smem_u32(scales) + (step % NS) * static_cast<uint32_t>(sizeof(PromptScales));
+                    mbar_wait(bar(C::SCALE + step % NS), (step / NS) & 1u, ctl, kCacheTimeout | C::SCALE);
+                    if (__any_sync(0xFFFFFFFFu, key0 + kPromptTile > masked_from)) {
+                        const int valid = static_cast<int>(masked_from) - static_cast<int>(key0);
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {   // (a bit a score: fewer instructions than a comparison each, 168 us against 173 with 16 prompts of 777)
+                            const int left = valid - w * 32;
+                            const uint32_t seen = left >= 32 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << left) - 1u;
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (!(seen >> e & 1u)) s[w * 32 + e] = -INFINITY;
+                        }
                     }
+                    // The reference moves when an exponent exceeds it by more than 8 (weights stay below 2^9); a row that has seen nothing
+                    // yet takes the first that it sees.
+                    const float top = prompt_top<kSame>(s, sc, coef, shrink);
+                    float alpha = 1.0f;
+                    if (__any_sync(0xFFFFFFFFu, top > m + kRowsSlack)) {
+                        if (top > m + kRowsSlack) alpha = prompt_reference<kWide>(top, m, coef, shrink, l);
+                    }
+                    const float ref = m == -INFINITY ? 0.0f : m;
+                    // the first quarter's weights are kept in registers: the last step's P V may still be reading P
+                    uint32_t pk[16];
+                    prompt_weights<0, kSame, kWide>(s, sc, coef, shrink, ref, pk, l);
+                    if (g > 0) {
+                        mbar_wait(bar(C::PV0 + i), (g - 1u) & 1u, ctl, kCacheTimeout | (C::PV0 + i));
+                        tc_fence_after();
+                    }
+                    __syncwarp();
+                    tmem_st16(tP, pk);
+                    prompt_weights<2, kSame, kWide>(s, sc, coef, shrink, ref, pk, l);
+                    tmem_st16(tP + 16, pk);
+                    prompt_weights<4, kSame, kWide>(s, sc, coef, shrink, ref, pk, l);
+                    tmem_st16(tP + 32, pk);
+                    prompt_weights<6, kSame, kWide>(s, sc, coef, shrink, ref, pk, l);
+                    tmem_st16(tP + 48, pk);
+                    if (j > 0 && __any_sync(0xFFFFFFFFu, alpha != 1.0f)) {   // (an item's first P V overwrites O)
+                        // here, where the scores' registers are free; the last step's P V has retired, and the next waits for P
+                        constexpr int kCols = 16;
+#pragma unroll 1
+                        for (int c = 0; c < H; c += kCols) {
+                            float o[kCols];
+                            uint32_t w[kCols];
+                            tmem_ld16(tO + c, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < kCols; ++e) w[e] = __float_as_uint(o[e] * alpha);
+                            tmem_st16(tO + c, w);
+                        }
+                    }
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(C::P0 + i));
                 }
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(C::P0 + i));
+            };
+            if (steps > 0) {
+                if (__builtin_expect(s_wide[k & 7u] != 0, 0)) pass(WideItem());
+                else pass(PlainItem());
             }
             // ---- the item's end: this row of O.  (The next item's first P V waits for P from these warps.)
             const bool any = steps > 0, there = row < it.n_rows;
@@ -690,22 +727,34 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
             if (leader) tc_commit(bar(last));
             __syncwarp();
             mbar_wait_certain(bar(last), 0, ctl, kCacheTimeout | static_cast<uint32_t>(last));
-        } else if (warp == 13 && lane == 0) {
+        } else if (warp == 13) {
             // ------------------------------------------------------------ items, in rounds of a CTA each, there and back: whoever had the
             // longest of a round has the shortest of the next
-            uint32_t nth = 0;
+            uint32_t nth = 0, k = 0;
             for (uint32_t round = 0;; ++round) {
                 const uint32_t index = round * gridDim.x + ((round & 1u) ? gridDim.x - 1u - blockIdx.x : blockIdx.x);
                 const bool end = round * gridDim.x >= p.items;
                 if (!end && index >= p.items) continue;
                 PromptItem it = {};
                 if (!end) it = prompt_item(p, index);
-                if (!end && it.step0 == 0 && !cache_length_ok(p.c, p.s, it.b)) cache_report(p.c.status, kCacheBadPosition);
-                if (nth >= kPromptItems && !mbar_wait(bar(C::IFREE + nth % kPromptItems), (nth / kPromptItems - 1u) & 1u, ctl, kCacheTimeout | C::IFREE)) break;
-                items[nth % kPromptItems] = it;
-                mbar_arrive(bar(C::ITEM + nth % kPromptItems));
+                if (!end && lane == 0 && it.step0 == 0 && !cache_length_ok(p.c, p.s, it.b)) cache_report(p.c.status, kCacheBadPosition);
+                const bool there = nth < kPromptItems || mbar_wait(bar(C::IFREE + nth % kPromptItems), (nth / kPromptItems - 1u) & 1u, ctl, kCacheTimeout | C::IFREE);
+                if (!__all_sync(0xFFFFFFFFu, there)) break;
+                if (lane == 0) {
+                    items[nth % kPromptItems] = it;
+                    mbar_arrive(bar(C::ITEM + nth % kPromptItems));
+                }
+                __syncwarp();
                 ++nth;
                 if (end) break;
+                if (it.steps == 0) continue;
+                const bool wide = prompt_wide(p, it.b, it.head, it.step0 * kPromptTile, min(it.farthest, (it.step0 + it.steps) * kPromptTile), lane);
+                if (lane == 0) {
+                    s_wide[k & 7u] = wide;
+                    mbar_arrive(bar(C::COEF + (k & 7u)));
+                }
+                __syncwarp();
+                ++k;
             }
         }
     }
@@ -743,7 +792,7 @@ __global__ void __launch_bounds__(128) fa_cache_prompt_join(const PromptArgs p) 
         const float2 ml = p.part_ml[slot(i)];
         if (ml.x == -INFINITY && ml.y == 0.0f) continue;   // a part without keys: its rows were not written
         const float f = ml.x == -INFINITY ? 0.0f : ex2_approx(ml.x - top);
-        sum += ml.y * f;
+        sum += times_power(ml.y, ml.x - top);
         if (lane * kWide < H)
 #pragma unroll
             for (uint32_t e = 0; e < kWide; e += 2) {

@@ -16,8 +16,9 @@
 //
 // Scales: the key scale is multiplied into the fp32 scores.  The value scale goes into the exponent: w = 2^(s + log2 scale - M)
 // with M the running maximum of just that exponent, so that P needs no second rounding and cannot leave fp16, whatever the
-// scales; the row sum takes it out again, l = sum over pages of (sum of w) / scale, in fp32.  M moves only when an exponent passes
-// it by more than 8 (w <= 2^8), so the sums are seldom rescaled.
+// scales; the row sum takes it out again, l = sum over pages of (sum of w) / scale, in fp32 (where scales lie
+// far apart, kSpanOfScales, by an exponential more a score).  M moves only when an exponent passes it by more than 8 (w <= 2^8), so the sums
+// are seldom rescaled.
 #pragma once
 
 #include "fa_cache.cuh"
@@ -319,6 +320,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[mt][j][e] = 0.0f;
 
+        float vtop = -INFINITY;   // log2 of the largest value scale that the warp has met
         for (uint32_t stage = 0; stage < n_stages; ++stage) {
             issue(stage + 1);
             cp_async_wait_group<1>();
@@ -381,6 +383,8 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
                     vinv[u] = exp2f(-vlog[u]);   // of the rounded logarithm, so that the two cancel
                     if (held_up != held_up) vinv[u] = held_up;
                 }
+                vtop = max3(vtop, vlog[0], vlog[1]);
+                const bool wide = fminf(vlog[0], vlog[1]) < vtop - kSpanOfScales;   // a page of the stage is far below that
                 const bool whole = max(at[0], at[1]) < kNoToken && max(at[0], at[1]) + 16 <= nearest;
                 uint32_t pf[MT][4][2], rest[MT][4][2];
 #pragma unroll
@@ -422,7 +426,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
                             by[u] = moves[u] ? ceilf(top[u]) : 0.0f;
                             f[u] = !moves[u] ? 1.0f : m[mt][u] == -INFINITY ? 0.0f : ex2_approx(-by[u]);
                             if (moves[u]) m[mt][u] = (m[mt][u] == -INFINITY ? 0.0f : m[mt][u]) + by[u];
-                            l[mt][u] *= f[u];
+                            l[mt][u] = times_power(l[mt][u], -by[u]);   // (0 before anything has been seen)
                         }
 #pragma unroll
                         for (int n = 0; n < 4; ++n)
@@ -432,6 +436,12 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
                         for (int j = 0; j < kTilesN; ++j)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) o[mt][j][e] *= f[e >> 1];
+                    }
+                    if (wide) {
+#pragma unroll
+                        for (int n = 0; n < 4; ++n)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) l[mt][e >> 1] += ex2_approx(s[mt][n][e] + (kSumLift - vlog[n >> 1])) * kSumUnlift;
                     }
                     float sum[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
 #pragma unroll
@@ -453,7 +463,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
                         for (int h2 = 0; h2 < 2; ++h2)   // (a page none of whose tokens the row sees adds nothing, whatever its scale)
-                            l[mt][u] += sum[h2][u] == 0.0f ? 0.0f : sum[h2][u] * vinv[h2];
+                            l[mt][u] += sum[h2][u] == 0.0f || wide ? 0.0f : sum[h2][u] * vinv[h2];
                 }
                 // ---- O += P V: 16 tokens at a time
 #pragma unroll
@@ -506,6 +516,12 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
                 if (t4 == 0) s_ml[warp * Cfg::kRows + mt * 16 + u * 8 + g] = make_float2(m[mt][u], l[mt][u]);
             }
         __syncthreads();   // every warp has read its last stage
+        if (tid < kRowsWarps * Cfg::kRows) {   // the warps' row sums, against the largest M of a row (which is read from the other half of the entries)
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kRowsWarps; ++w) top = fmaxf(top, s_ml[w * Cfg::kRows + tid % Cfg::kRows].x);
+            s_ml[tid].y = times_power(s_ml[tid].y, s_ml[tid].x - top);
+        }
         float* const area = reinterpret_cast<float*>(smem) + warp * (Cfg::kRows * H);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -536,8 +552,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
             for (int w = 0; w < kRowsWarps; ++w) top = fmaxf(top, s_ml[w * Cfg::kRows + r].x);
 #pragma unroll
             for (int w = 0; w < kRowsWarps; ++w) {
-                const float2 ml = s_ml[w * Cfg::kRows + r];
-                sum += ml.y * (ml.x == -INFINITY ? 0.0f : ex2_approx(ml.x - top));
+                sum += s_ml[w * Cfg::kRows + r].y;
                 const float2 y = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(smem) + (w * Cfg::kRows + r) * H +
                                                                   (d ^ (H >= 64 ? (r & 3u) * 2 : 0u)));
                 x.x += y.x, x.y += y.y;
@@ -602,7 +617,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fa_cache_join(const RowsArgs 
         const float f = ml.x == -INFINITY ? 0.0f : ex2_approx(ml.x - now);
         const float again = top == now || top == -INFINITY ? 1.0f : ex2_approx(top - now);   // for what the turns before have added up
         s_f[tid] = f;
-        sum = sum * again + ml.y * f;
+        sum = times_power(sum, top - now) + times_power(ml.y, ml.x - now);
 #pragma unroll
         for (int d = 0; d < kWide; ++d) x[d] *= again;
         top = now;
@@ -671,7 +686,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fa_cache_join_few(const RowsA
         for (int d = 16; d >= 1; d >>= 1) now = fmaxf(now, __shfl_xor_sync(0xFFFFFFFFu, now, d));
         const float f = ml.x == -INFINITY ? 0.0f : ex2_approx(ml.x - now);
         const float again = top == now || top == -INFINITY ? 1.0f : ex2_approx(top - now);
-        sum = sum * again + ml.y * f;
+        sum = times_power(sum, top - now) + times_power(ml.y, ml.x - now);
 #pragma unroll
         for (int d = 0; d < kWide; ++d) x[d] *= again;
         top = now;
