@@ -145,7 +145,8 @@ def cache_append(cache: KVCache, keys: torch.Tensor, values: torch.Tensor, table
     ``counts``    int32 [B]: how many of the T tokens sequence b has (default: all)
     ``queries``   [B, T, heads * head_dim]: rotated like the keys and returned as a new tensor, zeros where there is no token
     ``rotation``  (cos, sin), float32 [positions, head_dim / 2] each: keys and queries are rotated by their position, pairs of
-                  dimensions (i, i + head_dim / 2), or (2 i, 2 i + 1) with ``interleaved``
+                  dimensions (i, i + head_dim / 2), or (2 i, 2 i + 1) with ``interleaved``; tokens behind the last position are
+                  not appended, their queries come back as zeros, and ``read_status`` tells
 
     Each page keeps, by head, one power of two as the scale of its keys and one as that of its values, such that the largest
     magnitude comes to lie in the upper half of e4m3's range; where a later token needs a larger scale the page's codes move to it.

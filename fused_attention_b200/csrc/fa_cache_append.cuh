@@ -187,9 +187,11 @@ __global__ void __launch_bounds__(kAppendThreads, 5) fa_cache_append(const Appen
     const uint64_t first = block << p.c.page_shift;               // position of the block's first token
     if (first >= static_cast<uint64_t>(held) + n) return;
     const uint32_t begin = nth == 0 ? held & (p.c.page - 1) : 0u;   // slots [begin, end) are new
-    const uint32_t end = static_cast<uint32_t>(min(static_cast<uint64_t>(p.c.page), static_cast<uint64_t>(held) + n - first));
+    const uint32_t all = static_cast<uint32_t>(min(static_cast<uint64_t>(p.c.page), static_cast<uint64_t>(held) + n - first));
+    // (tokens behind the rotation's last position are not appended, neither their keys nor their values)
+    const uint32_t end = p.cos == nullptr ? all : static_cast<uint32_t>(min(static_cast<uint64_t>(all), max(static_cast<uint64_t>(p.positions), first) - first));
     int32_t page = -1;
-    const bool fits = held_signed >= 0 && block < p.s.width && (p.cos == nullptr || first + end <= p.positions);
+    const bool fits = held_signed >= 0 && block < p.s.width;
     if (fits) page = p.s.table[b * p.s.table_stride + block];   // (asked for ahead of the tokens, used behind them)
     const uint32_t j = tid % kPerToken, sub = tid / kPerToken;
     const uint8_t* rows = is_v ? p.values + b * p.values_b : p.keys + b * p.keys_b;
@@ -200,10 +202,9 @@ __global__ void __launch_bounds__(kAppendThreads, 5) fa_cache_append(const Appen
     RawSixteen raw;
     auto from = [&](uint32_t slot) { return load_sixteen<H>(rows + static_cast<uint32_t>(first + slot - held) * row_pitch, j); };
     if (begin + sub < end) raw = from(begin + sub);
-    if (!fits || static_cast<uint32_t>(page) >= p.c.n_pages) {
-        if (tid == 0) cache_report(p.c.status, fits ? kCacheBadPage : kCacheBadPosition);
-        return;
-    }
+    const bool known = static_cast<uint32_t>(page) < p.c.n_pages;
+    if (tid == 0 && (!known || end < all)) cache_report(p.c.status, fits && end == all ? kCacheBadPage : kCacheBadPosition);
+    if (!known || end <= begin) return;
     const bool turned = !is_v && p.cos != nullptr;
     auto values_of = [&](const RawSixteen& w, uint32_t slot) {
         Sixteen r = unpack_sixteen(w, bf16);
