@@ -42,12 +42,12 @@ constexpr int kScoreTiles = 4;     // of 16 query rows that a CTA holds at most
 constexpr int kTakeThreads = 256;
 constexpr int kTakeBinBits = 9;      // (32 queries on 20001 tokens, the whole call: 8 bits 17.3 us, 9 17.4, 10 18.3, 11 22.2; on 60000 in pages of 16: 76.1, 74.9, 76.0, 77.3)
 constexpr uint32_t kTakeBins = 1u << kTakeBinBits;
-constexpr uint32_t kTakeAlways = 0xFF800000u;   // score of a page that is taken whatever its bounds: infinity (NaN is above it)
+constexpr uint32_t kTakeAlways = 0xFFFFFFFFu;   // key of a page that is taken whatever its score
 
-// Whole numbers of the same order as the floats (a NaN above all).
+// Whole numbers of the same order as the floats (a NaN above all), below kTakeAlways.
 __device__ __forceinline__ uint32_t sortable(float x) {
     const uint32_t u = __float_as_uint(x + 0.0f);   // (-0 is 0)
-    return u ^ (u & 0x80000000u ? 0xFFFFFFFFu : 0x80000000u);
+    return min(u ^ (u & 0x80000000u ? 0xFFFFFFFFu : 0x80000000u), kTakeAlways - 1u);
 }
 
 // What the queries see: token t of `count` stands at position held - count + t; -1 where there is none.
@@ -236,9 +236,8 @@ __device__ __forceinline__ void score_pages(const SelectArgs& p, uint32_t b, uin
                     if (my_page < n_pages) {
                         const int64_t position = query_position(p.c, p.s, b, t);
                         const int64_t own = position >> p.c.page_shift;
-                        float score = my_scale == -1.0f ? -INFINITY : __fmul_rn(x, my_scale);
-                        if (my_page < p.first || static_cast<int64_t>(my_page) > own - static_cast<int64_t>(p.last)) score = INFINITY;
-                        uint32_t key = sortable(score);
+                        uint32_t key = sortable(my_scale == -1.0f ? -INFINITY : __fmul_rn(x, my_scale));
+                        if (my_page < p.first || static_cast<int64_t>(my_page) > own - static_cast<int64_t>(p.last)) key = kTakeAlways;
                         if (position < 0 || static_cast<int64_t>(my_page) > own) key = 0;   // behind the query
                         uint32_t* const at = p.keys + ((static_cast<uint64_t>(b) * p.s.T + t) * p.c.heads + head) * p.s.width + my_page;
                         *at = turn > 0 ? max(key, *at) : key;
@@ -331,7 +330,7 @@ __global__ void __launch_bounds__(kTakeThreads) fa_cache_take(const SelectArgs p
     // The range, without the pages that are always taken, or of those alone where there are more of them than are wanted.
     uint32_t low = kTakeAlways, high = 0, always = 0;
     each([&](uint32_t, uint32_t key) {
-        if (key >= kTakeAlways) ++always;
+        if (key == kTakeAlways) ++always;
         else low = min(low, key), high = max(high, key);
     });
     low = __reduce_min_sync(0xFFFFFFFFu, low), high = __reduce_max_sync(0xFFFFFFFFu, high), always = __reduce_add_sync(0xFFFFFFFFu, always);
@@ -340,8 +339,9 @@ __global__ void __launch_bounds__(kTakeThreads) fa_cache_take(const SelectArgs p
     always = 0;
 #pragma unroll
     for (uint32_t w = 0; w < kWarps; ++w) low = min(low, s_low[w]), high = max(high, s_high[w]), always += s_sum[w];
-    uint32_t want = p.keep - always, range = high - low;   // of the keys in [low, low + range], which are more than that
-    if (always >= p.keep) want = p.keep, low = kTakeAlways, range = ~kTakeAlways;
+    uint32_t want = p.keep - always;   // of the keys in [low, low + range], which are more than that
+    if (always >= p.keep) want = p.keep, low = high = kTakeAlways;
+    uint32_t range = high - low;
     uint32_t least, ties;   // taken: the keys above `least`, and the first `ties` that are equal to it
     for (;;) {
         const uint32_t shift = max(32 - __clz(range), kTakeBinBits) - kTakeBinBits;   // range >> shift < kTakeBins
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kTakeThreads) fa_cache_take(const SelectArgs p
             least = low, ties = want;
             break;
         }
-        range = (1u << shift) - 1u;
+        range = min((1u << shift) - 1u, high - low);   // (the highest bin may reach beyond `high`, to the pages that are always taken)
     }
     // how many that are above, equal the threads in front have
     uint32_t mine_above = 0, mine_equal = 0;

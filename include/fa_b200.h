@@ -362,7 +362,7 @@ int fa_b200_cache_append(const fa_b200_cache* cache, const fa_b200_sequences* se
  * stands at position lengths[b] - counts[b] + t.  Score of a page: with q8 = rint(q * (1 / max |q| * 127)) of a query head and
  * lo8, hi8 = rint(bound / 4), sum over the dimensions of max(q8 lo8, q8 hi8), a whole number; times max |q| * (1 / 127); the largest
  * of the query heads of the key/value head; times the page's key scale (each product and quotient rounded to fp32).  Ties go to the lower page.  The first `first` blocks
- * and the last `last` up to the query's own (at least one) are taken before all others.  Scratch: 4 * B * T * kv_heads *
+ * and the last `last` up to the query's own (at least one) are taken before all others, behind them pages whose score is not a number.  Scratch: 4 * B * T * kv_heads *
  * table_width bytes.
  */
 int fa_b200_cache_select(const fa_b200_cache* cache, const fa_b200_sequences* sequences, const void* queries, int64_t queries_batch_stride,
