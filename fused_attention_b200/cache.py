@@ -56,7 +56,8 @@ class KVCache:
 
     ``k``, ``v``            float8_e4m3fn [n_pages, kv_heads, page_size, head_dim], last axis contiguous, other strides multiples
                             of 16
-    ``k_scale``, ``v_scale``  float32 [n_pages, kv_heads], contiguous; a value is code * scale
+    ``k_scale``, ``v_scale``  float32 [n_pages, kv_heads], contiguous; a value is code * scale, 2^-100 to 2^120 (one below zero is taken
+                            for NaN)
     ``bounds``              float8_e4m3fn [n_pages, kv_heads, 2, head_dim], contiguous: lowest and highest key code
 
     The tensors are looked at once, here; they must not be moved or resized afterwards.  ``cache_create`` makes them.

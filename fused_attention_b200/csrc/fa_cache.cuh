@@ -157,6 +157,8 @@ __device__ __forceinline__ uint32_t floats_to_e4m3x2(float lo, float hi) {
 constexpr int kSpanOfScales = 95;
 // s - M lies between -121 and 108 for scales of 2^-100 to 2^120: exponentials are taken of it and 12, near the middle.
 constexpr float kSumLift = 12.0f, kSumUnlift = 0x1p-12f;
+// A scale; one below zero, which no append writes, is not a number.
+__device__ __forceinline__ float scale_or_nan(float x) { return x < 0.0f ? __int_as_float(0x7FC00000) : x; }
 // x * 2^d for d <= 0, also where 2^d is less than the smallest fp32 number.  (A d that is not a number counts as a small one.)
 __device__ __forceinline__ float times_power(float x, float d) {
     const float y = x * ex2_approx(fmaxf(d, -126.0f));

@@ -16,7 +16,7 @@
 // fa_cache_rows.cuh the exponent of a weight is score * (row's factor * key scale) + log2(value scale) - M, one multiply-add
 // a pair of scores with factors that change from group to group, and the row sum divides the value scale out again (items whose value
 // scales lie far apart, kSpanOfScales, go through a loop of their own that takes an exponential more a score).
-// A page whose scale is NaN becomes keys that are NaN and values that are zero, so that only rows that see it are NaN.
+// A page whose scale is NaN (or below zero) becomes keys that are NaN and values that are zero, so that only rows that see it are NaN.
 //
 // Bound by the tensor pipe and the exponentials as fa_fwd_pipelined is (per step and tile 1024 tensor clocks of products at
 // H = 128 and 1024 clocks of exponentials); what is added here is shared-memory traffic, 64 KB a step written by the loading
@@ -609,8 +609,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
             // ---- keys and values, K and V of a step in turn
 #pragma unroll 1
             for (uint32_t step = 0; step < it.steps; ++step, ++g) {
-                // groups without a page (lower byte), and with a scale that is NaN; whether the keys end within the step
-                const uint32_t gone = __ballot_sync(0xFFFFFFFFu, none) & 0xFFu, poisoned = __ballot_sync(0xFFFFFFFFu, ks != ks || vs != vs) & 0xFFu;
+                // groups without a page (lower byte), and with a scale that is NaN or below zero; whether the keys end within the step
+                const uint32_t gone = __ballot_sync(0xFFFFFFFFu, none) & 0xFFu, poisoned = __ballot_sync(0xFFFFFFFFu, !(ks >= 0.0f && vs >= 0.0f)) & 0xFFu;
                 const uint32_t left = it.farthest - (it.step0 + step) * kPromptTile;
                 const bool spoilt = (gone | poisoned) != 0 || left < kPromptTile;
                 ask(step + 1);
@@ -619,7 +619,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
                     if (n >= NS) mbar_wait(bar(C::EMPTY + n % NS), (n / NS - 1u) & 1u, ctl, kCacheTimeout | (C::EMPTY + n % NS));
                     if (is_v == 0 && lane < kGroups && warp == 8) {   // (the V tile of the step that had this entry has been let go of)
                         PromptScales& sc = scales[g % NS];
-                        const bool bad = ks != ks || vs != vs;
+                        const bool bad = !(ks >= 0.0f && vs >= 0.0f);
                         const float held_up = bad || !(vs > 0x1p-100f) ? (bad ? 1.0f : 0x1p-100f) : vs, vlog = __log2f(held_up);
                         sc.ks[lane] = bad ? 1.0f : ks;
                         sc.vlog[lane] = none ? -INFINITY : vlog;

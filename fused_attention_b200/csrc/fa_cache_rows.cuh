@@ -376,8 +376,8 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
                 float ks[2], vlog[2], vinv[2];
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    ks[u] = __uint_as_float(ld_shared_u32(meta + 4 * u));
-                    const float vs = __uint_as_float(ld_shared_u32(meta + 8 + 4 * u));
+                    ks[u] = scale_or_nan(__uint_as_float(ld_shared_u32(meta + 4 * u)));
+                    const float vs = scale_or_nan(__uint_as_float(ld_shared_u32(meta + 8 + 4 * u)));
                     const float held_up = vs < 0x1p-100f ? 0x1p-100f : vs;   // (a scale of zero has no logarithm)
                     vlog[u] = __log2f(held_up);
                     vinv[u] = exp2f(-vlog[u]);   // of the rounded logarithm, so that the two cancel

@@ -190,8 +190,8 @@ __device__ __forceinline__ void score_pages(const SelectArgs& p, uint32_t b, uin
                         }
                     }
             // scales of the pages that this lane writes: page p0 + lane % 16
-            const float scale_lo = __shfl_sync(0xFFFFFFFFu, there[0] ? scale[0] : -1.0f, (lane & 7u) * 4),
-                        scale_hi = __shfl_sync(0xFFFFFFFFu, there[1] ? scale[1] : -1.0f, (lane & 7u) * 4);
+            const float scale_lo = __shfl_sync(0xFFFFFFFFu, there[0] ? scale_or_nan(scale[0]) : -1.0f, (lane & 7u) * 4),
+                        scale_hi = __shfl_sync(0xFFFFFFFFu, there[1] ? scale_or_nan(scale[1]) : -1.0f, (lane & 7u) * 4);
             const float my_scale = lane & 8u ? scale_hi : scale_lo;
             if (p0 + stride < n_pages) {
                 ask_bounds(p0 + stride);

@@ -301,7 +301,7 @@ int fa_b200_describe_schedule(uint32_t B, uint32_t L, uint32_t F, uint32_t head_
  * fp32 scale for its keys and one for its values (a value is code * scale), and the bounds of its keys, the lowest and the
  * highest code by dimension.  The i-th block of page_size tokens of sequence b lies in page table[b][i].  The scales that
  * fa_b200_cache_append writes are powers of two from 2^-100 to 2^120; attention and selection take any others in this range, however
- * far apart (attention takes a value scale below 2^-100 for 2^-100).
+ * far apart (attention takes a value scale below 2^-100 for 2^-100).  A scale below zero counts as one that is not a number.
  *
  * What these functions are given is checked before anything is launched, as far as the host can see it.  What lies in device
  * memory (table, lengths, counts, selected pages) the kernels look at before they use it: tokens whose page is outside the
