@@ -242,6 +242,9 @@ def cache_attention(cache: KVCache, queries: torch.Tensor, table: torch.Tensor, 
     all keys of its sequence.  ``heads`` is a multiple of the cache's kv_heads, query head h goes with key/value head
     h // (heads // kv_heads).  ``pages`` int32 [B, T, kv_heads, keep], as ``cache_select`` returns it: only these blocks of the
     sequence, each at most once, -1 for nothing.  A query that sees no key, or that its sequence does not have, gets zeros.
+
+    Scores and sums are held in 32 bits.  The weights are rounded to fp16 for their product with the values; with fewer than 64 rows (T *
+    heads / kv_heads), or with ``pages``, fp16 calls multiply what that loses too: their error is little more than the result's rounding.
     """
     _require(isinstance(cache, KVCache), "the first argument must be a KVCache")
     _, _, attention, entries = _calls()

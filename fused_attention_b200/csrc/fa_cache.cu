@@ -136,7 +136,6 @@ constexpr uint64_t kMostCtas = 0x7FFFFFFFull;
 // ----------------------------------------------------------------------------- attention for few rows
 struct RowsPlan {
     uint32_t mt, rows, row_tiles, grid, min_units;
-    bool rest;
     uint64_t problems, units;   // units: of one problem, at most
     uint64_t o_bytes, ml_bytes, share_bytes;
     uint64_t scratch() const { return 16 + o_bytes + ml_bytes + share_bytes; }
@@ -163,9 +162,6 @@ RowsPlan plan_rows(uint32_t H, uint32_t heads, uint32_t group, uint32_t page, ui
     r.units = (tokens + fa::kRowsUnit - 1) / fa::kRowsUnit;
     r.problems = static_cast<uint64_t>(B) * heads * r.row_tiles;   // (below 2^31 in every call that is taken)
     const uint64_t ctas = static_cast<uint64_t>(sms) * (r.mt == 1 ? 3 : 2), all_units = r.problems * r.units;
-    // What the rounding of the weights takes away is multiplied too where results are fp16 and a CTA has few units (64 sequences of up
-    // to 8192 tokens, 75 units a CTA: 97 us without, 111 with; one of 301 tokens: 9.6 and 9.8).
-    r.rest = all_units <= 8 * ctas;
     // Problems of up to 512 tokens are not divided, those of up to 1024 where there is one for every CTA: joining costs more than what
     // is left of them takes.  (Tables of 512 tokens: 1 sequence of 8 heads 9.7 us, divided 10.5, 16 sequences 10.3 and 14.3; of 1024:
     // 1 sequence 14.7 and 10.4, 32 sequences of any lengths 21.5 and 19.1, 64 27.6 and 29.1, 256 74 and 84; of 2048: 64 41.5 and 41.1.)
@@ -182,8 +178,8 @@ RowsPlan plan_rows(uint32_t H, uint32_t heads, uint32_t group, uint32_t page, ui
 template <int H, int MT>
 int launch_rows(Device& d, uint32_t bit, const fa::RowsArgs& a, const RowsPlan& plan, cudaStream_t stream) {
     using Cfg = fa::RowsCfg<H, MT>;
-    const auto kernel = plan.rest ? &fa::fa_cache_rows<H, MT, true> : &fa::fa_cache_rows<H, MT, false>;
-    int rc = allow_smem(d, bit + (plan.rest ? 12 : 0), kernel, Cfg::kSmem);
+    const auto kernel = a.bf16 ? &fa::fa_cache_rows<H, MT, false> : &fa::fa_cache_rows<H, MT, true>;
+    int rc = allow_smem(d, bit + (a.bf16 ? 0 : 12), kernel, Cfg::kSmem);
     if (rc == FA_B200_OK) rc = launch(kernel, plan.grid, fa::kRowsWarps * 32, Cfg::kSmem, stream, a);
     if (rc != FA_B200_OK || plan.min_units == 0) return rc;
     const uint64_t rows = plan.problems * plan.rows;
@@ -422,13 +418,12 @@ int fa_b200_cache_attention(const fa_b200_cache* cache, const fa_b200_sequences*
             default: return launch_prompt<128>(*d, 41, b, plan, stream);
         }
     }
-    RowsPlan plan = plan_rows(H, a.c.heads, q_heads / a.c.heads, a.c.page, a.s.B, a.s.T, a.s.width, keep, static_cast<uint32_t>(d->sms.load()));
+    const RowsPlan plan = plan_rows(H, a.c.heads, q_heads / a.c.heads, a.c.page, a.s.B, a.s.T, a.s.width, keep, static_cast<uint32_t>(d->sms.load()));
     if (plan.problems * plan.rows > kMostCtas || plan.problems * (plan.units + fa::kRowsSetup) > 0xFFFFFFFFull) return FA_B200_ERR_SHAPE;
     if (scratch_bytes < plan.scratch()) return FA_B200_ERR_TOO_LARGE;
     a.q = static_cast<const uint8_t*>(queries), a.q_b = 2 * queries_batch_stride, a.q_t = 2 * queries_token_stride;
     a.y = static_cast<uint8_t*>(y), a.pages = pages_or_null, a.keep = keep;
     a.group = q_heads / a.c.heads, a.causal = (flags & FA_B200_CACHE_ALL_KEYS) ? 0u : 1u, a.bf16 = dtype == FA_B200_BF16;
-    plan.rest = plan.rest && dtype == FA_B200_FP16;
     a.rows = plan.rows, a.row_tiles = plan.row_tiles, a.min_units = plan.min_units;
     a.scale_log2 = scale_log2(H);
     uint8_t* const at = static_cast<uint8_t*>(scratch);

@@ -375,7 +375,8 @@ int fa_b200_cache_select(const fa_b200_cache* cache, const fa_b200_sequences* se
  * lengths[b] - counts[b] + t and sees the keys up to its own, or all with FA_B200_CACHE_ALL_KEYS.  With `pages`
  * ([B, T, kv_heads, keep], as fa_b200_cache_select writes them, -1 for nothing) only those blocks.  y is contiguous, of the
  * queries' type; a query that sees no key, or that its sequence does not have, gets zeros.  Scores, weights and sums are held in
- * fp32; the weights are rounded to fp16 for the product with V.  Scratch: as fa_b200_cache_attention_scratch says, on a 16-byte
+ * fp32; the weights are rounded to fp16 for the product with V.  In fp16 calls with `pages`, or with fewer than 64 rows (T * q_heads /
+ * kv_heads), what that rounding takes away is multiplied as well, so that an error is little more than the rounding of y.  Scratch: as fa_b200_cache_attention_scratch says, on a 16-byte
  * boundary.
  */
 int fa_b200_cache_attention(const fa_b200_cache* cache, const fa_b200_sequences* sequences, const void* queries, int64_t queries_batch_stride,
