@@ -68,18 +68,19 @@ class CachedDecoder:
         """(graph, tokens): a replay takes tokens [B, 1], appends them and leaves the most likely next ones in their place."""
         tokens = torch.zeros(len(self.lengths), 1, dtype=torch.int64, device="cuda")
 
-        def step() -> None:
-            tokens.copy_(self.forward(tokens, keep=keep).argmax(-1))
-        held = self.lengths.clone()
+        def step(counts: Optional[torch.Tensor] = None) -> None:
+            tokens.copy_(self.forward(tokens, counts, keep=keep).argmax(-1))
+        # Library handles and allocations come into being ahead of the capture, in a step without a token for any sequence: one that is
+        # appended and taken back would leave its page's scale enlarged and its bounds widened.
+        none = torch.zeros_like(self.lengths)
         stream = torch.cuda.Stream()
         stream.wait_stream(torch.cuda.current_stream())
-        with torch.cuda.stream(stream):   # (library handles and allocations come into being ahead of the capture)
-            step()
+        with torch.cuda.stream(stream):
+            step(none)
         torch.cuda.current_stream().wait_stream(stream)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             step()
-        self.lengths.copy_(held)   # (the token that was tried is written over by the next)
         return graph, tokens
 
 
