@@ -24,7 +24,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 EXTDIR = os.path.join(HERE, "ext")
 LIB = os.path.join(LIBDIR, "libfa_b200.so")
-DEBUG_LIB = os.path.join(LIBDIR, "libfa_b200_debug.so")   # the checked build (-DFA_DEBUG), used by one GPU test
+DEBUG_LIB = os.path.join(LIBDIR, "libfa_b200_debug.so")   # the checked build (-DFA_DEBUG), used by GPU tests
 CYCLES_LIB = os.path.join(LIBDIR, "libfa_b200_cycles.so")  # the clock-counting build (-DFA_CYCLES), see cycles.py
 TIMELINE_LIB = os.path.join(LIBDIR, "libfa_b200_timeline.so")  # ... with per-step time stamps (-DFA_TIMELINE) as well
 
@@ -58,12 +58,12 @@ def cache_sources() -> list[str]:
                                             "fa_ptx.cuh")] + [os.path.join(ROOT, "include", "fa_b200.h")]
 
 
-def build_cache_object(force: bool = False, verbose: bool = False) -> str:
-    """Compile csrc/fa_cache.cu, the key/value cache's part, once for all variants of the library."""
-    out = os.path.join(LIBDIR, "fa_cache.o")
+def build_cache_object(force: bool = False, verbose: bool = False, debug: bool = False) -> str:
+    """Compile csrc/fa_cache.cu, the key/value cache's part: once for the checked library (-DFA_DEBUG), once for all others."""
+    out = os.path.join(LIBDIR, "fa_cache_debug.o" if debug else "fa_cache.o")
     if force or _stale(out, cache_sources()):
         os.makedirs(LIBDIR, exist_ok=True)
-        flags = [f for f in NVCC_FLAGS if f != "-shared"]
+        flags = [f for f in NVCC_FLAGS if f != "-shared"] + (["-DFA_DEBUG"] if debug else [])
         subprocess.run([_nvcc(), *flags, "-I", os.path.join(ROOT, "include"), "-I", CSRC, *(["-Xptxas", "-v"] if verbose else []),
                         "-c", "-o", out, os.path.join(CSRC, "fa_cache.cu")], check=True)
     return out
@@ -74,14 +74,14 @@ def build_lib(force: bool = False, verbose: bool = False, debug: bool = False, c
     """Compile csrc/fa_b200.cu into lib/libfa_b200.so (cross-compiles without a GPU).
 
     ``debug`` builds lib/libfa_b200_debug.so instead, with -DFA_DEBUG: every TMA copy and tensor-memory
-    access checks its operands first (see the checked-build section of csrc/fa_ptx.cuh).
+    access checks its operands first (see the checked-build sections of csrc/fa_ptx.cuh and csrc/fa_cache.cuh).
     ``cycles`` builds lib/libfa_b200_cycles.so, with -DFA_CYCLES: CTA 0 of the warp-specialised kernels
     records time stamps and its SM clock count per launch (read by cycles.py).
     ``timeline`` builds lib/libfa_b200_timeline.so, with -DFA_CYCLES -DFA_TIMELINE: one warp per role of CTA 0 of
     the kernel on pairs of CTAs also stamps the events of every key step (cycles.py --timeline)."""
     os.makedirs(LIBDIR, exist_ok=True)
     out = DEBUG_LIB if debug else (TIMELINE_LIB if timeline else (CYCLES_LIB if cycles else LIB))
-    cache = build_cache_object(force=force and out == LIB, verbose=verbose)
+    cache = build_cache_object(force=force and out in (LIB, DEBUG_LIB), verbose=verbose, debug=debug)
     if not force and not _stale(out, lib_sources() + [cache]):
         return out
     cmd = [_nvcc(), *NVCC_FLAGS, "-I", os.path.join(ROOT, "include"), "-I", CSRC]

@@ -133,6 +133,14 @@ int rows_ok(const void* base, int64_t batch_stride, int64_t token_stride) {
 
 constexpr uint64_t kMostCtas = 0x7FFFFFFFull;
 
+// Checked build: what a call writes is filled with NaN (or places far outside) beforehand.
+#ifdef FA_DEBUG
+int poison(void* p, uint64_t bytes, int value, cudaStream_t stream) { return static_cast<int>(cudaMemsetAsync(p, value, bytes, stream)); }
+#define FA_CACHE_FILL(p, bytes, value, stream) if (const int poisoned = poison(p, bytes, value, stream)) return poisoned
+#else
+#define FA_CACHE_FILL(p, bytes, value, stream) do {} while (0)
+#endif
+
 // ----------------------------------------------------------------------------- attention for few rows
 struct RowsPlan {
     uint32_t mt, rows, row_tiles, grid, min_units;
@@ -299,6 +307,7 @@ int fa_b200_cache_append(const fa_b200_cache* cache, const fa_b200_sequences* se
     OnDevice on(device);
     if (on.rc != 0) return on.rc;
     const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+    if (queries_or_null) FA_CACHE_FILL(rotated, 2ull * a.s.B * a.s.T * q_heads * H, 0xFF, stream);
     switch (H) {
         case 16: return launch_append<16>(a, warp_tasks, task_ctas, stream);
         case 32: return launch_append<32>(a, warp_tasks, task_ctas, stream);
@@ -340,6 +349,8 @@ int fa_b200_cache_select(const fa_b200_cache* cache, const fa_b200_sequences* se
     OnDevice on(device);
     if (on.rc != 0) return on.rc;
     const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+    FA_CACHE_FILL(scratch, 4 * rows * a.s.width, 0xFF, stream);
+    FA_CACHE_FILL(pages, 4 * rows * keep, 0x7F, stream);
     const uint32_t grid = static_cast<uint32_t>(units < resident ? units : resident);
     const size_t smem = static_cast<size_t>(a.tiles) * (cache->head_dim / 16) * 2 * 32 * sizeof(uint4);   // 32 KB at most
     constexpr uint32_t kBlock = fa::kScoreWarps * 32;
@@ -411,6 +422,8 @@ int fa_b200_cache_attention(const fa_b200_cache* cache, const fa_b200_sequences*
         OnDevice on(device);
         if (on.rc != 0) return on.rc;
         const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+        FA_CACHE_FILL(y, 2ull * a.s.B * a.s.T * q_heads * H, 0xFF, stream);
+        FA_CACHE_FILL(scratch, plan.scratch(), 0xFF, stream);
         switch (H) {
             case 16: return launch_prompt<16>(*d, 32, b, plan, stream);
             case 32: return launch_prompt<32>(*d, 35, b, plan, stream);
@@ -433,6 +446,11 @@ int fa_b200_cache_attention(const fa_b200_cache* cache, const fa_b200_sequences*
     OnDevice on(device);
     if (on.rc != 0) return on.rc;
     const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+    FA_CACHE_FILL(y, 2ull * a.s.B * a.s.T * q_heads * H, 0xFF, stream);
+    FA_CACHE_FILL(scratch, plan.scratch(), 0xFF, stream);
+#ifdef FA_DEBUG
+    a.slots = plan.min_units == 0 ? 0 : 2ull * plan.grid, a.problems = plan.problems;
+#endif
     switch (H) {
         case 16: return launch_rows<16>(*d, 0, a, plan, stream);
         case 32: return launch_rows<32>(*d, 2, a, plan, stream);

@@ -43,6 +43,35 @@ __device__ __forceinline__ void cache_report(uint32_t* status, uint32_t code) {
     atomicAdd(status + 1, 1u);
 }
 
+// ----------------------------------------------------------------------------- checked build (-DFA_DEBUG)
+// Where an address is formed, of a table entry, a list, a scale, bounds or codes, a row of a tensor, a place of a tile in shared memory or of
+// scratch, the checked build looks at its indexes first.  A failed check leaves kRoleDebug | <what> in the cache's status word and skips
+// the access.  Tiles in shared memory are filled with NaN before anything is copied there, and the launcher fills outputs and scratch
+// with NaN before the launch.  (Tensor memory: fa_ptx.cuh.)  Normal builds contain none of this.
+#ifdef FA_DEBUG
+enum : uint32_t {
+    kDbgEntry = 0x20,   // of a table or a list of pages
+    kDbgCodes,          // codes, scales or bounds outside the cache
+    kDbgRow,            // a row of queries, keys, values, angles or results outside its tensor
+    kDbgTile,           // outside a tile in shared memory
+    kDbgScratch         // outside the call's scratch
+};
+__device__ __forceinline__ bool cache_checked(uint32_t* status, uint32_t what, bool ok) {
+    if (!ok) cache_report(status, kRoleDebug | what);
+    return ok;
+}
+__device__ __forceinline__ void cache_poison(uint32_t base, uint32_t bytes) {   // all threads of the CTA
+    for (uint32_t off = threadIdx.x * 16u; off + 16u <= bytes; off += blockDim.x * 16u)
+        st_shared_v4(base + off, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu);
+    __syncthreads();
+}
+#define FA_CACHE_OK(status, what, cond) cache_checked(status, what, cond)
+#define FA_CACHE_POISON(base, bytes) cache_poison(base, bytes)
+#else
+#define FA_CACHE_OK(status, what, cond) true
+#define FA_CACHE_POISON(base, bytes) do {} while (0)
+#endif
+
 // Tokens that sequence b holds, as far as the table has room for them.
 __device__ __forceinline__ uint32_t cache_length(const CacheView& c, const CacheSeqs& s, uint32_t b) {
     const int32_t n = s.lengths[b];

@@ -63,7 +63,8 @@ struct Angles {
 };
 template <int H>
 __device__ __forceinline__ Angles load_angles(const AppendArgs& p, uint32_t position, uint32_t j) {
-    Angles a;
+    Angles a = {};
+    if (!FA_CACHE_OK(p.c.status, kDbgRow, position < p.positions && 8 * j + 8 <= H / 2)) return a;
     const size_t at = static_cast<size_t>(position) * (H / 2);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(kAppendThreads, 5) fa_cache_append(const Appen
     if (blockIdx.x >= task_ctas) {   // ---- queries: 16 values of up to four heads a thread
         const uint32_t fours = (p.q_heads + kAppendHeads - 1) / kAppendHeads, i = (blockIdx.x - task_ctas) * kAppendThreads + threadIdx.x;
         const uint32_t j = i % kPerToken, four = i / kPerToken % fours, row = i / kPerToken / fours, b = row / p.s.T, t = row - b * p.s.T;
-        if (b >= p.s.B) return;
+        if (b >= p.s.B || !FA_CACHE_OK(p.c.status, kDbgRow, t < p.s.T && four * kAppendHeads < p.q_heads && 16 * j + 16 <= H)) return;
         const uint32_t head = four * kAppendHeads, n = min(kAppendHeads, p.q_heads - head);
         const uint8_t* const from = p.queries + b * p.queries_b + t * p.queries_t + static_cast<int64_t>(head) * (2 * H);
         uint8_t* const out = p.rotated + (static_cast<uint64_t>(row) * p.q_heads + head) * (2 * H) + 16 * j;
@@ -192,7 +193,7 @@ __global__ void __launch_bounds__(kAppendThreads, 5) fa_cache_append(const Appen
     const uint32_t end = p.cos == nullptr ? all : static_cast<uint32_t>(min(static_cast<uint64_t>(all), max(static_cast<uint64_t>(p.positions), first) - first));
     int32_t page = -1;
     const bool fits = held_signed >= 0 && block < p.s.width;
-    if (fits) page = p.s.table[b * p.s.table_stride + block];   // (asked for ahead of the tokens, used behind them)
+    if (fits && FA_CACHE_OK(p.c.status, kDbgEntry, b < p.s.B && block < p.s.width)) page = p.s.table[b * p.s.table_stride + block];   // (asked for ahead of the tokens, used behind them)
     const uint32_t j = tid % kPerToken, sub = tid / kPerToken;
     const uint8_t* rows = is_v ? p.values + b * p.values_b : p.keys + b * p.keys_b;
     const int64_t row_pitch = is_v ? p.values_t : p.keys_t;
@@ -200,7 +201,10 @@ __global__ void __launch_bounds__(kAppendThreads, 5) fa_cache_append(const Appen
     // Tokens are read for the scale and, from the caches, again for the codes: holding them takes registers that are worth more as
     // CTAs (34 us against 39 with four prompts of up to 2048); the first of each thread is asked for ahead of all else.
     RawSixteen raw;
-    auto from = [&](uint32_t slot) { return load_sixteen<H>(rows + static_cast<uint32_t>(first + slot - held) * row_pitch, j); };
+    auto from = [&](uint32_t slot) {
+        if (!FA_CACHE_OK(p.c.status, kDbgRow, b < p.s.B && first + slot >= held && first + slot - held < p.s.T && 16 * j + 16 <= H)) return RawSixteen{};
+        return load_sixteen<H>(rows + static_cast<uint32_t>(first + slot - held) * row_pitch, j);
+    };
     if (begin + sub < end) raw = from(begin + sub);
     const bool known = static_cast<uint32_t>(page) < p.c.n_pages;
     if (tid == 0 && (!known || end < all)) cache_report(p.c.status, fits && end == all ? kCacheBadPage : kCacheBadPosition);
@@ -262,6 +266,7 @@ __global__ void __launch_bounds__(kAppendThreads, 5) fa_cache_append(const Appen
     const float shrink = good ? before * inverse : 0.0f;
     if (grown) {   // the tokens that the page held move to the larger scale
         for (uint32_t slot = sub; slot < begin; slot += kTokens) {
+            if (!FA_CACHE_OK(p.c.status, kDbgCodes, slot < p.c.page && static_cast<uint32_t>(page) < p.c.n_pages)) break;
             uint4* const at = reinterpret_cast<uint4*>(base + slot * pitch + 16 * j);
             uint4 w = *at;
             w.x = good ? moved_codes(w.x, shrink) : 0u;
@@ -278,6 +283,7 @@ __global__ void __launch_bounds__(kAppendThreads, 5) fa_cache_append(const Appen
             w[i] = good ? floats_to_e4m3x2(r.a[2 * i] * inverse, r.a[2 * i + 1] * inverse) : 0u;
             w[4 + i] = good ? floats_to_e4m3x2(r.b[2 * i] * inverse, r.b[2 * i + 1] * inverse) : 0u;
         }
+        if (!FA_CACHE_OK(p.c.status, kDbgCodes, slot < p.c.page && static_cast<uint32_t>(page) < p.c.n_pages && 16 * j + 16 <= H)) return;
         uint8_t* const at = base + slot * pitch + 8 * j;
         *reinterpret_cast<uint2*>(at) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
         *reinterpret_cast<uint2*>(at + H / 2) = make_uint2(w[4] | (w[5] << 16), w[6] | (w[7] << 16));
@@ -305,7 +311,7 @@ __global__ void __launch_bounds__(kAppendThreads, 5) fa_cache_append(const Appen
                 }
             __syncthreads();
         }
-        if (tid < kPerToken) {
+        if (tid < kPerToken && FA_CACHE_OK(p.c.status, kDbgCodes, static_cast<uint32_t>(page) < p.c.n_pages && head < p.c.heads)) {
             uint8_t* const bounds = p.c.bounds + (static_cast<size_t>(page) * p.c.heads + head) * (2 * H);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {

@@ -113,6 +113,15 @@ __device__ __forceinline__ void ld_8_8(const uint8_t* from, uint4& w) {
 // on in shared memory.
 using PlainItem = std::integral_constant<bool, false>;
 using WideItem = std::integral_constant<bool, true>;   // value scales far apart
+#ifdef FA_DEBUG
+// Whether 16 tokens of a page begin `at` units of 16 bytes behind their head's first code.
+__device__ __forceinline__ bool codes_inside(const CacheView& c, bool is_v, uint32_t at) {
+    const uint64_t page = is_v ? c.v_page : c.k_page, token = is_v ? c.v_token : c.k_token, from = static_cast<uint64_t>(at) * 16u;
+    for (uint32_t in_page = 0; in_page < c.page; in_page += 16)
+        if (from >= in_page * token && (page == 0 ? from == in_page * token : (from - in_page * token) % page == 0 && (from - in_page * token) / page < c.n_pages)) return true;
+    return false;
+}
+#endif
 struct PromptItem {
     uint32_t b, head;
     uint32_t t0, first;             // the first row is row `first` of `group` of token t0
@@ -327,6 +336,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
         abort_flag = 0;
         fence_mbar_init();
     }
+#ifdef FA_DEBUG
+    if (tid == 0) g_dbg.tmem_base = 0, g_dbg.tmem_cols = 512, g_dbg.ctl = ctl;
+    for (uint32_t i = tid; i < sizeof(scales) / 4; i += kPromptThreads) reinterpret_cast<uint32_t*>(scales)[i] = 0xFFFFFFFFu;
+    for (uint32_t i = tid; i < sizeof(s_coef) / 4; i += kPromptThreads) reinterpret_cast<uint32_t*>(s_coef)[i] = 0xFFFFFFFFu;
+    FA_CACHE_POISON(base, (2 * C::kQBuffers + C::kSlots) * C::kTileBytes);
+    fence_proxy_async_smem();
+    auto tile_ok = [&](uint32_t at, uint32_t from, uint32_t tiles) { return at >= from && at + 16u <= from + tiles * C::kTileBytes; };
+#endif
     if (warp == 12) {
         tmem_alloc(smem_u32(&tmem_slot), 512);
         tmem_relinquish();
@@ -337,6 +354,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
     grid_dep_wait();
     grid_dep_launch();
     const uint32_t tmem = tmem_slot;
+#ifdef FA_DEBUG
+    if (tid == 0) g_dbg.tmem_base = tmem;
+    __syncthreads();
+#endif
     auto item_wait = [&](uint32_t n) { return mbar_wait(bar(C::ITEM + n % kPromptItems), (n / kPromptItems) & 1u, ctl, kCacheTimeout | C::ITEM); };
     auto item_done = [&](uint32_t n) {
         __syncwarp();
@@ -456,6 +477,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
                 const float f = masked_from == kNoToken || l == 0.0f ? 0.0f : 1.0f / l;
                 prompt_row(p, it.t0, it.first, row, t, h);
                 uint8_t* const to = p.y + ((static_cast<uint64_t>(it.b) * p.s.T + t) * (p.c.heads * p.group) + it.head * p.group + h) * (2 * H);
+                const bool inside = !there || FA_CACHE_OK(p.c.status, kDbgRow, it.b < p.s.B && t < p.s.T && h < p.group && it.head < p.c.heads);
                 constexpr int kCols = H < 32 ? 16 : 32;
 #pragma unroll 1
                 for (int c = 0; c < H; c += kCols) {
@@ -464,7 +486,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
                         tmem_ld<kCols>(tO + c, o);
                         tmem_wait_ld();
                     }
-                    if (there) {
+                    if (there && inside) {
 #pragma unroll
                         for (int e = 0; e < kCols; e += 8) {
                             uint4 w = make_uint4(0, 0, 0, 0);
@@ -478,14 +500,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
             } else {
                 const uint64_t at = static_cast<uint64_t>(slot) * (2 * kPromptTile) + row;
                 constexpr int kCols = H < 32 ? 16 : 32;
-                if (there) p.part_ml[at] = make_float2(masked_from == kNoToken || !any ? -INFINITY : m / shrink, masked_from == kNoToken || !any ? 0.0f : l);
+                const bool inside = FA_CACHE_OK(p.c.status, kDbgScratch, slot < p.items - p.whole);
+                if (there && inside) p.part_ml[at] = make_float2(masked_from == kNoToken || !any ? -INFINITY : m / shrink, masked_from == kNoToken || !any ? 0.0f : l);
                 if (any)
 #pragma unroll 1
                     for (int c = 0; c < H; c += kCols) {
                         float o[kCols];
                         tmem_ld<kCols>(tO + c, o);
                         tmem_wait_ld();
-                        if (there) {
+                        if (there && inside) {
 #pragma unroll
                             for (int e = 0; e < kCols; e += 4) *reinterpret_cast<float4*>(p.part_o + at * H + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                         }
@@ -522,7 +545,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
             uint32_t k_at = 0, v_at = 0;
             auto ask = [&](uint32_t step) {
                 const uint32_t at = (it.step0 + step) * kPromptTile + (lane & 7u) * 16u;
-                wanted = step < it.steps && at < it.farthest;
+                wanted = step < it.steps && at < it.farthest && FA_CACHE_OK(p.c.status, kDbgEntry, it.b < p.s.B && (at >> p.c.page_shift) < p.s.width);
                 entry = wanted ? table[at >> p.c.page_shift] : -1;
             };
             auto look_up = [&] {
@@ -546,6 +569,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
             auto load = [&](uint32_t c, bool is_v) {
                 const uint32_t group_at = __shfl_sync(0xFFFFFFFFu, is_v ? v_at : k_at, (c * kRowsPass + r_in) >> 4);
                 const uint8_t* const from = (is_v ? v_base : k_base) + static_cast<uint64_t>(group_at) * 16u;
+                if (!FA_CACHE_OK(p.c.status, kDbgCodes, it.head < p.c.heads && codes_inside(p.c, is_v != 0, group_at))) return;
                 if constexpr (H == 128) ld_8_8(from, codes[c]);   // eight codes of either operand box
                 else ld_16(from, codes[c]);
             };
@@ -562,7 +586,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
                     const uint32_t r = (pass + f) * kQRows + lt / kQLanes;
                     uint32_t t, h;
                     prompt_row(p, it.t0, it.first, r, t, h);
-                    const bool in = r < it.n_rows && t < it.count;
+                    const bool in = r < it.n_rows && t < it.count && FA_CACHE_OK(p.c.status, kDbgRow, it.b < p.s.B && t < p.s.T && h < p.group && it.head < p.c.heads);
                     ld_zero_16(p.q + (in ? it.b * p.q_b + t * p.q_t + static_cast<int64_t>(it.head * p.group + h) * (2 * H) + 16 * piece : 0), in, in_flight[f]);
                 }
 #pragma unroll
@@ -591,7 +615,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
                         w = make_uint4(x[0], x[1], x[2], x[3]);
                     }
                     constexpr uint32_t kPieces = C::kSwz / 16;   // of a box's row
-                    st_shared_v4(q_addr(k, r >> 7) + (piece / kPieces) * C::kBoxBytes + prompt_swizzled(r & 127u, piece % kPieces, C::kSwz), w.x, w.y, w.z, w.w);
+                    const uint32_t q_to = q_addr(k, r >> 7) + (piece / kPieces) * C::kBoxBytes + prompt_swizzled(r & 127u, piece % kPieces, C::kSwz);
+                    if (FA_CACHE_OK(p.c.status, kDbgTile, tile_ok(q_to, q_addr(k, r >> 7), 1))) st_shared_v4(q_to, w.x, w.y, w.z, w.w);
                     if (piece == 0) s_coef[k & 7u][r] = coef;
                 }
             }
@@ -646,12 +671,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) fa_cache_prompt(const Promp
                         constexpr uint32_t kPieces = C::kSwz / 16;
                         if constexpr (H == 128) {
                             const uint32_t at = to + prompt_swizzled(r, j16, C::kSwz);
-                            st_shared_v4(at, x[0], x[1], x[2], x[3]);
-                            st_shared_v4(at + C::kBoxBytes, x[4], x[5], x[6], x[7]);
+                            if (FA_CACHE_OK(p.c.status, kDbgTile, tile_ok(at, to, 1) && tile_ok(at + C::kBoxBytes, to, 1) && tile_ok(to, ring, NS))) {
+                                st_shared_v4(at, x[0], x[1], x[2], x[3]);
+                                st_shared_v4(at + C::kBoxBytes, x[4], x[5], x[6], x[7]);
+                            }
                         } else {
                             static_assert(H == 128 || H == C::kBoxCols, "one box");
-                            st_shared_v4(to + prompt_swizzled(r, (2 * j16) % kPieces, C::kSwz), x[0], x[1], x[2], x[3]);
-                            st_shared_v4(to + prompt_swizzled(r, (2 * j16 + 1) % kPieces, C::kSwz), x[4], x[5], x[6], x[7]);
+                            const uint32_t lower = to + prompt_swizzled(r, (2 * j16) % kPieces, C::kSwz), upper = to + prompt_swizzled(r, (2 * j16 + 1) % kPieces, C::kSwz);
+                            if (FA_CACHE_OK(p.c.status, kDbgTile, tile_ok(lower, to, 1) && tile_ok(upper, to, 1) && tile_ok(to, ring, NS))) {
+                                st_shared_v4(lower, x[0], x[1], x[2], x[3]);
+                                st_shared_v4(upper, x[4], x[5], x[6], x[7]);
+                            }
                         }
                         // what comes next takes the registers' place
                         load(c, is_v == 0);   // (behind the last step: the first page's, not used)

@@ -50,6 +50,9 @@ struct RowsArgs {
     float* part_o;           // [2 G slots, 16 MT rows, H]
     float2* part_ml;         // [2 G slots, 16 MT rows]
     int2* shares;            // [problems]: first and last CTA
+#ifdef FA_DEBUG
+    uint64_t slots, problems;   // that the scratch has room for
+#endif
 };
 
 template <int H, int MT>
@@ -131,6 +134,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
     float2* const s_ml = reinterpret_cast<float2*>(s_limit + Cfg::kRows);
     uint32_t* const s_share = reinterpret_cast<uint32_t*>(s_ml + kRowsWarps * Cfg::kRows);
     volatile uint32_t* const s_now = s_share + kShareWords + kRowsWarps;
+    FA_CACHE_POISON(smem_u32(smem), Cfg::kSmem);
     grid_dep_wait();
     grid_dep_launch();
     const bool bf16 = p.bf16 != 0;
@@ -198,13 +202,14 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
             if (stage + (lane >> 1) >= n_stages) return;
             uint32_t block = token >> p.c.page_shift;
             if (list != nullptr) {
-                const int32_t chosen = block < p.keep ? list[block] : -1;
+                const bool listed = FA_CACHE_OK(p.c.status, kDbgEntry, s_now[1] < static_cast<uint64_t>(p.s.B) * p.s.T * p.c.heads);
+                const int32_t chosen = listed && block < p.keep ? list[block] : -1;
                 if (chosen < 0) return;   // (not filled)
                 block = static_cast<uint32_t>(chosen);
             }
             const bool inside = block < p.s.width;
             const uint64_t at = (static_cast<uint64_t>(block) << p.c.page_shift) + (token & (p.c.page - 1));
-            if (inside) my_page = table[block];   // (an entry that no token reaches may be anything)
+            if (inside && FA_CACHE_OK(p.c.status, kDbgEntry, s_now[0] < p.s.B)) my_page = table[block];   // (an entry that no token reaches may be anything)
             bool bad = list != nullptr && !inside;
             if (!bad && at < farthest) {
                 bad = static_cast<uint32_t>(my_page) >= p.c.n_pages;
@@ -230,7 +235,8 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
                     const uint64_t ph = page < 0 ? 0u : static_cast<uint32_t>(page);
                     const uint8_t* k0 = k_base + ph * static_cast<uint32_t>(p.c.k_page) + in_page * static_cast<uint32_t>(p.c.k_token);
                     const uint8_t* v0 = v_base + ph * static_cast<uint32_t>(p.c.v_page) + in_page * static_cast<uint32_t>(p.c.v_token);
-                    if (!copies) {
+                    const bool holds = page < 0 || FA_CACHE_OK(p.c.status, kDbgCodes, static_cast<uint32_t>(page) < p.c.n_pages && head < p.c.heads && in_page + 16 <= p.c.page);
+                    if (!copies || !holds || !FA_CACHE_OK(p.c.status, kDbgTile, to + Cfg::kStageBytes <= smem_u32(smem) + Cfg::kRing)) {
                     } else if (page >= 0 && at + 16 <= farthest) {
 #pragma unroll
                         for (uint32_t r = 0; r < 16; r += kRowsAtOnce) {
@@ -263,7 +269,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
         uint32_t w[kHalves * kParts][kPart / 4];
         if (warp < 2 * MT) {
             const uint32_t i = (row0 + q_row) - q_token * p.group;
-            const bool in = q_row < n_rows && q_token < count;
+            const bool in = q_row < n_rows && q_token < count && FA_CACHE_OK(p.c.status, kDbgRow, b < p.s.B && q_token < p.s.T && i < p.group && head < p.c.heads);
             const uint8_t* const q_at = p.q + (in ? b * p.q_b + q_token * p.q_t + static_cast<int64_t>(head * p.group + i) * (2 * H) + 2 * t4 * kKeyBytes : 0);
 #pragma unroll
             for (int x = 0; x < kHalves * kParts; ++x) ld_or_zero<kPart>(q_at + 2 * ((x / kParts) * 64 + (x % kParts) * 8), in, w[x]);
@@ -562,15 +568,17 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
             if (alone) {
                 const uint32_t t = (row0 + r) / p.group, h = head * p.group + (row0 + r) % p.group;
                 const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+                if (!FA_CACHE_OK(p.c.status, kDbgRow, b < p.s.B && t < p.s.T && h < p.c.heads * p.group)) continue;
                 uint8_t* const to = p.y + ((static_cast<uint64_t>(b) * p.s.T + t) * (p.c.heads * p.group) + h) * (2 * H) + 2 * d;
                 *reinterpret_cast<uint32_t*>(to) = pack_16(x.x * f, x.y * f, bf16);
             } else {
                 const uint32_t s_at = s_now[5];
+                if (!FA_CACHE_OK(p.c.status, kDbgScratch, s_at < p.slots)) continue;
                 *reinterpret_cast<float2*>(p.part_o + (static_cast<uint64_t>(s_at) * Cfg::kRows + r) * H + d) = x;
                 if (d == 0) p.part_ml[static_cast<uint64_t>(s_at) * Cfg::kRows + r] = make_float2(top, sum);
             }
         }
-        if (tid == 0 && s_now[2] == 0 && p.min_units != 0) {   // who has a share of the problem, for fa_cache_join
+        if (tid == 0 && s_now[2] == 0 && p.min_units != 0 && FA_CACHE_OK(p.c.status, kDbgScratch, static_cast<uint64_t>(b) * per_seq + s_now[10] < p.problems)) {   // who has a share of the problem, for fa_cache_join
             p.shares[static_cast<uint64_t>(b) * per_seq + s_now[10]] = make_int2(alone ? -1 : static_cast<int>(s_now[5]), static_cast<int>(share_owner(s_share, s_now[4])));
         }
         unit = s_now[6], unit_end = s_now[7], before = s_now[8], b = s_now[9];
@@ -579,6 +587,11 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
     }
 }
 
+#ifdef FA_DEBUG
+__device__ __forceinline__ bool share_inside(const RowsArgs& p, uint64_t index, int2 share) {
+    return index < p.problems && share.y >= 0 && static_cast<uint32_t>(share.x) <= 2u * static_cast<uint32_t>(share.y) + 1u && 2ull * static_cast<uint32_t>(share.y) < p.slots;
+}
+#endif
 // Puts the parts of divided problems together: a CTA per problem and row, a warp per part in turn, several parts in flight.
 constexpr int kJoinWarps = 8;
 template <int H, int MT>
@@ -593,7 +606,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fa_cache_join(const RowsArgs 
     const uint64_t index = blockIdx.x / p.rows;
     const uint32_t r = blockIdx.x % p.rows;
     const int2 share = p.shares[index];
-    if (share.x < 0) return;
+    if (share.x < 0 || !FA_CACHE_OK(p.c.status, kDbgScratch, share_inside(p, index, share))) return;
     const uint32_t per_seq = p.c.heads * p.row_tiles;
     const uint32_t b = static_cast<uint32_t>(index / per_seq), problem = static_cast<uint32_t>(index % per_seq);
     const uint32_t head = problem / p.row_tiles, row = problem % p.row_tiles * p.rows + r;
@@ -671,7 +684,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fa_cache_join_few(const RowsA
     const uint64_t index = at / p.rows;
     if (index >= static_cast<uint64_t>(p.s.B) * per_seq) return;
     const int2 share = p.shares[index];
-    if (share.x < 0) return;
+    if (share.x < 0 || !FA_CACHE_OK(p.c.status, kDbgScratch, share_inside(p, index, share))) return;
     const uint32_t b = static_cast<uint32_t>(index / per_seq), problem = static_cast<uint32_t>(index % per_seq);
     const uint32_t head = problem / p.row_tiles, row = problem % p.row_tiles * p.rows + r;
     if (row >= p.s.T * p.group) return;

@@ -89,7 +89,7 @@ __device__ __forceinline__ void score_pages(const SelectArgs& p, uint32_t b, uin
             for (int u = 0; u < 2; ++u) {
                 const uint32_t r = u * 8 + g;
                 const uint32_t t = many ? t0 : t0 + tile * p.per_tile + r / p.group, i = many ? (turn * p.tiles + tile) * 16 + r : r % p.group;
-                const bool in = t < t_end && (many ? i < p.group : r < p.per_tile * p.group);
+                const bool in = t < t_end && (many ? i < p.group : r < p.per_tile * p.group) && FA_CACHE_OK(p.c.status, kDbgRow, b < p.s.B && t < p.s.T && i < p.group);
                 const uint8_t* const row = p.q + (in ? b * p.q_b + t * p.q_t + static_cast<int64_t>(head * p.group + i) * (2 * H) + 2 * t4 * kBytes : 0);
                 most[u] = 0.0f;
 #pragma unroll
@@ -139,7 +139,7 @@ __device__ __forceinline__ void score_pages(const SelectArgs& p, uint32_t b, uin
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 const uint32_t mine = p0 + 8 * n + g;
-                entry[n] = mine < n_pages ? p.s.table[b * p.s.table_stride + mine] : -1;
+                entry[n] = mine < n_pages && FA_CACHE_OK(p.c.status, kDbgEntry, b < p.s.B && mine < p.s.width) ? p.s.table[b * p.s.table_stride + mine] : -1;
             }
         };
         auto ask_bounds = [&](uint32_t p0) {
@@ -153,8 +153,9 @@ __device__ __forceinline__ void score_pages(const SelectArgs& p, uint32_t b, uin
                 // (a page that is not there: read the first, and never take it for its score)
                 const uint64_t at = static_cast<uint64_t>(page < 0 ? 0 : page) * p.c.heads + head;
                 there[n] = page >= 0;
-                scale[n] = p.c.k_scale[at];   // (nothing may wait for it here)
-                const uint8_t* const from = p.c.bounds + at * (2 * H) + t4 * kBytes;
+                const bool inside = FA_CACHE_OK(p.c.status, kDbgCodes, at < static_cast<uint64_t>(p.c.n_pages) * p.c.heads);
+                scale[n] = p.c.k_scale[inside ? at : 0];   // (nothing may wait for it here)
+                const uint8_t* const from = p.c.bounds + (inside ? at : 0) * (2 * H) + t4 * kBytes;
 #pragma unroll
                 for (int half = 0; half < kHalves; ++half)
 #pragma unroll
@@ -233,7 +234,7 @@ __device__ __forceinline__ void score_pages(const SelectArgs& p, uint32_t b, uin
                         best = x;
                         if (tile + 1 < p.tiles) break;
                     }
-                    if (my_page < n_pages) {
+                    if (my_page < n_pages && FA_CACHE_OK(p.c.status, kDbgScratch, my_page < p.s.width && t < p.s.T && head < p.c.heads)) {
                         const int64_t position = query_position(p.c, p.s, b, t);
                         const int64_t own = position >> p.c.page_shift;
                         uint32_t key = sortable(my_scale == -1.0f ? -INFINITY : __fmul_rn(x, my_scale));
@@ -252,6 +253,7 @@ __device__ __forceinline__ void score_pages(const SelectArgs& p, uint32_t b, uin
 template <int H>
 __global__ void __launch_bounds__(kScoreWarps * 32, kScoreCtas) fa_cache_scores(const SelectArgs p) {
     extern __shared__ __align__(16) uint4 s_frag[];   // [tiles][kSteps][positive, negative part][lane]
+    FA_CACHE_POISON(smem_u32(s_frag), p.tiles * (H / 16) * 2 * 32 * 16);
     __shared__ float s_qs[kScoreTiles][16];
     __shared__ float s_val[kScoreWarps][16][kScorePages + 1];
     grid_dep_wait();
@@ -312,12 +314,15 @@ __global__ void __launch_bounds__(kTakeThreads) fa_cache_take(const SelectArgs p
         return;
     }
     const uint32_t per = (n + kTakeThreads - 1) / kTakeThreads;   // keys of a thread, one behind the other
-    const uint32_t begin = min(n, tid * per), end = min(n, begin + per);
+    const uint32_t begin = min(n, tid * per), end = FA_CACHE_OK(p.c.status, kDbgScratch, n <= p.s.width && (kHeld == 0 || per <= kHeld)) ? min(n, begin + per) : begin;
     uint32_t mine[kHeld > 0 ? kHeld : 1];
     if (kHeld > 0) {
 #pragma unroll
         for (int i = 0; i < kHeld; ++i) mine[i] = begin + i < end ? keys[begin + i] : 0u;
     }
+    auto put = [&](uint32_t place, uint32_t i) {
+        if (FA_CACHE_OK(p.c.status, kDbgRow, place < p.keep && i < p.s.width)) out[place] = static_cast<int32_t>(i);
+    };
     auto each = [&](auto&& f) {
         if (kHeld > 0) {
 #pragma unroll
@@ -393,10 +398,10 @@ __global__ void __launch_bounds__(kTakeThreads) fa_cache_take(const SelectArgs p
     for (uint32_t w = 0; w < warp; ++w) front_above += s_scan[w][0], front_equal += s_scan[w][1];
     each([&](uint32_t i, uint32_t key) {
         if (key > least) {
-            out[front_above + min(front_equal, ties)] = static_cast<int32_t>(i);
+            put(front_above + min(front_equal, ties), i);
             ++front_above;
         } else if (key == least) {
-            if (front_equal < ties) out[front_above + front_equal] = static_cast<int32_t>(i);
+            if (front_equal < ties) put(front_above + front_equal, i);
             ++front_equal;
         }
     });

@@ -182,7 +182,8 @@ __device__ __forceinline__ bool mbar_wait_certain(uint32_t bar, uint32_t parity,
 }
 
 // ----------------------------------------------------------------------------- checked build (-DFA_DEBUG)
-// With -DFA_DEBUG every TMA copy and every tensor-memory access of the kernels checks its operands first:
+// With -DFA_DEBUG every TMA copy and every tensor-memory access of the kernels checks its operands first (for what the key/value cache's
+// kernels check beside that see fa_cache.cuh):
 // the shared-memory side lies inside the CTA's tile area and on a 1024-byte boundary, the innermost
 // coordinate is a multiple of 8 elements (16 bytes) and all coordinates lie inside the tensor, a store does
 // not start at a negative or out-of-range row, a tensor-memory access stays inside the CTA's allocation and
