@@ -186,8 +186,11 @@ RowsPlan plan_rows(uint32_t H, uint32_t heads, uint32_t group, uint32_t page, ui
 template <int H, int MT>
 int launch_rows(Device& d, uint32_t bit, const fa::RowsArgs& a, const RowsPlan& plan, cudaStream_t stream) {
     using Cfg = fa::RowsCfg<H, MT>;
-    const auto kernel = a.bf16 ? &fa::fa_cache_rows<H, MT, false> : &fa::fa_cache_rows<H, MT, true>;
-    int rc = allow_smem(d, bit + (a.bf16 ? 0 : 12), kernel, Cfg::kSmem);
+    const int rest = a.bf16 ? fa::kRestNone : MT == 1 && plan.rows <= 8 ? fa::kRestAbove : fa::kRestApart;
+    const auto kernel = rest == fa::kRestNone    ? &fa::fa_cache_rows<H, MT, fa::kRestNone>
+                        : rest == fa::kRestApart ? &fa::fa_cache_rows<H, MT, fa::kRestApart>
+                                                 : &fa::fa_cache_rows<H, MT, MT == 1 ? fa::kRestAbove : fa::kRestApart>;
+    int rc = allow_smem(d, bit + 8 * static_cast<uint32_t>(rest), kernel, Cfg::kSmem);
     if (rc == FA_B200_OK) rc = launch(kernel, plan.grid, fa::kRowsWarps * 32, Cfg::kSmem, stream, a);
     if (rc != FA_B200_OK || plan.min_units == 0) return rc;
     const uint64_t rows = plan.problems * plan.rows;

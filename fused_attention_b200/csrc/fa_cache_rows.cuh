@@ -115,9 +115,12 @@ __device__ __forceinline__ void ld_codes(uint32_t addr, uint32_t (&w)[kBytes / 4
 
 // kRest: what the weights lose when they are rounded to fp16 is multiplied too.  For results in fp16, whose own rounding is no larger: with
 // it the error is that of the results' rounding alone, without it 1.4 times that; in bf16 it would not show (1.01 times).  All fp16 calls
-// have it, so that how exact a sequence's results are does not depend on what else is in the call.  (64 sequences of 100 to 8192 tokens
-// 111 us, 97 without; one of 301 tokens 9.0 and 8.9.)
-template <int H, int MT, bool kRest>
+// have it, so that how exact a sequence's results are does not depend on what else is in the call.
+//   kRestApart   by a product of its own (64 sequences of 100 to 8192 tokens, 4 rows: 111 us, 97 without)
+//   kRestAbove   by the same product: a problem has eight rows at most then, and the m-tile's upper eight are what the weights of the lower
+//                ones have lost (those calls 96 us; one of 301 tokens 8.2 us, 9.0 with kRestApart)
+enum : int { kRestNone = 0, kRestApart, kRestAbove };
+template <int H, int MT, int kRest>
 __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cache_rows(const RowsArgs p) {
     using Cfg = RowsCfg<H, MT>;
     constexpr int kThreads = kRowsWarps * 32;
@@ -125,6 +128,9 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
     constexpr int kKeyBytes = H >= 64 ? 16 : H / 4;      // that a thread reads of a half
     constexpr int kValueBytes = H / 8;                   // that a thread reads of a value row
     constexpr int kTilesN = H / 8;                       // n-tiles of P V
+    constexpr bool kAbove = kRest == kRestAbove;
+    static_assert(!kAbove || MT == 1, "eight rows");
+    constexpr int kU = kAbove ? 1 : 2, kE = 2 * kU;      // a thread's rows of an m-tile, its scores of an n-tile
     extern __shared__ __align__(128) uint8_t smem[];
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, t4 = lane & 3u;
     const uint32_t ring = smem_u32(smem) + warp * (Cfg::kStages * Cfg::kStageBytes);
@@ -400,7 +406,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
                     // exponents against M, a whole number, so that with scales that are powers of two nothing is rounded but the result
                     float top[2] = {-INFINITY, -INFINITY}, cu[2][2], add[2][2];
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
+                    for (int u = 0; u < kU; ++u) {
                         const float ref = m[mt][u] == -INFINITY ? 0.0f : m[mt][u];
 #pragma unroll
                         for (int h2 = 0; h2 < 2; ++h2) cu[u][h2] = coef[mt][u] * ks[h2], add[u][h2] = vlog[h2] - ref;
@@ -408,20 +414,22 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
 #pragma unroll
                     for (int n = 0; n < 4; ++n)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) s[mt][n][e] = fmaf(s[mt][n][e], cu[e >> 1][n >> 1], add[e >> 1][n >> 1]);
+                        for (int e = 0; e < kE; ++e) s[mt][n][e] = fmaf(s[mt][n][e], cu[e >> 1][n >> 1], add[e >> 1][n >> 1]);
                     if (!whole) {
 #pragma unroll
                         for (int n = 0; n < 4; ++n)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
+                            for (int e = 0; e < kE; ++e) {
                                 const uint32_t pos = at[n >> 1] + (n & 1) * 8 + 2 * t4 + (e & 1);
                                 if (at[n >> 1] == kNoToken || pos >= limit[mt][e >> 1]) s[mt][n][e] = -INFINITY;
                             }
                     }
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) top[0] = max3(top[0], s[mt][n][0], s[mt][n][1]), top[1] = max3(top[1], s[mt][n][2], s[mt][n][3]);
+                    for (int n = 0; n < 4; ++n)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
+                        for (int u = 0; u < kU; ++u) top[u] = max3(top[u], s[mt][n][2 * u], s[mt][n][2 * u + 1]);
+#pragma unroll
+                    for (int u = 0; u < kU; ++u) {
                         top[u] = fmaxf(top[u], __shfl_xor_sync(0xFFFFFFFFu, top[u], 1));
                         top[u] = fmaxf(top[u], __shfl_xor_sync(0xFFFFFFFFu, top[u], 2));
                     }
@@ -430,7 +438,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
                     if (__any_sync(0xFFFFFFFFu, moves[0] || moves[1])) {
                         float f[2], by[2];
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) {
+                        for (int u = 0; u < kU; ++u) {
                             by[u] = moves[u] ? ceilf(top[u]) : 0.0f;
                             f[u] = !moves[u] ? 1.0f : m[mt][u] == -INFINITY ? 0.0f : ex2_approx(-by[u]);
                             if (moves[u]) m[mt][u] = (m[mt][u] == -INFINITY ? 0.0f : m[mt][u]) + by[u];
@@ -439,36 +447,40 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
 #pragma unroll
                         for (int n = 0; n < 4; ++n)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) s[mt][n][e] -= by[e >> 1];
+                            for (int e = 0; e < kE; ++e) s[mt][n][e] -= by[e >> 1];
 #pragma unroll
                         for (int j = 0; j < kTilesN; ++j)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) o[mt][j][e] *= f[e >> 1];
+                            for (int e = 0; e < 4; ++e) o[mt][j][e] *= f[kAbove ? 0 : e >> 1];
                     }
                     if (wide) {
 #pragma unroll
                         for (int n = 0; n < 4; ++n)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) l[mt][e >> 1] += ex2_approx(s[mt][n][e] + (kSumLift - vlog[n >> 1])) * kSumUnlift;
+                            for (int e = 0; e < kE; ++e) l[mt][e >> 1] += ex2_approx(s[mt][n][e] + (kSumLift - vlog[n >> 1])) * kSumUnlift;
                     }
                     float sum[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
+                        for (int e = 0; e < kE; ++e) {
                             s[mt][n][e] = ex2_approx(s[mt][n][e]);
                             sum[n >> 1][e >> 1] += s[mt][n][e];
                         }
                         pf[mt][n][0] = pack_half2(s[mt][n][0], s[mt][n][1]);
-                        pf[mt][n][1] = pack_half2(s[mt][n][2], s[mt][n][3]);
-                        if (kRest) {
+                        if (!kAbove) pf[mt][n][1] = pack_half2(s[mt][n][2], s[mt][n][3]);
+                        if (kAbove) {
+                            const float2 x = unpack_half2(pf[mt][n][0]);
+                            pf[mt][n][1] = pack_half2(s[mt][n][0] - x.x, s[mt][n][1] - x.y);
+                        }
+                        if (kRest == kRestApart) {
                             const float2 x = unpack_half2(pf[mt][n][0]), y = unpack_half2(pf[mt][n][1]);
                             rest[mt][n][0] = pack_half2(s[mt][n][0] - x.x, s[mt][n][1] - x.y);
                             rest[mt][n][1] = pack_half2(s[mt][n][2] - y.x, s[mt][n][3] - y.y);
                         }
                     }
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
+                    for (int u = 0; u < kU; ++u)
 #pragma unroll
                         for (int h2 = 0; h2 < 2; ++h2)   // (a page none of whose tokens the row sees adds nothing, whatever its scale)
                             l[mt][u] += sum[h2][u] == 0.0f || wide ? 0.0f : sum[h2][u] * vinv[h2];
@@ -502,7 +514,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
                             for (int mt = 0; mt < MT; ++mt) {
                                 const uint32_t a[4] = {pf[mt][2 * k16][0], pf[mt][2 * k16][1], pf[mt][2 * k16 + 1][0], pf[mt][2 * k16 + 1][1]};
                                 mma_m16n8k16(o[mt][4 * w + j], a, b0[j], b1[j]);
-                                if (kRest) {
+                                if (kRest == kRestApart) {
                                     const uint32_t r[4] = {rest[mt][2 * k16][0], rest[mt][2 * k16][1], rest[mt][2 * k16 + 1][0], rest[mt][2 * k16 + 1][1]};
                                     mma_m16n8k16(o[mt][4 * w + j], r, b0[j], b1[j]);
                                 }
@@ -534,7 +546,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < kU; ++u) {
                 const uint32_t r = mt * 16 + u * 8 + g;
                 float top = -INFINITY;
 #pragma unroll
@@ -547,7 +559,8 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsCfg<H, MT>::kCtas) fa_cac
                     for (int j = 0; j < kTilesN; j += 2) {
                         const uint32_t d = (2 * t4 + e) * kTilesN + j;
                         float2* const to = reinterpret_cast<float2*>(area + r * H + (d ^ (H >= 64 ? (g & 3u) * 2 : 0u)));
-                        *to = make_float2(o[mt][j][2 * u + e] * f, o[mt][j + 1][2 * u + e] * f);
+                        if (kAbove) *to = make_float2((o[mt][j][e] + o[mt][j][2 + e]) * f, (o[mt][j + 1][e] + o[mt][j + 1][2 + e]) * f);
+                        else *to = make_float2(o[mt][j][2 * u + e] * f, o[mt][j + 1][2 * u + e] * f);
                     }
             }
         __syncthreads();

@@ -21,7 +21,8 @@ def tight(cache, q, table, lengths, **kw):
     return want, bound - (2.0 ** -11 - 2.0 ** -21) * size
 
 
-@pytest.mark.parametrize("H,G,group,T,B,tokens,keep", [(128, 8, 4, 1, 64, 1100, 0), (64, 4, 2, 2, 130, 1200, 0), (32, 2, 8, 3, 100, 2300, 0), (128, 4, 4, 1, 64, 3000, 30)])
+@pytest.mark.parametrize("H,G,group,T,B,tokens,keep", [(128, 8, 4, 1, 64, 1100, 0), (64, 4, 2, 2, 130, 1200, 0), (32, 2, 8, 3, 100, 2300, 0), (128, 4, 4, 1, 64, 3000, 30),
+                                                       (64, 4, 8, 1, 100, 1100, 0), (128, 4, 3, 3, 100, 1100, 0), (16, 4, 16, 1, 100, 1100, 0), (64, 2, 17, 1, 5, 1100, 0), (64, 2, 12, 2, 40, 900, 9)])
 def test_many_sequences_are_as_exact_as_one(H, G, group, T, B, tokens, keep):
     page = 64
     width = -(-tokens // page)
