@@ -11,7 +11,12 @@ program keeps; nothing here reads them on the host, so all calls can be captured
   y = cache_attention(cache, queries, table, lengths, pages=cache_select(cache, queries, table, lengths, keep=64))
 
 Tensors of queries, keys and values are ``[B, T, heads * head_dim]``, fp16 or bf16, as those of ``attention_forward``; they may be
-slices of a larger tensor as long as the last axis is contiguous and every row starts on a 16-byte boundary.  There is no CPU path.
+slices of a larger tensor as long as the last axis is contiguous and every row starts on a 16-byte boundary.  There is no CPU path,
+and there are no gradients: results do not require one, whatever the inputs say.
+
+Tokens are taken back (drafted ones that were not accepted) by lowering ``lengths``.  The pages that they were on keep what they did to
+them until a page's first token is appended anew: a scale that they enlarged, the bits that older tokens of the page lost to it, bounds that
+still cover them, and a scale that is NaN if one of their values was not finite.
 """
 from __future__ import annotations
 
@@ -43,7 +48,7 @@ def _require(cond: bool, what: str) -> None:
 def _calls():
     """(append, select, attention, entries).  A native call answers None for what is not a plain call with every precondition met,
     which then goes through the checks and ctypes below; an int is the status of a launch that failed.  (One token of a short
-    sequence: attention 14.6 us a call and 18.8 through ctypes, with the same kernel.)"""
+    sequence on 301 keys: attention 8.1 us a call and 16.9 through ctypes, with the same kernel; append 5.6 and 25.)"""
     global _native
     if _native is None:
         lib = _lib.load()   # raises when the CUDA library is missing: no fallback
@@ -60,7 +65,7 @@ class KVCache:
                             for NaN)
     ``bounds``              float8_e4m3fn [n_pages, kv_heads, 2, head_dim], contiguous: lowest and highest key code
 
-    The tensors are looked at once, here; they must not be moved or resized afterwards.  ``cache_create`` makes them.
+    No code of a token may be NaN (``cache_append`` writes none): in a value it would reach queries that do not see the token.  The tensors are looked at once, here; they must not be moved or resized afterwards.  ``cache_create`` makes them.
     """
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, bounds: torch.Tensor):
@@ -199,10 +204,12 @@ def cache_select(cache: KVCache, queries: torch.Tensor, table: torch.Tensor, len
     """The ``keep`` pages that each query and key/value head should attend to: int32 [B, T, kv_heads, keep], ascending block
     indices of the sequence, -1 behind the last.
 
-    Among the pages up to the query's own those with the largest bound on any key's product with the query are taken (for
-    query heads that share a key/value head the largest of theirs), the lower page where two are equal; the ``first`` first
+    Among the pages up to the query's own those are taken whose keys, by the page's bounds, may have the largest product with the
+    query (for query heads that share a key/value head the largest of theirs), the lower page where two are equal; the ``first`` first
     and the ``last`` last ones in any case, before all others.  ``queries`` (rotated), ``table``, ``lengths`` and ``counts`` as
-    for ``cache_attention``.  The bounds are rounded to 8 bits for this, and so are the queries.
+    for ``cache_attention``.  Queries are rounded to 8 bits for this and bounds to multiples of four codes, to nearest, so that a score is
+    an estimate of the bound and not one itself.  Of the 64 best of 1000 pages of normal keys by the bounds as they are, 99.6 % are found;
+    with four dimensions 20 times as large as the others, beside which theirs become few multiples, 84 %.
     """
     _require(isinstance(cache, KVCache), "the first argument must be a KVCache")
     _, select, _, entries = _calls()

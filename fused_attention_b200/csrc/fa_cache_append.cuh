@@ -7,10 +7,10 @@
 // (subnormal) codes, since both scales are powers of two: a page that is filled token by token ends as close to its values as
 // one that is filled at once.  A value that is not finite makes the page's scale NaN and its codes zero.
 //
-// Bound by memory for prompts (2 bytes read and 1 written a value; 4 of up to 2048 tokens, 8 heads of 128 with 32 of queries: 25 to 31
-// us, about 3.5 TB/s, since a page's values are read to the end before its first code is written) and by the chain length -> table
-// entry -> old scale -> codes for single tokens, which is why a task is a warp there: B=256 sequences of 8 heads are 4096 tasks
-// (7.8 us; 17.6 with a CTA each).
+// Prompts: 4 of up to 2048 tokens, 8 heads of 128 with 32 of queries, ask for 94 MB and take 25 to 29 us, 3.2 to 3.7 TB/s (73 MB of that
+// reach DRAM in a launch by itself, 30 us); without queries, a third of the bytes, 14.6 us.  What holds either half below the memory's rate
+// has not been found out.  Single tokens are bound by the chain length -> table entry -> old scale -> codes, which is why a task is a
+// warp there: B=256 sequences of 8 heads are 4096 tasks (7.8 us; 17.6 with a CTA each).
 #pragma once
 
 #include "fa_cache.cuh"

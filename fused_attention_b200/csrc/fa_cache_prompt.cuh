@@ -15,14 +15,17 @@
 // Scales.  A step's keys have eight groups of 16 with a scale each for K and V (pages are 16 tokens or more).  As in
 // fa_cache_rows.cuh the exponent of a weight is score * (row's factor * key scale) + log2(value scale) - M, one multiply-add
 // a pair of scores with factors that change from group to group, and the row sum divides the value scale out again (items whose value
-// scales lie far apart, kSpanOfScales, go through a loop of their own that takes an exponential more a score).
+// scales lie far apart, kSpanOfScales, go through a loop of their own that takes an exponential more a score: the two cases below with
+// every other page zeros and the rest values up to 10^5, 564 and 198 us).
 // A page whose scale is NaN (or below zero) becomes keys that are NaN and values that are zero, so that only rows that see it are NaN.
 //
 // Bound by the tensor pipe and the exponentials as fa_fwd_pipelined is (per step and tile 1024 tensor clocks of products at
 // H = 128 and 1024 clocks of exponentials); what is added here is shared-memory traffic, 64 KB a step written by the loading
-// warps beside the 192 KB that the products read.  Measured: a prompt of 4096 tokens on 8000 keys, 32 heads of 128, 390 to 425 us,
-// 57 to 63 % of the products' peak; 16 prompts of 777 tokens, 16 heads of 64, 144 to 149 us.  A step of both tiles takes 4800 clocks, in
-// which the issuing and loading warps wait for the softmax: registers are what it lacks, a row's 128 scores leave few.
+// warps beside the 192 KB that the products read.  Measured: a prompt of 4096 tokens on 8000 keys, 32 heads of 128, 383 to 423 us,
+// 58 to 64 % of the products' peak (the tensor pipe busy 47 % of a launch by itself, 427 us); 16 prompts of 777 tokens, 16 heads of 64,
+// 146 to 151 us.  A step of both tiles takes about 4800 clocks, in which the issuing and loading warps wait for the softmax: registers are
+// what it lacks, a row's 128 scores leave few.  (fa_fwd_pair, whose keys have no scales and come as fp16, takes 2750 to 2800 for a step of
+// as many scores.)
 #pragma once
 
 #include <type_traits>
@@ -178,6 +181,7 @@ __device__ __forceinline__ bool prompt_wide(const PromptArgs& p, uint32_t b, uin
     int least = 255, most = 0;   // biased exponents
 #pragma unroll 2
     for (uint32_t block = (key0 >> p.c.page_shift) + lane; block < blocks; block += 32) {
+        if (!FA_CACHE_OK(p.c.status, kDbgEntry, b < p.s.B && block < p.s.width)) break;
         const uint32_t page = static_cast<uint32_t>(table[block]);
         if (page >= p.c.n_pages) continue;
         const int size = max(__float_as_int(p.c.v_scale[static_cast<uint64_t>(page) * p.c.heads + head]) >> 23, 27);   // (2^-100 at least)
@@ -286,7 +290,7 @@ __device__ __forceinline__ float prompt_top(const float (&s)[kPromptTile], uint3
 // A new reference for a row whose largest exponent is `top`, and the factor for O so far; `l` is multiplied by it.  Beside one of 2^22 and more an
 // exponent would not be known to a fraction, and a weight could exceed fp16: all the row's exponents are then shrunk by a power of
 // two that brings it below.  The largest stays the largest, and exponents of that size differ by whole numbers or not at all, so
-// that hardly anything but the largest counts before and after.
+// that hardly anything but the largest counts before and after (scores that tie beside value scales that differ are not weighed exactly there).
 template <bool kWide>
 __device__ __forceinline__ float prompt_reference(float top, float& m, float& coef, float& shrink, float& l) {
     const float grown = 1.0f / shrink, whole = top * grown;

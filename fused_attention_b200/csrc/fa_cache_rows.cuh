@@ -2,16 +2,16 @@
 //
 // The query heads that share a key/value head, and the sequence's T tokens, are rows of one problem: row t * group + i.  A
 // problem is 16 * MT of these rows of one sequence and key/value head (with a list of pages: the rows of one token).  What
-// bounds it is memory, 2 H bytes a token and head (64 sequences of up to 8192 tokens, 8 heads of 128: 97 us, 523 MB, 5.4 TB/s; 2 of
-// 131000, 4 heads: 55 us with the join, 268 MB), so the work is cut by keys: all problems' units of 128 tokens stand in one row, with
+// bounds it is memory, 2 H bytes a token and head (64 sequences of up to 8192 tokens, 8 heads of 128: 96 us, 523 MB, 5.4 TB/s; 2 of
+// 131000, 4 heads: 56 us with the join, 268 MB), so the work is cut by keys: all problems' units of 128 tokens stand in one row, with
 // kRowsSetup units in front of each problem's, CTA c of G takes units [c W / G, (c + 1) W / G) of the W there are, whatever problems
 // they belong to, and a problem that several CTAs share is put together by fa_cache_join or fa_cache_join_few.  Lengths are only
-// known on the device, so every CTA adds them up itself.  With 25 rows (16 sequences of up to 4001 tokens: 36 us, 2.1 TB/s) the
+// known on the device, so every CTA adds them up itself.  With 25 rows (16 sequences of up to 4001 tokens: 38 us, 2.0 TB/s) the
 // products and exponentials count beside the reading.
 //
 // Inside a CTA each warp takes 32 tokens of a unit, through a ring of its own in shared memory that cp.async fills: nobody
-// waits for another warp before the end of the problem.  Both products are mma.sync m16n8k16 in fp16 (tcgen05 would need 128
-// rows to be worth its tile): a thread reads the codes of its own fragment straight from the ring, the order of the dimensions
+// waits for another warp before the end of the problem.  Both products are mma.sync m16n8k16 in fp16 (with these rows a tcgen05 tile of
+// 128 would be mostly empty; one with the keys as its rows and these as its columns has not been tried): a thread reads the codes of its own fragment straight from the ring, the order of the dimensions
 // in Q K^T and of the tokens in P V being chosen so that they are 16 contiguous bytes, and turns them into fp16, which is exact.
 //
 // Scales: the key scale is multiplied into the fp32 scores.  The value scale goes into the exponent: w = 2^(s + log2 scale - M)

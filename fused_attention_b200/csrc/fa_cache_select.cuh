@@ -8,9 +8,10 @@
 // where q8 <= 0, so the sum is two matrix products, of the positive part of q8 with hi8 and of the negative part with lo8:
 // mma.sync m16n8k16 on fp16, which holds these numbers exactly.
 //
-// fa_cache_scores reads 2 H + 4 bytes a page and head: 84 MB in 32 us with 32 sequences of 30000 to 131072 tokens, 2.6 TB/s.  Reading
-// alone is not what bounds it: each value of the bounds is unpacked, rounded to 8 bits and packed again (about two instructions a
-// value), with three CTAs an SM, as many as its registers allow, to hide the way to memory.  The pages of all sequences are dealt
+// fa_cache_scores reads 2 H + 4 bytes a page and head: with 32 sequences of 30000 to 131072 tokens 95 MB of DRAM in 37 us, 2.6 TB/s, in a
+// launch by itself (the whole call, whose launches overlap, 37 us too).  Neither reading nor the products are near their limits:
+// unpacking and rounding the bounds takes about two instructions a value, some 5 us.  What it lacks is reads on their way: three CTAs
+// an SM, as many as its registers allow, hold one turn of bounds a warp.  The pages of all sequences are dealt
 // out to the CTAs in equal shares; a warp takes 16 pages at a time, whose bounds it asks for a turn ahead, and multiplies them by
 // all of the sequence's queries, which are rounded once a CTA; queries of several tokens share tiles of 16 rows.
 // fa_cache_take then finds the `keep` highest of a query's scores.

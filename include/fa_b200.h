@@ -348,7 +348,8 @@ typedef struct fa_b200_sequences {
  * A page's scale is the smallest power of two, 2^-100 at least, with which the largest magnitude of its tokens is 448 or less;
  * a page that held tokens keeps a larger one, and where its scale grows its old codes are moved to the new one (exact but for
  * subnormal codes).  Codes are rounded to nearest even.  A value that is not finite makes the scale of its page and head NaN and
- * the codes zero.  Sequences of one call must not append to the same page.
+ * the codes zero.  Sequences of one call must not append to the same page.  Where tokens are taken back by lowering a length, their
+ * page keeps the scale (a NaN too), the rounding of older tokens to it and the bounds until its first token is appended anew.
  */
 int fa_b200_cache_append(const fa_b200_cache* cache, const fa_b200_sequences* sequences, const void* keys, int64_t keys_batch_stride,
                          int64_t keys_token_stride, const void* values, int64_t values_batch_stride, int64_t values_token_stride,
@@ -376,7 +377,8 @@ int fa_b200_cache_select(const fa_b200_cache* cache, const fa_b200_sequences* se
  * ([B, T, kv_heads, keep], as fa_b200_cache_select writes them, -1 for nothing) only those blocks.  y is contiguous, of the
  * queries' type; a query that sees no key, or that its sequence does not have, gets zeros.  Scores, weights and sums are held in
  * fp32; the weights are rounded to fp16 for the product with V.  In fp16 calls with `pages`, or with fewer than 64 rows (T * q_heads /
- * kv_heads), what that rounding takes away is multiplied as well, so that an error is little more than the rounding of y.  Scratch: as fa_b200_cache_attention_scratch says, on a 16-byte
+ * kv_heads), what that rounding takes away is multiplied as well, so that an error is little more than the rounding of y.
+ * Among scores (times log2 e) of 2^22 and more, keys that tie on pages of different value scales are not weighed exactly.  Scratch: as fa_b200_cache_attention_scratch says, on a 16-byte
  * boundary.
  */
 int fa_b200_cache_attention(const fa_b200_cache* cache, const fa_b200_sequences* sequences, const void* queries, int64_t queries_batch_stride,
