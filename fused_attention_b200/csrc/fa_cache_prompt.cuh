@@ -16,7 +16,7 @@
 // fa_cache_rows.cuh the exponent of a weight is score * (row's factor * key scale) + log2(value scale) - M, one multiply-add
 // a pair of scores with factors that change from group to group, and the row sum divides the value scale out again (items whose value
 // scales lie far apart, kSpanOfScales, go through a loop of their own that takes an exponential more a score: the two cases below with
-// every other page zeros and the rest values up to 10^5, 564 and 198 us).
+// every other page zeros and the rest values up to 7 * 10^6, 564 and 198 us).
 // A page whose scale is NaN (or below zero) becomes keys that are NaN and values that are zero, so that only rows that see it are NaN.
 //
 // Bound by the tensor pipe and the exponentials as fa_fwd_pipelined is (per step and tile 1024 tensor clocks of products at

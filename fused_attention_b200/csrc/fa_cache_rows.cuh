@@ -11,8 +11,9 @@
 //
 // Inside a CTA each warp takes 32 tokens of a unit, through a ring of its own in shared memory that cp.async fills: nobody
 // waits for another warp before the end of the problem.  Both products are mma.sync m16n8k16 in fp16 (with these rows a tcgen05 tile of
-// 128 would be mostly empty; one with the keys as its rows and these as its columns has not been tried): a thread reads the codes of its own fragment straight from the ring, the order of the dimensions
-// in Q K^T and of the tokens in P V being chosen so that they are 16 contiguous bytes, and turns them into fp16, which is exact.
+// 128 would be mostly empty; one with the keys as its rows and these as its columns has not been tried): a thread reads the codes of
+// its own fragment straight from the ring, the order of the dimensions in Q K^T and of the tokens in P V being chosen so that they are 16
+// contiguous bytes, and turns them into fp16, which is exact.
 //
 // Scales: the key scale is multiplied into the fp32 scores.  The value scale goes into the exponent: w = 2^(s + log2 scale - M)
 // with M the running maximum of just that exponent, so that P needs no second rounding and cannot leave fp16, whatever the

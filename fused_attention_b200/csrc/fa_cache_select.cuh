@@ -10,8 +10,8 @@
 //
 // fa_cache_scores reads 2 H + 4 bytes a page and head: with 32 sequences of 30000 to 131072 tokens 95 MB of DRAM in 37 us, 2.6 TB/s, in a
 // launch by itself (the whole call, whose launches overlap, 37 us too).  Neither reading nor the products are near their limits:
-// unpacking and rounding the bounds takes about two instructions a value, some 5 us.  What it lacks is reads on their way: three CTAs
-// an SM, as many as its registers allow, hold one turn of bounds a warp.  The pages of all sequences are dealt
+// unpacking and rounding the bounds takes about two instructions a value, some 5 us.  What is left is the way from memory: three CTAs an
+// SM, as many as its registers allow, have one turn of bounds a warp on it (a longer queue has not been tried).  The pages of all sequences are dealt
 // out to the CTAs in equal shares; a warp takes 16 pages at a time, whose bounds it asks for a turn ahead, and multiplies them by
 // all of the sequence's queries, which are rounded once a CTA; queries of several tokens share tiles of 16 rows.
 // fa_cache_take then finds the `keep` highest of a query's scores.
