@@ -33,6 +33,13 @@ EXPORTED_SYMBOLS = (
     "fa_b200_cache_select",
     "fa_b200_cache_attention",
     "fa_b200_cache_attention_scratch",
+    "fa_b200_cache_copy",
+    "fa_b200_pages_fork",
+    "fa_b200_pages_reserve",
+    "fa_b200_pages_compact",
+    "fa_b200_latent_append",
+    "fa_b200_latent_attention",
+    "fa_b200_latent_attention_scratch",
 )
 
 # Status codes and flags, mirrored from include/fa_b200.h.
@@ -76,6 +83,24 @@ class Sequences(ctypes.Structure):
     """``fa_b200_sequences`` of include/fa_b200.h."""
     _fields_ = [(n, ctypes.c_void_p) for n in ("table", "lengths", "counts")] + [("table_stride", ctypes.c_int64)] + [
         (n, ctypes.c_uint32) for n in ("table_width", "B", "T")]
+
+
+class Pages(ctypes.Structure):
+    """``fa_b200_pages`` of include/fa_b200.h."""
+    _fields_ = [("refs", ctypes.c_void_p), ("status", ctypes.c_void_p), ("n_pages", ctypes.c_uint32)]
+
+
+class CopyArea(ctypes.Structure):
+    """``fa_b200_copy_area`` of include/fa_b200.h."""
+    _fields_ = [("base", ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in ("page_stride", "stride0", "stride1")] + [
+        (n, ctypes.c_uint32) for n in ("n0", "n1", "row_bytes")]
+
+
+class LatentCache(ctypes.Structure):
+    """``fa_b200_latent_cache`` of include/fa_b200.h."""
+    _fields_ = [("data", ctypes.c_void_p), ("status", ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in ("page_stride", "token_stride")] + [
+        (n, ctypes.c_uint32) for n in ("n_pages", "page_size", "latent_dim", "rope_dim")]
+
 
 _lock = threading.Lock()
 _lib = None
@@ -139,6 +164,22 @@ def load() -> ctypes.CDLL:
         lib.fa_b200_cache_attention.argtypes = [cache, seqs] + rows + [u32, u32, vp, u32, u32, vp, vp, u64, i32, vp]
         lib.fa_b200_cache_attention_scratch.restype = i32
         lib.fa_b200_cache_attention_scratch.argtypes = 8 * [u32] + [i32, ctypes.POINTER(u64)]
+        pages, heads3 = ctypes.POINTER(Pages), [vp, i64, i64, i64]
+        lib.fa_b200_cache_copy.restype = i32
+        lib.fa_b200_cache_copy.argtypes = [ctypes.POINTER(CopyArea), u32, u32, vp, vp, u32, vp, i32, vp]
+        lib.fa_b200_pages_fork.restype = i32
+        lib.fa_b200_pages_fork.argtypes = [pages, vp, i64, u32, u32, vp, vp, i32, vp]
+        lib.fa_b200_pages_reserve.restype = i32
+        lib.fa_b200_pages_reserve.argtypes = [pages, vp, i64, u32, u32, vp, vp, u32, u32, vp, vp, vp, vp, u64, i32, vp]
+        lib.fa_b200_pages_compact.restype = i32
+        lib.fa_b200_pages_compact.argtypes = [pages, vp, i64, u32, u32, vp, vp, vp, vp, vp, u64, i32, vp]
+        latent = ctypes.POINTER(LatentCache)
+        lib.fa_b200_latent_append.restype = i32
+        lib.fa_b200_latent_append.argtypes = [latent, seqs] + 2 * rows + heads3 + [u32, vp, vp, vp, vp, u32, u32, u32, i32, vp]
+        lib.fa_b200_latent_attention.restype = i32
+        lib.fa_b200_latent_attention.argtypes = [latent, seqs] + 2 * heads3 + [u32, ctypes.c_float, u32, u32, vp, vp, u64, i32, vp]
+        lib.fa_b200_latent_attention_scratch.restype = i32
+        lib.fa_b200_latent_attention_scratch.argtypes = 6 * [u32] + [i32, ctypes.POINTER(u64)]
         # for the extension module's calls
         lib.cache_entries = tuple(ctypes.cast(f, vp).value for f in (lib.fa_b200_cache_append, lib.fa_b200_cache_select, lib.fa_b200_cache_attention,
                                                                      lib.fa_b200_cache_attention_scratch))

@@ -53,20 +53,34 @@ def lib_sources() -> list[str]:
         os.path.join(ROOT, "include", "fa_b200.h")]
 
 
-def cache_sources() -> list[str]:
-    return [os.path.join(CSRC, f) for f in ("fa_cache.cu", "fa_cache.cuh", "fa_cache_append.cuh", "fa_cache_prompt.cuh", "fa_cache_rows.cuh", "fa_cache_select.cuh",
-                                            "fa_ptx.cuh")] + [os.path.join(ROOT, "include", "fa_b200.h")]
+# Source files of the caches' part and the headers that each includes: compiled on their own, once for the checked library
+# (-DFA_DEBUG) and once for all others.
+CACHE_PARTS = {
+    "fa_cache": ("fa_cache.cuh", "fa_cache_append.cuh", "fa_cache_prompt.cuh", "fa_cache_rows.cuh", "fa_cache_select.cuh", "fa_host.cuh", "fa_ptx.cuh"),
+    "fa_latent": ("fa_cache.cuh", "fa_latent.cuh", "fa_latent_rows.cuh", "fa_host.cuh", "fa_ptx.cuh"),
+    "fa_pages": ("fa_cache.cuh", "fa_pages.cuh", "fa_host.cuh", "fa_ptx.cuh"),
+}
 
 
-def build_cache_object(force: bool = False, verbose: bool = False, debug: bool = False) -> str:
-    """Compile csrc/fa_cache.cu, the key/value cache's part: once for the checked library (-DFA_DEBUG), once for all others."""
-    out = os.path.join(LIBDIR, "fa_cache_debug.o" if debug else "fa_cache.o")
-    if force or _stale(out, cache_sources()):
-        os.makedirs(LIBDIR, exist_ok=True)
-        flags = [f for f in NVCC_FLAGS if f != "-shared"] + (["-DFA_DEBUG"] if debug else [])
-        subprocess.run([_nvcc(), *flags, "-I", os.path.join(ROOT, "include"), "-I", CSRC, *(["-Xptxas", "-v"] if verbose else []),
-                        "-c", "-o", out, os.path.join(CSRC, "fa_cache.cu")], check=True)
-    return out
+def cache_sources(part: str = "fa_cache") -> list[str]:
+    return [os.path.join(CSRC, f) for f in (part + ".cu",) + CACHE_PARTS[part]] + [os.path.join(ROOT, "include", "fa_b200.h")]
+
+
+def build_cache_objects(force: bool = False, verbose: bool = False, debug: bool = False) -> list[str]:
+    """Compile the parts that are stale, side by side."""
+    os.makedirs(LIBDIR, exist_ok=True)
+    flags = [f for f in NVCC_FLAGS if f != "-shared"] + (["-DFA_DEBUG"] if debug else []) + (["-Xptxas", "-v"] if verbose else [])
+    outs, running = [], []
+    for part in CACHE_PARTS:
+        out = os.path.join(LIBDIR, part + ("_debug.o" if debug else ".o"))
+        outs.append(out)
+        if force or _stale(out, cache_sources(part)):
+            cmd = [_nvcc(), *flags, "-I", os.path.join(ROOT, "include"), "-I", CSRC, "-c", "-o", out, os.path.join(CSRC, part + ".cu")]
+            running.append((cmd, subprocess.Popen(cmd)))
+    failed = [cmd for cmd, process in running if process.wait() != 0]
+    if failed:
+        raise subprocess.CalledProcessError(1, failed[0])
+    return outs
 
 
 def build_lib(force: bool = False, verbose: bool = False, debug: bool = False, cycles: bool = False,
@@ -81,8 +95,8 @@ def build_lib(force: bool = False, verbose: bool = False, debug: bool = False, c
     the kernel on pairs of CTAs also stamps the events of every key step (cycles.py --timeline)."""
     os.makedirs(LIBDIR, exist_ok=True)
     out = DEBUG_LIB if debug else (TIMELINE_LIB if timeline else (CYCLES_LIB if cycles else LIB))
-    cache = build_cache_object(force=force and out in (LIB, DEBUG_LIB), verbose=verbose, debug=debug)
-    if not force and not _stale(out, lib_sources() + [cache]):
+    cache = build_cache_objects(force=force and out in (LIB, DEBUG_LIB), verbose=verbose, debug=debug)
+    if not force and not _stale(out, lib_sources() + cache):
         return out
     cmd = [_nvcc(), *NVCC_FLAGS, "-I", os.path.join(ROOT, "include"), "-I", CSRC]
     if debug:
@@ -93,7 +107,7 @@ def build_lib(force: bool = False, verbose: bool = False, debug: bool = False, c
         cmd += ["-DFA_CYCLES"]
     if verbose:
         cmd += ["-Xptxas", "-v"]
-    cmd += ["-o", out, os.path.join(CSRC, "fa_b200.cu"), cache]
+    cmd += ["-o", out, os.path.join(CSRC, "fa_b200.cu"), *cache]
     subprocess.run(cmd, check=True)
     return out
 

@@ -95,6 +95,7 @@ class KVCache:
         self._handle = _lib.Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), bounds.data_ptr(), self._status.data_ptr(),
                                   *k.stride()[:3], *v.stride()[:3], n, heads, page, H)
         self._address = ctypes.addressof(self._handle)
+        self._copy_areas = None   # (pages.py)
         # (pages on top of one another can be read, as those of a stand-in for a cache, but not written)
         self._writable = all(t.stride(i) > 0 or t.shape[i] == 1 for t in (k, v) for i in range(3))
 

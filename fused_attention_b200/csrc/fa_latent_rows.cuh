@@ -1,0 +1,709 @@
+// Attention over the cache of latent vectors, the absorbed form: queries that have been multiplied into the latent space.
+//
+//   s = scale * (q_latent . c + q_rope . r),  p = softmax(s),  y = sum of p c        for every head, over the same rows (c, r)
+//
+// Rows of the problem are the query heads of a sequence's tokens (row t * heads + h); a group is N of them (16, 32 or 64) of one
+// sequence.  The keys of all sequences, in tiles of 64, are dealt out evenly to `parts` CTAs a group, so that a sequence may be divided:
+// its parts leave numerators, maxima and sums in scratch, which fa_latent_join puts together.
+//
+// Both products are tcgen05 MMAs on the same tile in shared memory.  Scores are S[64 rows, 64 keys] = Q K^T with the rows as M; the result
+// is kept transposed, Y^T[128 dimensions, N] += C^T P^T, dimensions as M and rows as N: four such tiles hold 512 dimensions in 4 N
+// columns of tensor memory, where Y[128 rows, 512] would need all 512 columns and leave none for the scores; and of a group of 16 rows
+// only the scores (M = 64) cost more than 16 rows would have to.  256 threads:
+//
+//   warps 0-3  softmax: a warp 16 rows, four threads a row (tcgen05.ld.16x256b hands out scores that way); P into shared memory; at the
+//              end of a segment (a sequence's tiles in this CTA) the division and Y, a thread a dimension
+//   warp 4     fetches tiles by TMA: 64 keys of 128 dimensions a slot of one ring, of the rotary part a slot of another
+//   warp 5     issues the MMAs: the next tile's scores as its slots arrive, this tile's P as it is ready, whichever is first
+//   warps 6-7  queries into shared memory, a segment ahead
+//
+// What must not happen: a key that a row does not see reaching it, as 0 * NaN.  Tiles that some row of the group sees in part only (the
+// last ones of a sequence) are gone over in shared memory between the two products: keys behind the last that any row sees become zeros;
+// a key that some rows see and that holds an infinity or a NaN becomes zeros too, and rows that see it get a weight that is NaN.
+#pragma once
+
+#include <cuda.h>
+
+#include "fa_latent.cuh"
+
+namespace fa {
+
+constexpr int kLatentThreads = 256;
+constexpr uint32_t kLatentTile = 64;
+constexpr uint32_t kLatentSlot = kLatentTile * 128;   // bytes of 64 keys by 64 dimensions
+constexpr float kLatentSlack = 8.0f;                  // the reference moves when an exponent exceeds it by more: weights stay below 2^8
+constexpr uint32_t kSeesAll = 0xFFFFFFFFu;
+
+struct LatentRowsArgs {
+    LatentView c;
+    CacheSeqs s;
+    const uint8_t* q_latent;
+    const uint8_t* q_rope;
+    uint8_t* y;              // [B, T, heads, latent] contiguous
+    int64_t ql_b, ql_t, ql_h, qr_b, qr_t, qr_h;   // strides in bytes
+    uint32_t heads, rows, groups, group_rows;     // rows: T * heads, in `groups` of group_rows (the last may have fewer)
+    uint32_t parts, least;                        // CTAs a group; tiles that one has at least
+    uint32_t causal, bf16;
+    float scale_log2;        // scale * log2(e)
+    float* part_o;           // [parts * groups * 2, N, latent]
+    float2* part_ml;         // [parts * groups * 2, N]
+    int2* shares;            // [B]: first and last part of a sequence
+};
+
+template <int LC, int N>
+struct LatentCfg {
+    static constexpr int kPairs = LC / 2;                     // of 64-dimension chunks: slots of a tile
+    static constexpr int kPairSlots = LC == 8 ? 8 : LC == 4 ? 9 : 8, kRopeSlots = LC == 8 ? 2 : LC == 4 ? 4 : 8;
+    static constexpr int kPBuffers = N == 64 ? 1 : 2;
+    static constexpr uint32_t kQBytes = (LC + 1) * kLatentSlot, kPBytes = N * 128;
+    static constexpr uint32_t kOffPair = kQBytes, kOffRope = kOffPair + kPairSlots * 2 * kLatentSlot, kOffP = kOffRope + kRopeSlots * kLatentSlot;
+    static constexpr uint32_t kTiles = kOffP + kPBuffers * kPBytes;
+    static constexpr int kSmemBytes = kTiles + 1024;
+    static constexpr uint32_t kColS = kPairs * N <= 256 ? 256 : 512, kCols = 512;   // scores of even tiles at kColS, of odd ones 64 behind
+    static_assert(kPairs * N <= 256, "tensor memory");
+    // barriers
+    static constexpr int FULL = 0, EMPTY = FULL + kPairSlots, RFULL = EMPTY + kPairSlots, REMPTY = RFULL + kRopeSlots, QFULL = REMPTY + kRopeSlots, QEMPTY = QFULL + 1,
+                         S = QEMPTY + 1, P = S + 2, PV = P + 2, FINAL = PV + 2, kBarriers = FINAL + 1;
+};
+
+// Instruction descriptors (see make_idesc_f16): fp16 or bf16 operands, fp32 sums.
+__device__ __forceinline__ uint32_t idesc_16bit(uint32_t m, uint32_t n, bool a_mn, bool b_mn, bool bf16) {
+    return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+// 16 lanes x 64 columns: thread t receives of row t / 4 (v[4 j], v[4 j + 1]) and of row t / 4 + 8 (v[4 j + 2], v[4 j + 3]) columns 8 j + 2 (t % 4) and the next.
+__device__ __forceinline__ void tmem_ld_16x64(uint32_t taddr, float (&v)[32]) {
+    FA_DBG_TMEM(taddr, 64u);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]),
+          "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]),
+          "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// Of warps 0-3: all there, and whether any thread says so.
+__device__ __forceinline__ bool softmax_any(bool x) {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"(static_cast<uint32_t>(x)) : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void softmax_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
+
+// What rows see.  A sequence holds `held` tokens, of the call's T it has `count`, the last of those that it holds.
+struct LatentSeq {
+    uint32_t held, count;
+};
+__device__ __forceinline__ LatentSeq latent_seq(const LatentRowsArgs& p, uint32_t b) {
+    const CacheView c = plain_view(p.c);
+    return LatentSeq{cache_length(c, p.s, b), cache_count(p.s, b)};
+}
+// Keys [0, ...) that token t sees; 0 also where the sequence does not have it.
+__device__ __forceinline__ uint32_t latent_limit(const LatentRowsArgs& p, const LatentSeq& q, uint32_t t) {
+    if (t >= q.count) return 0;
+    if (!p.causal) return q.held;
+    return q.held + t >= q.count ? min(q.held, q.held + t - q.count + 1u) : 0u;
+}
+// Keys that some row of a group sees (its last token's, of those that the sequence has).
+__device__ __forceinline__ uint32_t latent_farthest(const LatentRowsArgs& p, const LatentSeq& q, uint32_t group) {
+    const uint32_t row0 = group * p.group_rows, t_first = row0 / p.heads, t_last = (min(p.rows, row0 + p.group_rows) - 1u) / p.heads;
+    if (t_first >= q.count) return 0;
+    return latent_limit(p, q, min(t_last, q.count - 1u));
+}
+__device__ __forceinline__ uint32_t latent_units(const LatentRowsArgs& p, uint32_t b) {
+    const LatentSeq q = latent_seq(p, b);
+    return q.count == 0 ? 0u : (q.held + kLatentTile - 1u) / kLatentTile;
+}
+
+// A CTA's way through its tiles, segment by segment.  All lanes of a warp.
+struct LatentWalk {
+    uint32_t unit, unit_end, b, before;   // next tile, end, its sequence, tiles of the sequences in front of that
+    uint32_t each, more;
+    // the segment at hand: tiles [t0, t1) of sequence `seq`, of which the group sees [t0, end)
+    uint32_t seq, t0, t1, end, farthest, first_unit, units;
+    bool whole, begins;                   // all of the sequence's tiles; its first among them
+    LatentSeq q;
+};
+__device__ __forceinline__ bool latent_start(const LatentRowsArgs& p, uint32_t part, LatentWalk& w) {
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t total = 0;
+    for (uint32_t b = lane; b < p.s.B; b += 32) total += latent_units(p, b);
+    total = __reduce_add_sync(0xFFFFFFFFu, total);
+    const uint32_t parts = min(p.parts, (total + p.least - 1u) / p.least);
+    if (part >= parts) return false;
+    w.each = total / parts, w.more = total - w.each * parts;
+    w.unit = part * w.each + min(part, w.more);
+    w.unit_end = (part + 1u) * w.each + min(part + 1u, w.more);
+    w.before = 0, w.b = 0;
+    for (uint32_t b0 = 0; b0 < p.s.B; b0 += 32) {
+        const uint32_t mine = b0 + lane < p.s.B ? latent_units(p, b0 + lane) : 0u;
+        uint32_t upto = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+            if (lane >= d) upto += x;
+        }
+        const uint32_t behind = __ballot_sync(0xFFFFFFFFu, w.before + upto > w.unit);
+        if (behind != 0) {
+            const uint32_t at = __ffs(behind) - 1;
+            w.b = b0 + at;
+            w.before += __shfl_sync(0xFFFFFFFFu, upto - mine, at);
+            break;
+        }
+        w.before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+    }
+    return true;
+}
+__device__ __forceinline__ uint32_t latent_owner(const LatentWalk& w, uint32_t unit) {
+    const uint32_t longer = w.more * (w.each + 1u);
+    return unit < longer ? unit / (w.each + 1u) : w.more + (unit - longer) / w.each;
+}
+// False: none is left.
+__device__ __forceinline__ bool latent_next(const LatentRowsArgs& p, uint32_t group, LatentWalk& w) {
+    while (w.unit < w.unit_end) {
+        const LatentSeq q = latent_seq(p, w.b);
+        const uint32_t units = q.count == 0 ? 0u : (q.held + kLatentTile - 1u) / kLatentTile;
+        if (units == 0) {
+            ++w.b;
+            continue;
+        }
+        w.q = q, w.seq = w.b, w.first_unit = w.before, w.units = units;
+        w.t0 = w.unit - w.before;
+        w.t1 = min(units, w.unit_end - w.before);
+        w.begins = w.t0 == 0, w.whole = w.begins && w.t1 == units;
+        w.farthest = latent_farthest(p, q, group);
+        w.end = max(w.t0, min(w.t1, (w.farthest + kLatentTile - 1u) / kLatentTile));
+        w.unit = w.before + w.t1;
+        if (w.t1 == units) w.before += units, ++w.b;
+        return true;
+    }
+    return false;
+}
+
+// 16 bytes of eight 16-bit values: whether one is an infinity or a NaN.
+__device__ __forceinline__ bool not_finite(const uint32_t (&w)[4], bool bf16) {
+    const uint32_t mask = bf16 ? 0x7F80u : 0x7C00u;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bad |= (w[i] & mask) == mask || (w[i] >> 16 & mask) == mask;
+    return bad;
+}
+
+template <int LC, int N>
+__global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid_constant__ CUtensorMap map, const LatentRowsArgs p) {
+    using C = LatentCfg<LC, N>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[C::kBarriers];
+    __shared__ float s_alpha[2][64], s_l[64], s_m[64];
+    __shared__ uint32_t s_absent[4];         // of tile g in entry g % 4: its 16-key groups without a page
+    __shared__ uint32_t s_bad[2][2];         // of the partly seen tile n in entry n % 2: keys that hold no finite numbers
+    __shared__ uint32_t tmem_slot, abort_flag;
+
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t bar0 = smem_u32(bars);
+    auto bar = [&](int i) { return bar0 + 8u * i; };
+    auto pair_addr = [&](uint32_t n) { return base + C::kOffPair + (n % C::kPairSlots) * (2 * kLatentSlot); };
+    auto rope_addr = [&](uint32_t n) { return base + C::kOffRope + (n % C::kRopeSlots) * kLatentSlot; };
+    auto p_addr = [&](uint32_t g) { return base + C::kOffP + (g % C::kPBuffers) * C::kPBytes; };
+    const WaitCtl ctl{p.c.status, &abort_flag, kWaitCapCycles, nullptr, 0};
+    const uint32_t group = blockIdx.x % p.groups, part = blockIdx.x / p.groups;
+    const uint32_t row0 = group * p.group_rows, n_rows = min(p.group_rows, p.rows - row0);
+    const bool bf16 = p.bf16 != 0;
+
+    if (tid == 0) {
+        for (int i = 0; i < C::kBarriers; ++i) mbar_init(bar(i), i == C::QFULL ? 64u : i >= C::P && i < C::PV ? 4u : 1u);
+        abort_flag = 0;
+        fence_mbar_init();
+        prefetch_tensormap(&map);
+    }
+    if (tid < 4) s_bad[tid >> 1][tid & 1] = 0;
+#ifdef FA_DEBUG
+    if (tid == 0) {
+        g_dbg.smem_lo = base, g_dbg.smem_hi = base + C::kTiles, g_dbg.F = p.c.latent + p.c.rope, g_dbg.L = p.c.page, g_dbg.B = p.c.n_pages + 1;
+        g_dbg.tmem_base = 0, g_dbg.tmem_cols = 512, g_dbg.ctl = ctl;
+    }
+    FA_CACHE_POISON(base, C::kTiles);
+    fence_proxy_async_smem();
+#endif
+    if (warp == 5) {
+        tmem_alloc(smem_u32(&tmem_slot), C::kCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    grid_dep_wait();
+    grid_dep_launch();
+    const uint32_t tmem = tmem_slot;
+#ifdef FA_DEBUG
+    if (tid == 0) g_dbg.tmem_base = tmem;
+    __syncthreads();
+#endif
+
+    LatentWalk w;
+    const bool any = latent_start(p, part, w);
+    if (warp < 4) {
+        // ---------------------------------------------------------------- softmax
+        const uint32_t lane_off = (warp * 32u) << 16;
+        const uint32_t ra = 16 * warp + lane / 4, quad = lane & 3u;
+        const bool mine = 16 * warp < N;      // rows of this warp
+        uint32_t g = 0, partly = 0;
+        for (uint32_t b = part; b < p.s.B; b += p.parts) {   // sequences without tokens
+            if (latent_units(p, b) != 0) continue;
+            uint8_t* const to = p.y + (static_cast<uint64_t>(b) * p.rows + row0) * (128 * LC);
+            for (uint32_t i = tid; i < n_rows * (8 * LC); i += 128) *reinterpret_cast<uint4*>(to + 16 * i) = make_uint4(0, 0, 0, 0);
+        }
+        while (any && latent_next(p, group, w)) {
+            if (group == 0 && w.begins && tid == 0)
+                p.shares[w.seq] = make_int2(static_cast<int>(part), static_cast<int>(latent_owner(w, w.first_unit + w.units - 1u)));
+            uint32_t limit[2];
+            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t r = ra + 8 * i;
+                limit[i] = r < n_rows ? latent_limit(p, w.q, (row0 + r) / p.heads) : 0u;
+                if (limit[i] == 0) limit[i] = kSeesAll;   // what becomes of such a row is not used
+            }
+            // keys that all rows see that see any: up to the first row's
+            uint32_t least = latent_limit(p, w.q, row0 / p.heads);
+            if (least == 0) {   // (tokens in front of the first key: found by every thread, rows are few)
+                least = w.farthest;
+                for (uint32_t t = row0 / p.heads; t <= (row0 + n_rows - 1u) / p.heads; ++t) {
+                    const uint32_t x = latent_limit(p, w.q, t);
+                    if (x != 0) {
+                        least = x;
+                        break;
+                    }
+                }
+            }
+            for (uint32_t tile = w.t0; tile < w.end; ++tile, ++g) {
+                const uint32_t key0 = tile * kLatentTile;
+                mbar_wait(bar(C::S + (g & 1u)), (g >> 1) & 1u, ctl, kCacheTimeout | C::S);
+                tc_fence_after();
+                __syncwarp();
+                float s[32];
+                if (mine) {
+                    tmem_ld_16x64(tmem + lane_off + C::kColS + 64 * (g & 1u), s);
+                    tmem_wait_ld();
+                }
+                // (the rotary slot's barrier: what the fetching warp has written about this tile is there)
+                mbar_wait(bar(C::RFULL + g % C::kRopeSlots), (g / C::kRopeSlots) & 1u, ctl, kCacheTimeout | C::RFULL);
+                const uint32_t absent = *reinterpret_cast<volatile uint32_t*>(&s_absent[g & 3u]);
+                uint32_t bad_lo = 0, bad_hi = 0;
+                if (key0 + kLatentTile > least || absent != 0) {
+                    if (key0 + kLatentTile > least) {
+                        // two threads a key: pieces of 16 bytes, four of each 64 dimensions
+                        const uint32_t key = tid >> 1, half = tid & 1u, at = key0 + key, swz = key & 7u;
+                        const bool behind = at >= w.farthest, some = !behind && at >= least;
+                        bool bad = false;
+#pragma unroll
+                        for (int c = 0; c < C::kPairs; ++c) mbar_wait(bar(C::FULL + (g * C::kPairs + c) % C::kPairSlots), ((g * C::kPairs + c) / C::kPairSlots) & 1u, ctl, kCacheTimeout | C::FULL);
+                        if (some) {
+                            for (uint32_t c = 0; c < LC; ++c)
+                                for (uint32_t j = 0; j < 4; ++j) {
+                                    uint32_t x[4];
+                                    ld_shared_v4(pair_addr(g * C::kPairs + c / 2) + (c & 1u) * kLatentSlot + key * 128 + (((4 * half + j) ^ swz) << 4), x);
+                                    bad |= not_finite(x, bf16);
+                                }
+                            for (uint32_t j = 0; j < 4; ++j) {
+                                uint32_t x[4];
+                                ld_shared_v4(rope_addr(g) + key * 128 + (((4 * half + j) ^ swz) << 4), x);
+                                bad |= not_finite(x, bf16);
+                            }
+                        }
+                        bad |= __shfl_xor_sync(0xFFFFFFFFu, bad, 1) != 0;
+                        if (behind || bad) {
+                            for (uint32_t c = 0; c < LC; ++c)
+                                for (uint32_t j = 0; j < 4; ++j)
+                                    st_shared_v4(pair_addr(g * C::kPairs + c / 2) + (c & 1u) * kLatentSlot + key * 128 + (((4 * half + j) ^ swz) << 4), 0, 0, 0, 0);
+                        }
+                        if (bad && half == 0) atomicOr(&s_bad[partly & 1u][key >> 5], 1u << (key & 31u));
+                        fence_proxy_async_smem();
+                        softmax_sync();
+                        bad_lo = *reinterpret_cast<volatile uint32_t*>(&s_bad[partly & 1u][0]);
+                        bad_hi = *reinterpret_cast<volatile uint32_t*>(&s_bad[partly & 1u][1]);
+                        ++partly;
+                        // (the other entry was last read two barriers ago)
+                        if (tid < 2) s_bad[partly & 1u][tid] = 0;
+                    }
+                    if (mine) {
+#pragma unroll
+                        for (uint32_t j = 0; j < 8; ++j) {
+                            const bool gone = absent >> (j >> 1) & 1u;
+#pragma unroll
+                            for (uint32_t e = 0; e < 4; ++e) {
+                                const uint32_t key = 8 * j + 2 * quad + (e & 1u);
+                                const bool bad = (key < 32 ? bad_lo >> key : bad_hi >> (key - 32)) & 1u;
+                                if (gone || key0 + key >= limit[e >> 1] || (key0 + key >= w.farthest)) s[4 * j + e] = -INFINITY;
+                                else if (bad) s[4 * j + e] = __int_as_float(0x7FC00000);
+                            }
+                        }
+                    }
+                }
+                // ---- the rows' references
+                float alpha[2] = {1.0f, 1.0f};
+                if (mine) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float top = fmaxf(s[2 * i], s[2 * i + 1]);
+#pragma unroll
+                        for (int j = 1; j < 8; ++j) top = max3(top, s[4 * j + 2 * i], s[4 * j + 2 * i + 1]);
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2)) * p.scale_log2;
+                        if (top > m[i] + kLatentSlack) {
+                            alpha[i] = ex2_approx(m[i] - top);
+                            m[i] = top;
+                            l[i] *= alpha[i];
+                        }
+                    }
+                    if (quad == 0) s_alpha[g & 1u][ra] = alpha[0], s_alpha[g & 1u][ra + 8] = alpha[1];
+                }
+                const bool moved = softmax_any(mine && tile > w.t0 && (alpha[0] != 1.0f || alpha[1] != 1.0f));
+                // ---- weights, rounded, and the sums of what they are rounded to
+                uint32_t pk[16];
+                if (mine) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float ref = m[i] == -INFINITY ? 0.0f : m[i];
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float w0 = ex2_approx(fmaf(s[4 * j + 2 * i], p.scale_log2, -ref)), w1 = ex2_approx(fmaf(s[4 * j + 2 * i + 1], p.scale_log2, -ref));
+                            pk[2 * j + i] = pack_16(w0, w1, bf16);
+                            const float2 y = unpack_16(pk[2 * j + i], bf16);
+                            sum += y.x + y.y;
+                        }
+                        l[i] += sum;
+                    }
+                }
+                // the last P V that read this buffer of P
+                if (g >= C::kPBuffers) {
+                    const uint32_t h = g - C::kPBuffers;
+                    mbar_wait(bar(C::PV + (h & 1u)), (h >> 1) & 1u, ctl, kCacheTimeout | C::PV);
+                }
+                if (mine) {
+                    const uint32_t to = p_addr(g) + ra * 128 + 4 * quad;
+#pragma unroll
+                    for (uint32_t j = 0; j < 8; ++j) {
+                        st_shared_u32(to + ((j ^ (ra & 7u)) << 4), pk[2 * j]);
+                        st_shared_u32(to + 8 * 128 + ((j ^ (ra & 7u)) << 4), pk[2 * j + 1]);
+                    }
+                    fence_proxy_async_smem();
+                }
+                if (moved) {   // rows are columns of Y^T: every warp multiplies all of them, in its dimensions
+                    mbar_wait(bar(C::PV + ((g - 1u) & 1u)), ((g - 1u) >> 1) & 1u, ctl, kCacheTimeout | C::PV);
+                    tc_fence_after();
+                    __syncwarp();
+#pragma unroll 1
+                    for (uint32_t c = 0; c < C::kPairs * N; c += 16) {
+                        float o[16];
+                        uint32_t x[16];
+                        tmem_ld16(tmem + lane_off + c, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (uint32_t e = 0; e < 16; ++e) x[e] = __float_as_uint(o[e] * s_alpha[g & 1u][(c + e) % N]);
+                        tmem_st16(tmem + lane_off + c, x);
+                    }
+                    tmem_wait_st();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(C::P + (g & 1u)));
+            }
+            // ---- the segment's end
+            if (mine) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 1);
+                    l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 2);
+                    if (limit[i] == kSeesAll) l[i] = 0.0f, m[i] = -INFINITY;   // sees nothing
+                    if (quad == 0) s_l[ra + 8 * i] = w.whole ? (l[i] == 0.0f ? 0.0f : 1.0f / l[i]) : l[i], s_m[ra + 8 * i] = m[i];
+                }
+            }
+            const bool tiles = w.end > w.t0;
+            if (tiles) {
+                mbar_wait(bar(C::PV + ((g - 1u) & 1u)), ((g - 1u) >> 1) & 1u, ctl, kCacheTimeout | C::PV);
+                tc_fence_after();
+            }
+            softmax_sync();
+            const uint32_t slot = 2u * blockIdx.x + (w.begins ? 1u : 0u);
+            if (!w.whole && tid < n_rows) p.part_ml[static_cast<uint64_t>(slot) * N + tid] = make_float2(s_m[tid], s_l[tid]);
+            if (tiles || w.whole) {
+#pragma unroll 1
+                for (uint32_t c = 0; c < C::kPairs * N; c += 16) {
+                    float o[16];
+                    if (tiles) {
+                        tmem_ld16(tmem + lane_off + c, o);
+                        tmem_wait_ld();
+                    }
+                    const uint32_t r0 = c % N, d = c / N * 128 + warp * 32 + lane;
+                    if (w.whole) {
+                        uint8_t* const to = p.y + ((static_cast<uint64_t>(w.seq) * p.rows + row0 + r0) * (64 * LC) + d) * 2;
+#pragma unroll
+                        for (uint32_t e = 0; e < 16; ++e) {
+                            const float f = s_l[r0 + e];
+                            const uint32_t x = f == 0.0f ? 0u : pack_16(o[e] * f, 0.0f, bf16);
+                            if (r0 + e < n_rows) *reinterpret_cast<uint16_t*>(to + e * (2 * 64 * LC)) = static_cast<uint16_t>(x);
+                        }
+                    } else {
+                        float* const to = p.part_o + (static_cast<uint64_t>(slot) * N + r0) * (64 * LC) + d;
+#pragma unroll
+                        for (uint32_t e = 0; e < 16; ++e)
+                            if (r0 + e < n_rows) to[e * (64 * LC)] = o[e];
+                    }
+                }
+            }
+            tc_fence_before();
+            softmax_sync();   // s_l and s_m are read
+        }
+    } else if (warp == 4) {
+        // ---------------------------------------------------------------- tiles
+        const bool leader = elect_one();
+        const uint32_t per_tile = p.c.page < kLatentTile ? kLatentTile >> p.c.page_shift : 1u;   // pages of a tile
+        const uint32_t box_rows = min(p.c.page, kLatentTile), box_bytes = box_rows * 128;
+        uint32_t g = 0, reports = 0, pairs = 0, ropes = 0;   // (pairs, ropes: slots filled)
+        bool ok = true;
+        while (ok && any && latent_next(p, group, w)) {
+            const int32_t* const table = p.s.table + w.seq * p.s.table_stride;
+            if (w.begins && group == 0 && lane == 0 && !cache_length_ok(plain_view(p.c), p.s, w.seq)) cache_report(p.c.status, kCacheBadPosition);
+            const uint32_t blocks = (w.q.held + p.c.page - 1u) >> p.c.page_shift;
+            uint32_t known = 0, from = 0;   // entries [from, from + known) are in the lanes
+            int32_t entry = -1;
+            for (uint32_t tile = w.t0; ok && tile < w.end; ++tile, ++g) {
+                const uint32_t key0 = tile * kLatentTile, first = key0 >> p.c.page_shift;
+                if (known == 0 || first + per_tile > from + known) {
+                    from = first, known = 32;
+                    entry = from + lane < blocks ? table[from + lane] : -1;
+                    const bool wrong = from + lane < blocks && static_cast<uint32_t>(entry) >= p.c.n_pages && (from + lane) * p.c.page < w.end * kLatentTile;
+                    if (wrong) ++reports;
+                    if (static_cast<uint32_t>(entry) >= p.c.n_pages) entry = static_cast<int32_t>(p.c.n_pages);   // outside: TMA fills with zeros
+                }
+                uint32_t gone = 0;   // a bit for each 16 keys
+                for (uint32_t i = 0; i < per_tile; ++i)
+                    if (static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, entry, first + i - from)) >= p.c.n_pages) gone |= (per_tile == 1 ? 15u : per_tile == 2 ? 3u : 1u) << (i * (4 / per_tile));
+                const uint32_t nr = g, y = per_tile == 1 ? key0 & (p.c.page - 1u) : 0u;
+                if (nr >= C::kRopeSlots) ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(C::REMPTY + nr % C::kRopeSlots), (nr / C::kRopeSlots - 1u) & 1u, ctl, kCacheTimeout | C::REMPTY));
+                if (!ok) break;
+                ++ropes;
+                if (leader) {
+                    *reinterpret_cast<volatile uint32_t*>(&s_absent[g & 3u]) = gone;
+                    mbar_expect_tx(bar(C::RFULL + nr % C::kRopeSlots), kLatentSlot);
+                }
+                for (uint32_t i = 0; i < per_tile; ++i) {
+                    const int32_t page = __shfl_sync(0xFFFFFFFFu, entry, first + i - from);
+                    if (leader) tma_load_3d(rope_addr(nr) + i * box_bytes, &map, bar(C::RFULL + nr % C::kRopeSlots), 64 * LC, static_cast<int32_t>(y), page);
+                }
+                for (uint32_t c = 0; c < C::kPairs; ++c) {
+                    const uint32_t n = g * C::kPairs + c;
+                    if (n >= C::kPairSlots) ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(C::EMPTY + n % C::kPairSlots), (n / C::kPairSlots - 1u) & 1u, ctl, kCacheTimeout | C::EMPTY));
+                    if (!ok) break;
+                    ++pairs;
+                    if (leader) mbar_expect_tx(bar(C::FULL + n % C::kPairSlots), 2 * kLatentSlot);
+                    for (uint32_t i = 0; i < per_tile; ++i) {
+                        const int32_t page = __shfl_sync(0xFFFFFFFFu, entry, first + i - from);
+                        if (leader) {
+                            tma_load_3d(pair_addr(n) + i * box_bytes, &map, bar(C::FULL + n % C::kPairSlots), static_cast<int32_t>(128 * c), static_cast<int32_t>(y), page);
+                            tma_load_3d(pair_addr(n) + kLatentSlot + i * box_bytes, &map, bar(C::FULL + n % C::kPairSlots), static_cast<int32_t>(128 * c + 64), static_cast<int32_t>(y), page);
+                        }
+                    }
+                }
+                __syncwarp();
+            }
+        }
+        if (reports != 0) cache_report(p.c.status, kCacheBadPage);
+        // What was asked for lands before the CTA ends: the MMAs have waited for it, unless a wait gave up.
+        if (*ctl.abort_flag != 0u) {
+            for (uint32_t i = 0; i < C::kPairSlots; ++i) {
+                const uint32_t uses = (pairs + C::kPairSlots - 1u - i) / C::kPairSlots;
+                if (uses > 0) mbar_wait_certain(bar(C::FULL + i), (uses - 1u) & 1u, ctl, kCacheTimeout | C::FULL);
+            }
+            for (uint32_t i = 0; i < C::kRopeSlots; ++i) {
+                const uint32_t uses = (ropes + C::kRopeSlots - 1u - i) / C::kRopeSlots;
+                if (uses > 0) mbar_wait_certain(bar(C::RFULL + i), (uses - 1u) & 1u, ctl, kCacheTimeout | C::RFULL);
+            }
+        }
+    } else if (warp == 5) {
+        // ---------------------------------------------------------------- MMAs
+        const bool leader = elect_one();
+        const uint32_t idesc_s = idesc_16bit(64, kLatentTile, false, false, bf16), idesc_y = idesc_16bit(128, N, true, false, bf16);
+        const uint32_t rope_steps = p.c.rope / 16;
+        uint32_t g_qk = 0, g_pv = 0, k = 0;           // tiles scored, multiplied; segments begun
+        bool pv_first = false, pv_pending = false;    // the tile whose P is awaited
+        bool more = any && latent_next(p, group, w);
+        while (more && w.end == w.t0) more = latent_next(p, group, w);
+        uint32_t tile = w.t0;
+        bool failed = false;
+        while (!failed && (more || pv_pending)) {
+            const bool first = more && tile == w.t0, last = more && tile + 1 == w.end;
+            uint32_t c = 0;
+            bool q_there = !first;
+            const uint32_t t_begin = wait_clock();
+            uint32_t turns = 0;
+            while ((more && c <= C::kPairs) || pv_pending) {
+                if (more && c <= C::kPairs) {
+                    if (!q_there) q_there = mbar_test(bar(C::QFULL), k & 1u);
+                    if (q_there) {
+                        const uint32_t n = g_qk * C::kPairs + c - 1u;
+                        if (mbar_test(bar(c == 0 ? C::RFULL + g_qk % C::kRopeSlots : C::FULL + n % C::kPairSlots), c == 0 ? (g_qk / C::kRopeSlots) & 1u : (n / C::kPairSlots) & 1u)) {
+                            const uint32_t tS = tmem + C::kColS + 64 * (g_qk & 1u);
+                            tc_fence_after();
+                            if (leader) {
+                                if (c == 0) {
+                                    const uint64_t dq = make_smem_desc<128>(base + LC * kLatentSlot, 16), dk = make_smem_desc<128>(rope_addr(g_qk), 16);
+                                    for (uint32_t ks = 0; ks < rope_steps; ++ks) mma_ss(tS, dq + 2 * ks, dk + 2 * ks, idesc_s, ks > 0 ? 1u : 0u);
+                                } else {
+                                    const uint64_t dq = make_smem_desc<128>(base + (c - 1u) * (2 * kLatentSlot), 16), dk = make_smem_desc<128>(pair_addr(n), 16);
+#pragma unroll
+                                    for (uint32_t ks = 0; ks < 8; ++ks) {
+                                        const uint32_t off = (ks >> 2) * (kLatentSlot >> 4) + (ks & 3u) * 2u;
+                                        mma_ss(tS, dq + off, dk + off, idesc_s, 1u);
+                                    }
+                                }
+                            }
+                            if (c == C::kPairs) {
+                                if (leader) {
+                                    tc_commit(bar(C::S + (g_qk & 1u)));
+                                    if (last) tc_commit(bar(C::QEMPTY));
+                                }
+                                if (last) ++k;
+                            }
+                            __syncwarp();
+                            ++c;
+                            turns = 0;
+                            continue;
+                        }
+                    }
+                }
+                if (pv_pending && mbar_test(bar(C::P + (g_pv & 1u)), (g_pv >> 1) & 1u)) {
+                    tc_fence_after();
+                    if (leader) {
+                        const uint64_t dp = make_smem_desc<128>(p_addr(g_pv), 16);
+#pragma unroll
+                        for (uint32_t d = 0; d < C::kPairs; ++d) {
+                            const uint32_t n = g_pv * C::kPairs + d;
+                            const uint64_t dc = make_smem_desc<128>(pair_addr(n), kLatentSlot);
+#pragma unroll
+                            for (uint32_t ks = 0; ks < 4; ++ks) mma_ss(tmem + d * N, dc + ks * (2048 >> 4), dp + 2 * ks, idesc_y, !pv_first || ks > 0 ? 1u : 0u);
+                            tc_commit(bar(C::EMPTY + n % C::kPairSlots));
+                        }
+                        tc_commit(bar(C::REMPTY + g_pv % C::kRopeSlots));   // (not with the scores: softmax looks at the tile and its barriers until here)
+                        tc_commit(bar(C::PV + (g_pv & 1u)));
+                    }
+                    __syncwarp();
+                    pv_pending = false;
+                    ++g_pv;
+                    turns = 0;
+                    continue;
+                }
+                if (++turns > 4096) {
+                    turns = 0;
+                    const bool late = wait_clock() - t_begin > static_cast<uint32_t>(kWaitCapCycles >> 16);
+                    if (late) wait_expired(ctl, kCacheTimeout | C::P);
+                    if (late || *ctl.abort_flag != 0u) {
+                        failed = true;
+                        break;
+                    }
+                }
+            }
+            if (failed || !more) break;
+            pv_pending = true, pv_first = first;
+            ++g_qk;
+            if (++tile == w.end) {
+                do more = latent_next(p, group, w);
+                while (more && w.end == w.t0);
+                tile = w.t0;
+            }
+        }
+        if (leader) tc_commit(bar(C::FINAL));
+        __syncwarp();
+        mbar_wait_certain(bar(C::FINAL), 0, ctl, kCacheTimeout | C::FINAL);
+    } else {
+        // ---------------------------------------------------------------- queries
+        const uint32_t lt = tid - 192u, rope_pieces = p.c.rope / 8;
+        uint32_t k = 0;
+        while (any && latent_next(p, group, w)) {
+            if (w.end == w.t0) continue;
+            if (k > 0) mbar_wait(bar(C::QEMPTY), (k - 1u) & 1u, ctl, kCacheTimeout | C::QEMPTY);
+            const uint32_t rows = k == 0 ? 64u : n_rows;   // (rows that are not there: zeros, once)
+            for (uint32_t i = lt; i < rows * (8 * LC); i += 64) {
+                const uint32_t r = i / (8 * LC), j = i % (8 * LC), t = (row0 + r) / p.heads, h = row0 + r - t * p.heads;
+                const bool in = r < n_rows;
+                cp_async_16_zero(base + (j / 8) * kLatentSlot + r * 128 + (((j & 7u) ^ (r & 7u)) << 4), p.q_latent + (in ? w.seq * p.ql_b + t * p.ql_t + h * p.ql_h + 16 * j : 0), in);
+            }
+            for (uint32_t i = lt; i < rows * rope_pieces; i += 64) {
+                const uint32_t r = i / rope_pieces, j = i % rope_pieces, t = (row0 + r) / p.heads, h = row0 + r - t * p.heads;
+                const bool in = r < n_rows;
+                cp_async_16_zero(base + LC * kLatentSlot + r * 128 + ((j ^ (r & 7u)) << 4), p.q_rope + (in ? w.seq * p.qr_b + t * p.qr_t + h * p.qr_h + 16 * j : 0), in);
+            }
+            cp_async_wait_all();
+            fence_proxy_async_smem();
+            mbar_arrive(bar(C::QFULL));
+            ++k;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (tid == 0) report_expired(ctl);
+    if (warp == 5) {
+        tc_fence_after();
+        tmem_dealloc(tmem, C::kCols);
+    }
+}
+
+// Puts the parts of divided sequences together.  A CTA has 128 dimensions of a row, its warps the parts in turn.
+constexpr int kLatentJoinWarps = 8;
+template <int LC, int N>
+__global__ void __launch_bounds__(kLatentJoinWarps * 32) fa_latent_join(const LatentRowsArgs p) {
+    __shared__ float4 s_o[kLatentJoinWarps][32];
+    __shared__ float s_sum[kLatentJoinWarps], s_top[kLatentJoinWarps];
+    grid_dep_wait();
+    grid_dep_launch();
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t dims = blockIdx.x % (LC / 2) * 128 + 4 * lane;
+    const uint64_t at = blockIdx.x / (LC / 2);
+    const uint32_t b = static_cast<uint32_t>(at / p.rows), row = static_cast<uint32_t>(at - static_cast<uint64_t>(b) * p.rows), group = row / p.group_rows, r = row - group * p.group_rows;
+    const LatentSeq q = latent_seq(p, b);
+    uint8_t* const to = p.y + (at * (64 * LC) + dims) * 2;
+    if (q.count == 0 || q.held == 0) return;
+    const int2 share = p.shares[b];
+    if (share.x == share.y) return;   // written where it was worked out
+    auto slot = [&](int part) { return (static_cast<uint64_t>(part) * p.groups + group) * 2u + (part == share.x ? 1u : 0u); };
+    float top = -INFINITY;
+    for (int i = share.x + static_cast<int>(threadIdx.x); i <= share.y; i += kLatentJoinWarps * 32) top = fmaxf(top, p.part_ml[slot(i) * N + r].x);
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    if (lane == 0) s_top[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kLatentJoinWarps; ++i) top = fmaxf(top, s_top[i]);
+    float4 o = make_float4(0, 0, 0, 0);
+    float sum = 0.0f;
+#pragma unroll 4
+    for (int i = share.x + static_cast<int>(warp); i <= share.y; i += kLatentJoinWarps) {
+        const float2 ml = p.part_ml[slot(i) * N + r];
+        if (ml.y == 0.0f) continue;   // nothing seen there
+        const float f = ex2_approx((ml.x == -INFINITY ? 0.0f : ml.x) - (top == -INFINITY ? 0.0f : top));
+        const float4 x = *reinterpret_cast<const float4*>(p.part_o + (slot(i) * N + r) * (64 * LC) + dims);
+        o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y), o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
+        sum = fmaf(ml.y, f, sum);
+    }
+    s_o[warp][lane] = o;
+    if (lane == 0) s_sum[warp] = sum;
+    __syncthreads();
+    if (warp != 0) return;
+    for (int i = 1; i < kLatentJoinWarps; ++i) {
+        const float4 x = s_o[i][lane];
+        o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w, sum += s_sum[i];
+    }
+    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+    *reinterpret_cast<uint2*>(to) = make_uint2(pack_16(o.x * f, o.y * f, p.bf16 != 0), pack_16(o.z * f, o.w * f, p.bf16 != 0));
+}
+
+}  // namespace fa

@@ -1,0 +1,454 @@
+// The pages of a cache: who holds them, sharing, pages of one's own, moving to the front; and copying what they hold.
+//
+// refs[p] is the number of table entries that hold page p, 0: it is free.  A table entry is a page or -1; anything else is reported and
+// taken for -1.  All results are whole numbers that depend on nothing but the inputs: counts change by atomic additions, whose order
+// does not matter, and where one of several has to be chosen the lowest is (a minimum, likewise).
+//
+// These kernels read and write a few kilobytes to a megabyte: what bounds them is the chain of dependent accesses and the launch, so that
+// each call is one launch (compacting: two) and no value crosses to the host.  Copying is bound by memory.
+#pragma once
+
+#include "fa_cache.cuh"
+
+namespace fa {
+
+// Status codes (kCacheBadPage, kCacheBadPosition beside them).
+constexpr uint32_t kPagesNone = 3u;    // a sequence needed a page and none was free
+constexpr uint32_t kPagesCount = 4u;   // counts that do not fit the table: a page was let go of that nobody held
+
+struct PagesView {
+    int32_t* refs;
+    uint32_t* status;   // four words: first code, number of reports, CTAs that are through (zero between calls), unused
+    uint32_t n;
+};
+struct PagesTable {
+    int32_t* at;        // [B, width], rows `stride` apart
+    int64_t stride;
+    uint32_t width, B;
+};
+
+__device__ __forceinline__ int32_t ld_cg(const int32_t* p) {
+    int32_t v;
+    asm volatile("ld.global.cg.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ int4 ld_cg(const int4* p) {
+    int4 v;
+    asm volatile("ld.global.cg.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ bool is_page(const PagesView& v, int32_t entry) { return static_cast<uint32_t>(entry) < v.n; }
+__device__ __forceinline__ void let_go(const PagesView& v, int32_t entry) {
+    if (!is_page(v, entry)) {
+        if (entry != -1) cache_report(v.status, kCacheBadPage);
+        return;
+    }
+    if (atomicSub(v.refs + entry, 1) <= 0) cache_report(v.status, kPagesCount);
+}
+
+// ----------------------------------------------------------------------------- fork
+// Columns of the table are independent: a CTA takes `cols` of them, holds all their entries in shared memory and puts them where they
+// belong, so the table can be changed in place.  The last CTA does so with the lengths.
+struct ForkArgs {
+    PagesView v;
+    PagesTable t;
+    int32_t* lengths;
+    const int32_t* parents;
+    uint32_t cols;
+};
+constexpr int kForkThreads = 256;
+__global__ void __launch_bounds__(kForkThreads) fa_pages_fork(const ForkArgs p) {
+    extern __shared__ int32_t s_old[];
+    grid_dep_wait();
+    grid_dep_launch();
+    const bool is_lengths = blockIdx.x == gridDim.x - 1;
+    const uint32_t col0 = blockIdx.x * p.cols, cols = is_lengths ? 1u : min(p.cols, p.t.width - col0);
+    int32_t* const base = is_lengths ? p.lengths : p.t.at + col0;
+    const int64_t stride = is_lengths ? 1 : p.t.stride;
+    for (uint32_t i = threadIdx.x; i < p.t.B * cols; i += kForkThreads) s_old[i] = base[(i / cols) * stride + i % cols];
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < p.t.B * cols; i += kForkThreads) {
+        const uint32_t b = i / cols, c = i % cols;
+        int32_t parent = p.parents[b];
+        if (parent < -1 || parent >= static_cast<int32_t>(p.t.B)) {   // stays as it is
+            if (is_lengths) cache_report(p.v.status, kCacheBadPosition);
+            parent = static_cast<int32_t>(b);
+        }
+        const int32_t before = s_old[i];
+        int32_t now = parent < 0 ? (is_lengths ? 0 : -1) : s_old[static_cast<uint32_t>(parent) * cols + c];
+        if (!is_lengths && now != -1 && !is_page(p.v, now)) {
+            cache_report(p.v.status, kCacheBadPage);
+            now = -1;
+        }
+        if (now == before) continue;
+        base[b * stride + c] = now;
+        if (is_lengths) continue;
+        let_go(p.v, before);
+        if (now >= 0) atomicAdd(p.v.refs + now, 1);
+    }
+}
+
+// ----------------------------------------------------------------------------- reserve
+// The first part, a warp a sequence: blocks behind those that are needed are let go of.  The last CTA to be through with that does the
+// rest, with `lanes` threads a sequence (as many as its tokens touch blocks, up to 32):
+//
+//   1  every entry that will be written to lets go of its page.  What is left of a page's count is the number of those that hold it and
+//      do not write to it
+//   2  where that is none all that hold the page write to it, and the lowest sequence keeps it: the count becomes minus (B - b) of the
+//      lowest b, by a minimum
+//   3  an entry keeps its page if it finds its own number there; all others want one.  Their ranks, in order of sequences and blocks
+//   4  the free pages (count 0), in ascending order, as many as are wanted
+//   5  each takes the one of its rank; where there is none left, the entry stays as it was and its sequence is granted fewer tokens
+struct ReserveArgs {
+    PagesView v;
+    PagesTable t;
+    const int32_t* lengths;
+    const int32_t* counts;   // null: `count` of each
+    int32_t* granted;        // [B]
+    int32_t* sources;        // [B]
+    int32_t* targets;
+    int32_t* list;           // [n]: free pages
+    uint32_t count, page_shift;
+};
+constexpr int kReserveThreads = 1024, kReserveWarps = kReserveThreads / 32;
+constexpr uint32_t kNoBlock = 0xFFFFFFFFu;
+
+struct Window {   // of the blocks that a sequence's new tokens touch
+    uint32_t held, count, first, need;
+    bool ok;
+};
+__device__ __forceinline__ Window reserve_window(const ReserveArgs& p, uint32_t b) {
+    Window w;
+    const int32_t held = p.lengths[b], count = p.counts ? p.counts[b] : static_cast<int32_t>(p.count);
+    const uint64_t room = min(static_cast<uint64_t>(p.t.width) << p.page_shift, static_cast<uint64_t>(0x7FFFFFFF));
+    w.ok = held >= 0 && count >= 0 && static_cast<uint64_t>(held) + static_cast<uint64_t>(count) <= room;
+    w.held = static_cast<uint32_t>(min(static_cast<uint64_t>(max(held, 0)), room));
+    w.count = static_cast<uint32_t>(min(static_cast<uint64_t>(max(count, 0)), room - w.held));
+    w.first = w.held >> p.page_shift;
+    w.need = (w.held + w.count + (1u << p.page_shift) - 1u) >> p.page_shift;
+    if (w.count == 0) w.first = w.need;   // nothing is written
+    return w;
+}
+// Sum of x over the threads in front of this one; `all`: of all threads.  All threads of the CTA.
+__device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t* s_warp, uint32_t& all) {
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    uint32_t upto = x;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+        if (lane >= d) upto += y;
+    }
+    __syncthreads();   // (s_warp may still be read from the last time)
+    if (lane == 31) s_warp[warp] = upto;
+    __syncthreads();
+    const uint32_t w = s_warp[lane];   // as many warps as lanes
+    uint32_t sums = w;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, sums, d);
+        if (lane >= d) sums += y;
+    }
+    all = __shfl_sync(0xFFFFFFFFu, sums, 31);
+    return __shfl_sync(0xFFFFFFFFu, sums - w, warp) + upto - x;
+}
+
+__global__ void __launch_bounds__(kReserveThreads) fa_pages_reserve(const ReserveArgs p) {
+    __shared__ uint32_t s_warp[32], s_most, s_last;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    if (tid == 0) s_most = 0;
+    grid_dep_wait();
+    grid_dep_launch();
+    for (uint32_t b = blockIdx.x * kReserveWarps + warp; b < p.t.B; b += gridDim.x * kReserveWarps) {
+        const Window w = reserve_window(p, b);
+        if (lane == 0 && !w.ok) cache_report(p.v.status, kCacheBadPosition);
+        int32_t* const row = p.t.at + b * p.t.stride;
+        for (uint32_t i = w.need + lane; i < p.t.width; i += 128) {   // four loads of a lane in flight
+            int32_t e[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) e[k] = i + 32 * k < p.t.width ? row[i + 32 * k] : -1;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (e[k] != -1) {
+                    let_go(p.v, e[k]);
+                    row[i + 32 * k] = -1;
+                }
+        }
+    }
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+        const uint32_t through = gridDim.x == 1 ? 0 : atomicAdd(p.v.status + 2, 1u);
+        s_last = through == gridDim.x - 1;
+        if (s_last && gridDim.x > 1) p.v.status[2] = 0;
+    }
+    __syncthreads();
+    if (!s_last) return;
+    __threadfence();
+
+    // how many blocks a sequence's tokens touch at most decides how many threads it gets
+    uint32_t most = 0;
+    for (uint32_t b = tid; b < p.t.B; b += kReserveThreads) {
+        const Window w = reserve_window(p, b);
+        most = max(most, w.need - w.first);
+    }
+    most = __reduce_max_sync(0xFFFFFFFFu, most);
+    if (lane == 0) atomicMax(&s_most, most);
+    __syncthreads();
+    most = s_most;
+    uint32_t shift = 0;
+    while (shift < 5 && (1u << shift) < most) ++shift;
+    const uint32_t lanes = 1u << shift, per = (most + lanes - 1) >> shift, at_once = kReserveThreads >> shift;
+    const uint32_t mine = tid >> shift, l = tid & (lanes - 1u);   // which of the sequences at hand, and of its lanes
+    // this thread's blocks [i0, i1) of sequence b
+    auto blocks = [&](uint32_t b, Window& w, uint32_t& i0, uint32_t& i1) {
+        i0 = i1 = 0;
+        if (b >= p.t.B) return;
+        w = reserve_window(p, b);
+        i0 = min(w.need, w.first + l * per), i1 = min(w.need, i0 + per);
+    };
+    for (int step = 1; step <= 2; ++step) {
+        for (uint32_t b0 = 0; b0 < p.t.B; b0 += at_once) {
+            const uint32_t b = b0 + mine;
+            Window w;
+            uint32_t i0, i1;
+            blocks(b, w, i0, i1);
+            for (uint32_t i = i0; i < i1; ++i) {
+                int32_t* const entry = p.t.at + b * p.t.stride + i;
+                const int32_t e = *entry;
+                if (!is_page(p.v, e)) {
+                    if (step == 1 && e != -1) {
+                        cache_report(p.v.status, kCacheBadPage);
+                        *entry = -1;
+                    }
+                } else if (step == 1) {
+                    if (atomicSub(p.v.refs + e, 1) <= 0) cache_report(p.v.status, kPagesCount);
+                } else if (ld_cg(p.v.refs + e) <= 0) {
+                    atomicMin(p.v.refs + e, -static_cast<int32_t>(p.t.B - b));
+                }
+            }
+        }
+        __syncthreads();
+    }
+    // 3: what is kept is marked in the table (as -2 - page), nobody else looks there; how many pages are wanted
+    uint32_t wanted = 0;
+    for (uint32_t b0 = 0; b0 < p.t.B; b0 += at_once) {
+        const uint32_t b = b0 + mine;
+        Window w;
+        uint32_t i0, i1;
+        blocks(b, w, i0, i1);
+        for (uint32_t i = i0; i < i1; ++i) {
+            int32_t* const entry = p.t.at + b * p.t.stride + i;
+            const int32_t e = *entry;
+            if (is_page(p.v, e) && ld_cg(p.v.refs + e) == -static_cast<int32_t>(p.t.B - b)) *entry = -2 - e;
+            else ++wanted;
+        }
+    }
+    uint32_t demand;
+    (void)sum_before(wanted, s_warp, demand);
+    // 4: free pages, 16 of a thread at a time
+    uint32_t found = 0;
+    for (uint32_t q0 = 0; q0 < p.v.n && found < demand; q0 += 16 * kReserveThreads) {
+        const uint32_t q = q0 + 16 * tid;
+        uint32_t free = 0;
+        if (q + 16 <= p.v.n && (reinterpret_cast<uintptr_t>(p.v.refs) & 15u) == 0) {
+            int4 x[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = ld_cg(reinterpret_cast<const int4*>(p.v.refs + q) + k);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                free |= ((x[k].x == 0) | (x[k].y == 0) << 1 | (x[k].z == 0) << 2 | (x[k].w == 0) << 3) << (4 * k);
+        } else {
+            for (uint32_t k = 0; k < 16 && q + k < p.v.n; ++k) free |= static_cast<uint32_t>(ld_cg(p.v.refs + q + k) == 0) << k;
+        }
+        uint32_t all, at = found + sum_before(__popc(free), s_warp, all);
+        for (; free != 0 && at < demand; free &= free - 1u) p.list[at++] = static_cast<int32_t>(q + __ffs(free) - 1);   // (demand may exceed n, `at` not)
+        found += all;
+    }
+    const uint32_t there = min(found, demand);
+    __syncthreads();   // (the list, by this CTA alone: visible to it)
+    // 5
+    uint32_t in_front = 0;
+    for (uint32_t b0 = 0; b0 < p.t.B; b0 += at_once) {
+        const uint32_t b = b0 + mine;
+        Window w;
+        uint32_t i0, i1, n = 0, all;
+        blocks(b, w, i0, i1);
+        for (uint32_t i = i0; i < i1; ++i) n += p.t.at[b * p.t.stride + i] >= -1;
+        uint32_t rank = in_front + sum_before(n, s_warp, all), refused = kNoBlock;
+        in_front += all;
+        int32_t source = -1, target = -1;
+        for (uint32_t i = i0; i < i1; ++i) {
+            int32_t* const entry = p.t.at + b * p.t.stride + i;
+            const int32_t e = *entry;
+            if (e < -1) {   // kept: from the sequence's number to one, whatever refused entries have added
+                *entry = -2 - e;
+                atomicAdd(p.v.refs + (-2 - e), static_cast<int32_t>(p.t.B - b) + 1);
+                continue;
+            }
+            if (rank < there) {
+                const int32_t page = p.list[rank];
+                *entry = page;
+                atomicAdd(p.v.refs + page, 1);
+                if (e >= 0 && i == w.held >> p.page_shift && (w.held & ((1u << p.page_shift) - 1u)) != 0) source = e, target = page;
+            } else {
+                if (e >= 0) atomicAdd(p.v.refs + e, 1);
+                refused = min(refused, i);
+                cache_report(p.v.status, kPagesNone);
+            }
+            ++rank;
+        }
+        for (uint32_t d = lanes >> 1; d >= 1; d >>= 1) refused = min(refused, __shfl_xor_sync(0xFFFFFFFFu, refused, d));
+        if (b < p.t.B && l == 0) {   // (the first of a sequence's lanes has the block that may be copied)
+            const uint32_t room = refused == kNoBlock ? w.count : max(refused << p.page_shift, w.held) - w.held;
+            p.granted[b] = static_cast<int32_t>(min(w.count, room));
+            p.sources[b] = source;
+            p.targets[b] = target;
+        }
+    }
+}
+
+// ----------------------------------------------------------------------------- compact
+// With n_used pages held, those from n_used on move to the free ones in front of it, the k-th to the k-th.  A CTA works out 4096 pages;
+// it counts those in front of them itself, from all of refs (13333 pages are 53 KB), so that no CTA waits for another.
+struct CompactArgs {
+    PagesView v;
+    PagesTable t;
+    int32_t* new_refs;    // [n]
+    int32_t* new_table;   // [B, width] contiguous
+    int32_t* sources;     // [n]
+    int32_t* targets;
+    int32_t* rank;        // [n]: which of the moves a page is, -1: it stays or is free
+    uint32_t* totals;     // used pages, moves
+};
+constexpr int kCompactThreads = 1024, kCompactPages = 4 * kCompactThreads;
+__global__ void __launch_bounds__(kCompactThreads) fa_pages_plan(const CompactArgs p) {
+    __shared__ uint32_t s_warp[32];
+    const uint32_t tid = threadIdx.x, n = p.v.n, base = blockIdx.x * kCompactPages;
+    grid_dep_wait();
+    grid_dep_launch();
+    uint32_t front = 0, rest = 0;   // used pages in front of this CTA's, and the others
+    for (uint32_t q = tid; q < n; q += kCompactThreads) {
+        const uint32_t used = p.v.refs[q] > 0;
+        if (q < base) front += used;
+        else rest += used;
+    }
+    uint32_t used_front, used_rest;
+    (void)sum_before(front, s_warp, used_front);
+    (void)sum_before(rest, s_warp, used_rest);
+    const uint32_t n_used = used_front + used_rest;
+    uint32_t low = 0, low_used;
+    for (uint32_t q = tid; q < n_used; q += kCompactThreads) low += p.v.refs[q] > 0;
+    (void)sum_before(low, s_warp, low_used);
+    const uint32_t moves = n_used - low_used;
+    if (blockIdx.x == 0 && tid == 0) p.totals[0] = n_used, p.totals[1] = moves;
+    int32_t r[4];
+    uint32_t used = 0, all;
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+        const uint32_t q = base + 4 * tid + k;
+        r[k] = q < n ? p.v.refs[q] : 0;
+        used += r[k] > 0;
+    }
+    uint32_t before = used_front + sum_before(used, s_warp, all);   // used pages in front of q
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+        const uint32_t q = base + 4 * tid + k;
+        if (q >= n) break;
+        const bool is_used = r[k] > 0;
+        const bool moves_on = is_used && q >= n_used;
+        p.rank[q] = moves_on ? static_cast<int32_t>(before - low_used) : -1;
+        if (moves_on) p.sources[before - low_used] = static_cast<int32_t>(q);
+        else if (!is_used && q < n_used) p.targets[q - before] = static_cast<int32_t>(q);
+        if (q >= n_used) p.new_refs[q] = 0;
+        else if (is_used) p.new_refs[q] = r[k];   // (the others: fa_pages_renumber)
+        if (q >= moves) p.sources[q] = -1, p.targets[q] = -1;
+        before += is_used;
+    }
+}
+__global__ void __launch_bounds__(256) fa_pages_renumber(const CompactArgs p) {
+    grid_dep_wait();
+    grid_dep_launch();
+    const uint64_t entries = static_cast<uint64_t>(p.t.B) * p.t.width;
+    const uint32_t n_used = p.totals[0], moves = p.totals[1];
+    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < entries || i < moves; i += gridDim.x * 256ull) {
+        if (i < moves) p.new_refs[p.targets[i]] = p.v.refs[p.sources[i]];
+        if (i >= entries) continue;
+        const uint64_t b = i / p.t.width;
+        int32_t e = p.t.at[static_cast<int64_t>(b) * p.t.stride + static_cast<int64_t>(i - b * p.t.width)];
+        if (!is_page(p.v, e)) {
+            if (e != -1) cache_report(p.v.status, kCacheBadPage);
+            e = -1;
+        } else if (p.v.refs[e] <= 0) {   // an entry that is not counted
+            cache_report(p.v.status, kPagesCount);
+            e = -1;
+        } else if (static_cast<uint32_t>(e) >= n_used) {
+            e = p.targets[p.rank[e]];
+        }
+        p.new_table[i] = e;
+    }
+}
+
+// ----------------------------------------------------------------------------- copy
+// Contents of pages, source to target, for up to kCopyAreas arrays: a page of an array is n0 x n1 rows of `row` bytes (one row where it
+// lies in one piece).  CTA (x, y) has the pairs x, x + gridDim.x, ... and of each page the y-th of gridDim.y equal parts.
+struct CopyArea {
+    uint8_t* base;
+    int64_t page, stride0, stride1;   // bytes
+    uint32_t n0, n1, row;             // row: a multiple of 16, or of 4
+};
+constexpr int kCopyAreas = 32;
+struct CopyArgs {
+    CopyArea area[kCopyAreas];
+    const int32_t* sources;
+    const int32_t* targets;
+    uint32_t* status;
+    uint32_t areas, pairs, n;   // n: pages of every array
+};
+constexpr int kCopyThreads = 256;
+constexpr int kCopyFlight = 8;   // loads of a thread in flight
+
+template <typename Piece>
+__device__ __forceinline__ void copy_part(const CopyArea& a, uint32_t source, uint32_t target, uint32_t part, uint32_t parts) {
+    const uint32_t in_row = a.row / sizeof(Piece);
+    const uint64_t pieces = static_cast<uint64_t>(a.n0) * a.n1 * in_row, end = pieces * (part + 1) / parts;
+    const uint8_t* const from = a.base + source * a.page;
+    uint8_t* const to = a.base + target * a.page;
+    auto place = [&](uint64_t i) -> int64_t {
+        if (a.n0 * a.n1 == 1) return static_cast<int64_t>(i * sizeof(Piece));
+        const uint32_t r = static_cast<uint32_t>(i / in_row), c = static_cast<uint32_t>(i - static_cast<uint64_t>(r) * in_row), r0 = r / a.n1;
+        return r0 * a.stride0 + (r - r0 * a.n1) * a.stride1 + static_cast<int64_t>(c * sizeof(Piece));
+    };
+    for (uint64_t i = pieces * part / parts + threadIdx.x; i < end; i += kCopyThreads * kCopyFlight) {
+        Piece x[kCopyFlight];
+        int64_t at[kCopyFlight];
+#pragma unroll
+        for (int k = 0; k < kCopyFlight; ++k)
+            if (i + k * kCopyThreads < end) x[k] = *reinterpret_cast<const Piece*>(from + (at[k] = place(i + k * kCopyThreads)));
+#pragma unroll
+        for (int k = 0; k < kCopyFlight; ++k)
+            if (i + k * kCopyThreads < end) *reinterpret_cast<Piece*>(to + at[k]) = x[k];
+    }
+}
+
+__global__ void __launch_bounds__(kCopyThreads) fa_cache_copy(const __grid_constant__ CopyArgs p) {
+    grid_dep_wait();
+    grid_dep_launch();
+    const uint32_t lane = threadIdx.x & 31u;
+    for (uint64_t i0 = blockIdx.x; i0 < p.pairs; i0 += 32ull * gridDim.x) {   // every warp looks at 32 of the CTA's pairs
+        const uint64_t i = i0 + static_cast<uint64_t>(lane) * gridDim.x;
+        const int32_t s = i < p.pairs ? p.sources[i] : -1, t = i < p.pairs ? p.targets[i] : -1;
+        const bool good = static_cast<uint32_t>(s) < p.n && static_cast<uint32_t>(t) < p.n;
+        if (!good && (s != -1 || t != -1) && i < p.pairs && threadIdx.x < 32 && blockIdx.y == 0) cache_report(p.status, kCacheBadPage);
+        for (uint32_t left = __ballot_sync(0xFFFFFFFFu, good && s != t); left != 0; left &= left - 1u) {
+            const int l = __ffs(left) - 1;
+            const uint32_t source = static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, s, l)), target = static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, t, l));
+            for (uint32_t k = 0; k < p.areas; ++k) {
+                const CopyArea& a = p.area[k];
+                if ((a.row & 15u) == 0) copy_part<uint4>(a, source, target, blockIdx.y, gridDim.y);
+                else copy_part<uint32_t>(a, source, target, blockIdx.y, gridDim.y);
+            }
+        }
+    }
+}
+
+}  // namespace fa

@@ -389,6 +389,103 @@ int fa_b200_cache_attention(const fa_b200_cache* cache, const fa_b200_sequences*
 int fa_b200_cache_attention_scratch(uint32_t head_dim, uint32_t kv_heads, uint32_t q_heads, uint32_t page_size, uint32_t B, uint32_t T,
                                     uint32_t table_width, uint32_t keep, int device, uint64_t out[1]);
 
+/*
+ * ---- The pages of a cache: fa_b200_pages_fork, fa_b200_pages_reserve, fa_b200_pages_compact, fa_b200_cache_copy.
+ *
+ * refs[p] is how many entries of the table [B, table_width] hold page p; 0: it is free.  An entry is a page or -1, a row holds a page
+ * once.  The functions keep refs and table in step; calls on one refs and table have to be ordered by streams.  All are asynchronous,
+ * repeat bit for bit and allocate nothing.  `status` receives the first code and the number of reports: 1 an entry that is neither a page
+ * nor -1 (taken for -1), 2 a length, count or parent outside, 3 no page was free, 4 refs and table are not in step.
+ */
+typedef struct fa_b200_pages {
+    int32_t* refs;       /* [n_pages] */
+    uint32_t* status;    /* four words, zero at first; the third is the library's between and within calls */
+    uint32_t n_pages;
+} fa_b200_pages;
+
+/*
+ * Row b of the table becomes what row parents[b] was, and lengths[b] what its length was, all at once and in place; -1: an empty row
+ * (its pages are let go of) and length 0.  A parent outside leaves a row as it is.  At most 57344 sequences.
+ */
+int fa_b200_pages_fork(const fa_b200_pages* pages, int32_t* table, int64_t table_stride, uint32_t table_width, uint32_t B, int32_t* lengths,
+                       const int32_t* parents, int device, void* cuda_stream);
+
+/*
+ * Gives every sequence the blocks that lengths[b] + counts[b] tokens need (counts NULL: `count` each) and no more: blocks behind them are
+ * let go of.  Blocks that the new tokens go to and that have no page get one, and so do those whose page others hold too, unless all that
+ * hold it are about to write to it: then the lowest sequence keeps it.  New pages are the lowest free ones, in the order of sequences and
+ * blocks.  sources[b], targets[b]: the page that held the beginning of a block, and the one that has taken its place (-1: none);
+ * fa_b200_cache_copy is to copy it before tokens are appended.  granted[b]: how many of the tokens have room, counts[b] unless pages ran out.
+ * Scratch: 4 * n_pages bytes.
+ */
+int fa_b200_pages_reserve(const fa_b200_pages* pages, int32_t* table, int64_t table_stride, uint32_t table_width, uint32_t B, const int32_t* lengths,
+                          const int32_t* counts_or_null, uint32_t count, uint32_t page_size, int32_t* granted, int32_t* sources, int32_t* targets,
+                          void* scratch, uint64_t scratch_bytes, int device, void* cuda_stream);
+
+/*
+ * The move of all pages that are held to the front: with n_used of them, the k-th of those from n_used on goes to the k-th free one in front
+ * of it.  Writes refs and table ([B, table_width] contiguous) as they are afterwards, and the moves: sources and targets [n_pages], -1 behind
+ * the last.  The old ones are left as they are.  Scratch: 4 * n_pages + 8 bytes.
+ */
+int fa_b200_pages_compact(const fa_b200_pages* pages, const int32_t* table, int64_t table_stride, uint32_t table_width, uint32_t B, int32_t* new_refs,
+                          int32_t* new_table, int32_t* sources, int32_t* targets, void* scratch, uint64_t scratch_bytes, int device, void* cuda_stream);
+
+/* An array of pages: page p is n0 x n1 rows of row_bytes, row (i, j) at base + p * page_stride + i * stride0 + j * stride1 (bytes; all of
+ * them multiples of 16 if row_bytes is, else of 4). */
+typedef struct fa_b200_copy_area {
+    void* base;
+    int64_t page_stride, stride0, stride1;
+    uint32_t n0, n1, row_bytes;
+} fa_b200_copy_area;
+
+/*
+ * Copies page sources[i] to page targets[i] in each of the arrays, all of n_pages pages; pairs with -1 are passed over.  No page may be
+ * a target twice, or a target and a source.  `areas` is read before the call returns.  status: two words, 1 a page outside.
+ */
+int fa_b200_cache_copy(const fa_b200_copy_area* areas, uint32_t n_areas, uint32_t n_pages, const int32_t* sources, const int32_t* targets, uint32_t pairs,
+                       uint32_t* status, int device, void* cuda_stream);
+
+/*
+ * ---- The paged cache of latent vectors: fa_b200_latent_append, fa_b200_latent_attention, and fa_b200_latent_prompt.
+ *
+ * A token has one row for all heads: latent_dim 16-bit values (128, 256 or 512) that are key and value at once, and behind them rope_dim
+ * (16, 32 or 64) that belong to the key and are rotated by the token's position.  Sequences, tables and what the status block receives are as
+ * with the 8-bit cache above.  All functions are asynchronous, repeat bit for bit and allocate nothing.
+ */
+typedef struct fa_b200_latent_cache {
+    void* data;          /* row t of page p at p * page_stride + t * token_stride (bytes, multiples of 16), on a 16-byte boundary */
+    uint32_t* status;    /* two words, zero until something is wrong */
+    int64_t page_stride, token_stride;
+    uint32_t n_pages, page_size, latent_dim, rope_dim;
+} fa_b200_latent_cache;
+
+/*
+ * Append T tokens to each sequence, at positions lengths[b], ...: latents [B, T, latent_dim] as they are, rope_keys [B, T, rope_dim] rotated
+ * (strides in elements, last axis contiguous, rows on 16-byte boundaries).  Rotated keys [B, T, rope_dim] and, with queries
+ * ([B, T, heads, rope_dim]), rotated queries are written out too, contiguous, rounded once; zeros where a sequence has no token or the
+ * rotation no position.  cos and sin: fp32 [positions, rope_dim / 2]; without them nothing is rotated.  Lengths are not changed.
+ */
+int fa_b200_latent_append(const fa_b200_latent_cache* cache, const fa_b200_sequences* sequences, const void* latents, int64_t latents_batch_stride,
+                          int64_t latents_token_stride, const void* rope_keys, int64_t keys_batch_stride, int64_t keys_token_stride, const void* queries_or_null,
+                          int64_t queries_batch_stride, int64_t queries_token_stride, int64_t queries_head_stride, uint32_t heads, void* rotated_keys,
+                          void* rotated_queries, const float* cos_or_null, const float* sin_or_null, uint32_t positions, uint32_t dtype, uint32_t flags, int device,
+                          void* cuda_stream);
+
+/*
+ * y = sum of softmax(scale * (q_latent . c + q_rope . r)) c over the rows (c, r) that a query sees, for queries that have been multiplied into
+ * the latent space: q_latent [B, T, heads, latent_dim], q_rope [B, T, heads, rope_dim] (rotated), y [B, T, heads, latent_dim] contiguous.  Queries
+ * are the last tokens of their sequences, as with fa_b200_cache_attention, FA_B200_CACHE_ALL_KEYS too.  Cache and queries have one type.
+ * Scores, sums and maxima are held in fp32, weights are rounded to the type for their product with c and summed as rounded.  A query that sees
+ * nothing, or that its sequence does not have, gets zeros.  Rows that a query does not see do not reach it, whatever they hold.  0 < scale < inf.
+ */
+int fa_b200_latent_attention(const fa_b200_latent_cache* cache, const fa_b200_sequences* sequences, const void* q_latent, int64_t ql_batch_stride,
+                             int64_t ql_token_stride, int64_t ql_head_stride, const void* q_rope, int64_t qr_batch_stride, int64_t qr_token_stride,
+                             int64_t qr_head_stride, uint32_t heads, float scale, uint32_t dtype, uint32_t flags, void* y, void* scratch, uint64_t scratch_bytes,
+                             int device, void* cuda_stream);
+
+/* out[0] = bytes of scratch that such a call needs, on a 16-byte boundary.  Pure arithmetic on the device's facts. */
+int fa_b200_latent_attention_scratch(uint32_t latent_dim, uint32_t heads, uint32_t page_size, uint32_t B, uint32_t T, uint32_t table_width, int device, uint64_t out[1]);
+
 #ifdef __cplusplus
 }
 #endif
