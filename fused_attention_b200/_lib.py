@@ -40,6 +40,8 @@ EXPORTED_SYMBOLS = (
     "fa_b200_latent_append",
     "fa_b200_latent_attention",
     "fa_b200_latent_attention_scratch",
+    "fa_b200_latent_prompt",
+    "fa_b200_latent_status",
 )
 
 # Status codes and flags, mirrored from include/fa_b200.h.
@@ -180,6 +182,10 @@ def load() -> ctypes.CDLL:
         lib.fa_b200_latent_attention.argtypes = [latent, seqs] + 2 * heads3 + [u32, ctypes.c_float, u32, u32, vp, vp, u64, i32, vp]
         lib.fa_b200_latent_attention_scratch.restype = i32
         lib.fa_b200_latent_attention_scratch.argtypes = 6 * [u32] + [i32, ctypes.POINTER(u64)]
+        lib.fa_b200_latent_prompt.restype = i32
+        lib.fa_b200_latent_prompt.argtypes = 3 * heads3 + rows + [vp, vp] + 6 * [u32] + [ctypes.c_float, u32, u32, vp, i32, vp]
+        lib.fa_b200_latent_status.restype = i32
+        lib.fa_b200_latent_status.argtypes = [i32, ctypes.POINTER(u32)]
         # for the extension module's calls
         lib.cache_entries = tuple(ctypes.cast(f, vp).value for f in (lib.fa_b200_cache_append, lib.fa_b200_cache_select, lib.fa_b200_cache_attention,
                                                                      lib.fa_b200_cache_attention_scratch))

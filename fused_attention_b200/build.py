@@ -57,7 +57,7 @@ def lib_sources() -> list[str]:
 # (-DFA_DEBUG) and once for all others.
 CACHE_PARTS = {
     "fa_cache": ("fa_cache.cuh", "fa_cache_append.cuh", "fa_cache_prompt.cuh", "fa_cache_rows.cuh", "fa_cache_select.cuh", "fa_host.cuh", "fa_ptx.cuh"),
-    "fa_latent": ("fa_cache.cuh", "fa_latent.cuh", "fa_latent_rows.cuh", "fa_host.cuh", "fa_ptx.cuh"),
+    "fa_latent": ("fa_cache.cuh", "fa_latent.cuh", "fa_latent_prompt.cuh", "fa_latent_rows.cuh", "fa_host.cuh", "fa_ptx.cuh"),
     "fa_pages": ("fa_cache.cuh", "fa_pages.cuh", "fa_host.cuh", "fa_ptx.cuh"),
 }
 

@@ -6,6 +6,7 @@
 #include "fa_b200.h"
 #include "fa_host.cuh"
 #include "fa_latent.cuh"
+#include "fa_latent_prompt.cuh"
 #include "fa_latent_rows.cuh"
 
 namespace {
@@ -219,6 +220,78 @@ int fa_b200_latent_attention(const fa_b200_latent_cache* cache, const fa_b200_se
         case 256: return launch_rows<4>(*d, 3, map, a, plan.n, stream);
         default: return launch_rows<8>(*d, 6, map, a, plan.n, stream);
     }
+}
+
+int fa_b200_latent_prompt(const void* q_nope, int64_t qn_batch_stride, int64_t qn_token_stride, int64_t qn_head_stride, const void* q_rope, int64_t qr_batch_stride,
+                          int64_t qr_token_stride, int64_t qr_head_stride, const void* expanded, int64_t kv_batch_stride, int64_t kv_token_stride,
+                          int64_t kv_head_stride, const void* rope_keys, int64_t rk_batch_stride, int64_t rk_token_stride, const int32_t* lengths_or_null,
+                          const int32_t* counts_or_null, uint32_t B, uint32_t T, uint32_t S, uint32_t heads, uint32_t nope_dim, uint32_t rope_dim, float scale,
+                          uint32_t dtype, uint32_t flags, void* y, int device, void* cuda_stream) {
+    int rc = rows_ok(q_nope, {qn_batch_stride, qn_token_stride, qn_head_stride});
+    if (rc == FA_B200_OK) rc = rows_ok(q_rope, {qr_batch_stride, qr_token_stride, qr_head_stride});
+    if (rc == FA_B200_OK) rc = rows_ok(expanded, {kv_batch_stride, kv_token_stride, kv_head_stride});
+    if (rc == FA_B200_OK) rc = rows_ok(rope_keys, {rk_batch_stride, rk_token_stride});
+    if (rc == FA_B200_OK) rc = rows_ok(y, {});
+    if (rc != FA_B200_OK) return rc;
+    if ((reinterpret_cast<uintptr_t>(lengths_or_null) | reinterpret_cast<uintptr_t>(counts_or_null)) & 3u) return FA_B200_ERR_ALIGNMENT;
+    if ((nope_dim != 64 && nope_dim != 128) || (rope_dim != 16 && rope_dim != 32 && rope_dim != 64)) return FA_B200_ERR_HEAD_DIM;
+    if (dtype > FA_B200_BF16) return FA_B200_ERR_DTYPE;
+    if (flags & ~FA_B200_CACHE_ALL_KEYS) return FA_B200_ERR_FLAGS;
+    if (B == 0 || T == 0 || S == 0 || heads == 0 || B > (1u << 24) || T > 0x3FFFFFFFu || S > 0x3FFFFFFFu || heads > (1u << 20) || !(scale > 0.0f) || !std::isfinite(scale)) return FA_B200_ERR_SHAPE;
+    const uint64_t pairs = (static_cast<uint64_t>(T) + 2 * fa::kExpandTile - 1) / (2 * fa::kExpandTile), items = pairs * B * heads;
+    if (static_cast<uint64_t>(B) * heads > kMostCtas || items > kMostCtas) return FA_B200_ERR_SHAPE;
+    fa::ExpandArgs a = {};
+    a.lengths = lengths_or_null, a.counts = counts_or_null, a.y = static_cast<uint8_t*>(y);
+    a.B = B, a.T = T, a.S = S, a.heads = heads, a.pairs = static_cast<uint32_t>(pairs), a.rope = rope_dim;
+    a.causal = (flags & FA_B200_CACHE_ALL_KEYS) ? 0u : 1u, a.bf16 = dtype == FA_B200_BF16, a.scale_log2 = static_cast<float>(scale * kLog2e);
+    Device* d = nullptr;
+    if ((rc = device_of(device, &d)) != FA_B200_OK) return rc;
+    OnDevice on(device);
+    if (on.rc != 0) return on.rc;
+    // {dimensions, heads, tokens, sequences}; boxes of 64 dimensions of one head by 128 tokens.  An axis of one is nowhere stepped along.
+    auto map_of = [&](CUtensorMap* map, const void* base, uint32_t dim, uint32_t n_heads, uint32_t tokens, int64_t batch, int64_t token, int64_t head) {
+        const cuuint64_t dims[4] = {dim, n_heads, tokens, B};
+        const cuuint64_t strides[3] = {static_cast<cuuint64_t>(n_heads > 1 ? 2 * head : 16), static_cast<cuuint64_t>(tokens > 1 ? 2 * token : 16),
+                                       static_cast<cuuint64_t>(B > 1 ? 2 * batch : 16)};
+        const cuuint32_t box[4] = {64, 1, fa::kExpandTile, 1};
+        return make_map<4>(map, base, dims, strides, box);
+    };
+    for (const int64_t stride : {B > 1 ? qn_batch_stride : 1, T > 1 ? qn_token_stride : 1, heads > 1 ? qn_head_stride : 1, B > 1 ? qr_batch_stride : 1,
+                                 T > 1 ? qr_token_stride : 1, heads > 1 ? qr_head_stride : 1, B > 1 ? kv_batch_stride : 1, S > 1 ? kv_token_stride : 1,
+                                 heads > 1 ? kv_head_stride : 1, B > 1 ? rk_batch_stride : 1, S > 1 ? rk_token_stride : 1})
+        if (stride <= 0 || stride >= (1ll << 38)) return FA_B200_ERR_SHAPE;
+    CUtensorMap q, qr, kv, r;
+    rc = map_of(&q, q_nope, nope_dim, heads, T, qn_batch_stride, qn_token_stride, qn_head_stride);
+    if (rc == FA_B200_OK) rc = map_of(&qr, q_rope, rope_dim, heads, T, qr_batch_stride, qr_token_stride, qr_head_stride);
+    if (rc == FA_B200_OK) rc = map_of(&kv, expanded, 2 * nope_dim, heads, S, kv_batch_stride, kv_token_stride, kv_head_stride);
+    if (rc == FA_B200_OK) rc = map_of(&r, rope_keys, rope_dim, 1, S, rk_batch_stride, rk_token_stride, 0);
+    if (rc != FA_B200_OK) return rc;
+    const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+#ifdef FA_DEBUG
+    if (const cudaError_t e = cudaMemsetAsync(y, 0xFF, 2ull * B * T * heads * nope_dim, stream)) return static_cast<int>(e);
+#endif
+    if (nope_dim == 64) {
+        if ((rc = allow_smem(*d, 9, &fa::fa_latent_prompt<64>, fa::ExpandCfg<64>::kSmemBytes)) != FA_B200_OK) return rc;
+        return launch(&fa::fa_latent_prompt<64>, static_cast<uint32_t>(items), fa::kExpandThreads, fa::ExpandCfg<64>::kSmemBytes, stream, q, qr, kv, r, a);
+    }
+    if ((rc = allow_smem(*d, 10, &fa::fa_latent_prompt<128>, fa::ExpandCfg<128>::kSmemBytes)) != FA_B200_OK) return rc;
+    return launch(&fa::fa_latent_prompt<128>, static_cast<uint32_t>(items), fa::kExpandThreads, fa::ExpandCfg<128>::kSmemBytes, stream, q, qr, kv, r, a);
+}
+
+int fa_b200_latent_status(int device, uint32_t out[2]) {
+    if (!out) return FA_B200_ERR_NULL_POINTER;
+    Device* d = nullptr;
+    const int rc = device_of(device, &d);
+    if (rc != FA_B200_OK) return rc;
+    OnDevice on(device);
+    if (on.rc != 0) return on.rc;
+    cudaError_t e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(out, fa::g_latent_status, 2 * sizeof(uint32_t));
+    if (e == cudaSuccess && (out[0] != 0 || out[1] != 0)) {
+        const uint32_t zero[2] = {0, 0};
+        e = cudaMemcpyToSymbol(fa::g_latent_status, zero, sizeof(zero));
+    }
+    return static_cast<int>(e);
 }
 
 }  // extern "C"

@@ -198,3 +198,51 @@ def latent_attention(cache: LatentCache, q_latent: torch.Tensor, q_rope: torch.T
         ctypes.byref(cache._handle), ctypes.byref(sequences), q_latent.data_ptr(), *_strides(q_latent), q_rope.data_ptr(), *_strides(q_rope), heads, scale,
         _DTYPES[cache.dtype], 0 if causal else _lib.CACHE_ALL_KEYS, out.data_ptr(), scratch.data_ptr(), scratch.numel(), cache._index, _raw_stream(cache._index)))
     return out
+
+
+def latent_prompt(q_nope: torch.Tensor, q_rope: torch.Tensor, expanded: torch.Tensor, rope_keys: torch.Tensor, *, scale: Optional[float] = None,
+                  lengths: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None, causal: bool = True,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of T queries a sequence with the keys and values of every head multiplied out of the latent vectors, [B, T, heads, nope_dim].
+
+    ``q_nope``    [B, T, heads, nope_dim] (64 or 128);  ``q_rope`` [B, T, heads, rope_dim], rotated
+    ``expanded``  [B, S, heads, 2 * nope_dim]: of each head its own part of the keys and behind it the values, ``latents @ W`` as it comes
+    ``rope_keys`` [B, S, rope_dim], rotated (``latent_append`` returns those of its tokens): the rest of the keys, the same for all heads
+    ``lengths``   int32 [B]: how many of the S tokens sequence b has (default: all);  ``counts`` int32 [B]: how many of the T queries (default: all)
+
+    ``softmax(scale (q_nope . k + q_rope . r)) v``, with ``scale`` ``(nope_dim + rope_dim) ** -0.5`` unless given.  The queries are the last tokens of
+    their sequences, as in ``latent_attention``, ``causal=False`` too.  A query that sees nothing, or that its sequence does not have, gets
+    zeros.  Keys and values that a query does not see do not reach it, whatever they hold.  Scores, maxima and sums are held in 32 bits; weights
+    are rounded to the tensors' type for their product with the values.  ``latent_status`` tells of lengths and counts outside, which are cut.
+    """
+    _check_rows(q_nope, "q_nope", None, None, (None, None, None, None))
+    B, T, heads, nope = q_nope.shape
+    index, dtype = q_nope.get_device(), q_nope.dtype
+    _require(nope in (64, 128), "nope_dim must be 64 or 128")
+    _check_rows(q_rope, "q_rope", dtype, index, (B, T, heads, None))
+    rope = q_rope.shape[3]
+    _require(rope in ROPE_DIMS, "rope_dim must be 16, 32 or 64")
+    _check_rows(expanded, "expanded", dtype, index, (B, None, heads, 2 * nope))
+    S = expanded.shape[1]
+    _check_rows(rope_keys, "rope_keys", dtype, index, (B, S, rope))
+    for t, name in ((q_nope, "q_nope"), (q_rope, "q_rope"), (expanded, "expanded"), (rope_keys, "rope_keys")):
+        _require(all(s > 0 or n == 1 for s, n in zip(t.stride(), t.shape)), f"the strides of {name} must be positive")
+    for t, name in ((lengths, "lengths"), (counts, "counts")):
+        if t is not None:
+            _require(isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.is_cuda and t.get_device() == index, f"{name} must be an int32 tensor on the queries' device")
+            _require(tuple(t.shape) == (B,) and (B == 1 or t.stride(0) == 1), f"{name} must be contiguous, of shape [B]")
+    scale = (nope + rope) ** -0.5 if scale is None else _check_scale(scale)
+    out = _check_out(out, q_nope, (B, T, heads, nope), index)
+    _lib.check(_lib.load().fa_b200_latent_prompt(
+        q_nope.data_ptr(), *_strides(q_nope), q_rope.data_ptr(), *_strides(q_rope), expanded.data_ptr(), *_strides(expanded), rope_keys.data_ptr(), *_strides(rope_keys),
+        None if lengths is None else lengths.data_ptr(), None if counts is None else counts.data_ptr(), B, T, S, heads, nope, rope, scale, _DTYPES[dtype],
+        0 if causal else _lib.CACHE_ALL_KEYS, out.data_ptr(), index, _raw_stream(index)))
+    return out
+
+
+def latent_status(device: int = 0) -> Tuple[int, int]:
+    """(first code, number of reports) of what ``latent_prompt``'s kernels found wrong on a device; clears it.  Synchronises.  The codes are those
+    of ``cache.STATUS``."""
+    out = (ctypes.c_uint32 * 2)()
+    _lib.check(_lib.load().fa_b200_latent_status(device, out))
+    return out[0], out[1]

@@ -486,6 +486,24 @@ int fa_b200_latent_attention(const fa_b200_latent_cache* cache, const fa_b200_se
 /* out[0] = bytes of scratch that such a call needs, on a 16-byte boundary.  Pure arithmetic on the device's facts. */
 int fa_b200_latent_attention_scratch(uint32_t latent_dim, uint32_t heads, uint32_t page_size, uint32_t B, uint32_t T, uint32_t table_width, int device, uint64_t out[1]);
 
+/*
+ * The same attention with keys and values multiplied out of the latent vectors, for prompts: queries [B, T, heads, nope_dim] and
+ * [B, T, heads, rope_dim] (rotated), expanded [B, S, heads, 2 * nope_dim], of each head its own part of the keys and behind it the values,
+ * rope_keys [B, S, rope_dim] (rotated), the same for all heads; y [B, T, heads, nope_dim] contiguous.  nope_dim 64 or 128, rope_dim 16, 32 or 64.
+ * y = softmax(scale * (q_nope . k + q_rope . r)) v, the queries the last counts[b] (NULL: T) of the lengths[b] (NULL: S) tokens of their
+ * sequences; FA_B200_CACHE_ALL_KEYS as above.  Strides in elements, positive where an axis has more than one entry.  Scores, sums and maxima are
+ * held in fp32, weights are rounded to the type for their product with v.  Keys that a query does not see do not reach it, whatever they hold.
+ */
+int fa_b200_latent_prompt(const void* q_nope, int64_t qn_batch_stride, int64_t qn_token_stride, int64_t qn_head_stride, const void* q_rope, int64_t qr_batch_stride,
+                          int64_t qr_token_stride, int64_t qr_head_stride, const void* expanded, int64_t kv_batch_stride, int64_t kv_token_stride,
+                          int64_t kv_head_stride, const void* rope_keys, int64_t rk_batch_stride, int64_t rk_token_stride, const int32_t* lengths_or_null,
+                          const int32_t* counts_or_null, uint32_t B, uint32_t T, uint32_t S, uint32_t heads, uint32_t nope_dim, uint32_t rope_dim, float scale,
+                          uint32_t dtype, uint32_t flags, void* y, int device, void* cuda_stream);
+
+/* out[0], out[1] = first code and number of reports of fa_b200_latent_prompt's launches on the device (2: a length or count outside, cut;
+ * 0x100 and above: a bounded wait expired); cleared when read.  Synchronises the device. */
+int fa_b200_latent_status(int device, uint32_t out[2]);
+
 #ifdef __cplusplus
 }
 #endif
