@@ -189,6 +189,9 @@ def load() -> ctypes.CDLL:
         # for the extension module's calls
         lib.cache_entries = tuple(ctypes.cast(f, vp).value for f in (lib.fa_b200_cache_append, lib.fa_b200_cache_select, lib.fa_b200_cache_attention,
                                                                      lib.fa_b200_cache_attention_scratch))
+        lib.latent_entries = tuple(ctypes.cast(f, vp).value for f in (lib.fa_b200_latent_append, lib.fa_b200_latent_attention, lib.fa_b200_latent_attention_scratch,
+                                                                      lib.fa_b200_latent_prompt))
+        lib.pages_entries = tuple(ctypes.cast(f, vp).value for f in (lib.fa_b200_pages_fork, lib.fa_b200_pages_reserve, lib.fa_b200_pages_compact, lib.fa_b200_cache_copy))
         _lib = lib
         return lib
 

@@ -16,6 +16,9 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <algorithm>
+#include <cmath>
+#include <limits>
+#include <vector>
 
 #include "fa_b200.h"
 
@@ -275,6 +278,257 @@ PyObject* cache_attention_through(PyObject*, PyObject* const* args, Py_ssize_t n
     END_HANDLE_TH_ERRORS
 }
 
+// ---- The calls of the latent cache and of pages, in the same manner.
+// 16-bit values of `type` on `device`, with every row on a 16-byte boundary; strides: of all axes but the last, 0 for one that is nowhere stepped along.
+bool plain_16bit(PyObject* o, at::Tensor& t, int device, int64_t dims, at::ScalarType type, int64_t* strides) {
+    if (!plain_cuda(o, t, device, dims) || t.scalar_type() != type || t.numel() == 0 || t.stride(dims - 1) != 1 || (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) != 0) return false;
+    for (int64_t i = 0; i + 1 < dims; ++i) {
+        strides[i] = t.size(i) > 1 ? t.stride(i) : 0;
+        if (strides[i] % 8 != 0 || t.size(i) > UINT32_MAX) return false;
+    }
+    return true;
+}
+bool dtype_code(PyObject* o, at::ScalarType& type) {
+    int64_t code = 0;
+    if (!whole(o, code) || code < 0 || code > 1) return false;
+    type = code == FA_B200_FP16 ? at::kHalf : at::kBFloat16;
+    return true;
+}
+// cos and sin, float32 [positions, half] each, from a tuple
+bool plain_rotation(PyObject* o, at::Tensor& cos, at::Tensor& sin, int device, int64_t half) {
+    if (!PyTuple_CheckExact(o) || PyTuple_GET_SIZE(o) != 2) return false;
+    for (int i = 0; i < 2; ++i) {
+        at::Tensor& t = i ? sin : cos;
+        if (!plain_cuda(PyTuple_GET_ITEM(o, i), t, device, 2) || t.scalar_type() != at::kFloat || t.size(1) != half || t.size(0) <= 0 || !t.is_contiguous() ||
+            (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) != 0 || t.sizes() != cos.sizes())
+            return false;
+    }
+    return true;
+}
+// A number above zero and below infinity, from a Python float or int.
+bool positive(PyObject* o, float& x) {
+    if (!PyFloat_CheckExact(o)) return false;
+    const double d = PyFloat_AS_DOUBLE(o);
+    x = static_cast<float>(d);
+    return x > 0.0f && x < std::numeric_limits<float>::infinity();
+}
+
+// (entry, cache, device, dtype, latents, rope_keys, table, lengths, counts, queries, rotation, interleaved) -> (keys, queries or None)
+PyObject* latent_append_through(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    int64_t device = 0;
+    at::ScalarType type;
+    if (n != 12 || at::impl::PythonTorchFunctionTLS::stack_len() > 0 || !whole(args[2], device) || !dtype_code(args[3], type)) Py_RETURN_NONE;
+    auto* const entry = address<decltype(fa_b200_latent_append)>(args[0]);
+    auto* const cache = address<const fa_b200_latent_cache>(args[1]);
+    if (!entry || !cache) Py_RETURN_NONE;
+    const int dev = static_cast<int>(device);
+    at::Tensor c, k, q, cos, sin, rotated;
+    int64_t cs[2], ks[2], qs[3] = {0, 0, 0};
+    Sequences seqs;
+    if (!plain_16bit(args[4], c, dev, 3, type, cs) || c.size(2) != cache->latent_dim || !plain_16bit(args[5], k, dev, 3, type, ks) || k.size(0) != c.size(0) ||
+        k.size(1) != c.size(1) || k.size(2) != cache->rope_dim || !seqs.take(args[6], args[7], args[8], dev, c))
+        Py_RETURN_NONE;
+    const bool with_q = args[9] != Py_None, turned = args[10] != Py_None;
+    if (with_q && (!plain_16bit(args[9], q, dev, 4, type, qs) || q.size(0) != c.size(0) || q.size(1) != c.size(1) || q.size(3) != cache->rope_dim)) Py_RETURN_NONE;
+    if (turned && !plain_rotation(args[10], cos, sin, dev, cache->rope_dim / 2)) Py_RETURN_NONE;
+    const int neighbours = PyObject_IsTrue(args[11]);
+    if (neighbours < 0) return nullptr;
+    at::Tensor keys = at::empty(k.sizes(), k.options());
+    if (with_q) rotated = at::empty(q.sizes(), q.options());
+    const int rc = entry(cache, &seqs.s, c.data_ptr(), cs[0], cs[1], k.data_ptr(), ks[0], ks[1], with_q ? q.data_ptr() : nullptr, qs[0], qs[1], qs[2],
+                         with_q ? static_cast<uint32_t>(q.size(2)) : 0, keys.data_ptr(), with_q ? rotated.data_ptr() : nullptr, turned ? cos.data_ptr<float>() : nullptr,
+                         turned ? sin.data_ptr<float>() : nullptr, turned ? static_cast<uint32_t>(std::min<int64_t>(cos.size(0), 0x7FFFFFFF)) : 0, dtype_of(c),
+                         neighbours ? FA_B200_CACHE_NEIGHBOURS : 0, dev, stream_of(dev));
+    if (rc != FA_B200_OK) return PyLong_FromLong(rc);
+    THPObjectPtr first(THPVariable_Wrap(std::move(keys))), second(with_q ? THPVariable_Wrap(std::move(rotated)) : Py_NewRef(Py_None));
+    if (!first || !second) return nullptr;
+    return PyTuple_Pack(2, first.get(), second.get());
+    END_HANDLE_TH_ERRORS
+}
+
+// (entry, entry for the scratch's size, cache, device, dtype, q_latent, q_rope, table, lengths, scale, counts, causal, out) -> y
+PyObject* latent_attention_through(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    int64_t device = 0;
+    at::ScalarType type;
+    float scale = 0;
+    if (n != 13 || at::impl::PythonTorchFunctionTLS::stack_len() > 0 || !whole(args[3], device) || !dtype_code(args[4], type) || !positive(args[9], scale)) Py_RETURN_NONE;
+    auto* const entry = address<decltype(fa_b200_latent_attention)>(args[0]);
+    auto* const size_of = address<decltype(fa_b200_latent_attention_scratch)>(args[1]);
+    auto* const cache = address<const fa_b200_latent_cache>(args[2]);
+    if (!entry || !size_of || !cache) Py_RETURN_NONE;
+    const int dev = static_cast<int>(device);
+    at::Tensor ql, qr, out;
+    int64_t ls[3], rs[3], os[3];
+    Sequences seqs;
+    if (!plain_16bit(args[5], ql, dev, 4, type, ls) || ql.size(3) != cache->latent_dim || !plain_16bit(args[6], qr, dev, 4, type, rs) || qr.size(0) != ql.size(0) ||
+        qr.size(1) != ql.size(1) || qr.size(2) != ql.size(2) || qr.size(3) != cache->rope_dim || !seqs.take(args[7], args[8], args[10], dev, ql))
+        Py_RETURN_NONE;
+    const bool given = args[12] != Py_None;
+    if (given && (!plain_16bit(args[12], out, dev, 4, type, os) || out.sizes() != ql.sizes() || !out.is_contiguous())) Py_RETURN_NONE;
+    const int causal = PyObject_IsTrue(args[11]);
+    if (causal < 0) return nullptr;
+    const uint32_t heads = static_cast<uint32_t>(ql.size(2));
+    uint64_t bytes[1] = {0};
+    int rc = size_of(cache->latent_dim, heads, cache->page_size, seqs.s.B, seqs.s.T, seqs.s.table_width, dev, bytes);
+    if (rc != FA_B200_OK) return PyLong_FromLong(rc);
+    if (!given) out = at::empty(ql.sizes(), ql.options());
+    const at::Tensor scratch = at::empty({static_cast<int64_t>(bytes[0])}, ql.options().dtype(at::kByte));
+    rc = entry(cache, &seqs.s, ql.data_ptr(), ls[0], ls[1], ls[2], qr.data_ptr(), rs[0], rs[1], rs[2], heads, scale, dtype_of(ql), causal ? 0 : FA_B200_CACHE_ALL_KEYS,
+               out.data_ptr(), scratch.data_ptr(), bytes[0], dev, stream_of(dev));
+    if (rc != FA_B200_OK) return PyLong_FromLong(rc);
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// (entry, q_nope, q_rope, expanded, rope_keys, scale or None, lengths, counts, causal, out) -> y
+PyObject* latent_prompt_through(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 10 || at::impl::PythonTorchFunctionTLS::stack_len() > 0 || !THPVariable_CheckExact(args[1])) Py_RETURN_NONE;
+    auto* const entry = address<decltype(fa_b200_latent_prompt)>(args[0]);
+    if (!entry) Py_RETURN_NONE;
+    const at::Tensor& first = THPVariable_Unpack(args[1]);
+    if (!first.defined() || !first.is_cuda() || (first.scalar_type() != at::kHalf && first.scalar_type() != at::kBFloat16)) Py_RETURN_NONE;
+    const int dev = first.get_device();
+    const at::ScalarType type = first.scalar_type();
+    at::Tensor qn, qr, kv, rk, lengths, counts, out;
+    int64_t ns[3], rs[3], vs[3], ks[2], os[3];
+    if (!plain_16bit(args[1], qn, dev, 4, type, ns) || !plain_16bit(args[2], qr, dev, 4, type, rs) || !plain_16bit(args[3], kv, dev, 4, type, vs) ||
+        !plain_16bit(args[4], rk, dev, 3, type, ks))
+        Py_RETURN_NONE;
+    const int64_t B = qn.size(0), T = qn.size(1), heads = qn.size(2), nope = qn.size(3), rope = qr.size(3), S = kv.size(1);
+    if ((nope != 64 && nope != 128) || (rope != 16 && rope != 32 && rope != 64) || qr.size(0) != B || qr.size(1) != T || qr.size(2) != heads || kv.size(0) != B ||
+        kv.size(2) != heads || kv.size(3) != 2 * nope || rk.size(0) != B || rk.size(1) != S || rk.size(2) != rope)
+        Py_RETURN_NONE;
+    float scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(nope + rope)));
+    if (args[5] != Py_None && !positive(args[5], scale)) Py_RETURN_NONE;
+    if ((args[6] != Py_None && !plain_ints(args[6], lengths, dev, 1, B)) || (args[7] != Py_None && !plain_ints(args[7], counts, dev, 1, B))) Py_RETURN_NONE;
+    const int causal = PyObject_IsTrue(args[8]);
+    if (causal < 0) return nullptr;
+    const bool given = args[9] != Py_None;
+    if (given && (!plain_16bit(args[9], out, dev, 4, type, os) || out.size(0) != B || out.size(1) != T || out.size(2) != heads || out.size(3) != nope || !out.is_contiguous())) Py_RETURN_NONE;
+    for (const int64_t stride : {B > 1 ? ns[0] : 1, T > 1 ? ns[1] : 1, heads > 1 ? ns[2] : 1, B > 1 ? rs[0] : 1, T > 1 ? rs[1] : 1, heads > 1 ? rs[2] : 1, B > 1 ? vs[0] : 1,
+                                 S > 1 ? vs[1] : 1, heads > 1 ? vs[2] : 1, B > 1 ? ks[0] : 1, S > 1 ? ks[1] : 1})
+        if (stride <= 0) Py_RETURN_NONE;
+    if (!given) out = at::empty({B, T, heads, nope}, qn.options());
+    const int rc = entry(qn.data_ptr(), ns[0], ns[1], ns[2], qr.data_ptr(), rs[0], rs[1], rs[2], kv.data_ptr(), vs[0], vs[1], vs[2], rk.data_ptr(), ks[0], ks[1],
+                         lengths.defined() ? lengths.data_ptr<int32_t>() : nullptr, counts.defined() ? counts.data_ptr<int32_t>() : nullptr, static_cast<uint32_t>(B),
+                         static_cast<uint32_t>(T), static_cast<uint32_t>(S), static_cast<uint32_t>(heads), static_cast<uint32_t>(nope), static_cast<uint32_t>(rope), scale,
+                         dtype_of(qn), causal ? 0 : FA_B200_CACHE_ALL_KEYS, out.data_ptr(), dev, stream_of(dev));
+    if (rc != FA_B200_OK) return PyLong_FromLong(rc);
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// A table [B, W] of whole numbers whose rows do not overlap.
+bool plain_table(PyObject* o, at::Tensor& t, int device) {
+    return plain_cuda(o, t, device, 2) && t.scalar_type() == at::kInt && t.size(0) > 0 && t.size(1) > 0 && t.size(0) <= UINT32_MAX && t.size(1) <= 0x7FFFFFFF &&
+           (t.size(1) == 1 || t.stride(1) == 1) && (t.size(0) == 1 || t.stride(0) >= t.size(1));
+}
+
+// (entry, pool, device, table, lengths, parents) -> True
+PyObject* pages_fork_through(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    int64_t device = 0;
+    if (n != 6 || at::impl::PythonTorchFunctionTLS::stack_len() > 0 || !whole(args[2], device)) Py_RETURN_NONE;
+    auto* const entry = address<decltype(fa_b200_pages_fork)>(args[0]);
+    auto* const pool = address<const fa_b200_pages>(args[1]);
+    if (!entry || !pool) Py_RETURN_NONE;
+    const int dev = static_cast<int>(device);
+    at::Tensor table, lengths, parents;
+    if (!plain_table(args[3], table, dev) || !plain_ints(args[4], lengths, dev, 1, table.size(0)) || !plain_ints(args[5], parents, dev, 1, table.size(0)) || table.size(0) > 57344)
+        Py_RETURN_NONE;
+    const int rc = entry(pool, table.data_ptr<int32_t>(), table.stride(0), static_cast<uint32_t>(table.size(1)), static_cast<uint32_t>(table.size(0)),
+                         lengths.data_ptr<int32_t>(), parents.data_ptr<int32_t>(), dev, stream_of(dev));
+    if (rc != FA_B200_OK) return PyLong_FromLong(rc);
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// (entry, pool, device, table, lengths, counts, page_size) -> (granted, sources, targets)
+PyObject* pages_reserve_through(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    int64_t device = 0, page = 0, count = 0;
+    if (n != 7 || at::impl::PythonTorchFunctionTLS::stack_len() > 0 || !whole(args[2], device) || !whole(args[6], page) || (page != 16 && page != 32 && page != 64 && page != 128))
+        Py_RETURN_NONE;
+    auto* const entry = address<decltype(fa_b200_pages_reserve)>(args[0]);
+    auto* const pool = address<const fa_b200_pages>(args[1]);
+    if (!entry || !pool) Py_RETURN_NONE;
+    const int dev = static_cast<int>(device);
+    at::Tensor table, lengths, counts;
+    if (!plain_table(args[3], table, dev) || !plain_ints(args[4], lengths, dev, 1, table.size(0))) Py_RETURN_NONE;
+    if (PyLong_CheckExact(args[5])) {
+        if (!whole(args[5], count) || count < 0 || count > 0x7FFFFFFF) Py_RETURN_NONE;
+    } else if (!plain_ints(args[5], counts, dev, 1, table.size(0))) {
+        Py_RETURN_NONE;
+    }
+    const int64_t B = table.size(0);
+    const at::Tensor all = at::empty({3, B}, table.options()), scratch = at::empty({static_cast<int64_t>(pool->n_pages)}, table.options());
+    int32_t* const to = all.data_ptr<int32_t>();
+    const int rc = entry(pool, table.data_ptr<int32_t>(), table.stride(0), static_cast<uint32_t>(table.size(1)), static_cast<uint32_t>(B), lengths.data_ptr<int32_t>(),
+                         counts.defined() ? counts.data_ptr<int32_t>() : nullptr, static_cast<uint32_t>(count), static_cast<uint32_t>(page), to, to + B, to + 2 * B,
+                         scratch.data_ptr(), 4 * static_cast<uint64_t>(pool->n_pages), dev, stream_of(dev));
+    if (rc != FA_B200_OK) return PyLong_FromLong(rc);
+    THPObjectPtr a(THPVariable_Wrap(all.select(0, 0))), b(THPVariable_Wrap(all.select(0, 1))), c(THPVariable_Wrap(all.select(0, 2)));
+    if (!a || !b || !c) return nullptr;
+    return PyTuple_Pack(3, a.get(), b.get(), c.get());
+    END_HANDLE_TH_ERRORS
+}
+
+// (entry, pool, device, table) -> (refs, table, sources, targets)
+PyObject* pages_compact_through(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    int64_t device = 0;
+    if (n != 4 || at::impl::PythonTorchFunctionTLS::stack_len() > 0 || !whole(args[2], device)) Py_RETURN_NONE;
+    auto* const entry = address<decltype(fa_b200_pages_compact)>(args[0]);
+    auto* const pool = address<const fa_b200_pages>(args[1]);
+    if (!entry || !pool) Py_RETURN_NONE;
+    const int dev = static_cast<int>(device);
+    at::Tensor table;
+    if (!plain_table(args[3], table, dev)) Py_RETURN_NONE;
+    const int64_t pages = pool->n_pages;
+    at::Tensor refs = at::empty({pages}, table.options()), renumbered = at::empty({table.size(0), table.size(1)}, table.options());
+    const at::Tensor moves = at::empty({2, pages}, table.options()), scratch = at::empty({pages + 2}, table.options());
+    int32_t* const to = moves.data_ptr<int32_t>();
+    const int rc = entry(pool, table.data_ptr<int32_t>(), table.stride(0), static_cast<uint32_t>(table.size(1)), static_cast<uint32_t>(table.size(0)), refs.data_ptr<int32_t>(),
+                         renumbered.data_ptr<int32_t>(), to, to + pages, scratch.data_ptr(), 4 * static_cast<uint64_t>(pages) + 8, dev, stream_of(dev));
+    if (rc != FA_B200_OK) return PyLong_FromLong(rc);
+    THPObjectPtr a(THPVariable_Wrap(std::move(refs))), b(THPVariable_Wrap(std::move(renumbered))), c(THPVariable_Wrap(moves.select(0, 0))), d(THPVariable_Wrap(moves.select(0, 1)));
+    if (!a || !b || !c || !d) return nullptr;
+    return PyTuple_Pack(4, a.get(), b.get(), c.get(), d.get());
+    END_HANDLE_TH_ERRORS
+}
+
+// (entry, ((address of areas, how many), ...) by cache, pages of a cache, address of the status, device, sources, targets) -> True
+PyObject* cache_copy_through(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    int64_t pages = 0, device = 0;
+    if (n != 7 || at::impl::PythonTorchFunctionTLS::stack_len() > 0 || !PyTuple_CheckExact(args[1]) || !whole(args[2], pages) || !whole(args[4], device)) Py_RETURN_NONE;
+    auto* const entry = address<decltype(fa_b200_cache_copy)>(args[0]);
+    auto* const status = address<uint32_t>(args[3]);
+    if (!entry || !status) Py_RETURN_NONE;
+    const int dev = static_cast<int>(device);
+    at::Tensor sources, targets;
+    if (!plain_cuda(args[5], sources, dev, 1) || sources.scalar_type() != at::kInt || sources.numel() == 0 || sources.numel() > 0x7FFFFFFF ||
+        (sources.numel() > 1 && sources.stride(0) != 1) || !plain_ints(args[6], targets, dev, 1, sources.size(0)))
+        Py_RETURN_NONE;
+    std::vector<fa_b200_copy_area> areas;
+    for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(args[1]); ++i) {
+        PyObject* const cache = PyTuple_GET_ITEM(args[1], i);
+        int64_t count = 0;
+        if (!PyTuple_CheckExact(cache) || PyTuple_GET_SIZE(cache) < 2 || !whole(PyTuple_GET_ITEM(cache, 1), count)) Py_RETURN_NONE;
+        auto* const from = address<const fa_b200_copy_area>(PyTuple_GET_ITEM(cache, 0));
+        if (!from) Py_RETURN_NONE;
+        areas.insert(areas.end(), from, from + count);
+    }
+    const int rc = entry(areas.data(), static_cast<uint32_t>(areas.size()), static_cast<uint32_t>(pages), sources.data_ptr<int32_t>(), targets.data_ptr<int32_t>(),
+                         static_cast<uint32_t>(sources.numel()), status, dev, stream_of(dev));
+    if (rc != FA_B200_OK) return PyLong_FromLong(rc);
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
 template <PyObject* (*kFunction)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyObject* native_function(const char* name) {
     static PyMethodDef def = {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kFunction)), METH_FASTCALL, nullptr};
@@ -291,4 +545,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.add_object("_cache_append_through", native_function<&cache_append_through>("_cache_append_through"));
     m.add_object("_cache_select_through", native_function<&cache_select_through>("_cache_select_through"));
     m.add_object("_cache_attention_through", native_function<&cache_attention_through>("_cache_attention_through"));
+    m.add_object("_latent_append_through", native_function<&latent_append_through>("_latent_append_through"));
+    m.add_object("_latent_attention_through", native_function<&latent_attention_through>("_latent_attention_through"));
+    m.add_object("_latent_prompt_through", native_function<&latent_prompt_through>("_latent_prompt_through"));
+    m.add_object("_pages_fork_through", native_function<&pages_fork_through>("_pages_fork_through"));
+    m.add_object("_pages_reserve_through", native_function<&pages_reserve_through>("_pages_reserve_through"));
+    m.add_object("_pages_compact_through", native_function<&pages_compact_through>("_pages_compact_through"));
+    m.add_object("_cache_copy_through", native_function<&cache_copy_through>("_cache_copy_through"));
 }

@@ -25,16 +25,29 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .api import _raw_stream
+from .api import _load_native, _raw_stream
 from .cache import PAGE_SIZES
 
 _DTYPES = {torch.float16: _lib.FP16, torch.bfloat16: _lib.BF16}
 LATENT_DIMS, ROPE_DIMS = (128, 256, 512), (16, 32, 64)
 
 
+_native = None   # the extension module's calls, and the library's entries that they go to
+
+
 def _require(cond: bool, what: str) -> None:
     if not cond:
         raise RuntimeError(f"latent: {what}")
+
+
+def _calls():
+    """(append, attention, prompt, entries): as in cache.py, None is the answer to what goes through the checks and ctypes below, an int the
+    status of a launch that failed."""
+    global _native
+    if _native is None:
+        lib = _lib.load()   # raises when the CUDA library is missing: no fallback
+        _native = tuple(_load_native(f"_latent_{name}_through") for name in ("append", "attention", "prompt")) + (lib.latent_entries,)
+    return _native
 
 
 class LatentCache:
@@ -54,7 +67,7 @@ class LatentCache:
         _require(data.stride(0) < 1 << 30 and data.stride(1) <= 1 << 23, "the strides of data must be below 2^30, its tokens' at most 2^23")
         _require(data.data_ptr() % 16 == 0, "data must start on a 16-byte boundary")
         self.data, self.n_pages, self.page_size, self.latent_dim, self.rope_dim = data, n, page, latent_dim, width - latent_dim
-        self.dtype, self.device, self._index = data.dtype, data.device, data.get_device()
+        self.dtype, self.device, self._index, self._code = data.dtype, data.device, data.get_device(), _DTYPES[data.dtype]
         self._status = torch.zeros(2, dtype=torch.int32, device=data.device)
         self._handle = _lib.LatentCache(data.data_ptr(), self._status.data_ptr(), 2 * data.stride(0), 2 * data.stride(1), n, page, latent_dim, self.rope_dim)
         self._address = ctypes.addressof(self._handle)
@@ -122,6 +135,13 @@ def latent_append(cache: LatentCache, latents: torch.Tensor, rope_keys: torch.Te
     appended to the same place (sequences may share full pages).
     """
     _require(isinstance(cache, LatentCache), "the first argument must be a LatentCache")
+    append, _, _, entries = _calls()
+    if cache._writable:
+        done = append(entries[0], cache._address, cache._index, cache._code, latents, rope_keys, table, lengths, counts, queries, rotation, interleaved)
+        if done is not None:
+            if done.__class__ is int:
+                _lib.check(done)
+            return done
     _check_rows(latents, "latents", cache.dtype, cache._index, (None, None, cache.latent_dim))
     B, T, _ = latents.shape
     _check_rows(rope_keys, "rope_keys", cache.dtype, cache._index, (B, T, cache.rope_dim))
@@ -187,6 +207,12 @@ def latent_attention(cache: LatentCache, q_latent: torch.Tensor, q_rope: torch.T
     and summed as rounded.
     """
     _require(isinstance(cache, LatentCache), "the first argument must be a LatentCache")
+    _, attention, _, entries = _calls()
+    y = attention(entries[1], entries[2], cache._address, cache._index, cache._code, q_latent, q_rope, table, lengths, scale, counts, causal, out)
+    if y is not None:
+        if y.__class__ is int:
+            _lib.check(y)
+        return y
     _check_rows(q_latent, "q_latent", cache.dtype, cache._index, (None, None, None, cache.latent_dim))
     B, T, heads, latent = q_latent.shape
     _check_rows(q_rope, "q_rope", cache.dtype, cache._index, (B, T, heads, cache.rope_dim))
@@ -215,6 +241,12 @@ def latent_prompt(q_nope: torch.Tensor, q_rope: torch.Tensor, expanded: torch.Te
     zeros.  Keys and values that a query does not see do not reach it, whatever they hold.  Scores, maxima and sums are held in 32 bits; weights
     are rounded to the tensors' type for their product with the values.  ``latent_status`` tells of lengths and counts outside, which are cut.
     """
+    _, _, prompt, entries = _calls()
+    y = prompt(entries[3], q_nope, q_rope, expanded, rope_keys, scale, lengths, counts, causal, out)
+    if y is not None:
+        if y.__class__ is int:
+            _lib.check(y)
+        return y
     _check_rows(q_nope, "q_nope", None, None, (None, None, None, None))
     B, T, heads, nope = q_nope.shape
     index, dtype = q_nope.get_device(), q_nope.dtype

@@ -18,12 +18,12 @@ table by streams.  There is no CPU path.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Sequence, Tuple, Union
+from typing import Optional, Tuple, Union
 
 import torch
 
 from . import _lib
-from .api import _raw_stream
+from .api import _load_native, _raw_stream
 from .cache import PAGE_SIZES, KVCache
 from .latent import LatentCache
 
@@ -32,21 +32,41 @@ STATUS = {0: "nothing", 1: "a table entry that is neither a page nor -1", 2: "a 
           4: "counts that do not fit the table"}
 
 
+_native = None   # the extension module's calls, and the library's entries that they go to
+
+
 def _require(cond: bool, what: str) -> None:
     if not cond:
         raise RuntimeError(f"pages: {what}")
 
 
+def _calls():
+    """(fork, reserve, compact, copy, entries): as in cache.py, None is the answer to what goes through the checks and ctypes below, an int the
+    status of a launch that failed."""
+    global _native
+    if _native is None:
+        lib = _lib.load()   # raises when the CUDA library is missing: no fallback
+        _native = tuple(_load_native(name) for name in ("_pages_fork_through", "_pages_reserve_through", "_pages_compact_through", "_cache_copy_through")) + (lib.pages_entries,)
+    return _native
+
+
+def _done(answer) -> bool:
+    if answer.__class__ is int:
+        _lib.check(answer)
+    return answer is not None
+
+
 class PagePool:
     """How many table entries hold each page: ``refs``, int32 [n_pages], contiguous; 0 is a free page."""
 
-    def __init__(self, refs: torch.Tensor):
+    def __init__(self, refs: torch.Tensor, _status: Optional[torch.Tensor] = None):
         _require(isinstance(refs, torch.Tensor) and refs.dtype == torch.int32, "refs must be an int32 tensor")
         _require(refs.is_cuda, "refs must be a CUDA tensor")
         _require(refs.dim() == 1 and 0 < refs.shape[0] < 0x7FFFFFFF and refs.is_contiguous(), "refs must be contiguous, of shape [n_pages]")
         self.refs, self.n_pages, self.device, self._index = refs, refs.shape[0], refs.device, refs.get_device()
-        self._status = torch.zeros(4, dtype=torch.int32, device=refs.device)
+        self._status = torch.zeros(4, dtype=torch.int32, device=refs.device) if _status is None else _status
         self._handle = _lib.Pages(refs.data_ptr(), self._status.data_ptr(), self.n_pages)
+        self._address = ctypes.addressof(self._handle)
 
     def read_status(self) -> Tuple[int, int]:
         """(first code, number of reports) of what the kernels found wrong; clears it.  Synchronises.  ``STATUS`` says what the codes mean."""
@@ -80,6 +100,10 @@ def pages_fork(pool: PagePool, table: torch.Tensor, lengths: torch.Tensor, paren
     written to a page of their own.  At most 57344 sequences.
     """
     _require(isinstance(pool, PagePool), "the first argument must be a PagePool")
+    fork, _, _, _, entries = _calls()
+    done = fork(entries[0], pool._address, pool._index, table, lengths, parents)
+    if _done(done):
+        return
     _check_ints(table, "table", pool, (None, None), True)
     B, W = table.shape
     _check_ints(lengths, "lengths", pool, (B,))
@@ -102,6 +126,10 @@ def pages_reserve(pool: PagePool, table: torch.Tensor, lengths: torch.Tensor, co
     ``granted[b]`` is counts[b], or fewer where pages ran out (or the table has no room): the ``counts`` of ``cache_append``.
     """
     _require(isinstance(pool, PagePool), "the first argument must be a PagePool")
+    _, reserve, _, _, entries = _calls()
+    done = reserve(entries[1], pool._address, pool._index, table, lengths, counts, page_size)
+    if _done(done):
+        return done
     _check_ints(table, "table", pool, (None, None), True)
     B, W = table.shape
     _check_ints(lengths, "lengths", pool, (B,))
@@ -127,6 +155,10 @@ def pages_compact(pool: PagePool, table: torch.Tensor) -> Tuple[PagePool, torch.
     old ones are left as they are.
     """
     _require(isinstance(pool, PagePool), "the first argument must be a PagePool")
+    _, _, compact, _, entries = _calls()
+    done = compact(entries[2], pool._address, pool._index, table)
+    if _done(done):
+        return (PagePool(done[0], pool._status),) + done[1:]
     _check_ints(table, "table", pool, (None, None))
     B, W = table.shape
     refs, sources, targets = torch.empty(3, pool.n_pages, dtype=torch.int32, device=pool.device).unbind(0)
@@ -135,11 +167,11 @@ def pages_compact(pool: PagePool, table: torch.Tensor) -> Tuple[PagePool, torch.
     _lib.check(_lib.load().fa_b200_pages_compact(
         ctypes.byref(pool._handle), table.data_ptr(), table.stride(0), W, B, refs.data_ptr(), new.data_ptr(), sources.data_ptr(), targets.data_ptr(),
         scratch.data_ptr(), 4 * scratch.numel(), pool._index, _raw_stream(pool._index)))
-    return PagePool(refs), new, sources, targets
+    return PagePool(refs, pool._status), new, sources, targets
 
 
 def _areas(cache):
-    """The arrays of a cache's pages as the library copies them; made once for each cache."""
+    """(address, how many, the array itself): the arrays of a cache's pages as the library copies them; made once for each cache."""
     if cache._copy_areas is None:
         if isinstance(cache, KVCache):
             n, heads, page, H = cache.k.shape
@@ -149,7 +181,8 @@ def _areas(cache):
         else:
             n, page, width = cache.data.shape
             areas = [_lib.CopyArea(cache.data.data_ptr(), 2 * cache.data.stride(0), 2 * cache.data.stride(1), 0, page, 1, 2 * width)]
-        cache._copy_areas = areas
+        array = (_lib.CopyArea * len(areas))(*areas)
+        cache._copy_areas = (ctypes.addressof(array), len(areas), array)
     return cache._copy_areas
 
 
@@ -165,11 +198,15 @@ def cache_copy(caches, sources: torch.Tensor, targets: torch.Tensor) -> None:
     first = caches[0]
     _require(all(c.n_pages == first.n_pages and c._index == first._index for c in caches), "the caches must have as many pages, on one device")
     _require(all(c._writable for c in caches), "the pages of a cache lie on top of one another: it cannot be copied to")
+    _, _, _, copy, entries = _calls()
+    areas, status = tuple(_areas(c) for c in caches), first._status.data_ptr()
+    if _done(copy(entries[3], areas, first.n_pages, status, first._index, sources, targets)):
+        return
     for t, name in ((sources, "sources"), (targets, "targets")):
         _require(isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.is_cuda and t.get_device() == first._index,
                  f"{name} must be an int32 tensor on the caches' device")
         _require(t.dim() == 1 and t.shape[0] > 0 and (t.shape[0] == 1 or t.stride(0) == 1), f"{name} must be contiguous, of shape [n]")
     _require(sources.shape == targets.shape, "targets must have the shape of sources")
-    areas = [a for c in caches for a in _areas(c)]
-    _lib.check(_lib.load().fa_b200_cache_copy((_lib.CopyArea * len(areas))(*areas), len(areas), first.n_pages, sources.data_ptr(), targets.data_ptr(), sources.shape[0],
-                                              first._status.data_ptr(), first._index, _raw_stream(first._index)))
+    both = [a for _, _, array in areas for a in array]
+    _lib.check(_lib.load().fa_b200_cache_copy((_lib.CopyArea * len(both))(*both), len(both), first.n_pages, sources.data_ptr(), targets.data_ptr(), sources.shape[0],
+                                              status, first._index, _raw_stream(first._index)))
