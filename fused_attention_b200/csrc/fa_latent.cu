@@ -82,9 +82,10 @@ struct LatentPlan {
 LatentPlan plan_rows(uint32_t latent, uint32_t heads, uint32_t page, uint32_t B, uint32_t T, uint32_t width, uint32_t sms) {
     LatentPlan r = {};
     r.rows = static_cast<uint64_t>(T) * heads;
-    r.n = r.rows <= 16 ? 16 : r.rows <= 32 ? 32 : 64;
-    r.groups = static_cast<uint32_t>((r.rows + r.n - 1) / r.n);
+    // As few groups as there can be, of equal size.
+    r.groups = static_cast<uint32_t>((r.rows + 63) / 64);
     r.group_rows = static_cast<uint32_t>((r.rows + r.groups - 1) / r.groups);
+    r.n = (r.group_rows + 15) / 16 * 16;
     r.groups = static_cast<uint32_t>((r.rows + r.group_rows - 1) / r.group_rows);
     const uint64_t tiles = static_cast<uint64_t>(B) * ((static_cast<uint64_t>(width) * page + fa::kLatentTile - 1) / fa::kLatentTile);
     r.least = r.n == 16 ? 2 : 4;
@@ -114,7 +115,10 @@ int launch_rows(Device& d, uint32_t bit, const CUtensorMap& map, const fa::Laten
 }
 template <int LC>
 int launch_rows(Device& d, uint32_t bit, const CUtensorMap& map, const fa::LatentRowsArgs& a, uint32_t n, cudaStream_t stream) {
-    return n == 16 ? launch_rows<LC, 16>(d, bit, map, a, stream) : n == 32 ? launch_rows<LC, 32>(d, bit + 1, map, a, stream) : launch_rows<LC, 64>(d, bit + 2, map, a, stream);
+    return n == 16   ? launch_rows<LC, 16>(d, bit, map, a, stream)
+           : n == 32 ? launch_rows<LC, 32>(d, bit + 1, map, a, stream)
+           : n == 48 ? launch_rows<LC, 48>(d, bit + 2, map, a, stream)
+                     : launch_rows<LC, 64>(d, bit + 3, map, a, stream);
 }
 
 }  // namespace
@@ -217,8 +221,8 @@ int fa_b200_latent_attention(const fa_b200_latent_cache* cache, const fa_b200_se
 #endif
     switch (a.c.latent) {
         case 128: return launch_rows<2>(*d, 0, map, a, plan.n, stream);
-        case 256: return launch_rows<4>(*d, 3, map, a, plan.n, stream);
-        default: return launch_rows<8>(*d, 6, map, a, plan.n, stream);
+        case 256: return launch_rows<4>(*d, 4, map, a, plan.n, stream);
+        default: return launch_rows<8>(*d, 8, map, a, plan.n, stream);
     }
 }
 
@@ -271,10 +275,10 @@ int fa_b200_latent_prompt(const void* q_nope, int64_t qn_batch_stride, int64_t q
     if (const cudaError_t e = cudaMemsetAsync(y, 0xFF, 2ull * B * T * heads * nope_dim, stream)) return static_cast<int>(e);
 #endif
     if (nope_dim == 64) {
-        if ((rc = allow_smem(*d, 9, &fa::fa_latent_prompt<64>, fa::ExpandCfg<64>::kSmemBytes)) != FA_B200_OK) return rc;
+        if ((rc = allow_smem(*d, 12, &fa::fa_latent_prompt<64>, fa::ExpandCfg<64>::kSmemBytes)) != FA_B200_OK) return rc;
         return launch(&fa::fa_latent_prompt<64>, static_cast<uint32_t>(items), fa::kExpandThreads, fa::ExpandCfg<64>::kSmemBytes, stream, q, qr, kv, r, a);
     }
-    if ((rc = allow_smem(*d, 10, &fa::fa_latent_prompt<128>, fa::ExpandCfg<128>::kSmemBytes)) != FA_B200_OK) return rc;
+    if ((rc = allow_smem(*d, 13, &fa::fa_latent_prompt<128>, fa::ExpandCfg<128>::kSmemBytes)) != FA_B200_OK) return rc;
     return launch(&fa::fa_latent_prompt<128>, static_cast<uint32_t>(items), fa::kExpandThreads, fa::ExpandCfg<128>::kSmemBytes, stream, q, qr, kv, r, a);
 }
 

@@ -2,20 +2,22 @@
 //
 //   s = scale * (q_latent . c + q_rope . r),  p = softmax(s),  y = sum of p c        for every head, over the same rows (c, r)
 //
-// Rows of the problem are the query heads of a sequence's tokens (row t * heads + h); a group is N of them (16, 32 or 64) of one
+// Rows of the problem are the query heads of a sequence's tokens (row t * heads + h); a group is N of them (16, 32, 48 or 64) of one
 // sequence.  The keys of all sequences, in tiles of 64, are dealt out evenly to `parts` CTAs a group, so that a sequence may be divided:
 // its parts leave numerators, maxima and sums in scratch, which fa_latent_join puts together.
 //
-// Both products are tcgen05 MMAs on the same tile in shared memory.  Scores are S[64 rows, 64 keys] = Q K^T with the rows as M; the result
-// is kept transposed, Y^T[128 dimensions, N] += C^T P^T, dimensions as M and rows as N: four such tiles hold 512 dimensions in 4 N
-// columns of tensor memory, where Y[128 rows, 512] would need all 512 columns and leave none for the scores; and of a group of 16 rows
-// only the scores (M = 64) cost more than 16 rows would have to.  256 threads:
+// Both products are tcgen05 MMAs on the same tile in shared memory, and both are kept transposed: S^T[64 keys, N] = C Q^T, and Y^T[128
+// dimensions, N] += C^T P^T.  Keys and dimensions are what an MMA's M is filled with, rows are its N, of which there may be few: four such
+// tiles hold 512 dimensions in 4 N columns of tensor memory, where Y[128 rows, 512] would need all 512 columns and leave none for the scores.
+// (Measured, clocks an MMA: M = 64 N = 16 or 32 27, N = 64 32; M = 128 N = 16 39, N = 32 40, N = 64 48.)  288 threads:
 //
-//   warps 0-3  softmax: a warp 16 rows, four threads a row (tcgen05.ld.16x256b hands out scores that way); P into shared memory; at the
-//              end of a segment (a sequence's tiles in this CTA) the division and Y, a thread a dimension
+//   warps 0-3  softmax: a warp 16 keys, eight threads a row and 16 keys (tcgen05.ld.16x256b hands out scores that way).  All share a row's
+//              reference; it is looked at again only where a score exceeds it by more than 2^8, so that a tile passes with no maximum being
+//              formed.  P into shared memory; at the end of a segment (a sequence's tiles in this CTA) the division and Y, a thread a dimension
 //   warp 4     fetches tiles by TMA: 64 keys of 128 dimensions a slot of one ring, of the rotary part a slot of another
-//   warp 5     issues the MMAs: the next tile's scores as its slots arrive, this tile's P as it is ready, whichever is first
-//   warps 6-7  queries into shared memory, a segment ahead
+//   warp 5, 6  issue the MMAs of the scores, of the results.  (One warp for both, as slots arrive: 94 us for 64 sequences of 100 to 8192
+//              tokens, 16 rows: a barrier's answer reaches a thread only behind the MMAs that it has queued, 575 clocks for 8 of them)
+//   warps 7-8  queries into shared memory, a segment ahead
 //
 // What must not happen: a key that a row does not see reaching it, as 0 * NaN.  Tiles that some row of the group sees in part only (the
 // last ones of a sequence) are gone over in shared memory between the two products: keys behind the last that any row sees become zeros;
@@ -28,7 +30,7 @@
 
 namespace fa {
 
-constexpr int kLatentThreads = 256;
+constexpr int kLatentThreads = 288;
 constexpr uint32_t kLatentTile = 64;
 constexpr uint32_t kLatentSlot = kLatentTile * 128;   // bytes of 64 keys by 64 dimensions
 constexpr float kLatentSlack = 8.0f;                  // the reference moves when an exponent exceeds it by more: weights stay below 2^8
@@ -53,40 +55,36 @@ struct LatentRowsArgs {
 template <int LC, int N>
 struct LatentCfg {
     static constexpr int kPairs = LC / 2;                     // of 64-dimension chunks: slots of a tile
-    static constexpr int kPairSlots = LC == 8 ? 8 : LC == 4 ? 9 : 8, kRopeSlots = LC == 8 ? 2 : LC == 4 ? 4 : 8;
-    static constexpr int kPBuffers = N == 64 ? 1 : 2;
-    static constexpr uint32_t kQBytes = (LC + 1) * kLatentSlot, kPBytes = N * 128;
+    static constexpr int kPitch = N == 16 ? 32 : N == 32 ? 64 : 128;   // bytes of a key's weights: a swizzle span
+    static constexpr int kPBuffers = N <= 32 ? 2 : 1;
+    static constexpr uint32_t kQChunk = N * 128, kQBytes = (LC + 1) * kQChunk, kPBytes = kLatentTile * kPitch;
+    // Slots: what is left of shared memory, three tiles' rotary parts (two, eight) and the rest for the other ring
+    static constexpr int kChunks = (229376 - kQBytes - kPBuffers * kPBytes) / kLatentSlot;
+    static constexpr int kRopeSlots = LC == 8 ? (kChunks >= 23 ? 3 : 2) : LC == 4 ? 4 : 8;
+    static constexpr int kPairSlots = (kChunks - kRopeSlots) / 2 < 12 ? (kChunks - kRopeSlots) / 2 : 12;
+    static_assert(kPairSlots >= kPairs && kPairSlots >= 2, "room for a tile");
     static constexpr uint32_t kOffPair = kQBytes, kOffRope = kOffPair + kPairSlots * 2 * kLatentSlot, kOffP = kOffRope + kRopeSlots * kLatentSlot;
+    static_assert(kOffPair % 1024 == 0 && kOffP % 1024 == 0 && kPBytes % 1024 == 0, "tiles on swizzle atoms");
     static constexpr uint32_t kTiles = kOffP + kPBuffers * kPBytes;
     static constexpr int kSmemBytes = kTiles + 1024;
-    static constexpr uint32_t kColS = kPairs * N <= 256 ? 256 : 512, kCols = 512;   // scores of even tiles at kColS, of odd ones 64 behind
-    static_assert(kPairs * N <= 256, "tensor memory");
+    static constexpr uint32_t kColS = kPairs * N, kCols = 512;   // scores of even tiles at kColS, of odd ones N behind
+    static_assert(kColS + 2 * N <= 512, "tensor memory");
     // barriers
     static constexpr int FULL = 0, EMPTY = FULL + kPairSlots, RFULL = EMPTY + kPairSlots, REMPTY = RFULL + kRopeSlots, QFULL = REMPTY + kRopeSlots, QEMPTY = QFULL + 1,
-                         S = QEMPTY + 1, P = S + 2, PV = P + 2, FINAL = PV + 2, kBarriers = FINAL + 1;
+                         S = QEMPTY + 1, P = S + 2, PV = P + 2, FINAL = PV + 2, kBarriers = FINAL + 2;
 };
 
 // Instruction descriptors (see make_idesc_f16): fp16 or bf16 operands, fp32 sums.
 __device__ __forceinline__ uint32_t idesc_16bit(uint32_t m, uint32_t n, bool a_mn, bool b_mn, bool bf16) {
     return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
-// 16 lanes x 64 columns: thread t receives of row t / 4 (v[4 j], v[4 j + 1]) and of row t / 4 + 8 (v[4 j + 2], v[4 j + 3]) columns 8 j + 2 (t % 4) and the next.
-__device__ __forceinline__ void tmem_ld_16x64(uint32_t taddr, float (&v)[32]) {
-    FA_DBG_TMEM(taddr, 64u);
-    asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]),
-          "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]),
-          "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
-        : "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    return ok != 0;
+// 16 lanes x 16 columns: thread t receives of lane t / 4 (v[4 j], v[4 j + 1]) and of lane t / 4 + 8 (v[4 j + 2], v[4 j + 3]) columns 8 j + 2 (t % 4) and the next.
+__device__ __forceinline__ void tmem_ld_16x16(uint32_t taddr, float* v) {
+    FA_DBG_TMEM(taddr, 16u);
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                 : "r"(taddr)
+                 : "memory");
 }
 // Of warps 0-3: all there, and whether any thread says so.
 __device__ __forceinline__ bool softmax_any(bool x) {
@@ -200,8 +198,13 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
     using C = LatentCfg<LC, N>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[C::kBarriers];
-    __shared__ float s_alpha[2][64], s_l[64], s_m[64];
-    __shared__ uint32_t s_absent[4];         // of tile g in entry g % 4: its 16-key groups without a page
+    // (shared memory is full: what is needed at a segment's end takes the places of what is not any more)
+    __shared__ float s_max[4][N], s_alpha[N];
+    __shared__ uint32_t s_limit[N];
+    float (&s_sum)[4][N] = s_max;
+    float (&s_m)[N] = s_alpha;
+    float* const s_l = reinterpret_cast<float*>(s_limit);
+    __shared__ uint32_t s_absent[8];         // of tile g in entry g % 8: its 16-key groups without a page
     __shared__ uint32_t s_bad[2][2];         // of the partly seen tile n in entry n % 2: keys that hold no finite numbers
     __shared__ uint32_t tmem_slot, abort_flag;
 
@@ -218,7 +221,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
     const bool bf16 = p.bf16 != 0;
 
     if (tid == 0) {
-        for (int i = 0; i < C::kBarriers; ++i) mbar_init(bar(i), i == C::QFULL ? 64u : i >= C::P && i < C::PV ? 4u : 1u);
+        for (int i = 0; i < C::kBarriers; ++i) mbar_init(bar(i), i == C::QFULL ? 64u : 1u);
         abort_flag = 0;
         fence_mbar_init();
         prefetch_tensormap(&map);
@@ -252,8 +255,8 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
     if (warp < 4) {
         // ---------------------------------------------------------------- softmax
         const uint32_t lane_off = (warp * 32u) << 16;
-        const uint32_t ra = 16 * warp + lane / 4, quad = lane & 3u;
-        const bool mine = 16 * warp < N;      // rows of this warp
+        const uint32_t quad = lane & 3u, key_a = 16 * warp + lane / 4;   // this thread's keys of a tile: key_a and key_a + 8; its rows: 8 j + 2 quad + e
+        constexpr int kBlocks = N / 8;
         uint32_t g = 0, partly = 0;
         for (uint32_t b = part; b < p.s.B; b += p.parts) {   // sequences without tokens
             if (latent_units(p, b) != 0) continue;
@@ -263,14 +266,13 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
         while (any && latent_next(p, group, w)) {
             if (group == 0 && w.begins && tid == 0)
                 p.shares[w.seq] = make_int2(static_cast<int>(part), static_cast<int>(latent_owner(w, w.first_unit + w.units - 1u)));
-            uint32_t limit[2];
-            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t r = ra + 8 * i;
-                limit[i] = r < n_rows ? latent_limit(p, w.q, (row0 + r) / p.heads) : 0u;
-                if (limit[i] == 0) limit[i] = kSeesAll;   // what becomes of such a row is not used
+            if (tid < N) {   // (what becomes of a row that sees nothing is not used)
+                const uint32_t x = tid < n_rows ? latent_limit(p, w.q, (row0 + tid) / p.heads) : 0u;
+                s_limit[tid] = x == 0 ? kSeesAll : x;
             }
+            float m[2 * kBlocks], l[2 * kBlocks];
+#pragma unroll
+            for (int i = 0; i < 2 * kBlocks; ++i) m[i] = -INFINITY, l[i] = 0.0f;
             // keys that all rows see that see any: up to the first row's
             uint32_t least = latent_limit(p, w.q, row0 / p.heads);
             if (least == 0) {   // (tokens in front of the first key: found by every thread, rows are few)
@@ -283,21 +285,21 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                     }
                 }
             }
+            softmax_sync();   // s_limit
             for (uint32_t tile = w.t0; tile < w.end; ++tile, ++g) {
                 const uint32_t key0 = tile * kLatentTile;
                 mbar_wait(bar(C::S + (g & 1u)), (g >> 1) & 1u, ctl, kCacheTimeout | C::S);
                 tc_fence_after();
                 __syncwarp();
-                float s[32];
-                if (mine) {
-                    tmem_ld_16x64(tmem + lane_off + C::kColS + 64 * (g & 1u), s);
-                    tmem_wait_ld();
-                }
+                float s[4 * kBlocks];
+#pragma unroll
+                for (int i = 0; i < N / 16; ++i) tmem_ld_16x16(tmem + lane_off + C::kColS + N * (g & 1u) + 16 * i, s + 8 * i);
                 // (the rotary slot's barrier: what the fetching warp has written about this tile is there)
                 mbar_wait(bar(C::RFULL + g % C::kRopeSlots), (g / C::kRopeSlots) & 1u, ctl, kCacheTimeout | C::RFULL);
-                const uint32_t absent = *reinterpret_cast<volatile uint32_t*>(&s_absent[g & 3u]);
-                uint32_t bad_lo = 0, bad_hi = 0;
+                const uint32_t absent = *reinterpret_cast<volatile uint32_t*>(&s_absent[g & 7u]);
+                tmem_wait_ld();
                 if (key0 + kLatentTile > least || absent != 0) {
+                    uint32_t bad_lo = 0, bad_hi = 0;
                     if (key0 + kLatentTile > least) {
                         // two threads a key: pieces of 16 bytes, four of each 64 dimensions
                         const uint32_t key = tid >> 1, half = tid & 1u, at = key0 + key, swz = key & 7u;
@@ -333,54 +335,18 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                         // (the other entry was last read two barriers ago)
                         if (tid < 2) s_bad[partly & 1u][tid] = 0;
                     }
-                    if (mine) {
 #pragma unroll
-                        for (uint32_t j = 0; j < 8; ++j) {
-                            const bool gone = absent >> (j >> 1) & 1u;
+                    for (uint32_t i = 0; i < 2; ++i) {
+                        const uint32_t key = key_a + 8 * i, at = key0 + key;
+                        const bool gone = (absent >> (key >> 4) & 1u) || at >= w.farthest, bad = (key < 32 ? bad_lo >> key : bad_hi >> (key - 32)) & 1u;
 #pragma unroll
-                            for (uint32_t e = 0; e < 4; ++e) {
-                                const uint32_t key = 8 * j + 2 * quad + (e & 1u);
-                                const bool bad = (key < 32 ? bad_lo >> key : bad_hi >> (key - 32)) & 1u;
-                                if (gone || key0 + key >= limit[e >> 1] || (key0 + key >= w.farthest)) s[4 * j + e] = -INFINITY;
-                                else if (bad) s[4 * j + e] = __int_as_float(0x7FC00000);
+                        for (uint32_t j = 0; j < kBlocks; ++j) {
+#pragma unroll
+                            for (uint32_t e = 0; e < 2; ++e) {
+                                if (gone || at >= s_limit[8 * j + 2 * quad + e]) s[4 * j + 2 * i + e] = -INFINITY;
+                                else if (bad) s[4 * j + 2 * i + e] = __int_as_float(0x7FC00000);
                             }
                         }
-                    }
-                }
-                // ---- the rows' references
-                float alpha[2] = {1.0f, 1.0f};
-                if (mine) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        float top = fmaxf(s[2 * i], s[2 * i + 1]);
-#pragma unroll
-                        for (int j = 1; j < 8; ++j) top = max3(top, s[4 * j + 2 * i], s[4 * j + 2 * i + 1]);
-                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2)) * p.scale_log2;
-                        if (top > m[i] + kLatentSlack) {
-                            alpha[i] = ex2_approx(m[i] - top);
-                            m[i] = top;
-                            l[i] *= alpha[i];
-                        }
-                    }
-                    if (quad == 0) s_alpha[g & 1u][ra] = alpha[0], s_alpha[g & 1u][ra + 8] = alpha[1];
-                }
-                const bool moved = softmax_any(mine && tile > w.t0 && (alpha[0] != 1.0f || alpha[1] != 1.0f));
-                // ---- weights, rounded, and the sums of what they are rounded to
-                uint32_t pk[16];
-                if (mine) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float ref = m[i] == -INFINITY ? 0.0f : m[i];
-                        float sum = 0.0f;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float w0 = ex2_approx(fmaf(s[4 * j + 2 * i], p.scale_log2, -ref)), w1 = ex2_approx(fmaf(s[4 * j + 2 * i + 1], p.scale_log2, -ref));
-                            pk[2 * j + i] = pack_16(w0, w1, bf16);
-                            const float2 y = unpack_16(pk[2 * j + i], bf16);
-                            sum += y.x + y.y;
-                        }
-                        l[i] += sum;
                     }
                 }
                 // the last P V that read this buffer of P
@@ -388,44 +354,105 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                     const uint32_t h = g - C::kPBuffers;
                     mbar_wait(bar(C::PV + (h & 1u)), (h >> 1) & 1u, ctl, kCacheTimeout | C::PV);
                 }
-                if (mine) {
-                    const uint32_t to = p_addr(g) + ra * 128 + 4 * quad;
+                // ---- weights by the rows' references, rounded; whether some score asks for another reference
+                uint32_t pk[2 * kBlocks];
+                auto weights = [&] {
 #pragma unroll
-                    for (uint32_t j = 0; j < 8; ++j) {
-                        st_shared_u32(to + ((j ^ (ra & 7u)) << 4), pk[2 * j]);
-                        st_shared_u32(to + 8 * 128 + ((j ^ (ra & 7u)) << 4), pk[2 * j + 1]);
+                    for (uint32_t j = 0; j < kBlocks; ++j) {
+                        const float r0 = m[2 * j] == -INFINITY ? 0.0f : m[2 * j], r1 = m[2 * j + 1] == -INFINITY ? 0.0f : m[2 * j + 1];
+#pragma unroll
+                        for (uint32_t i = 0; i < 2; ++i) {
+                            pk[2 * j + i] = pack_16(ex2_approx(fmaf(s[4 * j + 2 * i], p.scale_log2, -r0)), ex2_approx(fmaf(s[4 * j + 2 * i + 1], p.scale_log2, -r1)), bf16);
+                            const uint32_t row = key_a + 8 * i;
+                            st_shared_u32(p_addr(g) + row * C::kPitch + ((j ^ (row * C::kPitch >> 7 & (C::kPitch / 16 - 1))) << 4) + 4 * quad, pk[2 * j + i]);
+                        }
                     }
+                };
+                bool above = tile == w.t0;
+                if (!above) {
+#pragma unroll
+                    for (int j = 0; j < kBlocks; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            above |= fmaxf(s[4 * j + e], s[4 * j + 2 + e]) * p.scale_log2 > (m[2 * j + e] == -INFINITY ? -INFINITY : m[2 * j + e] + kLatentSlack);
+                    weights();
                     fence_proxy_async_smem();
+                    tc_fence_before();
                 }
-                if (moved) {   // rows are columns of Y^T: every warp multiplies all of them, in its dimensions
-                    mbar_wait(bar(C::PV + ((g - 1u) & 1u)), ((g - 1u) >> 1) & 1u, ctl, kCacheTimeout | C::PV);
-                    tc_fence_after();
-                    __syncwarp();
-#pragma unroll 1
-                    for (uint32_t c = 0; c < C::kPairs * N; c += 16) {
-                        float o[16];
-                        uint32_t x[16];
-                        tmem_ld16(tmem + lane_off + c, o);
-                        tmem_wait_ld();
+                if (softmax_any(above)) {
+                    // ---- the largest score of every row that it is too large for its reference
 #pragma unroll
-                        for (uint32_t e = 0; e < 16; ++e) x[e] = __float_as_uint(o[e] * s_alpha[g & 1u][(c + e) % N]);
-                        tmem_st16(tmem + lane_off + c, x);
+                    for (int j = 0; j < kBlocks; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float top = fmaxf(s[4 * j + e], s[4 * j + 2 + e]);
+#pragma unroll
+                            for (int d = 4; d <= 16; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+                            if (lane < 4) s_max[warp][8 * j + 2 * quad + e] = top;
+                        }
+                    softmax_sync();
+#pragma unroll
+                    for (int j = 0; j < kBlocks; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int r = 8 * j + 2 * quad + e;
+                            const float top = fmaxf(fmaxf(s_max[0][r], s_max[1][r]), fmaxf(s_max[2][r], s_max[3][r])) * p.scale_log2;
+                            float alpha = 1.0f;
+                            if (top > (m[2 * j + e] == -INFINITY ? -INFINITY : m[2 * j + e] + kLatentSlack)) {
+                                alpha = ex2_approx(m[2 * j + e] - top);
+                                m[2 * j + e] = top;
+                                l[2 * j + e] *= alpha;
+                            }
+                            if (tid < 4) s_alpha[r] = alpha;
+                        }
+                    weights();
+                    fence_proxy_async_smem();
+                    softmax_sync();
+                    if (tile > w.t0) {   // rows are columns of Y^T: every warp multiplies all of them, in its dimensions
+                        mbar_wait(bar(C::PV + ((g - 1u) & 1u)), ((g - 1u) >> 1) & 1u, ctl, kCacheTimeout | C::PV);
+                        tc_fence_after();
+                        __syncwarp();
+#pragma unroll 1
+                        for (uint32_t c = 0; c < C::kPairs * N; c += 16) {
+                            float o[16];
+                            uint32_t x[16];
+                            tmem_ld16(tmem + lane_off + c, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (uint32_t e = 0; e < 16; ++e) x[e] = __float_as_uint(o[e] * s_alpha[c % N + e]);
+                            tmem_st16(tmem + lane_off + c, x);
+                        }
+                        tmem_wait_st();
                     }
-                    tmem_wait_st();
+                    tc_fence_before();
+                    softmax_sync();
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(C::P + (g & 1u)));
+                if (tid == 0) mbar_arrive(bar(C::P + (g & 1u)));
+                // sums of the weights as they are rounded
+#pragma unroll
+                for (int j = 0; j < kBlocks; ++j) {
+                    const float2 x = unpack_16(pk[2 * j], bf16), y = unpack_16(pk[2 * j + 1], bf16);
+                    l[2 * j] += x.x + y.x;
+                    l[2 * j + 1] += x.y + y.y;
+                }
             }
             // ---- the segment's end
-            if (mine) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 1);
-                    l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 2);
-                    if (limit[i] == kSeesAll) l[i] = 0.0f, m[i] = -INFINITY;   // sees nothing
-                    if (quad == 0) s_l[ra + 8 * i] = w.whole ? (l[i] == 0.0f ? 0.0f : 1.0f / l[i]) : l[i], s_m[ra + 8 * i] = m[i];
+            for (int j = 0; j < kBlocks; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float x = l[2 * j + e];
+#pragma unroll
+                    for (int d = 4; d <= 16; d <<= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, d);
+                    if (lane < 4) s_sum[warp][8 * j + 2 * quad + e] = x;
+                    if (tid < 4) s_m[8 * j + 2 * quad + e] = m[2 * j + e];
                 }
+            softmax_sync();
+            if (tid < N) {
+                const float x = (s_sum[0][tid] + s_sum[1][tid]) + (s_sum[2][tid] + s_sum[3][tid]);
+                const bool none = s_limit[tid] == kSeesAll || x == 0.0f;
+                s_l[tid] = none ? 0.0f : w.whole ? 1.0f / x : x;
+                if (none) s_m[tid] = -INFINITY;
             }
             const bool tiles = w.end > w.t0;
             if (tiles) {
@@ -488,18 +515,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                 uint32_t gone = 0;   // a bit for each 16 keys
                 for (uint32_t i = 0; i < per_tile; ++i)
                     if (static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, entry, first + i - from)) >= p.c.n_pages) gone |= (per_tile == 1 ? 15u : per_tile == 2 ? 3u : 1u) << (i * (4 / per_tile));
-                const uint32_t nr = g, y = per_tile == 1 ? key0 & (p.c.page - 1u) : 0u;
-                if (nr >= C::kRopeSlots) ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(C::REMPTY + nr % C::kRopeSlots), (nr / C::kRopeSlots - 1u) & 1u, ctl, kCacheTimeout | C::REMPTY));
-                if (!ok) break;
-                ++ropes;
-                if (leader) {
-                    *reinterpret_cast<volatile uint32_t*>(&s_absent[g & 3u]) = gone;
-                    mbar_expect_tx(bar(C::RFULL + nr % C::kRopeSlots), kLatentSlot);
-                }
-                for (uint32_t i = 0; i < per_tile; ++i) {
-                    const int32_t page = __shfl_sync(0xFFFFFFFFu, entry, first + i - from);
-                    if (leader) tma_load_3d(rope_addr(nr) + i * box_bytes, &map, bar(C::RFULL + nr % C::kRopeSlots), 64 * LC, static_cast<int32_t>(y), page);
-                }
+                const uint32_t y = per_tile == 1 ? key0 & (p.c.page - 1u) : 0u;
                 for (uint32_t c = 0; c < C::kPairs; ++c) {
                     const uint32_t n = g * C::kPairs + c;
                     if (n >= C::kPairSlots) ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(C::EMPTY + n % C::kPairSlots), (n / C::kPairSlots - 1u) & 1u, ctl, kCacheTimeout | C::EMPTY));
@@ -513,6 +529,18 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                             tma_load_3d(pair_addr(n) + kLatentSlot + i * box_bytes, &map, bar(C::FULL + n % C::kPairSlots), static_cast<int32_t>(128 * c + 64), static_cast<int32_t>(y), page);
                         }
                     }
+                }
+                if (!ok) break;
+                if (g >= C::kRopeSlots) ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(C::REMPTY + g % C::kRopeSlots), (g / C::kRopeSlots - 1u) & 1u, ctl, kCacheTimeout | C::REMPTY));
+                if (!ok) break;
+                ++ropes;
+                if (leader) {
+                    *reinterpret_cast<volatile uint32_t*>(&s_absent[g & 7u]) = gone;
+                    mbar_expect_tx(bar(C::RFULL + g % C::kRopeSlots), kLatentSlot);
+                }
+                for (uint32_t i = 0; i < per_tile; ++i) {
+                    const int32_t page = __shfl_sync(0xFFFFFFFFu, entry, first + i - from);
+                    if (leader) tma_load_3d(rope_addr(g) + i * box_bytes, &map, bar(C::RFULL + g % C::kRopeSlots), 64 * LC, static_cast<int32_t>(y), page);
                 }
                 __syncwarp();
             }
@@ -529,118 +557,81 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                 if (uses > 0) mbar_wait_certain(bar(C::RFULL + i), (uses - 1u) & 1u, ctl, kCacheTimeout | C::RFULL);
             }
         }
-    } else if (warp == 5) {
-        // ---------------------------------------------------------------- MMAs
+    } else if (warp == 5 || warp == 6) {
+        // ---------------------------------------------------------------- MMAs: scores, results
         const bool leader = elect_one();
-        const uint32_t idesc_s = idesc_16bit(64, kLatentTile, false, false, bf16), idesc_y = idesc_16bit(128, N, true, false, bf16);
+        bool ok = true;   // once a wait has given up nothing more is issued
+        auto wait = [&](int x, uint32_t parity) { ok &= mbar_wait(bar(x), parity, ctl, kCacheTimeout | static_cast<uint32_t>(x)); };
+        const uint32_t idesc_s = idesc_16bit(kLatentTile, N, false, false, bf16), idesc_y = idesc_16bit(128, N, true, true, bf16);
         const uint32_t rope_steps = p.c.rope / 16;
-        uint32_t g_qk = 0, g_pv = 0, k = 0;           // tiles scored, multiplied; segments begun
-        bool pv_first = false, pv_pending = false;    // the tile whose P is awaited
-        bool more = any && latent_next(p, group, w);
-        while (more && w.end == w.t0) more = latent_next(p, group, w);
-        uint32_t tile = w.t0;
-        bool failed = false;
-        while (!failed && (more || pv_pending)) {
-            const bool first = more && tile == w.t0, last = more && tile + 1 == w.end;
-            uint32_t c = 0;
-            bool q_there = !first;
-            const uint32_t t_begin = wait_clock();
-            uint32_t turns = 0;
-            while ((more && c <= C::kPairs) || pv_pending) {
-                if (more && c <= C::kPairs) {
-                    if (!q_there) q_there = mbar_test(bar(C::QFULL), k & 1u);
-                    if (q_there) {
-                        const uint32_t n = g_qk * C::kPairs + c - 1u;
-                        if (mbar_test(bar(c == 0 ? C::RFULL + g_qk % C::kRopeSlots : C::FULL + n % C::kPairSlots), c == 0 ? (g_qk / C::kRopeSlots) & 1u : (n / C::kPairSlots) & 1u)) {
-                            const uint32_t tS = tmem + C::kColS + 64 * (g_qk & 1u);
-                            tc_fence_after();
-                            if (leader) {
-                                if (c == 0) {
-                                    const uint64_t dq = make_smem_desc<128>(base + LC * kLatentSlot, 16), dk = make_smem_desc<128>(rope_addr(g_qk), 16);
-                                    for (uint32_t ks = 0; ks < rope_steps; ++ks) mma_ss(tS, dq + 2 * ks, dk + 2 * ks, idesc_s, ks > 0 ? 1u : 0u);
-                                } else {
-                                    const uint64_t dq = make_smem_desc<128>(base + (c - 1u) * (2 * kLatentSlot), 16), dk = make_smem_desc<128>(pair_addr(n), 16);
-#pragma unroll
-                                    for (uint32_t ks = 0; ks < 8; ++ks) {
-                                        const uint32_t off = (ks >> 2) * (kLatentSlot >> 4) + (ks & 3u) * 2u;
-                                        mma_ss(tS, dq + off, dk + off, idesc_s, 1u);
-                                    }
-                                }
-                            }
-                            if (c == C::kPairs) {
-                                if (leader) {
-                                    tc_commit(bar(C::S + (g_qk & 1u)));
-                                    if (last) tc_commit(bar(C::QEMPTY));
-                                }
-                                if (last) ++k;
-                            }
-                            __syncwarp();
-                            ++c;
-                            turns = 0;
-                            continue;
-                        }
-                    }
-                }
-                if (pv_pending && mbar_test(bar(C::P + (g_pv & 1u)), (g_pv >> 1) & 1u)) {
+        uint32_t g = 0, k = 0;   // tiles; segments with tiles
+        while (any && latent_next(p, group, w)) {
+            if (w.end == w.t0) continue;
+            if (warp == 5) wait(C::QFULL, k & 1u);
+            for (uint32_t tile = w.t0; tile < w.end; ++tile, ++g) {
+                if (warp == 5) {
+                    // (whoever read the scores two tiles ago has given P)
+                    if (g >= 2) wait(C::P + (g & 1u), ((g >> 1) - 1u) & 1u);
+                    const uint32_t tS = tmem + C::kColS + N * (g & 1u);
+                    for (uint32_t c = 0; c < C::kPairs; ++c) wait(C::FULL + (g * C::kPairs + c) % C::kPairSlots, ((g * C::kPairs + c) / C::kPairSlots) & 1u);
+                    wait(C::RFULL + g % C::kRopeSlots, (g / C::kRopeSlots) & 1u);
                     tc_fence_after();
-                    if (leader) {
-                        const uint64_t dp = make_smem_desc<128>(p_addr(g_pv), 16);
+                    if (leader && ok) {
+#pragma unroll
+                        for (uint32_t c = 0; c < LC; ++c) {
+                            const uint64_t dk = make_smem_desc<128>(pair_addr(g * C::kPairs + c / 2) + (c & 1u) * kLatentSlot, 16), dq = make_smem_desc<128>(base + c * C::kQChunk, 16);
+#pragma unroll
+                            for (uint32_t ks = 0; ks < 4; ++ks) mma_ss(tS, dk + 2 * ks, dq + 2 * ks, idesc_s, c + ks > 0 ? 1u : 0u);
+                        }
+                        const uint64_t dk = make_smem_desc<128>(rope_addr(g), 16), dq = make_smem_desc<128>(base + LC * C::kQChunk, 16);
+                        for (uint32_t ks = 0; ks < rope_steps; ++ks) mma_ss(tS, dk + 2 * ks, dq + 2 * ks, idesc_s, 1u);
+                        tc_commit(bar(C::S + (g & 1u)));
+                        if (tile + 1 == w.end) tc_commit(bar(C::QEMPTY));
+                    }
+                } else {
+                    wait(C::P + (g & 1u), (g >> 1) & 1u);
+                    tc_fence_after();
+                    if (leader && ok) {
+                        const uint64_t dp = make_smem_desc<C::kPitch>(p_addr(g), 16);
 #pragma unroll
                         for (uint32_t d = 0; d < C::kPairs; ++d) {
-                            const uint32_t n = g_pv * C::kPairs + d;
+                            const uint32_t n = g * C::kPairs + d;
                             const uint64_t dc = make_smem_desc<128>(pair_addr(n), kLatentSlot);
 #pragma unroll
-                            for (uint32_t ks = 0; ks < 4; ++ks) mma_ss(tmem + d * N, dc + ks * (2048 >> 4), dp + 2 * ks, idesc_y, !pv_first || ks > 0 ? 1u : 0u);
+                            for (uint32_t ks = 0; ks < kLatentTile / 16; ++ks)
+                                mma_ss(tmem + d * N, dc + ks * (2048 >> 4), dp + ks * (16 * C::kPitch >> 4), idesc_y, tile > w.t0 || ks > 0 ? 1u : 0u);
                             tc_commit(bar(C::EMPTY + n % C::kPairSlots));
                         }
-                        tc_commit(bar(C::REMPTY + g_pv % C::kRopeSlots));   // (not with the scores: softmax looks at the tile and its barriers until here)
-                        tc_commit(bar(C::PV + (g_pv & 1u)));
-                    }
-                    __syncwarp();
-                    pv_pending = false;
-                    ++g_pv;
-                    turns = 0;
-                    continue;
-                }
-                if (++turns > 4096) {
-                    turns = 0;
-                    const bool late = wait_clock() - t_begin > static_cast<uint32_t>(kWaitCapCycles >> 16);
-                    if (late) wait_expired(ctl, kCacheTimeout | C::P);
-                    if (late || *ctl.abort_flag != 0u) {
-                        failed = true;
-                        break;
+                        tc_commit(bar(C::REMPTY + g % C::kRopeSlots));   // (not with the scores: softmax looks at the tile and its barriers until here)
+                        tc_commit(bar(C::PV + (g & 1u)));
                     }
                 }
+                __syncwarp();
             }
-            if (failed || !more) break;
-            pv_pending = true, pv_first = first;
-            ++g_qk;
-            if (++tile == w.end) {
-                do more = latent_next(p, group, w);
-                while (more && w.end == w.t0);
-                tile = w.t0;
-            }
+            ++k;
         }
-        if (leader) tc_commit(bar(C::FINAL));
+        // every product issued has to retire before tensor and shared memory are let go of
+        const int last = C::FINAL + (warp == 5 ? 0 : 1);
+        if (leader) tc_commit(bar(last));
         __syncwarp();
-        mbar_wait_certain(bar(C::FINAL), 0, ctl, kCacheTimeout | C::FINAL);
+        mbar_wait_certain(bar(last), 0, ctl, kCacheTimeout | static_cast<uint32_t>(last));
     } else {
         // ---------------------------------------------------------------- queries
-        const uint32_t lt = tid - 192u, rope_pieces = p.c.rope / 8;
+        const uint32_t lt = tid - 224u, rope_pieces = p.c.rope / 8;
         uint32_t k = 0;
         while (any && latent_next(p, group, w)) {
             if (w.end == w.t0) continue;
             if (k > 0) mbar_wait(bar(C::QEMPTY), (k - 1u) & 1u, ctl, kCacheTimeout | C::QEMPTY);
-            const uint32_t rows = k == 0 ? 64u : n_rows;   // (rows that are not there: zeros, once)
+            const uint32_t rows = k == 0 ? static_cast<uint32_t>(N) : n_rows;   // (rows that are not there: zeros, once)
             for (uint32_t i = lt; i < rows * (8 * LC); i += 64) {
                 const uint32_t r = i / (8 * LC), j = i % (8 * LC), t = (row0 + r) / p.heads, h = row0 + r - t * p.heads;
                 const bool in = r < n_rows;
-                cp_async_16_zero(base + (j / 8) * kLatentSlot + r * 128 + (((j & 7u) ^ (r & 7u)) << 4), p.q_latent + (in ? w.seq * p.ql_b + t * p.ql_t + h * p.ql_h + 16 * j : 0), in);
+                cp_async_16_zero(base + (j / 8) * C::kQChunk + r * 128 + (((j & 7u) ^ (r & 7u)) << 4), p.q_latent + (in ? w.seq * p.ql_b + t * p.ql_t + h * p.ql_h + 16 * j : 0), in);
             }
             for (uint32_t i = lt; i < rows * rope_pieces; i += 64) {
                 const uint32_t r = i / rope_pieces, j = i % rope_pieces, t = (row0 + r) / p.heads, h = row0 + r - t * p.heads;
                 const bool in = r < n_rows;
-                cp_async_16_zero(base + LC * kLatentSlot + r * 128 + ((j ^ (r & 7u)) << 4), p.q_rope + (in ? w.seq * p.qr_b + t * p.qr_t + h * p.qr_h + 16 * j : 0), in);
+                cp_async_16_zero(base + LC * C::kQChunk + r * 128 + ((j ^ (r & 7u)) << 4), p.q_rope + (in ? w.seq * p.qr_b + t * p.qr_t + h * p.qr_h + 16 * j : 0), in);
             }
             cp_async_wait_all();
             fence_proxy_async_smem();
