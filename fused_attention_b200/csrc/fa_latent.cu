@@ -111,7 +111,10 @@ int launch_rows(Device& d, uint32_t bit, const CUtensorMap& map, const fa::Laten
     int rc = allow_smem(d, bit, &fa::fa_latent_rows<LC, N>, fa::LatentCfg<LC, N>::kSmemBytes);
     if (rc == FA_B200_OK) rc = launch(&fa::fa_latent_rows<LC, N>, a.parts * a.groups, fa::kLatentThreads, fa::LatentCfg<LC, N>::kSmemBytes, stream, map, a);
     if (rc != FA_B200_OK || a.parts == 1) return rc;
-    return launch(&fa::fa_latent_join<LC, N>, a.s.B * a.rows * (LC / 2), fa::kLatentJoinWarps * 32, 0, stream, a);
+    // a sequence has about parts / B parts, and one more
+    const uint32_t items = a.s.B * a.rows * (LC / 2);
+    if (a.parts >= 8 * a.s.B) return launch(&fa::fa_latent_join<LC, N, true>, items, fa::kLatentJoinWarps * 32, 0, stream, a);
+    return launch(&fa::fa_latent_join<LC, N, false>, (items + fa::kLatentJoinWarps - 1) / fa::kLatentJoinWarps, fa::kLatentJoinWarps * 32, 0, stream, a);
 }
 template <int LC>
 int launch_rows(Device& d, uint32_t bit, const CUtensorMap& map, const fa::LatentRowsArgs& a, uint32_t n, cudaStream_t stream) {

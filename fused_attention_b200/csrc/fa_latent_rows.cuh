@@ -9,15 +9,16 @@
 // Both products are tcgen05 MMAs on the same tile in shared memory, and both are kept transposed: S^T[64 keys, N] = C Q^T, and Y^T[128
 // dimensions, N] += C^T P^T.  Keys and dimensions are what an MMA's M is filled with, rows are its N, of which there may be few: four such
 // tiles hold 512 dimensions in 4 N columns of tensor memory, where Y[128 rows, 512] would need all 512 columns and leave none for the scores.
-// (Measured, clocks an MMA: M = 64 N = 16 or 32 27, N = 64 32; M = 128 N = 16 39, N = 32 40, N = 64 48.)  288 threads:
+// (Measured, clocks an MMA: M = 64 N = 16 or 32 27, N = 64 32; M = 128 N = 16 39, N = 32 40, N = 64 48.)  320 threads:
 //
 //   warps 0-3  softmax: a warp 16 keys, eight threads a row and 16 keys (tcgen05.ld.16x256b hands out scores that way).  All share a row's
 //              reference; it is looked at again only where a score exceeds it by more than 2^8, so that a tile passes with no maximum being
 //              formed.  P into shared memory; at the end of a segment (a sequence's tiles in this CTA) the division and Y, a thread a dimension
-//   warp 4     fetches tiles by TMA: 64 keys of 128 dimensions a slot of one ring, of the rotary part a slot of another
-//   warp 5, 6  issue the MMAs of the scores, of the results.  (One warp for both, as slots arrive: 94 us for 64 sequences of 100 to 8192
+//   warp 4, 5  fetch tiles by TMA: 64 keys of 128 dimensions a slot of one ring, of the rotary part a slot of another.  (Two, because what a
+//              thread asks of a barrier behind a TMA copy takes 280 clocks: one warp alone brings in a tile of 512 dimensions in 2550)
+//   warp 6, 7  issue the MMAs of the scores, of the results.  (One warp for both, as slots arrive: 94 us for 64 sequences of 100 to 8192
 //              tokens, 16 rows: a barrier's answer reaches a thread only behind the MMAs that it has queued, 575 clocks for 8 of them)
-//   warps 7-8  queries into shared memory, a segment ahead
+//   warps 8-9  queries into shared memory, a segment ahead
 //
 // What must not happen: a key that a row does not see reaching it, as 0 * NaN.  Tiles that some row of the group sees in part only (the
 // last ones of a sequence) are gone over in shared memory between the two products: keys behind the last that any row sees become zeros;
@@ -30,7 +31,7 @@
 
 namespace fa {
 
-constexpr int kLatentThreads = 288;
+constexpr int kLatentThreads = 320;
 constexpr uint32_t kLatentTile = 64;
 constexpr uint32_t kLatentSlot = kLatentTile * 128;   // bytes of 64 keys by 64 dimensions
 constexpr float kLatentSlack = 8.0f;                  // the reference moves when an exponent exceeds it by more: weights stay below 2^8
@@ -130,8 +131,9 @@ struct LatentWalk {
 };
 __device__ __forceinline__ bool latent_start(const LatentRowsArgs& p, uint32_t part, LatentWalk& w) {
     const uint32_t lane = threadIdx.x & 31u;
-    uint32_t total = 0;
-    for (uint32_t b = lane; b < p.s.B; b += 32) total += latent_units(p, b);
+    uint32_t total = 0, kept = 0;
+    for (uint32_t b = lane; b < p.s.B; b += 32) total += kept = latent_units(p, b);
+    if (lane >= p.s.B) kept = 0;
     total = __reduce_add_sync(0xFFFFFFFFu, total);
     const uint32_t parts = min(p.parts, (total + p.least - 1u) / p.least);
     if (part >= parts) return false;
@@ -140,7 +142,7 @@ __device__ __forceinline__ bool latent_start(const LatentRowsArgs& p, uint32_t p
     w.unit_end = (part + 1u) * w.each + min(part + 1u, w.more);
     w.before = 0, w.b = 0;
     for (uint32_t b0 = 0; b0 < p.s.B; b0 += 32) {
-        const uint32_t mine = b0 + lane < p.s.B ? latent_units(p, b0 + lane) : 0u;
+        const uint32_t mine = p.s.B <= 32 ? kept : b0 + lane < p.s.B ? latent_units(p, b0 + lane) : 0u;
         uint32_t upto = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -235,7 +237,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
     FA_CACHE_POISON(base, C::kTiles);
     fence_proxy_async_smem();
 #endif
-    if (warp == 5) {
+    if (warp == 6) {
         tmem_alloc(smem_u32(&tmem_slot), C::kCols);
         tmem_relinquish();
     }
@@ -490,16 +492,18 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
             tc_fence_before();
             softmax_sync();   // s_l and s_m are read
         }
-    } else if (warp == 4) {
-        // ---------------------------------------------------------------- tiles
+    } else if (warp < 6) {
+        // ---------------------------------------------------------------- tiles: the first half of their dimensions, the second and the rotary part
+        const bool rear = warp == 5;
+        const uint32_t c_first = rear ? (C::kPairs + 1) / 2 : 0, c_end = rear ? C::kPairs : (C::kPairs + 1) / 2;
         const bool leader = elect_one();
         const uint32_t per_tile = p.c.page < kLatentTile ? kLatentTile >> p.c.page_shift : 1u;   // pages of a tile
         const uint32_t box_rows = min(p.c.page, kLatentTile), box_bytes = box_rows * 128;
-        uint32_t g = 0, reports = 0, pairs = 0, ropes = 0;   // (pairs, ropes: slots filled)
+        uint32_t g = 0, reports = 0, asked = 0;   // (asked: slots with a copy under way or done, up to this tile's)
         bool ok = true;
         while (ok && any && latent_next(p, group, w)) {
             const int32_t* const table = p.s.table + w.seq * p.s.table_stride;
-            if (w.begins && group == 0 && lane == 0 && !cache_length_ok(plain_view(p.c), p.s, w.seq)) cache_report(p.c.status, kCacheBadPosition);
+            if (!rear && w.begins && group == 0 && lane == 0 && !cache_length_ok(plain_view(p.c), p.s, w.seq)) cache_report(p.c.status, kCacheBadPosition);
             const uint32_t blocks = (w.q.held + p.c.page - 1u) >> p.c.page_shift;
             uint32_t known = 0, from = 0;   // entries [from, from + known) are in the lanes
             int32_t entry = -1;
@@ -509,18 +513,18 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                     from = first, known = 32;
                     entry = from + lane < blocks ? table[from + lane] : -1;
                     const bool wrong = from + lane < blocks && static_cast<uint32_t>(entry) >= p.c.n_pages && (from + lane) * p.c.page < w.end * kLatentTile;
-                    if (wrong) ++reports;
+                    if (wrong && !rear) ++reports;
                     if (static_cast<uint32_t>(entry) >= p.c.n_pages) entry = static_cast<int32_t>(p.c.n_pages);   // outside: TMA fills with zeros
                 }
                 uint32_t gone = 0;   // a bit for each 16 keys
                 for (uint32_t i = 0; i < per_tile; ++i)
                     if (static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, entry, first + i - from)) >= p.c.n_pages) gone |= (per_tile == 1 ? 15u : per_tile == 2 ? 3u : 1u) << (i * (4 / per_tile));
                 const uint32_t y = per_tile == 1 ? key0 & (p.c.page - 1u) : 0u;
-                for (uint32_t c = 0; c < C::kPairs; ++c) {
+                for (uint32_t c = c_first; c < c_end; ++c) {
                     const uint32_t n = g * C::kPairs + c;
                     if (n >= C::kPairSlots) ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(C::EMPTY + n % C::kPairSlots), (n / C::kPairSlots - 1u) & 1u, ctl, kCacheTimeout | C::EMPTY));
                     if (!ok) break;
-                    ++pairs;
+                    asked = g + 1;
                     if (leader) mbar_expect_tx(bar(C::FULL + n % C::kPairSlots), 2 * kLatentSlot);
                     for (uint32_t i = 0; i < per_tile; ++i) {
                         const int32_t page = __shfl_sync(0xFFFFFFFFu, entry, first + i - from);
@@ -531,9 +535,10 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                     }
                 }
                 if (!ok) break;
+                if (!rear) continue;
                 if (g >= C::kRopeSlots) ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(C::REMPTY + g % C::kRopeSlots), (g / C::kRopeSlots - 1u) & 1u, ctl, kCacheTimeout | C::REMPTY));
                 if (!ok) break;
-                ++ropes;
+                asked = g + 1;
                 if (leader) {
                     *reinterpret_cast<volatile uint32_t*>(&s_absent[g & 7u]) = gone;
                     mbar_expect_tx(bar(C::RFULL + g % C::kRopeSlots), kLatentSlot);
@@ -548,16 +553,15 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
         if (reports != 0) cache_report(p.c.status, kCacheBadPage);
         // What was asked for lands before the CTA ends: the MMAs have waited for it, unless a wait gave up.
         if (*ctl.abort_flag != 0u) {
-            for (uint32_t i = 0; i < C::kPairSlots; ++i) {
-                const uint32_t uses = (pairs + C::kPairSlots - 1u - i) / C::kPairSlots;
-                if (uses > 0) mbar_wait_certain(bar(C::FULL + i), (uses - 1u) & 1u, ctl, kCacheTimeout | C::FULL);
-            }
-            for (uint32_t i = 0; i < C::kRopeSlots; ++i) {
-                const uint32_t uses = (ropes + C::kRopeSlots - 1u - i) / C::kRopeSlots;
-                if (uses > 0) mbar_wait_certain(bar(C::RFULL + i), (uses - 1u) & 1u, ctl, kCacheTimeout | C::RFULL);
+            for (uint32_t tile = asked > C::kPairSlots ? asked - C::kPairSlots : 0; tile < asked; ++tile) {   // (what has landed answers at once)
+                for (uint32_t c = c_first; c < c_end; ++c) {
+                    const uint32_t n = tile * C::kPairs + c;
+                    if (n + C::kPairSlots >= asked * C::kPairs) mbar_wait_certain(bar(C::FULL + n % C::kPairSlots), (n / C::kPairSlots) & 1u, ctl, kCacheTimeout | C::FULL);
+                }
+                if (rear && tile + C::kRopeSlots >= asked) mbar_wait_certain(bar(C::RFULL + tile % C::kRopeSlots), (tile / C::kRopeSlots) & 1u, ctl, kCacheTimeout | C::RFULL);
             }
         }
-    } else if (warp == 5 || warp == 6) {
+    } else if (warp < 8) {
         // ---------------------------------------------------------------- MMAs: scores, results
         const bool leader = elect_one();
         bool ok = true;   // once a wait has given up nothing more is issued
@@ -567,9 +571,9 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
         uint32_t g = 0, k = 0;   // tiles; segments with tiles
         while (any && latent_next(p, group, w)) {
             if (w.end == w.t0) continue;
-            if (warp == 5) wait(C::QFULL, k & 1u);
+            if (warp == 6) wait(C::QFULL, k & 1u);
             for (uint32_t tile = w.t0; tile < w.end; ++tile, ++g) {
-                if (warp == 5) {
+                if (warp == 6) {
                     // (whoever read the scores two tiles ago has given P)
                     if (g >= 2) wait(C::P + (g & 1u), ((g >> 1) - 1u) & 1u);
                     const uint32_t tS = tmem + C::kColS + N * (g & 1u);
@@ -611,28 +615,32 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
             ++k;
         }
         // every product issued has to retire before tensor and shared memory are let go of
-        const int last = C::FINAL + (warp == 5 ? 0 : 1);
+        const int last = C::FINAL + (warp == 6 ? 0 : 1);
         if (leader) tc_commit(bar(last));
         __syncwarp();
         mbar_wait_certain(bar(last), 0, ctl, kCacheTimeout | static_cast<uint32_t>(last));
     } else {
         // ---------------------------------------------------------------- queries
-        const uint32_t lt = tid - 224u, rope_pieces = p.c.rope / 8;
+        const uint32_t lt = tid - 256u;
+        // rows [0, rows) of a tensor's part of the queries, `pieces` (a power of two, 64 at most) of 16 bytes each, to chunks at `to`
+        auto copy = [&](const uint8_t* from, int64_t t_stride, int64_t h_stride, uint32_t pieces, uint32_t rows, uint32_t to) {
+            const uint32_t j = lt & (pieces - 1u), step = 64u / pieces;
+            uint32_t r = lt / pieces, t = (row0 + r) / p.heads, h = row0 + r - t * p.heads;
+            const uint32_t chunk = to + (j >> 3) * C::kQChunk;
+#pragma unroll 4
+            for (; r < rows; r += step) {
+                const bool in = r < n_rows;   // (rows that are not there: zeros)
+                cp_async_16_zero(chunk + r * 128 + (((j & 7u) ^ (r & 7u)) << 4), in ? from + t * t_stride + h * h_stride + 16 * j : from, in);
+                for (h += step; h >= p.heads; h -= p.heads) ++t;
+            }
+        };
         uint32_t k = 0;
         while (any && latent_next(p, group, w)) {
             if (w.end == w.t0) continue;
             if (k > 0) mbar_wait(bar(C::QEMPTY), (k - 1u) & 1u, ctl, kCacheTimeout | C::QEMPTY);
-            const uint32_t rows = k == 0 ? static_cast<uint32_t>(N) : n_rows;   // (rows that are not there: zeros, once)
-            for (uint32_t i = lt; i < rows * (8 * LC); i += 64) {
-                const uint32_t r = i / (8 * LC), j = i % (8 * LC), t = (row0 + r) / p.heads, h = row0 + r - t * p.heads;
-                const bool in = r < n_rows;
-                cp_async_16_zero(base + (j / 8) * C::kQChunk + r * 128 + (((j & 7u) ^ (r & 7u)) << 4), p.q_latent + (in ? w.seq * p.ql_b + t * p.ql_t + h * p.ql_h + 16 * j : 0), in);
-            }
-            for (uint32_t i = lt; i < rows * rope_pieces; i += 64) {
-                const uint32_t r = i / rope_pieces, j = i % rope_pieces, t = (row0 + r) / p.heads, h = row0 + r - t * p.heads;
-                const bool in = r < n_rows;
-                cp_async_16_zero(base + LC * C::kQChunk + r * 128 + ((j ^ (r & 7u)) << 4), p.q_rope + (in ? w.seq * p.qr_b + t * p.qr_t + h * p.qr_h + 16 * j : 0), in);
-            }
+            const uint32_t rows = k == 0 ? static_cast<uint32_t>(N) : n_rows;
+            copy(p.q_latent + w.seq * p.ql_b, p.ql_t, p.ql_h, 8 * LC, rows, base);
+            copy(p.q_rope + w.seq * p.qr_b, p.qr_t, p.qr_h, p.c.rope / 8, rows, base + LC * C::kQChunk);
             cp_async_wait_all();
             fence_proxy_async_smem();
             mbar_arrive(bar(C::QFULL));
@@ -642,59 +650,65 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
     tc_fence_before();
     __syncthreads();
     if (tid == 0) report_expired(ctl);
-    if (warp == 5) {
+    if (warp == 6) {
         tc_fence_after();
         tmem_dealloc(tmem, C::kCols);
     }
 }
 
-// Puts the parts of divided sequences together.  A CTA has 128 dimensions of a row, its warps the parts in turn.
+// Puts the parts of divided sequences together: 128 dimensions of a row at a time.  By a warp (kWide false), where there are few parts, or by a
+// CTA whose warps take the parts in turn.
 constexpr int kLatentJoinWarps = 8;
-template <int LC, int N>
+template <int LC, int N, bool kWide>
 __global__ void __launch_bounds__(kLatentJoinWarps * 32) fa_latent_join(const LatentRowsArgs p) {
-    __shared__ float4 s_o[kLatentJoinWarps][32];
+    __shared__ float4 s_o[kWide ? kLatentJoinWarps : 1][32];
     __shared__ float s_sum[kLatentJoinWarps], s_top[kLatentJoinWarps];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint64_t item = kWide ? blockIdx.x : static_cast<uint64_t>(blockIdx.x) * kLatentJoinWarps + warp;
+    const uint32_t dims = static_cast<uint32_t>(item % (LC / 2)) * 128 + 4 * lane;
+    const uint64_t at = item / (LC / 2);
+    const uint32_t b = static_cast<uint32_t>(at / p.rows), row = static_cast<uint32_t>(at - static_cast<uint64_t>(b) * p.rows), group = row / p.group_rows, r = row - group * p.group_rows;
     grid_dep_wait();
     grid_dep_launch();
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    const uint32_t dims = blockIdx.x % (LC / 2) * 128 + 4 * lane;
-    const uint64_t at = blockIdx.x / (LC / 2);
-    const uint32_t b = static_cast<uint32_t>(at / p.rows), row = static_cast<uint32_t>(at - static_cast<uint64_t>(b) * p.rows), group = row / p.group_rows, r = row - group * p.group_rows;
-    const LatentSeq q = latent_seq(p, b);
-    uint8_t* const to = p.y + (at * (64 * LC) + dims) * 2;
-    if (q.count == 0 || q.held == 0) return;
+    if (b >= p.s.B) return;
+    // (what a sequence without tokens has for its share is not used: both are asked for at once)
     const int2 share = p.shares[b];
-    if (share.x == share.y) return;   // written where it was worked out
-    auto slot = [&](int part) { return (static_cast<uint64_t>(part) * p.groups + group) * 2u + (part == share.x ? 1u : 0u); };
+    if (latent_units(p, b) == 0 || share.x == share.y) return;   // written where it was worked out
+    auto slot = [&](int part) { return ((static_cast<uint64_t>(part) * p.groups + group) * 2u + (part == share.x ? 1u : 0u)) * N + r; };
     float top = -INFINITY;
-    for (int i = share.x + static_cast<int>(threadIdx.x); i <= share.y; i += kLatentJoinWarps * 32) top = fmaxf(top, p.part_ml[slot(i) * N + r].x);
+    for (int i = share.x + static_cast<int>(kWide ? threadIdx.x : lane); i <= share.y; i += kWide ? kLatentJoinWarps * 32 : 32) top = fmaxf(top, p.part_ml[slot(i)].x);
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-    if (lane == 0) s_top[warp] = top;
-    __syncthreads();
+    if (kWide) {
+        if (lane == 0) s_top[warp] = top;
+        __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kLatentJoinWarps; ++i) top = fmaxf(top, s_top[i]);
+        for (int i = 0; i < kLatentJoinWarps; ++i) top = fmaxf(top, s_top[i]);
+    }
+    if (top == -INFINITY) top = 0.0f;
     float4 o = make_float4(0, 0, 0, 0);
     float sum = 0.0f;
 #pragma unroll 4
-    for (int i = share.x + static_cast<int>(warp); i <= share.y; i += kLatentJoinWarps) {
-        const float2 ml = p.part_ml[slot(i) * N + r];
-        if (ml.y == 0.0f) continue;   // nothing seen there
-        const float f = ex2_approx((ml.x == -INFINITY ? 0.0f : ml.x) - (top == -INFINITY ? 0.0f : top));
-        const float4 x = *reinterpret_cast<const float4*>(p.part_o + (slot(i) * N + r) * (64 * LC) + dims);
+    for (int i = share.x + static_cast<int>(kWide ? warp : 0); i <= share.y; i += kWide ? kLatentJoinWarps : 1) {
+        const float2 ml = p.part_ml[slot(i)];
+        const float4 x = *reinterpret_cast<const float4*>(p.part_o + slot(i) * (64 * LC) + dims);
+        if (ml.y == 0.0f) continue;   // nothing seen there: what was read is nothing
+        const float f = ex2_approx((ml.x == -INFINITY ? 0.0f : ml.x) - top);
         o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y), o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
         sum = fmaf(ml.y, f, sum);
     }
-    s_o[warp][lane] = o;
-    if (lane == 0) s_sum[warp] = sum;
-    __syncthreads();
-    if (warp != 0) return;
-    for (int i = 1; i < kLatentJoinWarps; ++i) {
-        const float4 x = s_o[i][lane];
-        o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w, sum += s_sum[i];
+    if (kWide) {
+        s_o[warp][lane] = o;
+        if (lane == 0) s_sum[warp] = sum;
+        __syncthreads();
+        if (warp != 0) return;
+        for (int i = 1; i < kLatentJoinWarps; ++i) {
+            const float4 x = s_o[i][lane];
+            o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w, sum += s_sum[i];
+        }
     }
     const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-    *reinterpret_cast<uint2*>(to) = make_uint2(pack_16(o.x * f, o.y * f, p.bf16 != 0), pack_16(o.z * f, o.w * f, p.bf16 != 0));
+    *reinterpret_cast<uint2*>(p.y + (at * (64 * LC) + dims) * 2) = make_uint2(pack_16(o.x * f, o.y * f, p.bf16 != 0), pack_16(o.z * f, o.w * f, p.bf16 != 0));
 }
 
 }  // namespace fa
