@@ -9,16 +9,17 @@
 // Both products are tcgen05 MMAs on the same tile in shared memory, and both are kept transposed: S^T[64 keys, N] = C Q^T, and Y^T[128
 // dimensions, N] += C^T P^T.  Keys and dimensions are what an MMA's M is filled with, rows are its N, of which there may be few: four such
 // tiles hold 512 dimensions in 4 N columns of tensor memory, where Y[128 rows, 512] would need all 512 columns and leave none for the scores.
-// (Measured, clocks an MMA: M = 64 N = 16 or 32 27, N = 64 32; M = 128 N = 16 39, N = 32 40, N = 64 48.)  320 threads:
+// (Measured, clocks an MMA: M = 64 N = 16 or 32 27, N = 64 32; M = 128 N = 16 39, N = 32 40, N = 64 48.)  512 threads:
 //
-//   warps 0-3  softmax: a warp 16 keys, eight threads a row and 16 keys (tcgen05.ld.16x256b hands out scores that way).  All share a row's
-//              reference; it is looked at again only where a score exceeds it by more than 2^8, so that a tile passes with no maximum being
-//              formed.  P into shared memory; at the end of a segment (a sequence's tiles in this CTA) the division and Y, a thread a dimension
-//   warp 4, 5  fetch tiles by TMA: 64 keys of 128 dimensions a slot of one ring, of the rotary part a slot of another.  (Two, because what a
-//              thread asks of a barrier behind a TMA copy takes 280 clocks: one warp alone brings in a tile of 512 dimensions in 2550)
-//   warp 6, 7  issue the MMAs of the scores, of the results.  (One warp for both, as slots arrive: 94 us for 64 sequences of 100 to 8192
-//              tokens, 16 rows: a barrier's answer reaches a thread only behind the MMAs that it has queued, 575 clocks for 8 of them)
-//   warps 8-9  queries into shared memory, a segment ahead
+//   warps 0-7    softmax: a warp 16 keys and half of the rows, eight threads a row and 16 keys (tcgen05.ld.16x256b hands out scores that way).
+//                All share a row's reference; it is looked at again only where a score exceeds it by more than 2^8, so that a tile passes with
+//                no maximum being formed.  P into shared memory; at the end of a segment (a sequence's tiles in this CTA) the division and Y,
+//                a thread a dimension
+//   warps 8-11   fetch tiles by TMA: 64 keys of 128 dimensions a slot of one ring, of the rotary part a slot of another.  (Four, because what a
+//                thread asks of a barrier behind a TMA copy takes 280 clocks: one warp alone brings in a tile of 512 dimensions in 2550)
+//   warp 12, 13  issue the MMAs of the scores, of the results.  (One warp for both, as slots arrive: 94 us for 64 sequences of 100 to 8192
+//                tokens, 16 rows, where two took 72: a barrier's answer reaches a thread only behind the MMAs that it has queued)
+//   warps 14-15  queries into shared memory, a segment ahead; of the first segment the softmax warps do most
 //
 // What must not happen: a key that a row does not see reaching it, as 0 * NaN.  Tiles that some row of the group sees in part only (the
 // last ones of a sequence) are gone over in shared memory between the two products: keys behind the last that any row sees become zeros;
@@ -31,7 +32,8 @@
 
 namespace fa {
 
-constexpr int kLatentThreads = 320;
+constexpr int kLatentThreads = 512;
+constexpr uint32_t kLatentSoftmax = 256;              // threads of the softmax warps
 constexpr uint32_t kLatentTile = 64;
 constexpr uint32_t kLatentSlot = kLatentTile * 128;   // bytes of 64 keys by 64 dimensions
 constexpr float kLatentSlack = 8.0f;                  // the reference moves when an exponent exceeds it by more: weights stay below 2^8
@@ -79,21 +81,18 @@ struct LatentCfg {
 __device__ __forceinline__ uint32_t idesc_16bit(uint32_t m, uint32_t n, bool a_mn, bool b_mn, bool bf16) {
     return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
-// 16 lanes x 16 columns: thread t receives of lane t / 4 (v[4 j], v[4 j + 1]) and of lane t / 4 + 8 (v[4 j + 2], v[4 j + 3]) columns 8 j + 2 (t % 4) and the next.
-__device__ __forceinline__ void tmem_ld_16x16(uint32_t taddr, float* v) {
-    FA_DBG_TMEM(taddr, 16u);
-    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
-                 : "r"(taddr)
-                 : "memory");
+// 16 lanes x 8 columns: thread t receives of lane t / 4 (v[0], v[1]) and of lane t / 4 + 8 (v[2], v[3]) columns 2 (t % 4) and the next.
+__device__ __forceinline__ void tmem_ld_16x8(uint32_t taddr, float* v) {
+    FA_DBG_TMEM(taddr, 8u);
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(taddr) : "memory");
 }
-// Of warps 0-3: all there, and whether any thread says so.
+// Of warps 0-7: all there, and whether any thread says so.
 __device__ __forceinline__ bool softmax_any(bool x) {
     uint32_t r;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"(static_cast<uint32_t>(x)) : "memory");
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"(static_cast<uint32_t>(x)) : "memory");
     return r != 0;
 }
-__device__ __forceinline__ void softmax_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void softmax_sync() { asm volatile("barrier.cta.sync 1, 256;" ::: "memory"); }
 
 // What rows see.  A sequence holds `held` tokens, of the call's T it has `count`, the last of those that it holds.
 struct LatentSeq {
@@ -223,7 +222,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
     const bool bf16 = p.bf16 != 0;
 
     if (tid == 0) {
-        for (int i = 0; i < C::kBarriers; ++i) mbar_init(bar(i), i == C::QFULL ? 64u : 1u);
+        for (int i = 0; i < C::kBarriers; ++i) mbar_init(bar(i), i == C::QFULL ? 64u : i >= C::P && i < C::PV ? 8u : 1u);
         abort_flag = 0;
         fence_mbar_init();
         prefetch_tensormap(&map);
@@ -237,7 +236,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
     FA_CACHE_POISON(base, C::kTiles);
     fence_proxy_async_smem();
 #endif
-    if (warp == 6) {
+    if (warp == 12) {
         tmem_alloc(smem_u32(&tmem_slot), C::kCols);
         tmem_relinquish();
     }
@@ -252,20 +251,46 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
     __syncthreads();
 #endif
 
+    // Rows [0, rows) of a sequence's queries, as thread `who` of `of` (a multiple of 64; rows that are not there: zeros).
+    auto copy_queries = [&](uint32_t seq, uint32_t who, uint32_t of, uint32_t rows) {
+        auto copy = [&](const uint8_t* from, int64_t t_stride, int64_t h_stride, uint32_t pieces, uint32_t to) {   // `pieces` of 16 bytes each: a power of two, 64 at most
+            const uint32_t j = who & (pieces - 1u), step = of / pieces;
+            uint32_t r = who / pieces, t = (row0 + r) / p.heads, h = row0 + r - t * p.heads;
+            const uint32_t chunk = to + (j >> 3) * C::kQChunk;
+#pragma unroll 4
+            for (; r < rows; r += step) {
+                const bool in = r < n_rows;
+                cp_async_16_zero(chunk + r * 128 + (((j & 7u) ^ (r & 7u)) << 4), in ? from + t * t_stride + h * h_stride + 16 * j : from, in);
+                for (h += step; h >= p.heads; h -= p.heads) ++t;
+            }
+        };
+        copy(p.q_latent + seq * p.ql_b, p.ql_t, p.ql_h, 8 * LC, base);
+        copy(p.q_rope + seq * p.qr_b, p.qr_t, p.qr_h, p.c.rope / 8, base + LC * C::kQChunk);
+    };
+
     LatentWalk w;
     const bool any = latent_start(p, part, w);
-    if (warp < 4) {
+    if (warp < 8) {
         // ---------------------------------------------------------------- softmax
-        const uint32_t lane_off = (warp * 32u) << 16;
-        const uint32_t quad = lane & 3u, key_a = 16 * warp + lane / 4;   // this thread's keys of a tile: key_a and key_a + 8; its rows: 8 j + 2 quad + e
-        constexpr int kBlocks = N / 8;
+        const uint32_t lanes = warp & 3u, side = warp >> 2, lane_off = (lanes * 32u) << 16;
+        // this thread's keys of a tile: key_a and key_a + 8; its rows: first + 8 j + 2 quad + e
+        const uint32_t quad = lane & 3u, key_a = 16 * lanes + lane / 4, first = side * (N / 2);
+        constexpr int kBlocks = N / 16;
         uint32_t g = 0, partly = 0;
+        bool helped = false;   // with the first segment's queries
         for (uint32_t b = part; b < p.s.B; b += p.parts) {   // sequences without tokens
             if (latent_units(p, b) != 0) continue;
             uint8_t* const to = p.y + (static_cast<uint64_t>(b) * p.rows + row0) * (128 * LC);
-            for (uint32_t i = tid; i < n_rows * (8 * LC); i += 128) *reinterpret_cast<uint4*>(to + 16 * i) = make_uint4(0, 0, 0, 0);
+            for (uint32_t i = tid; i < n_rows * (8 * LC); i += kLatentSoftmax) *reinterpret_cast<uint4*>(to + 16 * i) = make_uint4(0, 0, 0, 0);
         }
         while (any && latent_next(p, group, w)) {
+            if (!helped && w.end > w.t0) {
+                copy_queries(w.seq, tid, kLatentSoftmax + 64u, N);
+                cp_async_wait_all();
+                fence_proxy_async_smem();
+                asm volatile("barrier.cta.arrive 2, 320;" ::: "memory");
+                helped = true;
+            }
             if (group == 0 && w.begins && tid == 0)
                 p.shares[w.seq] = make_int2(static_cast<int>(part), static_cast<int>(latent_owner(w, w.first_unit + w.units - 1u)));
             if (tid < N) {   // (what becomes of a row that sees nothing is not used)
@@ -295,7 +320,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                 __syncwarp();
                 float s[4 * kBlocks];
 #pragma unroll
-                for (int i = 0; i < N / 16; ++i) tmem_ld_16x16(tmem + lane_off + C::kColS + N * (g & 1u) + 16 * i, s + 8 * i);
+                for (int j = 0; j < kBlocks; ++j) tmem_ld_16x8(tmem + lane_off + C::kColS + N * (g & 1u) + first + 8 * j, s + 4 * j);
                 // (the rotary slot's barrier: what the fetching warp has written about this tile is there)
                 mbar_wait(bar(C::RFULL + g % C::kRopeSlots), (g / C::kRopeSlots) & 1u, ctl, kCacheTimeout | C::RFULL);
                 const uint32_t absent = *reinterpret_cast<volatile uint32_t*>(&s_absent[g & 7u]);
@@ -303,32 +328,28 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                 if (key0 + kLatentTile > least || absent != 0) {
                     uint32_t bad_lo = 0, bad_hi = 0;
                     if (key0 + kLatentTile > least) {
-                        // two threads a key: pieces of 16 bytes, four of each 64 dimensions
-                        const uint32_t key = tid >> 1, half = tid & 1u, at = key0 + key, swz = key & 7u;
+                        // four threads a key: pieces of 16 bytes, two of each 64 dimensions
+                        const uint32_t key = tid >> 2, part4 = tid & 3u, at = key0 + key, swz = key & 7u;
                         const bool behind = at >= w.farthest, some = !behind && at >= least;
                         bool bad = false;
 #pragma unroll
                         for (int c = 0; c < C::kPairs; ++c) mbar_wait(bar(C::FULL + (g * C::kPairs + c) % C::kPairSlots), ((g * C::kPairs + c) / C::kPairSlots) & 1u, ctl, kCacheTimeout | C::FULL);
-                        if (some) {
-                            for (uint32_t c = 0; c < LC; ++c)
-                                for (uint32_t j = 0; j < 4; ++j) {
-                                    uint32_t x[4];
-                                    ld_shared_v4(pair_addr(g * C::kPairs + c / 2) + (c & 1u) * kLatentSlot + key * 128 + (((4 * half + j) ^ swz) << 4), x);
-                                    bad |= not_finite(x, bf16);
-                                }
-                            for (uint32_t j = 0; j < 4; ++j) {
+                        auto piece = [&](uint32_t c, uint32_t j) {
+                            return (c == LC ? rope_addr(g) : pair_addr(g * C::kPairs + c / 2) + (c & 1u) * kLatentSlot) + key * 128 + (((2 * part4 + j) ^ swz) << 4);
+                        };
+                        if (some)
+#pragma unroll 1
+                            for (uint32_t c = 0; c < 2 * (LC + 1); ++c) {
                                 uint32_t x[4];
-                                ld_shared_v4(rope_addr(g) + key * 128 + (((4 * half + j) ^ swz) << 4), x);
+                                ld_shared_v4(piece(c >> 1, c & 1u), x);
                                 bad |= not_finite(x, bf16);
                             }
-                        }
                         bad |= __shfl_xor_sync(0xFFFFFFFFu, bad, 1) != 0;
-                        if (behind || bad) {
-                            for (uint32_t c = 0; c < LC; ++c)
-                                for (uint32_t j = 0; j < 4; ++j)
-                                    st_shared_v4(pair_addr(g * C::kPairs + c / 2) + (c & 1u) * kLatentSlot + key * 128 + (((4 * half + j) ^ swz) << 4), 0, 0, 0, 0);
-                        }
-                        if (bad && half == 0) atomicOr(&s_bad[partly & 1u][key >> 5], 1u << (key & 31u));
+                        bad |= __shfl_xor_sync(0xFFFFFFFFu, bad, 2) != 0;
+                        if (behind || bad)
+#pragma unroll 1
+                            for (uint32_t c = 0; c < 2 * LC; ++c) st_shared_v4(piece(c >> 1, c & 1u), 0, 0, 0, 0);
+                        if (bad && part4 == 0) atomicOr(&s_bad[partly & 1u][key >> 5], 1u << (key & 31u));
                         fence_proxy_async_smem();
                         softmax_sync();
                         bad_lo = *reinterpret_cast<volatile uint32_t*>(&s_bad[partly & 1u][0]);
@@ -345,31 +366,13 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                         for (uint32_t j = 0; j < kBlocks; ++j) {
 #pragma unroll
                             for (uint32_t e = 0; e < 2; ++e) {
-                                if (gone || at >= s_limit[8 * j + 2 * quad + e]) s[4 * j + 2 * i + e] = -INFINITY;
+                                if (gone || at >= s_limit[first + 8 * j + 2 * quad + e]) s[4 * j + 2 * i + e] = -INFINITY;
                                 else if (bad) s[4 * j + 2 * i + e] = __int_as_float(0x7FC00000);
                             }
                         }
                     }
                 }
-                // the last P V that read this buffer of P
-                if (g >= C::kPBuffers) {
-                    const uint32_t h = g - C::kPBuffers;
-                    mbar_wait(bar(C::PV + (h & 1u)), (h >> 1) & 1u, ctl, kCacheTimeout | C::PV);
-                }
-                // ---- weights by the rows' references, rounded; whether some score asks for another reference
-                uint32_t pk[2 * kBlocks];
-                auto weights = [&] {
-#pragma unroll
-                    for (uint32_t j = 0; j < kBlocks; ++j) {
-                        const float r0 = m[2 * j] == -INFINITY ? 0.0f : m[2 * j], r1 = m[2 * j + 1] == -INFINITY ? 0.0f : m[2 * j + 1];
-#pragma unroll
-                        for (uint32_t i = 0; i < 2; ++i) {
-                            pk[2 * j + i] = pack_16(ex2_approx(fmaf(s[4 * j + 2 * i], p.scale_log2, -r0)), ex2_approx(fmaf(s[4 * j + 2 * i + 1], p.scale_log2, -r1)), bf16);
-                            const uint32_t row = key_a + 8 * i;
-                            st_shared_u32(p_addr(g) + row * C::kPitch + ((j ^ (row * C::kPitch >> 7 & (C::kPitch / 16 - 1))) << 4) + 4 * quad, pk[2 * j + i]);
-                        }
-                    }
-                };
+                // ---- whether some score asks for another reference
                 bool above = tile == w.t0;
                 if (!above) {
 #pragma unroll
@@ -377,12 +380,9 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
 #pragma unroll
                         for (int e = 0; e < 2; ++e)
                             above |= fmaxf(s[4 * j + e], s[4 * j + 2 + e]) * p.scale_log2 > (m[2 * j + e] == -INFINITY ? -INFINITY : m[2 * j + e] + kLatentSlack);
-                    weights();
-                    fence_proxy_async_smem();
-                    tc_fence_before();
+                    above = softmax_any(above);
                 }
-                if (softmax_any(above)) {
-                    // ---- the largest score of every row that it is too large for its reference
+                if (above) {   // the largest score of every row; a new reference where it exceeds the old one by too much
 #pragma unroll
                     for (int j = 0; j < kBlocks; ++j)
 #pragma unroll
@@ -390,14 +390,14 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                             float top = fmaxf(s[4 * j + e], s[4 * j + 2 + e]);
 #pragma unroll
                             for (int d = 4; d <= 16; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-                            if (lane < 4) s_max[warp][8 * j + 2 * quad + e] = top;
+                            if (lane < 4) s_max[lanes][first + 8 * j + 2 * quad + e] = top;
                         }
                     softmax_sync();
 #pragma unroll
                     for (int j = 0; j < kBlocks; ++j)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            const int r = 8 * j + 2 * quad + e;
+                            const uint32_t r = first + 8 * j + 2 * quad + e;
                             const float top = fmaxf(fmaxf(s_max[0][r], s_max[1][r]), fmaxf(s_max[2][r], s_max[3][r])) * p.scale_log2;
                             float alpha = 1.0f;
                             if (top > (m[2 * j + e] == -INFINITY ? -INFINITY : m[2 * j + e] + kLatentSlack)) {
@@ -405,17 +405,15 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                                 m[2 * j + e] = top;
                                 l[2 * j + e] *= alpha;
                             }
-                            if (tid < 4) s_alpha[r] = alpha;
+                            if (lanes == 0 && lane < 4) s_alpha[r] = alpha;
                         }
-                    weights();
-                    fence_proxy_async_smem();
                     softmax_sync();
-                    if (tile > w.t0) {   // rows are columns of Y^T: every warp multiplies all of them, in its dimensions
+                    if (tile > w.t0) {   // rows are columns of Y^T: every warp multiplies all of them, in its dimensions, its side every other 16 columns
                         mbar_wait(bar(C::PV + ((g - 1u) & 1u)), ((g - 1u) >> 1) & 1u, ctl, kCacheTimeout | C::PV);
                         tc_fence_after();
                         __syncwarp();
 #pragma unroll 1
-                        for (uint32_t c = 0; c < C::kPairs * N; c += 16) {
+                        for (uint32_t c = 16 * side; c < C::kPairs * N; c += 32) {
                             float o[16];
                             uint32_t x[16];
                             tmem_ld16(tmem + lane_off + c, o);
@@ -426,10 +424,28 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                         }
                         tmem_wait_st();
                     }
-                    tc_fence_before();
-                    softmax_sync();
                 }
-                if (tid == 0) mbar_arrive(bar(C::P + (g & 1u)));
+                // the last P V that read this buffer of P
+                if (g >= C::kPBuffers) {
+                    const uint32_t h = g - C::kPBuffers;
+                    mbar_wait(bar(C::PV + (h & 1u)), (h >> 1) & 1u, ctl, kCacheTimeout | C::PV);
+                }
+                // ---- weights, rounded
+                uint32_t pk[2 * kBlocks];
+#pragma unroll
+                for (uint32_t j = 0; j < kBlocks; ++j) {
+                    const float r0 = m[2 * j] == -INFINITY ? 0.0f : m[2 * j], r1 = m[2 * j + 1] == -INFINITY ? 0.0f : m[2 * j + 1];
+#pragma unroll
+                    for (uint32_t i = 0; i < 2; ++i) {
+                        pk[2 * j + i] = pack_16(ex2_approx(fmaf(s[4 * j + 2 * i], p.scale_log2, -r0)), ex2_approx(fmaf(s[4 * j + 2 * i + 1], p.scale_log2, -r1)), bf16);
+                        const uint32_t row = key_a + 8 * i;
+                        st_shared_u32(p_addr(g) + row * C::kPitch + (((first / 8 + j) ^ (row * C::kPitch >> 7 & (C::kPitch / 16 - 1))) << 4) + 4 * quad, pk[2 * j + i]);
+                    }
+                }
+                fence_proxy_async_smem();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(C::P + (g & 1u)));
                 // sums of the weights as they are rounded
 #pragma unroll
                 for (int j = 0; j < kBlocks; ++j) {
@@ -439,6 +455,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                 }
             }
             // ---- the segment's end
+            softmax_sync();   // (s_alpha, s_limit are not read any more)
 #pragma unroll
             for (int j = 0; j < kBlocks; ++j)
 #pragma unroll
@@ -446,8 +463,8 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                     float x = l[2 * j + e];
 #pragma unroll
                     for (int d = 4; d <= 16; d <<= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, d);
-                    if (lane < 4) s_sum[warp][8 * j + 2 * quad + e] = x;
-                    if (tid < 4) s_m[8 * j + 2 * quad + e] = m[2 * j + e];
+                    if (lane < 4) s_sum[lanes][first + 8 * j + 2 * quad + e] = x;
+                    if (lanes == 0 && lane < 4) s_m[first + 8 * j + 2 * quad + e] = m[2 * j + e];
                 }
             softmax_sync();
             if (tid < N) {
@@ -466,13 +483,13 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
             if (!w.whole && tid < n_rows) p.part_ml[static_cast<uint64_t>(slot) * N + tid] = make_float2(s_m[tid], s_l[tid]);
             if (tiles || w.whole) {
 #pragma unroll 1
-                for (uint32_t c = 0; c < C::kPairs * N; c += 16) {
+                for (uint32_t c = 16 * side; c < C::kPairs * N; c += 32) {
                     float o[16];
                     if (tiles) {
                         tmem_ld16(tmem + lane_off + c, o);
                         tmem_wait_ld();
                     }
-                    const uint32_t r0 = c % N, d = c / N * 128 + warp * 32 + lane;
+                    const uint32_t r0 = c % N, d = c / N * 128 + lanes * 32 + lane;
                     if (w.whole) {
                         uint8_t* const to = p.y + ((static_cast<uint64_t>(w.seq) * p.rows + row0 + r0) * (64 * LC) + d) * 2;
 #pragma unroll
@@ -492,10 +509,10 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
             tc_fence_before();
             softmax_sync();   // s_l and s_m are read
         }
-    } else if (warp < 6) {
-        // ---------------------------------------------------------------- tiles: the first half of their dimensions, the second and the rotary part
-        const bool rear = warp == 5;
-        const uint32_t c_first = rear ? (C::kPairs + 1) / 2 : 0, c_end = rear ? C::kPairs : (C::kPairs + 1) / 2;
+    } else if (warp < 12) {
+        // ---------------------------------------------------------------- tiles: 128 dimensions of each, the last warp the rotary part too
+        const bool rear = warp == 11;
+        const uint32_t c_first = min(warp - 8u, static_cast<uint32_t>(C::kPairs)), c_end = min(warp - 7u, static_cast<uint32_t>(C::kPairs));
         const bool leader = elect_one();
         const uint32_t per_tile = p.c.page < kLatentTile ? kLatentTile >> p.c.page_shift : 1u;   // pages of a tile
         const uint32_t box_rows = min(p.c.page, kLatentTile), box_bytes = box_rows * 128;
@@ -503,7 +520,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
         bool ok = true;
         while (ok && any && latent_next(p, group, w)) {
             const int32_t* const table = p.s.table + w.seq * p.s.table_stride;
-            if (!rear && w.begins && group == 0 && lane == 0 && !cache_length_ok(plain_view(p.c), p.s, w.seq)) cache_report(p.c.status, kCacheBadPosition);
+            if (warp == 8 && w.begins && group == 0 && lane == 0 && !cache_length_ok(plain_view(p.c), p.s, w.seq)) cache_report(p.c.status, kCacheBadPosition);
             const uint32_t blocks = (w.q.held + p.c.page - 1u) >> p.c.page_shift;
             uint32_t known = 0, from = 0;   // entries [from, from + known) are in the lanes
             int32_t entry = -1;
@@ -513,7 +530,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                     from = first, known = 32;
                     entry = from + lane < blocks ? table[from + lane] : -1;
                     const bool wrong = from + lane < blocks && static_cast<uint32_t>(entry) >= p.c.n_pages && (from + lane) * p.c.page < w.end * kLatentTile;
-                    if (wrong && !rear) ++reports;
+                    if (wrong && warp == 8) ++reports;
                     if (static_cast<uint32_t>(entry) >= p.c.n_pages) entry = static_cast<int32_t>(p.c.n_pages);   // outside: TMA fills with zeros
                 }
                 uint32_t gone = 0;   // a bit for each 16 keys
@@ -561,7 +578,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                 if (rear && tile + C::kRopeSlots >= asked) mbar_wait_certain(bar(C::RFULL + tile % C::kRopeSlots), (tile / C::kRopeSlots) & 1u, ctl, kCacheTimeout | C::RFULL);
             }
         }
-    } else if (warp < 8) {
+    } else if (warp < 14) {
         // ---------------------------------------------------------------- MMAs: scores, results
         const bool leader = elect_one();
         bool ok = true;   // once a wait has given up nothing more is issued
@@ -571,22 +588,28 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
         uint32_t g = 0, k = 0;   // tiles; segments with tiles
         while (any && latent_next(p, group, w)) {
             if (w.end == w.t0) continue;
-            if (warp == 6) wait(C::QFULL, k & 1u);
+            if (warp == 12) wait(C::QFULL, k & 1u);
             for (uint32_t tile = w.t0; tile < w.end; ++tile, ++g) {
-                if (warp == 6) {
+                if (warp == 12) {
                     // (whoever read the scores two tiles ago has given P)
                     if (g >= 2) wait(C::P + (g & 1u), ((g >> 1) - 1u) & 1u);
                     const uint32_t tS = tmem + C::kColS + N * (g & 1u);
-                    for (uint32_t c = 0; c < C::kPairs; ++c) wait(C::FULL + (g * C::kPairs + c) % C::kPairSlots, ((g * C::kPairs + c) / C::kPairSlots) & 1u);
-                    wait(C::RFULL + g % C::kRopeSlots, (g / C::kRopeSlots) & 1u);
-                    tc_fence_after();
-                    if (leader && ok) {
+                    // (in two halves: the first goes on while the second's slots arrive)
+                    constexpr uint32_t kFront = (C::kPairs + 1) / 2;
 #pragma unroll
-                        for (uint32_t c = 0; c < LC; ++c) {
+                    for (uint32_t half = 0; half < 2; ++half) {
+                        const uint32_t c0 = half ? kFront : 0, c1 = half ? C::kPairs : kFront;
+                        for (uint32_t c = c0; c < c1; ++c) wait(C::FULL + (g * C::kPairs + c) % C::kPairSlots, ((g * C::kPairs + c) / C::kPairSlots) & 1u);
+                        if (half) wait(C::RFULL + g % C::kRopeSlots, (g / C::kRopeSlots) & 1u);
+                        tc_fence_after();
+                        if (!leader || !ok) continue;
+#pragma unroll
+                        for (uint32_t c = 2 * c0; c < 2 * c1; ++c) {
                             const uint64_t dk = make_smem_desc<128>(pair_addr(g * C::kPairs + c / 2) + (c & 1u) * kLatentSlot, 16), dq = make_smem_desc<128>(base + c * C::kQChunk, 16);
 #pragma unroll
                             for (uint32_t ks = 0; ks < 4; ++ks) mma_ss(tS, dk + 2 * ks, dq + 2 * ks, idesc_s, c + ks > 0 ? 1u : 0u);
                         }
+                        if (half == 0) continue;
                         const uint64_t dk = make_smem_desc<128>(rope_addr(g), 16), dq = make_smem_desc<128>(base + LC * C::kQChunk, 16);
                         for (uint32_t ks = 0; ks < rope_steps; ++ks) mma_ss(tS, dk + 2 * ks, dq + 2 * ks, idesc_s, 1u);
                         tc_commit(bar(C::S + (g & 1u)));
@@ -615,34 +638,26 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
             ++k;
         }
         // every product issued has to retire before tensor and shared memory are let go of
-        const int last = C::FINAL + (warp == 6 ? 0 : 1);
+        const int last = C::FINAL + (warp == 12 ? 0 : 1);
         if (leader) tc_commit(bar(last));
         __syncwarp();
         mbar_wait_certain(bar(last), 0, ctl, kCacheTimeout | static_cast<uint32_t>(last));
     } else {
         // ---------------------------------------------------------------- queries
-        const uint32_t lt = tid - 256u;
-        // rows [0, rows) of a tensor's part of the queries, `pieces` (a power of two, 64 at most) of 16 bytes each, to chunks at `to`
-        auto copy = [&](const uint8_t* from, int64_t t_stride, int64_t h_stride, uint32_t pieces, uint32_t rows, uint32_t to) {
-            const uint32_t j = lt & (pieces - 1u), step = 64u / pieces;
-            uint32_t r = lt / pieces, t = (row0 + r) / p.heads, h = row0 + r - t * p.heads;
-            const uint32_t chunk = to + (j >> 3) * C::kQChunk;
-#pragma unroll 4
-            for (; r < rows; r += step) {
-                const bool in = r < n_rows;   // (rows that are not there: zeros)
-                cp_async_16_zero(chunk + r * 128 + (((j & 7u) ^ (r & 7u)) << 4), in ? from + t * t_stride + h * h_stride + 16 * j : from, in);
-                for (h += step; h >= p.heads; h -= p.heads) ++t;
-            }
-        };
         uint32_t k = 0;
         while (any && latent_next(p, group, w)) {
             if (w.end == w.t0) continue;
             if (k > 0) mbar_wait(bar(C::QEMPTY), (k - 1u) & 1u, ctl, kCacheTimeout | C::QEMPTY);
-            const uint32_t rows = k == 0 ? static_cast<uint32_t>(N) : n_rows;
-            copy(p.q_latent + w.seq * p.ql_b, p.ql_t, p.ql_h, 8 * LC, rows, base);
-            copy(p.q_rope + w.seq * p.qr_b, p.qr_t, p.qr_h, p.c.rope / 8, rows, base + LC * C::kQChunk);
-            cp_async_wait_all();
-            fence_proxy_async_smem();
+            if (k == 0) {
+                copy_queries(w.seq, kLatentSoftmax + tid - 448u, kLatentSoftmax + 64u, N);
+                cp_async_wait_all();
+                fence_proxy_async_smem();
+                asm volatile("barrier.cta.sync 2, 320;" ::: "memory");   // the softmax warps' share is there
+            } else {
+                copy_queries(w.seq, tid - 448u, 64u, n_rows);
+                cp_async_wait_all();
+                fence_proxy_async_smem();
+            }
             mbar_arrive(bar(C::QFULL));
             ++k;
         }
@@ -650,7 +665,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
     tc_fence_before();
     __syncthreads();
     if (tid == 0) report_expired(ctl);
-    if (warp == 6) {
+    if (warp == 12) {
         tc_fence_after();
         tmem_dealloc(tmem, C::kCols);
     }
