@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
     float (&s_sum)[4][N] = s_max;
     float (&s_m)[N] = s_alpha;
     float* const s_l = reinterpret_cast<float*>(s_limit);
-    __shared__ uint32_t s_absent[8];         // of tile g in entry g % 8: its 16-key groups without a page
+    __shared__ uint32_t s_absent[16];        // of tile g in entry g % 16 (more than the ring has tiles): its 16-key groups without a page
     __shared__ uint32_t s_bad[2][2];         // of the partly seen tile n in entry n % 2: keys that hold no finite numbers
     __shared__ uint32_t tmem_slot, abort_flag;
 
@@ -321,9 +321,9 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                 float s[4 * kBlocks];
 #pragma unroll
                 for (int j = 0; j < kBlocks; ++j) tmem_ld_16x8(tmem + lane_off + C::kColS + N * (g & 1u) + first + 8 * j, s + 4 * j);
-                // (the rotary slot's barrier: what the fetching warp has written about this tile is there)
-                mbar_wait(bar(C::RFULL + g % C::kRopeSlots), (g / C::kRopeSlots) & 1u, ctl, kCacheTimeout | C::RFULL);
-                const uint32_t absent = *reinterpret_cast<volatile uint32_t*>(&s_absent[g & 7u]);
+                // (the first slot's barrier: what the fetching warp has written about this tile is there)
+                mbar_wait(bar(C::FULL + g * C::kPairs % C::kPairSlots), (g * C::kPairs / C::kPairSlots) & 1u, ctl, kCacheTimeout | C::FULL);
+                const uint32_t absent = *reinterpret_cast<volatile uint32_t*>(&s_absent[g & 15u]);
                 tmem_wait_ld();
                 if (key0 + kLatentTile > least || absent != 0) {
                     uint32_t bad_lo = 0, bad_hi = 0;
@@ -335,11 +335,11 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
 #pragma unroll
                         for (int c = 0; c < C::kPairs; ++c) mbar_wait(bar(C::FULL + (g * C::kPairs + c) % C::kPairSlots), ((g * C::kPairs + c) / C::kPairSlots) & 1u, ctl, kCacheTimeout | C::FULL);
                         auto piece = [&](uint32_t c, uint32_t j) {
-                            return (c == LC ? rope_addr(g) : pair_addr(g * C::kPairs + c / 2) + (c & 1u) * kLatentSlot) + key * 128 + (((2 * part4 + j) ^ swz) << 4);
+                            return pair_addr(g * C::kPairs + c / 2) + (c & 1u) * kLatentSlot + key * 128 + (((2 * part4 + j) ^ swz) << 4);
                         };
                         if (some)
 #pragma unroll 1
-                            for (uint32_t c = 0; c < 2 * (LC + 1); ++c) {
+                            for (uint32_t c = 0; c < 2 * LC; ++c) {
                                 uint32_t x[4];
                                 ld_shared_v4(piece(c >> 1, c & 1u), x);
                                 bad |= not_finite(x, bf16);
@@ -537,12 +537,25 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                 for (uint32_t i = 0; i < per_tile; ++i)
                     if (static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, entry, first + i - from)) >= p.c.n_pages) gone |= (per_tile == 1 ? 15u : per_tile == 2 ? 3u : 1u) << (i * (4 / per_tile));
                 const uint32_t y = per_tile == 1 ? key0 & (p.c.page - 1u) : 0u;
+                if (rear) {   // (its slot is let go of before the others)
+                    if (g >= C::kRopeSlots) ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(C::REMPTY + g % C::kRopeSlots), (g / C::kRopeSlots - 1u) & 1u, ctl, kCacheTimeout | C::REMPTY));
+                    if (!ok) break;
+                    asked = g + 1;
+                    if (leader) mbar_expect_tx(bar(C::RFULL + g % C::kRopeSlots), kLatentSlot);
+                    for (uint32_t i = 0; i < per_tile; ++i) {
+                        const int32_t page = __shfl_sync(0xFFFFFFFFu, entry, first + i - from);
+                        if (leader) tma_load_3d(rope_addr(g) + i * box_bytes, &map, bar(C::RFULL + g % C::kRopeSlots), 64 * LC, static_cast<int32_t>(y), page);
+                    }
+                }
                 for (uint32_t c = c_first; c < c_end; ++c) {
                     const uint32_t n = g * C::kPairs + c;
                     if (n >= C::kPairSlots) ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(C::EMPTY + n % C::kPairSlots), (n / C::kPairSlots - 1u) & 1u, ctl, kCacheTimeout | C::EMPTY));
                     if (!ok) break;
                     asked = g + 1;
-                    if (leader) mbar_expect_tx(bar(C::FULL + n % C::kPairSlots), 2 * kLatentSlot);
+                    if (leader) {
+                        if (c == 0) *reinterpret_cast<volatile uint32_t*>(&s_absent[g & 15u]) = gone;
+                        mbar_expect_tx(bar(C::FULL + n % C::kPairSlots), 2 * kLatentSlot);
+                    }
                     for (uint32_t i = 0; i < per_tile; ++i) {
                         const int32_t page = __shfl_sync(0xFFFFFFFFu, entry, first + i - from);
                         if (leader) {
@@ -552,18 +565,6 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                     }
                 }
                 if (!ok) break;
-                if (!rear) continue;
-                if (g >= C::kRopeSlots) ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(C::REMPTY + g % C::kRopeSlots), (g / C::kRopeSlots - 1u) & 1u, ctl, kCacheTimeout | C::REMPTY));
-                if (!ok) break;
-                asked = g + 1;
-                if (leader) {
-                    *reinterpret_cast<volatile uint32_t*>(&s_absent[g & 7u]) = gone;
-                    mbar_expect_tx(bar(C::RFULL + g % C::kRopeSlots), kLatentSlot);
-                }
-                for (uint32_t i = 0; i < per_tile; ++i) {
-                    const int32_t page = __shfl_sync(0xFFFFFFFFu, entry, first + i - from);
-                    if (leader) tma_load_3d(rope_addr(g) + i * box_bytes, &map, bar(C::RFULL + g % C::kRopeSlots), 64 * LC, static_cast<int32_t>(y), page);
-                }
                 __syncwarp();
             }
         }
@@ -594,7 +595,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                     // (whoever read the scores two tiles ago has given P)
                     if (g >= 2) wait(C::P + (g & 1u), ((g >> 1) - 1u) & 1u);
                     const uint32_t tS = tmem + C::kColS + N * (g & 1u);
-                    // (in two halves: the first goes on while the second's slots arrive)
+                    // In two halves: the first goes on while the second's slots arrive (32 sequences, 128 heads: 84 us, 88 in one, 90 slot by slot).
                     constexpr uint32_t kFront = (C::kPairs + 1) / 2;
 #pragma unroll
                     for (uint32_t half = 0; half < 2; ++half) {
@@ -604,14 +605,18 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                         tc_fence_after();
                         if (!leader || !ok) continue;
 #pragma unroll
-                        for (uint32_t c = 2 * c0; c < 2 * c1; ++c) {
-                            const uint64_t dk = make_smem_desc<128>(pair_addr(g * C::kPairs + c / 2) + (c & 1u) * kLatentSlot, 16), dq = make_smem_desc<128>(base + c * C::kQChunk, 16);
+                        for (uint32_t c = c0; c < c1; ++c) {
+                            const uint64_t dk = make_smem_desc<128>(pair_addr(g * C::kPairs + c), 16), dq = make_smem_desc<128>(base + c * (2 * C::kQChunk), 16);
 #pragma unroll
-                            for (uint32_t ks = 0; ks < 4; ++ks) mma_ss(tS, dk + 2 * ks, dq + 2 * ks, idesc_s, c + ks > 0 ? 1u : 0u);
+                            for (uint32_t ks = 0; ks < 8; ++ks)
+                                mma_ss(tS, dk + (ks >> 2) * (kLatentSlot >> 4) + 2 * (ks & 3u), dq + (ks >> 2) * (C::kQChunk >> 4) + 2 * (ks & 3u), idesc_s, c + ks > 0 ? 1u : 0u);
                         }
                         if (half == 0) continue;
                         const uint64_t dk = make_smem_desc<128>(rope_addr(g), 16), dq = make_smem_desc<128>(base + LC * C::kQChunk, 16);
                         for (uint32_t ks = 0; ks < rope_steps; ++ks) mma_ss(tS, dk + 2 * ks, dq + 2 * ks, idesc_s, 1u);
+                        tc_commit(bar(C::REMPTY + g % C::kRopeSlots));
+                    }
+                    if (leader && ok) {
                         tc_commit(bar(C::S + (g & 1u)));
                         if (tile + 1 == w.end) tc_commit(bar(C::QEMPTY));
                     }
@@ -629,7 +634,6 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                                 mma_ss(tmem + d * N, dc + ks * (2048 >> 4), dp + ks * (16 * C::kPitch >> 4), idesc_y, tile > w.t0 || ks > 0 ? 1u : 0u);
                             tc_commit(bar(C::EMPTY + n % C::kPairSlots));
                         }
-                        tc_commit(bar(C::REMPTY + g % C::kRopeSlots));   // (not with the scores: softmax looks at the tile and its barriers until here)
                         tc_commit(bar(C::PV + (g & 1u)));
                     }
                 }
