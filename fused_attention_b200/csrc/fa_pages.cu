@@ -10,7 +10,7 @@ bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0
 int pages_of(const fa_b200_pages* pages, fa::PagesView* v) {
     if (!pages || !pages->refs || !pages->status) return FA_B200_ERR_NULL_POINTER;
     if (!aligned4(pages->refs) || !aligned4(pages->status)) return FA_B200_ERR_ALIGNMENT;
-    if (pages->n_pages == 0 || pages->n_pages > 0x7FFFFFFEu) return FA_B200_ERR_SHAPE;
+    if (pages->n_pages == 0 || pages->n_pages >= (1u << 30)) return FA_B200_ERR_SHAPE;
     v->refs = pages->refs, v->status = pages->status, v->n = pages->n_pages;
     return FA_B200_OK;
 }
@@ -69,7 +69,8 @@ int fa_b200_pages_reserve(const fa_b200_pages* pages, int32_t* table, int64_t ta
     if ((rc = device_of(device, &d)) != FA_B200_OK) return rc;
     OnDevice on(device);
     if (on.rc != 0) return on.rc;
-    const uint32_t ctas = (B + fa::kReserveWarps - 1) / fa::kReserveWarps, sms = static_cast<uint32_t>(d->sms.load());
+    a.alone = B <= fa::kAloneRows && static_cast<uint64_t>(B) * table_width <= fa::kAloneEntries;
+    const uint32_t ctas = a.alone ? 1 : (B + fa::kReserveWarps - 1) / fa::kReserveWarps, sms = static_cast<uint32_t>(d->sms.load());
     return launch(&fa::fa_pages_reserve, ctas < sms ? ctas : sms, fa::kReserveThreads, 0, static_cast<cudaStream_t>(cuda_stream), a);
 }
 
@@ -122,7 +123,9 @@ int fa_b200_cache_copy(const fa_b200_copy_area* areas, uint32_t n_areas, uint32_
         fa::CopyArgs a = {};
         a.sources = sources, a.targets = targets, a.status = status, a.pairs = pairs, a.n = n_pages;
         a.areas = n_areas - first < fa::kCopyAreas ? n_areas - first : fa::kCopyAreas;
-        uint64_t page_bytes = 0;
+        // Eight CTAs an SM in all, if there are as many parts of 16 KB (half of what a CTA has in flight at once) and more.
+        const uint32_t ctas = 8 * sms, share = (ctas + pairs - 1) / pairs;
+        uint32_t parts = 0;
         for (uint32_t i = 0; i < a.areas; ++i) {
             const fa_b200_copy_area& x = areas[first + i];
             fa::CopyArea& y = a.area[i];
@@ -131,13 +134,12 @@ int fa_b200_cache_copy(const fa_b200_copy_area* areas, uint32_t n_areas, uint32_
             // in as few rows as it lies in
             if (y.n1 > 1 && y.stride1 == y.row && static_cast<uint64_t>(y.row) * y.n1 < (1u << 31)) y.row *= y.n1, y.n1 = 1;
             if (y.n0 > 1 && y.n1 == 1 && y.stride0 == y.row && static_cast<uint64_t>(y.row) * y.n0 < (1u << 31)) y.row *= y.n0, y.n0 = 1;
-            page_bytes += static_cast<uint64_t>(y.n0) * y.n1 * y.row;
+            const uint64_t most = static_cast<uint64_t>(y.n0) * y.n1 * y.row / 16384;
+            y.parts = static_cast<uint32_t>(most < 1 ? 1 : most < share ? most : share);
+            if (y.parts > 64) y.parts = 64;
+            parts += y.parts;
         }
-        // Eight CTAs an SM in all, a page in parts of 32 KB (what a CTA has in flight at once) or more.
-        const uint32_t ctas = 8 * sms, most = static_cast<uint32_t>(page_bytes / 32768 < 1 ? 1 : page_bytes / 32768 > 64 ? 64 : page_bytes / 32768);
-        uint32_t parts = ctas / (pairs < ctas ? pairs : ctas);
-        parts = parts < 1 ? 1 : parts > most ? most : parts;
-        const uint32_t x = pairs < ctas / parts ? pairs : ctas / parts;
+        const uint32_t most_x = (ctas + parts - 1) / parts, x = pairs < most_x ? pairs : most_x;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(x, parts, 1), cfg.blockDim = dim3(fa::kCopyThreads, 1, 1), cfg.stream = static_cast<cudaStream_t>(cuda_stream);
         cudaLaunchAttribute attr[1];

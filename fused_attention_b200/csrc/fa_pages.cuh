@@ -58,22 +58,26 @@ struct ForkArgs {
 };
 constexpr int kForkThreads = 256;
 __global__ void __launch_bounds__(kForkThreads) fa_pages_fork(const ForkArgs p) {
-    extern __shared__ int32_t s_old[];
+    extern __shared__ int32_t s_old[];   // [B, cols]
     grid_dep_wait();
     grid_dep_launch();
     const bool is_lengths = blockIdx.x == gridDim.x - 1;
     const uint32_t col0 = blockIdx.x * p.cols, cols = is_lengths ? 1u : min(p.cols, p.t.width - col0);
     int32_t* const base = is_lengths ? p.lengths : p.t.at + col0;
     const int64_t stride = is_lengths ? 1 : p.t.stride;
-    for (uint32_t i = threadIdx.x; i < p.t.B * cols; i += kForkThreads) s_old[i] = base[(i / cols) * stride + i % cols];
+    const uint32_t all = p.t.B * cols;
+    auto parent_of = [&](uint32_t b) {
+        const int32_t parent = p.parents[b];
+        if (parent >= -1 && parent < static_cast<int32_t>(p.t.B)) return parent;
+        if (is_lengths) cache_report(p.v.status, kCacheBadPosition);   // stays as it is
+        return static_cast<int32_t>(b);
+    };
+    const int32_t first = threadIdx.x < all ? p.parents[threadIdx.x / cols] : 0;   // (asked for with the entries)
+    for (uint32_t i = threadIdx.x; i < all; i += kForkThreads) s_old[i] = base[(i / cols) * stride + i % cols];
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < p.t.B * cols; i += kForkThreads) {
+    for (uint32_t i = threadIdx.x; i < all; i += kForkThreads) {
         const uint32_t b = i / cols, c = i % cols;
-        int32_t parent = p.parents[b];
-        if (parent < -1 || parent >= static_cast<int32_t>(p.t.B)) {   // stays as it is
-            if (is_lengths) cache_report(p.v.status, kCacheBadPosition);
-            parent = static_cast<int32_t>(b);
-        }
+        const int32_t parent = i < kForkThreads && first >= -1 && first < static_cast<int32_t>(p.t.B) ? first : parent_of(b);
         const int32_t before = s_old[i];
         int32_t now = parent < 0 ? (is_lengths ? 0 : -1) : s_old[static_cast<uint32_t>(parent) * cols + c];
         if (!is_lengths && now != -1 && !is_page(p.v, now)) {
@@ -89,16 +93,18 @@ __global__ void __launch_bounds__(kForkThreads) fa_pages_fork(const ForkArgs p) 
 }
 
 // ----------------------------------------------------------------------------- reserve
-// The first part, a warp a sequence: blocks behind those that are needed are let go of.  The last CTA to be through with that does the
-// rest, with `lanes` threads a sequence (as many as its tokens touch blocks, up to 32):
+// First, blocks behind those that are needed are let go of.  Where the table is small the one CTA that does the rest does that too;
+// otherwise CTAs take sequences, a warp each, and the last to be through goes on, with `lanes` threads a sequence (as many as its tokens
+// touch blocks, up to 32):
 //
-//   1  every entry that will be written to lets go of its page.  What is left of a page's count is the number of those that hold it and
-//      do not write to it
-//   2  where that is none all that hold the page write to it, and the lowest sequence keeps it: the count becomes minus (B - b) of the
+//   1  the free pages (count 0), in ascending order, as many as blocks are written to
+//   2  entries that are written to and whose page is held by others too let go of it.  What is left of a page's count is the number of
+//      those that hold it and do not write to it
+//   3  where that is none all that hold the page write to it, and the lowest sequence keeps it: the count becomes minus (B - b) of the
 //      lowest b, by a minimum
-//   3  an entry keeps its page if it finds its own number there; all others want one.  Their ranks, in order of sequences and blocks
-//   4  the free pages (count 0), in ascending order, as many as are wanted
-//   5  each takes the one of its rank; where there is none left, the entry stays as it was and its sequence is granted fewer tokens
+//   4  an entry keeps its page if it finds its own number there; the others want one.  (Without shared pages 2 to 4 are passed over)
+//   5  each takes the page of its rank, in order of sequences and blocks; where there is none left, the entry stays as it was and its
+//      sequence is granted fewer tokens
 struct ReserveArgs {
     PagesView v;
     PagesTable t;
@@ -108,7 +114,7 @@ struct ReserveArgs {
     int32_t* sources;        // [B]
     int32_t* targets;
     int32_t* list;           // [n]: free pages
-    uint32_t count, page_shift;
+    uint32_t count, page_shift, alone;   // alone: one CTA, which lets go of blocks as well
 };
 constexpr int kReserveThreads = 1024, kReserveWarps = kReserveThreads / 32;
 constexpr uint32_t kNoBlock = 0xFFFFFFFFu;
@@ -152,48 +158,96 @@ __device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t* s_warp, uin
     return __shfl_sync(0xFFFFFFFFu, sums - w, warp) + upto - x;
 }
 
+// Which of pages [q, q + 16) are free.
+__device__ __forceinline__ uint32_t free_of_16(const PagesView& v, uint32_t q) {
+    uint32_t free = 0;
+    if (q + 16 <= v.n && (reinterpret_cast<uintptr_t>(v.refs) & 15u) == 0) {
+        int4 x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = ld_cg(reinterpret_cast<const int4*>(v.refs + q) + k);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) free |= ((x[k].x == 0) | (x[k].y == 0) << 1 | (x[k].z == 0) << 2 | (x[k].w == 0) << 3) << (4 * k);
+    } else {
+        for (uint32_t k = 0; k < 16 && q + k < v.n; ++k) free |= static_cast<uint32_t>(ld_cg(v.refs + q + k) == 0) << k;
+    }
+    return free;
+}
+// A table of this many entries and sequences is gone over by one CTA, eight entries of a thread at a time.
+constexpr uint32_t kAloneEntries = 32768, kAloneRows = 2048;
+
 __global__ void __launch_bounds__(kReserveThreads) fa_pages_reserve(const ReserveArgs p) {
-    __shared__ uint32_t s_warp[32], s_most, s_last;
+    __shared__ uint32_t s_warp[32], s_most, s_last, s_need[kAloneRows];
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     if (tid == 0) s_most = 0;
     grid_dep_wait();
     grid_dep_launch();
-    for (uint32_t b = blockIdx.x * kReserveWarps + warp; b < p.t.B; b += gridDim.x * kReserveWarps) {
-        const Window w = reserve_window(p, b);
-        if (lane == 0 && !w.ok) cache_report(p.v.status, kCacheBadPosition);
-        int32_t* const row = p.t.at + b * p.t.stride;
-        for (uint32_t i = w.need + lane; i < p.t.width; i += 128) {   // four loads of a lane in flight
-            int32_t e[4];
+    uint32_t free = free_of_16(p.v, 16 * tid), most = 0, bound = 0;   // (asked for along with the lengths)
+    auto count_in = [&](const Window& w) {
+        most = max(most, w.need - w.first);
+        bound += w.need - w.first;
+    };
+    bool let = false;
+    if (p.alone) {
+        for (uint32_t b = tid; b < p.t.B; b += kReserveThreads) {
+            const Window w = reserve_window(p, b);
+            if (!w.ok) cache_report(p.v.status, kCacheBadPosition);
+            count_in(w);
+            s_need[b] = w.need;
+        }
+        __syncthreads();
+        const uint32_t entries = p.t.B * p.t.width;
+        for (uint32_t i = tid; i < entries; i += 8 * kReserveThreads) {
+            int32_t e[8];
+            int32_t* at[8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) e[k] = i + 32 * k < p.t.width ? row[i + 32 * k] : -1;
+            for (uint32_t k = 0; k < 8; ++k) {
+                const uint32_t j = i + k * kReserveThreads, b = j / p.t.width, c = j - b * p.t.width;
+                at[k] = p.t.at + b * p.t.stride + c;
+                e[k] = j < entries && c >= s_need[b] ? *at[k] : -1;
+            }
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+            for (uint32_t k = 0; k < 8; ++k)
                 if (e[k] != -1) {
                     let_go(p.v, e[k]);
-                    row[i + 32 * k] = -1;
+                    *at[k] = -1;
+                    let = true;
                 }
         }
+    } else {
+        for (uint32_t b = blockIdx.x * kReserveWarps + warp; b < p.t.B; b += gridDim.x * kReserveWarps) {
+            const Window w = reserve_window(p, b);
+            if (lane == 0 && !w.ok) cache_report(p.v.status, kCacheBadPosition);
+            int32_t* const row = p.t.at + b * p.t.stride;
+            for (uint32_t i = w.need + lane; i < p.t.width; i += 128) {   // four loads of a lane in flight
+                int32_t e[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) e[k] = i + 32 * k < p.t.width ? row[i + 32 * k] : -1;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (e[k] != -1) {
+                        let_go(p.v, e[k]);
+                        row[i + 32 * k] = -1;
+                    }
+            }
+        }
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+            const uint32_t through = atomicAdd(p.v.status + 2, 1u);
+            s_last = through == gridDim.x - 1;
+            if (s_last) p.v.status[2] = 0;
+        }
+        __syncthreads();
+        if (!s_last) return;
+        __threadfence();
+        let = true;
+        for (uint32_t b = tid; b < p.t.B; b += kReserveThreads) count_in(reserve_window(p, b));
     }
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) {
-        const uint32_t through = gridDim.x == 1 ? 0 : atomicAdd(p.v.status + 2, 1u);
-        s_last = through == gridDim.x - 1;
-        if (s_last && gridDim.x > 1) p.v.status[2] = 0;
-    }
-    __syncthreads();
-    if (!s_last) return;
-    __threadfence();
 
     // how many blocks a sequence's tokens touch at most decides how many threads it gets
-    uint32_t most = 0;
-    for (uint32_t b = tid; b < p.t.B; b += kReserveThreads) {
-        const Window w = reserve_window(p, b);
-        most = max(most, w.need - w.first);
-    }
     most = __reduce_max_sync(0xFFFFFFFFu, most);
     if (lane == 0) atomicMax(&s_most, most);
-    __syncthreads();
+    if (__syncthreads_or(let)) free = free_of_16(p.v, 16 * tid);
     most = s_most;
     uint32_t shift = 0;
     while (shift < 5 && (1u << shift) < most) ++shift;
@@ -206,31 +260,20 @@ __global__ void __launch_bounds__(kReserveThreads) fa_pages_reserve(const Reserv
         w = reserve_window(p, b);
         i0 = min(w.need, w.first + l * per), i1 = min(w.need, i0 + per);
     };
-    for (int step = 1; step <= 2; ++step) {
-        for (uint32_t b0 = 0; b0 < p.t.B; b0 += at_once) {
-            const uint32_t b = b0 + mine;
-            Window w;
-            uint32_t i0, i1;
-            blocks(b, w, i0, i1);
-            for (uint32_t i = i0; i < i1; ++i) {
-                int32_t* const entry = p.t.at + b * p.t.stride + i;
-                const int32_t e = *entry;
-                if (!is_page(p.v, e)) {
-                    if (step == 1 && e != -1) {
-                        cache_report(p.v.status, kCacheBadPage);
-                        *entry = -1;
-                    }
-                } else if (step == 1) {
-                    if (atomicSub(p.v.refs + e, 1) <= 0) cache_report(p.v.status, kPagesCount);
-                } else if (ld_cg(p.v.refs + e) <= 0) {
-                    atomicMin(p.v.refs + e, -static_cast<int32_t>(p.t.B - b));
-                }
-            }
-        }
-        __syncthreads();
+    // 1: 16 of a thread at a time
+    uint32_t all_bound, found = 0;
+    (void)sum_before(bound, s_warp, all_bound);
+    for (uint32_t q0 = 0; q0 < p.v.n && found < all_bound; q0 += 16 * kReserveThreads) {
+        const uint32_t q = q0 + 16 * tid;
+        if (q0 > 0) free = free_of_16(p.v, q);
+        uint32_t all, at = found + sum_before(__popc(free), s_warp, all);
+        for (; free != 0 && at < all_bound; free &= free - 1u) p.list[at++] = static_cast<int32_t>(q + __ffs(free) - 1);   // (`at` stays below n)
+        found += all;
     }
-    // 3: what is kept is marked in the table (as -2 - page), nobody else looks there; how many pages are wanted
+    // 2 to 4; what is kept is marked in the table, where nobody else looks: -2 - page if it was held alone, -2 - n - page if it is the lowest
+    // sequence's (n is below 2^30).  How many pages are wanted
     uint32_t wanted = 0;
+    bool shared = false;
     for (uint32_t b0 = 0; b0 < p.t.B; b0 += at_once) {
         const uint32_t b = b0 + mine;
         Window w;
@@ -239,33 +282,45 @@ __global__ void __launch_bounds__(kReserveThreads) fa_pages_reserve(const Reserv
         for (uint32_t i = i0; i < i1; ++i) {
             int32_t* const entry = p.t.at + b * p.t.stride + i;
             const int32_t e = *entry;
-            if (is_page(p.v, e) && ld_cg(p.v.refs + e) == -static_cast<int32_t>(p.t.B - b)) *entry = -2 - e;
-            else ++wanted;
+            if (!is_page(p.v, e)) {
+                if (e != -1) {
+                    cache_report(p.v.status, kCacheBadPage);
+                    *entry = -1;
+                }
+                ++wanted;
+            } else {
+                const int32_t holders = ld_cg(p.v.refs + e);
+                if (holders > 1) shared = true;
+                else *entry = -2 - e;
+                if (holders < 1) cache_report(p.v.status, kPagesCount);
+            }
+        }
+    }
+    if (__syncthreads_or(shared)) {
+        for (int step = 2; step <= 4; ++step) {
+            for (uint32_t b0 = 0; b0 < p.t.B; b0 += at_once) {
+                const uint32_t b = b0 + mine;
+                Window w;
+                uint32_t i0, i1;
+                blocks(b, w, i0, i1);
+                for (uint32_t i = i0; i < i1; ++i) {
+                    int32_t* const entry = p.t.at + b * p.t.stride + i;
+                    const int32_t e = *entry, own = -static_cast<int32_t>(p.t.B - b);
+                    if (e < 0) continue;   // wanted, or kept already
+                    if (step == 2) atomicSub(p.v.refs + e, 1);
+                    else if (step == 3 && ld_cg(p.v.refs + e) <= 0) atomicMin(p.v.refs + e, own);
+                    else if (step == 4) {
+                        if (ld_cg(p.v.refs + e) == own) *entry = -2 - static_cast<int32_t>(p.v.n) - e;
+                        else ++wanted;
+                    }
+                }
+            }
+            __syncthreads();
         }
     }
     uint32_t demand;
     (void)sum_before(wanted, s_warp, demand);
-    // 4: free pages, 16 of a thread at a time
-    uint32_t found = 0;
-    for (uint32_t q0 = 0; q0 < p.v.n && found < demand; q0 += 16 * kReserveThreads) {
-        const uint32_t q = q0 + 16 * tid;
-        uint32_t free = 0;
-        if (q + 16 <= p.v.n && (reinterpret_cast<uintptr_t>(p.v.refs) & 15u) == 0) {
-            int4 x[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = ld_cg(reinterpret_cast<const int4*>(p.v.refs + q) + k);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                free |= ((x[k].x == 0) | (x[k].y == 0) << 1 | (x[k].z == 0) << 2 | (x[k].w == 0) << 3) << (4 * k);
-        } else {
-            for (uint32_t k = 0; k < 16 && q + k < p.v.n; ++k) free |= static_cast<uint32_t>(ld_cg(p.v.refs + q + k) == 0) << k;
-        }
-        uint32_t all, at = found + sum_before(__popc(free), s_warp, all);
-        for (; free != 0 && at < demand; free &= free - 1u) p.list[at++] = static_cast<int32_t>(q + __ffs(free) - 1);   // (demand may exceed n, `at` not)
-        found += all;
-    }
     const uint32_t there = min(found, demand);
-    __syncthreads();   // (the list, by this CTA alone: visible to it)
     // 5
     uint32_t in_front = 0;
     for (uint32_t b0 = 0; b0 < p.t.B; b0 += at_once) {
@@ -280,9 +335,14 @@ __global__ void __launch_bounds__(kReserveThreads) fa_pages_reserve(const Reserv
         for (uint32_t i = i0; i < i1; ++i) {
             int32_t* const entry = p.t.at + b * p.t.stride + i;
             const int32_t e = *entry;
-            if (e < -1) {   // kept: from the sequence's number to one, whatever refused entries have added
-                *entry = -2 - e;
-                atomicAdd(p.v.refs + (-2 - e), static_cast<int32_t>(p.t.B - b) + 1);
+            if (e < -1) {   // kept
+                const int32_t page = -2 - e, n_pages = static_cast<int32_t>(p.v.n);
+                if (page < n_pages) {
+                    *entry = page;
+                } else {   // the count goes from the sequence's number to one, whatever refused entries have added
+                    *entry = page - n_pages;
+                    atomicAdd(p.v.refs + (page - n_pages), static_cast<int32_t>(p.t.B - b) + 1);
+                }
                 continue;
             }
             if (rank < there) {
@@ -326,19 +386,22 @@ __global__ void __launch_bounds__(kCompactThreads) fa_pages_plan(const CompactAr
     const uint32_t tid = threadIdx.x, n = p.v.n, base = blockIdx.x * kCompactPages;
     grid_dep_wait();
     grid_dep_launch();
-    uint32_t front = 0, rest = 0;   // used pages in front of this CTA's, and the others
-    for (uint32_t q = tid; q < n; q += kCompactThreads) {
-        const uint32_t used = p.v.refs[q] > 0;
-        if (q < base) front += used;
-        else rest += used;
-    }
-    uint32_t used_front, used_rest;
-    (void)sum_before(front, s_warp, used_front);
-    (void)sum_before(rest, s_warp, used_rest);
-    const uint32_t n_used = used_front + used_rest;
-    uint32_t low = 0, low_used;
-    for (uint32_t q = tid; q < n_used; q += kCompactThreads) low += p.v.refs[q] > 0;
-    (void)sum_before(low, s_warp, low_used);
+    // used pages among [0, end) and how many of them are in front of `cut`; eight of a thread in flight
+    auto count = [&](uint32_t end, uint32_t cut, uint32_t& front, uint32_t& all) {
+        uint32_t x = 0, y = 0;
+        for (uint32_t q = tid; q < end; q += 8 * kCompactThreads) {
+            int32_t r[8];
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) r[k] = q + k * kCompactThreads < end ? p.v.refs[q + k * kCompactThreads] : 0;
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) x += r[k] > 0 && q + k * kCompactThreads < cut, y += r[k] > 0;
+        }
+        (void)sum_before(x, s_warp, front);
+        (void)sum_before(y, s_warp, all);
+    };
+    uint32_t used_front, n_used, low_used, same;
+    count(n, base, used_front, n_used);
+    count(n_used, 0, same, low_used);
     const uint32_t moves = n_used - low_used;
     if (blockIdx.x == 0 && tid == 0) p.totals[0] = n_used, p.totals[1] = moves;
     int32_t r[4];
@@ -390,11 +453,12 @@ __global__ void __launch_bounds__(256) fa_pages_renumber(const CompactArgs p) {
 
 // ----------------------------------------------------------------------------- copy
 // Contents of pages, source to target, for up to kCopyAreas arrays: a page of an array is n0 x n1 rows of `row` bytes (one row where it
-// lies in one piece).  CTA (x, y) has the pairs x, x + gridDim.x, ... and of each page the y-th of gridDim.y equal parts.
+// lies in one piece).  CTAs are dealt out by parts of a page, `parts` equal ones of each array, first: CTA (x, y) has part y of the pairs x,
+// x + gridDim.x, ...  Every thread has eight pieces of 16 bytes in flight.
 struct CopyArea {
     uint8_t* base;
     int64_t page, stride0, stride1;   // bytes
-    uint32_t n0, n1, row;             // row: a multiple of 16, or of 4
+    uint32_t n0, n1, row, parts;      // row: a multiple of 16, or of 4
 };
 constexpr int kCopyAreas = 32;
 struct CopyArgs {
@@ -405,48 +469,59 @@ struct CopyArgs {
     uint32_t areas, pairs, n;   // n: pages of every array
 };
 constexpr int kCopyThreads = 256;
-constexpr int kCopyFlight = 8;   // loads of a thread in flight
+constexpr int kCopyFlight = 8;
 
 template <typename Piece>
-__device__ __forceinline__ void copy_part(const CopyArea& a, uint32_t source, uint32_t target, uint32_t part, uint32_t parts) {
+__device__ __forceinline__ void copy_part(const CopyArea& a, uint32_t source, uint32_t target, uint32_t part) {
     const uint32_t in_row = a.row / sizeof(Piece);
-    const uint64_t pieces = static_cast<uint64_t>(a.n0) * a.n1 * in_row, end = pieces * (part + 1) / parts;
+    const uint64_t pieces = static_cast<uint64_t>(a.n0) * a.n1 * in_row, begin = pieces * part / a.parts, end = pieces * (part + 1) / a.parts;
     const uint8_t* const from = a.base + source * a.page;
     uint8_t* const to = a.base + target * a.page;
-    auto place = [&](uint64_t i) -> int64_t {
-        if (a.n0 * a.n1 == 1) return static_cast<int64_t>(i * sizeof(Piece));
+    if (a.n0 * a.n1 == 1) {
+        for (uint64_t i = begin + threadIdx.x; i < end; i += kCopyThreads * kCopyFlight) {
+            Piece x[kCopyFlight];
+#pragma unroll
+            for (int k = 0; k < kCopyFlight; ++k)
+                if (i + k * kCopyThreads < end) x[k] = reinterpret_cast<const Piece*>(from)[i + k * kCopyThreads];
+#pragma unroll
+            for (int k = 0; k < kCopyFlight; ++k)
+                if (i + k * kCopyThreads < end) reinterpret_cast<Piece*>(to)[i + k * kCopyThreads] = x[k];
+        }
+        return;
+    }
+    auto place = [&](uint64_t i) {
         const uint32_t r = static_cast<uint32_t>(i / in_row), c = static_cast<uint32_t>(i - static_cast<uint64_t>(r) * in_row), r0 = r / a.n1;
         return r0 * a.stride0 + (r - r0 * a.n1) * a.stride1 + static_cast<int64_t>(c * sizeof(Piece));
     };
-    for (uint64_t i = pieces * part / parts + threadIdx.x; i < end; i += kCopyThreads * kCopyFlight) {
-        Piece x[kCopyFlight];
-        int64_t at[kCopyFlight];
+    for (uint64_t i = begin + threadIdx.x; i < end; i += kCopyThreads * 4) {
+        Piece x[4];
 #pragma unroll
-        for (int k = 0; k < kCopyFlight; ++k)
-            if (i + k * kCopyThreads < end) x[k] = *reinterpret_cast<const Piece*>(from + (at[k] = place(i + k * kCopyThreads)));
+        for (int k = 0; k < 4; ++k)
+            if (i + k * kCopyThreads < end) x[k] = *reinterpret_cast<const Piece*>(from + place(i + k * kCopyThreads));
 #pragma unroll
-        for (int k = 0; k < kCopyFlight; ++k)
-            if (i + k * kCopyThreads < end) *reinterpret_cast<Piece*>(to + at[k]) = x[k];
+        for (int k = 0; k < 4; ++k)
+            if (i + k * kCopyThreads < end) *reinterpret_cast<Piece*>(to + place(i + k * kCopyThreads)) = x[k];
     }
 }
 
-__global__ void __launch_bounds__(kCopyThreads) fa_cache_copy(const __grid_constant__ CopyArgs p) {
+__global__ void __launch_bounds__(kCopyThreads, 3) fa_cache_copy(const __grid_constant__ CopyArgs p) {
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t k = 0, part = blockIdx.y;
+    while (part >= p.area[k].parts) part -= p.area[k++].parts;   // (gridDim.y is their sum)
+    const CopyArea& a = p.area[k];
     grid_dep_wait();
     grid_dep_launch();
-    const uint32_t lane = threadIdx.x & 31u;
     for (uint64_t i0 = blockIdx.x; i0 < p.pairs; i0 += 32ull * gridDim.x) {   // every warp looks at 32 of the CTA's pairs
         const uint64_t i = i0 + static_cast<uint64_t>(lane) * gridDim.x;
         const int32_t s = i < p.pairs ? p.sources[i] : -1, t = i < p.pairs ? p.targets[i] : -1;
         const bool good = static_cast<uint32_t>(s) < p.n && static_cast<uint32_t>(t) < p.n;
-        if (!good && (s != -1 || t != -1) && i < p.pairs && threadIdx.x < 32 && blockIdx.y == 0) cache_report(p.status, kCacheBadPage);
+        if (!good && ((s != -1 && static_cast<uint32_t>(s) >= p.n) || (t != -1 && static_cast<uint32_t>(t) >= p.n)) && threadIdx.x < 32 && blockIdx.y == 0)
+            cache_report(p.status, kCacheBadPage);
         for (uint32_t left = __ballot_sync(0xFFFFFFFFu, good && s != t); left != 0; left &= left - 1u) {
-            const int l = __ffs(left) - 1;
-            const uint32_t source = static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, s, l)), target = static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, t, l));
-            for (uint32_t k = 0; k < p.areas; ++k) {
-                const CopyArea& a = p.area[k];
-                if ((a.row & 15u) == 0) copy_part<uint4>(a, source, target, blockIdx.y, gridDim.y);
-                else copy_part<uint32_t>(a, source, target, blockIdx.y, gridDim.y);
-            }
+            const int from = __ffs(left) - 1;
+            const uint32_t source = static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, s, from)), target = static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, t, from));
+            if ((a.row & 15u) == 0) copy_part<uint4>(a, source, target, part);
+            else copy_part<uint32_t>(a, source, target, part);
         }
     }
 }

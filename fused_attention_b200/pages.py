@@ -62,7 +62,7 @@ class PagePool:
     def __init__(self, refs: torch.Tensor, _status: Optional[torch.Tensor] = None):
         _require(isinstance(refs, torch.Tensor) and refs.dtype == torch.int32, "refs must be an int32 tensor")
         _require(refs.is_cuda, "refs must be a CUDA tensor")
-        _require(refs.dim() == 1 and 0 < refs.shape[0] < 0x7FFFFFFF and refs.is_contiguous(), "refs must be contiguous, of shape [n_pages]")
+        _require(refs.dim() == 1 and 0 < refs.shape[0] < 1 << 30 and refs.is_contiguous(), "refs must be contiguous, of shape [n_pages]")
         self.refs, self.n_pages, self.device, self._index = refs, refs.shape[0], refs.device, refs.get_device()
         self._status = torch.zeros(4, dtype=torch.int32, device=refs.device) if _status is None else _status
         self._handle = _lib.Pages(refs.data_ptr(), self._status.data_ptr(), self.n_pages)
@@ -78,7 +78,7 @@ class PagePool:
 
 def page_pool_create(n_pages: int, device="cuda") -> PagePool:
     """A pool whose pages are all free."""
-    _require(0 < n_pages < 0x7FFFFFFF, "n_pages must be positive and below 2^31 - 1")
+    _require(0 < n_pages < 1 << 30, "n_pages must be positive and below 2^30")
     return PagePool(torch.zeros(n_pages, dtype=torch.int32, device=device))
 
 
