@@ -177,6 +177,7 @@ constexpr uint32_t kAloneEntries = 32768, kAloneRows = 2048;
 
 __global__ void __launch_bounds__(kReserveThreads) fa_pages_reserve(const ReserveArgs p) {
     __shared__ uint32_t s_warp[32], s_most, s_last, s_need[kAloneRows];
+    __shared__ int32_t s_list[kReserveThreads];
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     if (tid == 0) s_most = 0;
     grid_dep_wait();
@@ -260,6 +261,20 @@ __global__ void __launch_bounds__(kReserveThreads) fa_pages_reserve(const Reserv
         w = reserve_window(p, b);
         i0 = min(w.need, w.first + l * per), i1 = min(w.need, i0 + per);
     };
+    // Where no sequence's tokens touch more than a block for each of its threads, and all are at hand at once, entries stay in registers
+    // and the free pages in shared memory: the calls between two tokens of a decoder.
+    const bool at_hand = per <= 1 && p.t.B <= at_once;
+    Window own_w = {};
+    uint32_t own_i = 0;
+    bool writes = false;
+    int32_t own_e = -1;
+    if (at_hand && mine < p.t.B) {
+        own_w = reserve_window(p, mine);
+        own_i = own_w.first + l;
+        writes = own_i < own_w.need;
+        if (writes) own_e = p.t.at[mine * p.t.stride + own_i];
+    }
+    int32_t* const list = at_hand ? s_list : p.list;
     // 1: 16 of a thread at a time
     uint32_t all_bound, found = 0;
     (void)sum_before(bound, s_warp, all_bound);
@@ -267,8 +282,61 @@ __global__ void __launch_bounds__(kReserveThreads) fa_pages_reserve(const Reserv
         const uint32_t q = q0 + 16 * tid;
         if (q0 > 0) free = free_of_16(p.v, q);
         uint32_t all, at = found + sum_before(__popc(free), s_warp, all);
-        for (; free != 0 && at < all_bound; free &= free - 1u) p.list[at++] = static_cast<int32_t>(q + __ffs(free) - 1);   // (`at` stays below n)
+        for (; free != 0 && at < all_bound; free &= free - 1u) list[at++] = static_cast<int32_t>(q + __ffs(free) - 1);   // (`at` stays below n)
         found += all;
+    }
+    if (at_hand) {
+        bool is_shared = false, keeps = false;
+        if (writes && own_e != -1) {
+            if (!is_page(p.v, own_e)) {
+                cache_report(p.v.status, kCacheBadPage);
+                own_e = -1;
+            } else {
+                const int32_t holders = ld_cg(p.v.refs + own_e);
+                is_shared = holders > 1, keeps = !is_shared;
+                if (holders < 1) cache_report(p.v.status, kPagesCount);
+            }
+        }
+        if (__syncthreads_or(is_shared)) {
+            const int32_t own = -static_cast<int32_t>(p.t.B - mine);
+            if (is_shared) atomicSub(p.v.refs + own_e, 1);
+            __syncthreads();
+            const bool all_write = is_shared && ld_cg(p.v.refs + own_e) <= 0;
+            if (all_write) atomicMin(p.v.refs + own_e, own);
+            __syncthreads();
+            if (all_write && ld_cg(p.v.refs + own_e) == own) {
+                keeps = true;
+                is_shared = false;
+            }
+            __syncthreads();   // everyone has looked
+            if (keeps && all_write) atomicAdd(p.v.refs + own_e, 1 - own);   // from the sequence's number to one, whatever refused entries add
+        }
+        uint32_t demand;
+        const uint32_t rank = sum_before(writes && !keeps, s_warp, demand), there = min(found, demand);
+        uint32_t refused = kNoBlock;
+        int32_t source = -1, target = -1;
+        if (writes && !keeps) {
+            int32_t* const entry = p.t.at + mine * p.t.stride + own_i;
+            if (rank < there) {
+                const int32_t page = s_list[rank];
+                *entry = page;
+                p.v.refs[page] = 1;
+                if (own_e >= 0 && l == 0 && (own_w.held & ((1u << p.page_shift) - 1u)) != 0) source = own_e, target = page;
+            } else {
+                if (own_e >= 0) atomicAdd(p.v.refs + own_e, 1);
+                else *entry = -1;
+                refused = own_i;
+                cache_report(p.v.status, kPagesNone);
+            }
+        }
+        for (uint32_t d = lanes >> 1; d >= 1; d >>= 1) refused = min(refused, __shfl_xor_sync(0xFFFFFFFFu, refused, d));
+        if (mine < p.t.B && l == 0) {
+            const uint32_t room = refused == kNoBlock ? own_w.count : max(refused << p.page_shift, own_w.held) - own_w.held;
+            p.granted[mine] = static_cast<int32_t>(min(own_w.count, room));
+            p.sources[mine] = source;
+            p.targets[mine] = target;
+        }
+        return;
     }
     // 2 to 4; what is kept is marked in the table, where nobody else looks: -2 - page if it was held alone, -2 - n - page if it is the lowest
     // sequence's (n is below 2^30).  How many pages are wanted
