@@ -5,14 +5,17 @@
 // A CTA has 256 query rows (two tiles of 128) of one sequence and head, and goes over the keys that the last of them sees in steps of 128,
 // as fa_cache_prompt.cuh does: scores in tensor memory, a softmax thread a row, P (16 bits) into tensor memory, Y in tensor memory.  The
 // score's contraction has NOPE + rope dimensions, the last chunk of 64 of which is the rotary part, fetched from the tensor that all heads
-// share.  Operands come by TMA in chunks of 128 rows by 64 dimensions into a ring: a step's key chunks, then its value chunks.  384 threads:
+// share.  Operands come by TMA in chunks of 128 rows by 64 dimensions into two rings, of
+// keys and of values.  384 threads:
 //
 //   warps 0-3, 4-7   softmax of query tile 0 / 1, a thread a row
-//   warp 8           fetches queries and the ring's chunks
+//   warp 8           fetches queries and keys
 //   warp 9, 10       issue Q K^T, P V
-//   warp 11          goes over the values of steps that some row sees in part only: keys behind the last that any row sees become zeros, and
-//                    so do keys that hold an infinity or a NaN, whose weights become NaN for the rows that see them.  0 * NaN reaches nobody
+//   warp 11          fetches values, and goes over those of steps that some row sees in part only: keys behind the last that any row sees become
+//                    zeros, and so do keys that hold an infinity or a NaN, whose weights become NaN for the rows that see them.  0 * NaN
+//                    reaches nobody
 //
+// (In one ring, values of a step come to stand in the way of keys two steps later: 4030 clocks a step instead of KSTEP, at NOPE = 128.)
 // At NOPE = 128 both tiles' scores take turns on one 128-column buffer (tensor memory: 128 + 2 * 64 of P + 2 * 128 of Y), which the other
 // tile's P V covers; at 64 each has its own.  Items with the most keys go first.
 #pragma once
@@ -41,14 +44,16 @@ struct ExpandArgs {
 template <int NOPE>
 struct ExpandCfg {
     static constexpr int kNope = NOPE / 64, kKey = kNope + 1;             // chunks of keys' own part, of keys
-    static constexpr int kSlots = 8, kStep = kKey + kNope;                // of the ring; chunks of a step
+    // Steps in the rings: what shared memory has room for, keys first (they come to be used in one go).  A barrier a step and not a chunk: a
+    // wait that stands behind MMAs and commits costs the issuing warps 280 clocks.
+    static constexpr int kKSlots = kNope == 2 ? 2 : 3, kVSlots = kNope == 2 ? 1 : 4;
     static constexpr bool kSharedS = NOPE == 128;
     static constexpr uint32_t kColS0 = 0, kColS1 = kSharedS ? 0 : 128, kColP0 = kSharedS ? 128 : 256, kColP1 = kColP0 + 64, kColO0 = kColP1 + 64,
                               kColO1 = kColO0 + NOPE;
     static_assert(kColO1 + NOPE <= 512, "tensor memory");
-    static constexpr uint32_t kOffRing = 2 * kKey * kExpandChunk, kTiles = kOffRing + kSlots * kExpandChunk;
+    static constexpr uint32_t kOffK = 2 * kKey * kExpandChunk, kOffV = kOffK + kKSlots * kKey * kExpandChunk, kTiles = kOffV + kVSlots * kNope * kExpandChunk;
     static constexpr int kSmemBytes = kTiles + 1024;
-    static constexpr int QFULL = 0, FULL = 1, EMPTY = FULL + kSlots, S = EMPTY + kSlots, SFREE = S + 2, P = SFREE + 2, PV = P + 2, BAD = PV + 2, FINAL = BAD + 4,
+    static constexpr int QFULL = 0, KFULL = 1, KEMPTY = KFULL + kKSlots, VFULL = KEMPTY + kKSlots, VEMPTY = VFULL + kVSlots, S = VEMPTY + kVSlots, SFREE = S + 2, P = SFREE + 2, PV = P + 2, BAD = PV + 2, FINAL = BAD + 4,
                          kBarriers = FINAL + 2;
     // 168 registers a thread at launch, so twice the softmax warps' and the others' are 504 at most
     static constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
@@ -87,12 +92,13 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t bar0 = smem_u32(bars);
     auto bar = [&](int i) { return bar0 + 8u * i; };
-    auto slot_addr = [&](uint32_t n) { return base + C::kOffRing + (n % C::kSlots) * kExpandChunk; };
+    auto k_addr = [&](uint32_t j, uint32_t c) { return base + C::kOffK + ((j % C::kKSlots) * C::kKey + c) * kExpandChunk; };
+    auto v_addr = [&](uint32_t j, uint32_t c) { return base + C::kOffV + ((j % C::kVSlots) * C::kNope + c) * kExpandChunk; };
     const WaitCtl ctl{g_latent_status, &abort_flag, kWaitCapCycles, nullptr, 0};
     const bool bf16 = p.bf16 != 0;
 
     if (tid == 0) {
-        for (int i = 0; i < C::kBarriers; ++i) mbar_init(bar(i), i >= C::SFREE && i < C::PV ? 4u : i >= C::EMPTY && i < C::S ? 2u : 1u);
+        for (int i = 0; i < C::kBarriers; ++i) mbar_init(bar(i), i >= C::SFREE && i < C::PV ? 4u : 1u);
         abort_flag = 0;
         fence_mbar_init();
         prefetch_tensormap(&map_q), prefetch_tensormap(&map_qr), prefetch_tensormap(&map_kv), prefetch_tensormap(&map_r);
@@ -262,82 +268,76 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
     } else {
         setmaxnreg_dec<C::kOtherRegs>();
         if (warp == 8) {
-            // ------------------------------------------------------------ operands
+            // ------------------------------------------------------------ queries, keys: a head's own part, the rotary part
             const bool leader = elect_one();
             bool ok = true;
-            uint32_t n = 0;
+            uint32_t n = 0;   // steps asked for
             if (all > 0 && leader) {
                 mbar_expect_tx(bar(C::QFULL), 2 * C::kKey * kExpandChunk);
                 for (uint32_t i = 0; i < 2; ++i)
                     for (uint32_t c = 0; c < C::kKey; ++c)
                         tma_load_4d(base + (i * C::kKey + c) * kExpandChunk, c < C::kNope ? &map_q : &map_qr, bar(C::QFULL), c < C::kNope ? 64 * c : 0, head, row0 + i * kExpandTile, b);
             }
-            for (uint32_t j = 0; ok && j < all; ++j) {
-                for (uint32_t c = 0; c < C::kStep; ++c, ++n) {
-                    if (n >= C::kSlots) ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(C::EMPTY + n % C::kSlots), (n / C::kSlots - 1u) & 1u, ctl, kCacheTimeout | (C::EMPTY + n % C::kSlots)));
-                    if (!ok) break;
-                    if (leader) {
-                        const uint32_t full = bar(C::FULL + n % C::kSlots);
-                        mbar_expect_tx(full, kExpandChunk);
-                        // the head's keys, the rotary keys, the head's values
-                        if (c == C::kNope) tma_load_4d(slot_addr(n), &map_r, full, 0, 0, j * kExpandTile, b);
-                        else tma_load_4d(slot_addr(n), &map_kv, full, 64 * (c < C::kNope ? c : c - 1u), head, j * kExpandTile, b);
-                    }
-                    __syncwarp();
+            for (; n < all; ++n) {
+                if (n >= C::kKSlots) ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(C::KEMPTY + n % C::kKSlots), (n / C::kKSlots - 1u) & 1u, ctl, kCacheTimeout | C::KEMPTY));
+                if (!ok) break;
+                if (leader) {
+                    const uint32_t full = bar(C::KFULL + n % C::kKSlots);
+                    mbar_expect_tx(full, C::kKey * kExpandChunk);
+                    for (uint32_t c = 0; c < C::kNope; ++c) tma_load_4d(k_addr(n, c), &map_kv, full, 64 * c, head, n * kExpandTile, b);
+                    tma_load_4d(k_addr(n, C::kNope), &map_r, full, 0, 0, n * kExpandTile, b);
                 }
+                __syncwarp();
             }
             // What was asked for lands before the CTA ends: the MMAs have waited for it, unless a wait gave up.
             if (*ctl.abort_flag != 0u) {
                 if (all > 0) mbar_wait_certain(bar(C::QFULL), 0, ctl, kCacheTimeout | C::QFULL);
-                for (uint32_t i = 0; i < C::kSlots; ++i) {
-                    const uint32_t uses = (n + C::kSlots - 1u - i) / C::kSlots;
-                    if (uses > 0) mbar_wait_certain(bar(C::FULL + i), (uses - 1u) & 1u, ctl, kCacheTimeout | C::FULL);
-                }
+                for (uint32_t x = n > C::kKSlots ? n - C::kKSlots : 0; x < n; ++x) mbar_wait_certain(bar(C::KFULL + x % C::kKSlots), (x / C::kKSlots) & 1u, ctl, kCacheTimeout | C::KFULL);
             }
         } else if (warp == 11) {
-            // ------------------------------------------------------------ values of steps that are seen in part
-            // A chunk's place is let go of by this warp too, so that no phase of its barriers passes unseen here.
-            auto arrived = [&](uint32_t at) { mbar_wait(bar(C::FULL + at % C::kSlots), (at / C::kSlots) & 1u, ctl, kCacheTimeout | (C::FULL + at % C::kSlots)); };
-            auto let_go = [&](uint32_t at) {
-                if (lane == 0) mbar_arrive(bar(C::EMPTY + at % C::kSlots));
-            };
-            for (uint32_t at = 0; at < all * C::kStep; ++at) {
-                const uint32_t j = at / C::kStep;
-                if (j >= partly && at % C::kStep == C::kKey) break;
-                arrived(at);
-                let_go(at);
-            }
-            for (uint32_t j = partly; j < all; ++j) {
-                const uint32_t n = j - partly, key0 = j * kExpandTile;
-                if (j > partly)
-                    for (uint32_t c = 0; c < C::kKey; ++c) arrived(j * C::kStep + c), let_go(j * C::kStep + c);
+            // ------------------------------------------------------------ values
+            const bool leader = elect_one();
+            bool ok = true;
+            uint32_t n = 0;   // steps asked for
+            for (; n < all; ++n) {
+                const uint32_t j = n;
+                if (n >= C::kVSlots) ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(C::VEMPTY + n % C::kVSlots), (n / C::kVSlots - 1u) & 1u, ctl, kCacheTimeout | C::VEMPTY));
+                if (!ok) break;
+                if (leader) {
+                    const uint32_t full = bar(C::VFULL + n % C::kVSlots);
+                    mbar_expect_tx(full, C::kNope * kExpandChunk);
+                    for (uint32_t c = 0; c < C::kNope; ++c) tma_load_4d(v_addr(n, c), &map_kv, full, NOPE + 64 * c, head, n * kExpandTile, b);
+                }
+                __syncwarp();
+                if (j < partly) continue;
+                // a step that some row sees in part
+                const uint32_t nth = j - partly, key0 = j * kExpandTile;
                 uint32_t bad[4] = {0, 0, 0, 0};   // this lane's keys: lane + 32 k
-                for (uint32_t c = 0; c < C::kNope; ++c) {
-                    const uint32_t at = j * C::kStep + C::kKey + c;
-                    arrived(at);
+                mbar_wait(bar(C::VFULL + j % C::kVSlots), (j / C::kVSlots) & 1u, ctl, kCacheTimeout | C::VFULL);
+                for (uint32_t c = 0; c < C::kNope; ++c)
                     for (uint32_t k = 0; k < 4; ++k) {
                         const uint32_t key = lane + 32 * k;
                         if (key0 + key < least || key0 + key >= farthest) continue;
                         for (uint32_t q = 0; q < 8; ++q) {
                             uint32_t x[4];
-                            ld_shared_v4(slot_addr(at) + key * 128 + ((q ^ (key & 7u)) << 4), x);
+                            ld_shared_v4(v_addr(j, c) + key * 128 + ((q ^ (key & 7u)) << 4), x);
                             bad[k] |= not_finite(x, bf16);
                         }
                     }
-                }
                 for (uint32_t k = 0; k < 4; ++k) {
                     const uint32_t key = lane + 32 * k;
                     if (bad[k] || key0 + key >= farthest)
                         for (uint32_t c = 0; c < C::kNope; ++c)
-                            for (uint32_t q = 0; q < 8; ++q) st_shared_v4(slot_addr(j * C::kStep + C::kKey + c) + key * 128 + (q << 4), 0, 0, 0, 0);
+                            for (uint32_t q = 0; q < 8; ++q) st_shared_v4(v_addr(j, c) + key * 128 + (q << 4), 0, 0, 0, 0);
                     const uint32_t which = __ballot_sync(0xFFFFFFFFu, bad[k] != 0);
-                    if (lane == 0) *reinterpret_cast<volatile uint32_t*>(&s_bad[n & 3u][k]) = which;
+                    if (lane == 0) *reinterpret_cast<volatile uint32_t*>(&s_bad[nth & 3u][k]) = which;
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
-                for (uint32_t c = 0; c < C::kNope; ++c) let_go(j * C::kStep + C::kKey + c);
-                if (lane == 0) mbar_arrive(bar(C::BAD + (n & 3u)));
+                if (lane == 0) mbar_arrive(bar(C::BAD + (nth & 3u)));
             }
+            if (*ctl.abort_flag != 0u)
+                for (uint32_t x = n > C::kVSlots ? n - C::kVSlots : 0; x < n; ++x) mbar_wait_certain(bar(C::VFULL + x % C::kVSlots), (x / C::kVSlots) & 1u, ctl, kCacheTimeout | C::VFULL);
         } else {
             // ------------------------------------------------------------ warp 9: Q K^T, warp 10: P V
             const bool leader = elect_one();
@@ -348,9 +348,8 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
             uint32_t uses = 0;
             if (warp == 9 && all > 0) wait(C::QFULL, 0);
             for (uint32_t j = 0; j < all; ++j) {
-                const uint32_t n = j * C::kStep + (warp == 9 ? 0 : C::kKey);
-                const uint32_t chunks = warp == 9 ? C::kKey : C::kNope;
-                for (uint32_t c = 0; c < chunks; ++c) wait(C::FULL + (n + c) % C::kSlots, ((n + c) / C::kSlots) & 1u);
+                if (warp == 9) wait(C::KFULL + j % C::kKSlots, (j / C::kKSlots) & 1u);
+                else wait(C::VFULL + j % C::kVSlots, (j / C::kVSlots) & 1u);
 #pragma unroll
                 for (uint32_t i = 0; i < 2; ++i) {
                     if (j >= steps[i]) continue;
@@ -364,7 +363,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
                             const uint32_t tS = tmem + (i ? C::kColS1 : C::kColS0);
 #pragma unroll
                             for (uint32_t c = 0; c < C::kKey; ++c) {
-                                const uint64_t dq = make_smem_desc<128>(base + (i * C::kKey + c) * kExpandChunk, 16), dk = make_smem_desc<128>(slot_addr(n + c), 16);
+                                const uint64_t dq = make_smem_desc<128>(base + (i * C::kKey + c) * kExpandChunk, 16), dk = make_smem_desc<128>(k_addr(j, c), 16);
                                 const uint32_t ks_end = c < C::kNope ? 4u : rope_steps;
                                 for (uint32_t ks = 0; ks < ks_end; ++ks) mma_ss(tS, dq + 2 * ks, dk + 2 * ks, idesc_s, c + ks > 0 ? 1u : 0u);
                             }
@@ -376,7 +375,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
                         if (leader && ok) {
 #pragma unroll
                             for (uint32_t c = 0; c < C::kNope; ++c) {
-                                const uint64_t dv = make_smem_desc<128>(slot_addr(n + c), 16);
+                                const uint64_t dv = make_smem_desc<128>(v_addr(j, c), 16);
 #pragma unroll
                                 for (uint32_t ks = 0; ks < kExpandTile / 16; ++ks)
                                     mma_ts(tmem + (i ? C::kColO1 : C::kColO0) + 64 * c, tmem + (i ? C::kColP1 : C::kColP0) + 8 * ks, dv + ks * (2048 >> 4), idesc_y, j + ks > 0 ? 1u : 0u);
@@ -385,8 +384,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
                         }
                     }
                 }
-                if (leader && ok)
-                    for (uint32_t c = 0; c < chunks; ++c) tc_commit(bar(C::EMPTY + (n + c) % C::kSlots));
+                if (leader && ok) tc_commit(bar(warp == 9 ? C::KEMPTY + j % C::kKSlots : C::VEMPTY + j % C::kVSlots));
                 __syncwarp();
             }
             const int last = C::FINAL + (warp == 9 ? 0 : 1);
