@@ -124,6 +124,14 @@ int launch_rows(Device& d, uint32_t bit, const CUtensorMap& map, const fa::Laten
                      : launch_rows<LC, 64>(d, bit + 3, map, a, stream);
 }
 
+template <int NOPE, bool kBf16>
+int launch_prompt(Device& d, uint32_t bit, uint32_t ctas, cudaStream_t stream, const CUtensorMap& q, const CUtensorMap& qr, const CUtensorMap& kv, const CUtensorMap& r,
+                  const fa::ExpandArgs& a) {
+    const int rc = allow_smem(d, bit, &fa::fa_latent_prompt<NOPE, kBf16>, fa::ExpandCfg<NOPE>::kSmemBytes);
+    if (rc != FA_B200_OK) return rc;
+    return launch(&fa::fa_latent_prompt<NOPE, kBf16>, ctas, fa::kExpandThreads, fa::ExpandCfg<NOPE>::kSmemBytes, stream, q, qr, kv, r, a);
+}
+
 }  // namespace
 
 extern "C" {
@@ -250,7 +258,7 @@ int fa_b200_latent_prompt(const void* q_nope, int64_t qn_batch_stride, int64_t q
     fa::ExpandArgs a = {};
     a.lengths = lengths_or_null, a.counts = counts_or_null, a.y = static_cast<uint8_t*>(y);
     a.B = B, a.T = T, a.S = S, a.heads = heads, a.pairs = static_cast<uint32_t>(pairs), a.rope = rope_dim;
-    a.causal = (flags & FA_B200_CACHE_ALL_KEYS) ? 0u : 1u, a.bf16 = dtype == FA_B200_BF16, a.scale_log2 = static_cast<float>(scale * kLog2e);
+    a.causal = (flags & FA_B200_CACHE_ALL_KEYS) ? 0u : 1u, a.scale_log2 = static_cast<float>(scale * kLog2e);
     Device* d = nullptr;
     if ((rc = device_of(device, &d)) != FA_B200_OK) return rc;
     OnDevice on(device);
@@ -277,12 +285,9 @@ int fa_b200_latent_prompt(const void* q_nope, int64_t qn_batch_stride, int64_t q
 #ifdef FA_DEBUG
     if (const cudaError_t e = cudaMemsetAsync(y, 0xFF, 2ull * B * T * heads * nope_dim, stream)) return static_cast<int>(e);
 #endif
-    if (nope_dim == 64) {
-        if ((rc = allow_smem(*d, 12, &fa::fa_latent_prompt<64>, fa::ExpandCfg<64>::kSmemBytes)) != FA_B200_OK) return rc;
-        return launch(&fa::fa_latent_prompt<64>, static_cast<uint32_t>(items), fa::kExpandThreads, fa::ExpandCfg<64>::kSmemBytes, stream, q, qr, kv, r, a);
-    }
-    if ((rc = allow_smem(*d, 13, &fa::fa_latent_prompt<128>, fa::ExpandCfg<128>::kSmemBytes)) != FA_B200_OK) return rc;
-    return launch(&fa::fa_latent_prompt<128>, static_cast<uint32_t>(items), fa::kExpandThreads, fa::ExpandCfg<128>::kSmemBytes, stream, q, qr, kv, r, a);
+    const uint32_t ctas = static_cast<uint32_t>(items);
+    if (nope_dim == 64) return dtype == FA_B200_BF16 ? launch_prompt<64, true>(*d, 12, ctas, stream, q, qr, kv, r, a) : launch_prompt<64, false>(*d, 13, ctas, stream, q, qr, kv, r, a);
+    return dtype == FA_B200_BF16 ? launch_prompt<128, true>(*d, 14, ctas, stream, q, qr, kv, r, a) : launch_prompt<128, false>(*d, 15, ctas, stream, q, qr, kv, r, a);
 }
 
 int fa_b200_latent_status(int device, uint32_t out[2]) {

@@ -37,7 +37,7 @@ struct ExpandArgs {
     const int32_t* lengths;   // [B] or null: S each
     const int32_t* counts;    // [B] or null: T each
     uint8_t* y;               // [B, T, heads, NOPE] contiguous
-    uint32_t B, T, S, heads, pairs, rope, causal, bf16;
+    uint32_t B, T, S, heads, pairs, rope, causal;
     float scale_log2;
 };
 
@@ -78,7 +78,7 @@ __device__ __forceinline__ float largest_of_32(const float* x) {
     return max3(a, b, fmaxf(x[30], x[31]));
 }
 
-template <int NOPE>
+template <int NOPE, bool kBf16>
 __global__ void __launch_bounds__(kExpandThreads, 1)
     fa_latent_prompt(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_qr, const __grid_constant__ CUtensorMap map_kv,
                      const __grid_constant__ CUtensorMap map_r, const ExpandArgs p) {
@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
     auto k_addr = [&](uint32_t j, uint32_t c) { return base + C::kOffK + ((j % C::kKSlots) * C::kKey + c) * kExpandChunk; };
     auto v_addr = [&](uint32_t j, uint32_t c) { return base + C::kOffV + ((j % C::kVSlots) * C::kNope + c) * kExpandChunk; };
     const WaitCtl ctl{g_latent_status, &abort_flag, kWaitCapCycles, nullptr, 0};
-    const bool bf16 = p.bf16 != 0;
+    constexpr bool bf16 = kBf16;
 
     if (tid == 0) {
         for (int i = 0; i < C::kBarriers; ++i) mbar_init(bar(i), i >= C::SFREE && i < C::PV ? 4u : 1u);
@@ -205,8 +205,9 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
                     unpack_f32x2(fma_f32x2(pack_f32x2(s[q * 32 + 2 * e], s[q * 32 + 2 * e + 1]), scale2, ref2), x0, x1);
                     const float w0 = ex2_approx(x0), w1 = ex2_approx(x1);
                     pk[e] = pack_16(w0, w1, bf16);
-                    if (e & 1) sum_b = add_f32x2(sum_b, pack_f32x2(w0, w1));
-                    else sum_a = add_f32x2(sum_a, pack_f32x2(w0, w1));
+                    const float2 y = unpack_16(pk[e], bf16);   // summed as rounded
+                    if (e & 1) sum_b = add_f32x2(sum_b, pack_f32x2(y.x, y.y));
+                    else sum_a = add_f32x2(sum_a, pack_f32x2(y.x, y.y));
                 }
                 if (q == 0) {
                     if (j > 0) {
