@@ -280,6 +280,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
         bool helped = false;   // with the first segment's queries
         for (uint32_t b = part; b < p.s.B; b += p.parts) {   // sequences without tokens
             if (latent_units(p, b) != 0) continue;
+            if (group == 0 && tid == 0 && !cache_length_ok(plain_view(p.c), p.s, b)) cache_report(p.c.status, kCacheBadPosition);
             uint8_t* const to = p.y + (static_cast<uint64_t>(b) * p.rows + row0) * (128 * LC);
             for (uint32_t i = tid; i < n_rows * (8 * LC); i += kLatentSoftmax) *reinterpret_cast<uint4*>(to + 16 * i) = make_uint4(0, 0, 0, 0);
         }
