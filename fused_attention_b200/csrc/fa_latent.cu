@@ -87,8 +87,10 @@ LatentPlan plan_rows(uint32_t latent, uint32_t heads, uint32_t page, uint32_t B,
     r.group_rows = static_cast<uint32_t>((r.rows + r.groups - 1) / r.groups);
     r.n = (r.group_rows + 15) / 16 * 16;
     r.groups = static_cast<uint32_t>((r.rows + r.group_rows - 1) / r.group_rows);
-    const uint64_t tiles = static_cast<uint64_t>(B) * ((static_cast<uint64_t>(width) * page + fa::kLatentTile - 1) / fa::kLatentTile);
-    r.least = r.n == 16 ? 2 : 4;
+    const uint64_t each = (static_cast<uint64_t>(width) * page + fa::kLatentTile - 1) / fa::kLatentTile, tiles = B * each;   // at most
+    // Two tiles a CTA at least (us, with 1, 2, 3 and 4 or 8: 1 sequence of 1000 tokens 16 heads 10.0, 10.4, -, 13.7; 128 heads 14.6, 14.5, 17.1,
+    // 18.6; 4 of 2000 32 heads 16.5, 13.7, 17.3, 15.3; 1 of 4000 128 heads 20.8, 17.4, 18.2, 18.6).
+    r.least = 2;
     // As many parts as fill the SMs, in one round, or in up to four where fewer would leave more than a tenth of them idle.
     uint64_t parts = 1;
     double best = 0;
@@ -99,7 +101,12 @@ LatentPlan plan_rows(uint32_t latent, uint32_t heads, uint32_t page, uint32_t B,
     }
     const uint64_t most = (tiles + r.least - 1) / r.least;
     r.parts = static_cast<uint32_t>(parts < most ? parts : most);
-    const uint64_t slots = r.parts == 1 ? 0 : 2ull * r.parts * r.groups;
+    // Short sequences are not divided where they give a quarter of the SMs something to do: what would be left of them takes less than
+    // joining, which costs the more the more rows there are.  (us whole and divided: 64 sequences of 100 to 512 tokens, 16 heads, 16.6 and
+    // 19.8, 16 of them 15.7 and 14.8, 1 of 301 12.1 and 9.8, 64 of 500 to 1000 26.7 and 23.7; 128 heads, 64 of 100 to 512 25 and 42, of 500 to
+    // 1000 39 and 54.)
+    if (each <= (r.n <= 32 ? 8u : 16u) && static_cast<uint64_t>(B) * r.groups >= sms / 4) r.parts = B, r.least = 0;
+    const uint64_t slots = r.parts == 1 || r.least == 0 ? 0 : 2ull * r.parts * r.groups;
     r.o_bytes = slots * r.n * latent * 4;
     r.ml_bytes = slots * r.n * 8;
     r.share_bytes = static_cast<uint64_t>(B) * 8;
@@ -110,7 +117,7 @@ template <int LC, int N>
 int launch_rows(Device& d, uint32_t bit, const CUtensorMap& map, const fa::LatentRowsArgs& a, cudaStream_t stream) {
     int rc = allow_smem(d, bit, &fa::fa_latent_rows<LC, N>, fa::LatentCfg<LC, N>::kSmemBytes);
     if (rc == FA_B200_OK) rc = launch(&fa::fa_latent_rows<LC, N>, a.parts * a.groups, fa::kLatentThreads, fa::LatentCfg<LC, N>::kSmemBytes, stream, map, a);
-    if (rc != FA_B200_OK || a.parts == 1) return rc;
+    if (rc != FA_B200_OK || a.parts == 1 || a.least == 0) return rc;
     // a sequence has about parts / B parts, and one more
     const uint32_t items = a.s.B * a.rows * (LC / 2);
     if (a.parts >= 8 * a.s.B) return launch(&fa::fa_latent_join<LC, N, true>, items, fa::kLatentJoinWarps * 32, 0, stream, a);

@@ -47,7 +47,7 @@ struct LatentRowsArgs {
     uint8_t* y;              // [B, T, heads, latent] contiguous
     int64_t ql_b, ql_t, ql_h, qr_b, qr_t, qr_h;   // strides in bytes
     uint32_t heads, rows, groups, group_rows;     // rows: T * heads, in `groups` of group_rows (the last may have fewer)
-    uint32_t parts, least;                        // CTAs a group; tiles that one has at least
+    uint32_t parts, least;                        // CTAs a group; tiles that one has at least (0: a CTA has a sequence, none is divided)
     uint32_t causal, bf16;
     float scale_log2;        // scale * log2(e)
     float* part_o;           // [parts * groups * 2, N, latent]
@@ -110,6 +110,7 @@ __device__ __forceinline__ uint32_t latent_limit(const LatentRowsArgs& p, const 
 }
 // Keys that some row of a group sees (its last token's, of those that the sequence has).
 __device__ __forceinline__ uint32_t latent_farthest(const LatentRowsArgs& p, const LatentSeq& q, uint32_t group) {
+    if (p.s.T == 1) return q.count == 0 ? 0u : q.held;   // (in front of two divisions that stand in a token's way)
     const uint32_t row0 = group * p.group_rows, t_first = row0 / p.heads, t_last = (min(p.rows, row0 + p.group_rows) - 1u) / p.heads;
     if (t_first >= q.count) return 0;
     return latent_limit(p, q, min(t_last, q.count - 1u));
@@ -130,6 +131,11 @@ struct LatentWalk {
 };
 __device__ __forceinline__ bool latent_start(const LatentRowsArgs& p, uint32_t part, LatentWalk& w) {
     const uint32_t lane = threadIdx.x & 31u;
+    if (p.least == 0) {
+        w.unit = w.before = 0, w.b = part, w.each = 1, w.more = 0;
+        w.unit_end = latent_units(p, part);
+        return w.unit_end != 0;
+    }
     uint32_t total = 0, kept = 0;
     for (uint32_t b = lane; b < p.s.B; b += 32) total += kept = latent_units(p, b);
     if (lane >= p.s.B) kept = 0;
@@ -295,14 +301,14 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
             if (group == 0 && w.begins && tid == 0)
                 p.shares[w.seq] = make_int2(static_cast<int>(part), static_cast<int>(latent_owner(w, w.first_unit + w.units - 1u)));
             if (tid < N) {   // (what becomes of a row that sees nothing is not used)
-                const uint32_t x = tid < n_rows ? latent_limit(p, w.q, (row0 + tid) / p.heads) : 0u;
+                const uint32_t x = tid < n_rows ? latent_limit(p, w.q, p.s.T == 1 ? 0u : (row0 + tid) / p.heads) : 0u;
                 s_limit[tid] = x == 0 ? kSeesAll : x;
             }
             float m[2 * kBlocks], l[2 * kBlocks];
 #pragma unroll
             for (int i = 0; i < 2 * kBlocks; ++i) m[i] = -INFINITY, l[i] = 0.0f;
             // keys that all rows see that see any: up to the first row's
-            uint32_t least = latent_limit(p, w.q, row0 / p.heads);
+            uint32_t least = p.s.T == 1 ? w.farthest : latent_limit(p, w.q, row0 / p.heads);
             if (least == 0) {   // (tokens in front of the first key: found by every thread, rows are few)
                 least = w.farthest;
                 for (uint32_t t = row0 / p.heads; t <= (row0 + n_rows - 1u) / p.heads; ++t) {
