@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
     };
 
     LatentWalk w;
-    const bool any = latent_start(p, part, w);
+    const bool any = latent_start(p, part, w) && latent_next(p, group, w);   // (the first segment is worked out by all roles together: one way through the code)
     if (warp < 8) {
         // ---------------------------------------------------------------- softmax
         const uint32_t lanes = warp & 3u, side = warp >> 2, lane_off = (lanes * 32u) << 16;
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
             uint8_t* const to = p.y + (static_cast<uint64_t>(b) * p.rows + row0) * (128 * LC);
             for (uint32_t i = tid; i < n_rows * (8 * LC); i += kLatentSoftmax) *reinterpret_cast<uint4*>(to + 16 * i) = make_uint4(0, 0, 0, 0);
         }
-        while (any && latent_next(p, group, w)) {
+        for (bool more = any; more; more = latent_next(p, group, w)) {
             if (!helped && w.end > w.t0) {
                 copy_queries(w.seq, tid, kLatentSoftmax + 64u, N);
                 cp_async_wait_all();
@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
         const uint32_t box_rows = min(p.c.page, kLatentTile), box_bytes = box_rows * 128;
         uint32_t g = 0, reports = 0, asked = 0;   // (asked: slots with a copy under way or done, up to this tile's)
         bool ok = true;
-        while (ok && any && latent_next(p, group, w)) {
+        for (bool more = any; ok && more; more = latent_next(p, group, w)) {
             const int32_t* const table = p.s.table + w.seq * p.s.table_stride;
             if (warp == 8 && w.begins && group == 0 && lane == 0 && !cache_length_ok(plain_view(p.c), p.s, w.seq)) cache_report(p.c.status, kCacheBadPosition);
             const uint32_t blocks = (w.q.held + p.c.page - 1u) >> p.c.page_shift;
@@ -594,7 +594,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
         const uint32_t idesc_s = idesc_16bit(kLatentTile, N, false, false, bf16), idesc_y = idesc_16bit(128, N, true, true, bf16);
         const uint32_t rope_steps = p.c.rope / 16;
         uint32_t g = 0, k = 0;   // tiles; segments with tiles
-        while (any && latent_next(p, group, w)) {
+        for (bool more = any; more; more = latent_next(p, group, w)) {
             if (w.end == w.t0) continue;
             if (warp == 12) wait(C::QFULL, k & 1u);
             for (uint32_t tile = w.t0; tile < w.end; ++tile, ++g) {
@@ -656,7 +656,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
     } else {
         // ---------------------------------------------------------------- queries
         uint32_t k = 0;
-        while (any && latent_next(p, group, w)) {
+        for (bool more = any; more; more = latent_next(p, group, w)) {
             if (w.end == w.t0) continue;
             if (k > 0) mbar_wait(bar(C::QEMPTY), (k - 1u) & 1u, ctl, kCacheTimeout | C::QEMPTY);
             if (k == 0) {
