@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
             const uint32_t chunk = to + (j >> 3) * C::kQChunk;
 #pragma unroll 4
             for (; r < rows; r += step) {
-                const bool in = r < n_rows;
+                const bool in = r < n_rows && FA_CACHE_OK(p.c.status, kDbgRow, seq < p.s.B && t < p.s.T && h < p.heads);
                 cp_async_16_zero(chunk + r * 128 + (((j & 7u) ^ (r & 7u)) << 4), in ? from + t * t_stride + h * h_stride + 16 * j : from, in);
                 for (h += step; h >= p.heads; h -= p.heads) ++t;
             }
@@ -488,7 +488,8 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
             softmax_sync();
             const uint32_t slot = 2u * blockIdx.x + (w.begins ? 1u : 0u);
             if (!w.whole && tid < n_rows) p.part_ml[static_cast<uint64_t>(slot) * N + tid] = make_float2(s_m[tid], s_l[tid]);
-            if (tiles || w.whole) {
+            const bool inside = w.whole ? FA_CACHE_OK(p.c.status, kDbgRow, w.seq < p.s.B && row0 + n_rows <= p.rows) : FA_CACHE_OK(p.c.status, kDbgScratch, slot < 2u * p.parts * p.groups);
+            if ((tiles || w.whole) && inside) {
 #pragma unroll 1
                 for (uint32_t c = 16 * side; c < C::kPairs * N; c += 32) {
                     float o[16];
@@ -535,7 +536,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                 const uint32_t key0 = tile * kLatentTile, first = key0 >> p.c.page_shift;
                 if (known == 0 || first + per_tile > from + known) {
                     from = first, known = 32;
-                    entry = from + lane < blocks ? table[from + lane] : -1;
+                    entry = from + lane < blocks && FA_CACHE_OK(p.c.status, kDbgEntry, w.seq < p.s.B && from + lane < p.s.width) ? table[from + lane] : -1;
                     const bool wrong = from + lane < blocks && static_cast<uint32_t>(entry) >= p.c.n_pages && (from + lane) * p.c.page < w.end * kLatentTile;
                     if (wrong && warp == 8) ++reports;
                     if (static_cast<uint32_t>(entry) >= p.c.n_pages) entry = static_cast<int32_t>(p.c.n_pages);   // outside: TMA fills with zeros
