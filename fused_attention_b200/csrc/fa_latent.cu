@@ -1,8 +1,6 @@
 // C entry points of the paged cache of latent vectors (include/fa_b200.h): checks, the choice of a kernel, launches.
 #include <cuda.h>
 
-#include <cmath>
-
 #include "fa_b200.h"
 #include "fa_host.cuh"
 #include "fa_latent.cuh"
@@ -73,6 +71,9 @@ int rows_ok(const void* base, std::initializer_list<int64_t> strides) {
         if (!multiple16(2 * s)) return FA_B200_ERR_ALIGNMENT;
     return FA_B200_OK;
 }
+
+// (so that its product with log2 e is a normal number too)
+bool scale_ok(float scale) { return scale >= 0x1p-126f && scale <= 1e38f; }
 
 struct LatentPlan {
     uint32_t n, groups, group_rows, parts, least;
@@ -207,7 +208,7 @@ int fa_b200_latent_attention(const fa_b200_latent_cache* cache, const fa_b200_se
     if (!aligned16(scratch)) return FA_B200_ERR_ALIGNMENT;
     if (dtype > FA_B200_BF16) return FA_B200_ERR_DTYPE;
     if (flags & ~FA_B200_CACHE_ALL_KEYS) return FA_B200_ERR_FLAGS;
-    if (heads == 0 || !(scale > 0.0f) || !std::isfinite(scale)) return FA_B200_ERR_SHAPE;
+    if (heads == 0 || !scale_ok(scale)) return FA_B200_ERR_SHAPE;
     if (static_cast<uint64_t>(a.s.T) * heads > 0x3FFFFFFFull) return FA_B200_ERR_SHAPE;
     Device* d = nullptr;
     if ((rc = device_of(device, &d)) != FA_B200_OK) return rc;
@@ -259,7 +260,7 @@ int fa_b200_latent_prompt(const void* q_nope, int64_t qn_batch_stride, int64_t q
     if ((nope_dim != 64 && nope_dim != 128) || (rope_dim != 16 && rope_dim != 32 && rope_dim != 64)) return FA_B200_ERR_HEAD_DIM;
     if (dtype > FA_B200_BF16) return FA_B200_ERR_DTYPE;
     if (flags & ~FA_B200_CACHE_ALL_KEYS) return FA_B200_ERR_FLAGS;
-    if (B == 0 || T == 0 || S == 0 || heads == 0 || B > (1u << 24) || T > 0x3FFFFFFFu || S > 0x3FFFFFFFu || heads > (1u << 20) || !(scale > 0.0f) || !std::isfinite(scale)) return FA_B200_ERR_SHAPE;
+    if (B == 0 || T == 0 || S == 0 || heads == 0 || B > (1u << 24) || T > 0x3FFFFFFFu || S > 0x3FFFFFFFu || heads > (1u << 20) || !scale_ok(scale)) return FA_B200_ERR_SHAPE;
     const uint64_t pairs = (static_cast<uint64_t>(T) + 2 * fa::kExpandTile - 1) / (2 * fa::kExpandTile), items = pairs * B * heads;
     if (static_cast<uint64_t>(B) * heads > kMostCtas || items > kMostCtas) return FA_B200_ERR_SHAPE;
     fa::ExpandArgs a = {};

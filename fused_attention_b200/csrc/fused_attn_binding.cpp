@@ -17,7 +17,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <limits>
 #include <vector>
 
 #include "fa_b200.h"
@@ -305,12 +304,11 @@ bool plain_rotation(PyObject* o, at::Tensor& cos, at::Tensor& sin, int device, i
     }
     return true;
 }
-// A number above zero and below infinity, from a Python float or int.
+// A scale that the library takes, from a Python float.
 bool positive(PyObject* o, float& x) {
     if (!PyFloat_CheckExact(o)) return false;
-    const double d = PyFloat_AS_DOUBLE(o);
-    x = static_cast<float>(d);
-    return x > 0.0f && x < std::numeric_limits<float>::infinity();
+    x = static_cast<float>(PyFloat_AS_DOUBLE(o));
+    return x >= 0x1p-126f && x <= 1e38f;
 }
 
 // (entry, cache, device, dtype, latents, rope_keys, table, lengths, counts, queries, rotation, interleaved) -> (keys, queries or None)

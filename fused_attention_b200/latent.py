@@ -181,7 +181,7 @@ def _scratch_bytes(latent: int, heads: int, page: int, B: int, T: int, width: in
 
 
 def _check_scale(scale) -> float:
-    _require(isinstance(scale, (int, float)) and 0 < scale < math.inf, "scale must be a positive, finite number")
+    _require(isinstance(scale, (int, float)) and 2.0 ** -126 <= scale <= 1e38, "scale must be a positive number, 2^-126 to 10^38")
     return float(scale)
 
 

@@ -18,7 +18,7 @@ table by streams.  There is no CPU path.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Tuple, Union
+from typing import Tuple, Union
 
 import torch
 
@@ -59,14 +59,21 @@ def _done(answer) -> bool:
 class PagePool:
     """How many table entries hold each page: ``refs``, int32 [n_pages], contiguous; 0 is a free page."""
 
-    def __init__(self, refs: torch.Tensor, _status: Optional[torch.Tensor] = None):
+    def __init__(self, refs: torch.Tensor):
         _require(isinstance(refs, torch.Tensor) and refs.dtype == torch.int32, "refs must be an int32 tensor")
         _require(refs.is_cuda, "refs must be a CUDA tensor")
         _require(refs.dim() == 1 and 0 < refs.shape[0] < 1 << 30 and refs.is_contiguous(), "refs must be contiguous, of shape [n_pages]")
-        self.refs, self.n_pages, self.device, self._index = refs, refs.shape[0], refs.device, refs.get_device()
-        self._status = torch.zeros(4, dtype=torch.int32, device=refs.device) if _status is None else _status
-        self._handle = _lib.Pages(refs.data_ptr(), self._status.data_ptr(), self.n_pages)
+        self._set(refs, refs.shape[0], refs.device, refs.get_device(), torch.zeros(4, dtype=torch.int32, device=refs.device))
+
+    def _set(self, refs, n_pages, device, index, status) -> "PagePool":
+        self.refs, self.n_pages, self.device, self._index, self._status = refs, n_pages, device, index, status
+        self._handle = _lib.Pages(refs.data_ptr(), status.data_ptr(), n_pages)
         self._address = ctypes.addressof(self._handle)
+        return self
+
+    def _with(self, refs: torch.Tensor) -> "PagePool":
+        """A pool of other counts of the same pages, which reports where this one does."""
+        return PagePool.__new__(PagePool)._set(refs, self.n_pages, self.device, self._index, self._status)
 
     def read_status(self) -> Tuple[int, int]:
         """(first code, number of reports) of what the kernels found wrong; clears it.  Synchronises.  ``STATUS`` says what the codes mean."""
@@ -158,7 +165,7 @@ def pages_compact(pool: PagePool, table: torch.Tensor) -> Tuple[PagePool, torch.
     _, _, compact, _, entries = _calls()
     done = compact(entries[2], pool._address, pool._index, table)
     if _done(done):
-        return (PagePool(done[0], pool._status),) + done[1:]
+        return (pool._with(done[0]),) + done[1:]
     _check_ints(table, "table", pool, (None, None))
     B, W = table.shape
     refs, sources, targets = torch.empty(3, pool.n_pages, dtype=torch.int32, device=pool.device).unbind(0)
@@ -167,7 +174,7 @@ def pages_compact(pool: PagePool, table: torch.Tensor) -> Tuple[PagePool, torch.
     _lib.check(_lib.load().fa_b200_pages_compact(
         ctypes.byref(pool._handle), table.data_ptr(), table.stride(0), W, B, refs.data_ptr(), new.data_ptr(), sources.data_ptr(), targets.data_ptr(),
         scratch.data_ptr(), 4 * scratch.numel(), pool._index, _raw_stream(pool._index)))
-    return PagePool(refs, pool._status), new, sources, targets
+    return pool._with(refs), new, sources, targets
 
 
 def _areas(cache):
@@ -192,14 +199,18 @@ def cache_copy(caches, sources: torch.Tensor, targets: torch.Tensor) -> None:
     ``sources``, ``targets`` int32 [n] on the caches' device; pairs with -1 are passed over.  No page may be a target twice, or a target and
     a source.  The caches have as many pages each; a page outside is reported in the first one's ``read_status``.
     """
-    caches = (caches,) if isinstance(caches, (KVCache, LatentCache)) else caches
-    _require(isinstance(caches, (list, tuple)) and len(caches) > 0 and all(isinstance(c, (KVCache, LatentCache)) for c in caches),
-             "the first argument must be a KVCache, a LatentCache or a list of them")
+    if caches.__class__ not in (list, tuple):
+        caches = (caches,)
+    _require(len(caches) > 0 and isinstance(caches[0], (KVCache, LatentCache)), "the first argument must be a KVCache, a LatentCache or a list of them")
     first = caches[0]
-    _require(all(c.n_pages == first.n_pages and c._index == first._index for c in caches), "the caches must have as many pages, on one device")
-    _require(all(c._writable for c in caches), "the pages of a cache lie on top of one another: it cannot be copied to")
+    areas = []
+    for c in caches:
+        _require(isinstance(c, (KVCache, LatentCache)), "the first argument must be a KVCache, a LatentCache or a list of them")
+        _require(c.n_pages == first.n_pages and c._index == first._index, "the caches must have as many pages, on one device")
+        _require(c._writable, "the pages of a cache lie on top of one another: it cannot be copied to")
+        areas.append(c._copy_areas or _areas(c))
+    areas, status = tuple(areas), first._status.data_ptr()
     _, _, _, copy, entries = _calls()
-    areas, status = tuple(_areas(c) for c in caches), first._status.data_ptr()
     if _done(copy(entries[3], areas, first.n_pages, status, first._index, sources, targets)):
         return
     for t, name in ((sources, "sources"), (targets, "targets")):

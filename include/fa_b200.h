@@ -476,7 +476,7 @@ int fa_b200_latent_append(const fa_b200_latent_cache* cache, const fa_b200_seque
  * the latent space: q_latent [B, T, heads, latent_dim], q_rope [B, T, heads, rope_dim] (rotated), y [B, T, heads, latent_dim] contiguous.  Queries
  * are the last tokens of their sequences, as with fa_b200_cache_attention, FA_B200_CACHE_ALL_KEYS too.  Cache and queries have one type.
  * Scores, sums and maxima are held in fp32, weights are rounded to the type for their product with c and summed as rounded.  A query that sees
- * nothing, or that its sequence does not have, gets zeros.  Rows that a query does not see do not reach it, whatever they hold.  0 < scale < inf.
+ * nothing, or that its sequence does not have, gets zeros.  Rows that a query does not see do not reach it, whatever they hold.  scale: 2^-126 to 10^38.
  */
 int fa_b200_latent_attention(const fa_b200_latent_cache* cache, const fa_b200_sequences* sequences, const void* q_latent, int64_t ql_batch_stride,
                              int64_t ql_token_stride, int64_t ql_head_stride, const void* q_rope, int64_t qr_batch_stride, int64_t qr_token_stride,

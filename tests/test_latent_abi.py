@@ -93,7 +93,7 @@ def test_attention_rejections(lib):
         assert attention(lib, **bad) == _lib.ERR_NULL_POINTER
     assert attention(lib, qlh=516) == _lib.ERR_ALIGNMENT
     assert attention(lib, flags=1) == _lib.ERR_FLAGS
-    for bad in (dict(heads=0), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")), dict(scale=float("nan")), dict(heads=1 << 31)):
+    for bad in (dict(heads=0), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")), dict(scale=float("nan")), dict(scale=1e-39), dict(scale=2e38), dict(heads=1 << 31)):
         assert attention(lib, **bad) == _lib.ERR_SHAPE
 
 

@@ -45,7 +45,7 @@ def pool_of(table, n):
 
 
 @pytest.mark.parametrize("B,W,page,n,T", [(1, 3, 16, 5, 1), (5, 6, 32, 40, 1), (33, 9, 16, 400, 1), (40, 20, 64, 900, 300), (300, 7, 128, 2500, 1), (7, 300, 16, 3000, 2000),
-                                          (2100, 4, 16, 9000, 1), (600, 70, 16, 30000, 40)])
+                                          (2100, 4, 16, 9000, 1), (600, 70, 16, 30000, 40), (300, 150, 16, 50000, 1)])
 def test_reserve(B, W, page, n, T):
     """Any counts, shared blocks of every kind, blocks behind the need; tables one CTA goes over and larger ones."""
     rng = random.Random(B * W)
