@@ -178,11 +178,14 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
                     const int left = valid - w * 32;
                     const uint32_t seen = left >= 32 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << left) - 1u;
                     const uint32_t bad = *reinterpret_cast<volatile uint32_t*>(&s_bad[n & 3u][w]);
+                    if (bad != 0) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        if (!(seen >> e & 1u)) s[w * 32 + e] = -INFINITY;
-                        else if (bad >> e & 1u) s[w * 32 + e] = __int_as_float(0x7FC00000);
+                        for (int e = 0; e < 32; ++e)
+                            if (bad >> e & 1u) s[w * 32 + e] = __int_as_float(0x7FC00000);
                     }
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (!(seen >> e & 1u)) s[w * 32 + e] = -INFINITY;
                 }
             }
             const float top = fmaxf(fmaxf(largest_of_32(s), largest_of_32(s + 32)), fmaxf(largest_of_32(s + 64), largest_of_32(s + 96))) * p.scale_log2;
@@ -319,11 +322,11 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
                     for (uint32_t k = 0; k < 4; ++k) {
                         const uint32_t key = lane + 32 * k;
                         if (key0 + key < least || key0 + key >= farthest) continue;
-                        for (uint32_t q = 0; q < 8; ++q) {
-                            uint32_t x[4];
-                            ld_shared_v4(v_addr(j, c) + key * 128 + ((q ^ (key & 7u)) << 4), x);
-                            bad[k] |= not_finite(x, bf16);
-                        }
+                        uint32_t x[8][4];   // the key's row of the chunk, in any order
+#pragma unroll
+                        for (uint32_t q = 0; q < 8; ++q) ld_shared_v4(v_addr(j, c) + key * 128 + ((q ^ (key & 7u)) << 4), x[q]);
+#pragma unroll
+                        for (uint32_t q = 0; q < 8; ++q) bad[k] |= not_finite(x[q], bf16);
                     }
                 for (uint32_t k = 0; k < 4; ++k) {
                     const uint32_t key = lane + 32 * k;
