@@ -23,6 +23,10 @@ __device__ __forceinline__ CacheView plain_view(const LatentView& v) {
 }
 
 // ----------------------------------------------------------------------------- append
+// Bound by memory for prompts (4 of up to 2048 tokens, 32 heads of 64, 60 MB with the zeros of queries past `counts`: 15 to 19 us, 3 to 4 TB/s;
+// asking for the rows ahead of the length, and so for absent tokens' too, took 18), by the launch and length -> table entry -> row for single
+// tokens (128 of them 2.3 us in a graph, 6.7 a call).
+//
 // A CTA a token, a thread 16 bytes of the latent vector or 16 values of a rotary part: one of the key's, one of a query head's.  Products
 // and sums of the rotation are rounded one by one in fp32, its results once to the tensors' type.
 struct LatentAppendArgs {

@@ -5,8 +5,7 @@
 // A CTA has 256 query rows (two tiles of 128) of one sequence and head, and goes over the keys that the last of them sees in steps of 128,
 // as fa_cache_prompt.cuh does: scores in tensor memory, a softmax thread a row, P (16 bits) into tensor memory, Y in tensor memory.  The
 // score's contraction has NOPE + rope dimensions, the last chunk of 64 of which is the rotary part, fetched from the tensor that all heads
-// share.  Operands come by TMA in chunks of 128 rows by 64 dimensions into two rings, of
-// keys and of values.  384 threads:
+// share.  Operands come by TMA in chunks of 128 rows by 64 dimensions into two rings, of keys and of values.  384 threads:
 //
 //   warps 0-3, 4-7   softmax of query tile 0 / 1, a thread a row
 //   warp 8           fetches queries and keys
@@ -15,7 +14,12 @@
 //                    zeros, and so do keys that hold an infinity or a NaN, whose weights become NaN for the rows that see them.  0 * NaN
 //                    reaches nobody
 //
-// (In one ring, values of a step come to stand in the way of keys two steps later: 4030 clocks a step instead of KSTEP, at NOPE = 128.)
+// Bound by the tensor pipe and the exponentials as fa_fwd_pipelined is: at NOPE = 128 a step of both tiles has 2560 tensor clocks of products and
+// 2048 of exponentials, and takes 3450.  (In one ring, values of a step came to stand in the way of keys two steps later: 4030.  With a barrier a
+// chunk and not a step it stayed at 4080: every wait that stands behind MMAs and commits costs the issuing warp 280 clocks.)  4096 tokens on 6000
+// keys, 20 heads of 128 + 64: 222 us, 0.93 PFLOP/s, 56 % of the products' measured peak; 8 prompts of 777, 12 heads of 64 + 32, 40 us.  An item's
+// beginning, end and up to three partly seen steps are what the second has most of.  Persistent CTAs, items dealt out there and back, were
+// slower, 236 and 54: items' lengths differ, and the hardware deals out better.
 // At NOPE = 128 both tiles' scores take turns on one 128-column buffer (tensor memory: 128 + 2 * 64 of P + 2 * 128 of Y), which the other
 // tile's P V covers; at 64 each has its own.  Items with the most keys go first.
 #pragma once

@@ -21,6 +21,11 @@
 //                tokens, 16 rows, where two took 72: a barrier's answer reaches a thread only behind the MMAs that it has queued)
 //   warps 14-15  queries into shared memory, a segment ahead; of the first segment the softmax warps do most
 //
+// Measured: 64 sequences of 100 to 8192 tokens, 16 rows, 64 us (306 MB, 4.7 TB/s; steady tiles of 73.7 KB take 2900 to 3000 clocks, the memory's
+// share 2830; the rest is the way to the first tile, 4 us, CTAs that the memory serves later than others, 5, and the join); 32 of 1000 to 8192, 128
+// rows in two groups, 83 us (tiles take 3000 clocks where their MMAs take 1920: with 74 KB of queries the ring has two tiles, and what one passes
+// through from its slots' asking to their letting go, 5700 clocks, is the bound).
+//
 // What must not happen: a key that a row does not see reaching it, as 0 * NaN.  Tiles that some row of the group sees in part only (the
 // last ones of a sequence) are gone over in shared memory between the two products: keys behind the last that any row sees become zeros;
 // a key that some rows see and that holds an infinity or a NaN becomes zeros too, and rows that see it get a weight that is NaN.

@@ -5,7 +5,9 @@
 // does not matter, and where one of several has to be chosen the lowest is (a minimum, likewise).
 //
 // These kernels read and write a few kilobytes to a megabyte: what bounds them is the chain of dependent accesses and the launch, so that
-// each call is one launch (compacting: two) and no value crosses to the host.  Copying is bound by memory.
+// each call is one launch (compacting: two) and no value crosses to the host.  Copying is bound by memory.  Measured in a graph: a step of 8 beams
+// of an 8-bit cache (fork, reserve, copy of 4 pages) 11 us, of 256 beams of two latent caches (141 pages of 147 KB) 21, of which copying takes 7.6
+// (5.5 TB/s); 10000 pages planned in 11 us, 2381 of 133 KB moved in 115 (5.5 TB/s, 84 % of a plain copy's).
 #pragma once
 
 #include "fa_cache.cuh"
