@@ -34,6 +34,7 @@ EXPORTED_SYMBOLS = (
     "fa_b200_cache_attention",
     "fa_b200_cache_attention_scratch",
     "fa_b200_cache_copy",
+    "fa_b200_describe_copy",
     "fa_b200_pages_fork",
     "fa_b200_pages_reserve",
     "fa_b200_pages_compact",
@@ -169,6 +170,8 @@ def load() -> ctypes.CDLL:
         pages, heads3 = ctypes.POINTER(Pages), [vp, i64, i64, i64]
         lib.fa_b200_cache_copy.restype = i32
         lib.fa_b200_cache_copy.argtypes = [ctypes.POINTER(CopyArea), u32, u32, vp, vp, u32, vp, i32, vp]
+        lib.fa_b200_describe_copy.restype = i32
+        lib.fa_b200_describe_copy.argtypes = [ctypes.POINTER(CopyArea), ctypes.POINTER(u32)]
         lib.fa_b200_pages_fork.restype = i32
         lib.fa_b200_pages_fork.argtypes = [pages, vp, i64, u32, u32, vp, vp, i32, vp]
         lib.fa_b200_pages_reserve.restype = i32

@@ -22,6 +22,26 @@ int table_of(const int32_t* table, int64_t stride, uint32_t width, uint32_t B, f
     return FA_B200_OK;
 }
 
+// Of what every address in an array of pages is a multiple.
+uint64_t unit_of(const void* base, int64_t page_stride, uint32_t n0, int64_t stride0, uint32_t n1, int64_t stride1, uint32_t row) {
+    const uint64_t all = reinterpret_cast<uintptr_t>(base) | static_cast<uint64_t>(page_stride) | row | (n0 > 1 ? static_cast<uint64_t>(stride0) : 0) |
+                         (n1 > 1 ? static_cast<uint64_t>(stride1) : 0);
+    return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
+}
+// An array in as few rows as it lies in.  What a thread takes at a time is decided by those and where they begin: rows that lie behind one another may
+// make one of a multiple of 16 bytes that does not begin on such a boundary.
+int area_of(const fa_b200_copy_area& x, fa::CopyArea* y) {
+    if (!x.base) return FA_B200_ERR_NULL_POINTER;
+    if (x.n0 == 0 || x.n1 == 0 || x.row_bytes == 0 || static_cast<uint64_t>(x.n0) * x.n1 > 0x7FFFFFFFull) return FA_B200_ERR_SHAPE;
+    if (unit_of(x.base, x.page_stride, x.n0, x.stride0, x.n1, x.stride1, x.row_bytes) < (x.row_bytes % 16 == 0 ? 16u : 4u)) return FA_B200_ERR_ALIGNMENT;
+    y->base = static_cast<uint8_t*>(x.base), y->page = x.page_stride, y->stride0 = x.stride0, y->stride1 = x.stride1;
+    y->n0 = x.n0, y->n1 = x.n1, y->row = x.row_bytes;
+    if (y->n1 > 1 && y->stride1 == y->row && static_cast<uint64_t>(y->row) * y->n1 < (1u << 31)) y->row *= y->n1, y->n1 = 1;
+    if (y->n0 > 1 && y->n1 == 1 && y->stride0 == y->row && static_cast<uint64_t>(y->row) * y->n0 < (1u << 31)) y->row *= y->n0, y->n0 = 1;
+    y->unit = static_cast<uint32_t>(unit_of(y->base, y->page, y->n0, y->stride0, y->n1, y->stride1, y->row));
+    return FA_B200_OK;
+}
+
 constexpr uint32_t kForkMost = 57344;   // sequences whose entries of one column fit shared memory
 constexpr int kForkSmem = 4 * kForkMost;
 
@@ -104,18 +124,13 @@ int fa_b200_cache_copy(const fa_b200_copy_area* areas, uint32_t n_areas, uint32_
     if (!areas || !sources || !targets || !status) return FA_B200_ERR_NULL_POINTER;
     if (!aligned4(sources) || !aligned4(targets) || !aligned4(status)) return FA_B200_ERR_ALIGNMENT;
     if (n_areas == 0 || n_pages == 0 || n_pages > 0x7FFFFFFFu || pairs == 0 || pairs > 0x7FFFFFFFu) return FA_B200_ERR_SHAPE;
+    int rc = FA_B200_OK;
     for (uint32_t i = 0; i < n_areas; ++i) {
-        const fa_b200_copy_area& x = areas[i];
-        if (!x.base) return FA_B200_ERR_NULL_POINTER;
-        if (x.n0 == 0 || x.n1 == 0 || x.row_bytes == 0 || static_cast<uint64_t>(x.n0) * x.n1 > 0x7FFFFFFFull) return FA_B200_ERR_SHAPE;
-        const uint64_t unit = x.row_bytes % 16 == 0 ? 16 : 4;
-        const uint64_t all = reinterpret_cast<uintptr_t>(x.base) | static_cast<uint64_t>(x.page_stride) | x.row_bytes |
-                             (x.n0 > 1 ? static_cast<uint64_t>(x.stride0) : 0) | (x.n1 > 1 ? static_cast<uint64_t>(x.stride1) : 0);
-        if (all % unit != 0) return FA_B200_ERR_ALIGNMENT;
+        fa::CopyArea y = {};
+        if ((rc = area_of(areas[i], &y)) != FA_B200_OK) return rc;
     }
     Device* d = nullptr;
-    int rc = device_of(device, &d);
-    if (rc != FA_B200_OK) return rc;
+    if ((rc = device_of(device, &d)) != FA_B200_OK) return rc;
     OnDevice on(device);
     if (on.rc != 0) return on.rc;
     const uint32_t sms = static_cast<uint32_t>(d->sms.load());
@@ -127,13 +142,8 @@ int fa_b200_cache_copy(const fa_b200_copy_area* areas, uint32_t n_areas, uint32_
         const uint32_t ctas = 8 * sms, share = (ctas + pairs - 1) / pairs;
         uint32_t parts = 0;
         for (uint32_t i = 0; i < a.areas; ++i) {
-            const fa_b200_copy_area& x = areas[first + i];
             fa::CopyArea& y = a.area[i];
-            y.base = static_cast<uint8_t*>(x.base), y.page = x.page_stride, y.stride0 = x.stride0, y.stride1 = x.stride1;
-            y.n0 = x.n0, y.n1 = x.n1, y.row = x.row_bytes;
-            // in as few rows as it lies in
-            if (y.n1 > 1 && y.stride1 == y.row && static_cast<uint64_t>(y.row) * y.n1 < (1u << 31)) y.row *= y.n1, y.n1 = 1;
-            if (y.n0 > 1 && y.n1 == 1 && y.stride0 == y.row && static_cast<uint64_t>(y.row) * y.n0 < (1u << 31)) y.row *= y.n0, y.n0 = 1;
+            (void)area_of(areas[first + i], &y);   // (looked at above)
             const uint64_t most = static_cast<uint64_t>(y.n0) * y.n1 * y.row / 16384;
             y.parts = static_cast<uint32_t>(most < 1 ? 1 : most < share ? most : share);
             if (y.parts > 64) y.parts = 64;
@@ -150,6 +160,15 @@ int fa_b200_cache_copy(const fa_b200_copy_area* areas, uint32_t n_areas, uint32_
         rc = static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
         if (rc != FA_B200_OK) return rc;
     }
+    return FA_B200_OK;
+}
+
+int fa_b200_describe_copy(const fa_b200_copy_area* area, uint32_t out[4]) {
+    if (!area || !out) return FA_B200_ERR_NULL_POINTER;
+    fa::CopyArea y = {};
+    const int rc = area_of(*area, &y);
+    if (rc != FA_B200_OK) return rc;
+    out[0] = y.n0, out[1] = y.n1, out[2] = y.row, out[3] = y.unit;
     return FA_B200_OK;
 }
 

@@ -523,12 +523,13 @@ __global__ void __launch_bounds__(256) fa_pages_renumber(const CompactArgs p) {
 
 // ----------------------------------------------------------------------------- copy
 // Contents of pages, source to target, for up to kCopyAreas arrays: a page of an array is n0 x n1 rows of `row` bytes (one row where it
-// lies in one piece).  CTAs are dealt out by parts of a page, `parts` equal ones of each array, first: CTA (x, y) has part y of the pairs x,
+// lies in one piece), taken 16 or 4 bytes at a time.  CTAs are dealt out by parts of a page, `parts` equal ones of each array, first: CTA (x, y) has part y of the pairs x,
 // x + gridDim.x, ...  Every thread has eight pieces of 16 bytes in flight.
 struct CopyArea {
     uint8_t* base;
     int64_t page, stride0, stride1;   // bytes
-    uint32_t n0, n1, row, parts;      // row: a multiple of 16, or of 4
+    uint32_t n0, n1, row, parts;
+    uint32_t unit;                    // 16 if base, strides and row are multiples of that, else 4
 };
 constexpr int kCopyAreas = 32;
 struct CopyArgs {
@@ -590,7 +591,7 @@ __global__ void __launch_bounds__(kCopyThreads, 3) fa_cache_copy(const __grid_co
         for (uint32_t left = __ballot_sync(0xFFFFFFFFu, good && s != t); left != 0; left &= left - 1u) {
             const int from = __ffs(left) - 1;
             const uint32_t source = static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, s, from)), target = static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, t, from));
-            if ((a.row & 15u) == 0) copy_part<uint4>(a, source, target, part);
+            if (a.unit == 16) copy_part<uint4>(a, source, target, part);
             else copy_part<uint32_t>(a, source, target, part);
         }
     }

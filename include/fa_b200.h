@@ -445,6 +445,10 @@ typedef struct fa_b200_copy_area {
 int fa_b200_cache_copy(const fa_b200_copy_area* areas, uint32_t n_areas, uint32_t n_pages, const int32_t* sources, const int32_t* targets, uint32_t pairs,
                        uint32_t* status, int device, void* cuda_stream);
 
+/* How an array is copied: out[0], out[1], out[2] = its rows n0 x n1 and their bytes once rows that lie behind one another are one, out[3] = bytes
+ * that a thread takes at a time, 16 or 4.  Pure arithmetic, no CUDA call; it is what fa_b200_cache_copy itself uses. */
+int fa_b200_describe_copy(const fa_b200_copy_area* area, uint32_t out[4]);
+
 /*
  * ---- The paged cache of latent vectors: fa_b200_latent_append, fa_b200_latent_attention, and fa_b200_latent_prompt.
  *
