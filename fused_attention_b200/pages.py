@@ -183,7 +183,8 @@ def _areas(cache):
         if isinstance(cache, KVCache):
             n, heads, page, H = cache.k.shape
             areas = [_lib.CopyArea(t.data_ptr(), *t.stride()[:3], heads, page, H) for t in (cache.k, cache.v)]
-            areas += [_lib.CopyArea(t.data_ptr(), 4 * heads, 0, 0, 1, 1, 4 * heads) for t in (cache.k_scale, cache.v_scale)]
+            # (a row a head, because scales may start on any 4-byte boundary; the library takes them in one where that can be)
+            areas += [_lib.CopyArea(t.data_ptr(), 4 * heads, 0, 4, 1, heads, 4) for t in (cache.k_scale, cache.v_scale)]
             areas.append(_lib.CopyArea(cache.bounds.data_ptr(), 2 * H * heads, 0, 0, 1, 1, 2 * H * heads))
         else:
             n, page, width = cache.data.shape
