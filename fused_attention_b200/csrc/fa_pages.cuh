@@ -102,8 +102,9 @@ __global__ void __launch_bounds__(kForkThreads) fa_pages_fork(const ForkArgs p) 
 //   1  the free pages (count 0), in ascending order, as many as blocks are written to
 //   2  entries that are written to and whose page is held by others too let go of it.  What is left of a page's count is the number of
 //      those that hold it and do not write to it
-//   3  where that is none all that hold the page write to it, and the lowest sequence keeps it: the count becomes minus (B - b) of the
-//      lowest b, by a minimum
+//   3  where that is none all that hold the page write to it, and the sequence with the most tokens on it keeps it, the lowest of several: the
+//      count becomes the least of their numbers (keeper_number).  The others may find no page and stay on this one, and where the keeper goes on
+//      none of them has a token
 //   4  an entry keeps its page if it finds its own number there; the others want one.  (Without shared pages 2 to 4 are passed over)
 //   5  each takes the page of its rank, in order of sequences and blocks; where there is none left, the entry stays as it was and its
 //      sequence is granted fewer tokens
@@ -137,6 +138,14 @@ __device__ __forceinline__ Window reserve_window(const ReserveArgs& p, uint32_t 
     if (w.count == 0) w.first = w.need;   // nothing is written
     return w;
 }
+// A sequence's number among those that might keep the page of block i: the lower, the more tokens it has there, and among several the lower it is.
+// Below zero, and none twice.  (The page is written to, so that it has room: 127 tokens at most, and with up to 2^24 sequences 128 B is 2^31.)
+__device__ __forceinline__ int32_t keeper_number(const ReserveArgs& p, const Window& w, uint32_t b, uint32_t i) {
+    const uint32_t begins = i << p.page_shift, tokens = w.held > begins ? w.held - begins : 0u;
+    return static_cast<int32_t>(0u - (tokens * p.t.B + (p.t.B - b)));
+}
+// What takes a count from such a number to one, whatever is added beside it (the count passes 2^31 on the way, which additions do not mind).
+__device__ __forceinline__ int32_t keeper_to_one(int32_t number) { return static_cast<int32_t>(1u - static_cast<uint32_t>(number)); }
 // Sum of x over the threads in front of this one; `all`: of all threads.  All threads of the CTA.
 __device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t* s_warp, uint32_t& all) {
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
@@ -300,7 +309,7 @@ __global__ void __launch_bounds__(kReserveThreads) fa_pages_reserve(const Reserv
             }
         }
         if (__syncthreads_or(is_shared)) {
-            const int32_t own = -static_cast<int32_t>(p.t.B - mine);
+            const int32_t own = keeper_number(p, own_w, mine, own_i);
             if (is_shared) atomicSub(p.v.refs + own_e, 1);
             __syncthreads();
             const bool all_write = is_shared && ld_cg(p.v.refs + own_e) <= 0;
@@ -311,7 +320,7 @@ __global__ void __launch_bounds__(kReserveThreads) fa_pages_reserve(const Reserv
                 is_shared = false;
             }
             __syncthreads();   // everyone has looked
-            if (keeps && all_write) atomicAdd(p.v.refs + own_e, 1 - own);   // from the sequence's number to one, whatever refused entries add
+            if (keeps && all_write) atomicAdd(p.v.refs + own_e, keeper_to_one(own));   // (refused entries add theirs)
         }
         uint32_t demand;
         const uint32_t rank = sum_before(writes && !keeps, s_warp, demand), there = min(found, demand);
@@ -340,8 +349,8 @@ __global__ void __launch_bounds__(kReserveThreads) fa_pages_reserve(const Reserv
         }
         return;
     }
-    // 2 to 4; what is kept is marked in the table, where nobody else looks: -2 - page if it was held alone, -2 - n - page if it is the lowest
-    // sequence's (n is below 2^30).  How many pages are wanted
+    // 2 to 4; what is kept is marked in the table, where nobody else looks: -2 - page if it was held alone, -2 - n - page if all that hold it write
+    // to it (n is below 2^30).  How many pages are wanted
     uint32_t wanted = 0;
     bool shared = false;
     for (uint32_t b0 = 0; b0 < p.t.B; b0 += at_once) {
@@ -375,7 +384,7 @@ __global__ void __launch_bounds__(kReserveThreads) fa_pages_reserve(const Reserv
                 blocks(b, w, i0, i1);
                 for (uint32_t i = i0; i < i1; ++i) {
                     int32_t* const entry = p.t.at + b * p.t.stride + i;
-                    const int32_t e = *entry, own = -static_cast<int32_t>(p.t.B - b);
+                    const int32_t e = *entry, own = keeper_number(p, w, b, i);
                     if (e < 0) continue;   // wanted, or kept already
                     if (step == 2) atomicSub(p.v.refs + e, 1);
                     else if (step == 3 && ld_cg(p.v.refs + e) <= 0) atomicMin(p.v.refs + e, own);
@@ -409,9 +418,9 @@ __global__ void __launch_bounds__(kReserveThreads) fa_pages_reserve(const Reserv
                 const int32_t page = -2 - e, n_pages = static_cast<int32_t>(p.v.n);
                 if (page < n_pages) {
                     *entry = page;
-                } else {   // the count goes from the sequence's number to one, whatever refused entries have added
+                } else {
                     *entry = page - n_pages;
-                    atomicAdd(p.v.refs + (page - n_pages), static_cast<int32_t>(p.t.B - b) + 1);
+                    atomicAdd(p.v.refs + (page - n_pages), keeper_to_one(keeper_number(p, w, b, i)));
                 }
                 continue;
             }

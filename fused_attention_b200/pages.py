@@ -127,10 +127,12 @@ def pages_reserve(pool: PagePool, table: torch.Tensor, lengths: torch.Tensor, co
     ``counts`` int32 [B], or a number for all: how many tokens will be appended.  Blocks behind them are let go of (drafted tokens that were
     taken back by lowering ``lengths``; with ``counts`` 0 and a length of 0 a whole sequence).  Blocks that the new tokens go to
     and that have no page get one; so do those whose page others hold too, unless all that hold it are about to write to it: then the
-    lowest sequence keeps it.  New pages are the lowest free ones in order of sequences and blocks.  Where such a block holds tokens
+    sequence with the most tokens on it keeps it, the lowest of several.  New pages are the lowest free ones in order of sequences and blocks.  Where such a block holds tokens
     already, sources[b] is the page that it was on and targets[b] the new one (-1 elsewhere): ``cache_copy`` has to come before the append.
 
-    ``granted[b]`` is counts[b], or fewer where pages ran out (or the table has no room): the ``counts`` of ``cache_append``.
+    ``granted[b]`` is counts[b], or fewer where pages ran out (or the table has no room): the ``counts`` of ``cache_append``.  A sequence that finds
+    no page in place of a shared one stays on it with the tokens it has; whoever keeps the page goes on behind all of them.  (The scales of an
+    8-bit cache are the page's: what goes on there may enlarge them, as tokens that were taken back may have.)
     """
     _require(isinstance(pool, PagePool), "the first argument must be a PagePool")
     _, reserve, _, _, entries = _calls()

@@ -413,8 +413,8 @@ int fa_b200_pages_fork(const fa_b200_pages* pages, int32_t* table, int64_t table
 /*
  * Gives every sequence the blocks that lengths[b] + counts[b] tokens need (counts NULL: `count` each) and no more: blocks behind them are
  * let go of.  Blocks that the new tokens go to and that have no page get one, and so do those whose page others hold too, unless all that
- * hold it are about to write to it: then the lowest sequence keeps it.  New pages are the lowest free ones, in the order of sequences and
- * blocks.  sources[b], targets[b]: the page that held the beginning of a block, and the one that has taken its place (-1: none);
+ * hold it are about to write to it: then the sequence with the most tokens on it keeps it, the lowest of several.  New pages are the lowest
+ * free ones, in the order of sequences and blocks; a block that finds none stays as it was, and nothing is written to it.  sources[b], targets[b]: the page that held the beginning of a block, and the one that has taken its place (-1: none);
  * fa_b200_cache_copy is to copy it before tokens are appended.  granted[b]: how many of the tokens have room, counts[b] unless pages ran out.
  * Scratch: 4 * n_pages bytes.
  */

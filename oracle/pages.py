@@ -33,9 +33,13 @@ def reserve(table, lengths, counts, n, page):
     for b in range(B):
         for i in range(W):
             if table[b][i] >= 0:
-                holders.setdefault(table[b][i], []).append(b)
+                holders.setdefault(table[b][i], []).append((b, i))
                 if first[b] <= i < need[b]:
-                    writers.setdefault(table[b][i], []).append(b)
+                    writers.setdefault(table[b][i], []).append((b, i))
+    def keeper(p):
+        """Of those that hold a page the one with the most tokens on it, the lowest of several: nobody else's tokens lie where it goes on."""
+        return max(holders[p], key=lambda at: (max(0, lengths[at[0]] - at[1] * page), -at[0]))
+
     free = iter([p for p in range(n) if refs[p] == 0])
     granted, sources, targets = [], [-1] * B, [-1] * B
     for b in range(B):
@@ -43,7 +47,7 @@ def reserve(table, lengths, counts, n, page):
         room = count
         for i in range(first[b], need[b]):
             p = table[b][i]
-            if p >= 0 and (len(holders[p]) == 1 or (sorted(writers[p]) == sorted(holders[p]) and b == min(holders[p]))):
+            if p >= 0 and (len(holders[p]) == 1 or (writers[p] == holders[p] and (b, i) == keeper(p))):
                 continue
             new = next(free, None)
             if new is None:
