@@ -90,8 +90,12 @@ int fa_b200_pages_reserve(const fa_b200_pages* pages, int32_t* table, int64_t ta
     OnDevice on(device);
     if (on.rc != 0) return on.rc;
     a.alone = B <= fa::kAloneRows && static_cast<uint64_t>(B) * table_width <= fa::kAloneEntries;
-    const uint32_t ctas = a.alone ? 1 : (B + fa::kReserveWarps - 1) / fa::kReserveWarps, sms = static_cast<uint32_t>(d->sms.load());
-    return launch(&fa::fa_pages_reserve, ctas < sms ? ctas : sms, fa::kReserveThreads, 0, static_cast<cudaStream_t>(cuda_stream), a);
+    const cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+    if (!a.alone) {
+        const uint32_t ctas = (B + fa::kReserveWarps - 1) / fa::kReserveWarps, sms = static_cast<uint32_t>(d->sms.load());
+        if ((rc = launch(&fa::fa_pages_release, ctas < sms ? ctas : sms, fa::kReserveThreads, 0, stream, a)) != FA_B200_OK) return rc;
+    }
+    return launch(&fa::fa_pages_reserve, 1, fa::kReserveThreads, 0, stream, a);
 }
 
 int fa_b200_pages_compact(const fa_b200_pages* pages, const int32_t* table, int64_t table_stride, uint32_t table_width, uint32_t B, int32_t* new_refs,

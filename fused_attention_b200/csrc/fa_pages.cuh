@@ -5,7 +5,7 @@
 // does not matter, and where one of several has to be chosen the lowest is (a minimum, likewise).
 //
 // These kernels read and write a few kilobytes to a megabyte: what bounds them is the chain of dependent accesses and the launch, so that
-// each call is one launch (compacting: two) and no value crosses to the host.  Copying is bound by memory.  Measured in a graph: a step of 8 beams
+// each call is one launch (compacting, and reserving in a large table: two) and no value crosses to the host.  Copying is bound by memory.  Measured in a graph: a step of 8 beams
 // of an 8-bit cache (fork, reserve, copy of 4 pages) 11 us, of 256 beams of two latent caches (141 pages of 147 KB) 21, of which copying takes 7.6
 // (5.5 TB/s); 10000 pages planned in 11 us, 2381 of 133 KB moved in 115 (5.5 TB/s, 84 % of a plain copy's).
 #pragma once
@@ -20,7 +20,7 @@ constexpr uint32_t kPagesCount = 4u;   // counts that do not fit the table: a pa
 
 struct PagesView {
     int32_t* refs;
-    uint32_t* status;   // four words: first code, number of reports, CTAs that are through (zero between calls), unused
+    uint32_t* status;   // first code, number of reports; pools of one cache may share them
     uint32_t n;
 };
 struct PagesTable {
@@ -95,9 +95,10 @@ __global__ void __launch_bounds__(kForkThreads) fa_pages_fork(const ForkArgs p) 
 }
 
 // ----------------------------------------------------------------------------- reserve
-// First, blocks behind those that are needed are let go of.  Where the table is small the one CTA that does the rest does that too;
-// otherwise CTAs take sequences, a warp each, and the last to be through goes on, with `lanes` threads a sequence (as many as its tokens
-// touch blocks, up to 32):
+// First, blocks behind those that are needed are let go of.  Where the table is small the one CTA that does the rest does that too; otherwise CTAs
+// take sequences, a warp each, in a launch of their own.  (Finding the last CTA of one launch takes a counter that is zero beforehand, and calls on
+// several tables must not meet there.  In a graph two launches are no slower: 256 sequences of 20 blocks in a table of 2048 11.2 us, 11.6 with a counter;
+// 1000 in one of 64 7.7 and 8.9.  A call that the host is slower with than the device, as the latter's 14 us, was 9.)  One CTA does the rest, with `lanes` threads a sequence (as many as its tokens touch blocks, up to 32):
 //
 //   1  the free pages (count 0), in ascending order, as many as blocks are written to
 //   2  entries that are written to and whose page is held by others too let go of it.  What is left of a page's count is the number of
@@ -117,7 +118,7 @@ struct ReserveArgs {
     int32_t* sources;        // [B]
     int32_t* targets;
     int32_t* list;           // [n]: free pages
-    uint32_t count, page_shift, alone;   // alone: one CTA, which lets go of blocks as well
+    uint32_t count, page_shift, alone;   // alone: the one CTA lets go of blocks as well
 };
 constexpr int kReserveThreads = 1024, kReserveWarps = kReserveThreads / 32;
 constexpr uint32_t kNoBlock = 0xFFFFFFFFu;
@@ -186,10 +187,32 @@ __device__ __forceinline__ uint32_t free_of_16(const PagesView& v, uint32_t q) {
 // A table of this many entries and sequences is gone over by one CTA, eight entries of a thread at a time.
 constexpr uint32_t kAloneEntries = 32768, kAloneRows = 2048;
 
+__global__ void __launch_bounds__(kReserveThreads) fa_pages_release(const ReserveArgs p) {
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    grid_dep_wait();
+    grid_dep_launch();
+    for (uint32_t b = blockIdx.x * kReserveWarps + warp; b < p.t.B; b += gridDim.x * kReserveWarps) {
+        const Window w = reserve_window(p, b);
+        if (lane == 0 && !w.ok) cache_report(p.v.status, kCacheBadPosition);
+        int32_t* const row = p.t.at + b * p.t.stride;
+        for (uint32_t i = w.need + lane; i < p.t.width; i += 128) {   // four loads of a lane in flight
+            int32_t e[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) e[k] = i + 32 * k < p.t.width ? row[i + 32 * k] : -1;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (e[k] != -1) {
+                    let_go(p.v, e[k]);
+                    row[i + 32 * k] = -1;
+                }
+        }
+    }
+}
+
 __global__ void __launch_bounds__(kReserveThreads) fa_pages_reserve(const ReserveArgs p) {
-    __shared__ uint32_t s_warp[32], s_most, s_last, s_need[kAloneRows];
+    __shared__ uint32_t s_warp[32], s_most, s_need[kAloneRows];
     __shared__ int32_t s_list[kReserveThreads];
-    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u;
     if (tid == 0) s_most = 0;
     grid_dep_wait();
     grid_dep_launch();
@@ -226,34 +249,8 @@ __global__ void __launch_bounds__(kReserveThreads) fa_pages_reserve(const Reserv
                 }
         }
     } else {
-        for (uint32_t b = blockIdx.x * kReserveWarps + warp; b < p.t.B; b += gridDim.x * kReserveWarps) {
-            const Window w = reserve_window(p, b);
-            if (lane == 0 && !w.ok) cache_report(p.v.status, kCacheBadPosition);
-            int32_t* const row = p.t.at + b * p.t.stride;
-            for (uint32_t i = w.need + lane; i < p.t.width; i += 128) {   // four loads of a lane in flight
-                int32_t e[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) e[k] = i + 32 * k < p.t.width ? row[i + 32 * k] : -1;
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (e[k] != -1) {
-                        let_go(p.v, e[k]);
-                        row[i + 32 * k] = -1;
-                    }
-            }
-        }
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) {
-            const uint32_t through = atomicAdd(p.v.status + 2, 1u);
-            s_last = through == gridDim.x - 1;
-            if (s_last) p.v.status[2] = 0;
-        }
-        __syncthreads();
-        if (!s_last) return;
-        __threadfence();
-        let = true;
         for (uint32_t b = tid; b < p.t.B; b += kReserveThreads) count_in(reserve_window(p, b));
+        __syncthreads();   // s_most
     }
 
     // how many blocks a sequence's tokens touch at most decides how many threads it gets

@@ -72,7 +72,7 @@ class PagePool:
         return self
 
     def _with(self, refs: torch.Tensor) -> "PagePool":
-        """A pool of other counts of the same pages, which reports where this one does."""
+        """A pool of other counts of the same pages, which reports where this one does; otherwise calls on the two have nothing in common."""
         return PagePool.__new__(PagePool)._set(refs, self.n_pages, self.device, self._index, self._status)
 
     def read_status(self) -> Tuple[int, int]:

@@ -399,7 +399,7 @@ int fa_b200_cache_attention_scratch(uint32_t head_dim, uint32_t kv_heads, uint32
  */
 typedef struct fa_b200_pages {
     int32_t* refs;       /* [n_pages] */
-    uint32_t* status;    /* four words, zero at first; the third is the library's between and within calls */
+    uint32_t* status;    /* four words, of which the first two are written; pools may share them */
     uint32_t n_pages;
 } fa_b200_pages;
 
