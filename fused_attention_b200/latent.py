@@ -72,8 +72,11 @@ class LatentCache:
         self._handle = _lib.LatentCache(data.data_ptr(), self._status.data_ptr(), 2 * data.stride(0), 2 * data.stride(1), n, page, latent_dim, self.rope_dim)
         self._address = ctypes.addressof(self._handle)
         self._copy_areas = None
-        # (rows on top of one another can be read, but not written)
-        self._writable = data.stride(1) >= width and (data.stride(0) >= (page - 1) * data.stride(1) + width or n == 1)
+        # (rows on top of one another can be read, but not written; pages may lie among one another's tokens)
+        reach, self._writable = width, True
+        for stride, size in sorted((data.stride(i), data.shape[i]) for i in range(2) if data.shape[i] > 1):
+            self._writable = self._writable and stride >= reach
+            reach += stride * (size - 1)
 
     def read_status(self) -> Tuple[int, int]:
         """(first code, number of reports) of what the kernels found wrong in table, lengths or counts; clears it.  Synchronises.  The codes are
