@@ -102,9 +102,11 @@ LatentPlan plan_rows(uint32_t latent, uint32_t heads, uint32_t page, uint32_t B,
     }
     const uint64_t most = (tiles + r.least - 1) / r.least;
     r.parts = static_cast<uint32_t>(parts < most ? parts : most);
-    // Short sequences are not divided where they give a quarter of the SMs something to do: what would be left of them takes less than
-    // joining, which costs the more the more rows there are.  (us whole and divided: 64 sequences of 100 to 512 tokens, 16 heads, 16.6 and
-    // 19.8, 16 of them 15.7 and 14.8, 1 of 301 12.1 and 9.8, 64 of 500 to 1000 26.7 and 23.7; 128 heads, 64 of 100 to 512 25 and 42, of 500 to
+    // Sequences that the table has little room for are not divided where they give a quarter of the SMs something to do: what would be left of them
+    // takes less than joining, which costs the more the more rows there are.  It is the table's width that decides, since lengths are known on the
+    // device alone: short sequences in a wide table are divided.  (64 of 500 to 1000 tokens, 128 heads, with L2 flushed: 47 us in a table of 1024
+    // tokens, 62 in one of 131072; 16 heads 35 and 33.  In tables as wide as the longest, us whole and divided: 64 sequences of 100 to 512 tokens,
+    // 16 heads, 16.6 and 19.8, 16 of them 15.7 and 14.8, 1 of 301 12.1 and 9.8, 64 of 500 to 1000 26.7 and 23.7; 128 heads, 64 of 100 to 512 25 and 42, of 500 to
     // 1000 39 and 54.)
     if (each <= (r.n <= 32 ? 8u : 16u) && static_cast<uint64_t>(B) * r.groups >= sms / 4) r.parts = B, r.least = 0;
     const uint64_t slots = r.parts == 1 || r.least == 0 ? 0 : 2ull * r.parts * r.groups;

@@ -17,9 +17,10 @@
 // Bound by the tensor pipe and the exponentials as fa_fwd_pipelined is: at NOPE = 128 a step of both tiles has 2560 tensor clocks of products and
 // 2048 of exponentials, and takes 3450.  (In one ring, values of a step came to stand in the way of keys two steps later: 4030.  With a barrier a
 // chunk and not a step it stayed at 4080: every wait that stands behind MMAs and commits costs the issuing warp 280 clocks.)  4096 tokens on 6000
-// keys, 20 heads of 128 + 64: 222 us, 0.93 PFLOP/s, 56 % of the products' measured peak; 8 prompts of 777, 12 heads of 64 + 32, 40 us.  An item's
-// beginning, end and up to three partly seen steps are what the second has most of.  Persistent CTAs, items dealt out there and back, were
-// slower, 236 and 54: items' lengths differ, and the hardware deals out better.
+// keys, 20 heads of 128 + 64: 222 to 249 us from box to box, 0.83 to 0.93 PFLOP/s, 50 to 56 % of the products' measured peak; 8 prompts of up to
+// 777, 12 heads of 64 + 32, 39 to 43 us.  An item's beginning, end and up to three partly seen steps are what the second has most of, and CTAs that
+// find nothing to do because `counts` is lower.  Persistent CTAs, items dealt out there and back, were slower, 236 and 54: items' lengths differ,
+// and the hardware deals out better.
 // At NOPE = 128 both tiles' scores take turns on one 128-column buffer (tensor memory: 128 + 2 * 64 of P + 2 * 128 of Y), which the other
 // tile's P V covers; at 64 each has its own.  Items with the most keys go first.
 #pragma once
@@ -155,10 +156,9 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
     if (warp < 8) {
         // ---------------------------------------------------------------- softmax of tile i
         setmaxnreg_inc<C::kSoftmaxRegs>();
-        const uint32_t i = warp >> 2, r = tid & 127u, lane_off = ((warp & 3u) * 32u) << 16, t = row0 + tid;
+        const uint32_t i = warp >> 2, lane_off = ((warp & 3u) * 32u) << 16, t = row0 + tid;
         const uint32_t tS = tmem + lane_off + (i ? C::kColS1 : C::kColS0), tP = tmem + lane_off + (i ? C::kColP1 : C::kColP0), tO = tmem + lane_off + (i ? C::kColO1 : C::kColO0);
         const uint32_t limit = limit_of(t), masked_from = limit == 0 ? kSeesAll : limit;   // (a row that sees nothing waits for nobody; it is written as zeros)
-        (void)r;
         float m = -INFINITY, l = 0.0f;
         const uint32_t mine = steps[i];
 #pragma unroll 1
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
                     float x0, x1;
                     unpack_f32x2(fma_f32x2(pack_f32x2(s[q * 32 + 2 * e], s[q * 32 + 2 * e + 1]), scale2, ref2), x0, x1);
                     const float w0 = ex2_approx(x0), w1 = ex2_approx(x1);
-                    pk[e] = pack_16(w0, w1, bf16);
+                    pk[e] = pack_16(w0, w1, bf16);   // as in fa_latent_rows: an MMA takes one type of both operands
                     const float2 y = unpack_16(pk[e], bf16);   // summed as rounded
                     if (e & 1) sum_b = add_f32x2(sum_b, pack_f32x2(y.x, y.y));
                     else sum_a = add_f32x2(sum_a, pack_f32x2(y.x, y.y));

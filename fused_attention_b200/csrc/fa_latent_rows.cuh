@@ -21,9 +21,9 @@
 //                tokens, 16 rows, where two took 72: a barrier's answer reaches a thread only behind the MMAs that it has queued)
 //   warps 14-15  queries into shared memory, a segment ahead; of the first segment the softmax warps do most
 //
-// Measured: 64 sequences of 100 to 8192 tokens, 16 rows, 64 us (306 MB, 4.7 TB/s; steady tiles of 73.7 KB take 2900 to 3000 clocks, the memory's
+// Measured: 64 sequences of 100 to 8192 tokens, 16 rows, 64 to 69 us from box to box (306 MB, 4.4 to 4.8 TB/s; steady tiles of 73.7 KB take 2900 to 3000 clocks, the memory's
 // share 2830; the rest is the way to the first tile, 4 us, CTAs that the memory serves later than others, 5, and the join); 32 of 1000 to 8192, 128
-// rows in two groups, 83 us (tiles take 3000 clocks where their MMAs take 1920: with 74 KB of queries the ring has two tiles, and what one passes
+// rows in two groups, 82 to 90 us (tiles take 3000 clocks where their MMAs take 1920: with 74 KB of queries the ring has two tiles, and what one passes
 // through from its slots' asking to their letting go, 5700 clocks, is the bound).
 //
 // What must not happen: a key that a row does not see reaching it, as 0 * NaN.  Tiles that some row of the group sees in part only (the
@@ -442,7 +442,8 @@ __global__ void __launch_bounds__(kLatentThreads, 1) fa_latent_rows(const __grid
                     const uint32_t h = g - C::kPBuffers;
                     mbar_wait(bar(C::PV + (h & 1u)), (h >> 1) & 1u, ctl, kCacheTimeout | C::PV);
                 }
-                // ---- weights, rounded
+                // ---- weights, rounded to the rows' type: an MMA takes one type of both operands, and a second product for what that takes away
+                // would double P V.  (The result is off by 1.2 times its own rounding)
                 uint32_t pk[2 * kBlocks];
 #pragma unroll
                 for (uint32_t j = 0; j < kBlocks; ++j) {

@@ -2,12 +2,12 @@
 //
 // refs[p] is the number of table entries that hold page p, 0: it is free.  A table entry is a page or -1; anything else is reported and
 // taken for -1.  All results are whole numbers that depend on nothing but the inputs: counts change by atomic additions, whose order
-// does not matter, and where one of several has to be chosen the lowest is (a minimum, likewise).
+// does not matter, and where one of several has to be chosen it is by a minimum, likewise.
 //
 // These kernels read and write a few kilobytes to a megabyte: what bounds them is the chain of dependent accesses and the launch, so that
-// each call is one launch (compacting, and reserving in a large table: two) and no value crosses to the host.  Copying is bound by memory.  Measured in a graph: a step of 8 beams
-// of an 8-bit cache (fork, reserve, copy of 4 pages) 11 us, of 256 beams of two latent caches (141 pages of 147 KB) 21, of which copying takes 7.6
-// (5.5 TB/s); 10000 pages planned in 11 us, 2381 of 133 KB moved in 115 (5.5 TB/s, 84 % of a plain copy's).
+// each call is one launch (compacting, and reserving in a large table: two) and no value crosses to the host.  Copying is bound by memory.
+// Measured in a graph: a step of 8 beams of an 8-bit cache (fork, reserve, copy of 4 pages) 11 us, of 256 beams of two latent caches (141 pages of
+// 147 KB) 21, of which copying takes 7.6 (5.5 TB/s); 10000 pages planned in 11 us, 2381 of 133 KB moved in 115 (5.5 TB/s, 84 % of a plain copy's).
 #pragma once
 
 #include "fa_cache.cuh"
@@ -97,8 +97,9 @@ __global__ void __launch_bounds__(kForkThreads) fa_pages_fork(const ForkArgs p) 
 // ----------------------------------------------------------------------------- reserve
 // First, blocks behind those that are needed are let go of.  Where the table is small the one CTA that does the rest does that too; otherwise CTAs
 // take sequences, a warp each, in a launch of their own.  (Finding the last CTA of one launch takes a counter that is zero beforehand, and calls on
-// several tables must not meet there.  In a graph two launches are no slower: 256 sequences of 20 blocks in a table of 2048 11.2 us, 11.6 with a counter;
-// 1000 in one of 64 7.7 and 8.9.  A call that the host is slower with than the device, as the latter's 14 us, was 9.)  One CTA does the rest, with `lanes` threads a sequence (as many as its tokens touch blocks, up to 32):
+// several tables must not meet there.  In a graph two launches are no slower: 256 sequences of 20 blocks in a table of 2048 11.2 us, 11.6 with a
+// counter; 1000 in one of 64 7.7 and 8.9.  The second launch costs the host 5 us, so that an eager call of the latter takes 14, not 9.)
+// One CTA does the rest, with `lanes` threads a sequence (as many as its tokens touch blocks, up to 32):
 //
 //   1  the free pages (count 0), in ascending order, as many as blocks are written to
 //   2  entries that are written to and whose page is held by others too let go of it.  What is left of a page's count is the number of
@@ -445,7 +446,8 @@ __global__ void __launch_bounds__(kReserveThreads) fa_pages_reserve(const Reserv
 
 // ----------------------------------------------------------------------------- compact
 // With n_used pages held, those from n_used on move to the free ones in front of it, the k-th to the k-th.  A CTA works out 4096 pages;
-// it counts those in front of them itself, from all of refs (13333 pages are 53 KB), so that no CTA waits for another.
+// it counts those in front of them itself, from all of refs (13333 pages are 53 KB), so that no CTA waits for another.  What is read
+// grows with the square of the pages: a call takes 21 us for 10000 and for 100000 of them, 170 for a million, 2 ms for 4 and 32 for 16 million.
 struct CompactArgs {
     PagesView v;
     PagesTable t;
@@ -529,8 +531,8 @@ __global__ void __launch_bounds__(256) fa_pages_renumber(const CompactArgs p) {
 
 // ----------------------------------------------------------------------------- copy
 // Contents of pages, source to target, for up to kCopyAreas arrays: a page of an array is n0 x n1 rows of `row` bytes (one row where it
-// lies in one piece), taken 16 or 4 bytes at a time.  CTAs are dealt out by parts of a page, `parts` equal ones of each array, first: CTA (x, y) has part y of the pairs x,
-// x + gridDim.x, ...  Every thread has eight pieces of 16 bytes in flight.
+// lies in one piece), taken 16 or 4 bytes at a time.  CTAs are dealt out by parts of a page, `parts` equal ones of each array, first: CTA (x, y)
+// has part y of the pairs x, x + gridDim.x, ...  Every thread has eight pieces of 16 bytes in flight.
 struct CopyArea {
     uint8_t* base;
     int64_t page, stride0, stride1;   // bytes

@@ -79,8 +79,8 @@ class LatentCache:
             reach += stride * (size - 1)
 
     def read_status(self) -> Tuple[int, int]:
-        """(first code, number of reports) of what the kernels found wrong in table, lengths or counts; clears it.  Synchronises.  The codes are
-        those of ``cache.STATUS``; 0x100 and above: a bounded wait expired."""
+        """(first code, number of reports) of what the kernels found wrong in table and lengths; clears it.  Synchronises.  The codes are those of
+        ``cache.STATUS``; 0x100 and above: a bounded wait expired.  (Counts are cut to 0 to T and not reported.)"""
         code, reports = self._status.tolist()
         if code or reports:
             self._status.zero_()

@@ -425,7 +425,7 @@ int fa_b200_pages_reserve(const fa_b200_pages* pages, int32_t* table, int64_t ta
 /*
  * The move of all pages that are held to the front: with n_used of them, the k-th of those from n_used on goes to the k-th free one in front
  * of it.  Writes refs and table ([B, table_width] contiguous) as they are afterwards, and the moves: sources and targets [n_pages], -1 behind
- * the last.  The old ones are left as they are.  Scratch: 4 * n_pages + 8 bytes.
+ * the last.  The old ones are left as they are.  Beyond 100000 pages time grows with their square.  Scratch: 4 * n_pages + 8 bytes.
  */
 int fa_b200_pages_compact(const fa_b200_pages* pages, const int32_t* table, int64_t table_stride, uint32_t table_width, uint32_t B, int32_t* new_refs,
                           int32_t* new_table, int32_t* sources, int32_t* targets, void* scratch, uint64_t scratch_bytes, int device, void* cuda_stream);
